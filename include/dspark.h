@@ -463,6 +463,145 @@ typedef struct dspark_p2p_gather_args {
  * sets the device status word. */
 int dspark_p2p_allgather(const dspark_p2p_gather_args* args, void* stream);
 
+/* ---- one round with a drafted tree ------------------------------------------------------
+ * The operators a speculative round with a tree of drafted tokens runs besides the projections:
+ * pack the trees, rotate and append q / k / v, attend over the cache, accept against the
+ * target's probabilities, keep the accepted path. Requests are packed: request b owns rows
+ * cu_rows[b] .. cu_rows[b + 1] - 1 (device int32 [B + 1], cu_rows[0] = 0), its first row is the
+ * pending token (the tree's root) and parent[r] is the place, within the request, of row r's
+ * parent (-1 for the root; a parent comes before its children). Extends the reference's tree
+ * rounds (src/mlx_dspark/tree.py) to any number of nodes, ragged over requests, and to sampled
+ * targets (src/mlx_dspark/sampling.py). */
+
+/* Per row: row_pos = kv_len[b] + depth (rotary position), row_slot = kv_len[b] + place (cache
+ * slot), row_req = b, and anc = bits of the row itself and its ancestors (anc_words uint32 words
+ * a row, bit j of word j / 32: place j). kv_len_new[b] = kv_len[b] + rows. parent may be NULL
+ * (each block a chain). A row whose parent is not before it counts as a second root. Outputs may
+ * be NULL. Rows of a request beyond 32 * anc_words get no bits of those places. */
+int dspark_tree_pack(const int32_t* cu_rows, const int32_t* parent, const int32_t* kv_len, int B,
+                     int R, int32_t* row_pos, int32_t* row_slot, int32_t* row_req, uint32_t* anc,
+                     int anc_words, int32_t* kv_len_new, void* stream);
+
+#define DSPARK_ROPE_HALF 0         /* pairs (i, i + rot / 2) */
+#define DSPARK_ROPE_INTERLEAVED 1  /* pairs (2 i, 2 i + 1) */
+
+/* Rotary positions of packed q and k rows with the append of k and v to the cache:
+ * (a, b) -> mscale * (a cos t - b sin t, b cos t + a sin t) for each pair i < rot / 2 of a head's
+ * first `rot` values, t = row_pos[r] * (frequency i); the rest of the head passes. freq[i] is the
+ * frequency as a fraction of a turn in 64-bit fixed point (f / 2 pi * 2^64), so that positions of
+ * any length keep their phase to 2^-32 of a turn. Optional per-head RMS norm (q_norm / k_norm [D])
+ * before the rotation. All in fp32, rounded once. Rotated k and v go to cache row
+ * (row_req[r] or 0, head, row_slot[r]); a row outside the cache is not written and the device
+ * status word records it. q_out may be q. k NULL (Hk 0): q alone. D % 16 == 0, D <= 512,
+ * rot % 16 == 0, bf16 or fp16, head_dim contiguous. */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_strides[2], k_strides[2], v_strides[2];  /* elements {row, head} */
+  void* q_out;
+  int64_t qo_strides[2];
+  void* k_cache;
+  void* v_cache;
+  int64_t kc_strides[3], vc_strides[3];              /* elements {batch, head, position} */
+  const uint64_t* freq;                              /* device [rot / 2] */
+  const int32_t* row_pos;                            /* device [R] */
+  const int32_t* row_slot;                           /* device [R] */
+  const int32_t* row_req;                            /* device [R] or NULL */
+  const void* q_norm;                                /* [D] or NULL */
+  const void* k_norm;
+  float mscale, eps;
+  int dtype, layout;
+  int R, Hq, Hk, D, rot, cap, batch;
+} dspark_rope_args;
+
+int dspark_rope_append(const dspark_rope_args* a, void* stream);
+
+/* Attention of packed tree rows over the cache: row i of request b sees its first
+ * kv_len[b] - rows(b) keys and, of its tree's rows(b) keys after them, those whose bit is set in
+ * its anc words; anc NULL: every place up to its own (a chain, or a prompt's chunk).
+ * out = softmax(scale q.k) . v over the visible keys, zeros where there are none; keys that a row
+ * does not see take no part whatever they hold. k / v [kv_batch, Hk, cap, D] with strides
+ * {batch, head, position}: request b's keys start at position kv_start[b] (or 0) of batch entry b,
+ * or of entry 0 when kv_batch is 1. kv_len counts are cut at the cache's end. max_rows bounds
+ * rows(b) (it only chooses the launch). bf16 or fp16, D 64 or 128, 16-byte aligned rows.
+ * Scratch: dspark_tree_attn_workspace bytes, nothing to clear; calls that overlap on the GPU
+ * need their own. */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  int64_t q_strides[2], o_strides[2];  /* elements {row, head} */
+  int64_t k_strides[3], v_strides[3];  /* elements {batch, head, position} */
+  const int32_t* cu_rows;              /* device [B + 1] */
+  const int32_t* kv_len;               /* device [B], the tree's rows included */
+  const int32_t* kv_start;             /* device [B] or NULL */
+  const uint32_t* anc;                 /* device [R, anc_words] or NULL */
+  void* workspace;
+  size_t ws_bytes;
+  float scale;
+  int dtype, anc_words, max_rows;
+  int R, B, Hq, Hk, D, cap, kv_batch;
+} dspark_tree_attn_args;
+
+int dspark_tree_attn(const dspark_tree_attn_args* a, void* stream);
+size_t dspark_tree_attn_workspace(int B, int Hq, int Hk, int D, int max_rows);
+
+/* Verification of drafted tokens against the target's probabilities p = softmax(logits / T) from
+ * given random numbers (T = temperature[b], NULL: 1; T = 0: all mass on the first largest
+ * logit). u [R] uniform in [0, 1), one a row; noise [B, V] exponential, one row a request.
+ * Walk from the root: at row r,
+ *   chain (parent NULL): the next row's token x is accepted iff u[r] * q(x) < p_r(x), q the draft
+ *     distribution x was drawn from (row r of draft; draft NULL or T = 0: q(x) = 1);
+ *   tree: the children in order, each token once; accepted is the first whose running sum of
+ *     p_r(x) exceeds u[r] (proposals without a distribution; draft must be NULL).
+ * next_tok = argmax of w(v) / noise[b, v], first on ties, with w = max(p - q, 0) after a
+ * rejection with a draft distribution, p without the tokens tried at the last row otherwise
+ * (both: p itself where w is zero everywhere). Each emitted token then has the target's
+ * distribution. n_accept = accepted drafts; path[cu + i] = place of the i-th kept row (0 .. n),
+ * -1 after; prob[r] = p_parent(ids[r]) (1 for a root); lens[b] (optional) loses the rejected rows.
+ * A request without rows: n 0, next -1, length kept. Logits -inf or NaN have probability 0, +inf
+ * counts as the largest finite value; a row with no mass accepts nothing and gives next -1.
+ * logits bf16, fp16 or fp32, draft bf16, fp16 or fp32 (draft_dtype). max_rows bounds the rows of a
+ * request (<= 1024); rows beyond it are not accepted. */
+#define DSPARK_DTYPE_F32 2
+typedef struct {
+  const void* logits;
+  const void* draft;
+  int64_t ld_logits, ld_draft, ld_noise;
+  const int32_t* ids;
+  const int32_t* cu_rows;
+  const int32_t* parent;
+  const float* u;
+  const float* noise;
+  const float* temperature;
+  int32_t* n_accept;
+  int32_t* next_tok;
+  float* prob;      /* or NULL */
+  int32_t* path;    /* or NULL */
+  int32_t* lens;    /* or NULL */
+  void* workspace;
+  size_t ws_bytes;
+  int dtype, draft_dtype;
+  int R, B, V, max_rows;
+} dspark_sample_args;
+
+int dspark_sample_accept(const dspark_sample_args* a, void* stream);
+size_t dspark_sample_workspace(int R, int B, int V);
+
+/* Keep the accepted path of each request: with base = lens[b] - n_accept[b] - 1 (lens after the
+ * accept), cache row base + path[cu_rows[b] + i] moves to base + i for i <= n_accept[b], in every
+ * one of n_layers K and V caches (k_layers / v_layers: device arrays of n_layers pointers, all of
+ * the strides {batch, head, position}). path ascends. kv_start as in dspark_tree_attn; batch entry
+ * b, or 0 when kv_batch is 1. Rows outside the cache are skipped (the status word records it).
+ * D * elem_size a multiple of 16, 16-byte aligned rows. */
+int dspark_kv_keep_path(void* const* k_layers, void* const* v_layers, int n_layers,
+                        const int64_t k_strides[3], const int64_t v_strides[3],
+                        const int32_t* path, const int32_t* cu_rows, const int32_t* n_accept,
+                        const int32_t* lens, const int32_t* kv_start, int B, int H, int D,
+                        int elem_size, int cap, int kv_batch, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

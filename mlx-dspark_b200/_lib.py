@@ -94,6 +94,38 @@ class QKV(C.Structure):
                 ("q_strides", i64 * 3), ("s_strides", i64 * 3), ("bits", i32)]
 
 
+class RopeArgs(C.Structure):
+    """``dspark_rope_args`` (include/dspark.h)."""
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("q_strides", i64 * 2), ("k_strides", i64 * 2),
+                ("v_strides", i64 * 2), ("q_out", vp), ("qo_strides", i64 * 2), ("k_cache", vp),
+                ("v_cache", vp), ("kc_strides", i64 * 3), ("vc_strides", i64 * 3), ("freq", vp),
+                ("row_pos", vp), ("row_slot", vp), ("row_req", vp), ("q_norm", vp),
+                ("k_norm", vp), ("mscale", f32), ("eps", f32), ("dtype", i32), ("layout", i32),
+                ("R", i32), ("Hq", i32), ("Hk", i32), ("D", i32), ("rot", i32), ("cap", i32),
+                ("batch", i32)]
+
+
+class TreeAttnArgs(C.Structure):
+    """``dspark_tree_attn_args`` (include/dspark.h)."""
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("out", vp), ("q_strides", i64 * 2),
+                ("o_strides", i64 * 2), ("k_strides", i64 * 3), ("v_strides", i64 * 3),
+                ("cu_rows", vp), ("kv_len", vp), ("kv_start", vp), ("anc", vp), ("workspace", vp),
+                ("ws_bytes", sz), ("scale", f32), ("dtype", i32), ("anc_words", i32),
+                ("max_rows", i32), ("R", i32), ("B", i32), ("Hq", i32), ("Hk", i32), ("D", i32),
+                ("cap", i32), ("kv_batch", i32)]
+
+
+class SampleArgs(C.Structure):
+    """``dspark_sample_args`` (include/dspark.h)."""
+    _fields_ = [("logits", vp), ("draft", vp), ("ld_logits", i64), ("ld_draft", i64),
+                ("ld_noise", i64), ("ids", vp), ("cu_rows", vp), ("parent", vp), ("u", vp),
+                ("noise", vp), ("temperature", vp), ("n_accept", vp), ("next_tok", vp),
+                ("prob", vp), ("path", vp), ("lens", vp), ("workspace", vp), ("ws_bytes", sz),
+                ("dtype", i32), ("draft_dtype", i32), ("R", i32), ("B", i32), ("V", i32),
+                ("max_rows", i32)]
+
+
+ROPE_HALF, ROPE_INTERLEAVED = range(2)
 EPI_PLAIN, EPI_RESID, EPI_SWIGLU, EPI_QKROPE = range(4)
 
 _SIGS = {
@@ -145,6 +177,14 @@ _SIGS = {
     "dspark_verify_forward": (i32, [C.POINTER(Model), C.POINTER(FwdBuffers), vp, i32, i32, i32,
                                     i32, vp, i64, vp]),
     "dspark_verify_prepare": (i32, [vp, i32, C.POINTER(FwdBuffers), vp]),
+    "dspark_tree_pack": (i32, [vp, vp, vp, i32, i32, vp, vp, vp, vp, i32, vp, vp]),
+    "dspark_rope_append": (i32, [C.POINTER(RopeArgs), vp]),
+    "dspark_tree_attn": (i32, [C.POINTER(TreeAttnArgs), vp]),
+    "dspark_tree_attn_workspace": (sz, [i32, i32, i32, i32, i32]),
+    "dspark_sample_accept": (i32, [C.POINTER(SampleArgs), vp]),
+    "dspark_sample_workspace": (sz, [i32, i32, i32]),
+    "dspark_kv_keep_path": (i32, [vp, vp, i32, P_i64, P_i64, vp, vp, vp, vp, vp, i32, i32, i32, i32,
+                                  i32, i32, vp]),
 }
 
 EXPORTED = tuple(_SIGS)

@@ -35,3 +35,31 @@ def require_cuda(*ts: torch.Tensor) -> torch.device:
 
 def elem_strides(t: torch.Tensor, n: int = 3) -> list[int]:
     return [int(s) for s in t.stride()[:n]]
+
+
+def on_device(first: torch.Tensor, *rest: torch.Tensor | None):
+    """The CUDA device of ``first``, with every other tensor (``None`` skipped) on it, and the
+    current stream there. Launches go to the current device, so it has to be that one."""
+    dev = first.device
+    if dev.type != "cuda":
+        raise _lib.DSparkUnsupported(
+            _lib.ERR_UNSUPPORTED, f"tensor on {dev}: dspark kernels run on CUDA only "
+            "(there is no CPU path)")
+    for t in rest:
+        if t is not None and t.device != dev:
+            raise _lib.DSparkError(_lib.ERR_ARG, f"tensors on {dev} and {t.device}")
+    if dev.index != torch.cuda.current_device():
+        raise _lib.DSparkError(_lib.ERR_ARG, f"tensors on {dev}, which is not the current device")
+    _lib.ensure_init(dev.index)
+    return dev, torch.cuda.current_stream(dev).cuda_stream
+
+
+def int32(name: str, t: torch.Tensor | None, n: int | None = None) -> torch.Tensor | None:
+    """``t``, checked to be contiguous int32 (and of ``n`` values): what the kernels index."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        raise _lib.DSparkError(_lib.ERR_ARG, f"{name} must be contiguous int32, got {t.dtype}")
+    if n is not None and t.numel() != n:
+        raise _lib.DSparkError(_lib.ERR_ARG, f"{name} has {t.numel()} values, {n} are needed")
+    return t
