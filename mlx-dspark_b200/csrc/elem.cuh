@@ -4,6 +4,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace dspark {
@@ -13,6 +15,7 @@ struct Elem;
 
 template <>
 struct Elem<bf16> {
+  static constexpr uint32_t kExpMask = 0x7F80u;
   static __device__ __forceinline__ float to_f(bf16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ bf16 from_f(float v) { return __float2bfloat16_rn(v); }
   static __device__ __forceinline__ float2 unpack(uint32_t w) {
@@ -23,6 +26,7 @@ struct Elem<bf16> {
 
 template <>
 struct Elem<__half> {
+  static constexpr uint32_t kExpMask = 0x7C00u;
   static __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
   static __device__ __forceinline__ float2 unpack(uint32_t w) {

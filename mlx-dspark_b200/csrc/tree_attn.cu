@@ -1,89 +1,861 @@
 // Attention of drafted trees over the cache (dspark_tree_attn): packed rows of ragged requests, each
-// row seeing its request's cached prefix and its own ancestors.
+// row seeing its request's cached prefix and its own ancestors, on the 5th-generation tensor cores.
 //
-// Simple form: one warp a (row, query head); 32 keys at a time, a lane a key for the scores
-// (running maximum and sum in fp32), a lane D / 32 values of the output for the weighted sum.
+// out_i = sum_j p_ij v_j / sum_j p_ij, p_ij = exp(scale q_i.k_j - m_i): one pass over the keys with a
+// running maximum m_i and sum (fp32). The G = Hq / Hk query heads of a kv head share its keys, so
+// the rows of one product are (node, head of the group): node * G + g.
+//
+// Units and segments. A unit is 128 keys of one item: an item is up to 256 rows of one (request, kv
+// head). All units of the call are numbered (request, head, rows, keys) and cut into equal contiguous
+// ranges, one a CTA (one CTA per SM), from the lengths on the device: requests of any mix of lengths
+// load the SMs evenly without the host knowing them. A CTA walks its range as segments (a run of
+// keys of one item). A segment that covers its item writes the output; else it leaves an
+// unnormalised fp32 part (m, sum, O) in the workspace, at most two a CTA, and the merge kernel joins
+// the parts of an item in order (no atomics: results do not depend on timing).
+//
+// CTA: two slots of 128 rows (TMEM lanes), each with a softmax warpgroup, a score tile S (TMEM,
+// overwritten by the 16-bit weights P) and an output accumulator O (TMEM).
+//  * items of more than 128 rows: the slots are the two halves of the rows and share each K/V tile;
+//  * items of up to 128 rows: the slots take the even and the odd key tiles of the segment and
+//    are joined through shared memory at its end.
+// Either way one slot's softmax runs under the other slot's products. One producer thread streams
+// K and V tiles by TMA through a ring (the order the products use them), one thread issues the
+// products: S = Q K^T (both from shared memory, K-major), O += P V (P from tensor memory, V from
+// shared memory as it lies, keys along K, so N-major). A thread of a softmax warpgroup owns a row:
+// no shuffles. The maximum in use is only raised when a tile exceeds it by more than 2^8: the
+// weights then stay within fp16 / fp32 range and O is rarely rescaled.
+//
+// Keys that a row does not see take no part whatever they hold: scores are replaced by -inf, V rows
+// past the request's keys are zeroed in shared memory, and a non-finite V among the tree's own keys
+// is taken out of the tile and added only to the rows that see it (fix_values / add_hidden).
+#include <algorithm>
+
 #include "elem.cuh"
 #include "host_common.h"
+#include "tcgen05.cuh"
 
 namespace dspark {
 namespace tattn {
 
-// The request that owns packed row r: the largest b with cu[b] <= r, or -1 past the last row.
-__device__ __forceinline__ int owner(const int32_t* cu, int B, int r) {
-  if (r >= cu[B]) return -1;
-  int lo = 0, hi = B - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cu[mid] <= r) lo = mid; else hi = mid - 1;
-  }
-  return lo;
+constexpr int BN = 128;       // keys a tile
+constexpr int ROWS = 128;     // rows a slot
+constexpr int NTHR = 384;     // two softmax warpgroups, producer, MMA, two idle warps
+constexpr int WARP_TMA = 8, WARP_MMA = 9;
+
+template <int D>
+struct Lay {
+  static constexpr int TILE = BN * D * 2;         // a K or V tile (and a slot's Q)
+  static constexpr int HALF = BN * 128;           // 64 values of 128 rows, 128-byte swizzled
+  static constexpr int NB = D == 128 ? 5 : 10;    // ring buffers
+  static constexpr int Q = 0;
+  static constexpr int RING = 2 * TILE;
+  static constexpr int BARS = RING + NB * TILE;
+  static constexpr int NBAR = 2 * NB + 2 + 2 + 2 + 2 + 1;
+  static constexpr int STAT = (BARS + NBAR * 8 + 15) / 16 * 16;  // slot 1's (m, l) by row, flags, scan
+  static constexpr int TOTAL = STAT + ROWS * 8 + 256 + 1024;     // slack to align the base
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(32) simple_kernel(const dspark_tree_attn_args a) {
-  pdl_launch_dependents();
-  pdl_wait();
-  constexpr int VPL = D / 32;
-  const int r = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  const int b = owner(a.cu_rows, a.B, r);
-  if (b < 0) return;
-  __shared__ float qs[D];
-  const T* q = static_cast<const T*>(a.q) + r * a.q_strides[0] + h * a.q_strides[1];
-  for (int d = lane; d < D; d += 32) qs[d] = Elem<T>::to_f(q[d]) * a.scale;
-  __syncwarp();
-  const int r0 = a.cu_rows[b], rows = a.cu_rows[b + 1] - r0, i = r - r0;
-  const int start = a.kv_start ? a.kv_start[b] : 0;
-  const int len = min(a.kv_len[b], a.cap - start), first = a.kv_len[b] - rows;
-  const int hk = h / (a.Hq / a.Hk), kb = a.kv_batch == 1 ? 0 : b;
-  const T* kp = static_cast<const T*>(a.k) + kb * a.k_strides[0] + hk * a.k_strides[1] +
-                int64_t(start) * a.k_strides[2];
-  const T* vp = static_cast<const T*>(a.v) + kb * a.v_strides[0] + hk * a.v_strides[1] +
-                int64_t(start) * a.v_strides[2];
-  float m = -INFINITY, l = 0.f, o[VPL];
+__device__ __forceinline__ void ld_x32(uint32_t taddr, float* d) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, "
+      "[%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
 #pragma unroll
-  for (int e = 0; e < VPL; ++e) o[e] = 0.f;
-  for (int j0 = 0; j0 < len; j0 += 32) {
-    const int j = j0 + lane, t = j - first;
-    bool sees = j < len;
-    if (sees && t >= 0)
-      sees = a.anc ? t < 32 * a.anc_words &&
-                         ((a.anc[int64_t(r) * a.anc_words + (t >> 5)] >> (t & 31)) & 1u)
-                   : t <= i;
-    float s = -INFINITY;
-    if (sees) {
-      s = 0.f;
-      const T* kr = kp + int64_t(j) * a.k_strides[2];
-      for (int d = 0; d < D; ++d) s += qs[d] * Elem<T>::to_f(kr[d]);
+  for (int i = 0; i < 32; ++i) d[i] = __uint_as_float(r[i]);
+}
+
+// D[tmem] (+)= A[smem] . B[smem]^T
+__device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                        uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 128-byte-swizzled operand: K-major (lbo unused, 8-row groups 1024 bytes apart) or MN-major (lbo
+// between 64-value blocks of MN, 8-row groups of K 1024 bytes apart).
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo) {
+  uint64_t d = 0;
+  d |= uint64_t((addr >> 4) & 0x3FFF);
+  d |= uint64_t((lbo >> 4) & 0x3FFF) << 16;
+  d |= uint64_t(1024 >> 4) << 32;
+  d |= uint64_t(1) << 46;
+  d |= uint64_t(2) << 61;
+  return d;
+}
+
+__device__ __forceinline__ void named_sync(int id, int n) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
+}
+
+// ------------------------------------------------------------------ units, ranges, segments
+
+__device__ __forceinline__ int rows_of(const dspark_tree_attn_args& a, int b, int& r0) {
+  r0 = min(max(a.cu_rows[b], 0), a.R);
+  return min(max(a.cu_rows[b + 1] - r0, 0), a.R - r0);
+}
+
+__device__ __forceinline__ int start_of(const dspark_tree_attn_args& a, int b) {
+  return a.kv_start ? min(max(a.kv_start[b], 0), a.cap) : 0;
+}
+
+// Row blocks and key tiles of request b (a request of rows but no keys has one tile, all hidden).
+__device__ __forceinline__ void extents(const dspark_tree_attn_args& a, int b, int& M, int& T) {
+  int r0;
+  const int n = rows_of(a, b, r0);
+  M = (n * (a.Hq / a.Hk) + 2 * ROWS - 1) / (2 * ROWS);
+  T = max(1, (min(a.kv_len[b], a.cap - start_of(a, b)) + BN - 1) / BN);
+}
+
+__device__ __forceinline__ int64_t units_of(const dspark_tree_attn_args& a, int b) {
+  int M, T;
+  extents(a, b, M, T);
+  return int64_t(M) * T * a.Hk;
+}
+
+struct Place {
+  int64_t total;  // units of the call
+  int64_t base;   // first unit of request b
+  int b;          // request that holds the unit looked up
+};
+
+// All threads of the block: the total number of units and, for the unit `of(total)`, its request.
+// `scan` holds 32 + 4 values.
+template <typename F>
+__device__ Place locate(const dspark_tree_attn_args& a, int64_t* scan, F&& of) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+  auto block_scan = [&](int64_t v, int64_t& sum) {  // inclusive scan over the block
+    int64_t x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
     }
-    float mt = s;
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
-    const float mn = fmaxf(m, mt);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    const float keep = expf(m - base);
-    const float p = sees ? expf(s - base) : 0.f;
-    float ps = p;
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, x);
-    l = l * keep + ps;
-    m = mn;
-#pragma unroll
-    for (int e = 0; e < VPL; ++e) o[e] *= keep;
-    unsigned live = __ballot_sync(0xffffffffu, sees);
-    while (live) {
-      const int x = __ffs(live) - 1;
-      live &= live - 1;
-      const float px = __shfl_sync(0xffffffffu, p, x);
-      const T* vr = vp + int64_t(j0 + x) * a.v_strides[2];
-#pragma unroll
-      for (int e = 0; e < VPL; ++e) o[e] += px * Elem<T>::to_f(vr[lane + 32 * e]);
+    __syncthreads();
+    if (lane == 31) scan[warp] = x;
+    __syncthreads();
+    int64_t before = 0;
+    sum = 0;
+    for (int w = 0; w < nw; ++w) {
+      if (w < warp) before += scan[w];
+      sum += scan[w];
+    }
+    return before + x;
+  };
+  const int64_t mine = tid < a.B ? units_of(a, tid) : 0;
+  int64_t sum, total;
+  const int64_t incl = block_scan(mine, sum);
+  total = sum;
+  for (int b0 = blockDim.x; b0 < a.B; b0 += blockDim.x) {
+    block_scan(b0 + tid < a.B ? units_of(a, b0 + tid) : 0, sum);
+    total += sum;
+  }
+  const int64_t u = of(total);
+  int64_t* found = scan + 32;  // base, request
+  if (tid == 0) found[1] = a.B;
+  __syncthreads();
+  if (u < total) {
+    if (mine > 0 && u < incl && u >= incl - mine) {
+      found[0] = incl - mine;
+      found[1] = tid;
+    }
+    __syncthreads();
+    int64_t at = 0;
+    if (a.B > int(blockDim.x)) {
+      block_scan(mine, at);
+      for (int b0 = blockDim.x; b0 < a.B; b0 += blockDim.x) {
+        const int64_t v = b0 + tid < a.B ? units_of(a, b0 + tid) : 0;
+        const int64_t x = at + block_scan(v, sum);
+        if (v > 0 && u < x && u >= x - v) {
+          found[0] = x - v;
+          found[1] = b0 + tid;
+        }
+        at += sum;
+      }
     }
   }
-  T* out = static_cast<T*>(a.out) + r * a.o_strides[0] + h * a.o_strides[1];
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __syncthreads();
+  return Place{total, found[0], int(found[1])};
+}
+
+__device__ __forceinline__ int64_t range_begin(int64_t total, int c, int n) { return total * c / n; }
+
+// One run of key tiles of one item.
+struct Segment {
+  int b, h, rows, r0;   // request, kv head, its packed rows
+  int row_base, live;   // first (node, head) row of the item, its rows (<= 256)
+  int t0, t1, T;        // tiles [t0, t1) of T
+  int len, first;       // keys, keys before the tree
+  int start, kb;        // cache position and batch entry
+  bool pair;
+};
+
+struct Walker {
+  int64_t u, end, base;
+  int b;
+  __device__ __forceinline__ bool next(const dspark_tree_attn_args& a, Segment& s) {
+    if (u >= end) return false;
+    int M, T;
+    extents(a, b, M, T);
+    int64_t n = int64_t(M) * T * a.Hk;
+    while (u >= base + n) {
+      base += n;
+      extents(a, ++b, M, T);
+      n = int64_t(M) * T * a.Hk;
+    }
+    const int G = a.Hq / a.Hk;
+    const int64_t local = u - base;
+    const int im = int(local / T);
+    s.b = b;
+    s.T = T;
+    s.t0 = int(local - int64_t(im) * T);
+    s.t1 = int(min(int64_t(T), s.t0 + (end - u)));
+    s.h = im / M;
+    s.row_base = (im - s.h * M) * 2 * ROWS;
+    s.rows = rows_of(a, b, s.r0);
+    s.live = min(s.rows * G - s.row_base, 2 * ROWS);
+    s.pair = s.live > ROWS;
+    s.start = start_of(a, b);
+    s.len = max(0, min(a.kv_len[b], a.cap - s.start));
+    s.first = a.kv_len[b] - s.rows;
+    s.kb = a.kv_batch == 1 ? 0 : b;
+    u += s.t1 - s.t0;
+    return true;
+  }
+};
+
+// Ring use (within the segment) of the V tile of local tile t: the order of loads is K0 V0 K1 V1 ..
+// (pair) or K0 K1 V0 K2 V1 .. (tiles alternate between the slots).
+__device__ __forceinline__ int v_use(bool pair, int t, int n) {
+  return pair ? 2 * t + 1 : t == n - 1 ? 2 * n - 1 : 2 * t + 2;
+}
+
+// Whether a row (its ancestor words, or its place in a chain) sees tree place j.
+__device__ __forceinline__ bool sees(const uint32_t* anc, int words, int place, int j) {
+  return anc ? j < 32 * words && ((anc[j >> 5] >> (j & 31)) & 1u) : j <= place;
+}
+
+// The 128 visibility bits of a tile for one row; key k0 + c is bit c.
+__device__ __forceinline__ void tile_bits(const dspark_tree_attn_args& a, const Segment& s, int r, int i,
+                                          int k0, uint32_t* w) {
 #pragma unroll
-  for (int e = 0; e < VPL; ++e) out[lane + 32 * e] = Elem<T>::from_f(o[e] * inv);
+  for (int x = 0; x < 4; ++x) {
+    const int j = k0 + 32 * x - s.first;  // tree place of the word's first key
+    uint32_t bits;
+    if (j > -32) {
+      uint32_t lo = 0, hi = 0;  // tree places [jw, jw + 64) that the row sees
+      const int jw = j >= 0 ? j >> 5 : -1;
+      if (a.anc) {
+        const uint32_t* row = a.anc + int64_t(r) * a.anc_words;
+        lo = jw >= 0 && jw < a.anc_words ? row[jw] : jw < 0 ? 0xffffffffu : 0u;
+        hi = jw + 1 < a.anc_words ? row[jw + 1] : 0u;
+      } else {
+        const int n0 = i + 1 - 32 * jw, n1 = n0 - 32;
+        lo = jw < 0 || n0 >= 32 ? 0xffffffffu : n0 > 0 ? (1u << n0) - 1u : 0u;
+        hi = n1 >= 32 ? 0xffffffffu : n1 > 0 ? (1u << n1) - 1u : 0u;
+      }
+      bits = __funnelshift_r(lo, hi, uint32_t(j - 32 * jw));
+    } else {
+      bits = 0xffffffffu;
+    }
+    const int n = s.len - (k0 + 32 * x);  // keys that exist
+    w[x] = n >= 32 ? bits : n > 0 ? bits & ((1u << n) - 1u) : 0u;
+  }
+}
+
+// A tile whose V rows are not all plain values of visible or cached keys: rows past the request's
+// keys are zeroed; non-finite values among the tree's keys are zeroed and reported (add_hidden
+// gives them to the rows that see them). Thread x of the warpgroup has key x of the tile.
+template <typename T, int D>
+__device__ __noinline__ void fix_values(uint8_t* tile, int key, int len, int first, int* flag,
+                                        int seg) {
+  const int x = threadIdx.x & 127;
+  const bool past = key + x >= len;
+  if (!past && key + x < first) return;
+  const uint32_t em = Elem<T>::kExpMask;
+  bool bad = false;
+#pragma unroll 4
+  for (int c = 0; c < D / 8; ++c) {
+    uint4* p = reinterpret_cast<uint4*>(tile + (c >> 3) * Lay<D>::HALF + x * 128 + (((c & 7) ^ (x & 7)) << 4));
+    if (past) {
+      *p = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      uint4 v = *p;
+      uint32_t* w = &v.x;
+      bool hit = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if ((w[e] & em) == em) { w[e] &= 0xffff0000u; hit = true; }
+        if ((w[e] & (em << 16)) == (em << 16)) { w[e] &= 0x0000ffffu; hit = true; }
+      }
+      if (hit) {
+        *p = v;
+        bad = true;
+      }
+    }
+  }
+  if (bad) *flag = seg;
+}
+
+// The non-finite values that fix_values took out of the segment's tiles, added to what a row that
+// sees them has stored (`out`: the output, or `part`: the fp32 part).
+template <typename T>
+struct Hidden {
+  const T* v;             // the request's first value row of this kv head
+  int64_t stride;
+  const uint32_t* anc;    // the row's words, or null
+  int words, place, k0, k1, first, D;
+};
+
+template <typename T>
+__device__ __noinline__ void add_hidden(const Hidden<T> x, T* out, float* part) {
+  for (int k = x.k0; k < x.k1; ++k) {
+    if (!sees(x.anc, x.words, x.place, k - x.first)) continue;
+    for (int d = 0; d < x.D; ++d) {
+      const float v = Elem<T>::to_f(x.v[int64_t(k) * x.stride + d]);
+      if (isfinite(v)) continue;
+      if (part) part[d] += v;
+      else out[d] = Elem<T>::from_f(Elem<T>::to_f(out[d]) + v);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ workspace
+
+// Part `which` of CTA c: 256 rows of D values, then 256 (m, l).
+template <int D>
+__device__ __forceinline__ float* part(float* ws, int c, int which) {
+  return ws + int64_t(2 * c + which) * (2 * ROWS) * (D + 2);
+}
+
+// ------------------------------------------------------------------ the kernel
+
+template <typename T, int D>
+__global__ void __launch_bounds__(NTHR, 1)
+    attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                const dspark_tree_attn_args a, const float c_log2, const float q_sign, int* status) {
+  typedef Lay<D> L;
+  constexpr int NB = L::NB;
+  constexpr uint32_t FMT = std::is_same<T, bf16>::value ? 1u : 0u;
+  constexpr uint32_t ID_QK = (1u << 4) | (FMT << 7) | (FMT << 10) | (uint32_t(BN >> 3) << 17) |
+                             (uint32_t(ROWS >> 4) << 24);
+  constexpr uint32_t ID_PV = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) |
+                             (uint32_t(D >> 3) << 17) | (uint32_t(ROWS >> 4) << 24);
+  constexpr uint32_t O_COL = 256;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_align_up<1024>(smem_raw);
+  uint8_t* ring = smem + L::RING;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BARS);
+  uint64_t* empty = full + NB;
+  uint64_t* q_full = empty + NB;
+  uint64_t* s_full = q_full + 2;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* fin = o_full + 2;
+  float2* stat = reinterpret_cast<float2*>(smem + L::STAT);
+  int* flag = reinterpret_cast<int*>(smem + L::STAT + ROWS * 8);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(flag + 2);
+  __shared__ int64_t scan[36];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < NB; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 128);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_full[i], 1);
+      flag[i] = 0;
+    }
+    mbar_init(fin, 1);
+    fence_mbar_init();
+    prefetch_tmap(&kmap);
+    prefetch_tmap(&vmap);
+  }
+  if (warp == WARP_MMA) tcg::tmem_alloc(tmem_slot, 512);
+  pdl_launch_dependents();
+  pdl_wait();
+  const int cta = blockIdx.x, n_cta = gridDim.x;
+  const Place pl = locate(a, scan, [&](int64_t total) { return range_begin(total, cta, n_cta); });
+  tcg::tc_fence_before();
+  __syncthreads();
+  tcg::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Walker wk{range_begin(pl.total, cta, n_cta), range_begin(pl.total, cta + 1, n_cta), pl.base, pl.b};
+  Segment s;
+  bool ok = true;
+
+  if (warp < 8) {
+    // ---------------------------------------------------------------- softmax, slot = warpgroup
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int slot = warp >> 2, row = tid & 127;
+    const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lane_base + uint32_t(slot * 128);
+    const uint32_t t_o = tmem + lane_base + O_COL + uint32_t(slot * 128);
+    uint8_t* qs = smem + L::Q + slot * L::TILE;
+    const int G = a.Hq / a.Hk;
+    uint32_t n_s = 0, n_o = 0;  // completed phases of s_full / o_full
+    int use0 = 0;               // ring uses before this segment
+    // flag[seg & 1] == seg: a hidden non-finite value in segment `seg`. One slot may be a segment
+    // ahead of the other, never two: the products of a segment need both slots' weights.
+    for (int seg = 1; wk.next(a, s); ++seg) {
+      const int n = s.t1 - s.t0;
+      const int steps = s.pair ? n : (n - slot + 1) >> 1;
+      const int my = s.row_base + (s.pair ? slot * ROWS : 0) + row;  // (node, head) row of this thread
+      const bool alive = my < s.rows * G;
+      const int place = alive ? my / G : 0;
+      const bool warp_alive = s.row_base + (s.pair ? slot * ROWS : 0) + (warp & 3) * 32 < s.rows * G;
+      float m = -INFINITY, l = 0.f;
+      if (steps > 0) {
+        // this slot's Q tile; the last scores that read the old one have arrived
+        constexpr int CH = D / 8;  // 16-byte chunks a row
+        const int c = row % CH;
+        const T* q = static_cast<const T*>(a.q);
+#pragma unroll
+        for (int part8 = 0; part8 < CH / 8; ++part8) {
+          uint4 v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int rr = row / CH + (part8 * 8 + i) * (128 / CH);
+            const int x = my - row + rr;
+            v[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (x < s.rows * G) {
+              const int node = x / G, hq = s.h * G + x - node * G;
+              v[i] = ldcg_v4(q + int64_t(s.r0 + node) * a.q_strides[0] + hq * a.q_strides[1] + c * 8);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int rr = row / CH + (part8 * 8 + i) * (128 / CH);
+            if (q_sign != 1.f) {
+              uint32_t* w = &v[i].x;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 f = Elem<T>::unpack(w[e]);
+                w[e] = Elem<T>::pack(f.x * q_sign, f.y * q_sign);
+              }
+            }
+            *reinterpret_cast<uint4*>(qs + (c >> 3) * L::HALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
+          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&q_full[slot]);
+      }
+      for (int j = 0; j < steps; ++j) {
+        const int t = s.pair ? j : 2 * j + slot;  // tile of the segment
+        const int k0 = (s.t0 + t) * BN;
+        if (ok) ok = mbar_wait(&s_full[slot], n_s & 1, status, kErrWaitMma);
+        ++n_s;
+        tcg::tc_fence_after();
+        const bool edge = k0 + BN > s.first || k0 + BN > s.len;
+        if (warp_alive) {
+          float x[128];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ld_x32(t_s + uint32_t(32 * i), x + 32 * i);
+          tcg::tmem_wait_ld();
+          if (edge) {
+            uint32_t w[4];
+            tile_bits(a, s, s.r0 + place, place, k0, w);
+#pragma unroll
+            for (int i = 0; i < 128; ++i) x[i] = (w[i >> 5] >> (i & 31)) & 1u ? x[i] : -INFINITY;
+          }
+          float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+          for (int i = 4; i < 128; i += 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], x[i + e]);
+          }
+          const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const bool raise = (mt - m) * c_log2 > 8.f;
+          if (__any_sync(0xffffffffu, raise)) {
+            const float mn = raise ? mt : m;
+            const float f = raise ? ex2((m - mn) * c_log2) : 1.f;
+            m = mn;
+            l *= f;
+            if (j > 0) {
+#pragma unroll
+              for (int i = 0; i < D / 32; ++i) {
+                float o[32];
+                ld_x32(t_o + uint32_t(32 * i), o);
+                tcg::tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] *= f;
+                tcg::tmem_st32(t_o + uint32_t(32 * i), reinterpret_cast<const uint32_t*>(o));
+              }
+            }
+          }
+          const float mc = m == -INFINITY ? 0.f : m * c_log2;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t p[32];
+#pragma unroll
+            for (int i = 0; i < 64; i += 4) {
+              float e[4];
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                e[y] = ex2(fmaf(x[64 * h + i + y], c_log2, -mc));
+                sum[y] += e[y];
+              }
+              p[i / 2] = Elem<T>::pack(e[0], e[1]);
+              p[i / 2 + 1] = Elem<T>::pack(e[2], e[3]);
+            }
+            tcg::tmem_st32(t_s + uint32_t(32 * h), p);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+        if (edge && (slot == 0 || !s.pair)) {
+          const int g = use0 + v_use(s.pair, t, n);
+          if (ok) ok = mbar_wait(&full[g % NB], uint32_t(g / NB) & 1u, status, kErrWaitKV);
+          fix_values<T, D>(ring + (g % NB) * L::TILE, k0, s.len, s.first, flag + (seg & 1), seg);
+          fence_proxy_async_smem();
+        }
+        tcg::tmem_wait_st();
+        tcg::tc_fence_before();
+        mbar_arrive(&p_full[slot]);
+      }
+      use0 += 2 * n;
+      // ---- end of the segment
+      if (steps > 0) {
+        if (ok) ok = mbar_wait(&o_full[slot], n_o & 1, status, kErrWaitMma);
+        ++n_o;
+        tcg::tc_fence_after();
+      }
+      const bool whole = s.t0 == 0 && s.t1 == s.T;
+      float* xch = reinterpret_cast<float*>(smem + L::Q);  // [D][128] fp32: both Q tiles
+      if (!s.pair) named_sync(1, 256);  // both slots are done with their Q tiles (and flags are set)
+      if (!s.pair && slot == 1) {
+        stat[row] = make_float2(m, l);
+        if (steps > 0 && warp_alive) {
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            float o[32];
+            ld_x32(t_o + uint32_t(32 * i), o);
+            tcg::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) xch[(32 * i + e) * 128 + row] = o[e];
+          }
+        }
+        named_sync(1, 256);
+      } else {
+        float f0 = 1.f, f1 = 0.f;
+        bool both = false;
+        if (!s.pair) {
+          named_sync(1, 256);
+          if (n > 1) {
+            const float2 st = stat[row];
+            const float mn = fmaxf(m, st.x), ref = mn == -INFINITY ? 0.f : mn;
+            f0 = ex2((m - ref) * c_log2);
+            f1 = ex2((st.x - ref) * c_log2);
+            l = l * f0 + st.y * f1;
+            m = mn;
+            both = true;
+          }
+        }
+        const bool hidden = *reinterpret_cast<volatile int*>(&flag[seg & 1]) == seg;
+        if (warp_alive) {
+          const int hq = s.h * G + my - place * G;
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          float* pp = whole ? nullptr : part<D>(static_cast<float*>(a.workspace), cta, s.t0 == 0 ? 1 : 0);
+          const int prow = (s.pair ? slot * ROWS : 0) + row;
+          T* out = static_cast<T*>(a.out) + int64_t(s.r0 + place) * a.o_strides[0] + hq * a.o_strides[1];
+          if (!whole && alive)
+            reinterpret_cast<float2*>(pp + 2 * ROWS * D)[prow] = make_float2(m * c_log2, l);
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            float o[32];
+            ld_x32(t_o + uint32_t(32 * i), o);
+            tcg::tmem_wait_ld();
+            if (both) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = o[e] * f0 + xch[(32 * i + e) * 128 + row] * f1;
+            }
+            if (alive) {
+              if (whole) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                  uint4 v;
+                  v.x = Elem<T>::pack(o[e] * inv, o[e + 1] * inv);
+                  v.y = Elem<T>::pack(o[e + 2] * inv, o[e + 3] * inv);
+                  v.z = Elem<T>::pack(o[e + 4] * inv, o[e + 5] * inv);
+                  v.w = Elem<T>::pack(o[e + 6] * inv, o[e + 7] * inv);
+                  *reinterpret_cast<uint4*>(out + 32 * i + e) = l == 0.f ? make_uint4(0u, 0u, 0u, 0u) : v;
+                }
+              } else {
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                  *reinterpret_cast<float4*>(pp + int64_t(prow) * D + 32 * i + e) =
+                      make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+              }
+            }
+          }
+          if (hidden && alive) {
+            Hidden<T> hd;
+            hd.v = static_cast<const T*>(a.v) + s.kb * a.v_strides[0] + s.h * a.v_strides[1] +
+                   int64_t(s.start) * a.v_strides[2];
+            hd.stride = a.v_strides[2];
+            hd.anc = a.anc ? a.anc + int64_t(s.r0 + place) * a.anc_words : nullptr;
+            hd.words = a.anc_words;
+            hd.place = place;
+            hd.k0 = max(s.t0 * BN, max(s.first, 0));
+            hd.k1 = min(s.t1 * BN, s.len);
+            hd.first = s.first;
+            hd.D = D;
+            add_hidden<T>(hd, out, whole ? nullptr : pp + int64_t(prow) * D);
+          }
+        }
+      }
+      if (!s.pair) {
+        named_sync(1, 256);  // the exchange has been read: the next segment's Q may land there
+      }
+      tcg::tc_fence_before();
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == WARP_TMA) {
+      // -------------------------------------------------------------- producer
+      if (lane == 0) {
+        int g = 0;
+        auto load = [&](const CUtensorMap* map, int tile) {
+          const int x = g % NB;
+          if (g >= NB && ok)
+            ok = mbar_wait(&empty[x], uint32_t(g / NB - 1) & 1u, status, kErrWaitKVEmpty);
+          if (!ok) return;
+          mbar_arrive_expect_tx(&full[x], L::TILE);
+#pragma unroll
+          for (int d = 0; d < D / 64; ++d)
+            tma_load_4d(ring + x * L::TILE + d * L::HALF, map, &full[x], d * 64,
+                        s.start + (s.t0 + tile) * BN, s.h, s.kb);
+          ++g;
+        };
+        while (ok && wk.next(a, s)) {
+          const int n = s.t1 - s.t0;
+          load(&kmap, 0);
+          if (!s.pair && n > 1) load(&kmap, 1);
+          const int ahead = s.pair ? 1 : 2;
+          for (int t = 0; t < n && ok; ++t) {
+            load(&vmap, t);
+            if (t + ahead < n) load(&kmap, t + ahead);
+          }
+        }
+        // no copy may still be in flight when the CTA exits
+        for (int i = max(0, g - NB); i < g; ++i)
+          mbar_wait(&full[i % NB], uint32_t(i / NB) & 1u, status, kErrWaitKV);
+      }
+      __syncwarp();
+    } else if (warp == WARP_MMA) {
+      // -------------------------------------------------------------- products
+      if (tcg::elect_one()) {
+        int g = 0;
+        uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0};
+        bool issued = false;
+        auto take = [&]() {  // the next ring buffer, filled
+          const int x = g % NB;
+          if (ok) ok = mbar_wait(&full[x], uint32_t(g / NB) & 1u, status, kErrWaitKV);
+          tcg::tc_fence_after();
+          ++g;
+          return x;
+        };
+        auto scores = [&](int slot, int x) {
+          if (!ok) return;
+          const uint64_t qd = desc_sw128(smem_u32(smem + L::Q + slot * L::TILE), 16);
+          const uint64_t kd = desc_sw128(smem_u32(ring + x * L::TILE), 16);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint64_t off = uint64_t((k >> 2) * (L::HALF >> 4) + (k & 3) * 2);
+            umma_ss(tmem + uint32_t(slot * 128), qd + off, kd + off, ID_QK, k ? 1u : 0u);
+          }
+          tcg::umma_commit(&s_full[slot]);
+          issued = true;
+        };
+        auto values = [&](int slot, int x, bool first) {
+          if (ok) ok = mbar_wait(&p_full[slot], n_p[slot]++ & 1u, status, kErrWaitMma);
+          if (!ok) return;
+          tcg::tc_fence_after();
+          const uint64_t vd = desc_sw128(smem_u32(ring + x * L::TILE), L::HALF);
+#pragma unroll
+          for (int k = 0; k < BN / 16; ++k)
+            tcg::umma_ts(tmem + O_COL + uint32_t(slot * 128), tmem + uint32_t(slot * 128 + 8 * k),
+                         vd + uint64_t(k * (2048 >> 4)), ID_PV, first && k == 0 ? 0u : 1u);
+          issued = true;
+        };
+        auto release = [&](int x) {
+          if (ok) tcg::umma_commit(&empty[x]);
+        };
+        auto q_ready = [&](int slot) {
+          if (ok) ok = mbar_wait(&q_full[slot], n_q[slot]++ & 1u, status, kErrWaitMma);
+          tcg::tc_fence_after();
+        };
+        while (ok && wk.next(a, s)) {
+          const int n = s.t1 - s.t0;
+          if (s.pair) {
+            int x = take();
+            q_ready(0);
+            scores(0, x);
+            q_ready(1);
+            scores(1, x);
+            release(x);
+            for (int t = 0; t < n && ok; ++t) {
+              const int v = take();
+              const bool more = t + 1 < n;
+              values(0, v, t == 0);
+              if (!more && ok) tcg::umma_commit(&o_full[0]);
+              if (more) {
+                x = take();
+                scores(0, x);
+              }
+              values(1, v, t == 0);
+              release(v);
+              if (more) {
+                scores(1, x);
+                release(x);
+              } else if (ok) {
+                tcg::umma_commit(&o_full[1]);
+              }
+            }
+          } else {
+            for (int z = 0; z < min(n, 2); ++z) {
+              const int x = take();
+              q_ready(z);
+              scores(z, x);
+              release(x);
+            }
+            for (int t = 0; t < n && ok; ++t) {
+              const int v = take(), z = t & 1;
+              values(z, v, t < 2);
+              release(v);
+              if (t + 2 < n) {
+                const int x = take();
+                scores(z, x);
+                release(x);
+              } else if (ok) {
+                tcg::umma_commit(&o_full[z]);
+              }
+            }
+          }
+        }
+        if (issued) {  // nothing may write tensor memory after the CTA releases it
+          tcg::umma_commit(fin);
+          mbar_wait(fin, 0, status, kErrWaitMma);
+        }
+      }
+      __syncwarp();
+    }
+  }
+  tcg::tc_fence_before();
+  __syncthreads();
+  tcg::tc_fence_after();
+  if (warp == WARP_MMA) tcg::tmem_dealloc(tmem, 512);
+}
+
+// Joins the parts of the item that the boundary between CTAs c and c + 1 cuts (once: at the item's
+// first boundary). Block (c, y): rows 32 y .. 32 y + 31 of the item, a warp a row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) merge_kernel(const dspark_tree_attn_args a, const int n_cta) {
+  pdl_launch_dependents();
+  pdl_wait();
+  __shared__ int64_t scan[36];
+  const int c = blockIdx.x;
+  const Place pl = locate(a, scan, [&](int64_t total) { return range_begin(total, c + 1, n_cta); });
+  const int64_t u = range_begin(pl.total, c + 1, n_cta);
+  if (u >= pl.total || u == range_begin(pl.total, c, n_cta)) return;
+  int M, T_;
+  extents(a, pl.b, M, T_);
+  const int64_t im = (u - pl.base) / T_, u0 = pl.base + im * T_;
+  if (u == u0 || range_begin(pl.total, c, n_cta) > u0) return;  // cut elsewhere, or before
+  const int h = int(im / M), row_base = int(im - int64_t(h) * M) * 2 * ROWS, G = a.Hq / a.Hk;
+  int r0;
+  const int rows = rows_of(a, pl.b, r0);
+  const int live = min(rows * G - row_base, 2 * ROWS);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* ws = static_cast<float*>(a.workspace);
+  constexpr int VPL = D / 32;
+  for (int i = blockIdx.y * 32 + warp; i < min(live, int(blockIdx.y) * 32 + 32); i += 8) {
+    float m = -INFINITY, l = 0.f, o[VPL];
+#pragma unroll
+    for (int e = 0; e < VPL; ++e) o[e] = 0.f;
+    for (int x = c; x < n_cta; ++x) {
+      if (x > c && range_begin(pl.total, x, n_cta) >= u0 + T_) break;
+      if (x > c && range_begin(pl.total, x, n_cta) == range_begin(pl.total, x + 1, n_cta)) continue;
+      const float* p = part<D>(ws, x, x == c ? 1 : 0);
+      const float2 st = __ldcg(reinterpret_cast<const float2*>(p + 2 * ROWS * D) + i);
+      const float mn = fmaxf(m, st.x), ref = mn == -INFINITY ? 0.f : mn;
+      const float f0 = ex2(m - ref), f1 = ex2(st.x - ref);
+      m = mn;
+      l = l * f0 + st.y * f1;
+#pragma unroll
+      for (int e = 0; e < VPL; ++e) o[e] = o[e] * f0 + __ldcg(p + int64_t(i) * D + lane + 32 * e) * f1;
+    }
+    const int x = row_base + i, node = x / G, hq = h * G + x - node * G;
+    T* out = static_cast<T*>(a.out) + int64_t(r0 + node) * a.o_strides[0] + hq * a.o_strides[1];
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int e = 0; e < VPL; ++e) out[lane + 32 * e] = Elem<T>::from_f(l == 0.f ? 0.f : o[e] * inv);
+  }
+}
+
+static int grid_of(int device) { return sm_count(device); }
+
+template <typename T, int D>
+static int launch(const dspark_tree_attn_args& a, cudaStream_t s) {
+  const int dev = current_device();
+  int* st = status_word(dev);
+  CUtensorMap maps[2];
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* str = i ? a.v_strides : a.k_strides;
+    // a dimension of one entry is never stepped: any valid stride does
+    const uint64_t e = 2;
+    const uint64_t ss = a.cap > 1 ? str[2] * e : D * e;
+    const uint64_t sh = a.Hk > 1 ? str[1] * e : D * e;
+    const uint64_t sb = a.kv_batch > 1 ? str[0] * e : D * e;
+    const uint64_t dims[4] = {uint64_t(D), uint64_t(a.cap), uint64_t(a.Hk), uint64_t(a.kv_batch)};
+    const uint64_t strides[3] = {ss, sh, sb};
+    const uint32_t box[4] = {64, BN, 1, 1};
+    if (!encode_tmap_nd(&maps[i], std::is_same<T, bf16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        4, i ? a.v : a.k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return fail(DSPARK_ERR_UNSUPPORTED, "tree_attn: cache strides {%lld, %lld, %lld}",
+                  (long long)str[0], (long long)str[1], (long long)str[2]);
+  }
+  const int n_cta = grid_of(dev);
+  const size_t smem = Lay<D>::TOTAL;
+  DSPARK_CUDA_TRY(configure_once((const void*)attn_kernel<T, D>, int(smem),
+                                 [&] {
+                                   return cudaFuncSetAttribute(attn_kernel<T, D>,
+                                                               cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                               int(smem));
+                                 }),
+                  "tree_attn: shared memory");
+  // the running maximum needs a positive factor: the scale's sign goes into q
+  const float c = fabsf(a.scale) * 1.4426950408889634f;
+  const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
+  DSPARK_CUDA_TRY(launch_ex(attn_kernel<T, D>, dim3(n_cta), dim3(NTHR), smem, s, 1, true, maps[0], maps[1],
+                            a, sign == 0.f ? 1.f : c, sign, st),
+                  "tree_attn");
+  const int rows = std::min(2 * ROWS, a.max_rows * (a.Hq / a.Hk));
+  DSPARK_CUDA_TRY(launch_ex(merge_kernel<T, D>, dim3(n_cta, (rows + 31) / 32), dim3(256), 0, s, 1, true, a,
+                            n_cta),
+                  "tree_attn merge");
+  return DSPARK_OK;
 }
 
 }  // namespace tattn
@@ -94,8 +866,8 @@ using namespace dspark;
 extern "C" {
 
 size_t dspark_tree_attn_workspace(int B, int Hq, int Hk, int D, int max_rows) {
-  (void)B; (void)Hq; (void)Hk; (void)D; (void)max_rows;
-  return 0;
+  if (B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || D <= 0 || max_rows <= 0) return 0;
+  return size_t(tattn::grid_of(current_device())) * 2 * (2 * tattn::ROWS) * (D + 2) * sizeof(float);
 }
 
 int dspark_tree_attn(const dspark_tree_attn_args* p, void* stream) {
@@ -111,20 +883,20 @@ int dspark_tree_attn(const dspark_tree_attn_args* p, void* stream) {
   if (a.R == 0 || a.B == 0) return DSPARK_OK;
   if (a.kv_batch != 1 && a.kv_batch < a.B)
     return fail(DSPARK_ERR_ARG, "tree_attn: %d requests, %d cache entries", a.B, a.kv_batch);
+  if (a.cap == 0 || a.max_rows == 0) return fail(DSPARK_ERR_ARG, "tree_attn: empty cache or max_rows 0");
   if (!a.q || !a.k || !a.v || !a.out || !a.cu_rows || !a.kv_len)
     return fail(DSPARK_ERR_ARG, "tree_attn: null pointer");
   if (a.anc && a.anc_words <= 0) return fail(DSPARK_ERR_ARG, "tree_attn: %d words a row", a.anc_words);
+  bool aligned = true;
+  for (const void* x : {a.q, a.k, a.v, (const void*)a.out}) aligned &= reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  for (int i = 0; i < 2; ++i) aligned &= a.q_strides[i] % 8 == 0 && a.o_strides[i] % 8 == 0;
+  for (int i = 0; i < 3; ++i) aligned &= a.k_strides[i] % 8 == 0 && a.v_strides[i] % 8 == 0;
+  if (!aligned) return fail(DSPARK_ERR_UNSUPPORTED, "tree_attn: rows must be 16-byte aligned");
+  if (!a.workspace || a.ws_bytes < dspark_tree_attn_workspace(a.B, a.Hq, a.Hk, a.D, a.max_rows))
+    return fail(DSPARK_ERR_ARG, "tree_attn: workspace of %zu bytes", a.ws_bytes);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-#define DSPARK_TATTN(T, DD)                                                                        \
-  DSPARK_CUDA_TRY(launch_ex(tattn::simple_kernel<T, DD>, dim3(a.R, a.Hq), dim3(32), 0, s, 1, true, a), \
-                  "tree_attn")
-  if (a.dtype == DSPARK_DTYPE_BF16) {
-    if (a.D == 128) DSPARK_TATTN(bf16, 128); else DSPARK_TATTN(bf16, 64);
-  } else {
-    if (a.D == 128) DSPARK_TATTN(__half, 128); else DSPARK_TATTN(__half, 64);
-  }
-#undef DSPARK_TATTN
-  return DSPARK_OK;
+  if (a.dtype == DSPARK_DTYPE_BF16) return a.D == 128 ? tattn::launch<bf16, 128>(a, s) : tattn::launch<bf16, 64>(a, s);
+  return a.D == 128 ? tattn::launch<__half, 128>(a, s) : tattn::launch<__half, 64>(a, s);
 }
 
 }  // extern "C"
