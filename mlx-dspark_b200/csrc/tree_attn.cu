@@ -39,7 +39,7 @@ namespace tattn {
 
 constexpr int BN = 128;       // keys a tile
 constexpr int ROWS = 128;     // rows a slot
-constexpr int NTHR = 384;     // two softmax warpgroups, producer, MMA, two idle warps
+constexpr int NTHR = 384;     // two softmax warpgroups; producer, MMA and two idle warps
 constexpr int WARP_TMA = 8, WARP_MMA = 9;
 
 template <int D>
@@ -49,16 +49,55 @@ struct Lay {
   static constexpr int NB = D == 128 ? 5 : 10;    // ring buffers
   static constexpr int Q = 0;
   static constexpr int RING = 2 * TILE;
-  static constexpr int BARS = RING + NB * TILE;
-  static constexpr int NBAR = 2 * NB + 2 + 2 + 2 + 2 + 1;
-  static constexpr int STAT = (BARS + NBAR * 8 + 15) / 16 * 16;  // slot 1's (m, l) by row, flags, scan
-  static constexpr int TOTAL = STAT + ROWS * 8 + 256 + 1024;     // slack to align the base
+  static constexpr int M1 = RING + NB * TILE;     // slot 1's (m, l) at the segment's end; a scan
+  static constexpr int FLAG = M1 + ROWS * 8;
+  static constexpr int SEG = FLAG + 16;             // [slot] the softmax threads' segment and walker
+  static constexpr int BARS = SEG + 2 * 96;
+  static constexpr int NBAR = 2 * NB + 2 + 2 + 2 + 2 + 2 + 1;
+  static constexpr int TOTAL = BARS + NBAR * 8;
+  static_assert(TOTAL <= 232448, "shared memory of one SM");
 };
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two fp32 values in one 64-bit register, and the packed operations on them (sm_100).
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// The largest of three; NaN if one of them is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+__device__ __forceinline__ void st_x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 
 __device__ __forceinline__ void ld_x32(uint32_t taddr, float* d) {
@@ -90,13 +129,14 @@ __device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t a_desc, uint64
 
 // 128-byte-swizzled operand: K-major (lbo unused, 8-row groups 1024 bytes apart) or MN-major (lbo
 // between 64-value blocks of MN, 8-row groups of K 1024 bytes apart).
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo) {
-  uint64_t d = 0;
-  d |= uint64_t((addr >> 4) & 0x3FFF);
-  d |= uint64_t((lbo >> 4) & 0x3FFF) << 16;
-  d |= uint64_t(1024 >> 4) << 32;
-  d |= uint64_t(1) << 46;
-  d |= uint64_t(2) << 61;
+// Only the low word (address, lbo) varies: steps along the tile are added to it.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) {
+  return ((addr >> 4) & 0x3FFF) | ((lbo >> 4) << 16);
+}
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t lo) {
+  constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);  // sbo, version, 128-byte swizzle
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(HI));
   return d;
 }
 
@@ -194,7 +234,9 @@ __device__ Place locate(const dspark_tree_attn_args& a, int64_t* scan, F&& of) {
   return Place{total, found[0], int(found[1])};
 }
 
-__device__ __forceinline__ int64_t range_begin(int64_t total, int c, int n) { return total * c / n; }
+__device__ __forceinline__ int64_t range_begin(int64_t total, int c, int n) {
+  return n ? min(total, total * c / n) : 0;
+}
 
 // One run of key tiles of one item.
 struct Segment {
@@ -207,7 +249,7 @@ struct Segment {
 };
 
 struct Walker {
-  int64_t u, end, base;
+  int64_t u, end, base;  // next unit, end of the range, first unit of request b
   int b;
   __device__ __forceinline__ bool next(const dspark_tree_attn_args& a, Segment& s) {
     if (u >= end) return false;
@@ -240,6 +282,15 @@ struct Walker {
   }
 };
 
+// What the softmax threads of a slot share: the segment at hand and where the next one starts. It
+// lives in shared memory because their registers hold scores.
+struct Shared {
+  Segment s;
+  int more;
+  Walker w;
+};
+static_assert(sizeof(Shared) <= 96, "Lay::SEG");
+
 // Ring use (within the segment) of the V tile of local tile t: the order of loads is K0 V0 K1 V1 ..
 // (pair) or K0 K1 V0 K2 V1 .. (tiles alternate between the slots).
 __device__ __forceinline__ int v_use(bool pair, int t, int n) {
@@ -251,7 +302,13 @@ __device__ __forceinline__ bool sees(const uint32_t* anc, int words, int place, 
   return anc ? j < 32 * words && ((anc[j >> 5] >> (j & 31)) & 1u) : j <= place;
 }
 
-// The 128 visibility bits of a tile for one row; key k0 + c is bit c.
+// The place within its request of a slot's row (0 where there is none).
+__device__ __forceinline__ int place_of(const dspark_tree_attn_args& a, const Segment& s, int slot, int row) {
+  const int G = a.Hq / a.Hk, my = s.row_base + (s.pair ? slot * ROWS : 0) + row;
+  return my < s.rows * G ? my / G : 0;
+}
+
+// The visibility bits of a tile's keys for one row; key k0 + c is bit c.
 __device__ __forceinline__ void tile_bits(const dspark_tree_attn_args& a, const Segment& s, int r, int i,
                                           int k0, uint32_t* w) {
 #pragma unroll
@@ -338,10 +395,18 @@ __device__ __noinline__ void add_hidden(const Hidden<T> x, T* out, float* part) 
 
 // ------------------------------------------------------------------ workspace
 
-// Part `which` of CTA c: 256 rows of D values, then 256 (m, l).
+// What the merge needs to know of an item cut by CTA c's end (its first part is c's second one, the
+// others are the first parts of CTAs c + 1 ..): written by c, parts 0 where there is none.
+struct Cut {
+  int parts, r0, live, row_base, h, pad[3];
+};
+constexpr int MAX_CTA = 256;
+
+// The workspace: a Cut a CTA, then part `which` of CTA c: 256 rows of D values, then 256 (m, l).
 template <int D>
-__device__ __forceinline__ float* part(float* ws, int c, int which) {
-  return ws + int64_t(2 * c + which) * (2 * ROWS) * (D + 2);
+__device__ __forceinline__ float* part(void* ws, int c, int which) {
+  return reinterpret_cast<float*>(static_cast<Cut*>(ws) + MAX_CTA) +
+         int64_t(2 * c + which) * (2 * ROWS) * (D + 2);
 }
 
 // ------------------------------------------------------------------ the kernel
@@ -358,31 +423,36 @@ __global__ void __launch_bounds__(NTHR, 1)
   constexpr uint32_t ID_PV = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) |
                              (uint32_t(D >> 3) << 17) | (uint32_t(ROWS >> 4) << 24);
   constexpr uint32_t O_COL = 256;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_align_up<1024>(smem_raw);
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* ring = smem + L::RING;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BARS);
   uint64_t* empty = full + NB;
   uint64_t* q_full = empty + NB;
   uint64_t* s_full = q_full + 2;
   uint64_t* p_full = s_full + 2;
-  uint64_t* o_full = p_full + 2;
+  uint64_t* p_part = p_full + 2;
+  uint64_t* o_full = p_part + 2;
   uint64_t* fin = o_full + 2;
-  float2* stat = reinterpret_cast<float2*>(smem + L::STAT);
-  int* flag = reinterpret_cast<int*>(smem + L::STAT + ROWS * 8);
+  float2* ml1 = reinterpret_cast<float2*>(smem + L::M1);
+  int* flag = reinterpret_cast<int*>(smem + L::FLAG);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(flag + 2);
-  __shared__ int64_t scan[36];
+  int64_t* scan = reinterpret_cast<int64_t*>(smem + L::M1);  // before the first segment's end
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (smem_u32(smem) & 1023u) {  // the swizzled tiles need it; never seen without static arrays
+    if (tid == 0) report_error(status, 0x205);
+    return;
+  }
   if (tid == 0) {
     for (int i = 0; i < NB; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 128);
+    for (int i = 0; i < 2; ++i) {  // the softmax barriers count warps
+      mbar_init(&q_full[i], 4);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_part[i], 4);
+      mbar_init(&p_full[i], 4);
       mbar_init(&o_full[i], 1);
       flag[i] = 0;
     }
@@ -394,79 +464,101 @@ __global__ void __launch_bounds__(NTHR, 1)
   if (warp == WARP_MMA) tcg::tmem_alloc(tmem_slot, 512);
   pdl_launch_dependents();
   pdl_wait();
-  const int cta = blockIdx.x, n_cta = gridDim.x;
-  const Place pl = locate(a, scan, [&](int64_t total) { return range_begin(total, cta, n_cta); });
+  const int cta = blockIdx.x;
+  // with fewer units than CTAs, the first `total` CTAs take one each
+  const Place pl = locate(a, scan, [&](int64_t total) {
+    return range_begin(total, cta, int(min(int64_t(gridDim.x), total)));
+  });
+  const int n_cta = int(min(int64_t(gridDim.x), pl.total));
   tcg::tc_fence_before();
   __syncthreads();
   tcg::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Walker wk{range_begin(pl.total, cta, n_cta), range_begin(pl.total, cta + 1, n_cta), pl.base, pl.b};
-  Segment s;
+  Walker wk{0, 0, pl.base, pl.b};
+  if (cta < n_cta) {
+    wk.u = range_begin(pl.total, cta, n_cta);
+    wk.end = range_begin(pl.total, cta + 1, n_cta);
+  }
   bool ok = true;
 
-  if (warp < 8) {
-    // ---------------------------------------------------------------- softmax, slot = warpgroup
+  if (warp < WARP_TMA) {
+    // ------------------------------------------- softmax: slot = warpgroup, row = TMEM lane
+    // (registers: 256 * 216 + 128 * 72 = 384 * 168, what the block was launched with)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int slot = warp >> 2, row = tid & 127;
-    const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lane_base + uint32_t(slot * 128);
-    const uint32_t t_o = tmem + lane_base + O_COL + uint32_t(slot * 128);
-    uint8_t* qs = smem + L::Q + slot * L::TILE;
-    const int G = a.Hq / a.Hk;
+    const uint32_t t_s = tmem + (uint32_t((warp & 3) * 32) << 16) + uint32_t(slot * 128);
+    const uint32_t t_o = t_s + O_COL;
+    Shared& sh = *reinterpret_cast<Shared*>(smem + L::SEG + 96 * slot);
+    const Segment& s = sh.s;
+    if (row == 0) {
+      sh.more = wk.next(a, sh.s);
+      sh.w = wk;
+    }
+    named_sync(1 + slot, 128);
+    if (tid == 0) static_cast<Cut*>(a.workspace)[cta] = Cut{};
     uint32_t n_s = 0, n_o = 0;  // completed phases of s_full / o_full
     int use0 = 0;               // ring uses before this segment
+    auto arrive = [&](uint64_t* bar) {  // this warp's stores to tensor memory are done
+      tcg::tmem_wait_st();
+      tcg::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
     // flag[seg & 1] == seg: a hidden non-finite value in segment `seg`. One slot may be a segment
     // ahead of the other, never two: the products of a segment need both slots' weights.
-    for (int seg = 1; wk.next(a, s); ++seg) {
+    for (int seg = 1; sh.more; ++seg) {
       const int n = s.t1 - s.t0;
-      const int steps = s.pair ? n : (n - slot + 1) >> 1;
-      const int my = s.row_base + (s.pair ? slot * ROWS : 0) + row;  // (node, head) row of this thread
-      const bool alive = my < s.rows * G;
-      const int place = alive ? my / G : 0;
-      const bool warp_alive = s.row_base + (s.pair ? slot * ROWS : 0) + (warp & 3) * 32 < s.rows * G;
+      const bool pair = s.pair;
+      const int steps = pair ? n : (n - slot + 1) >> 1;
+      const int tile0 = pair ? s.t0 : s.t0 + slot, tstep = pair ? 1 : 2;
+      const int edge0 = min(s.first, s.len) - BN;  // a tile from a later key on has hidden keys
+      bool warp_alive;
+      {
+        const int G = a.Hq / a.Hk;
+        warp_alive = s.row_base + (pair ? slot * ROWS : 0) + (warp & 3) * 32 < s.rows * G;
+      }
       float m = -INFINITY, l = 0.f;
       if (steps > 0) {
         // this slot's Q tile; the last scores that read the old one have arrived
-        constexpr int CH = D / 8;  // 16-byte chunks a row
-        const int c = row % CH;
+        constexpr int CH = D / 8;            // 16-byte chunks a row
+        constexpr int STEP = ROWS / CH;      // rows the warpgroup loads at a time
+        const int c = row % CH, first_row = row / CH;
+        const int G = a.Hq / a.Hk, row0 = s.row_base + (pair ? slot * ROWS : 0);
+        uint8_t* qs = smem + L::Q + slot * L::TILE;
         const T* q = static_cast<const T*>(a.q);
+        uint4 v[CH];
 #pragma unroll
-        for (int part8 = 0; part8 < CH / 8; ++part8) {
-          uint4 v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int rr = row / CH + (part8 * 8 + i) * (128 / CH);
-            const int x = my - row + rr;
-            v[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (x < s.rows * G) {
-              const int node = x / G, hq = s.h * G + x - node * G;
-              v[i] = ldcg_v4(q + int64_t(s.r0 + node) * a.q_strides[0] + hq * a.q_strides[1] + c * 8);
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int rr = row / CH + (part8 * 8 + i) * (128 / CH);
-            if (q_sign != 1.f) {
-              uint32_t* w = &v[i].x;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 f = Elem<T>::unpack(w[e]);
-                w[e] = Elem<T>::pack(f.x * q_sign, f.y * q_sign);
-              }
-            }
-            *reinterpret_cast<uint4*>(qs + (c >> 3) * L::HALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
+        for (int i = 0; i < CH; ++i) {
+          const int x = row0 + first_row + i * STEP;
+          v[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (x < s.rows * G) {
+            const int node = x / G, hq = s.h * G + x - node * G;
+            v[i] = ldcg_v4(q + int64_t(s.r0 + node) * a.q_strides[0] + hq * a.q_strides[1] + c * 8);
           }
         }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const int rr = first_row + i * STEP;
+          if (q_sign != 1.f) {
+            uint32_t* w = &v[i].x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = Elem<T>::unpack(w[e]);
+              w[e] = Elem<T>::pack(f.x * q_sign, f.y * q_sign);
+            }
+          }
+          *reinterpret_cast<uint4*>(qs + (c >> 3) * L::HALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
+        }
         fence_proxy_async_smem();
-        mbar_arrive(&q_full[slot]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[slot]);
       }
       for (int j = 0; j < steps; ++j) {
-        const int t = s.pair ? j : 2 * j + slot;  // tile of the segment
-        const int k0 = (s.t0 + t) * BN;
+        const int k0 = (tile0 + j * tstep) * BN;
+        const bool edge = k0 > edge0;
         if (ok) ok = mbar_wait(&s_full[slot], n_s & 1, status, kErrWaitMma);
         ++n_s;
         tcg::tc_fence_after();
-        const bool edge = k0 + BN > s.first || k0 + BN > s.len;
         if (warp_alive) {
           float x[128];
 #pragma unroll
@@ -474,17 +566,23 @@ __global__ void __launch_bounds__(NTHR, 1)
           tcg::tmem_wait_ld();
           if (edge) {
             uint32_t w[4];
+            const int place = place_of(a, s, slot, row);
             tile_bits(a, s, s.r0 + place, place, k0, w);
 #pragma unroll
             for (int i = 0; i < 128; ++i) x[i] = (w[i >> 5] >> (i & 31)) & 1u ? x[i] : -INFINITY;
           }
-          float mx[4] = {x[0], x[1], x[2], x[3]};
+          float mx[8];
 #pragma unroll
-          for (int i = 4; i < 128; i += 4) {
+          for (int e = 0; e < 8; ++e) mx[e] = max3(x[2 * e], x[2 * e + 1], x[16 + e]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], x[i + e]);
+          for (int i = 24; i < 120; i += 16) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx[e] = max3(mx[e], x[i + 2 * e], x[i + 2 * e + 1]);
           }
-          const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[120 + 2 * e], x[120 + 2 * e + 1]);
+          const float mt = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max3(mx[6], mx[7], mx[7]));
+          if (!(mt < INFINITY)) m = NAN;  // a visible score of +inf or NaN: the row is NaN
           const bool raise = (mt - m) * c_log2 > 8.f;
           if (__any_sync(0xffffffffu, raise)) {
             const float mn = raise ? mt : m;
@@ -493,45 +591,59 @@ __global__ void __launch_bounds__(NTHR, 1)
             l *= f;
             if (j > 0) {
 #pragma unroll
-              for (int i = 0; i < D / 32; ++i) {
-                float o[32];
-                ld_x32(t_o + uint32_t(32 * i), o);
+              for (int i = 0; i < D / 16; ++i) {
+                float o[16];
+                tcg::tmem_ld16(t_o + uint32_t(16 * i), o);
                 tcg::tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] *= f;
-                tcg::tmem_st32(t_o + uint32_t(32 * i), reinterpret_cast<const uint32_t*>(o));
+                for (int e = 0; e < 16; ++e) o[e] *= f;
+                st_x16(t_o + uint32_t(16 * i), reinterpret_cast<const uint32_t*>(o));
               }
             }
           }
           const float mc = m == -INFINITY ? 0.f : m * c_log2;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const f32x2 c2 = pack2(c_log2, c_log2), nm2 = pack2(-mc, -mc);
+          f32x2 sum[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t p[32];
+          for (int e = 0; e < 4; ++e) sum[e] = pack2(0.f, 0.f);
+          // pair by pair, sums and packing LAG pairs behind the exponentials: the special-function
+          // unit (8 cycles a warp instruction) then never waits for them
+          constexpr int LAG = 4;
+          f32x2 e[64];
+          uint32_t p[64];
 #pragma unroll
-            for (int i = 0; i < 64; i += 4) {
-              float e[4];
-#pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                e[y] = ex2(fmaf(x[64 * h + i + y], c_log2, -mc));
-                sum[y] += e[y];
-              }
-              p[i / 2] = Elem<T>::pack(e[0], e[1]);
-              p[i / 2 + 1] = Elem<T>::pack(e[2], e[3]);
+          for (int i = 0; i < 64 + LAG; ++i) {
+            if (i < 64) {
+              float e0, e1;
+              unpack2(fma2(pack2(x[2 * i], x[2 * i + 1]), c2, nm2), e0, e1);
+              e[i] = pack2(ex2(e0), ex2(e1));
             }
-            tcg::tmem_st32(t_s + uint32_t(32 * h), p);
+            const int z = i - LAG;
+            if (z >= 0) {
+              float e0, e1;
+              unpack2(e[z], e0, e1);
+              sum[z & 3] = add2(sum[z & 3], e[z]);
+              p[z] = Elem<T>::pack(e0, e1);
+              if ((z & 15) == 15) st_x16(t_s + uint32_t(z - 15), p + z - 15);
+              if (z == 47 && !edge) arrive(&p_part[slot]);  // three quarters' products may start
+            }
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          float s0, s1;
+          unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
+          l += s0 + s1;
+        } else if (!edge) {
+          arrive(&p_part[slot]);
         }
-        if (edge && (slot == 0 || !s.pair)) {
-          const int g = use0 + v_use(s.pair, t, n);
-          if (ok) ok = mbar_wait(&full[g % NB], uint32_t(g / NB) & 1u, status, kErrWaitKV);
-          fix_values<T, D>(ring + (g % NB) * L::TILE, k0, s.len, s.first, flag + (seg & 1), seg);
-          fence_proxy_async_smem();
+        if (edge) {
+          if (slot == 0 || !pair) {
+            const int g = use0 + v_use(pair, k0 / BN - s.t0, n);
+            if (ok) ok = mbar_wait(&full[g % NB], uint32_t(g / NB) & 1u, status, kErrWaitKV);
+            fix_values<T, D>(ring + (g % NB) * L::TILE, k0, s.len, s.first, flag + (seg & 1), seg);
+            fence_proxy_async_smem();
+          }
+          arrive(&p_part[slot]);  // not before: V had to be looked at
         }
-        tcg::tmem_wait_st();
-        tcg::tc_fence_before();
-        mbar_arrive(&p_full[slot]);
+        arrive(&p_full[slot]);
       }
       use0 += 2 * n;
       // ---- end of the segment
@@ -541,10 +653,14 @@ __global__ void __launch_bounds__(NTHR, 1)
         tcg::tc_fence_after();
       }
       const bool whole = s.t0 == 0 && s.t1 == s.T;
-      float* xch = reinterpret_cast<float*>(smem + L::Q);  // [D][128] fp32: both Q tiles
-      if (!s.pair) named_sync(1, 256);  // both slots are done with their Q tiles (and flags are set)
-      if (!s.pair && slot == 1) {
-        stat[row] = make_float2(m, l);
+      const int G = a.Hq / a.Hk;
+      const int my = s.row_base + (pair ? slot * ROWS : 0) + row;  // (node, head) row of this thread
+      const bool alive = my < s.rows * G;
+      const int place = alive ? my / G : 0;
+      float* xch = reinterpret_cast<float*>(smem + L::Q) + row;  // [D][128] fp32: both Q tiles
+      if (!pair) named_sync(3, 256);  // both slots are done with their Q tiles
+      if (!pair && slot == 1) {
+        ml1[row] = make_float2(m, l);
         if (steps > 0 && warp_alive) {
 #pragma unroll
           for (int i = 0; i < D / 32; ++i) {
@@ -552,17 +668,17 @@ __global__ void __launch_bounds__(NTHR, 1)
             ld_x32(t_o + uint32_t(32 * i), o);
             tcg::tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) xch[(32 * i + e) * 128 + row] = o[e];
+            for (int e = 0; e < 32; ++e) xch[(32 * i + e) * ROWS] = o[e];
           }
         }
-        named_sync(1, 256);
+        named_sync(3, 256);
       } else {
         float f0 = 1.f, f1 = 0.f;
         bool both = false;
-        if (!s.pair) {
-          named_sync(1, 256);
+        if (!pair) {
+          named_sync(3, 256);
           if (n > 1) {
-            const float2 st = stat[row];
+            const float2 st = ml1[row];
             const float mn = fmaxf(m, st.x), ref = mn == -INFINITY ? 0.f : mn;
             f0 = ex2((m - ref) * c_log2);
             f1 = ex2((st.x - ref) * c_log2);
@@ -575,8 +691,8 @@ __global__ void __launch_bounds__(NTHR, 1)
         if (warp_alive) {
           const int hq = s.h * G + my - place * G;
           const float inv = l == 0.f ? 0.f : 1.f / l;
-          float* pp = whole ? nullptr : part<D>(static_cast<float*>(a.workspace), cta, s.t0 == 0 ? 1 : 0);
-          const int prow = (s.pair ? slot * ROWS : 0) + row;
+          float* pp = whole ? nullptr : part<D>(a.workspace, cta, s.t0 == 0 ? 1 : 0);
+          const int prow = (pair ? slot * ROWS : 0) + row;
           T* out = static_cast<T*>(a.out) + int64_t(s.r0 + place) * a.o_strides[0] + hq * a.o_strides[1];
           if (!whole && alive)
             reinterpret_cast<float2*>(pp + 2 * ROWS * D)[prow] = make_float2(m * c_log2, l);
@@ -587,7 +703,7 @@ __global__ void __launch_bounds__(NTHR, 1)
             tcg::tmem_wait_ld();
             if (both) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = o[e] * f0 + xch[(32 * i + e) * 128 + row] * f1;
+              for (int e = 0; e < 32; ++e) o[e] = o[e] * f0 + xch[(32 * i + e) * ROWS] * f1;
             }
             if (alive) {
               if (whole) {
@@ -624,13 +740,23 @@ __global__ void __launch_bounds__(NTHR, 1)
           }
         }
       }
-      if (!s.pair) {
-        named_sync(1, 256);  // the exchange has been read: the next segment's Q may land there
+      // the exchange and the segment have been read: the next ones may land there
+      if (pair) named_sync(1 + slot, 128); else named_sync(3, 256);
+      if (row == 0) {
+        if (slot == 0 && s.t0 == 0 && s.t1 < s.T) {  // this CTA's end cuts the item
+          const int64_t stop = sh.w.u - s.t1 + s.T;
+          int x = cta + 1;
+          while (x < n_cta && range_begin(pl.total, x, n_cta) < stop) ++x;
+          static_cast<Cut*>(a.workspace)[cta] = Cut{x - cta, s.r0, s.live, s.row_base, s.h, {0, 0, 0}};
+        }
+        sh.more = sh.w.next(a, sh.s);
       }
       tcg::tc_fence_before();
+      named_sync(1 + slot, 128);
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    Segment s;
     if (warp == WARP_TMA) {
       // -------------------------------------------------------------- producer
       if (lane == 0) {
@@ -664,99 +790,125 @@ __global__ void __launch_bounds__(NTHR, 1)
       __syncwarp();
     } else if (warp == WARP_MMA) {
       // -------------------------------------------------------------- products
-      if (tcg::elect_one()) {
-        int g = 0;
-        uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0};
-        bool issued = false;
-        auto take = [&]() {  // the next ring buffer, filled
-          const int x = g % NB;
-          if (ok) ok = mbar_wait(&full[x], uint32_t(g / NB) & 1u, status, kErrWaitKV);
-          tcg::tc_fence_after();
-          ++g;
-          return x;
-        };
-        auto scores = [&](int slot, int x) {
-          if (!ok) return;
-          const uint64_t qd = desc_sw128(smem_u32(smem + L::Q + slot * L::TILE), 16);
-          const uint64_t kd = desc_sw128(smem_u32(ring + x * L::TILE), 16);
+      // The whole warp walks and waits; one lane issues. What an instruction needs is then the same in
+      // every lane and can sit in uniform registers.
+      const uint32_t leader = tcg::elect_one() ? 1u : 0u;
+      const uint32_t q_lo = desc_lo(smem_u32(smem + L::Q), 16), ring_a = smem_u32(ring);
+      int x_ring = 0, g_phase = 0;
+      uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0};
+      bool issued = false;
+      auto take = [&]() {  // the next ring buffer, filled
+        const int x = x_ring;
+        if (ok) ok = mbar_wait(&full[x], uint32_t(g_phase), status, kErrWaitKV);
+        tcg::tc_fence_after();
+        if (++x_ring == NB) {
+          x_ring = 0;
+          g_phase ^= 1;
+        }
+        return x;
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (leader) tcg::umma_commit(bar);
+      };
+      auto scores = [&](int slot, int x) {
+        if (!ok) return;
+        const uint32_t qd = q_lo + uint32_t(slot) * (L::TILE >> 4);
+        const uint32_t kd = desc_lo(ring_a + uint32_t(x) * L::TILE, 16);
+        if (leader) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
-            const uint64_t off = uint64_t((k >> 2) * (L::HALF >> 4) + (k & 3) * 2);
-            umma_ss(tmem + uint32_t(slot * 128), qd + off, kd + off, ID_QK, k ? 1u : 0u);
+            const uint32_t off = uint32_t((k >> 2) * (L::HALF >> 4) + (k & 3) * 2);
+            umma_ss(tmem + uint32_t(slot * 128), desc_sw128(qd + off), desc_sw128(kd + off), ID_QK,
+                    k ? 1u : 0u);
           }
           tcg::umma_commit(&s_full[slot]);
-          issued = true;
-        };
-        auto values = [&](int slot, int x, bool first) {
-          if (ok) ok = mbar_wait(&p_full[slot], n_p[slot]++ & 1u, status, kErrWaitMma);
-          if (!ok) return;
-          tcg::tc_fence_after();
-          const uint64_t vd = desc_sw128(smem_u32(ring + x * L::TILE), L::HALF);
+        }
+        issued = true;
+      };
+      auto values = [&](int slot, int x, bool first) {
+        const uint32_t vd = desc_lo(ring_a + uint32_t(x) * L::TILE, L::HALF);
+        const uint32_t ph = n_p[slot]++ & 1u;
+        const uint32_t d = tmem + O_COL + uint32_t(slot * 128), p = tmem + uint32_t(slot * 128);
+        if (ok) ok = mbar_wait(&p_part[slot], ph, status, kErrWaitMma);
+        if (!ok) return;
+        tcg::tc_fence_after();
+        if (leader) {
 #pragma unroll
-          for (int k = 0; k < BN / 16; ++k)
-            tcg::umma_ts(tmem + O_COL + uint32_t(slot * 128), tmem + uint32_t(slot * 128 + 8 * k),
-                         vd + uint64_t(k * (2048 >> 4)), ID_PV, first && k == 0 ? 0u : 1u);
-          issued = true;
-        };
-        auto release = [&](int x) {
-          if (ok) tcg::umma_commit(&empty[x]);
-        };
-        auto q_ready = [&](int slot) {
-          if (ok) ok = mbar_wait(&q_full[slot], n_q[slot]++ & 1u, status, kErrWaitMma);
-          tcg::tc_fence_after();
-        };
-        while (ok && wk.next(a, s)) {
-          const int n = s.t1 - s.t0;
-          if (s.pair) {
-            int x = take();
-            q_ready(0);
-            scores(0, x);
-            q_ready(1);
-            scores(1, x);
-            release(x);
-            for (int t = 0; t < n && ok; ++t) {
-              const int v = take();
-              const bool more = t + 1 < n;
-              values(0, v, t == 0);
-              if (!more && ok) tcg::umma_commit(&o_full[0]);
-              if (more) {
-                x = take();
-                scores(0, x);
-              }
-              values(1, v, t == 0);
-              release(v);
-              if (more) {
-                scores(1, x);
-                release(x);
-              } else if (ok) {
-                tcg::umma_commit(&o_full[1]);
-              }
+          for (int k = 0; k < 6; ++k)
+            tcg::umma_ts(d, p + uint32_t(8 * k), desc_sw128(vd + uint32_t(k * (2048 >> 4))), ID_PV,
+                    first && k == 0 ? 0u : 1u);
+        }
+        ok = mbar_wait(&p_full[slot], ph, status, kErrWaitMma);
+        if (!ok) return;
+        tcg::tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int k = 6; k < BN / 16; ++k)
+            tcg::umma_ts(d, p + uint32_t(8 * k), desc_sw128(vd + uint32_t(k * (2048 >> 4))), ID_PV, 1u);
+        }
+      };
+      auto release = [&](int x) {
+        if (ok) commit(&empty[x]);
+      };
+      auto q_ready = [&](int slot) {
+        if (ok) ok = mbar_wait(&q_full[slot], n_q[slot]++ & 1u, status, kErrWaitMma);
+        tcg::tc_fence_after();
+      };
+      while (__all_sync(0xffffffffu, ok) && wk.next(a, s)) {
+        const int n = __shfl_sync(0xffffffffu, s.t1 - s.t0, 0);
+        const bool pair = __shfl_sync(0xffffffffu, int(s.pair), 0);
+        if (pair) {
+          int x = take();
+          q_ready(0);
+          scores(0, x);
+          q_ready(1);
+          scores(1, x);
+          release(x);
+          for (int t = 0; t < n; ++t) {
+            const int v = take();
+            const bool more = t + 1 < n;
+            values(0, v, t == 0);
+            if (more) {
+              x = take();
+              scores(0, x);
+            } else if (ok) {
+              commit(&o_full[0]);
             }
-          } else {
-            for (int z = 0; z < min(n, 2); ++z) {
+            values(1, v, t == 0);
+            release(v);
+            if (more) {
+              scores(1, x);
+              release(x);
+            } else if (ok) {
+              commit(&o_full[1]);
+            }
+            if (!__all_sync(0xffffffffu, ok)) break;
+          }
+        } else {
+          for (int z = 0; z < min(n, 2); ++z) {
+            const int x = take();
+            q_ready(z);
+            scores(z, x);
+            release(x);
+          }
+          for (int t = 0; t < n; ++t) {
+            const int v = take(), z = t & 1;
+            values(z, v, t < 2);
+            release(v);
+            if (t + 2 < n) {
               const int x = take();
-              q_ready(z);
               scores(z, x);
               release(x);
+            } else if (ok) {
+              commit(&o_full[z]);
             }
-            for (int t = 0; t < n && ok; ++t) {
-              const int v = take(), z = t & 1;
-              values(z, v, t < 2);
-              release(v);
-              if (t + 2 < n) {
-                const int x = take();
-                scores(z, x);
-                release(x);
-              } else if (ok) {
-                tcg::umma_commit(&o_full[z]);
-              }
-            }
+            if (!__all_sync(0xffffffffu, ok)) break;
           }
         }
-        if (issued) {  // nothing may write tensor memory after the CTA releases it
-          tcg::umma_commit(fin);
-          mbar_wait(fin, 0, status, kErrWaitMma);
-        }
+      }
+      if (issued) {  // nothing may write tensor memory after the CTA releases it
+        commit(fin);
+        mbar_wait(fin, 0, status, kErrWaitMma);
       }
       __syncwarp();
     }
@@ -767,53 +919,84 @@ __global__ void __launch_bounds__(NTHR, 1)
   if (warp == WARP_MMA) tcg::tmem_dealloc(tmem, 512);
 }
 
-// Joins the parts of the item that the boundary between CTAs c and c + 1 cuts (once: at the item's
-// first boundary). Block (c, y): rows 32 y .. 32 y + 31 of the item, a warp a row.
+// Joins the parts of the cut items. Block (k, y): rows 8 y .. 8 y + 7 of the k-th cut item, a warp a
+// row; the row's parts are read by all lanes at
+// once (their maxima and sums one part a lane) and added in order.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) merge_kernel(const dspark_tree_attn_args a, const int n_cta) {
+__global__ void __launch_bounds__(MAX_CTA) merge_kernel(const dspark_tree_attn_args a, const int n_cta) {
+  __shared__ int before[MAX_CTA / 32], found;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) found = -1;
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ int64_t scan[36];
-  const int c = blockIdx.x;
-  const Place pl = locate(a, scan, [&](int64_t total) { return range_begin(total, c + 1, n_cta); });
-  const int64_t u = range_begin(pl.total, c + 1, n_cta);
-  if (u >= pl.total || u == range_begin(pl.total, c, n_cta)) return;
-  int M, T_;
-  extents(a, pl.b, M, T_);
-  const int64_t im = (u - pl.base) / T_, u0 = pl.base + im * T_;
-  if (u == u0 || range_begin(pl.total, c, n_cta) > u0) return;  // cut elsewhere, or before
-  const int h = int(im / M), row_base = int(im - int64_t(h) * M) * 2 * ROWS, G = a.Hq / a.Hk;
-  int r0;
-  const int rows = rows_of(a, pl.b, r0);
-  const int live = min(rows * G - row_base, 2 * ROWS);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* ws = static_cast<float*>(a.workspace);
+  const int tid = threadIdx.x;
+  const bool is_cut = tid < n_cta && __ldcg(&static_cast<const Cut*>(a.workspace)[tid].parts) != 0;
+  const unsigned cuts = __ballot_sync(0xffffffffu, is_cut);
+  if (lane == 0) before[warp] = __popc(cuts);
+  __syncthreads();
+  int rank = __popc(cuts & ((1u << lane) - 1u));
+  for (int w = 0; w < warp; ++w) rank += before[w];
+  if (is_cut && rank == int(blockIdx.x)) found = tid;
+  __syncthreads();
+  const int c = found;
+  if (c < 0) return;
+  const int4* cp = reinterpret_cast<const int4*>(static_cast<const Cut*>(a.workspace) + c);
+  const int4 c0 = __ldcg(cp), c1 = __ldcg(cp + 1);
+  const int parts = c0.x, r0 = c0.y, live = c0.z, row_base = c0.w, h = c1.x;
+  const int i = blockIdx.y * 8 + warp;
+  if (i >= live) return;
   constexpr int VPL = D / 32;
-  for (int i = blockIdx.y * 32 + warp; i < min(live, int(blockIdx.y) * 32 + 32); i += 8) {
-    float m = -INFINITY, l = 0.f, o[VPL];
+  constexpr int64_t STRIDE = int64_t(2) * (2 * ROWS) * (D + 2);  // floats between the CTAs' parts
+  const float* first = part<D>(a.workspace, c, 1);
+  const float* rest = part<D>(a.workspace, c + 1, 0);
+  auto at = [&](int x) { return x == 0 ? first : rest + (x - 1) * STRIDE; };
+  float m = -INFINITY;
+  for (int x = lane; x < parts; x += 32) {
+    const float v = __ldcg(at(x) + 2 * ROWS * D + 2 * i);
+    m = v == v ? fmaxf(m, v) : v;
+  }
 #pragma unroll
-    for (int e = 0; e < VPL; ++e) o[e] = 0.f;
-    for (int x = c; x < n_cta; ++x) {
-      if (x > c && range_begin(pl.total, x, n_cta) >= u0 + T_) break;
-      if (x > c && range_begin(pl.total, x, n_cta) == range_begin(pl.total, x + 1, n_cta)) continue;
-      const float* p = part<D>(ws, x, x == c ? 1 : 0);
-      const float2 st = __ldcg(reinterpret_cast<const float2*>(p + 2 * ROWS * D) + i);
-      const float mn = fmaxf(m, st.x), ref = mn == -INFINITY ? 0.f : mn;
-      const float f0 = ex2(m - ref), f1 = ex2(st.x - ref);
-      m = mn;
-      l = l * f0 + st.y * f1;
+  for (int o = 16; o > 0; o >>= 1) {
+    const float v = __shfl_xor_sync(0xffffffffu, m, o);
+    m = m == m && v == v ? fmaxf(m, v) : NAN;
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[VPL];
 #pragma unroll
-      for (int e = 0; e < VPL; ++e) o[e] = o[e] * f0 + __ldcg(p + int64_t(i) * D + lane + 32 * e) * f1;
+  for (int e = 0; e < VPL; ++e) o[e] = 0.f;
+  for (int x0 = 0; x0 < parts; x0 += 32) {
+    float w = 0.f, lx = 0.f;
+    if (x0 + lane < parts) {
+      const float2 st = __ldcg(reinterpret_cast<const float2*>(at(x0 + lane) + 2 * ROWS * D) + i);
+      w = ex2(st.x - ref);
+      lx = st.y * w;
     }
-    const int x = row_base + i, node = x / G, hq = h * G + x - node * G;
-    T* out = static_cast<T*>(a.out) + int64_t(r0 + node) * a.o_strides[0] + hq * a.o_strides[1];
-    const float inv = 1.f / l;
 #pragma unroll
-    for (int e = 0; e < VPL; ++e) out[lane + 32 * e] = Elem<T>::from_f(l == 0.f ? 0.f : o[e] * inv);
+    for (int s = 16; s > 0; s >>= 1) lx += __shfl_xor_sync(0xffffffffu, lx, s);
+    l += lx;
+    const int nx = min(32, parts - x0);
+#pragma unroll 8
+    for (int x = 0; x < nx; ++x) {
+      const float f = __shfl_sync(0xffffffffu, w, x);
+      const float* p = at(x0 + x) + int64_t(i) * D + lane * VPL;
+      float v[VPL];
+      if (VPL == 4) *reinterpret_cast<float4*>(v) = __ldcg(reinterpret_cast<const float4*>(p));
+      else *reinterpret_cast<float2*>(v) = __ldcg(reinterpret_cast<const float2*>(p));
+#pragma unroll
+      for (int e = 0; e < VPL; ++e) o[e] += v[e] * f;
+    }
+  }
+  const int G = a.Hq / a.Hk, x = row_base + i, node = x / G, hq = h * G + x - node * G;
+  T* out = static_cast<T*>(a.out) + int64_t(r0 + node) * a.o_strides[0] + hq * a.o_strides[1] + lane * VPL;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int e = 0; e < VPL; e += 2) {
+    if (l == 0.f) o[e] = o[e + 1] = 0.f;
+    *reinterpret_cast<uint32_t*>(out + e) = Elem<T>::pack(o[e] * inv, o[e + 1] * inv);
   }
 }
 
-static int grid_of(int device) { return sm_count(device); }
+static int grid_of(int device) { return std::min(sm_count(device), MAX_CTA); }
 
 template <typename T, int D>
 static int launch(const dspark_tree_attn_args& a, cudaStream_t s) {
@@ -851,8 +1034,10 @@ static int launch(const dspark_tree_attn_args& a, cudaStream_t s) {
   DSPARK_CUDA_TRY(launch_ex(attn_kernel<T, D>, dim3(n_cta), dim3(NTHR), smem, s, 1, true, maps[0], maps[1],
                             a, sign == 0.f ? 1.f : c, sign, st),
                   "tree_attn");
-  const int rows = std::min(2 * ROWS, a.max_rows * (a.Hq / a.Hk));
-  DSPARK_CUDA_TRY(launch_ex(merge_kernel<T, D>, dim3(n_cta, (rows + 31) / 32), dim3(256), 0, s, 1, true, a,
+  const int rows = int(std::min<int64_t>(2 * ROWS, int64_t(std::min(a.max_rows, a.R)) * (a.Hq / a.Hk)));
+  const int64_t items = int64_t(a.B) * a.Hk * ((int64_t(std::min(a.max_rows, a.R)) * (a.Hq / a.Hk) + 2 * ROWS - 1) / (2 * ROWS));
+  const int cuts = int(std::min<int64_t>(n_cta, items));  // at most one a CTA and one an item
+  DSPARK_CUDA_TRY(launch_ex(merge_kernel<T, D>, dim3(cuts, (rows + 7) / 8), dim3(MAX_CTA), 0, s, 1, true, a,
                             n_cta),
                   "tree_attn merge");
   return DSPARK_OK;
@@ -867,7 +1052,8 @@ extern "C" {
 
 size_t dspark_tree_attn_workspace(int B, int Hq, int Hk, int D, int max_rows) {
   if (B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || D <= 0 || max_rows <= 0) return 0;
-  return size_t(tattn::grid_of(current_device())) * 2 * (2 * tattn::ROWS) * (D + 2) * sizeof(float);
+  return tattn::MAX_CTA * sizeof(tattn::Cut) +
+         size_t(tattn::grid_of(current_device())) * 2 * (2 * tattn::ROWS) * (D + 2) * sizeof(float);
 }
 
 int dspark_tree_attn(const dspark_tree_attn_args* p, void* stream) {
