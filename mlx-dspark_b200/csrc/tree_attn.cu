@@ -6,12 +6,13 @@
 // the rows of one product are (node, head of the group): node * G + g.
 //
 // Units and segments. A unit is 128 keys of one item: an item is up to 256 rows of one (request, kv
-// head). All units of the call are numbered (request, head, rows, keys) and cut into equal contiguous
+// head). All units of the call are numbered (request, head, rows, keys) and cut into contiguous
 // ranges, one a CTA (one CTA per SM), from the lengths on the device: requests of any mix of lengths
-// load the SMs evenly without the host knowing them. A CTA walks its range as segments (a run of
-// keys of one item). A segment that covers its item writes the output; else it leaves an
-// unnormalised fp32 part (m, sum, O) in the workspace, at most two a CTA, and the merge kernel joins
-// the parts of an item in order (no atomics: results do not depend on timing).
+// load the SMs evenly without the host knowing them (locate). A CTA walks its range as segments (a run
+// of keys of one item). A segment that covers its item writes the output; else it leaves an
+// fp32 part (O and the logarithm of its sum) in the workspace, at most two a CTA; when all parts of an item
+// are there, each of its CTAs joins a share of the rows, the parts in order (so results do not depend
+// on timing). They wait for one another, so the launch is cooperative: all CTAs run at once.
 //
 // CTA: two slots of 128 rows (TMEM lanes), each with a softmax warpgroup, a score tile S (TMEM,
 // overwritten by the 16-bit weights P) and an output accumulator O (TMEM).
@@ -29,6 +30,8 @@
 // past the request's keys are zeroed in shared memory, and a non-finite V among the tree's own keys
 // is taken out of the tile and added only to the rows that see it (fix_values / add_hidden).
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 
 #include "elem.cuh"
 #include "host_common.h"
@@ -49,10 +52,11 @@ struct Lay {
   static constexpr int NB = D == 128 ? 5 : 10;    // ring buffers
   static constexpr int Q = 0;
   static constexpr int RING = 2 * TILE;
-  static constexpr int M1 = RING + NB * TILE;     // slot 1's (m, l) at the segment's end; a scan
+  static constexpr int M1 = RING + NB * TILE;     // slot 1's (m, l) at the segment's end
   static constexpr int FLAG = M1 + ROWS * 8;
   static constexpr int SEG = FLAG + 16;             // [slot] the softmax threads' segment and walker
-  static constexpr int BARS = SEG + 2 * 96;
+  static constexpr int CUTS = SEG + 2 * 96;         // the CTA's parts of cut items
+  static constexpr int BARS = CUTS + 2 * 32 + 16;
   static constexpr int NBAR = 2 * NB + 2 + 2 + 2 + 2 + 2 + 1;
   static constexpr int TOTAL = BARS + NBAR * 8;
   static_assert(TOTAL <= 232448, "shared memory of one SM");
@@ -61,6 +65,12 @@ struct Lay {
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -163,79 +173,105 @@ __device__ __forceinline__ void extents(const dspark_tree_attn_args& a, int b, i
   T = max(1, (min(a.kv_len[b], a.cap - start_of(a, b)) + BN - 1) / BN);
 }
 
-__device__ __forceinline__ int64_t units_of(const dspark_tree_attn_args& a, int b) {
-  int M, T;
-  extents(a, b, M, T);
-  return int64_t(M) * T * a.Hk;
-}
-
-struct Place {
-  int64_t total;  // units of the call
-  int64_t base;   // first unit of request b
-  int b;          // request that holds the unit looked up
+// A CTA's range of units. Either all units are dealt out equally (the first total % n CTAs have one
+// more) and a range may cross from item to item, or each item has CTAs of its own.
+struct Range {
+  int u, end;        // units [u, end)
+  int b, base;       // request of unit u, the request's first unit
+  int first, parts;  // an item's own CTAs: the first one, how many; parts 0: dealt out equally
+  int total, n;      // units of the call, CTAs that have any
+  __device__ __forceinline__ int dealt(int c) const {
+    const int q = n ? total / n : 0;
+    return c < n ? c * q + min(c, total - q * n) : total;
+  }
 };
 
-// All threads of the block: the total number of units and, for the unit `of(total)`, its request.
-// `scan` holds 32 + 4 values.
-template <typename F>
-__device__ Place locate(const dspark_tree_attn_args& a, int64_t* scan, F&& of) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
-  auto block_scan = [&](int64_t v, int64_t& sum) {  // inclusive scan over the block
-    int64_t x = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) scan[warp] = x;
-    __syncthreads();
-    int64_t before = 0;
-    sum = 0;
-    for (int w = 0; w < nw; ++w) {
-      if (w < warp) before += scan[w];
-      sum += scan[w];
-    }
-    return before + x;
-  };
-  const int64_t mine = tid < a.B ? units_of(a, tid) : 0;
-  int64_t sum, total;
-  const int64_t incl = block_scan(mine, sum);
-  total = sum;
-  for (int b0 = blockDim.x; b0 < a.B; b0 += blockDim.x) {
-    block_scan(b0 + tid < a.B ? units_of(a, b0 + tid) : 0, sum);
-    total += sum;
-  }
-  const int64_t u = of(total);
-  int64_t* found = scan + 32;  // base, request
-  if (tid == 0) found[1] = a.B;
-  __syncthreads();
-  if (u < total) {
-    if (mine > 0 && u < incl && u >= incl - mine) {
-      found[0] = incl - mine;
-      found[1] = tid;
-    }
-    __syncthreads();
-    int64_t at = 0;
-    if (a.B > int(blockDim.x)) {
-      block_scan(mine, at);
-      for (int b0 = blockDim.x; b0 < a.B; b0 += blockDim.x) {
-        const int64_t v = b0 + tid < a.B ? units_of(a, b0 + tid) : 0;
-        const int64_t x = at + block_scan(v, sum);
-        if (v > 0 && u < x && u >= x - v) {
-          found[0] = x - v;
-          found[1] = b0 + tid;
-        }
-        at += sum;
-      }
-    }
-  }
-  __syncthreads();
-  return Place{total, found[0], int(found[1])};
+// CTAs of one item among n when items have their own: one each, and the others by the tiles.
+__device__ __forceinline__ int ctas_of(int T, int n, int items, int total) {
+  return min(T, 1 + int(int64_t(T) * (n - items) / total));
 }
 
-__device__ __forceinline__ int64_t range_begin(int64_t total, int c, int n) {
-  return n ? min(total, total * c / n) : 0;
+// Every warp for itself, no barrier. Items get their own CTAs unless the longest range then has OWN
+// tiles more than an equal deal: what a second segment costs (its Q, its parts, the refilled
+// pipeline) is about that many tiles: 61 rows over 16k keys, 8 items: 40 us for the CTAs with two
+// segments of together 7 tiles, 24 us for those with one.
+constexpr int OWN = 8;
+__device__ Range locate(const dspark_tree_attn_args& a, int cta, int n_cta) {
+  const int lane = threadIdx.x & 31;
+  auto scan = [&](int v) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += y;
+    }
+    return v;
+  };
+  int M0 = 0, T0 = 1;  // the lane's own request of the first 32
+  if (lane < a.B) extents(a, lane, M0, T0);
+  auto shape = [&](int b, int& M, int& T) {
+    M = 0;
+    T = 1;
+    if (b < 32) {
+      M = M0;
+      T = T0;
+    } else if (b < a.B) {
+      extents(a, b, M, T);
+    }
+  };
+  int items = 0, total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    int M, T;
+    shape(b0 + lane, M, T);
+    items += M * a.Hk;
+    total += M * T * a.Hk;
+  }
+  items = __reduce_add_sync(0xffffffffu, items);
+  total = __reduce_add_sync(0xffffffffu, total);
+  Range r{0, 0, a.B, 0, 0, 0, total, min(n_cta, total)};
+  if (total == 0) return r;
+  bool own = items <= n_cta;
+  if (own) {
+    int longest = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      int M, T;
+      shape(b0 + lane, M, T);
+      const int c = ctas_of(T, n_cta, items, total);
+      if (M) longest = max(longest, (T + c - 1) / c);
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    own = longest <= (total + n_cta - 1) / n_cta + OWN;
+  }
+  const int want = own ? cta : r.dealt(cta);  // in CTAs or in units
+  if (!own && want >= total) return r;
+  int at = 0, units = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    int M, T;
+    shape(b0 + lane, M, T);
+    const int c = own ? ctas_of(T, n_cta, items, total) : T;
+    const int v = M * a.Hk * c, x = scan(v), n = M * T * a.Hk, y = scan(n);
+    const unsigned hit = __ballot_sync(0xffffffffu, v > 0 && want < at + x && want >= at + x - v);
+    if (hit) {
+      const int k = __ffs(hit) - 1;
+      r.b = b0 + k;
+      r.base = units + __shfl_sync(0xffffffffu, y - n, k);
+      if (own) {
+        const int ck = __shfl_sync(0xffffffffu, c, k), Tk = __shfl_sync(0xffffffffu, T, k);
+        const int local = want - (at + __shfl_sync(0xffffffffu, x - v, k));
+        const int im = local / ck, s = local - im * ck;
+        r.u = r.base + im * Tk + Tk * s / ck;
+        r.end = r.base + im * Tk + Tk * (s + 1) / ck;
+        r.first = cta - s;
+        r.parts = ck;
+      } else {
+        r.u = want;
+        r.end = r.dealt(cta + 1);
+      }
+      return r;
+    }
+    at += __shfl_sync(0xffffffffu, x, 31);
+    units += __shfl_sync(0xffffffffu, y, 31);
+  }
+  return r;
 }
 
 // One run of key tiles of one item.
@@ -249,25 +285,24 @@ struct Segment {
 };
 
 struct Walker {
-  int64_t u, end, base;  // next unit, end of the range, first unit of request b
+  int u, end, base;  // next unit, end of the range, first unit of request b
   int b;
   __device__ __forceinline__ bool next(const dspark_tree_attn_args& a, Segment& s) {
     if (u >= end) return false;
     int M, T;
     extents(a, b, M, T);
-    int64_t n = int64_t(M) * T * a.Hk;
+    int n = M * T * a.Hk;
     while (u >= base + n) {
       base += n;
       extents(a, ++b, M, T);
-      n = int64_t(M) * T * a.Hk;
+      n = M * T * a.Hk;
     }
     const int G = a.Hq / a.Hk;
-    const int64_t local = u - base;
-    const int im = int(local / T);
+    const int local = u - base, im = local / T;
     s.b = b;
     s.T = T;
-    s.t0 = int(local - int64_t(im) * T);
-    s.t1 = int(min(int64_t(T), s.t0 + (end - u)));
+    s.t0 = local - im * T;
+    s.t1 = min(T, s.t0 + (end - u));
     s.h = im / M;
     s.row_base = (im - s.h * M) * 2 * ROWS;
     s.rows = rows_of(a, b, s.r0);
@@ -338,40 +373,48 @@ __device__ __forceinline__ void tile_bits(const dspark_tree_attn_args& a, const 
 
 // A tile whose V rows are not all plain values of visible or cached keys: rows past the request's
 // keys are zeroed; non-finite values among the tree's keys are zeroed and reported (add_hidden
-// gives them to the rows that see them). Thread x of the warpgroup has key x of the tile.
+// gives them to the rows that see them). Thread x of the warpgroup has key x of the tile. A 16-bit
+// value is not finite iff its exponent is all ones: adding one to the exponent field then carries
+// into the sign's place, for both values of a word at once.
 template <typename T, int D>
 __device__ __noinline__ void fix_values(uint8_t* tile, int key, int len, int first, int* flag,
                                         int seg) {
   const int x = threadIdx.x & 127;
   const bool past = key + x >= len;
   if (!past && key + x < first) return;
-  const uint32_t em = Elem<T>::kExpMask;
-  bool bad = false;
-#pragma unroll 4
-  for (int c = 0; c < D / 8; ++c) {
-    uint4* p = reinterpret_cast<uint4*>(tile + (c >> 3) * Lay<D>::HALF + x * 128 + (((c & 7) ^ (x & 7)) << 4));
-    if (past) {
-      *p = make_uint4(0u, 0u, 0u, 0u);
-    } else {
-      uint4 v = *p;
-      uint32_t* w = &v.x;
-      bool hit = false;
+  constexpr uint32_t em = Elem<T>::kExpMask, one = em & (0u - em);
+  constexpr uint32_t MASK = em | (em << 16), ADD = one | (one << 16), TOP = 0x80008000u;
+  auto at = [&](int c) {
+    return reinterpret_cast<uint4*>(tile + (c >> 3) * Lay<D>::HALF + x * 128 + (((c & 7) ^ (x & 7)) << 4));
+  };
+  if (past) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if ((w[e] & em) == em) { w[e] &= 0xffff0000u; hit = true; }
-        if ((w[e] & (em << 16)) == (em << 16)) { w[e] &= 0x0000ffffu; hit = true; }
-      }
-      if (hit) {
-        *p = v;
-        bad = true;
-      }
-    }
+    for (int c = 0; c < D / 8; ++c) *at(c) = make_uint4(0u, 0u, 0u, 0u);
+    return;
   }
-  if (bad) *flag = seg;
+  uint32_t bad = 0;
+#pragma unroll
+  for (int c = 0; c < D / 8; ++c) {
+    const uint4 v = *at(c);
+    bad |= ((v.x & MASK) + ADD) | ((v.y & MASK) + ADD) | ((v.z & MASK) + ADD) | ((v.w & MASK) + ADD);
+  }
+  if (!(bad & TOP)) return;
+  for (int c = 0; c < D / 8; ++c) {
+    uint4 v = *at(c);
+    uint32_t* w = &v.x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t b = ((w[e] & MASK) + ADD) & TOP;
+      if (b & 0x8000u) w[e] &= 0xffff0000u;
+      if (b & 0x80000000u) w[e] &= 0x0000ffffu;
+    }
+    *at(c) = v;
+  }
+  *flag = seg;
 }
 
 // The non-finite values that fix_values took out of the segment's tiles, added to what a row that
-// sees them has stored (`out`: the output, or `part`: the fp32 part).
+// sees them has stored (`out`: the output, or `part`: the fp32 part, 256 values a step).
 template <typename T>
 struct Hidden {
   const T* v;             // the request's first value row of this kv head
@@ -387,7 +430,7 @@ __device__ __noinline__ void add_hidden(const Hidden<T> x, T* out, float* part) 
     for (int d = 0; d < x.D; ++d) {
       const float v = Elem<T>::to_f(x.v[int64_t(k) * x.stride + d]);
       if (isfinite(v)) continue;
-      if (part) part[d] += v;
+      if (part) part[d * 2 * ROWS] += v;
       else out[d] = Elem<T>::from_f(Elem<T>::to_f(out[d]) + v);
     }
   }
@@ -395,18 +438,127 @@ __device__ __noinline__ void add_hidden(const Hidden<T> x, T* out, float* part) 
 
 // ------------------------------------------------------------------ workspace
 
-// What the merge needs to know of an item cut by CTA c's end (its first part is c's second one, the
-// others are the first parts of CTAs c + 1 ..): written by c, parts 0 where there is none.
+// A cut item as one of its CTAs sees it: the CTA of its first part, how many there are (one CTA after
+// the other), and its rows.
 struct Cut {
-  int parts, r0, live, row_base, h, pad[3];
+  int first, parts, r0, live, row_base, h, pad[2];
 };
-constexpr int MAX_CTA = 256;
+constexpr int MAX_CTA = 160;
 
-// The workspace: a Cut a CTA, then part `which` of CTA c: 256 rows of D values, then 256 (m, l).
+// The workspace: a count a CTA (of the item whose first part it has), then part `which` of CTA c: D
+// values (divided by the part's sum) and the logarithm of the sum, m + log2 l, of 256 rows (row
+// innermost, as a warp of 32 rows writes them). An item's first part is its CTA's part 1, the others
+// are part 0.
 template <int D>
 __device__ __forceinline__ float* part(void* ws, int c, int which) {
-  return reinterpret_cast<float*>(static_cast<Cut*>(ws) + MAX_CTA) +
-         int64_t(2 * c + which) * (2 * ROWS) * (D + 2);
+  return reinterpret_cast<float*>(static_cast<uint64_t*>(ws) + MAX_CTA) +
+         int64_t(2 * c + which) * (2 * ROWS) * (D + 1);
+}
+
+// Counts live in memory that nobody clears: a word that does not carry this launch's tag counts as
+// zero (the first to see it so puts the tag there, everybody else adds). Whoever counts last puts a
+// zero back, so that a replayed launch (same tag) starts anew.
+__device__ __forceinline__ void count_up(uint64_t* word, uint64_t tag, int last) {
+  unsigned long long* p = reinterpret_cast<unsigned long long*>(word);
+  const unsigned long long seen = *reinterpret_cast<volatile unsigned long long*>(p);
+  if ((seen & ~0xffffull) != tag) {
+    if (atomicCAS(p, seen, tag | 1ull) == seen) {
+      if (last == 1) *reinterpret_cast<volatile unsigned long long*>(p) = 0;
+      return;
+    }
+  }
+  if (int((atomicAdd(p, 1ull) & 0xffffu) + 1) == last) *reinterpret_cast<volatile unsigned long long*>(p) = 0;
+}
+__device__ __forceinline__ bool wait_count(const uint64_t* word, uint64_t tag, int n, int* status) {
+  const uint64_t t0 = globaltimer_ns(), limit = wait_limit_ns(status);
+  while (true) {
+    uint64_t v;
+    asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(word) : "memory");
+    if ((v & ~0xffffull) == tag && int(v & 0xffffu) >= n) return true;
+    if (globaltimer_ns() - t0 > limit) {
+      report_error(status, kErrWaitPeer);
+      return false;
+    }
+  }
+}
+
+// The 256 softmax threads, after the CTA's last segment: its share of the join of each item that it has
+// a part of. First the weights of all parts' rows into shared memory, whose tiles are no longer needed;
+// then blocks of 32 rows (lanes) x 4 values (a warp), dealt out over the item's CTAs. Twelve parts'
+// values are in flight at a time.
+template <typename T, int D>
+__device__ __noinline__ void join_parts(const dspark_tree_attn_args& a, const Cut* cuts, int n_cuts, int cta,
+                                        uint64_t tag, uint8_t* smem, int* status) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.Hq / a.Hk;
+  uint64_t* count = static_cast<uint64_t*>(a.workspace);
+  if (tid == 0) {
+    __threadfence();
+    for (int k = 0; k < n_cuts; ++k) count_up(&count[cuts[k].first], tag, 2 * cuts[k].parts);
+  }
+  constexpr int64_t STRIDE = int64_t(2) * (2 * ROWS) * (D + 1);  // floats between the CTAs' parts
+  static_assert(MAX_CTA * 2 * ROWS * 4 <= Lay<D>::M1, "the weights' room");
+  float* w = reinterpret_cast<float*>(smem);  // [parts][256]
+  for (int k = 0; k < n_cuts; ++k) {
+    const Cut c = cuts[k];
+    if (tid == 0) wait_count(&count[c.first], tag, c.parts, status);
+    named_sync(3, 256);
+    const float* first = part<D>(a.workspace, c.first, 1);
+    const float* rest = part<D>(a.workspace, c.first, 0);
+    auto at = [&](int x) { return x == 0 ? first : rest + x * STRIDE; };
+    const int live = c.live, rounds = (live + 31) / 32;
+    if (tid < live) {
+      float m = -INFINITY, sum = 0.f;
+      constexpr int HELD = 24;  // parts whose sums stay in registers
+      float v[HELD];
+#pragma unroll
+      for (int x = 0; x < HELD; ++x) v[x] = x < c.parts ? __ldcg(at(x) + 2 * ROWS * D + tid) : -INFINITY;
+#pragma unroll
+      for (int x = 0; x < HELD; ++x) m = max3(m, v[x], v[x]);
+#pragma unroll 8
+      for (int x = HELD; x < c.parts; ++x) {
+        const float y = __ldcg(at(x) + 2 * ROWS * D + tid);
+        w[x * 2 * ROWS + tid] = y;
+        m = max3(m, y, y);
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int x = 0; x < HELD; ++x) {
+        v[x] = ex2(v[x] - ref);
+        sum += v[x];
+      }
+      for (int x = HELD; x < c.parts; ++x) {
+        const float f = ex2(w[x * 2 * ROWS + tid] - ref);
+        w[x * 2 * ROWS + tid] = f;
+        sum += f;
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int x = 0; x < HELD; ++x)
+        if (x < c.parts) w[x * 2 * ROWS + tid] = v[x] * inv;
+      for (int x = HELD; x < c.parts; ++x) w[x * 2 * ROWS + tid] *= inv;
+    }
+    named_sync(3, 256);
+    for (int z = (cta - c.first) + c.parts * warp; z < rounds * (D / 4); z += c.parts * 8) {
+      const int i = (z % rounds) * 32 + lane, d0 = z / rounds * 4;
+      if (i >= live) continue;
+      float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 12
+      for (int x = 0; x < c.parts; ++x) {
+        const float* p = at(x) + d0 * (2 * ROWS) + i;
+        const float f = w[x * 2 * ROWS + i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += __ldcg(p + e * (2 * ROWS)) * f;
+      }
+      const int x = c.row_base + i, node = x / G, hq = c.h * G + x - node * G;
+      T* out = static_cast<T*>(a.out) + int64_t(c.r0 + node) * a.o_strides[0] + hq * a.o_strides[1] + d0;
+      *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack(o[0], o[1]), Elem<T>::pack(o[2], o[3]));
+    }
+    named_sync(3, 256);  // all have read the parts
+    if (tid == 0) {
+      __threadfence();
+      count_up(&count[c.first], tag, 2 * c.parts);
+    }
+  }
 }
 
 // ------------------------------------------------------------------ the kernel
@@ -414,7 +566,8 @@ __device__ __forceinline__ float* part(void* ws, int c, int which) {
 template <typename T, int D>
 __global__ void __launch_bounds__(NTHR, 1)
     attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                const dspark_tree_attn_args a, const float c_log2, const float q_sign, int* status) {
+                const dspark_tree_attn_args a, const float c_log2, const float q_sign,
+                const uint64_t tag, int* status) {
   typedef Lay<D> L;
   constexpr int NB = L::NB;
   constexpr uint32_t FMT = std::is_same<T, bf16>::value ? 1u : 0u;
@@ -436,7 +589,6 @@ __global__ void __launch_bounds__(NTHR, 1)
   float2* ml1 = reinterpret_cast<float2*>(smem + L::M1);
   int* flag = reinterpret_cast<int*>(smem + L::FLAG);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(flag + 2);
-  int64_t* scan = reinterpret_cast<int64_t*>(smem + L::M1);  // before the first segment's end
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (smem_u32(smem) & 1023u) {  // the swizzled tiles need it; never seen without static arrays
@@ -465,20 +617,12 @@ __global__ void __launch_bounds__(NTHR, 1)
   pdl_launch_dependents();
   pdl_wait();
   const int cta = blockIdx.x;
-  // with fewer units than CTAs, the first `total` CTAs take one each
-  const Place pl = locate(a, scan, [&](int64_t total) {
-    return range_begin(total, cta, int(min(int64_t(gridDim.x), total)));
-  });
-  const int n_cta = int(min(int64_t(gridDim.x), pl.total));
+  const Range range = locate(a, cta, gridDim.x);
   tcg::tc_fence_before();
   __syncthreads();
   tcg::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Walker wk{0, 0, pl.base, pl.b};
-  if (cta < n_cta) {
-    wk.u = range_begin(pl.total, cta, n_cta);
-    wk.end = range_begin(pl.total, cta + 1, n_cta);
-  }
+  Walker wk{range.u, range.end, range.base, range.b};
   bool ok = true;
 
   if (warp < WARP_TMA) {
@@ -495,7 +639,9 @@ __global__ void __launch_bounds__(NTHR, 1)
       sh.w = wk;
     }
     named_sync(1 + slot, 128);
-    if (tid == 0) static_cast<Cut*>(a.workspace)[cta] = Cut{};
+    Cut* cuts = reinterpret_cast<Cut*>(smem + L::CUTS);
+    int* n_cuts = reinterpret_cast<int*>(cuts + 2);
+    if (tid == 0) *n_cuts = 0;
     uint32_t n_s = 0, n_o = 0;  // completed phases of s_full / o_full
     int use0 = 0;               // ring uses before this segment
     auto arrive = [&](uint64_t* bar) {  // this warp's stores to tensor memory are done
@@ -524,16 +670,23 @@ __global__ void __launch_bounds__(NTHR, 1)
         constexpr int STEP = ROWS / CH;      // rows the warpgroup loads at a time
         const int c = row % CH, first_row = row / CH;
         const int G = a.Hq / a.Hk, row0 = s.row_base + (pair ? slot * ROWS : 0);
+        const int live = min(ROWS, s.rows * G - row0);  // rows past it are never looked at
         uint8_t* qs = smem + L::Q + slot * L::TILE;
-        const T* q = static_cast<const T*>(a.q);
+        const T* q = static_cast<const T*>(a.q) + int64_t(s.r0) * a.q_strides[0] +
+                     s.h * G * a.q_strides[1] + c * 8;
+        const int dn = STEP / G, dg = STEP - dn * G;  // a step in (node, head of the group)
+        int node = (row0 + first_row) / G, g = row0 + first_row - node * G;
         uint4 v[CH];
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-          const int x = row0 + first_row + i * STEP;
           v[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (x < s.rows * G) {
-            const int node = x / G, hq = s.h * G + x - node * G;
-            v[i] = ldcg_v4(q + int64_t(s.r0 + node) * a.q_strides[0] + hq * a.q_strides[1] + c * 8);
+          if (first_row + i * STEP < live)
+            v[i] = ldcg_v4(q + node * a.q_strides[0] + g * a.q_strides[1]);
+          node += dn;
+          g += dg;
+          if (g >= G) {
+            g -= G;
+            ++node;
           }
         }
 #pragma unroll
@@ -547,7 +700,8 @@ __global__ void __launch_bounds__(NTHR, 1)
               w[e] = Elem<T>::pack(f.x * q_sign, f.y * q_sign);
             }
           }
-          *reinterpret_cast<uint4*>(qs + (c >> 3) * L::HALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
+          if (rr < live)
+            *reinterpret_cast<uint4*>(qs + (c >> 3) * L::HALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -556,6 +710,17 @@ __global__ void __launch_bounds__(NTHR, 1)
       for (int j = 0; j < steps; ++j) {
         const int k0 = (tile0 + j * tstep) * BN;
         const bool edge = k0 > edge0;
+        uint32_t bits[4];
+        if (edge) {  // while the scores are under way: who sees what, and V put right
+          const int place = place_of(a, s, slot, row);
+          tile_bits(a, s, s.r0 + place, place, k0, bits);
+          if (slot == 0 || !pair) {
+            const int g = use0 + v_use(pair, k0 / BN - s.t0, n);
+            if (ok) ok = mbar_wait(&full[g % NB], uint32_t(g / NB) & 1u, status, kErrWaitKV);
+            fix_values<T, D>(ring + (g % NB) * L::TILE, k0, s.len, s.first, flag + (seg & 1), seg);
+            fence_proxy_async_smem();
+          }
+        }
         if (ok) ok = mbar_wait(&s_full[slot], n_s & 1, status, kErrWaitMma);
         ++n_s;
         tcg::tc_fence_after();
@@ -565,11 +730,8 @@ __global__ void __launch_bounds__(NTHR, 1)
           for (int i = 0; i < 4; ++i) ld_x32(t_s + uint32_t(32 * i), x + 32 * i);
           tcg::tmem_wait_ld();
           if (edge) {
-            uint32_t w[4];
-            const int place = place_of(a, s, slot, row);
-            tile_bits(a, s, s.r0 + place, place, k0, w);
 #pragma unroll
-            for (int i = 0; i < 128; ++i) x[i] = (w[i >> 5] >> (i & 31)) & 1u ? x[i] : -INFINITY;
+            for (int i = 0; i < 128; ++i) x[i] = (bits[i >> 5] >> (i & 31)) & 1u ? x[i] : -INFINITY;
           }
           float mx[8];
 #pragma unroll
@@ -625,23 +787,14 @@ __global__ void __launch_bounds__(NTHR, 1)
               sum[z & 3] = add2(sum[z & 3], e[z]);
               p[z] = Elem<T>::pack(e0, e1);
               if ((z & 15) == 15) st_x16(t_s + uint32_t(z - 15), p + z - 15);
-              if (z == 47 && !edge) arrive(&p_part[slot]);  // three quarters' products may start
+              if (z == 47) arrive(&p_part[slot]);  // three quarters' products may start
             }
           }
           float s0, s1;
           unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
           l += s0 + s1;
-        } else if (!edge) {
+        } else {
           arrive(&p_part[slot]);
-        }
-        if (edge) {
-          if (slot == 0 || !pair) {
-            const int g = use0 + v_use(pair, k0 / BN - s.t0, n);
-            if (ok) ok = mbar_wait(&full[g % NB], uint32_t(g / NB) & 1u, status, kErrWaitKV);
-            fix_values<T, D>(ring + (g % NB) * L::TILE, k0, s.len, s.first, flag + (seg & 1), seg);
-            fence_proxy_async_smem();
-          }
-          arrive(&p_part[slot]);  // not before: V had to be looked at
         }
         arrive(&p_full[slot]);
       }
@@ -694,8 +847,7 @@ __global__ void __launch_bounds__(NTHR, 1)
           float* pp = whole ? nullptr : part<D>(a.workspace, cta, s.t0 == 0 ? 1 : 0);
           const int prow = (pair ? slot * ROWS : 0) + row;
           T* out = static_cast<T*>(a.out) + int64_t(s.r0 + place) * a.o_strides[0] + hq * a.o_strides[1];
-          if (!whole && alive)
-            reinterpret_cast<float2*>(pp + 2 * ROWS * D)[prow] = make_float2(m * c_log2, l);
+          if (!whole) pp[2 * ROWS * D + prow] = m * c_log2 + lg2(l);
 #pragma unroll
           for (int i = 0; i < D / 32; ++i) {
             float o[32];
@@ -705,22 +857,18 @@ __global__ void __launch_bounds__(NTHR, 1)
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] = o[e] * f0 + xch[(32 * i + e) * ROWS] * f1;
             }
-            if (alive) {
-              if (whole) {
+            if (!whole) {
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                  uint4 v;
-                  v.x = Elem<T>::pack(o[e] * inv, o[e + 1] * inv);
-                  v.y = Elem<T>::pack(o[e + 2] * inv, o[e + 3] * inv);
-                  v.z = Elem<T>::pack(o[e + 4] * inv, o[e + 5] * inv);
-                  v.w = Elem<T>::pack(o[e + 6] * inv, o[e + 7] * inv);
-                  *reinterpret_cast<uint4*>(out + 32 * i + e) = l == 0.f ? make_uint4(0u, 0u, 0u, 0u) : v;
-                }
-              } else {
+              for (int e = 0; e < 32; ++e) pp[(32 * i + e) * (2 * ROWS) + prow] = l == 0.f ? 0.f : o[e] * inv;
+            } else if (alive) {
 #pragma unroll
-                for (int e = 0; e < 32; e += 4)
-                  *reinterpret_cast<float4*>(pp + int64_t(prow) * D + 32 * i + e) =
-                      make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+              for (int e = 0; e < 32; e += 8) {
+                uint4 v;
+                v.x = Elem<T>::pack(o[e] * inv, o[e + 1] * inv);
+                v.y = Elem<T>::pack(o[e + 2] * inv, o[e + 3] * inv);
+                v.z = Elem<T>::pack(o[e + 4] * inv, o[e + 5] * inv);
+                v.w = Elem<T>::pack(o[e + 6] * inv, o[e + 7] * inv);
+                *reinterpret_cast<uint4*>(out + 32 * i + e) = l == 0.f ? make_uint4(0u, 0u, 0u, 0u) : v;
               }
             }
           }
@@ -736,24 +884,31 @@ __global__ void __launch_bounds__(NTHR, 1)
             hd.k1 = min(s.t1 * BN, s.len);
             hd.first = s.first;
             hd.D = D;
-            add_hidden<T>(hd, out, whole ? nullptr : pp + int64_t(prow) * D);
+            add_hidden<T>(hd, out, whole ? nullptr : pp + prow);
           }
         }
       }
       // the exchange and the segment have been read: the next ones may land there
       if (pair) named_sync(1 + slot, 128); else named_sync(3, 256);
       if (row == 0) {
-        if (slot == 0 && s.t0 == 0 && s.t1 < s.T) {  // this CTA's end cuts the item
-          const int64_t stop = sh.w.u - s.t1 + s.T;
-          int x = cta + 1;
-          while (x < n_cta && range_begin(pl.total, x, n_cta) < stop) ++x;
-          static_cast<Cut*>(a.workspace)[cta] = Cut{x - cta, s.r0, s.live, s.row_base, s.h, {0, 0, 0}};
+        if (slot == 0 && !whole) {
+          int c0 = range.first, n_parts = range.parts;
+          if (n_parts == 0) {
+            const int begin = sh.w.u - s.t1, end = begin + s.T;  // the item's units
+            int c1 = cta + 1;
+            for (c0 = cta; c0 > 0 && range.dealt(c0) > begin; --c0) {}
+            while (range.dealt(c1) < end) ++c1;
+            n_parts = c1 - c0;
+          }
+          cuts[(*n_cuts)++] = Cut{c0, n_parts, s.r0, s.live, s.row_base, s.h, {0, 0}};
         }
         sh.more = sh.w.next(a, sh.s);
       }
       tcg::tc_fence_before();
       named_sync(1 + slot, 128);
     }
+    named_sync(3, 256);  // this CTA's parts are written
+    if (*n_cuts) join_parts<T, D>(a, cuts, *n_cuts, cta, tag, smem + L::Q, status);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     Segment s;
@@ -919,83 +1074,6 @@ __global__ void __launch_bounds__(NTHR, 1)
   if (warp == WARP_MMA) tcg::tmem_dealloc(tmem, 512);
 }
 
-// Joins the parts of the cut items. Block (k, y): rows 8 y .. 8 y + 7 of the k-th cut item, a warp a
-// row; the row's parts are read by all lanes at
-// once (their maxima and sums one part a lane) and added in order.
-template <typename T, int D>
-__global__ void __launch_bounds__(MAX_CTA) merge_kernel(const dspark_tree_attn_args a, const int n_cta) {
-  __shared__ int before[MAX_CTA / 32], found;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) found = -1;
-  pdl_launch_dependents();
-  pdl_wait();
-  const int tid = threadIdx.x;
-  const bool is_cut = tid < n_cta && __ldcg(&static_cast<const Cut*>(a.workspace)[tid].parts) != 0;
-  const unsigned cuts = __ballot_sync(0xffffffffu, is_cut);
-  if (lane == 0) before[warp] = __popc(cuts);
-  __syncthreads();
-  int rank = __popc(cuts & ((1u << lane) - 1u));
-  for (int w = 0; w < warp; ++w) rank += before[w];
-  if (is_cut && rank == int(blockIdx.x)) found = tid;
-  __syncthreads();
-  const int c = found;
-  if (c < 0) return;
-  const int4* cp = reinterpret_cast<const int4*>(static_cast<const Cut*>(a.workspace) + c);
-  const int4 c0 = __ldcg(cp), c1 = __ldcg(cp + 1);
-  const int parts = c0.x, r0 = c0.y, live = c0.z, row_base = c0.w, h = c1.x;
-  const int i = blockIdx.y * 8 + warp;
-  if (i >= live) return;
-  constexpr int VPL = D / 32;
-  constexpr int64_t STRIDE = int64_t(2) * (2 * ROWS) * (D + 2);  // floats between the CTAs' parts
-  const float* first = part<D>(a.workspace, c, 1);
-  const float* rest = part<D>(a.workspace, c + 1, 0);
-  auto at = [&](int x) { return x == 0 ? first : rest + (x - 1) * STRIDE; };
-  float m = -INFINITY;
-  for (int x = lane; x < parts; x += 32) {
-    const float v = __ldcg(at(x) + 2 * ROWS * D + 2 * i);
-    m = v == v ? fmaxf(m, v) : v;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float v = __shfl_xor_sync(0xffffffffu, m, o);
-    m = m == m && v == v ? fmaxf(m, v) : NAN;
-  }
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[VPL];
-#pragma unroll
-  for (int e = 0; e < VPL; ++e) o[e] = 0.f;
-  for (int x0 = 0; x0 < parts; x0 += 32) {
-    float w = 0.f, lx = 0.f;
-    if (x0 + lane < parts) {
-      const float2 st = __ldcg(reinterpret_cast<const float2*>(at(x0 + lane) + 2 * ROWS * D) + i);
-      w = ex2(st.x - ref);
-      lx = st.y * w;
-    }
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) lx += __shfl_xor_sync(0xffffffffu, lx, s);
-    l += lx;
-    const int nx = min(32, parts - x0);
-#pragma unroll 8
-    for (int x = 0; x < nx; ++x) {
-      const float f = __shfl_sync(0xffffffffu, w, x);
-      const float* p = at(x0 + x) + int64_t(i) * D + lane * VPL;
-      float v[VPL];
-      if (VPL == 4) *reinterpret_cast<float4*>(v) = __ldcg(reinterpret_cast<const float4*>(p));
-      else *reinterpret_cast<float2*>(v) = __ldcg(reinterpret_cast<const float2*>(p));
-#pragma unroll
-      for (int e = 0; e < VPL; ++e) o[e] += v[e] * f;
-    }
-  }
-  const int G = a.Hq / a.Hk, x = row_base + i, node = x / G, hq = h * G + x - node * G;
-  T* out = static_cast<T*>(a.out) + int64_t(r0 + node) * a.o_strides[0] + hq * a.o_strides[1] + lane * VPL;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int e = 0; e < VPL; e += 2) {
-    if (l == 0.f) o[e] = o[e + 1] = 0.f;
-    *reinterpret_cast<uint32_t*>(out + e) = Elem<T>::pack(o[e] * inv, o[e + 1] * inv);
-  }
-}
-
 static int grid_of(int device) { return std::min(sm_count(device), MAX_CTA); }
 
 template <typename T, int D>
@@ -1020,6 +1098,10 @@ static int launch(const dspark_tree_attn_args& a, cudaStream_t s) {
                   (long long)str[0], (long long)str[1], (long long)str[2]);
   }
   const int n_cta = grid_of(dev);
+  // the units are counted in 32 bits
+  const int64_t G = a.Hq / a.Hk;
+  if ((int64_t(a.R) * G / (2 * ROWS) + a.B) * a.Hk * ((int64_t(a.cap) + BN - 1) / BN + 1) > 0x7fffffff)
+    return fail(DSPARK_ERR_UNSUPPORTED, "tree_attn: %d rows over %d positions in one call", a.R, a.cap);
   const size_t smem = Lay<D>::TOTAL;
   DSPARK_CUDA_TRY(configure_once((const void*)attn_kernel<T, D>, int(smem),
                                  [&] {
@@ -1031,15 +1113,12 @@ static int launch(const dspark_tree_attn_args& a, cudaStream_t s) {
   // the running maximum needs a positive factor: the scale's sign goes into q
   const float c = fabsf(a.scale) * 1.4426950408889634f;
   const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
-  DSPARK_CUDA_TRY(launch_ex(attn_kernel<T, D>, dim3(n_cta), dim3(NTHR), smem, s, 1, true, maps[0], maps[1],
-                            a, sign == 0.f ? 1.f : c, sign, st),
+  static std::atomic<uint64_t> launches{uint64_t(std::chrono::steady_clock::now().time_since_epoch().count())};
+  const uint64_t tag = (launches.fetch_add(1, std::memory_order_relaxed) * 0x9E3779B97F4A7C15ull | 1ull << 63) &
+                       ~0xffffull;
+  DSPARK_CUDA_TRY(launch_all_at_once(attn_kernel<T, D>, dim3(n_cta), dim3(NTHR), smem, s, maps[0], maps[1],
+                                     a, sign == 0.f ? 1.f : c, sign, tag, st),
                   "tree_attn");
-  const int rows = int(std::min<int64_t>(2 * ROWS, int64_t(std::min(a.max_rows, a.R)) * (a.Hq / a.Hk)));
-  const int64_t items = int64_t(a.B) * a.Hk * ((int64_t(std::min(a.max_rows, a.R)) * (a.Hq / a.Hk) + 2 * ROWS - 1) / (2 * ROWS));
-  const int cuts = int(std::min<int64_t>(n_cta, items));  // at most one a CTA and one an item
-  DSPARK_CUDA_TRY(launch_ex(merge_kernel<T, D>, dim3(cuts, (rows + 7) / 8), dim3(MAX_CTA), 0, s, 1, true, a,
-                            n_cta),
-                  "tree_attn merge");
   return DSPARK_OK;
 }
 
@@ -1052,8 +1131,8 @@ extern "C" {
 
 size_t dspark_tree_attn_workspace(int B, int Hq, int Hk, int D, int max_rows) {
   if (B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || D <= 0 || max_rows <= 0) return 0;
-  return tattn::MAX_CTA * sizeof(tattn::Cut) +
-         size_t(tattn::grid_of(current_device())) * 2 * (2 * tattn::ROWS) * (D + 2) * sizeof(float);
+  return tattn::MAX_CTA * sizeof(uint64_t) +
+         size_t(tattn::grid_of(current_device())) * 2 * (2 * tattn::ROWS) * (D + 1) * sizeof(float);
 }
 
 int dspark_tree_attn(const dspark_tree_attn_args* p, void* stream) {
