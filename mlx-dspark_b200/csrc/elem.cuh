@@ -42,6 +42,9 @@ template <>
 struct Elem<float> {
   static __device__ __forceinline__ float to_f(float v) { return v; }
   static __device__ __forceinline__ float from_f(float v) { return v; }
+  static __device__ __forceinline__ float2 unpack(uint32_t w) {  // one value to a word
+    return make_float2(__uint_as_float(w), 0.f);
+  }
 };
 
 }  // namespace dspark

@@ -1,9 +1,21 @@
 // Verification of drafted tokens against the target's probabilities from given random numbers
-// (dspark_sample_accept).
+// (dspark_sample_accept): two kernels chained by programmatic dependent launch.
 //
-// Simple form: one block a logits row for its maximum, sum and first largest logit; one block a
-// request for the walk and the token after it.
+// stat_kernel: (row, slice) blocks read each logits row that decides something (one with a child) once:
+// running maximum and sum of exp2((l - m) log2e / T) in fp32, one (m, s, first largest) a slice. Rows
+// without a child (a chain's last, a tree's leaves) are not read: the token after them needs no sum.
+//
+// pick_kernel: (request, slice) blocks join the slices' sums, walk the block or tree (every block of a
+// request for itself, from a few hundred bytes), then read the one row that the next token comes from,
+// with its noise and draft rows, once: the slice's best score and its place. The request's last block
+// compares the slices in order (no result depends on timing) and writes the token.
+//  * after a rejection with a draft distribution the score is max(p - q, 0) / e, with the row's sum;
+//  * otherwise argmax p / e = argmax (l - ref) log2e / T - log2 e for any ref of the row: no sum, and
+//    no rounding of p to zero. ref is the largest logit so far, so that scores stay near zero.
+// Bound: HBM (each deciding row once), or the two launches for a single block.
 #include <float.h>
+
+#include <algorithm>
 
 #include "elem.cuh"
 #include "host_common.h"
@@ -11,37 +23,38 @@
 namespace dspark {
 namespace sample {
 
-// A logit as the formulas take it: NaN has no mass, +inf is the largest finite value.
-__device__ __forceinline__ float clean(float x) { return x == x ? fminf(x, FLT_MAX) : -INFINITY; }
+constexpr int THREADS = 256;
+constexpr int MAX_ROWS = 1024;
+constexpr int MAX_SLICE = 65536;   // values of one pick block (its bitmap: 8 KB)
+constexpr float LOG2E = 1.4426950408889634f;
 
-struct RowStat {
-  float m, s;  // largest logit, sum of exp((l - m) / T)
+struct Stat {
+  float m, s;  // largest logit, sum of exp((l - m) / T) of a slice
   int top;     // first place of the largest logit
   int pad;
 };
 
-// exp((l - m) / T); zero without mass (l = -inf, also where m is).
-__device__ __forceinline__ float mass(float l, float m, float T) {
-  return l == -INFINITY ? 0.f : expf((l - m) / T);
-}
+struct Pick {  // a slice's best: score relative to ref, place (NONE: no token with mass may be kept)
+  float ref, score;
+  int place, pad;
+};
+constexpr int NONE = 0x7fffffff;
 
+// A logit as the formulas take it: NaN has no mass, +inf is the largest finite value.
+__device__ __forceinline__ float clean(float x) { return x == x ? fminf(x, FLT_MAX) : -INFINITY; }
 __device__ __forceinline__ bool greedy(float T) { return !(T > 0.f); }
-
-template <typename T>
-__device__ __forceinline__ float prob_at(const T* row, int v, int V, const RowStat& st, float temp) {
-  if (v < 0 || v >= V || !(st.s > 0.f)) return 0.f;
-  if (greedy(temp)) return v == st.top ? 1.f : 0.f;
-  return mass(clean(Elem<T>::to_f(row[v])), st.m, temp) / st.s;
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-__device__ __forceinline__ int owner(const int32_t* cu, int B, int r) {
-  if (r >= cu[B]) return -1;
-  int lo = 0, hi = B - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cu[mid] <= r) lo = mid; else hi = mid - 1;
-  }
-  return lo;
+// log2e / T, kept off zero and infinity, where the differences of -inf and equal logits would be lost.
+__device__ __forceinline__ float slope(float T) { return fminf(fmaxf(LOG2E / T, FLT_MIN), 1e30f); }
+
+// exp((l - m) / T), c = log2e / T. (-inf - -inf has no mass either.)
+__device__ __forceinline__ float mass(float l, float m, float c) {
+  return l == -INFINITY ? 0.f : ex2((l - m) * c);
 }
 
 __device__ __forceinline__ void better(float& bv, int& bi, float v, int i) {
@@ -51,62 +64,217 @@ __device__ __forceinline__ void better(float& bv, int& bi, float v, int i) {
   }
 }
 
-__device__ void block_best(float& v, int& i) {
-  __shared__ float sv[32];
-  __shared__ int si[32];
+// Values of 16 bytes of a row.
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float ov = __shfl_xor_sync(0xffffffffu, v, o);
-    const int oi = __shfl_xor_sync(0xffffffffu, i, o);
-    better(v, i, ov, oi);
+    for (int i = 0; i < 4; ++i) {
+      if (sizeof(T) == 4) {
+        x[i] = __uint_as_float(w[i]);
+      } else {
+        const float2 f = Elem<T>::unpack(w[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
+    }
   }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) {
-    sv[threadIdx.x >> 5] = v;
-    si[threadIdx.x >> 5] = i;
-  }
-  __syncthreads();
-  v = sv[0];
-  i = si[0];
-  for (int w = 1; w < int(blockDim.x >> 5); ++w) better(v, i, sv[w], si[w]);
+};
+
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
 }
 
+struct Running {
+  float m = -INFINITY, s = 0.f;
+  int top = 0x7fffffff;
+};
+
+// Joins two slices' maxima and sums.
+__device__ __forceinline__ void join(Running& a, float m, float s, int top, float c, bool arg) {
+  if (arg) {
+    better(a.m, a.top, m, top);
+    return;
+  }
+  const float mn = fmaxf(a.m, m);
+  a.s = a.s * mass(a.m, mn, c) + s * mass(m, mn, c);
+  a.m = mn;
+}
+
+// grid R * slices: block (r, slice). Also clears the requests' counts for the next kernel.
 template <typename T>
-__global__ void __launch_bounds__(512) stat_simple_kernel(const dspark_sample_args a, RowStat* stat) {
+__global__ void __launch_bounds__(THREADS) stat_kernel(const dspark_sample_args a, Stat* stat,
+                                                       unsigned* done, const int slices) {
   pdl_launch_dependents();
   pdl_wait();
-  const int r = blockIdx.x, b = owner(a.cu_rows, a.B, r);
+  const int tid = threadIdx.x;
+  for (int b = blockIdx.x * THREADS + tid; b < a.B; b += gridDim.x * THREADS) done[b] = 0;
+  const int r = blockIdx.x / slices, slice = blockIdx.x - r * slices;
+  // the request of row r, and whether the row has a child
+  __shared__ int s_b;
+  if (tid == 0) s_b = -1;
+  __syncthreads();
+  for (int b = tid; b < a.B; b += THREADS)
+    if (a.cu_rows[b] <= r && r < a.cu_rows[b + 1]) s_b = b;
+  __syncthreads();
+  const int b = s_b;
   if (b < 0) return;
-  const float temp = a.temperature ? a.temperature[b] : 1.f;
-  const T* row = static_cast<const T*>(a.logits) + int64_t(r) * a.ld_logits;
-  float m = -INFINITY;
-  int top = 0x7fffffff;
-  for (int v = threadIdx.x; v < a.V; v += blockDim.x) better(m, top, clean(Elem<T>::to_f(row[v])), v);
-  block_best(m, top);
-  float s = 0.f;
-  if (greedy(temp)) {
-    s = m == -INFINITY ? 0.f : 1.f;
+  const int r0 = a.cu_rows[b], rows = min(a.cu_rows[b + 1], a.R) - r0;
+  bool has = false;
+  if (a.parent) {
+    for (int j = r - r0 + 1 + tid; j < rows; j += THREADS) has |= a.parent[r0 + j] == r - r0;
   } else {
-    for (int v = threadIdx.x; v < a.V; v += blockDim.x) s += mass(clean(Elem<T>::to_f(row[v])), m, temp);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    __shared__ float ss[32];
-    if ((threadIdx.x & 31) == 0) ss[threadIdx.x >> 5] = s;
-    __syncthreads();
-    s = 0.f;
-    for (int w = 0; w < int(blockDim.x >> 5); ++w) s += ss[w];
+    has = r + 1 < r0 + rows;
   }
-  if (threadIdx.x == 0) stat[r] = RowStat{m, s, top, 0};
+  if (!__syncthreads_or(has)) return;
+  const float temp = a.temperature ? a.temperature[b] : 1.f;
+  const bool arg = greedy(temp);
+  const float c = arg ? 0.f : slope(temp);
+  const T* row = static_cast<const T*>(a.logits) + int64_t(r) * a.ld_logits;
+  constexpr int N = Vec<T>::N;
+  // whole 16-byte vectors between the row's unaligned ends
+  const int head = min(a.V, int((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / int(sizeof(T)));
+  const int nv = (a.V - head) / N;
+  const int v0 = int(int64_t(nv) * slice / slices), v1 = int(int64_t(nv) * (slice + 1) / slices);
+  Running run;
+  auto one = [&](int i) {
+    const float x = clean(Elem<T>::to_f(row[i]));
+    join(run, x, x == -INFINITY ? 0.f : 1.f, i, c, arg);
+  };
+  if (slice == 0 && tid < head) one(tid);
+  if (slice == slices - 1 && tid < a.V - head - nv * N) one(head + nv * N + tid);
+  const T* body = row + head;
+  constexpr int U = 4;  // vectors in flight a thread
+  for (int v = v0 + tid; v < v1; v += U * THREADS) {
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v + u * THREADS < v1) raw[u] = ld_stream(body + int64_t(v + u * THREADS) * N);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (v + u * THREADS >= v1) break;
+      float x[N];
+      Vec<T>::unpack(raw[u], x);
+      if (arg) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) better(run.m, run.top, clean(x[e]), head + (v + u * THREADS) * N + e);
+      } else {
+        float mx = fmaxf(x[0], x[1]);  // passes over NaN
+#pragma unroll
+        for (int e = 2; e < N; ++e) mx = fmaxf(mx, x[e]);
+        if (mx > run.m) {
+          if (mx == INFINITY) {  // rare: +inf counts as the largest finite value
+            mx = FLT_MAX;
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = fminf(x[e], FLT_MAX);
+          }
+          run.s *= mass(run.m, mx, c);
+          run.m = mx;
+        }
+        if (run.m == FLT_MAX) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) x[e] = fminf(x[e], FLT_MAX);
+        }
+        if (run.m != -INFINITY) {
+          float sum[2] = {0.f, 0.f};
+#pragma unroll
+          for (int e = 0; e < N; ++e) sum[e & 1] += ex2(fmaxf((x[e] - run.m) * c, -INFINITY));  // NaN: none
+          run.s += sum[0] + sum[1];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    join(run, __shfl_xor_sync(0xffffffffu, run.m, o), __shfl_xor_sync(0xffffffffu, run.s, o),
+         __shfl_xor_sync(0xffffffffu, run.top, o), c, arg);
+  __shared__ Stat part[THREADS / 32];
+  if ((tid & 31) == 0) part[tid >> 5] = Stat{run.m, run.s, run.top, 0};
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < THREADS / 32; ++w) join(run, part[w].m, part[w].s, part[w].top, c, arg);
+    stat[int64_t(r) * slices + slice] = Stat{run.m, run.s, run.top, 0};
+  }
 }
+
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// How the next token is scored.
+enum Mode : int {
+  kLargest,  // greedy: the logit
+  kFree,     // any token, no sum known: (l - ref) c - log2 e
+  kBarred,   // tokens tried are out, masses that are zero in 32 bits are none: the same, ref = m
+  kRest      // max(p - q, 0) / e
+};
+
+struct Scorer {
+  Mode mode;
+  float m, c, inv;  // row's maximum and 1 / sum (kBarred, kRest), log2e / T
+  float ref, best;
+  int place;
+  // places come in ascending order: the first of equal scores stays
+  __device__ __forceinline__ void take(float score, int i) {
+    if (score > best) {
+      best = score;
+      place = i;
+    }
+  }
+  __device__ __forceinline__ void rebase(float mx) {  // kFree, before values up to mx
+    if (!(mx > ref)) return;
+    mx = fminf(mx, FLT_MAX);
+    if (mx > ref) {
+      best += ref == -INFINITY ? 0.f : (ref - mx) * c;
+      ref = mx;
+    }
+  }
+  __device__ __forceinline__ void look(float l, float q, float e, int i, bool barred) {
+    if (mode == kRest) {
+      const float p = ex2(fminf(fmaxf((l - m) * c, -INFINITY), 0.f)) * inv;
+      take((p - q) * rcp(e), i);
+    } else if (mode == kLargest) {
+      if (!barred) take(clean(l), i);
+    } else {
+      l = clean(l);
+      const float d = (l - ref) * c;
+      if (!barred && l != -INFINITY && (mode == kFree || d >= -149.f)) take(d - lg2(e), i);
+    }
+  }
+};
 
 template <typename T, typename Q>
-__global__ void __launch_bounds__(512) pick_simple_kernel(const dspark_sample_args a, const RowStat* stat) {
+__global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args a, const Stat* stat,
+                                                       Pick* picks, unsigned* done, const int slices,
+                                                       const int blocks) {
   pdl_launch_dependents();
+  __shared__ float s_p[MAX_ROWS];           // p of each row's token given its parent
+  __shared__ float s_m[MAX_ROWS], s_s[MAX_ROWS];
+  __shared__ int s_up[MAX_ROWS], s_id[MAX_ROWS];  // a tree's parents and tokens
+  __shared__ float s_u[MAX_ROWS];
+  __shared__ int s_tried[MAX_ROWS];         // tokens tried at the last row
+  __shared__ uint32_t s_map[MAX_SLICE / 32];  // those of them in this block's slice
+  __shared__ int s_last, s_n, s_ntried, s_fail;
   pdl_wait();
-  const int b = blockIdx.x;
-  const int r0 = a.cu_rows[b], rows = a.cu_rows[b + 1] - r0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int b = blockIdx.x / blocks, slice = blockIdx.x - b * blocks;
+  const bool lead = slice == 0;  // this block writes what does not depend on the slice
+  const int r0 = max(a.cu_rows[b], 0), rows = min(a.cu_rows[b + 1], a.R) - r0;
   if (rows <= 0) {
-    if (threadIdx.x == 0) {
+    if (lead && tid == 0) {
       a.n_accept[b] = 0;
       a.next_tok[b] = -1;
     }
@@ -114,78 +282,273 @@ __global__ void __launch_bounds__(512) pick_simple_kernel(const dspark_sample_ar
   }
   const int seen = min(rows, a.max_rows);  // rows that can be accepted
   const float temp = a.temperature ? a.temperature[b] : 1.f;
+  const bool arg = greedy(temp);
+  const float c = arg ? 0.f : slope(temp);
   const T* logits = static_cast<const T*>(a.logits);
   const Q* draft = static_cast<const Q*>(a.draft);
-  auto p = [&](int r, int v) { return prob_at(logits + int64_t(r) * a.ld_logits, v, a.V, stat[r], temp); };
-  auto up = [&](int i) { return a.parent ? a.parent[r0 + i] : i - 1; };
-  if (a.prob)
-    for (int i = threadIdx.x; i < rows; i += blockDim.x) {
-      const int u = up(i);
-      a.prob[r0 + i] = u >= 0 && u < i ? p(r0 + u, a.ids[r0 + i]) : 1.f;
+  auto up = [&](int i) {
+    const int u = a.parent ? a.parent[r0 + i] : i - 1;
+    return u < i ? u : -1;  // a parent that is not before its child is none
+  };
+
+  // p of every row's token (beyond `seen` too: they are reported), and the sums of the rows that the
+  // walk can end at; eight lanes a row. A chain's rows are decided here.
+  if (tid == 0) s_fail = MAX_ROWS;
+  if (a.parent) {
+    for (int i = tid; i < seen; i += THREADS) {
+      s_up[i] = up(i);
+      s_id[i] = a.ids[r0 + i];
+      s_u[i] = a.u[r0 + i];
     }
-  __shared__ int s_last, s_n;
-  if (threadIdx.x == 0) {
-    int cur = 0, n = 0;
-    if (a.path) a.path[r0] = 0;
-    for (bool more = true; more;) {
-      more = false;
-      float run = 0.f;
-      for (int j = cur + 1; j < seen; ++j) {
-        if (up(j) != cur) continue;
-        const int x = a.ids[r0 + j];
-        bool twin = false;
-        for (int e = cur + 1; e < j; ++e) twin |= up(e) == cur && a.ids[r0 + e] == x;
-        if (twin) continue;
-        bool ok;
-        const float px = p(r0 + cur, x);
-        if (a.parent) {
-          run += px;
-          ok = a.u[r0 + cur] < run;
-        } else {
-          const float q = draft && !greedy(temp) && x >= 0 && x < a.V
-                              ? Elem<Q>::to_f(draft[int64_t(r0 + cur) * a.ld_draft + x]) : 1.f;
-          ok = a.u[r0 + cur] * q < px;
-        }
-        if (ok) {
-          cur = j;
-          ++n;
-          if (a.path) a.path[r0 + n] = j;
-          more = true;
-          break;
-        }
-        if (!a.parent) break;
+  }
+  __syncthreads();
+  for (int i0 = tid >> 3; i0 < ((rows + 3) & ~3); i0 += THREADS / 8) {
+    const int u = i0 < rows ? up(i0) : -1;
+    Running run;
+    float l = -INFINITY, q = 1.f, chance = 0.f;
+    int x = -1;
+    if (u >= 0) {
+      x = a.ids[r0 + i0];
+      if (x >= 0 && x < a.V) {
+        l = clean(Elem<T>::to_f(logits[int64_t(r0 + u) * a.ld_logits + x]));
+        if (draft && !arg) q = Elem<Q>::to_f(draft[int64_t(r0 + u) * a.ld_draft + x]);
+      }
+      if (!a.parent) chance = a.u[r0 + u];
+      for (int k = tid & 7; k < slices; k += 8) {
+        const Stat st = stat[int64_t(r0 + u) * slices + k];
+        join(run, st.m, st.s, st.top, c, arg);
       }
     }
-    s_last = cur;
-    s_n = n;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1)
+      join(run, __shfl_xor_sync(0xffffffffu, run.m, o), __shfl_xor_sync(0xffffffffu, run.s, o),
+           __shfl_xor_sync(0xffffffffu, run.top, o), c, arg);
+    if ((tid & 7) == 0 && i0 < rows) {
+      float p = 1.f;
+      if (u >= 0) {
+        if (arg) p = run.m != -INFINITY && x == run.top ? 1.f : 0.f;
+        else p = run.s > 0.f ? mass(l, run.m, c) / run.s : 0.f;
+      }
+      if (lead && a.prob) a.prob[r0 + i0] = p;
+      if (i0 < seen) {
+        s_p[i0] = p;
+        if (u >= 0) {  // every child of u writes the same
+          s_m[u] = run.m;
+          s_s[u] = run.s;
+          if (!a.parent) {
+            if (!(chance * q < p)) atomicMin(&s_fail, u);
+            s_id[i0] = x;
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+
+  // the walk
+  if (!a.parent) {
+    const int stop = min(s_fail, seen - 1);
+    if (tid == 0) {
+      s_last = s_n = stop;
+      s_ntried = stop + 1 < seen ? 1 : 0;
+      if (s_ntried) s_tried[0] = s_id[stop + 1];
+    }
+    if (lead && a.path)
+      for (int i = tid; i < rows; i += THREADS) a.path[r0 + i] = i <= stop ? i : -1;
+  } else {
+    if (warp == 0) {
+      int cur = 0, n = 0, tried = 0;
+      if (lead && a.path && lane == 0) a.path[r0] = 0;
+      for (bool on = true; on;) {
+        on = false;
+        tried = 0;
+        float run = 0.f;
+        const float u = s_u[cur];
+        for (int j0 = cur + 1; j0 < seen && !on; j0 += 32) {
+          const int j = j0 + lane;
+          unsigned kids = __ballot_sync(0xffffffffu, j < seen && s_up[min(j, seen - 1)] == cur);
+          while (kids) {
+            const int k = j0 + __ffs(kids) - 1;
+            kids &= kids - 1;
+            const int x = s_id[k];
+            bool twin = false;
+            for (int t = lane; t < tried; t += 32) twin |= s_tried[t] == x;
+            if (__any_sync(0xffffffffu, twin)) continue;
+            if (lane == 0) s_tried[tried] = x;
+            __syncwarp();
+            ++tried;
+            run += s_p[k];
+            if (u < run) {
+              cur = k;
+              ++n;
+              if (lead && a.path && lane == 0) a.path[r0 + n] = k;
+              on = true;
+              break;
+            }
+          }
+        }
+      }
+      if (lane == 0) {
+        s_last = cur;
+        s_n = n;
+        s_ntried = tried;
+      }
+    }
+  }
+  __syncthreads();
+  if (a.parent && lead && a.path)
+    for (int i = s_n + 1 + tid; i < rows; i += THREADS) a.path[r0 + i] = -1;
+  const int last = s_last, n = s_n, ntried = s_ntried;
+  if (lead && tid == 0) {
     a.n_accept[b] = n;
     if (a.lens) a.lens[b] = max(0, a.lens[b] - (rows - 1 - n));
   }
-  __syncthreads();
-  const int last = s_last, n = s_n;
-  if (a.path)
-    for (int i = n + 1 + threadIdx.x; i < rows; i += blockDim.x) a.path[r0 + i] = -1;
-  const RowStat st = stat[r0 + last];
-  const bool rest = !a.parent && draft && !greedy(temp) && last + 1 < seen;
-  const Q* qrow = draft ? draft + int64_t(r0 + last) * a.ld_draft : nullptr;
+
+  // the token after it
+  const bool rest = draft && !arg && last + 1 < seen;  // a chain's rejection with a distribution
+  const T* row = logits + int64_t(r0 + last) * a.ld_logits;
+  const Q* qrow = rest ? draft + int64_t(r0 + last) * a.ld_draft : nullptr;
   const float* e = a.noise + int64_t(b) * a.ld_noise;
-  float wv = 0.f, pv = 0.f;
-  int wi = 0x7fffffff, pi = 0x7fffffff;
-  for (int v = threadIdx.x; v < a.V; v += blockDim.x) {
-    const float pr = p(r0 + last, v);
-    float w = pr;
-    if (rest) {
-      w = fmaxf(pr - Elem<Q>::to_f(qrow[v]), 0.f);
-    } else {
-      for (int j = last + 1; j < seen; ++j)
-        if (up(j) == last && a.ids[r0 + j] == v) w = 0.f;
+  const int w0 = int(int64_t(a.V) * slice / blocks) & ~7;
+  const int w1 = slice + 1 == blocks ? a.V : int(int64_t(a.V) * (slice + 1) / blocks) & ~7;
+  const bool bar = !rest && ntried > 0;
+  if (bar) {
+    for (int i = tid; i < (w1 - w0 + 31) / 32; i += THREADS) s_map[i] = 0;
+    __syncthreads();
+    for (int t = tid; t < ntried; t += THREADS) {
+      const int x = s_tried[t];
+      if (x >= w0 && x < w1) atomicOr(&s_map[(x - w0) >> 5], 1u << ((x - w0) & 31));
     }
-    if (w > 0.f) better(wv, wi, w / e[v], v);
-    if (pr > 0.f) better(pv, pi, pr / e[v], v);
+    __syncthreads();
   }
-  block_best(wv, wi);
-  block_best(pv, pi);
-  if (threadIdx.x == 0) a.next_tok[b] = !(st.s > 0.f) ? -1 : wi != 0x7fffffff ? wi : pi;
+  auto out = [&](int i) { return bar && ((s_map[(i - w0) >> 5] >> ((i - w0) & 31)) & 1u); };
+  Scorer sc;
+  sc.mode = rest ? kRest : arg ? kLargest : bar ? kBarred : kFree;
+  sc.m = ntried ? s_m[last] : 0.f;
+  sc.c = c;
+  sc.inv = rest && s_s[last] > 0.f ? 1.f / s_s[last] : 0.f;
+  sc.ref = sc.mode == kBarred ? sc.m : sc.mode == kFree ? -INFINITY : 0.f;
+  sc.best = rest ? 0.f : -INFINITY;
+  sc.place = NONE;
+  auto single = [&](int i) {
+    const float l = Elem<T>::to_f(row[i]);
+    if (sc.mode == kFree) sc.rebase(l);
+    sc.look(l, rest ? Elem<Q>::to_f(qrow[i]) : 0.f, e[i], i, out(i));
+  };
+  const bool aligned = ((reinterpret_cast<uintptr_t>(row) | reinterpret_cast<uintptr_t>(e) |
+                         reinterpret_cast<uintptr_t>(qrow)) & 15) == 0;
+  if (aligned) {
+    constexpr int U = 2;  // groups of eight values in flight a thread
+    const int wv = w1 & ~7;
+    for (int i0 = w0 + tid * 8; i0 < wv; i0 += U * THREADS * 8) {
+      uint4 ez[U][2], xl[U][sizeof(T) / 2], ql[U][sizeof(Q) / 2];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int i = i0 + k * THREADS * 8;
+        if (i >= wv) break;
+        ez[k][0] = ld_stream(e + i);
+        ez[k][1] = ld_stream(e + i + 4);
+        xl[k][0] = ld_stream(row + i);
+        if (sizeof(T) == 4) xl[k][sizeof(T) / 2 - 1] = ld_stream(row + i + 4);
+        if (rest) {
+          ql[k][0] = ld_stream(qrow + i);
+          if (sizeof(Q) == 4) ql[k][sizeof(Q) / 2 - 1] = ld_stream(qrow + i + 4);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int i = i0 + k * THREADS * 8;
+        if (i >= wv) break;
+        float x[8], q[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, z[8];
+        Vec<float>::unpack(ez[k][0], z);
+        Vec<float>::unpack(ez[k][1], z + 4);
+        Vec<T>::unpack(xl[k][0], x);
+        if (sizeof(T) == 4) Vec<T>::unpack(xl[k][sizeof(T) / 2 - 1], x + 4);
+        if (rest) {
+          Vec<Q>::unpack(ql[k][0], q);
+          if (sizeof(Q) == 4) Vec<Q>::unpack(ql[k][sizeof(Q) / 2 - 1], q + 4);
+        }
+        if (sc.mode == kFree) {
+          float mx = fmaxf(x[0], x[1]);
+#pragma unroll
+          for (int y = 2; y < 8; ++y) mx = fmaxf(mx, x[y]);
+          sc.rebase(mx);
+        }
+        const uint32_t map = bar ? s_map[(i - w0) >> 5] >> ((i - w0) & 31) : 0u;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) sc.look(x[y], q[y], z[y], i + y, (map >> y) & 1u);
+      }
+    }
+    for (int i = wv + tid; i < w1; i += THREADS) single(i);
+  } else {
+#pragma unroll 4
+    for (int i = w0 + tid; i < w1; i += THREADS) single(i);
+  }
+
+  // the best of the slice, then of the request's slices; scores of different refs by the difference of
+  // the refs, in 64 bits (greedy and kRest: the refs are zero). inf - inf of equal scores is a tie.
+  auto beats = [&](const Pick& x, const Pick& y) {
+    if (x.place == NONE || y.place == NONE) return y.place == NONE && x.place != NONE;
+    const double d = (double(x.ref) - double(y.ref)) * c + (double(x.score) - double(y.score));
+    return d > 0 || (!(d < 0) && x.place < y.place);
+  };
+  __shared__ Pick s_pick[THREADS / 32];
+  auto block_best = [&](Pick mine) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const Pick other{__shfl_xor_sync(0xffffffffu, mine.ref, o), __shfl_xor_sync(0xffffffffu, mine.score, o),
+                       __shfl_xor_sync(0xffffffffu, mine.place, o), 0};
+      if (beats(other, mine)) mine = other;
+    }
+    __syncthreads();
+    if (lane == 0) s_pick[warp] = mine;
+    __syncthreads();
+    mine = s_pick[0];
+    for (int w = 1; w < THREADS / 32; ++w)
+      if (beats(s_pick[w], mine)) mine = s_pick[w];
+    return mine;
+  };
+  const Pick mine = block_best(Pick{sc.ref, sc.best, sc.place, 0});
+  __shared__ bool s_final;
+  if (tid == 0) {
+    picks[int64_t(b) * blocks + slice] = mine;
+    __threadfence();
+    s_final = atomicAdd(&done[b], 1u) + 1 == unsigned(blocks);
+  }
+  __syncthreads();
+  if (!s_final) return;
+  __threadfence();
+  Pick win{0.f, 0.f, NONE, 0};
+  for (int k = tid; k < blocks; k += THREADS) {
+    const int4 raw = __ldcg(reinterpret_cast<const int4*>(&picks[int64_t(b) * blocks + k]));
+    const Pick x{__int_as_float(raw.x), __int_as_float(raw.y), raw.z, 0};
+    if (beats(x, win)) win = x;
+  }
+  win = block_best(win);
+  if (win.place == NONE && (rest || bar)) {
+    // nothing is left of the row's mass (only by rounding): the token is drawn from all of it
+    Scorer all = sc;
+    all.mode = arg ? kLargest : kBarred;
+    all.ref = arg ? 0.f : sc.m;
+    all.best = -INFINITY;
+    all.place = NONE;
+    for (int i = tid; i < a.V; i += THREADS) all.look(Elem<T>::to_f(row[i]), 0.f, e[i], i, false);
+    win = block_best(Pick{all.ref, all.best, all.place, 0});
+  }
+  if (tid == 0) a.next_tok[b] = win.place == NONE ? -1 : win.place;
+}
+
+// Slices of a row for stat_kernel: of 64 KB, so that many rows do not end in a half-filled last round of
+// blocks; with few rows more, blocks for eight an SM (a chain) or 32 (a tree: more than half of its
+// rows are leaves, whose blocks end at once); at least 2048 values each.
+static int slices_of(int R, int V, int size, bool tree, int sms) {
+  const int want = ((tree ? 32 : 8) * sms + R - 1) / std::max(R, 1);
+  return std::max(1, std::min(std::max(want, int(int64_t(V) * size / 65536)), V / 2048));
+}
+// Blocks of a request for pick_kernel: 16 an SM over all requests.
+static int blocks_of(int B, int V, int sms) {
+  const int want = (16 * sms + B - 1) / std::max(B, 1);
+  return std::max((V + MAX_SLICE - 1) / MAX_SLICE, std::max(1, std::min(want, V / 2048)));
 }
 
 }  // namespace sample
@@ -196,15 +559,17 @@ using namespace dspark;
 extern "C" {
 
 size_t dspark_sample_workspace(int R, int B, int V) {
-  (void)B; (void)V;
-  return R > 0 ? size_t(R) * sizeof(sample::RowStat) : 0;
+  if (R <= 0 || B <= 0 || V <= 0) return 0;
+  const int sms = sm_count(current_device());
+  return size_t(R) * sample::slices_of(R, V, 4, true, sms) * sizeof(sample::Stat) +
+         size_t(B) * sample::blocks_of(B, V, sms) * sizeof(sample::Pick) + size_t(B) * sizeof(unsigned);
 }
 
 int dspark_sample_accept(const dspark_sample_args* p, void* stream) {
   if (!p) return fail(DSPARK_ERR_ARG, "sample_accept: null argument");
   const dspark_sample_args& a = *p;
   if (a.R < 0 || a.B < 0 || a.V <= 0) return fail(DSPARK_ERR_ARG, "sample_accept: bad shape");
-  if (a.max_rows < 1 || a.max_rows > 1024)
+  if (a.max_rows < 1 || a.max_rows > sample::MAX_ROWS)
     return fail(DSPARK_ERR_UNSUPPORTED, "sample_accept: max_rows %d (1..1024)", a.max_rows);
   if (a.dtype < DSPARK_DTYPE_BF16 || a.dtype > DSPARK_DTYPE_F32 ||
       (a.draft && (a.draft_dtype < DSPARK_DTYPE_BF16 || a.draft_dtype > DSPARK_DTYPE_F32)))
@@ -219,20 +584,27 @@ int dspark_sample_accept(const dspark_sample_args* p, void* stream) {
   if (a.R && a.ld_logits < a.V) return fail(DSPARK_ERR_ARG, "sample_accept: logits rows overlap");
   if (a.ws_bytes < dspark_sample_workspace(a.R, a.B, a.V) || (a.R && !a.workspace))
     return fail(DSPARK_ERR_ARG, "sample_accept: workspace of %zu bytes", a.ws_bytes);
+  const int sms = sm_count(current_device());
+  const int slices = sample::slices_of(a.R, a.V, a.dtype == DSPARK_DTYPE_F32 ? 4 : 2, a.parent != nullptr, sms), blocks = sample::blocks_of(a.B, a.V, sms);
+  if (int64_t(a.R) * slices > 0x7fffffff || int64_t(a.B) * blocks > 0x7fffffff)
+    return fail(DSPARK_ERR_UNSUPPORTED, "sample_accept: %d rows, %d requests", a.R, a.B);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  sample::RowStat* st = static_cast<sample::RowStat*>(a.workspace);
-#define DSPARK_STAT(T)                                                                              \
-  DSPARK_CUDA_TRY(launch_ex(sample::stat_simple_kernel<T>, dim3(a.R), dim3(512), 0, s, 1, true, a, st), \
+  sample::Stat* st = static_cast<sample::Stat*>(a.workspace);
+  sample::Pick* picks = reinterpret_cast<sample::Pick*>(st + int64_t(a.R) * slices);
+  unsigned* done = reinterpret_cast<unsigned*>(picks + int64_t(a.B) * blocks);
+#define DSPARK_STAT(T)                                                                             \
+  DSPARK_CUDA_TRY(launch_ex(sample::stat_kernel<T>, dim3(a.R * slices), dim3(sample::THREADS), 0, s, 1, \
+                            true, a, st, done, slices),                                            \
+                  "sample_accept: sums")
+#define DSPARK_PICK(T, Q)                                                                          \
+  DSPARK_CUDA_TRY(launch_ex(sample::pick_kernel<T, Q>, dim3(a.B * blocks), dim3(sample::THREADS), 0, s, \
+                            1, true, a, (const sample::Stat*)st, picks, done, slices, blocks),            \
                   "sample_accept")
-#define DSPARK_PICK(T, Q)                                                                           \
-  DSPARK_CUDA_TRY(launch_ex(sample::pick_simple_kernel<T, Q>, dim3(a.B), dim3(512), 0, s, 1, true, a, \
-                            (const sample::RowStat*)st),                                            \
-                  "sample_accept")
-#define DSPARK_PICK_Q(T)                                                                            \
-  do {                                                                                              \
-    if (a.draft && a.draft_dtype == DSPARK_DTYPE_F32) DSPARK_PICK(T, float);                        \
-    else if (a.draft && a.draft_dtype == DSPARK_DTYPE_F16) DSPARK_PICK(T, __half);                  \
-    else DSPARK_PICK(T, bf16);                                                                      \
+#define DSPARK_PICK_Q(T)                                                                           \
+  do {                                                                                             \
+    if (a.draft && a.draft_dtype == DSPARK_DTYPE_F32) DSPARK_PICK(T, float);                       \
+    else if (a.draft && a.draft_dtype == DSPARK_DTYPE_F16) DSPARK_PICK(T, __half);                 \
+    else DSPARK_PICK(T, bf16);                                                                     \
   } while (0)
   if (a.R) {
     if (a.dtype == DSPARK_DTYPE_BF16) DSPARK_STAT(bf16);
