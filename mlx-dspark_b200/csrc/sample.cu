@@ -64,10 +64,62 @@ __device__ __forceinline__ void better(float& bv, int& bi, float v, int i) {
   }
 }
 
+// Two fp32 values in one 64-bit register, and the packed operations on them (sm_100).
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// The larger of both halves of two words, NaN if one is.
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, bf16) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, __half) {
+  uint32_t r;
+  asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, float) {
+  return __float_as_uint(max3_nan(__uint_as_float(a), __uint_as_float(b), __uint_as_float(b)));
+}
+
 // Values of 16 bytes of a row.
 template <typename T>
 struct Vec {
   static constexpr int N = 16 / sizeof(T);
+  // The largest value of n vectors, NaN if there is one.
+  static __device__ __forceinline__ float largest(const uint4* raw, int n) {
+    uint32_t m = raw[0].x;
+#pragma unroll
+    for (int u = 0; u < n; ++u) {
+      const uint32_t a = max2_nan(raw[u].x, raw[u].y, T()), b = max2_nan(raw[u].z, raw[u].w, T());
+      m = max2_nan(m, max2_nan(a, b, T()), T());
+    }
+    if (sizeof(T) == 4) return __uint_as_float(m);
+    const float2 f = Elem<T>::unpack(m);
+    return max3_nan(f.x, f.y, f.y);
+  }
   static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -98,6 +150,7 @@ struct Running {
 
 // Joins two slices' maxima and sums.
 __device__ __forceinline__ void join(Running& a, float m, float s, int top, float c, bool arg) {
+  // (a maximum of -inf has no mass, whatever s says)
   if (arg) {
     better(a.m, a.top, m, top);
     return;
@@ -150,44 +203,64 @@ __global__ void __launch_bounds__(THREADS) stat_kernel(const dspark_sample_args 
   if (slice == 0 && tid < head) one(tid);
   if (slice == slices - 1 && tid < a.V - head - nv * N) one(head + nv * N + tid);
   const T* body = row + head;
-  constexpr int U = 4;  // vectors in flight a thread
-  for (int v = v0 + tid; v < v1; v += U * THREADS) {
-    uint4 raw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v + u * THREADS < v1) raw[u] = ld_stream(body + int64_t(v + u * THREADS) * N);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (v + u * THREADS >= v1) break;
+  if (arg) {
+    for (int v = v0 + tid; v < v1; v += THREADS) {
       float x[N];
-      Vec<T>::unpack(raw[u], x);
-      if (arg) {
+      Vec<T>::unpack(ld_stream(body + int64_t(v) * N), x);
 #pragma unroll
-        for (int e = 0; e < N; ++e) better(run.m, run.top, clean(x[e]), head + (v + u * THREADS) * N + e);
-      } else {
-        float mx = fmaxf(x[0], x[1]);  // passes over NaN
+      for (int e = 0; e < N; ++e) better(run.m, run.top, clean(x[e]), head + v * N + e);
+    }
+  } else {
+    // groups of G vectors under one maximum; the loop is bound by instructions as much as by HBM, so
+    // values go in pairs, and only a group whose maximum is NaN or +inf is looked at one by one
+    constexpr int G = sizeof(T) == 4 ? 4 : 2, U = 4;  // U vectors in flight a thread
+    const f32x2 c2 = pack2(c, c);
+    auto group = [&](const uint4* raw) {
+      float mx = Vec<T>::largest(raw, G);
+      if (!(mx < INFINITY)) {
+        for (int u = 0; u < G; ++u) {
+          float x[N];
+          Vec<T>::unpack(raw[u], x);
 #pragma unroll
-        for (int e = 2; e < N; ++e) mx = fmaxf(mx, x[e]);
-        if (mx > run.m) {
-          if (mx == INFINITY) {  // rare: +inf counts as the largest finite value
-            mx = FLT_MAX;
-#pragma unroll
-            for (int e = 0; e < N; ++e) x[e] = fminf(x[e], FLT_MAX);
-          }
-          run.s *= mass(run.m, mx, c);
-          run.m = mx;
+          for (int e = 0; e < N; ++e) join(run, clean(x[e]), 1.f, 0, c, false);
         }
-        if (run.m == FLT_MAX) {
+        return;
+      }
+      if (mx > run.m) {
+        run.s *= mass(run.m, mx, c);
+        run.m = mx;
+      }
+      if (run.m == -INFINITY) return;
+      const f32x2 m2 = pack2(-run.m, -run.m);
+      f32x2 sum[2] = {0ull, 0ull};
 #pragma unroll
-          for (int e = 0; e < N; ++e) x[e] = fminf(x[e], FLT_MAX);
-        }
-        if (run.m != -INFINITY) {
-          float sum[2] = {0.f, 0.f};
+      for (int u = 0; u < G; ++u) {
+        float x[N];
+        Vec<T>::unpack(raw[u], x);
 #pragma unroll
-          for (int e = 0; e < N; ++e) sum[e & 1] += ex2(fmaxf((x[e] - run.m) * c, -INFINITY));  // NaN: none
-          run.s += sum[0] + sum[1];
+        for (int e = 0; e < N; e += 2) {
+          float p0, p1;
+          unpack2(mul2(add2(pack2(x[e], x[e + 1]), m2), c2), p0, p1);
+          sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(ex2(p0), ex2(p1)));
         }
       }
+      float s0, s1;
+      unpack2(add2(sum[0], sum[1]), s0, s1);
+      run.s += s0 + s1;
+    };
+    int v = v0 + tid;
+    for (; v + (U - 1) * THREADS < v1; v += U * THREADS) {
+      uint4 raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = ld_stream(body + int64_t(v + u * THREADS) * N);
+#pragma unroll
+      for (int u = 0; u < U; u += G) group(raw + u);
+    }
+    for (; v < v1; v += THREADS) {
+      float x[N];
+      Vec<T>::unpack(ld_stream(body + int64_t(v) * N), x);
+#pragma unroll
+      for (int e = 0; e < N; ++e) join(run, clean(x[e]), 1.f, 0, c, false);
     }
   }
 #pragma unroll
@@ -223,7 +296,6 @@ enum Mode : int {
 };
 
 struct Scorer {
-  Mode mode;
   float m, c, inv;  // row's maximum and 1 / sum (kBarred, kRest), log2e / T
   float ref, best;
   int place;
@@ -242,6 +314,7 @@ struct Scorer {
       ref = mx;
     }
   }
+  template <Mode mode>
   __device__ __forceinline__ void look(float l, float q, float e, int i, bool barred) {
     if (mode == kRest) {
       const float p = ex2(fminf(fmaxf((l - m) * c, -INFINITY), 0.f)) * inv;
@@ -423,21 +496,28 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
   }
   auto out = [&](int i) { return bar && ((s_map[(i - w0) >> 5] >> ((i - w0) & 31)) & 1u); };
   Scorer sc;
-  sc.mode = rest ? kRest : arg ? kLargest : bar ? kBarred : kFree;
+  const Mode mode = rest ? kRest : arg ? kLargest : bar ? kBarred : kFree;
   sc.m = ntried ? s_m[last] : 0.f;
   sc.c = c;
   sc.inv = rest && s_s[last] > 0.f ? 1.f / s_s[last] : 0.f;
-  sc.ref = sc.mode == kBarred ? sc.m : sc.mode == kFree ? -INFINITY : 0.f;
+  sc.ref = mode == kBarred ? sc.m : mode == kFree ? -INFINITY : 0.f;
   sc.best = rest ? 0.f : -INFINITY;
   sc.place = NONE;
-  auto single = [&](int i) {
-    const float l = Elem<T>::to_f(row[i]);
-    if (sc.mode == kFree) sc.rebase(l);
-    sc.look(l, rest ? Elem<Q>::to_f(qrow[i]) : 0.f, e[i], i, out(i));
-  };
   const bool aligned = ((reinterpret_cast<uintptr_t>(row) | reinterpret_cast<uintptr_t>(e) |
                          reinterpret_cast<uintptr_t>(qrow)) & 15) == 0;
-  if (aligned) {
+  auto scan = [&](auto mode_c) {
+    constexpr Mode MODE = decltype(mode_c)::value;
+    constexpr bool REST = MODE == kRest;
+    auto single = [&](int i) {
+      const float l = Elem<T>::to_f(row[i]);
+      if (MODE == kFree) sc.rebase(l);
+      sc.look<MODE>(l, REST ? Elem<Q>::to_f(qrow[i]) : 0.f, e[i], i, out(i));
+    };
+    if (!aligned) {
+#pragma unroll 4
+      for (int i = w0 + tid; i < w1; i += THREADS) single(i);
+      return;
+    }
     constexpr int U = 2;  // groups of eight values in flight a thread
     const int wv = w1 & ~7;
     for (int i0 = w0 + tid * 8; i0 < wv; i0 += U * THREADS * 8) {
@@ -450,7 +530,7 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
         ez[k][1] = ld_stream(e + i + 4);
         xl[k][0] = ld_stream(row + i);
         if (sizeof(T) == 4) xl[k][sizeof(T) / 2 - 1] = ld_stream(row + i + 4);
-        if (rest) {
+        if (REST) {
           ql[k][0] = ld_stream(qrow + i);
           if (sizeof(Q) == 4) ql[k][sizeof(Q) / 2 - 1] = ld_stream(qrow + i + 4);
         }
@@ -464,26 +544,27 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
         Vec<float>::unpack(ez[k][1], z + 4);
         Vec<T>::unpack(xl[k][0], x);
         if (sizeof(T) == 4) Vec<T>::unpack(xl[k][sizeof(T) / 2 - 1], x + 4);
-        if (rest) {
+        if (REST) {
           Vec<Q>::unpack(ql[k][0], q);
           if (sizeof(Q) == 4) Vec<Q>::unpack(ql[k][sizeof(Q) / 2 - 1], q + 4);
         }
-        if (sc.mode == kFree) {
+        if (MODE == kFree) {
           float mx = fmaxf(x[0], x[1]);
 #pragma unroll
           for (int y = 2; y < 8; ++y) mx = fmaxf(mx, x[y]);
           sc.rebase(mx);
         }
-        const uint32_t map = bar ? s_map[(i - w0) >> 5] >> ((i - w0) & 31) : 0u;
+        const uint32_t map = !REST && bar ? s_map[(i - w0) >> 5] >> ((i - w0) & 31) : 0u;
 #pragma unroll
-        for (int y = 0; y < 8; ++y) sc.look(x[y], q[y], z[y], i + y, (map >> y) & 1u);
+        for (int y = 0; y < 8; ++y) sc.look<MODE>(x[y], q[y], z[y], i + y, (map >> y) & 1u);
       }
     }
     for (int i = wv + tid; i < w1; i += THREADS) single(i);
-  } else {
-#pragma unroll 4
-    for (int i = w0 + tid; i < w1; i += THREADS) single(i);
-  }
+  };
+  if (mode == kRest) scan(std::integral_constant<Mode, kRest>());
+  else if (mode == kLargest) scan(std::integral_constant<Mode, kLargest>());
+  else if (mode == kBarred) scan(std::integral_constant<Mode, kBarred>());
+  else scan(std::integral_constant<Mode, kFree>());
 
   // the best of the slice, then of the request's slices; scores of different refs by the difference of
   // the refs, in 64 bits (greedy and kRest: the refs are zero). inf - inf of equal scores is a tie.
@@ -528,11 +609,13 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
   if (win.place == NONE && (rest || bar)) {
     // nothing is left of the row's mass (only by rounding): the token is drawn from all of it
     Scorer all = sc;
-    all.mode = arg ? kLargest : kBarred;
     all.ref = arg ? 0.f : sc.m;
     all.best = -INFINITY;
     all.place = NONE;
-    for (int i = tid; i < a.V; i += THREADS) all.look(Elem<T>::to_f(row[i]), 0.f, e[i], i, false);
+    for (int i = tid; i < a.V; i += THREADS) {
+      if (arg) all.look<kLargest>(Elem<T>::to_f(row[i]), 0.f, e[i], i, false);
+      else all.look<kBarred>(Elem<T>::to_f(row[i]), 0.f, e[i], i, false);
+    }
     win = block_best(Pick{all.ref, all.best, all.place, 0});
   }
   if (tid == 0) a.next_tok[b] = win.place == NONE ? -1 : win.place;
