@@ -96,28 +96,34 @@ class RopeTable:
         turns = [int(round(x / (2 * math.pi) % 1.0 * 2.0 ** 64)) % 2 ** 64 for x in self.inv_freq]
         self.freq = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns],
                                  dtype=torch.int64, device=device)
-        self._layout = _LAYOUTS[layout]
+        self.freq_ptr, self.layout_code = self.freq.data_ptr(), _LAYOUTS[layout]
 
 
-def _last_contiguous(name: str, t: torch.Tensor) -> torch.Tensor:
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
+_pack = _lib.packer(_lib.RopeArgs)
+
+
+def _strides(name: str, t: torch.Tensor) -> tuple:
+    """``t``'s strides, the last of them checked to be 1."""
+    st = t.stride()
+    if st[-1] != 1 and t.shape[-1] > 1:
         raise _lib.DSparkUnsupported(_lib.ERR_UNSUPPORTED, f"{name}: head_dim must be contiguous")
-    return t
+    return st
 
 
-def _dtype(*named) -> int:
-    first = named[0][1].dtype
-    for name, t in named:
-        if t is not None and t.dtype != first:
-            raise _lib.DSparkUnsupported(_lib.ERR_UNSUPPORTED, f"{name} is {t.dtype}, not {first}")
-    if first not in _DT:
-        raise _lib.DSparkUnsupported(_lib.ERR_UNSUPPORTED, f"{first} (bf16 or fp16)")
-    return _DT[first]
+def _dtype(first: torch.Tensor, *rest: torch.Tensor | None) -> int:
+    dt = first.dtype
+    for t in rest:
+        if t is not None and t.dtype is not dt:
+            raise _lib.DSparkUnsupported(_lib.ERR_UNSUPPORTED, f"tensors of {dt} and {t.dtype}")
+    code = _DT.get(dt)
+    if code is None:
+        raise _lib.DSparkUnsupported(_lib.ERR_UNSUPPORTED, f"{dt} (bf16 or fp16)")
+    return code
 
 
-def _norm_weight(name: str, w: torch.Tensor | None, D: int):
+def _norm_weight(name: str, w: torch.Tensor | None, D: int) -> int:
     if w is None:
-        return None
+        return 0
     if w.numel() != D or not w.is_contiguous():
         raise _lib.DSparkError(_lib.ERR_ARG, f"{name} must be a contiguous [{D}]")
     return w.data_ptr()
@@ -133,35 +139,31 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: RopeTa
     ``[B, Hk, cap, D]``. Returns the rotated q (``q_out``, which may be ``q``). All tensors may be
     strided views with head_dim contiguous. ``row_*`` are int32 ``[R]`` on the device; rows outside
     the cache are dropped and recorded in the device status."""
-    dev, stream = on_device(q, k, v, k_cache, v_cache, row_pos, row_slot, row_req, q_norm, k_norm,
-                            q_out, table.freq)
-    if q.ndim != 3 or k.ndim != 3 or k_cache.ndim != 4:
+    stream = on_device(q, k, v, k_cache, v_cache, row_pos, row_slot, row_req, q_norm, k_norm, q_out,
+                       table.freq)
+    shape, cache = q.shape, k_cache.shape
+    if len(shape) != 3 or k.ndim != 3 or len(cache) != 4:
         raise _lib.DSparkError(_lib.ERR_ARG, "rope_append: q / k [R, H, D], caches [B, H, cap, D]")
-    R, Hq, D = q.shape
-    B, Hk, cap, Dc = k_cache.shape
-    if k.shape != (R, Hk, D) or v.shape != k.shape or v_cache.shape != k_cache.shape or Dc != D:
-        raise _lib.DSparkError(_lib.ERR_ARG, f"rope_append: q {tuple(q.shape)}, k {tuple(k.shape)}, "
-                               f"v {tuple(v.shape)}, caches {tuple(k_cache.shape)}")
+    R, Hq, D = shape
+    B, Hk, cap, Dc = cache
+    if k.shape != (R, Hk, D) or v.shape != k.shape or v_cache.shape != cache or Dc != D:
+        raise _lib.DSparkError(_lib.ERR_ARG, f"rope_append: q {tuple(shape)}, k {tuple(k.shape)}, "
+                               f"v {tuple(v.shape)}, caches {tuple(cache)}")
     if D != table.head_dim:
         raise _lib.DSparkError(_lib.ERR_ARG, f"head_dim {D}, the table's is {table.head_dim}")
     if q_out is None:
-        q_out = torch.empty((R, Hq, D), dtype=q.dtype, device=dev)
-    elif q_out.shape != q.shape:
-        raise _lib.DSparkError(_lib.ERR_ARG, f"q_out {tuple(q_out.shape)} for {tuple(q.shape)}")
-    for name, t in (("q", q), ("k", k), ("v", v), ("q_out", q_out), ("k_cache", k_cache),
-                    ("v_cache", v_cache)):
-        _last_contiguous(name, t)
-    dt = _dtype(("q", q), ("k", k), ("v", v), ("q_out", q_out), ("k_cache", k_cache),
-                ("v_cache", v_cache), ("q_norm", q_norm), ("k_norm", k_norm))
-    int32("row_pos", row_pos, R), int32("row_slot", row_slot, R), int32("row_req", row_req, R)
-    a = _lib.RopeArgs(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride()[:2], k.stride()[:2], v.stride()[:2],
-        q_out.data_ptr(), q_out.stride()[:2], k_cache.data_ptr(), v_cache.data_ptr(),
-        k_cache.stride()[:3], v_cache.stride()[:3], table.freq.data_ptr(), row_pos.data_ptr(),
-        row_slot.data_ptr(), None if row_req is None else row_req.data_ptr(),
-        _norm_weight("q_norm", q_norm, D), _norm_weight("k_norm", k_norm, D), table.mscale, eps, dt,
-        table._layout, R, Hq, Hk, D, table.rotary_dim, cap, B)
-    _lib.check(_lib.lib.dspark_rope_append(a, stream))
+        q_out = torch.empty((R, Hq, D), dtype=q.dtype, device=q.device)
+    elif q_out.shape != shape:
+        raise _lib.DSparkError(_lib.ERR_ARG, f"q_out {tuple(q_out.shape)} for {tuple(shape)}")
+    qs, ks, vs, os = _strides("q", q), _strides("k", k), _strides("v", v), _strides("q_out", q_out)
+    kc, vc = _strides("k_cache", k_cache), _strides("v_cache", v_cache)
+    dt = _dtype(q, k, v, q_out, k_cache, v_cache, q_norm, k_norm)
+    _lib.check(_lib.lib.dspark_rope_append(_pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
+        q_out.data_ptr(), os[0], os[1], k_cache.data_ptr(), v_cache.data_ptr(), kc[0], kc[1], kc[2],
+        vc[0], vc[1], vc[2], table.freq_ptr, int32("row_pos", row_pos, R), int32("row_slot", row_slot, R),
+        int32("row_req", row_req, R), _norm_weight("q_norm", q_norm, D), _norm_weight("k_norm", k_norm, D),
+        table.mscale, eps, dt, table.layout_code, R, Hq, Hk, D, table.rotary_dim, cap, B), stream))
     return q_out
 
 
@@ -170,21 +172,18 @@ def rotate(x: torch.Tensor, table: RopeTable, row_pos: torch.Tensor, *,
            out: torch.Tensor | None = None) -> torch.Tensor:
     """Rotate packed rows ``x [R, H, D]`` to ``row_pos`` (int32 ``[R]``), no cache; ``out`` may be
     ``x``."""
-    dev, stream = on_device(x, row_pos, norm, out, table.freq)
+    stream = on_device(x, row_pos, norm, out, table.freq)
     if x.ndim != 3 or x.shape[2] != table.head_dim:
         raise _lib.DSparkError(_lib.ERR_ARG, f"rotate: {tuple(x.shape)}, head_dim {table.head_dim}")
     R, H, D = x.shape
     if out is None:
-        out = torch.empty((R, H, D), dtype=x.dtype, device=dev)
+        out = torch.empty((R, H, D), dtype=x.dtype, device=x.device)
     elif out.shape != x.shape:
         raise _lib.DSparkError(_lib.ERR_ARG, f"out {tuple(out.shape)} for {tuple(x.shape)}")
-    _last_contiguous("x", x), _last_contiguous("out", out)
-    dt = _dtype(("x", x), ("out", out), ("norm", norm))
-    int32("row_pos", row_pos, R)
-    a = _lib.RopeArgs(q=x.data_ptr(), q_strides=x.stride()[:2], q_out=out.data_ptr(),
-                      qo_strides=out.stride()[:2], freq=table.freq.data_ptr(),
-                      row_pos=row_pos.data_ptr(), q_norm=_norm_weight("norm", norm, D),
-                      mscale=table.mscale, eps=eps, dtype=dt, layout=table._layout, R=R, Hq=H, Hk=0,
-                      D=D, rot=table.rotary_dim)
-    _lib.check(_lib.lib.dspark_rope_append(a, stream))
+    xs, os = _strides("x", x), _strides("out", out)
+    dt = _dtype(x, out, norm)
+    _lib.check(_lib.lib.dspark_rope_append(_pack(
+        x.data_ptr(), 0, 0, xs[0], xs[1], 0, 0, 0, 0, out.data_ptr(), os[0], os[1], 0, 0, 0, 0, 0, 0, 0, 0,
+        table.freq_ptr, int32("row_pos", row_pos, R), 0, 0, _norm_weight("norm", norm, D), 0, table.mscale,
+        eps, dt, table.layout_code, R, H, 0, D, table.rotary_dim, 0, 0), stream))
     return out

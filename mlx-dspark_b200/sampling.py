@@ -16,16 +16,21 @@ from ._torch import int32, on_device
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-def _rows_of(name: str, t: torch.Tensor, rows: int, V: int) -> torch.Tensor:
-    if t.ndim != 2 or t.shape[0] != rows or t.shape[1] != V or (V > 1 and t.stride(1) != 1):
+_pack = _lib.packer(_lib.SampleArgs)
+
+
+def _rows_of(name: str, t: torch.Tensor, rows: int, V: int) -> int:
+    """Row stride of ``t``, checked to be ``[rows, V]`` with contiguous rows."""
+    st = t.stride()
+    if t.shape != (rows, V) or (V > 1 and st[1] != 1):
         raise _lib.DSparkError(_lib.ERR_ARG, f"{name} {tuple(t.shape)}: [{rows}, {V}] with contiguous rows")
-    return t
+    return st[0]
 
 
-def _f32(name: str, t: torch.Tensor | None, n: int):
+def _f32(name: str, t: torch.Tensor | None, n: int) -> int:
     if t is None:
-        return None
-    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+        return 0
+    if t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous():
         raise _lib.DSparkError(_lib.ERR_ARG, f"{name} must be {n} contiguous float32 values")
     return t.data_ptr()
 
@@ -51,34 +56,32 @@ def sample_accept(logits: torch.Tensor, ids: torch.Tensor, cu_rows: torch.Tensor
     drafts), ``next``, ``prob`` (p of each row's token given its parent, 1 for roots) and ``path``
     (kept places of each request in order, then -1); ``lens`` (int32 ``[B]``, tokens cached after the
     verify's append) loses the rejected rows in place. ``max_rows`` (<= 1024) bounds a block."""
-    dev, stream = on_device(logits, ids, cu_rows, u, noise, temperature, draft_probs, parent, lens)
+    stream = on_device(logits, ids, cu_rows, u, noise, temperature, draft_probs, parent, lens)
     R, B = ids.numel(), cu_rows.numel() - 1
     V = logits.shape[-1]
-    _rows_of("logits", logits, R, V), _rows_of("noise", noise, B, V)
-    if logits.dtype not in _DT or (draft_probs is not None and draft_probs.dtype not in _DT):
-        raise _lib.DSparkUnsupported(_lib.ERR_UNSUPPORTED, f"logits {logits.dtype} (bf16, fp16 or fp32)")
-    if noise.dtype != torch.float32:
-        raise _lib.DSparkError(_lib.ERR_ARG, f"noise is {noise.dtype}, not float32")
+    ld, ld_noise = _rows_of("logits", logits, R, V), _rows_of("noise", noise, B, V)
+    dt, ddt, draft, ld_draft = _DT.get(logits.dtype), 0, 0, 0
     if draft_probs is not None:
-        _rows_of("draft_probs", draft_probs, R, V)
-    int32("ids", ids), int32("cu_rows", cu_rows), int32("parent", parent, R), int32("lens", lens, B)
+        ld_draft = _rows_of("draft_probs", draft_probs, R, V)
+        draft, ddt = draft_probs.data_ptr(), _DT.get(draft_probs.dtype)
+    if dt is None or ddt is None:
+        raise _lib.DSparkUnsupported(_lib.ERR_UNSUPPORTED, "logits and draft_probs: bf16, fp16 or fp32")
+    if noise.dtype is not torch.float32:
+        raise _lib.DSparkError(_lib.ERR_ARG, f"noise is {noise.dtype}, not float32")
     if out is None:
-        e = dict(dtype=torch.int32, device=dev)
+        e = dict(dtype=torch.int32, device=logits.device)
         out = {"n": torch.empty(B, **e), "next": torch.empty(B, **e),
-               "prob": torch.empty(R, dtype=torch.float32, device=dev), "path": torch.empty(R, **e)}
+               "prob": torch.empty(R, dtype=torch.float32, device=logits.device),
+               "path": torch.empty(R, **e)}
     else:
-        int32("n", out["n"], B), int32("next", out["next"], B), int32("path", out["path"], R)
         on_device(logits, out["n"], out["next"], out["prob"], out["path"])
-    n = int(_lib.lib.dspark_sample_workspace(R, B, V))
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    a = _lib.SampleArgs(
-        logits.data_ptr(), None if draft_probs is None else draft_probs.data_ptr(), logits.stride(0),
-        0 if draft_probs is None else draft_probs.stride(0), noise.stride(0), ids.data_ptr(),
-        cu_rows.data_ptr(), None if parent is None else parent.data_ptr(), _f32("u", u, R),
-        noise.data_ptr(), _f32("temperature", temperature, B), out["n"].data_ptr(),
-        out["next"].data_ptr(), _f32("prob", out["prob"], R), out["path"].data_ptr(),
-        None if lens is None else lens.data_ptr(), None if ws is None else ws.data_ptr(), n,
-        _DT[logits.dtype], 0 if draft_probs is None else _DT[draft_probs.dtype], R, B, V, max_rows)
-    _lib.check(_lib.lib.dspark_sample_accept(a, stream))
+    n = _lib.lib.dspark_sample_workspace(R, B, V)
+    ws = torch.empty(n, dtype=torch.uint8, device=logits.device) if n else None
+    _lib.check(_lib.lib.dspark_sample_accept(_pack(
+        logits.data_ptr(), draft, ld, ld_draft, ld_noise, int32("ids", ids), int32("cu_rows", cu_rows),
+        int32("parent", parent, R), _f32("u", u, R), noise.data_ptr(), _f32("temperature", temperature, B),
+        int32("n", out["n"], B), int32("next", out["next"], B), _f32("prob", out["prob"], R),
+        int32("path", out["path"], R), int32("lens", lens, B), ws.data_ptr() if n else 0, n, dt, ddt, R, B, V,
+        max_rows), stream))
     out["lens"] = lens
     return out

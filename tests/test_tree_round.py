@@ -42,6 +42,20 @@ def test_ctypes_mirrors_match_the_header_layout(tmp_path):
     assert {k: int(v) for k, v in (line.split() for line in out.splitlines())} == want
 
 
+def test_packed_arguments_are_the_structs():
+    for py in _MIRRORS:
+        cls = getattr(_lib, py)
+        flat, args = [], {}
+        for k, (name, t) in enumerate(cls._fields_):
+            if hasattr(t, "_length_"):
+                args[name] = tuple(1000 * k + i for i in range(t._length_))
+                flat += args[name]
+            else:
+                args[name] = k + 1
+                flat.append(k + 1)
+        assert _lib.packer(cls)(*flat) == bytes(cls(**args))
+
+
 def _fake():
     buf = (C.c_uint8 * 64)()
     return C.cast(buf, C.c_void_p).value
@@ -53,7 +67,7 @@ def test_rope_refusals():
               layout=0, R=1, Hq=2, Hk=1, D=64, rot=64, cap=8, batch=1)
 
     def rc(**kw):
-        return _lib.lib.dspark_rope_append(_lib.RopeArgs(**{**ok, **kw}), None)
+        return _lib.lib.dspark_rope_append(C.byref(_lib.RopeArgs(**{**ok, **kw})), None)
 
     assert rc(dtype=2) == _lib.ERR_UNSUPPORTED and "dtype" in _lib.last_error()
     assert rc(D=72) == _lib.ERR_UNSUPPORTED and "head_dim" in _lib.last_error()
@@ -73,7 +87,7 @@ def test_tree_attn_refusals():
               o_strides=(256, 64), k_strides=s3, v_strides=s3)
 
     def rc(**kw):
-        return _lib.lib.dspark_tree_attn(_lib.TreeAttnArgs(**{**ok, **kw}), None)
+        return _lib.lib.dspark_tree_attn(C.byref(_lib.TreeAttnArgs(**{**ok, **kw})), None)
 
     assert rc(dtype=2) == _lib.ERR_UNSUPPORTED and "dtype" in _lib.last_error()
     assert rc(D=96) == _lib.ERR_UNSUPPORTED and "head_dim" in _lib.last_error()
@@ -89,7 +103,7 @@ def test_sample_accept_refusals():
               ws_bytes=1 << 40, ld_logits=100, ld_noise=100, dtype=0, R=4, B=1, V=100, max_rows=4)
 
     def rc(**kw):
-        return _lib.lib.dspark_sample_accept(_lib.SampleArgs(**{**ok, **kw}), None)
+        return _lib.lib.dspark_sample_accept(C.byref(_lib.SampleArgs(**{**ok, **kw})), None)
 
     assert rc(dtype=3) == _lib.ERR_UNSUPPORTED and rc(draft=p, draft_dtype=-1) == _lib.ERR_UNSUPPORTED
     assert rc(draft=p, parent=p) == _lib.ERR_UNSUPPORTED and "draft" in _lib.last_error()
