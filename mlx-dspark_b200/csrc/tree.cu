@@ -58,33 +58,49 @@ __global__ void __launch_bounds__(256) pack_kernel(const int32_t* cu, const int3
   }
 }
 
-// Simple form: one warp a (layer, K or V, request, head); each lane owns 16-byte columns and moves
-// the path's rows in ascending order. A row's source never lies before its destination and sources
-// ascend, so a destination is read by no later row and no row needs to wait for another column.
-__global__ void __launch_bounds__(32) keep_simple_kernel(
+// A lane owns a 16-byte column of one head's rows in one cache and moves the path's rows in ascending
+// order, KEEP_U at a time. A row's source never lies before its destination and sources ascend, so a
+// destination is read by no later row, and no column depends on another. Grid: x columns of all
+// heads, y requests, z caches (K and V of every layer). Bound: latency, or HBM with a large batch; only
+// rows that move are touched.
+constexpr int KEEP_U = 8;
+__global__ void __launch_bounds__(128) keep_kernel(
     void* const* k_layers, void* const* v_layers, int64_t k_b, int64_t k_h, int64_t k_t, int64_t v_b,
     int64_t v_h, int64_t v_t, const int32_t* path, const int32_t* cu, const int32_t* n_accept,
-    const int32_t* lens, const int32_t* kv_start, int row_bytes, int cap, int kv_batch, int* status) {
+    const int32_t* lens, const int32_t* kv_start, int chunks, int H, int cap, int kv_batch, int* status) {
   pdl_launch_dependents();
   pdl_wait();
-  const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z >> 1;
+  const int col = blockIdx.x * 128 + threadIdx.x, b = blockIdx.y, layer = blockIdx.z >> 1;
   const bool is_v = blockIdx.z & 1;
-  const int rows = cu[b + 1] - cu[b];
-  const int n = min(n_accept[b], rows - 1);
-  const int base = lens[b] - n_accept[b] - 1 + (kv_start ? kv_start[b] : 0);
-  const int64_t bs = is_v ? v_b : k_b, hs = is_v ? v_h : k_h, ts = is_v ? v_t : k_t;
-  uint8_t* p = static_cast<uint8_t*>(is_v ? v_layers[layer] : k_layers[layer]) +
-               (kv_batch == 1 ? 0 : b) * bs + h * hs;
-  for (int i = 0; i <= n; ++i) {
-    const int src = path[cu[b] + i];
-    if (src == i) continue;
-    if (src < i || src >= rows || base < 0 || base + src >= cap) {
-      if (threadIdx.x == 0) report_error(status, 0x204);
+  const int r0 = cu[b], rows = cu[b + 1] - r0, na = n_accept[b];
+  const int start = kv_start ? kv_start[b] : 0, base = lens[b] - na - 1 + start;
+  const int n = min(na, rows - 1);
+  uint8_t* p = static_cast<uint8_t*>(is_v ? v_layers[layer] : k_layers[layer]);
+  if (col >= H * chunks) return;
+  const int h = col / chunks, c = col - h * chunks;
+  const int64_t ts = is_v ? v_t : k_t;
+  p += (kv_batch == 1 ? 0 : b) * (is_v ? v_b : k_b) + h * (is_v ? v_h : k_h) + int64_t(base) * ts + c * 16;
+  for (int i0 = 0; i0 <= n; i0 += KEEP_U) {
+    int src[KEEP_U];
+    bool stop = false;
+#pragma unroll
+    for (int u = 0; u < KEEP_U; ++u) src[u] = i0 + u <= n ? path[r0 + i0 + u] : i0 + u;
+    uint4 v[KEEP_U];
+#pragma unroll
+    for (int u = 0; u < KEEP_U; ++u) {
+      if (src[u] != i0 + u) {
+        stop |= src[u] < i0 + u || src[u] >= rows || base < 0 || base + src[u] >= cap;
+        if (!stop) v[u] = *reinterpret_cast<const uint4*>(p + int64_t(src[u]) * ts);
+        else src[u] = i0 + u;  // outside the cache or out of order: nothing from here on
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < KEEP_U; ++u)
+      if (src[u] != i0 + u) *reinterpret_cast<uint4*>(p + int64_t(i0 + u) * ts) = v[u];
+    if (stop) {
+      report_error(status, 0x204);
       return;
     }
-    for (int d = threadIdx.x * 16; d < row_bytes; d += 512)
-      *reinterpret_cast<uint4*>(p + int64_t(base + i) * ts + d) =
-          *reinterpret_cast<const uint4*>(p + int64_t(base + src) * ts + d);
   }
 }
 
@@ -131,11 +147,12 @@ int dspark_kv_keep_path(void* const* k_layers, void* const* v_layers, int n_laye
   if (B > 65535 || n_layers > 32767)
     return fail(DSPARK_ERR_UNSUPPORTED, "kv_keep_path: %d requests, %d layers", B, n_layers);
   const int64_t e = elem_size;
-  DSPARK_CUDA_TRY(launch_ex(tree::keep_simple_kernel, dim3(H, B, 2 * n_layers), dim3(32), 0,
+  const int chunks = int(row_bytes / 16);
+  DSPARK_CUDA_TRY(launch_ex(tree::keep_kernel, dim3((H * chunks + 127) / 128, B, 2 * n_layers), dim3(128), 0,
                             reinterpret_cast<cudaStream_t>(stream), 1, true, k_layers, v_layers,
                             k_strides[0] * e, k_strides[1] * e, k_strides[2] * e, v_strides[0] * e,
                             v_strides[1] * e, v_strides[2] * e, path, cu_rows, n_accept, lens,
-                            kv_start, int(row_bytes), cap, kv_batch, status_word(current_device())),
+                            kv_start, chunks, H, cap, kv_batch, status_word(current_device())),
                   "kv_keep_path");
   return DSPARK_OK;
 }
