@@ -5,11 +5,11 @@
 // running maximum m_i and sum (fp32). The G = Hq / Hk query heads of a kv head share its keys, so
 // the rows of one product are (node, head of the group): node * G + g.
 //
-// Units and segments. A unit is 128 keys of one item: an item is up to 256 rows of one (request, kv
-// head). All units of the call are numbered (request, head, rows, keys) and cut into contiguous
-// ranges, one a CTA (one CTA per SM), from the lengths on the device: requests of any mix of lengths
-// load the SMs evenly without the host knowing them (locate). A CTA walks its range as segments (a run
-// of keys of one item). A segment that covers its item writes the output; else it leaves an
+// Items and segments. An item is up to 256 rows of one (request, kv head), its work a run of tiles of 128
+// keys. The work of the call, in order (request, head, rows, keys), is cut into contiguous shares, one
+// a CTA (one CTA per SM), from the lengths on the device: requests of any mix of lengths load the SMs
+// evenly without the host knowing them (locate). A CTA walks its share as segments (a run of tiles of
+// one item). A segment that covers its item writes the output; else it leaves an
 // fp32 part (O and the logarithm of its sum) in the workspace, at most two a CTA; when all parts of an item
 // are there, each of its CTAs joins a share of the rows, the parts in order (so results do not depend
 // on timing). They wait for one another, so the launch is cooperative: all CTAs run at once.
@@ -54,8 +54,8 @@ struct Lay {
   static constexpr int RING = 2 * TILE;
   static constexpr int M1 = RING + NB * TILE;     // slot 1's (m, l) at the segment's end
   static constexpr int FLAG = M1 + ROWS * 8;
-  static constexpr int SEG = FLAG + 16;             // [slot] the softmax threads' segment and walker
-  static constexpr int CUTS = SEG + 2 * 96;         // the CTA's parts of cut items
+  static constexpr int SEGS = FLAG + 16;            // [slot] the softmax threads' segment and walker
+  static constexpr int CUTS = SEGS + 2 * 112;        // the CTA's parts of cut items
   static constexpr int BARS = CUTS + 2 * 32 + 16;
   static constexpr int NBAR = 2 * NB + 2 + 2 + 2 + 2 + 2 + 1;
   static constexpr int TOTAL = BARS + NBAR * 8;
@@ -165,21 +165,41 @@ __device__ __forceinline__ int start_of(const dspark_tree_attn_args& a, int b) {
   return a.kv_start ? min(max(a.kv_start[b], 0), a.cap) : 0;
 }
 
-// Row blocks and key tiles of request b (a request of rows but no keys has one tile, all hidden).
-__device__ __forceinline__ void extents(const dspark_tree_attn_args& a, int b, int& M, int& T) {
+// Row blocks and key tiles of request b (a request of rows but no keys has one tile, all hidden), and
+// what a tile of the last row block costs.
+struct Shape {
+  int M, T, wl;
+};
+
+// Costs in half microseconds, as measured: a tile of one row block streams from HBM (64 KB in 1.5 us
+// with all SMs at it), one of two row blocks is held by its products and exponentials (2 us), and a
+// segment has its Q, its pipeline's fill and its O (6 us). 64 requests of 256 to 16k keys, dealt out
+// by tiles alone: 114 to 372 us a CTA.
+constexpr int ONE = 3, PAIR = 4, SEG = 12;
+
+__device__ __forceinline__ Shape shape_of(const dspark_tree_attn_args& a, int b) {
   int r0;
-  const int n = rows_of(a, b, r0);
-  M = (n * (a.Hq / a.Hk) + 2 * ROWS - 1) / (2 * ROWS);
-  T = max(1, (min(a.kv_len[b], a.cap - start_of(a, b)) + BN - 1) / BN);
+  const int rows = rows_of(a, b, r0) * (a.Hq / a.Hk);
+  Shape s;
+  s.M = (rows + 2 * ROWS - 1) / (2 * ROWS);
+  s.T = max(1, (min(a.kv_len[b], a.cap - start_of(a, b)) + BN - 1) / BN);
+  s.wl = rows - (s.M - 1) * 2 * ROWS > ROWS ? PAIR : ONE;
+  return s;
 }
 
-// A CTA's range of units. Either all units are dealt out equally (the first total % n CTAs have one
-// more) and a range may cross from item to item, or each item has CTAs of its own.
+// Cost of all row blocks of one head.
+__device__ __forceinline__ int cost_of(const Shape& s) {
+  return s.M ? (s.M - 1) * (SEG + PAIR * s.T) + SEG + s.wl * s.T : 0;
+}
+
+// A CTA's work: either an equal share [x, end) of the summed cost of all items, which may cross from
+// item to item, or (parts > 0) tiles [t0, t1) of one item that has CTAs of its own.
 struct Range {
-  int u, end;        // units [u, end)
-  int b, base;       // request of unit u, the request's first unit
-  int first, parts;  // an item's own CTAs: the first one, how many; parts 0: dealt out equally
-  int total, n;      // units of the call, CTAs that have any
+  int x, end;         // in costs
+  int b, base;        // request of x (or of the item), the request's first cost
+  int im, t0, t1;     // own: item of the request, its tiles
+  int first, parts;   // own: the item's first CTA, how many
+  int total, n;       // summed cost, CTAs that share it
   __device__ __forceinline__ int dealt(int c) const {
     const int q = n ? total / n : 0;
     return c < n ? c * q + min(c, total - q * n) : total;
@@ -187,14 +207,14 @@ struct Range {
 };
 
 // CTAs of one item among n when items have their own: one each, and the others by the tiles.
-__device__ __forceinline__ int ctas_of(int T, int n, int items, int total) {
-  return min(T, 1 + int(int64_t(T) * (n - items) / total));
+__device__ __forceinline__ int ctas_of(int T, int n, int items, int tiles) {
+  return min(T, 1 + int(int64_t(T) * (n - items) / tiles));
 }
 
 // Every warp for itself, no barrier. Items get their own CTAs unless the longest range then has OWN
-// tiles more than an equal deal: what a second segment costs (its Q, its parts, the refilled
-// pipeline) is about that many tiles: 61 rows over 16k keys, 8 items: 40 us for the CTAs with two
-// segments of together 7 tiles, 24 us for those with one.
+// tiles more than an equal deal: what a second segment costs is about that many tiles: 61 rows over
+// 16k keys, 8 items: 40 us for the CTAs with two segments of together 7 tiles, 24 us for those with
+// one.
 constexpr int OWN = 8;
 __device__ Range locate(const dspark_tree_attn_args& a, int cta, int n_cta) {
   const int lane = threadIdx.x & 31;
@@ -206,70 +226,60 @@ __device__ Range locate(const dspark_tree_attn_args& a, int cta, int n_cta) {
     }
     return v;
   };
-  int M0 = 0, T0 = 1;  // the lane's own request of the first 32
-  if (lane < a.B) extents(a, lane, M0, T0);
-  auto shape = [&](int b, int& M, int& T) {
-    M = 0;
-    T = 1;
-    if (b < 32) {
-      M = M0;
-      T = T0;
-    } else if (b < a.B) {
-      extents(a, b, M, T);
-    }
-  };
-  int items = 0, total = 0;
+  Shape mine{0, 1, ONE};  // the lane's own request of the first 32
+  if (lane < a.B) mine = shape_of(a, lane);
+  auto shape = [&](int b) { return b < 32 ? mine : b < a.B ? shape_of(a, b) : Shape{0, 1, ONE}; };
+  int items = 0, tiles = 0, total = 0;
   for (int b0 = 0; b0 < a.B; b0 += 32) {
-    int M, T;
-    shape(b0 + lane, M, T);
-    items += M * a.Hk;
-    total += M * T * a.Hk;
+    const Shape s = shape(b0 + lane);
+    items += s.M * a.Hk;
+    tiles += s.M * s.T * a.Hk;
+    total += cost_of(s) * a.Hk;
   }
   items = __reduce_add_sync(0xffffffffu, items);
+  tiles = __reduce_add_sync(0xffffffffu, tiles);
   total = __reduce_add_sync(0xffffffffu, total);
-  Range r{0, 0, a.B, 0, 0, 0, total, min(n_cta, total)};
-  if (total == 0) return r;
+  // shares are wider than any tile's cost, so that an item's parts lie in neighbouring CTAs
+  Range r{0, 0, a.B, 0, 0, 0, 0, 0, 0, total, min(n_cta, max(1, total / (2 * PAIR)))};
+  if (tiles == 0) return r;
   bool own = items <= n_cta;
   if (own) {
     int longest = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
-      int M, T;
-      shape(b0 + lane, M, T);
-      const int c = ctas_of(T, n_cta, items, total);
-      if (M) longest = max(longest, (T + c - 1) / c);
+      const Shape s = shape(b0 + lane);
+      const int c = ctas_of(s.T, n_cta, items, tiles);
+      if (s.M) longest = max(longest, (s.T + c - 1) / c);
     }
     longest = __reduce_max_sync(0xffffffffu, longest);
-    own = longest <= (total + n_cta - 1) / n_cta + OWN;
+    own = longest <= (tiles + n_cta - 1) / n_cta + OWN;
   }
-  const int want = own ? cta : r.dealt(cta);  // in CTAs or in units
+  const int want = own ? cta : r.dealt(cta);  // in CTAs or in costs
   if (!own && want >= total) return r;
-  int at = 0, units = 0;
+  int at = 0;
   for (int b0 = 0; b0 < a.B; b0 += 32) {
-    int M, T;
-    shape(b0 + lane, M, T);
-    const int c = own ? ctas_of(T, n_cta, items, total) : T;
-    const int v = M * a.Hk * c, x = scan(v), n = M * T * a.Hk, y = scan(n);
+    const Shape s = shape(b0 + lane);
+    const int c = ctas_of(s.T, n_cta, items, tiles);
+    const int v = own ? s.M * a.Hk * c : cost_of(s) * a.Hk, x = scan(v);
     const unsigned hit = __ballot_sync(0xffffffffu, v > 0 && want < at + x && want >= at + x - v);
     if (hit) {
       const int k = __ffs(hit) - 1;
       r.b = b0 + k;
-      r.base = units + __shfl_sync(0xffffffffu, y - n, k);
+      r.base = at + __shfl_sync(0xffffffffu, x - v, k);
       if (own) {
-        const int ck = __shfl_sync(0xffffffffu, c, k), Tk = __shfl_sync(0xffffffffu, T, k);
-        const int local = want - (at + __shfl_sync(0xffffffffu, x - v, k));
-        const int im = local / ck, s = local - im * ck;
-        r.u = r.base + im * Tk + Tk * s / ck;
-        r.end = r.base + im * Tk + Tk * (s + 1) / ck;
-        r.first = cta - s;
+        const int ck = __shfl_sync(0xffffffffu, c, k), Tk = __shfl_sync(0xffffffffu, s.T, k);
+        const int local = want - r.base, im = local / ck, part = local - im * ck;
+        r.im = im;
+        r.t0 = Tk * part / ck;
+        r.t1 = Tk * (part + 1) / ck;
+        r.first = cta - part;
         r.parts = ck;
       } else {
-        r.u = want;
+        r.x = want;
         r.end = r.dealt(cta + 1);
       }
       return r;
     }
     at += __shfl_sync(0xffffffffu, x, 31);
-    units += __shfl_sync(0xffffffffu, y, 31);
   }
   return r;
 }
@@ -285,26 +295,26 @@ struct Segment {
 };
 
 struct Walker {
-  int u, end, base;  // next unit, end of the range, first unit of request b
-  int b;
-  __device__ __forceinline__ bool next(const dspark_tree_attn_args& a, Segment& s) {
-    if (u >= end) return false;
-    int M, T;
-    extents(a, b, M, T);
-    int n = M * T * a.Hk;
-    while (u >= base + n) {
-      base += n;
-      extents(a, ++b, M, T);
-      n = M * T * a.Hk;
-    }
+  int x, end, base, b;        // next cost, end of the share, first cost of request b
+  int start, w;               // of the item last given: its first cost, a tile's cost
+  int im, t0, t1;             // own: the one segment (t1 0: given)
+  __device__ __forceinline__ Walker(const Range& r)
+      : x(r.x), end(r.end), base(r.base), b(r.b), start(0), w(ONE), im(r.im), t0(r.t0), t1(r.t1) {}
+
+  // First tile of the item at or after a cost.
+  static __device__ __forceinline__ int tile_at(int y, int start, int w, int T) {
+    const int d = y - start - SEG;
+    return d <= 0 ? 0 : min(T, (d + w - 1) / w);
+  }
+  __device__ __forceinline__ void fill(const dspark_tree_attn_args& a, Segment& s, const Shape& sh, int im_,
+                                       int t0_, int t1_) {
     const int G = a.Hq / a.Hk;
-    const int local = u - base, im = local / T;
     s.b = b;
-    s.T = T;
-    s.t0 = local - im * T;
-    s.t1 = min(T, s.t0 + (end - u));
-    s.h = im / M;
-    s.row_base = (im - s.h * M) * 2 * ROWS;
+    s.T = sh.T;
+    s.t0 = t0_;
+    s.t1 = t1_;
+    s.h = im_ / sh.M;
+    s.row_base = (im_ - s.h * sh.M) * 2 * ROWS;
     s.rows = rows_of(a, b, s.r0);
     s.live = min(s.rows * G - s.row_base, 2 * ROWS);
     s.pair = s.live > ROWS;
@@ -312,8 +322,34 @@ struct Walker {
     s.len = max(0, min(a.kv_len[b], a.cap - s.start));
     s.first = a.kv_len[b] - s.rows;
     s.kb = a.kv_batch == 1 ? 0 : b;
-    u += s.t1 - s.t0;
-    return true;
+  }
+  __device__ __forceinline__ bool next(const dspark_tree_attn_args& a, Segment& s) {
+    if (t1 > 0) {
+      fill(a, s, shape_of(a, b), im, t0, t1);
+      t1 = 0;
+      return true;
+    }
+    while (x < end) {
+      const Shape sh = shape_of(a, b);
+      const int head = cost_of(sh);
+      if (x >= base + head * a.Hk) {
+        base += head * a.Hk;
+        ++b;
+        continue;
+      }
+      const int local = x - base, h = local / head, rem = local - h * head;
+      const int full = SEG + PAIR * sh.T, m = min(rem / full, sh.M - 1);
+      start = base + h * head + m * full;
+      w = m + 1 < sh.M ? PAIR : sh.wl;
+      const int stop = start + SEG + w * sh.T;
+      const int u0 = tile_at(x, start, w, sh.T), u1 = end >= stop ? sh.T : tile_at(end, start, w, sh.T);
+      x = stop;
+      if (u0 < u1) {
+        fill(a, s, sh, h * sh.M + m, u0, u1);
+        return true;
+      }
+    }
+    return false;
   }
 };
 
@@ -323,8 +359,8 @@ struct Shared {
   Segment s;
   int more;
   Walker w;
-};
-static_assert(sizeof(Shared) <= 96, "Lay::SEG");
+};  // (constructed by assignment)
+static_assert(sizeof(Shared) <= 112, "Lay::SEGS");
 
 // Ring use (within the segment) of the V tile of local tile t: the order of loads is K0 V0 K1 V1 ..
 // (pair) or K0 K1 V0 K2 V1 .. (tiles alternate between the slots).
@@ -622,7 +658,7 @@ __global__ void __launch_bounds__(NTHR, 1)
   __syncthreads();
   tcg::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Walker wk{range.u, range.end, range.base, range.b};
+  Walker wk(range);
   bool ok = true;
 
   if (warp < WARP_TMA) {
@@ -632,7 +668,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     const int slot = warp >> 2, row = tid & 127;
     const uint32_t t_s = tmem + (uint32_t((warp & 3) * 32) << 16) + uint32_t(slot * 128);
     const uint32_t t_o = t_s + O_COL;
-    Shared& sh = *reinterpret_cast<Shared*>(smem + L::SEG + 96 * slot);
+    Shared& sh = *reinterpret_cast<Shared*>(smem + L::SEGS + 112 * slot);
     const Segment& s = sh.s;
     if (row == 0) {
       sh.more = wk.next(a, sh.s);
@@ -894,10 +930,10 @@ __global__ void __launch_bounds__(NTHR, 1)
         if (slot == 0 && !whole) {
           int c0 = range.first, n_parts = range.parts;
           if (n_parts == 0) {
-            const int begin = sh.w.u - s.t1, end = begin + s.T;  // the item's units
+            const int from = sh.w.start + SEG;  // cost of the item's first tile
             int c1 = cta + 1;
-            for (c0 = cta; c0 > 0 && range.dealt(c0) > begin; --c0) {}
-            while (range.dealt(c1) < end) ++c1;
+            for (c0 = cta; c0 > 0 && range.dealt(c0) > from; --c0) {}
+            while (c1 < range.n && range.dealt(c1) <= from + sh.w.w * (s.T - 1)) ++c1;
             n_parts = c1 - c0;
           }
           cuts[(*n_cuts)++] = Cut{c0, n_parts, s.r0, s.live, s.row_base, s.h, {0, 0}};
@@ -1098,9 +1134,9 @@ static int launch(const dspark_tree_attn_args& a, cudaStream_t s) {
                   (long long)str[0], (long long)str[1], (long long)str[2]);
   }
   const int n_cta = grid_of(dev);
-  // the units are counted in 32 bits
+  // costs are summed in 32 bits
   const int64_t G = a.Hq / a.Hk;
-  if ((int64_t(a.R) * G / (2 * ROWS) + a.B) * a.Hk * ((int64_t(a.cap) + BN - 1) / BN + 1) > 0x7fffffff)
+  if ((int64_t(a.R) * G / (2 * ROWS) + a.B) * a.Hk * (PAIR * ((int64_t(a.cap) + BN - 1) / BN + 1) + SEG) > 0x7fffffff)
     return fail(DSPARK_ERR_UNSUPPORTED, "tree_attn: %d rows over %d positions in one call", a.R, a.cap);
   const size_t smem = Lay<D>::TOTAL;
   DSPARK_CUDA_TRY(configure_once((const void*)attn_kernel<T, D>, int(smem),
