@@ -18,10 +18,12 @@
 // overwritten by the 16-bit weights P) and an output accumulator O (TMEM).
 //  * items of more than 128 rows: the slots are the two halves of the rows and share each K/V tile;
 //  * items of up to 128 rows: the slots take the even and the odd key tiles of the segment and
-//    are joined through shared memory at its end.
+//    are joined at its end (each warpgroup reads half of both slots' O: their rows have the same
+//    lanes).
 // Either way one slot's softmax runs under the other slot's products. One producer thread streams
-// K and V tiles by TMA through a ring (the order the products use them), one thread issues the
-// products: S = Q K^T (both from shared memory, K-major), O += P V (P from tensor memory, V from
+// K and V tiles by TMA through a ring (the order the products use them); two preparing warps walk ahead
+// and load the next segment's Q as soon as the last scores have read the old one, under the end of the
+// softmax and the output of the old segment; one thread issues the products: S = Q K^T (both from shared memory, K-major), O += P V (P from tensor memory, V from
 // shared memory as it lies, keys along K, so N-major). A thread of a softmax warpgroup owns a row:
 // no shuffles. The maximum in use is only raised when a tile exceeds it by more than 2^8: the
 // weights then stay within fp16 / fp32 range and O is rarely rescaled.
@@ -42,8 +44,8 @@ namespace tattn {
 
 constexpr int BN = 128;       // keys a tile
 constexpr int ROWS = 128;     // rows a slot
-constexpr int NTHR = 384;     // two softmax warpgroups; producer, MMA and two idle warps
-constexpr int WARP_TMA = 8, WARP_MMA = 9;
+constexpr int NTHR = 384;     // two softmax warpgroups; producer, MMA and two preparing warps
+constexpr int WARP_TMA = 8, WARP_MMA = 9, WARP_PREP = 10;
 
 template <int D>
 struct Lay {
@@ -52,12 +54,12 @@ struct Lay {
   static constexpr int NB = D == 128 ? 5 : 10;    // ring buffers
   static constexpr int Q = 0;
   static constexpr int RING = 2 * TILE;
-  static constexpr int M1 = RING + NB * TILE;     // slot 1's (m, l) at the segment's end
-  static constexpr int FLAG = M1 + ROWS * 8;
-  static constexpr int SEGS = FLAG + 16;            // [slot] the softmax threads' segment and walker
-  static constexpr int CUTS = SEGS + 2 * 112;        // the CTA's parts of cut items
+  static constexpr int ML = RING + NB * TILE;     // [slot][row] (m, l) at the segment's end
+  static constexpr int FLAG = ML + 2 * ROWS * 8;
+  static constexpr int SEGS = FLAG + 16;            // two segments for the softmax threads
+  static constexpr int CUTS = SEGS + 2 * 64;        // the CTA's parts of cut items
   static constexpr int BARS = CUTS + 2 * 32 + 16;
-  static constexpr int NBAR = 2 * NB + 2 + 2 + 2 + 2 + 2 + 1;
+  static constexpr int NBAR = 2 * NB + 2 * 8 + 1;
   static constexpr int TOTAL = BARS + NBAR * 8;
   static_assert(TOTAL <= 232448, "shared memory of one SM");
 };
@@ -152,6 +154,18 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t lo) {
 
 __device__ __forceinline__ void named_sync(int id, int n) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
+}
+
+// named_sync that tells all its threads whether `ok` held in every one of them.
+__device__ __forceinline__ bool named_all(int id, int n, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(uint32_t(ok)), "r"(id), "r"(n)
+      : "memory");
+  return r != 0;
 }
 
 // ------------------------------------------------------------------ units, ranges, segments
@@ -353,14 +367,12 @@ struct Walker {
   }
 };
 
-// What the softmax threads of a slot share: the segment at hand and where the next one starts. It
-// lives in shared memory because their registers hold scores.
-struct Shared {
+// A segment as the preparing warps hand it to the softmax threads.
+struct Handed {
   Segment s;
   int more;
-  Walker w;
-};  // (constructed by assignment)
-static_assert(sizeof(Shared) <= 112, "Lay::SEGS");
+};
+static_assert(sizeof(Handed) <= 64, "Lay::SEGS");
 
 // Ring use (within the segment) of the V tile of local tile t: the order of loads is K0 V0 K1 V1 ..
 // (pair) or K0 K1 V0 K2 V1 .. (tiles alternate between the slots).
@@ -456,14 +468,14 @@ struct Hidden {
   const T* v;             // the request's first value row of this kv head
   int64_t stride;
   const uint32_t* anc;    // the row's words, or null
-  int words, place, k0, k1, first, D;
+  int words, place, k0, k1, first, d0, d1;
 };
 
 template <typename T>
 __device__ __noinline__ void add_hidden(const Hidden<T> x, T* out, float* part) {
   for (int k = x.k0; k < x.k1; ++k) {
     if (!sees(x.anc, x.words, x.place, k - x.first)) continue;
-    for (int d = 0; d < x.D; ++d) {
+    for (int d = x.d0; d < x.d1; ++d) {
       const float v = Elem<T>::to_f(x.v[int64_t(k) * x.stride + d]);
       if (isfinite(v)) continue;
       if (part) part[d * 2 * ROWS] += v;
@@ -532,7 +544,7 @@ __device__ __noinline__ void join_parts(const dspark_tree_attn_args& a, const Cu
     for (int k = 0; k < n_cuts; ++k) count_up(&count[cuts[k].first], tag, 2 * cuts[k].parts);
   }
   constexpr int64_t STRIDE = int64_t(2) * (2 * ROWS) * (D + 1);  // floats between the CTAs' parts
-  static_assert(MAX_CTA * 2 * ROWS * 4 <= Lay<D>::M1, "the weights' room");
+  static_assert(MAX_CTA * 2 * ROWS * 4 <= Lay<D>::ML, "the weights' room");
   float* w = reinterpret_cast<float*>(smem);  // [parts][256]
   for (int k = 0; k < n_cuts; ++k) {
     const Cut c = cuts[k];
@@ -602,12 +614,12 @@ __device__ __noinline__ void join_parts(const dspark_tree_attn_args& a, const Cu
 template <typename T, int D>
 __global__ void __launch_bounds__(NTHR, 1)
     attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                const dspark_tree_attn_args a, const float c_log2, const float q_sign,
+                const dspark_tree_attn_args a, const float c_log2, const uint32_t q_neg,
                 const uint64_t tag, int* status) {
   typedef Lay<D> L;
   constexpr int NB = L::NB;
   constexpr uint32_t FMT = std::is_same<T, bf16>::value ? 1u : 0u;
-  constexpr uint32_t ID_QK = (1u << 4) | (FMT << 7) | (FMT << 10) | (uint32_t(BN >> 3) << 17) |
+  const uint32_t ID_QK = q_neg | (1u << 4) | (FMT << 7) | (FMT << 10) | (uint32_t(BN >> 3) << 17) |
                              (uint32_t(ROWS >> 4) << 24);
   constexpr uint32_t ID_PV = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) |
                              (uint32_t(D >> 3) << 17) | (uint32_t(ROWS >> 4) << 24);
@@ -621,8 +633,13 @@ __global__ void __launch_bounds__(NTHR, 1)
   uint64_t* p_full = s_full + 2;
   uint64_t* p_part = p_full + 2;
   uint64_t* o_full = p_part + 2;
-  uint64_t* fin = o_full + 2;
-  float2* ml1 = reinterpret_cast<float2*>(smem + L::M1);
+  uint64_t* q_empty = o_full + 2;
+  uint64_t* seg_full = q_empty + 2;
+  uint64_t* seg_empty = seg_full + 2;
+  uint64_t* fin = seg_empty + 2;
+  float2* ml = reinterpret_cast<float2*>(smem + L::ML);
+  Cut* cuts = reinterpret_cast<Cut*>(smem + L::CUTS);
+  int* n_cuts = reinterpret_cast<int*>(cuts + 2);
   int* flag = reinterpret_cast<int*>(smem + L::FLAG);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(flag + 2);
 
@@ -636,8 +653,11 @@ __global__ void __launch_bounds__(NTHR, 1)
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {  // the softmax barriers count warps
-      mbar_init(&q_full[i], 4);
+    for (int i = 0; i < 2; ++i) {  // p_*, q_full and seg_empty count warps
+      mbar_init(&q_full[i], 2);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&seg_full[i], 1);
+      mbar_init(&seg_empty[i], 8);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_part[i], 4);
       mbar_init(&p_full[i], 4);
@@ -645,6 +665,7 @@ __global__ void __launch_bounds__(NTHR, 1)
       flag[i] = 0;
     }
     mbar_init(fin, 1);
+    *n_cuts = 0;
     fence_mbar_init();
     prefetch_tmap(&kmap);
     prefetch_tmap(&vmap);
@@ -668,18 +689,9 @@ __global__ void __launch_bounds__(NTHR, 1)
     const int slot = warp >> 2, row = tid & 127;
     const uint32_t t_s = tmem + (uint32_t((warp & 3) * 32) << 16) + uint32_t(slot * 128);
     const uint32_t t_o = t_s + O_COL;
-    Shared& sh = *reinterpret_cast<Shared*>(smem + L::SEGS + 112 * slot);
-    const Segment& s = sh.s;
-    if (row == 0) {
-      sh.more = wk.next(a, sh.s);
-      sh.w = wk;
-    }
-    named_sync(1 + slot, 128);
-    Cut* cuts = reinterpret_cast<Cut*>(smem + L::CUTS);
-    int* n_cuts = reinterpret_cast<int*>(cuts + 2);
-    if (tid == 0) *n_cuts = 0;
-    uint32_t n_s = 0, n_o = 0;  // completed phases of s_full / o_full
-    int use0 = 0;               // ring uses before this segment
+    uint32_t n_s = 0;              // completed phases of s_full
+    uint32_t n_o0 = 0, n_o1 = 0;   // of o_full
+    int use0 = 0;                  // ring uses before this segment
     auto arrive = [&](uint64_t* bar) {  // this warp's stores to tensor memory are done
       tcg::tmem_wait_st();
       tcg::tc_fence_before();
@@ -688,61 +700,22 @@ __global__ void __launch_bounds__(NTHR, 1)
     };
     // flag[seg & 1] == seg: a hidden non-finite value in segment `seg`. One slot may be a segment
     // ahead of the other, never two: the products of a segment need both slots' weights.
-    for (int seg = 1; sh.more; ++seg) {
+    for (int seg = 1;; ++seg) {
+      const int hand = (seg - 1) & 1;
+      const Handed& sh = *reinterpret_cast<const Handed*>(smem + L::SEGS + 64 * hand);
+      if (ok) ok = mbar_wait(&seg_full[hand], uint32_t((seg - 1) >> 1) & 1u, status, kErrWaitPeer);
+      // after a wait that ran out all leave together: the barriers below count all of them
+      ok = named_all(3, 256, ok);
+      if (!ok || !sh.more) break;
+      const Segment& s = sh.s;
       const int n = s.t1 - s.t0;
       const bool pair = s.pair;
       const int steps = pair ? n : (n - slot + 1) >> 1;
       const int tile0 = pair ? s.t0 : s.t0 + slot, tstep = pair ? 1 : 2;
       const int edge0 = min(s.first, s.len) - BN;  // a tile from a later key on has hidden keys
-      bool warp_alive;
-      {
-        const int G = a.Hq / a.Hk;
-        warp_alive = s.row_base + (pair ? slot * ROWS : 0) + (warp & 3) * 32 < s.rows * G;
-      }
+      const int G = a.Hq / a.Hk;
+      const bool warp_alive = s.row_base + (pair ? slot * ROWS : 0) + (warp & 3) * 32 < s.rows * G;
       float m = -INFINITY, l = 0.f;
-      if (steps > 0) {
-        // this slot's Q tile; the last scores that read the old one have arrived
-        constexpr int CH = D / 8;            // 16-byte chunks a row
-        constexpr int STEP = ROWS / CH;      // rows the warpgroup loads at a time
-        const int c = row % CH, first_row = row / CH;
-        const int G = a.Hq / a.Hk, row0 = s.row_base + (pair ? slot * ROWS : 0);
-        const int live = min(ROWS, s.rows * G - row0);  // rows past it are never looked at
-        uint8_t* qs = smem + L::Q + slot * L::TILE;
-        const T* q = static_cast<const T*>(a.q) + int64_t(s.r0) * a.q_strides[0] +
-                     s.h * G * a.q_strides[1] + c * 8;
-        const int dn = STEP / G, dg = STEP - dn * G;  // a step in (node, head of the group)
-        int node = (row0 + first_row) / G, g = row0 + first_row - node * G;
-        uint4 v[CH];
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          v[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (first_row + i * STEP < live)
-            v[i] = ldcg_v4(q + node * a.q_strides[0] + g * a.q_strides[1]);
-          node += dn;
-          g += dg;
-          if (g >= G) {
-            g -= G;
-            ++node;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          const int rr = first_row + i * STEP;
-          if (q_sign != 1.f) {
-            uint32_t* w = &v[i].x;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 f = Elem<T>::unpack(w[e]);
-              w[e] = Elem<T>::pack(f.x * q_sign, f.y * q_sign);
-            }
-          }
-          if (rr < live)
-            *reinterpret_cast<uint4*>(qs + (c >> 3) * L::HALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full[slot]);
-      }
       for (int j = 0; j < steps; ++j) {
         const int k0 = (tile0 + j * tstep) * BN;
         const bool edge = k0 > edge0;
@@ -835,120 +808,165 @@ __global__ void __launch_bounds__(NTHR, 1)
         arrive(&p_full[slot]);
       }
       use0 += 2 * n;
-      // ---- end of the segment
-      if (steps > 0) {
-        if (ok) ok = mbar_wait(&o_full[slot], n_o & 1, status, kErrWaitMma);
-        ++n_o;
-        tcg::tc_fence_after();
-      }
+      // ---- end of the segment: with one row block, both slots' O of half of the values
+      if (ok && steps > 0) ok = mbar_wait(&o_full[slot], (slot ? n_o1 : n_o0) & 1, status, kErrWaitMma);
+      const bool both = !pair && n > 1;
+      if (ok && both) ok = mbar_wait(&o_full[slot ^ 1], (slot ? n_o0 : n_o1) & 1, status, kErrWaitMma);
+      if (!pair && slot == 1 && n == 1 && ok) ok = mbar_wait(&o_full[0], n_o0 & 1, status, kErrWaitMma);
+      ++n_o0;
+      n_o1 += pair || n > 1;
+      tcg::tc_fence_after();
       const bool whole = s.t0 == 0 && s.t1 == s.T;
-      const int G = a.Hq / a.Hk;
       const int my = s.row_base + (pair ? slot * ROWS : 0) + row;  // (node, head) row of this thread
       const bool alive = my < s.rows * G;
       const int place = alive ? my / G : 0;
-      float* xch = reinterpret_cast<float*>(smem + L::Q) + row;  // [D][128] fp32: both Q tiles
-      if (!pair) named_sync(3, 256);  // both slots are done with their Q tiles
-      if (!pair && slot == 1) {
-        ml1[row] = make_float2(m, l);
-        if (steps > 0 && warp_alive) {
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            float o[32];
-            ld_x32(t_o + uint32_t(32 * i), o);
-            tcg::tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) xch[(32 * i + e) * ROWS] = o[e];
-          }
-        }
+      float f0 = 1.f, f1 = 0.f;
+      if (!pair) {
+        ml[slot * ROWS + row] = make_float2(m, l);
         named_sync(3, 256);
-      } else {
-        float f0 = 1.f, f1 = 0.f;
-        bool both = false;
-        if (!pair) {
-          named_sync(3, 256);
-          if (n > 1) {
-            const float2 st = ml1[row];
-            const float mn = fmaxf(m, st.x), ref = mn == -INFINITY ? 0.f : mn;
-            f0 = ex2((m - ref) * c_log2);
-            f1 = ex2((st.x - ref) * c_log2);
-            l = l * f0 + st.y * f1;
-            m = mn;
-            both = true;
-          }
-        }
-        const bool hidden = *reinterpret_cast<volatile int*>(&flag[seg & 1]) == seg;
-        if (warp_alive) {
-          const int hq = s.h * G + my - place * G;
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          float* pp = whole ? nullptr : part<D>(a.workspace, cta, s.t0 == 0 ? 1 : 0);
-          const int prow = (pair ? slot * ROWS : 0) + row;
-          T* out = static_cast<T*>(a.out) + int64_t(s.r0 + place) * a.o_strides[0] + hq * a.o_strides[1];
-          if (!whole) pp[2 * ROWS * D + prow] = m * c_log2 + lg2(l);
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            float o[32];
-            ld_x32(t_o + uint32_t(32 * i), o);
-            tcg::tmem_wait_ld();
-            if (both) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = o[e] * f0 + xch[(32 * i + e) * ROWS] * f1;
-            }
-            if (!whole) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) pp[(32 * i + e) * (2 * ROWS) + prow] = l == 0.f ? 0.f : o[e] * inv;
-            } else if (alive) {
-#pragma unroll
-              for (int e = 0; e < 32; e += 8) {
-                uint4 v;
-                v.x = Elem<T>::pack(o[e] * inv, o[e + 1] * inv);
-                v.y = Elem<T>::pack(o[e + 2] * inv, o[e + 3] * inv);
-                v.z = Elem<T>::pack(o[e + 4] * inv, o[e + 5] * inv);
-                v.w = Elem<T>::pack(o[e + 6] * inv, o[e + 7] * inv);
-                *reinterpret_cast<uint4*>(out + 32 * i + e) = l == 0.f ? make_uint4(0u, 0u, 0u, 0u) : v;
-              }
-            }
-          }
-          if (hidden && alive) {
-            Hidden<T> hd;
-            hd.v = static_cast<const T*>(a.v) + s.kb * a.v_strides[0] + s.h * a.v_strides[1] +
-                   int64_t(s.start) * a.v_strides[2];
-            hd.stride = a.v_strides[2];
-            hd.anc = a.anc ? a.anc + int64_t(s.r0 + place) * a.anc_words : nullptr;
-            hd.words = a.anc_words;
-            hd.place = place;
-            hd.k0 = max(s.t0 * BN, max(s.first, 0));
-            hd.k1 = min(s.t1 * BN, s.len);
-            hd.first = s.first;
-            hd.D = D;
-            add_hidden<T>(hd, out, whole ? nullptr : pp + prow);
-          }
-        }
+        const float2 a0 = ml[row], a1 = ml[ROWS + row];
+        const float mn = fmaxf(a0.x, a1.x), ref = mn == -INFINITY ? 0.f : mn;
+        f0 = ex2((a0.x - ref) * c_log2);
+        f1 = ex2((a1.x - ref) * c_log2);
+        l = a0.y * f0 + a1.y * f1;
+        m = mn;
       }
-      // the exchange and the segment have been read: the next ones may land there
-      if (pair) named_sync(1 + slot, 128); else named_sync(3, 256);
-      if (row == 0) {
-        if (slot == 0 && !whole) {
-          int c0 = range.first, n_parts = range.parts;
-          if (n_parts == 0) {
-            const int from = sh.w.start + SEG;  // cost of the item's first tile
-            int c1 = cta + 1;
-            for (c0 = cta; c0 > 0 && range.dealt(c0) > from; --c0) {}
-            while (c1 < range.n && range.dealt(c1) <= from + sh.w.w * (s.T - 1)) ++c1;
-            n_parts = c1 - c0;
+      const bool hidden = *reinterpret_cast<volatile int*>(&flag[seg & 1]) == seg;
+      if (warp_alive) {
+        const int hq = s.h * G + my - place * G;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        float* pp = whole ? nullptr : part<D>(a.workspace, cta, s.t0 == 0 ? 1 : 0);
+        const int prow = (pair ? slot * ROWS : 0) + row;
+        // 32-value chunks: all of the slot's own, or every second one of both slots'
+        const int i0 = pair ? 0 : slot * (D / 64), i1 = pair ? D / 32 : i0 + D / 64;
+        const uint32_t t_0 = pair ? t_o : tmem + (uint32_t((warp & 3) * 32) << 16) + O_COL;
+        T* out = static_cast<T*>(a.out) + int64_t(s.r0 + place) * a.o_strides[0] + hq * a.o_strides[1];
+        if (!whole && (pair || slot == 0)) pp[2 * ROWS * D + prow] = m * c_log2 + lg2(l);
+#pragma unroll 1
+        for (int i = i0; i < i1; ++i) {
+          float o[32];
+          ld_x32(t_0 + uint32_t(32 * i), o);
+          tcg::tmem_wait_ld();
+          if (both) {
+            float o1[32];
+            ld_x32(t_0 + 128u + uint32_t(32 * i), o1);
+            tcg::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = o[e] * f0 + o1[e] * f1;
           }
-          cuts[(*n_cuts)++] = Cut{c0, n_parts, s.r0, s.live, s.row_base, s.h, {0, 0}};
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) pp[(32 * i + e) * (2 * ROWS) + prow] = l == 0.f ? 0.f : o[e] * inv;
+          } else if (alive) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint4 v;
+              v.x = Elem<T>::pack(o[e] * inv, o[e + 1] * inv);
+              v.y = Elem<T>::pack(o[e + 2] * inv, o[e + 3] * inv);
+              v.z = Elem<T>::pack(o[e + 4] * inv, o[e + 5] * inv);
+              v.w = Elem<T>::pack(o[e + 6] * inv, o[e + 7] * inv);
+              *reinterpret_cast<uint4*>(out + 32 * i + e) = l == 0.f ? make_uint4(0u, 0u, 0u, 0u) : v;
+            }
+          }
         }
-        sh.more = sh.w.next(a, sh.s);
+        if (hidden && alive) {
+          Hidden<T> hd;
+          hd.v = static_cast<const T*>(a.v) + s.kb * a.v_strides[0] + s.h * a.v_strides[1] +
+                 int64_t(s.start) * a.v_strides[2];
+          hd.stride = a.v_strides[2];
+          hd.anc = a.anc ? a.anc + int64_t(s.r0 + place) * a.anc_words : nullptr;
+          hd.words = a.anc_words;
+          hd.place = place;
+          hd.k0 = max(s.t0 * BN, max(s.first, 0));
+          hd.k1 = min(s.t1 * BN, s.len);
+          hd.first = s.first;
+          hd.d0 = 32 * i0;
+          hd.d1 = 32 * i1;
+          add_hidden<T>(hd, out, whole ? nullptr : pp + prow);
+        }
       }
       tcg::tc_fence_before();
-      named_sync(1 + slot, 128);
+      if (!pair) named_sync(3, 256);  // both have read both: the next weights may be given
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_empty[hand]);
     }
-    named_sync(3, 256);  // this CTA's parts are written
-    if (*n_cuts) join_parts<T, D>(a, cuts, *n_cuts, cta, tag, smem + L::Q, status);
+    ok = named_all(3, 256, ok);  // this CTA's parts are written
+    if (ok && *n_cuts) join_parts<T, D>(a, cuts, *n_cuts, cta, tag, smem + L::Q, status);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     Segment s;
-    if (warp == WARP_TMA) {
+    if (warp >= WARP_PREP) {
+      // -------------------------------------------------------------- segments and Q, ahead
+      constexpr int CH = D / 8, STEP = 64 / CH;  // 16-byte chunks a row, rows the 64 threads load at a time
+      const int t = tid - WARP_PREP * 32, c = t % CH, first_row = t / CH, G = a.Hq / a.Hk;
+      uint32_t n_q[2] = {0, 0};
+      auto load_q = [&](int slot) {
+        if (n_q[slot] > 0 && ok) ok = mbar_wait(&q_empty[slot], (n_q[slot] - 1) & 1u, status, kErrWaitMma);
+        ++n_q[slot];
+        const int row0 = s.row_base + (s.pair ? slot * ROWS : 0);
+        const int live = min(ROWS, s.rows * G - row0);  // rows past it are never looked at
+        const T* q = static_cast<const T*>(a.q) + int64_t(s.r0) * a.q_strides[0] + s.h * G * a.q_strides[1] + c * 8;
+        const uint32_t dst = smem_u32(smem + L::Q + slot * L::TILE) + uint32_t((c >> 3) * L::HALF);
+        const int dn = STEP / G, dg = STEP - dn * G;  // a step in (node, head of the group)
+        int node = (row0 + first_row) / G, g = row0 + first_row - node * G;
+        for (int r = first_row; r < live; r += STEP) {
+          cp_async_16_zfill(dst + uint32_t(r * 128 + (((c & 7) ^ (r & 7)) << 4)),
+                            q + node * a.q_strides[0] + g * a.q_strides[1], true);
+          node += dn;
+          g += dg;
+          if (g >= G) {
+            g -= G;
+            ++node;
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      auto give_q = [&](int slot) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[slot]);
+      };
+      for (int k = 0;; ++k) {
+        const bool more = __all_sync(0xffffffffu, ok) && wk.next(a, s);
+        const int hand = k & 1;
+        if (warp == WARP_PREP) {
+          if (k >= 2 && ok) ok = mbar_wait(&seg_empty[hand], uint32_t((k >> 1) - 1) & 1u, status, kErrWaitPeer);
+          if (lane == 0) {
+            Handed* h = reinterpret_cast<Handed*>(smem + L::SEGS + 64 * hand);
+            if (more) {
+              h->s = s;
+              if (s.t0 > 0 || s.t1 < s.T) {
+                int c0 = range.first, n_parts = range.parts;
+                if (n_parts == 0) {
+                  const int from = wk.start + SEG;  // cost of the item's first tile
+                  int c1 = cta + 1;
+                  for (c0 = cta; c0 > 0 && range.dealt(c0) > from; --c0) {}
+                  while (c1 < range.n && range.dealt(c1) <= from + wk.w * (s.T - 1)) ++c1;
+                  n_parts = c1 - c0;
+                }
+                cuts[(*n_cuts)++] = Cut{c0, n_parts, s.r0, s.live, s.row_base, s.h, {0, 0}};
+              }
+            }
+            h->more = more;
+            mbar_arrive(&seg_full[hand]);
+          }
+        }
+        if (!more) break;
+        const bool two = s.pair || s.t1 - s.t0 > 1;
+        load_q(0);
+        if (two) {
+          load_q(1);
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+          give_q(0);
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+          give_q(1);
+        } else {
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+          give_q(0);
+        }
+      }
+      __syncwarp();
+    } else if (warp == WARP_TMA) {
       // -------------------------------------------------------------- producer
       if (lane == 0) {
         int g = 0;
@@ -1001,7 +1019,7 @@ __global__ void __launch_bounds__(NTHR, 1)
       auto commit = [&](uint64_t* bar) {
         if (leader) tcg::umma_commit(bar);
       };
-      auto scores = [&](int slot, int x) {
+      auto scores = [&](int slot, int x, bool last) {
         if (!ok) return;
         const uint32_t qd = q_lo + uint32_t(slot) * (L::TILE >> 4);
         const uint32_t kd = desc_lo(ring_a + uint32_t(x) * L::TILE, 16);
@@ -1013,6 +1031,7 @@ __global__ void __launch_bounds__(NTHR, 1)
                     k ? 1u : 0u);
           }
           tcg::umma_commit(&s_full[slot]);
+          if (last) tcg::umma_commit(&q_empty[slot]);  // the segment's last use of this Q
         }
         issued = true;
       };
@@ -1051,9 +1070,9 @@ __global__ void __launch_bounds__(NTHR, 1)
         if (pair) {
           int x = take();
           q_ready(0);
-          scores(0, x);
+          scores(0, x, n == 1);
           q_ready(1);
-          scores(1, x);
+          scores(1, x, n == 1);
           release(x);
           for (int t = 0; t < n; ++t) {
             const int v = take();
@@ -1061,14 +1080,14 @@ __global__ void __launch_bounds__(NTHR, 1)
             values(0, v, t == 0);
             if (more) {
               x = take();
-              scores(0, x);
+              scores(0, x, t + 2 == n);
             } else if (ok) {
               commit(&o_full[0]);
             }
             values(1, v, t == 0);
             release(v);
             if (more) {
-              scores(1, x);
+              scores(1, x, t + 2 == n);
               release(x);
             } else if (ok) {
               commit(&o_full[1]);
@@ -1079,7 +1098,7 @@ __global__ void __launch_bounds__(NTHR, 1)
           for (int z = 0; z < min(n, 2); ++z) {
             const int x = take();
             q_ready(z);
-            scores(z, x);
+            scores(z, x, z + 2 >= n);
             release(x);
           }
           for (int t = 0; t < n; ++t) {
@@ -1088,7 +1107,7 @@ __global__ void __launch_bounds__(NTHR, 1)
             release(v);
             if (t + 2 < n) {
               const int x = take();
-              scores(z, x);
+              scores(z, x, t + 4 >= n);
               release(x);
             } else if (ok) {
               commit(&o_full[z]);
@@ -1146,14 +1165,15 @@ static int launch(const dspark_tree_attn_args& a, cudaStream_t s) {
                                                                int(smem));
                                  }),
                   "tree_attn: shared memory");
-  // the running maximum needs a positive factor: the scale's sign goes into q
-  const float c = fabsf(a.scale) * 1.4426950408889634f;
-  const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
+  // the running maximum needs a positive factor: a negative scale goes into the product (A negated),
+  // and zero becomes one that leaves all weights equal
+  const float c = a.scale == 0.f ? 1e-30f : fabsf(a.scale) * 1.4426950408889634f;
+  const uint32_t neg = a.scale < 0.f ? 1u << 13 : 0u;
   static std::atomic<uint64_t> launches{uint64_t(std::chrono::steady_clock::now().time_since_epoch().count())};
   const uint64_t tag = (launches.fetch_add(1, std::memory_order_relaxed) * 0x9E3779B97F4A7C15ull | 1ull << 63) &
                        ~0xffffull;
   DSPARK_CUDA_TRY(launch_all_at_once(attn_kernel<T, D>, dim3(n_cta), dim3(NTHR), smem, s, maps[0], maps[1],
-                                     a, sign == 0.f ? 1.f : c, sign, tag, st),
+                                     a, c, neg, tag, st),
                   "tree_attn");
   return DSPARK_OK;
 }

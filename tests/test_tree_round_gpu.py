@@ -246,6 +246,40 @@ def test_tree_sdpa_large_scores_and_late_maximum(cuda):
     _check_attn(out, q, k, v, counts, lens, parents, D ** -0.5, BF)
 
 
+@pytest.mark.parametrize("scale", [-0.11, 0.0, 2.0])
+def test_tree_sdpa_scales(cuda, scale):
+    """A negative scale, a scale of zero (the mean of what is seen), and a large one."""
+    from mlx_dspark_b200 import tree
+
+    counts, lens, Hq, Hk, D = [7, 150], [400, 333], 4, 2, 64
+    rng = random.Random(4)
+    parents = [ref.random_parents(n, rng) for n in counts]
+    q, k, v = _attn_case(cuda, HF, counts, lens, Hq, Hk, D, parents, 11)
+    anc = _i32([w for p in parents for w in ref.words_of(ref.ancestors(p), 5)], cuda)
+    out = tree.tree_sdpa(q.to(cuda), k.to(cuda), v.to(cuda), _cu(counts, cuda), _i32(lens, cuda), anc,
+                         scale=scale, max_nodes=150)
+    _check_attn(out, q, k, v, counts, lens, parents, scale, HF)
+
+
+@pytest.mark.parametrize("batch,nodes,longest", [(40, 9, 700), (23, 70, 900), (200, 3, 300), (9, 33, 5000)])
+def test_tree_sdpa_ragged_batches(cuda, batch, nodes, longest):
+    """Many requests of mixed sizes: shares that cross from request to request, items in several
+    parts, requests beyond one warp's lookup, idle ones between."""
+    from mlx_dspark_b200 import tree
+
+    rng = random.Random(batch)
+    counts = [rng.choice([0, 1, rng.randint(1, nodes)]) for _ in range(batch)]
+    lens = [max(n, rng.choice([n, rng.randint(1, longest)])) for n in counts]
+    Hq, Hk, D = 4, 2, 64
+    parents = [ref.random_parents(n, rng) if n else [] for n in counts]
+    q, k, v = _attn_case(cuda, BF, counts, lens, Hq, Hk, D, parents, batch)
+    words = tree.anc_words(nodes)
+    anc = _i32([w for p in parents if p for w in ref.words_of(ref.ancestors(p), words)], cuda)
+    out = tree.tree_sdpa(q.to(cuda), k.to(cuda), v.to(cuda), _cu(counts, cuda), _i32(lens, cuda), anc,
+                         scale=D ** -0.5, max_nodes=nodes)
+    _check_attn(out, q, k, v, counts, lens, parents, D ** -0.5, BF)
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 def test_tree_sdpa_hidden_keys_take_no_part(cuda, bad):
     """A branch with non-finite keys and values spoils its own descendants only."""
