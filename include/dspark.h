@@ -475,11 +475,12 @@ int dspark_p2p_allgather(const dspark_p2p_gather_args* args, void* stream);
 
 /* Per row: row_pos = kv_len[b] + depth (rotary position), row_slot = kv_len[b] + place (cache
  * slot), row_req = b, and anc = bits of the row itself and its ancestors (anc_words uint32 words
- * a row, bit j of word j / 32: place j). kv_len_new[b] = kv_len[b] + rows. parent may be NULL
+ * a row, bit j of word j / 32: place j). kv_len_new[b] = kv_len[b] + rows. With kv_start (a pool of
+ * positions as one batch entry) row_slot counts from kv_start[b] and row_req is 0. parent may be NULL
  * (each block a chain). A row whose parent is not before it counts as a second root. Outputs may
  * be NULL. Rows of a request beyond 32 * anc_words get no bits of those places. */
-int dspark_tree_pack(const int32_t* cu_rows, const int32_t* parent, const int32_t* kv_len, int B,
-                     int R, int32_t* row_pos, int32_t* row_slot, int32_t* row_req, uint32_t* anc,
+int dspark_tree_pack(const int32_t* cu_rows, const int32_t* parent, const int32_t* kv_len,
+                     const int32_t* kv_start, int B, int R, int32_t* row_pos, int32_t* row_slot, int32_t* row_req, uint32_t* anc,
                      int anc_words, int32_t* kv_len_new, void* stream);
 
 #define DSPARK_ROPE_HALF 0         /* pairs (i, i + rot / 2) */
@@ -589,6 +590,32 @@ typedef struct {
 
 int dspark_sample_accept(const dspark_sample_args* a, void* stream);
 size_t dspark_sample_workspace(int R, int B, int V);
+
+/* dspark_verify_forward for packed trees: the same embedding, projections, norms and lm_head; between
+ * the QKV projection and the O projection each layer runs dspark_rope_append (with the layer's q / k
+ * norms) and dspark_tree_attn instead of the fused epilogue and the block attention. `t` holds the
+ * round's metadata (dspark_tree_pack) and scratch: qkv bf16 [R, (Hq + 2 Hk) * head_dim], and the tree
+ * attention's workspace. The caches are the model's pools with a stride kv_sb between kv_batch entries.
+ * R <= buf->rows_cap; the packing arrays in buf are not used. */
+typedef struct {
+  const int32_t* cu_rows;
+  const int32_t* row_pos;
+  const int32_t* row_slot;
+  const int32_t* row_req;
+  const int32_t* kv_len;    /* [B], the trees' rows included */
+  const int32_t* kv_start;  /* [B] or NULL */
+  const uint32_t* anc;
+  const uint64_t* freq;     /* rotary frequencies as in dspark_rope_append */
+  void* qkv;
+  void* attn_ws;
+  size_t attn_ws_bytes;
+  int64_t kv_sb;            /* elements between the caches' batch entries */
+  float mscale;
+  int anc_words, max_rows, layout, rot, cap, kv_batch;
+} dspark_tree_fwd;
+
+int dspark_tree_forward(const dspark_model* m, const dspark_fwd_buffers* buf, const dspark_tree_fwd* t,
+                        const int32_t* ids, int R, int B, void* logits, int64_t ld_logits, void* stream);
 
 /* Keep the accepted path of each request: with base = lens[b] - n_accept[b] - 1 (lens after the
  * accept), cache row base + path[cu_rows[b] + i] moves to base + i for i <= n_accept[b], in every

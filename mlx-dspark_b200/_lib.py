@@ -115,6 +115,14 @@ class TreeAttnArgs(C.Structure):
                 ("cap", i32), ("kv_batch", i32)]
 
 
+class TreeFwd(C.Structure):
+    """``dspark_tree_fwd`` (include/dspark.h)."""
+    _fields_ = [("cu_rows", vp), ("row_pos", vp), ("row_slot", vp), ("row_req", vp), ("kv_len", vp),
+                ("kv_start", vp), ("anc", vp), ("freq", vp), ("qkv", vp), ("attn_ws", vp),
+                ("attn_ws_bytes", sz), ("kv_sb", i64), ("mscale", f32), ("anc_words", i32),
+                ("max_rows", i32), ("layout", i32), ("rot", i32), ("cap", i32), ("kv_batch", i32)]
+
+
 class SampleArgs(C.Structure):
     """``dspark_sample_args`` (include/dspark.h)."""
     _fields_ = [("logits", vp), ("draft", vp), ("ld_logits", i64), ("ld_draft", i64),
@@ -192,7 +200,9 @@ _SIGS = {
     "dspark_verify_forward": (i32, [C.POINTER(Model), C.POINTER(FwdBuffers), vp, i32, i32, i32,
                                     i32, vp, i64, vp]),
     "dspark_verify_prepare": (i32, [vp, i32, C.POINTER(FwdBuffers), vp]),
-    "dspark_tree_pack": (i32, [vp, vp, vp, i32, i32, vp, vp, vp, vp, i32, vp, vp]),
+    "dspark_tree_pack": (i32, [vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, i32, vp, vp]),
+    "dspark_tree_forward": (i32, [C.POINTER(Model), C.POINTER(FwdBuffers), C.POINTER(TreeFwd), vp, i32,
+                                  i32, vp, i64, vp]),
     "dspark_rope_append": (i32, [vp, vp]),
     "dspark_tree_attn": (i32, [vp, vp]),
     "dspark_tree_attn_workspace": (sz, [i32, i32, i32, i32, i32]),

@@ -601,14 +601,17 @@ int dspark_verify_prepare(int32_t* len, int R, const dspark_fwd_buffers* b, void
     if (_rc != DSPARK_OK) return _rc; \
   } while (0)
 
-int dspark_verify_forward(const dspark_model* m, const dspark_fwd_buffers* buf, const int32_t* ids,
-                          int R, int B, int qL_max, int L_max, void* logits, int64_t ld_logits,
-                          void* stream) {
-  if (!m || !buf || !ids || !logits || !m->layers) return fail(DSPARK_ERR_ARG, "forward: null");
+}  // extern "C"
+
+// The layer loop of dspark_verify_forward (tree NULL) and dspark_tree_forward.
+static int forward(const dspark_model* m, const dspark_fwd_buffers* buf, const dspark_tree_fwd* tree,
+                   const int32_t* ids, int R, int B, int qL_max, int L_max, void* logits,
+                   int64_t ld_logits, void* stream) {
   if (m->head_dim != 128) return fail(DSPARK_ERR_UNSUPPORTED, "forward: head_dim %d (needs 128)", m->head_dim);
   const int rows_cap = buf->rows_cap > 0 ? buf->rows_cap : 32;
   if (R < 1 || R > rows_cap) return fail(DSPARK_ERR_UNSUPPORTED, "forward: R=%d rows (1..%d)", R, rows_cap);
-  if (qL_max < 1 || qL_max > 32) return fail(DSPARK_ERR_UNSUPPORTED, "forward: qL_max=%d (1..32)", qL_max);
+  if (!tree && (qL_max < 1 || qL_max > 32))
+    return fail(DSPARK_ERR_UNSUPPORTED, "forward: qL_max=%d (1..32)", qL_max);
   if (m->hidden % 512 || m->intermediate % 512)
     return fail(DSPARK_ERR_UNSUPPORTED, "forward: hidden / intermediate must be multiples of 512");
   cudaStream_t s = as_stream(stream);
@@ -626,7 +629,7 @@ int dspark_verify_forward(const dspark_model* m, const dspark_fwd_buffers* buf, 
     size_t need = 0;
     for (int l = 0; l < m->n_layers; ++l) {
       const dspark_layer& L = m->layers[l];
-      need = std::max({need, qmm::wide_ws_bytes(R, H, L.qkv.N, qmm::EPI_QKROPE, true),
+      need = std::max({need, qmm::wide_ws_bytes(R, H, L.qkv.N, tree ? qmm::EPI_PLAIN : qmm::EPI_QKROPE, true),
                        qmm::wide_ws_bytes(R, L.o.K, L.o.N, qmm::EPI_RESID, false),
                        qmm::wide_ws_bytes(R, H, L.gate_up.N, qmm::EPI_SWIGLU, true),
                        qmm::wide_ws_bytes(R, L.down.K, L.down.N, qmm::EPI_RESID, false)});
@@ -645,7 +648,9 @@ int dspark_verify_forward(const dspark_model* m, const dspark_fwd_buffers* buf, 
 
   for (int l = 0; l < m->n_layers; ++l) {
     const dspark_layer& L = m->layers[l];
-    // fused QKV projection + input RMSNorm + q/k RMSNorm + RoPE + cache write
+    // fused QKV projection + input RMSNorm + q/k RMSNorm + RoPE + cache write (a tree: the projection
+    // and the input norm)
+    const int epi_qkv = tree ? qmm::EPI_PLAIN : qmm::EPI_QKROPE;
     for (int r0 = 0; r0 < R; r0 += kChunk) {
       const int mr = std::min(kChunk, R - r0);
       qmm::QmmParams p;
@@ -666,15 +671,50 @@ int dspark_verify_forward(const dspark_model* m, const dspark_fwd_buffers* buf, 
       p.kv_cap = m->kv_cap;
       p.row_pos = buf->row_pos + r0; p.row_kv = buf->row_kv + r0;
       p.out = xq; p.ldo = 0;
+      if (tree) {
+        p.out = static_cast<bf16*>(tree->qkv) + int64_t(r0) * L.qkv.N;
+        p.ldo = L.qkv.N;
+      }
       if (wide) {
-        DSPARK_TRY(qmm::run_wide(p, qmm::EPI_QKROPE, buf->wide_ws, buf->wide_ws_bytes, s));
+        DSPARK_TRY(qmm::run_wide(p, epi_qkv, buf->wide_ws, buf->wide_ws_bytes, s));
       } else {
-        qmm::QmmPlan pl = cached_plan(p.N, p.K, p.bits, qmm::EPI_QKROPE, mr);
-        DSPARK_TRY(qmm::run(p, qmm::EPI_QKROPE, &pl, s));
+        qmm::QmmPlan pl = cached_plan(p.N, p.K, p.bits, epi_qkv, mr);
+        DSPARK_TRY(qmm::run(p, epi_qkv, &pl, s));
       }
     }
-    // verify attention over each request's cache slot
-    {
+    if (tree) {
+      const int64_t row = L.qkv.N;
+      const bf16* qkv = static_cast<const bf16*>(tree->qkv);
+      dspark_rope_args r = {};
+      r.q = qkv; r.k = qkv + int64_t(Hq) * D; r.v = qkv + int64_t(Hq + Hk) * D;
+      r.q_strides[0] = r.k_strides[0] = r.v_strides[0] = row;
+      r.q_strides[1] = r.k_strides[1] = r.v_strides[1] = D;
+      r.q_out = xq; r.qo_strides[0] = int64_t(Hq) * D; r.qo_strides[1] = D;
+      r.k_cache = L.k_cache; r.v_cache = L.v_cache;
+      r.kc_strides[0] = r.vc_strides[0] = tree->kv_sb;
+      r.kc_strides[1] = m->k_sh; r.kc_strides[2] = m->k_ss;
+      r.vc_strides[1] = m->v_sh; r.vc_strides[2] = m->v_ss;
+      r.freq = tree->freq; r.row_pos = tree->row_pos; r.row_slot = tree->row_slot; r.row_req = tree->row_req;
+      r.q_norm = L.q_norm; r.k_norm = L.k_norm;
+      r.mscale = tree->mscale; r.eps = m->rms_eps; r.dtype = DSPARK_DTYPE_BF16; r.layout = tree->layout;
+      r.R = R; r.Hq = Hq; r.Hk = Hk; r.D = D; r.rot = tree->rot; r.cap = tree->cap; r.batch = tree->kv_batch;
+      DSPARK_TRY(dspark_rope_append(&r, stream));
+      dspark_tree_attn_args a = {};
+      a.q = xq; a.k = L.k_cache; a.v = L.v_cache; a.out = at;
+      a.q_strides[0] = a.o_strides[0] = int64_t(Hq) * D;
+      a.q_strides[1] = a.o_strides[1] = D;
+      for (int i = 0; i < 3; ++i) {
+        a.k_strides[i] = r.kc_strides[i];
+        a.v_strides[i] = r.vc_strides[i];
+      }
+      a.cu_rows = tree->cu_rows; a.kv_len = tree->kv_len; a.kv_start = tree->kv_start; a.anc = tree->anc;
+      a.workspace = tree->attn_ws; a.ws_bytes = tree->attn_ws_bytes;
+      a.scale = 1.0f / std::sqrt(float(D)); a.dtype = DSPARK_DTYPE_BF16;
+      a.anc_words = tree->anc_words; a.max_rows = tree->max_rows;
+      a.R = R; a.B = B; a.Hq = Hq; a.Hk = Hk; a.D = D; a.cap = tree->cap; a.kv_batch = tree->kv_batch;
+      DSPARK_TRY(dspark_tree_attn(&a, stream));
+    } else {
+      // verify attention over each request's cache slot
       attn::AttnParams a;
       a.q = xq; a.q_sh = D; a.q_si = int64_t(Hq) * D;
       a.o = at; a.o_sh = D; a.o_si = int64_t(Hq) * D;
@@ -775,6 +815,23 @@ int dspark_verify_forward(const dspark_model* m, const dspark_fwd_buffers* buf, 
     }
   }
   return DSPARK_OK;
+}
+
+extern "C" {
+
+int dspark_verify_forward(const dspark_model* m, const dspark_fwd_buffers* buf, const int32_t* ids,
+                          int R, int B, int qL_max, int L_max, void* logits, int64_t ld_logits,
+                          void* stream) {
+  if (!m || !buf || !ids || !logits || !m->layers) return fail(DSPARK_ERR_ARG, "forward: null");
+  return forward(m, buf, nullptr, ids, R, B, qL_max, L_max, logits, ld_logits, stream);
+}
+
+int dspark_tree_forward(const dspark_model* m, const dspark_fwd_buffers* buf, const dspark_tree_fwd* t,
+                        const int32_t* ids, int R, int B, void* logits, int64_t ld_logits, void* stream) {
+  if (!m || !buf || !t || !ids || !logits || !m->layers) return fail(DSPARK_ERR_ARG, "tree_forward: null");
+  if (!t->cu_rows || !t->row_pos || !t->row_slot || !t->kv_len || !t->freq || !t->qkv)
+    return fail(DSPARK_ERR_ARG, "tree_forward: null metadata or scratch");
+  return forward(m, buf, t, ids, R, B, 0, 0, logits, ld_logits, stream);
 }
 
 }  // extern "C"

@@ -9,7 +9,8 @@ namespace tree {
 // One block a request, one thread a row: the row walks up its ancestors (places descend, so the
 // words of its bit row are finished from the top down).
 __global__ void __launch_bounds__(256) pack_kernel(const int32_t* cu, const int32_t* parent,
-                                                   const int32_t* kv_len, int R, int32_t* row_pos,
+                                                   const int32_t* kv_len, const int32_t* kv_start, int R,
+                                                   int32_t* row_pos,
                                                    int32_t* row_slot, int32_t* row_req,
                                                    uint32_t* anc, int words, int32_t* kv_len_new) {
   pdl_launch_dependents();
@@ -53,8 +54,8 @@ __global__ void __launch_bounds__(256) pack_kernel(const int32_t* cu, const int3
       }
     }
     if (row_pos) row_pos[r] = L0 + depth;
-    if (row_slot) row_slot[r] = L0 + i;
-    if (row_req) row_req[r] = b;
+    if (row_slot) row_slot[r] = L0 + i + (kv_start ? kv_start[b] : 0);
+    if (row_req) row_req[r] = kv_start ? 0 : b;
   }
 }
 
@@ -111,8 +112,8 @@ using namespace dspark;
 
 extern "C" {
 
-int dspark_tree_pack(const int32_t* cu_rows, const int32_t* parent, const int32_t* kv_len, int B,
-                     int R, int32_t* row_pos, int32_t* row_slot, int32_t* row_req, uint32_t* anc,
+int dspark_tree_pack(const int32_t* cu_rows, const int32_t* parent, const int32_t* kv_len,
+                     const int32_t* kv_start, int B, int R, int32_t* row_pos, int32_t* row_slot, int32_t* row_req, uint32_t* anc,
                      int anc_words, int32_t* kv_len_new, void* stream) {
   if (B < 0 || R < 0) return fail(DSPARK_ERR_ARG, "tree_pack: bad shape (%d requests, %d rows)", B, R);
   if (B == 0) return DSPARK_OK;
@@ -120,7 +121,7 @@ int dspark_tree_pack(const int32_t* cu_rows, const int32_t* parent, const int32_
   if (anc && anc_words <= 0) return fail(DSPARK_ERR_ARG, "tree_pack: %d words a row", anc_words);
   DSPARK_CUDA_TRY(launch_ex(tree::pack_kernel, dim3(B), dim3(256), 0,
                             reinterpret_cast<cudaStream_t>(stream), 1, true, cu_rows, parent, kv_len,
-                            R, row_pos, row_slot, row_req, anc, anc_words, kv_len_new),
+                            kv_start, R, row_pos, row_slot, row_req, anc, anc_words, kv_len_new),
                   "tree_pack");
   return DSPARK_OK;
 }

@@ -185,11 +185,12 @@ struct Shape {
   int M, T, wl;
 };
 
-// Costs in half microseconds, as measured: a tile of one row block streams from HBM (64 KB in 1.5 us
-// with all SMs at it), one of two row blocks is held by its products and exponentials (2 us), and a
-// segment has its Q, its pipeline's fill and its O (6 us). 64 requests of 256 to 16k keys, dealt out
-// by tiles alone: 114 to 372 us a CTA.
-constexpr int ONE = 3, PAIR = 4, SEG = 12;
+// Costs in half microseconds, fitted to CTA times over ragged batches: a tile of one row block 1 us
+// (more when HBM holds it: 64 KB take 1.5 us with all SMs at it), one of two row blocks 2 us, and a
+// segment 7 us (its Q, its pipeline's fill, its O, its share of the joins). 64 requests of 256 to 16k
+// keys: 372 us for the last CTA when dealt out by tiles alone, 206 us for the call by these costs (3, 4
+// and 12: 250; 2, 4 and 8: 218).
+constexpr int ONE = 2, PAIR = 4, SEG = 14;
 
 __device__ __forceinline__ Shape shape_of(const dspark_tree_attn_args& a, int b) {
   int r0;
@@ -894,7 +895,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     if (ok && *n_cuts) join_parts<T, D>(a, cuts, *n_cuts, cta, tag, smem + L::Q, status);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    Segment s;
+    Segment s{};
     if (warp >= WARP_PREP) {
       // -------------------------------------------------------------- segments and Q, ahead
       constexpr int CH = D / 8, STEP = 64 / CH;  // 16-byte chunks a row, rows the 64 threads load at a time

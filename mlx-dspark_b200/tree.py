@@ -26,12 +26,13 @@ def anc_words(max_nodes: int) -> int:
 
 
 def pack(cu_rows: torch.Tensor, parent: torch.Tensor | None, kv_len: torch.Tensor, n_rows: int,
-         max_nodes: int, out: dict | None = None) -> dict:
+         max_nodes: int, kv_start: torch.Tensor | None = None, out: dict | None = None) -> dict:
     """Device-side metadata of one packed round: ``row_pos`` (cached tokens + depth), ``row_slot``
     (cached tokens + place), ``row_req``, ``anc`` (int32 ``[R, words]`` bit rows of each node and its
     ancestors) and ``kv_len_new``. ``kv_len`` int32 ``[B]``: tokens cached before the round;
-    ``parent`` int32 ``[R]``: places within the request, -1 for the root (``None``: chains)."""
-    stream = on_device(cu_rows, parent, kv_len)
+    ``parent`` int32 ``[R]``: places within the request, -1 for the root (``None``: chains).
+    With ``kv_start`` (a position-major pool) the slots count from it and ``row_req`` is 0."""
+    stream = on_device(cu_rows, parent, kv_len, kv_start)
     R, B = int(n_rows), kv_len.numel()
     words = anc_words(max_nodes)
     if out is None:
@@ -44,8 +45,9 @@ def pack(cu_rows: torch.Tensor, parent: torch.Tensor | None, kv_len: torch.Tenso
     at = {k: int32(k, out[k], n) for k, n in (("row_pos", R), ("row_slot", R), ("row_req", R),
                                               ("anc", R * words), ("kv_len_new", B))}
     _lib.check(_lib.lib.dspark_tree_pack(
-        int32("cu_rows", cu_rows, B + 1), int32("parent", parent, R), int32("kv_len", kv_len), B, R,
-        at["row_pos"], at["row_slot"], at["row_req"], at["anc"], words, at["kv_len_new"], stream))
+        int32("cu_rows", cu_rows, B + 1), int32("parent", parent, R), int32("kv_len", kv_len),
+        int32("kv_start", kv_start, B), B, R, at["row_pos"], at["row_slot"],
+        at["row_req"], at["anc"], words, at["kv_len_new"], stream))
     return out
 
 

@@ -18,7 +18,7 @@ from mlx_dspark_b200 import DSparkError, DSparkUnsupported, _lib, rope, sampling
 
 ROOT = Path(__file__).resolve().parents[1]
 _MIRRORS = {"RopeArgs": "dspark_rope_args", "TreeAttnArgs": "dspark_tree_attn_args",
-            "SampleArgs": "dspark_sample_args"}
+            "SampleArgs": "dspark_sample_args", "TreeFwd": "dspark_tree_fwd"}
 
 
 def test_ctypes_mirrors_match_the_header_layout(tmp_path):
@@ -123,8 +123,8 @@ def test_keep_path_and_pack_refusals():
     assert rc(d=9) == _lib.ERR_UNSUPPORTED and rc(strides=_lib.i64_array([64, 64, 9])) == _lib.ERR_UNSUPPORTED
     assert rc(B=3, kvb=2) == _lib.ERR_ARG and rc(kvb=0) == _lib.ERR_ARG
     assert rc(n=0) == _lib.OK and rc(B=0) == _lib.OK
-    assert _lib.lib.dspark_tree_pack(None, None, p, 1, 1, None, None, None, None, 0, None, None) == _lib.ERR_ARG
-    assert _lib.lib.dspark_tree_pack(p, None, p, 1, 1, None, None, None, p, 0, None, None) == _lib.ERR_ARG
+    assert _lib.lib.dspark_tree_pack(None, None, p, None, 1, 1, None, None, None, None, 0, None, None) == _lib.ERR_ARG
+    assert _lib.lib.dspark_tree_pack(p, None, p, None, 1, 1, None, None, None, p, 0, None, None) == _lib.ERR_ARG
 
 
 def test_cpu_tensors_are_refused():
