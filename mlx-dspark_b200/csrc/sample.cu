@@ -621,16 +621,19 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
   if (tid == 0) a.next_tok[b] = win.place == NONE ? -1 : win.place;
 }
 
-// Slices of a row for stat_kernel: of 64 KB, so that many rows do not end in a half-filled last round of
-// blocks; with few rows more, blocks for eight an SM (a chain) or 32 (a tree: more than half of its
-// rows are leaves, whose blocks end at once); at least 2048 values each.
+// Slices of a row for stat_kernel: of 128 KB, so that many rows do not end in a half-filled last round
+// of blocks (2192 rows of 304 KB: 158 us a call; of 64 KB 175, whole rows 184); with few rows more,
+// blocks for eight an SM (a chain) or 32 (a tree: more than half of its rows are leaves, whose blocks
+// end at once); at least 2048 values each.
 static int slices_of(int R, int V, int size, bool tree, int sms) {
   const int want = ((tree ? 32 : 8) * sms + R - 1) / std::max(R, 1);
-  return std::max(1, std::min(std::max(want, int(int64_t(V) * size / 65536)), V / 2048));
+  return std::max(1, std::min(std::max(want, int(int64_t(V) * size / 131072)), V / 2048));
 }
-// Blocks of a request for pick_kernel: 16 an SM over all requests.
+// Blocks of a request for pick_kernel: four an SM over all requests, which all run at once and walk
+// side by side (16 trees: 41 us a call; six an SM: 46), but at least four a request (256 requests: 158
+// us; three: 165, ten: 168).
 static int blocks_of(int B, int V, int sms) {
-  const int want = (16 * sms + B - 1) / std::max(B, 1);
+  const int want = std::max(4, (4 * sms + B - 1) / std::max(B, 1));
   return std::max((V + MAX_SLICE - 1) / MAX_SLICE, std::max(1, std::min(want, V / 2048)));
 }
 

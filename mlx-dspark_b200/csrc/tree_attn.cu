@@ -721,19 +721,22 @@ __global__ void __launch_bounds__(NTHR, 1)
         const int k0 = (tile0 + j * tstep) * BN;
         const bool edge = k0 > edge0;
         uint32_t bits[4];
-        if (edge) {  // while the scores are under way: who sees what, and V put right
+        if (edge) {  // while the scores are under way: who sees what
           const int place = place_of(a, s, slot, row);
           tile_bits(a, s, s.r0 + place, place, k0, bits);
-          if (slot == 0 || !pair) {
-            const int g = use0 + v_use(pair, k0 / BN - s.t0, n);
-            if (ok) ok = mbar_wait(&full[g % NB], uint32_t(g / NB) & 1u, status, kErrWaitKV);
-            fix_values<T, D>(ring + (g % NB) * L::TILE, k0, s.len, s.first, flag + (seg & 1), seg);
-            fence_proxy_async_smem();
-          }
         }
         if (ok) ok = mbar_wait(&s_full[slot], n_s & 1, status, kErrWaitMma);
         ++n_s;
         tcg::tc_fence_after();
+        if (edge && (slot == 0 || !pair)) {
+          // V put right. Not before the scores: they are made of K(t), and the previous use of V(t)'s
+          // buffer was loaded before K(t) (at most NB - 2 uses lie between), so the parity waited for
+          // here cannot be that of an earlier, still missing load
+          const int g = use0 + v_use(pair, k0 / BN - s.t0, n);
+          if (ok) ok = mbar_wait(&full[g % NB], uint32_t(g / NB) & 1u, status, kErrWaitKV);
+          fix_values<T, D>(ring + (g % NB) * L::TILE, k0, s.len, s.first, flag + (seg & 1), seg);
+          fence_proxy_async_smem();
+        }
         if (warp_alive) {
           float x[128];
 #pragma unroll

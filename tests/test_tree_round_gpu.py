@@ -280,6 +280,48 @@ def test_tree_sdpa_ragged_batches(cuda, batch, nodes, longest):
     _check_attn(out, q, k, v, counts, lens, parents, D ** -0.5, BF)
 
 
+@pytest.mark.parametrize("batch,nodes,longest,Hq,Hk", [(48, 2, 4000, 16, 8), (20, 19, 3000, 8, 4),
+                                                       (24, 40, 2000, 8, 4)])
+def test_tree_sdpa_back_to_back(cuda, batch, nodes, longest, Hq, Hk):
+    """Calls on two states in turn with nothing between them, head_dim 128 (the short ring): many
+    segments a CTA, whose last tiles are put right while other tiles are still on their way. Every
+    row of every call against the form in 64 bits: p rounded to the type, the output too."""
+    from mlx_dspark_b200 import tree
+
+    rng = random.Random(batch)
+    counts = [rng.randint(1, nodes) for _ in range(batch)]
+    D, words, calls = 128, tree.anc_words(nodes), []
+    for k in range(2):
+        lens = [max(n, rng.randint(1, longest)) for n in counts]
+        parents = [ref.random_parents(n, rng) for n in counts]
+        g = torch.Generator(device=cuda).manual_seed(k)
+        q = torch.randn(sum(counts), Hq, D, device=cuda, generator=g).to(HF)
+        kc, vc = (torch.randn(batch, Hk, max(lens) + 5, D, device=cuda, generator=g).to(HF) for _ in range(2))
+        anc = _i32([w for p in parents for w in ref.words_of(ref.ancestors(p), words)], cuda)
+        want, bound, r0 = torch.empty(q.shape, device=cuda, dtype=torch.float64), torch.empty_like(q, dtype=torch.float64), 0
+        for b, n in enumerate(counts):
+            sees = torch.ones(n, lens[b], dtype=torch.bool)
+            for i, a in enumerate(ref.ancestors(parents[b])):
+                sees[i, lens[b] - n :] = False
+                sees[i, [lens[b] - n + j for j in a]] = True
+            qb = q[r0 : r0 + n].double().view(n, Hk, Hq // Hk, D)
+            z = torch.einsum("nhgd,hld->hgnl", qb, kc[b, :, : lens[b]].double()) * D ** -0.5
+            w = torch.softmax(z.masked_fill(~sees.to(cuda), float("-inf")), -1)
+            v = vc[b, :, : lens[b]].double()
+            o = torch.einsum("hgnl,hld->nhgd", w, v).reshape(n, Hq, D)
+            absum = torch.einsum("hgnl,hld->nhgd", w, v.abs()).reshape(n, Hq, D)
+            want[r0 : r0 + n] = o
+            bound[r0 : r0 + n] = (U[HF] + 1e-4) * absum + U[HF] * o.abs() + 2.0 ** -25 * v.abs().sum(1).amax() + 1e-7
+            r0 += n
+        calls.append((q, kc, vc, _cu(counts, cuda), _i32(lens, cuda), anc, want, bound))
+    outs = []
+    for k in range(24):
+        c = calls[k % 2]
+        outs.append(tree.tree_sdpa(*c[:6], scale=D ** -0.5, max_nodes=nodes))
+    for k, out in enumerate(outs):
+        assert ((out.double() - calls[k % 2][6]).abs() <= calls[k % 2][7]).all(), k
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 def test_tree_sdpa_hidden_keys_take_no_part(cuda, bad):
     """A branch with non-finite keys and values spoils its own descendants only."""
