@@ -667,7 +667,10 @@ int dspark_sample_accept(const dspark_sample_args* p, void* stream) {
     return fail(DSPARK_ERR_ARG, "sample_accept: null pointer");
   if (a.parent && a.draft)
     return fail(DSPARK_ERR_UNSUPPORTED, "sample_accept: a tree's proposals carry no draft distribution");
-  if (a.R && a.ld_logits < a.V) return fail(DSPARK_ERR_ARG, "sample_accept: logits rows overlap");
+  // a stride of 0 is one row for all; anything else below V would overlap
+  if (a.R && ((a.ld_logits && a.ld_logits < a.V) || (a.ld_noise && a.ld_noise < a.V) ||
+              (a.draft && a.ld_draft && a.ld_draft < a.V)))
+    return fail(DSPARK_ERR_ARG, "sample_accept: rows of %d values overlap", a.V);
   if (a.ws_bytes < dspark_sample_workspace(a.R, a.B, a.V) || (a.R && !a.workspace))
     return fail(DSPARK_ERR_ARG, "sample_accept: workspace of %zu bytes", a.ws_bytes);
   const int sms = sm_count(current_device());

@@ -223,7 +223,7 @@ struct Range {
 
 // CTAs of one item among n when items have their own: one each, and the others by the tiles.
 __device__ __forceinline__ int ctas_of(int T, int n, int items, int tiles) {
-  return min(T, 1 + int(int64_t(T) * (n - items) / tiles));
+  return min(T, 1 + int(uint32_t(T) * uint32_t(n - items) / uint32_t(tiles)));  // T < 2^24: one cache
 }
 
 // Every warp for itself, no barrier. Items get their own CTAs unless the longest range then has OWN
@@ -533,13 +533,14 @@ __device__ __forceinline__ bool wait_count(const uint64_t* word, uint64_t tag, i
 
 // The 256 softmax threads, after the CTA's last segment: its share of the join of each item that it has
 // a part of. First the weights of all parts' rows into shared memory, whose tiles are no longer needed;
-// then blocks of 32 rows (lanes) x 4 values (a warp), dealt out over the item's CTAs. Twelve parts'
+// then blocks of 32 rows (lanes) x 4 values (a warp), dealt out over the item's CTAs. Sixteen parts'
 // values are in flight at a time.
 template <typename T, int D>
-__device__ __noinline__ void join_parts(const dspark_tree_attn_args& a, const Cut* cuts, int n_cuts, int cta,
-                                        uint64_t tag, uint8_t* smem, int* status) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.Hq / a.Hk;
-  uint64_t* count = static_cast<uint64_t*>(a.workspace);
+__device__ __noinline__ void join_parts(void* workspace, T* o_base, int64_t o_row, int64_t o_head, int G,
+                                        const Cut* cuts, int n_cuts, int cta, uint64_t tag, uint8_t* smem,
+                                        int* status) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint64_t* count = static_cast<uint64_t*>(workspace);
   if (tid == 0) {
     __threadfence();
     for (int k = 0; k < n_cuts; ++k) count_up(&count[cuts[k].first], tag, 2 * cuts[k].parts);
@@ -551,8 +552,10 @@ __device__ __noinline__ void join_parts(const dspark_tree_attn_args& a, const Cu
     const Cut c = cuts[k];
     if (tid == 0) wait_count(&count[c.first], tag, c.parts, status);
     named_sync(3, 256);
-    const float* first = part<D>(a.workspace, c.first, 1);
-    const float* rest = part<D>(a.workspace, c.first, 0);
+    // the count has been seen: the last to say so clears it, beside the others' work
+    if (tid == 255) count_up(&count[c.first], tag, 2 * c.parts);
+    const float* first = part<D>(workspace, c.first, 1);
+    const float* rest = part<D>(workspace, c.first, 0);
     auto at = [&](int x) { return x == 0 ? first : rest + x * STRIDE; };
     const int live = c.live, rounds = (live + 31) / 32;
     if (tid < live) {
@@ -591,7 +594,7 @@ __device__ __noinline__ void join_parts(const dspark_tree_attn_args& a, const Cu
       const int i = (z % rounds) * 32 + lane, d0 = z / rounds * 4;
       if (i >= live) continue;
       float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 12
+#pragma unroll 16
       for (int x = 0; x < c.parts; ++x) {
         const float* p = at(x) + d0 * (2 * ROWS) + i;
         const float f = w[x * 2 * ROWS + i];
@@ -599,14 +602,10 @@ __device__ __noinline__ void join_parts(const dspark_tree_attn_args& a, const Cu
         for (int e = 0; e < 4; ++e) o[e] += __ldcg(p + e * (2 * ROWS)) * f;
       }
       const int x = c.row_base + i, node = x / G, hq = c.h * G + x - node * G;
-      T* out = static_cast<T*>(a.out) + int64_t(c.r0 + node) * a.o_strides[0] + hq * a.o_strides[1] + d0;
+      T* out = o_base + int64_t(c.r0 + node) * o_row + hq * o_head + d0;
       *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack(o[0], o[1]), Elem<T>::pack(o[2], o[3]));
     }
-    named_sync(3, 256);  // all have read the parts
-    if (tid == 0) {
-      __threadfence();
-      count_up(&count[c.first], tag, 2 * c.parts);
-    }
+    named_sync(3, 256);  // the weights have been read: the next item's may land there
   }
 }
 
@@ -895,7 +894,9 @@ __global__ void __launch_bounds__(NTHR, 1)
       if (lane == 0) mbar_arrive(&seg_empty[hand]);
     }
     ok = named_all(3, 256, ok);  // this CTA's parts are written
-    if (ok && *n_cuts) join_parts<T, D>(a, cuts, *n_cuts, cta, tag, smem + L::Q, status);
+    if (ok && *n_cuts)
+      join_parts<T, D>(a.workspace, static_cast<T*>(a.out), a.o_strides[0], a.o_strides[1], a.Hq / a.Hk, cuts,
+                       *n_cuts, cta, tag, smem + L::Q, status);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     Segment s{};
@@ -1157,9 +1158,10 @@ static int launch(const dspark_tree_attn_args& a, cudaStream_t s) {
                   (long long)str[0], (long long)str[1], (long long)str[2]);
   }
   const int n_cta = grid_of(dev);
-  // costs are summed in 32 bits
+  // costs are summed in 32 bits, and tiles times CTAs too
   const int64_t G = a.Hq / a.Hk;
-  if ((int64_t(a.R) * G / (2 * ROWS) + a.B) * a.Hk * (PAIR * ((int64_t(a.cap) + BN - 1) / BN + 1) + SEG) > 0x7fffffff)
+  if ((int64_t(a.R) * G / (2 * ROWS) + a.B) * a.Hk * (PAIR * ((int64_t(a.cap) + BN - 1) / BN + 1) + SEG) > 0x7fffffff ||
+      a.cap / BN >= 1 << 24)
     return fail(DSPARK_ERR_UNSUPPORTED, "tree_attn: %d rows over %d positions in one call", a.R, a.cap);
   const size_t smem = Lay<D>::TOTAL;
   DSPARK_CUDA_TRY(configure_once((const void*)attn_kernel<T, D>, int(smem),
