@@ -270,9 +270,14 @@ __global__ void __launch_bounds__(THREADS) stat_kernel(const dspark_sample_args 
   __shared__ Stat part[THREADS / 32];
   if ((tid & 31) == 0) part[tid >> 5] = Stat{run.m, run.s, run.top, 0};
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < THREADS / 32; ++w) join(run, part[w].m, part[w].s, part[w].top, c, arg);
-    stat[int64_t(r) * slices + slice] = Stat{run.m, run.s, run.top, 0};
+  if (tid < 32) {
+    const Stat st = part[tid & (THREADS / 32 - 1)];
+    run.m = st.m, run.s = st.s, run.top = st.top;
+#pragma unroll
+    for (int o = THREADS / 64; o > 0; o >>= 1)
+      join(run, __shfl_xor_sync(0xffffffffu, run.m, o), __shfl_xor_sync(0xffffffffu, run.s, o),
+           __shfl_xor_sync(0xffffffffu, run.top, o), c, arg);
+    if (tid == 0) stat[int64_t(r) * slices + slice] = Stat{run.m, run.s, run.top, 0};
   }
 }
 
@@ -365,7 +370,7 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
   };
 
   // p of every row's token (beyond `seen` too: they are reported), and the sums of the rows that the
-  // walk can end at; eight lanes a row. A chain's rows are decided here.
+  // walk can end at; eight lanes a row, a warp where every row has one (few rows have many slices). A chain's rows are decided here.
   if (tid == 0) s_fail = MAX_ROWS;
   if (a.parent) {
     for (int i = tid; i < seen; i += THREADS) {
@@ -375,7 +380,8 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
     }
   }
   __syncthreads();
-  for (int i0 = tid >> 3; i0 < ((rows + 3) & ~3); i0 += THREADS / 8) {
+  const int span = rows <= THREADS / 32 ? 32 : 8, sub = tid & (span - 1);
+  for (int i0 = tid / span; i0 < ((rows + 3) & ~3); i0 += THREADS / span) {
     const int u = i0 < rows ? up(i0) : -1;
     Running run;
     float l = -INFINITY, q = 1.f, chance = 0.f;
@@ -387,16 +393,15 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
         if (draft && !arg) q = Elem<Q>::to_f(draft[int64_t(r0 + u) * a.ld_draft + x]);
       }
       if (!a.parent) chance = a.u[r0 + u];
-      for (int k = tid & 7; k < slices; k += 8) {
+      for (int k = sub; k < slices; k += span) {
         const Stat st = stat[int64_t(r0 + u) * slices + k];
         join(run, st.m, st.s, st.top, c, arg);
       }
     }
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1)
+    for (int o = span / 2; o > 0; o >>= 1)
       join(run, __shfl_xor_sync(0xffffffffu, run.m, o), __shfl_xor_sync(0xffffffffu, run.s, o),
            __shfl_xor_sync(0xffffffffu, run.top, o), c, arg);
-    if ((tid & 7) == 0 && i0 < rows) {
+    if (sub == 0 && i0 < rows) {
       float p = 1.f;
       if (u >= 0) {
         if (arg) p = run.m != -INFINITY && x == run.top ? 1.f : 0.f;
@@ -584,9 +589,13 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
     __syncthreads();
     if (lane == 0) s_pick[warp] = mine;
     __syncthreads();
-    mine = s_pick[0];
-    for (int w = 1; w < THREADS / 32; ++w)
-      if (beats(s_pick[w], mine)) mine = s_pick[w];
+    mine = s_pick[lane & (THREADS / 32 - 1)];
+#pragma unroll
+    for (int o = THREADS / 64; o > 0; o >>= 1) {
+      const Pick other{__shfl_xor_sync(0xffffffffu, mine.ref, o), __shfl_xor_sync(0xffffffffu, mine.score, o),
+                       __shfl_xor_sync(0xffffffffu, mine.place, o), 0};
+      if (beats(other, mine)) mine = other;
+    }
     return mine;
   };
   const Pick mine = block_best(Pick{sc.ref, sc.best, sc.place, 0});
@@ -624,10 +633,11 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
 // Slices of a row for stat_kernel: of 128 KB, so that many rows do not end in a half-filled last round
 // of blocks (2192 rows of 304 KB: 158 us a call; of 64 KB 175, whole rows 184); with few rows more,
 // blocks for eight an SM (a chain) or 32 (a tree: more than half of its rows are leaves, whose blocks
-// end at once); at least 2048 values each.
+// end at once); at least 8192 values each (five rows of 151936:
+// 13 us a call; 4096: 14.5, 2048: 15).
 static int slices_of(int R, int V, int size, bool tree, int sms) {
   const int want = ((tree ? 32 : 8) * sms + R - 1) / std::max(R, 1);
-  return std::max(1, std::min(std::max(want, int(int64_t(V) * size / 131072)), V / 2048));
+  return std::max(1, std::min(std::max(want, int(int64_t(V) * size / 131072)), V / 8192));
 }
 // Blocks of a request for pick_kernel: four an SM over all requests, which all run at once and walk
 // side by side (16 trees: 41 us a call; six an SM: 46), but at least four a request (256 requests: 158

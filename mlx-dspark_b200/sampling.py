@@ -8,6 +8,8 @@ src/mlx_dspark/sampling.py).
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -17,6 +19,11 @@ _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 _pack = _lib.packer(_lib.SampleArgs)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(R: int, B: int, V: int, device: int) -> int:
+    return _lib.lib.dspark_sample_workspace(R, B, V)
 
 
 def _rows_of(name: str, t: torch.Tensor, rows: int, V: int) -> int:
@@ -54,7 +61,8 @@ def sample_accept(logits: torch.Tensor, ids: torch.Tensor, cu_rows: torch.Tensor
     The token after the path is drawn by ``argmax(w / noise)``: ``w = max(p - q, 0)`` after a
     rejection with ``draft_probs``, else ``p`` without the tokens just tried. Returns ``n`` (accepted
     drafts), ``next``, ``prob`` (p of each row's token given its parent, 1 for roots) and ``path``
-    (kept places of each request in order, then -1); ``lens`` (int32 ``[B]``, tokens cached after the
+    (kept places of each request in order, then -1); ``out``, a former call's result for as many rows and
+    requests, is written again (its workspace too, on one stream). ``lens`` (int32 ``[B]``, tokens cached after the
     verify's append) loses the rejected rows in place. ``max_rows`` (<= 1024) bounds a block."""
     stream = on_device(logits, ids, cu_rows, u, noise, temperature, draft_probs, parent, lens)
     R, B = ids.numel(), cu_rows.numel() - 1
@@ -75,8 +83,13 @@ def sample_accept(logits: torch.Tensor, ids: torch.Tensor, cu_rows: torch.Tensor
                "path": torch.empty(R, **e)}
     else:
         on_device(logits, out["n"], out["next"], out["prob"], out["path"])
-    n = _lib.lib.dspark_sample_workspace(R, B, V)
-    ws = torch.empty(n, dtype=torch.uint8, device=logits.device) if n else None
+    n = _workspace(R, B, V, logits.get_device())
+    # a graph has to own what its replays write, a stream what the allocator may hand on in its order
+    kept, ws = out.get("workspace", (None, None))
+    if n and (kept != stream or ws.numel() < n or torch._C._cuda_isCurrentStreamCapturing()):
+        ws = torch.empty(n, dtype=torch.uint8, device=logits.device)
+        if not torch._C._cuda_isCurrentStreamCapturing():
+            out["workspace"] = stream, ws
     _lib.check(_lib.lib.dspark_sample_accept(_pack(
         logits.data_ptr(), draft, ld, ld_draft, ld_noise, int32("ids", ids), int32("cu_rows", cu_rows),
         int32("parent", parent, R), _f32("u", u, R), noise.data_ptr(), _f32("temperature", temperature, B),

@@ -542,6 +542,29 @@ def test_sample_accept_ties_go_to_the_first(cuda):
     assert got["next"].tolist() == [31003, 31003]
 
 
+def test_sample_accept_into_a_former_result(cuda):
+    """The tensors and the workspace of a former call are used again, also for more slices a row and on
+    another stream, with the result of a call that makes its own."""
+    from mlx_dspark_b200 import sampling
+
+    out = None
+    side = torch.cuda.Stream()
+    g = torch.Generator().manual_seed(7)
+    for V, stream in ((500, None), (90000, None), (30011, side), (90000, side), (500, None)):
+        logits = torch.randn(6, V, generator=g).to(cuda)
+        u, noise = torch.rand(6, generator=g).to(cuda), torch.empty(2, V).exponential_(generator=g).to(cuda)
+        ids = _i32([0] + logits[:3].argmax(1).tolist() + [1] + logits[4:5].argmax(1).tolist(), cuda)
+        a = (logits, ids, _cu([4, 2], cuda), u, noise)
+        kw = dict(temperature=torch.tensor([0.1, 0.3], device=cuda), max_rows=4)
+        want = sampling.sample_accept(*a, **kw)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            out = sampling.sample_accept(*a, **kw, out=out)
+        torch.cuda.synchronize()
+        for k in ("n", "next", "prob", "path"):
+            assert torch.equal(out[k], want[k]), (V, k)
+
+
 @pytest.mark.parametrize("form", ["chain", "draft", "tree"])
 def test_sample_accept_keeps_the_targets_distribution(cuda, form):
     """The first emitted token of 60000 rounds is distributed as p: each frequency within five
