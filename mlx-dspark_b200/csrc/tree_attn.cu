@@ -494,116 +494,158 @@ struct Cut {
 };
 constexpr int MAX_CTA = 160;
 
-// The workspace: a count a CTA (of the item whose first part it has), then part `which` of CTA c: D
-// values (divided by the part's sum) and the logarithm of the sum, m + log2 l, of 256 rows (row
+// The workspace: a count a CTA (of the item whose first part it has), two flags a CTA (of its parts),
+// then part `which` of CTA c: D values (divided by the part's sum) and the logarithm of the sum, m + log2 l, of 256 rows (row
 // innermost, as a warp of 32 rows writes them). An item's first part is its CTA's part 1, the others
 // are part 0.
 template <int D>
 __device__ __forceinline__ float* part(void* ws, int c, int which) {
-  return reinterpret_cast<float*>(static_cast<uint64_t*>(ws) + MAX_CTA) +
+  return reinterpret_cast<float*>(static_cast<uint64_t*>(ws) + 3 * MAX_CTA) +
          int64_t(2 * c + which) * (2 * ROWS) * (D + 1);
 }
 
-// Counts live in memory that nobody clears: a word that does not carry this launch's tag counts as
-// zero (the first to see it so puts the tag there, everybody else adds). Whoever counts last puts a
-// zero back, so that a replayed launch (same tag) starts anew.
-__device__ __forceinline__ void count_up(uint64_t* word, uint64_t tag, int last) {
-  unsigned long long* p = reinterpret_cast<unsigned long long*>(word);
-  const unsigned long long seen = *reinterpret_cast<volatile unsigned long long*>(p);
-  if ((seen & ~0xffffull) != tag) {
-    if (atomicCAS(p, seen, tag | 1ull) == seen) {
-      if (last == 1) *reinterpret_cast<volatile unsigned long long*>(p) = 0;
-      return;
-    }
-  }
-  if (int((atomicAdd(p, 1ull) & 0xffffu) + 1) == last) *reinterpret_cast<volatile unsigned long long*>(p) = 0;
+// Flags and counts live in memory that nobody clears beforehand: a flag is up when it is this launch's
+// tag, a count without the tag is zero. A flag costs its writer no answer from L2; a count of the parts
+// took three (1.3 us). The last of an item's CTAs to say that it has seen all flags puts zeros back,
+// so that a replayed launch (same tag) starts anew.
+__device__ __forceinline__ uint64_t* flag_of(void* ws, int c, int which) {
+  return static_cast<uint64_t*>(ws) + MAX_CTA + 2 * c + which;
 }
-__device__ __forceinline__ bool wait_count(const uint64_t* word, uint64_t tag, int n, int* status) {
+__device__ __forceinline__ void seen_all(void* ws, int first, int parts, uint64_t tag) {
+  unsigned long long* p = static_cast<unsigned long long*>(ws) + first;
+  __threadfence();
+  const unsigned long long seen = *reinterpret_cast<volatile unsigned long long*>(p);
+  int n = 0;
+  if ((seen & ~0xffffull) != tag && atomicCAS(p, seen, tag | 1ull) == seen) n = 1;
+  if (n == 0) n = int(atomicAdd(p, 1ull) & 0xffffu) + 1;
+  if (n != parts) return;
+  *reinterpret_cast<volatile unsigned long long*>(p) = 0;
+  for (int x = 0; x < parts; ++x) *reinterpret_cast<volatile uint64_t*>(flag_of(ws, first + x, x == 0)) = 0;
+}
+__device__ __forceinline__ void wait_flag(const uint64_t* word, uint64_t tag, int* status) {
   const uint64_t t0 = globaltimer_ns(), limit = wait_limit_ns(status);
   while (true) {
     uint64_t v;
     asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(word) : "memory");
-    if ((v & ~0xffffull) == tag && int(v & 0xffffu) >= n) return true;
+    if (v == tag) return;
     if (globaltimer_ns() - t0 > limit) {
       report_error(status, kErrWaitPeer);
-      return false;
+      return;
     }
   }
 }
 
+// One warp beside the softmax threads' join: it shows the CTA's parts and waits for the other CTAs',
+// so that nobody else waits for what it tells them afterwards.
+__device__ __noinline__ void show_and_wait(void* workspace, const Cut* cuts, int n_cuts, int cta, uint64_t tag,
+                                           int* status) {
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) {
+    __threadfence();
+    for (int k = 0; k < n_cuts; ++k)
+      asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(flag_of(workspace, cta, cuts[k].first == cta)),
+                   "l"(tag)
+                   : "memory");
+  }
+  __syncwarp();
+  for (int k = 0; k < n_cuts; ++k) {
+    const int first = cuts[k].first, parts = cuts[k].parts;
+    for (int x = lane; x < parts; x += 32) wait_flag(flag_of(workspace, first + x, x == 0), tag, status);
+    named_sync(4, 288);
+    if (lane == 0) seen_all(workspace, first, parts, tag);
+    __syncwarp();
+  }
+}
+
 // The 256 softmax threads, after the CTA's last segment: its share of the join of each item that it has
-// a part of. First the weights of all parts' rows into shared memory, whose tiles are no longer needed;
-// then blocks of 32 rows (lanes) x 4 values (a warp), dealt out over the item's CTAs. Sixteen parts'
-// values are in flight at a time.
+// a part of. The weights of all parts' rows go into shared memory, whose tiles are no longer needed; the
+// sums are dealt out over the item's CTAs in blocks of 32 rows (lanes) x 4 values (a warp). The values of
+// the first HELD parts are under way together, the first block's beside the weights.
 template <typename T, int D>
 __device__ __noinline__ void join_parts(void* workspace, T* o_base, int64_t o_row, int64_t o_head, int G,
-                                        const Cut* cuts, int n_cuts, int cta, uint64_t tag, uint8_t* smem,
-                                        int* status) {
+                                        const Cut* cuts, int n_cuts, int cta, uint8_t* smem) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  uint64_t* count = static_cast<uint64_t*>(workspace);
-  if (tid == 0) {
-    __threadfence();
-    for (int k = 0; k < n_cuts; ++k) count_up(&count[cuts[k].first], tag, 2 * cuts[k].parts);
-  }
   constexpr int64_t STRIDE = int64_t(2) * (2 * ROWS) * (D + 1);  // floats between the CTAs' parts
+  // One request's parts with 8 kv heads on 148 SMs. Code that runs once is paid by its length: with 20
+  // the same 16 parts (one token over 2k keys) take 14.3 us a call, with 18 13.6; of more than 18 parts
+  // the rest comes a latency later (18 parts, 61 nodes over 16k: 34.9 us; with 16 held 36.0).
+  constexpr int HELD = 18;
   static_assert(MAX_CTA * 2 * ROWS * 4 <= Lay<D>::ML, "the weights' room");
   float* w = reinterpret_cast<float*>(smem);  // [parts][256]
   for (int k = 0; k < n_cuts; ++k) {
     const Cut c = cuts[k];
-    if (tid == 0) wait_count(&count[c.first], tag, c.parts, status);
-    named_sync(3, 256);
-    // the count has been seen: the last to say so clears it, beside the others' work
-    if (tid == 255) count_up(&count[c.first], tag, 2 * c.parts);
+    named_sync(4, 288);  // show_and_wait has seen the item's flags
     const float* first = part<D>(workspace, c.first, 1);
     const float* rest = part<D>(workspace, c.first, 0);
     auto at = [&](int x) { return x == 0 ? first : rest + x * STRIDE; };
-    const int live = c.live, rounds = (live + 31) / 32;
+    const int live = c.live, rounds = (live + 31) / 32, blocks = rounds * (D / 4);
+    float v[HELD], m = -INFINITY;
     if (tid < live) {
-      float m = -INFINITY, sum = 0.f;
-      constexpr int HELD = 24;  // parts whose sums stay in registers
-      float v[HELD];
 #pragma unroll
       for (int x = 0; x < HELD; ++x) v[x] = x < c.parts ? __ldcg(at(x) + 2 * ROWS * D + tid) : -INFINITY;
-#pragma unroll
-      for (int x = 0; x < HELD; ++x) m = max3(m, v[x], v[x]);
-#pragma unroll 8
-      for (int x = HELD; x < c.parts; ++x) {
-        const float y = __ldcg(at(x) + 2 * ROWS * D + tid);
-        w[x * 2 * ROWS + tid] = y;
-        m = max3(m, y, y);
-      }
-      const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int x = 0; x < HELD; ++x) {
-        v[x] = ex2(v[x] - ref);
-        sum += v[x];
-      }
-      for (int x = HELD; x < c.parts; ++x) {
-        const float f = ex2(w[x * 2 * ROWS + tid] - ref);
-        w[x * 2 * ROWS + tid] = f;
-        sum += f;
-      }
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-      for (int x = 0; x < HELD; ++x)
-        if (x < c.parts) w[x * 2 * ROWS + tid] = v[x] * inv;
-      for (int x = HELD; x < c.parts; ++x) w[x * 2 * ROWS + tid] *= inv;
     }
-    named_sync(3, 256);
-    for (int z = (cta - c.first) + c.parts * warp; z < rounds * (D / 4); z += c.parts * 8) {
+    bool weighed = false;
+    for (int z = (cta - c.first) + c.parts * warp; !weighed || z < blocks; z += c.parts * 8) {
       const int i = (z % rounds) * 32 + lane, d0 = z / rounds * 4;
-      if (i >= live) continue;
-      float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 16
-      for (int x = 0; x < c.parts; ++x) {
-        const float* p = at(x) + d0 * (2 * ROWS) + i;
-        const float f = w[x * 2 * ROWS + i];
+      const bool mine = z < blocks && i < live;
+      float o[HELD][4];
+      if (mine) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += __ldcg(p + e * (2 * ROWS)) * f;
+        for (int x = 0; x < HELD; ++x) {
+          const float* p = at(x) + d0 * (2 * ROWS) + i;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[x][e] = x < c.parts ? __ldcg(p + e * (2 * ROWS)) : 0.f;
+        }
       }
-      const int x = c.row_base + i, node = x / G, hq = c.h * G + x - node * G;
-      T* out = o_base + int64_t(c.r0 + node) * o_row + hq * o_head + d0;
-      *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack(o[0], o[1]), Elem<T>::pack(o[2], o[3]));
+      if (!weighed) {
+        if (tid < live) {
+          float sum = 0.f;
+#pragma unroll
+          for (int x = 0; x < HELD; ++x) m = max3(m, v[x], v[x]);
+#pragma unroll 8
+          for (int x = HELD; x < c.parts; ++x) {
+            const float y = __ldcg(at(x) + 2 * ROWS * D + tid);
+            w[x * 2 * ROWS + tid] = y;
+            m = max3(m, y, y);
+          }
+          const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+          for (int x = 0; x < HELD; ++x) {
+            v[x] = ex2(v[x] - ref);
+            sum += v[x];
+          }
+          for (int x = HELD; x < c.parts; ++x) {
+            const float f = ex2(w[x * 2 * ROWS + tid] - ref);
+            w[x * 2 * ROWS + tid] = f;
+            sum += f;
+          }
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+          for (int x = 0; x < HELD; ++x) w[x * 2 * ROWS + tid] = v[x] * inv;  // (zero behind the last part)
+          for (int x = HELD; x < c.parts; ++x) w[x * 2 * ROWS + tid] *= inv;
+        }
+        named_sync(3, 256);
+        weighed = true;
+      }
+      if (mine) {
+        float r[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < HELD; ++x) {
+          const float f = w[x * 2 * ROWS + i];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r[e] += o[x][e] * f;
+        }
+#pragma unroll 8
+        for (int x = HELD; x < c.parts; ++x) {
+          const float* p = at(x) + d0 * (2 * ROWS) + i;
+          const float f = w[x * 2 * ROWS + i];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r[e] += __ldcg(p + e * (2 * ROWS)) * f;
+        }
+        const int x = c.row_base + i, node = x / G, hq = c.h * G + x - node * G;
+        T* out = o_base + int64_t(c.r0 + node) * o_row + hq * o_head + d0;
+        *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack(r[0], r[1]), Elem<T>::pack(r[2], r[3]));
+      }
     }
     named_sync(3, 256);  // the weights have been read: the next item's may land there
   }
@@ -893,10 +935,10 @@ __global__ void __launch_bounds__(NTHR, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&seg_empty[hand]);
     }
-    ok = named_all(3, 256, ok);  // this CTA's parts are written
+    ok = named_all(4, 288, ok);  // this CTA's parts are written
     if (ok && *n_cuts)
       join_parts<T, D>(a.workspace, static_cast<T*>(a.out), a.o_strides[0], a.o_strides[1], a.Hq / a.Hk, cuts,
-                       *n_cuts, cta, tag, smem + L::Q, status);
+                       *n_cuts, cta, smem + L::Q);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     Segment s{};
@@ -1002,6 +1044,7 @@ __global__ void __launch_bounds__(NTHR, 1)
           mbar_wait(&full[i % NB], uint32_t(i / NB) & 1u, status, kErrWaitKV);
       }
       __syncwarp();
+      if (named_all(4, 288, true) && *n_cuts) show_and_wait(a.workspace, cuts, *n_cuts, cta, tag, status);
     } else if (warp == WARP_MMA) {
       // -------------------------------------------------------------- products
       // The whole warp walks and waits; one lane issues. What an instruction needs is then the same in
@@ -1193,7 +1236,7 @@ extern "C" {
 
 size_t dspark_tree_attn_workspace(int B, int Hq, int Hk, int D, int max_rows) {
   if (B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || D <= 0 || max_rows <= 0) return 0;
-  return tattn::MAX_CTA * sizeof(uint64_t) +
+  return 3 * tattn::MAX_CTA * sizeof(uint64_t) +
          size_t(tattn::grid_of(current_device())) * 2 * (2 * tattn::ROWS) * (D + 1) * sizeof(float);
 }
 
