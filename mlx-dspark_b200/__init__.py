@@ -8,6 +8,9 @@ Modules mirror the reference operator surface (``src/mlx_dspark/``):
 * :mod:`.kvcache` / :mod:`.batch_engine` — per-row KV cache with in-place rollback (K3) and
   the ragged continuous-batching step built on the device (K4),
 * :mod:`.target` — a Qwen3-shaped dense target whose verify forward chains the fused kernels,
+* :mod:`.rope`, :mod:`.tree`, :mod:`.sampling` — rounds of drafted trees for sampled targets: rotary
+  positions and append, attention with ancestor masks, accept, the kept path; :mod:`.tree_engine`
+  runs them together over a target,
 * :mod:`.quant` — MLX-layout affine quantization of device tensors.
 
 All compute runs in ``libdspark.so`` (hand-written sm_100a CUDA) through a C ABI; torch only

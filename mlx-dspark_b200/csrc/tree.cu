@@ -63,7 +63,8 @@ __global__ void __launch_bounds__(256) pack_kernel(const int32_t* cu, const int3
 // order, KEEP_U at a time. A row's source never lies before its destination and sources ascend, so a
 // destination is read by no later row, and no column depends on another. Grid: x columns of all
 // heads, y requests, z caches (K and V of every layer). Bound: latency, or HBM with a large batch; only
-// rows that move are touched.
+// rows that move are touched. Measured in a graph: 36 layers of 8 heads of 128, one request 2.0 us, 64
+// requests 10.2 us (7.2 TB/s of moved bytes: part of them still in L2).
 constexpr int KEEP_U = 8;
 __global__ void __launch_bounds__(128) keep_kernel(
     void* const* k_layers, void* const* v_layers, int64_t k_b, int64_t k_h, int64_t k_t, int64_t v_b,

@@ -28,6 +28,11 @@
 // no shuffles. The maximum in use is only raised when a tile exceeds it by more than 2^8: the
 // weights then stay within fp16 / fp32 range and O is rarely rescaled.
 //
+// Bound: HBM up to about 200 rows an item (64 ragged requests of 256 to 16k keys: 196-217 us, 0.69 to
+// 0.75 of a plain copy's rate), above that the chain of softmax and products (two trees of 384 nodes, 64/8
+// heads, 32k keys: 880 us, 940 TFLOP/s at the power cap: 3750 clocks a tile of 256 x 128, 2048 of them
+// products); a chain of latencies for few tiles (one token over 2k keys 13.6 us, 61 nodes over 16k 35 us).
+//
 // Keys that a row does not see take no part whatever they hold: scores are replaced by -inf, V rows
 // past the request's keys are zeroed in shared memory, and a non-finite V among the tree's own keys
 // is taken out of the tile and added only to the rows that see it (fix_values / add_hidden).
@@ -188,8 +193,8 @@ struct Shape {
 // Costs in half microseconds, fitted to CTA times over ragged batches: a tile of one row block 1 us
 // (more when HBM holds it: 64 KB take 1.5 us with all SMs at it), one of two row blocks 2 us, and a
 // segment 7 us (its Q, its pipeline's fill, its O, its share of the joins). 64 requests of 256 to 16k
-// keys: 372 us for the last CTA when dealt out by tiles alone, 206 us for the call by these costs (3, 4
-// and 12: 250; 2, 4 and 8: 218).
+// keys: 372 us for the last CTA when dealt out by tiles alone; the call by these costs 206 us, by 3, 4 and
+// 12: 250, by 2, 4 and 8: 218 (each before the later steps that make it 196).
 constexpr int ONE = 2, PAIR = 4, SEG = 14;
 
 __device__ __forceinline__ Shape shape_of(const dspark_tree_attn_args& a, int b) {
