@@ -13,8 +13,8 @@
 //  * otherwise argmax p / e = argmax (l - ref) log2e / T - log2 e for any ref of the row: no sum, and
 //    no rounding of p to zero. ref is the largest logit so far, so that scores stay near zero.
 // Bound: HBM (each deciding row once), or the two launches for a single block. Measured over 151,936
-// tokens: 256 chains of up to 16 rows 158 us (0.87 of a plain copy), 16 trees of up to 61 nodes 40 us
-// (0.51: blocks of rows without a child and the walk's latency), five rows 13 us.
+// tokens: 256 chains of up to 16 rows 153 us (0.89 of a plain copy), 16 trees of up to 61 nodes 38 us
+// (0.54: blocks of rows without a child and the walk's latency), five rows 12 us.
 #include <float.h>
 
 #include <algorithm>
@@ -145,6 +145,13 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
   return v;
 }
 
+// Whole 16-byte pieces of [p, p + bytes) into L2.
+__device__ __forceinline__ void prefetch_l2(const void* p, int bytes) {
+  const uintptr_t at = (reinterpret_cast<uintptr_t>(p) + 15) & ~uintptr_t(15);
+  const int n = (bytes - int(at - reinterpret_cast<uintptr_t>(p))) & ~15;
+  if (n > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(at), "r"(n) : "memory");
+}
+
 struct Running {
   float m = -INFINITY, s = 0.f;
   int top = 0x7fffffff;
@@ -160,6 +167,26 @@ __device__ __forceinline__ void join(Running& a, float m, float s, int top, floa
   const float mn = fmaxf(a.m, m);
   a.s = a.s * mass(a.m, mn, c) + s * mass(m, mn, c);
   a.m = mn;
+}
+
+// The largest of a warp's values.
+__device__ __forceinline__ float warp_max(float x) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Joins a warp's maxima and sums, the same result in every lane.
+__device__ __forceinline__ void warp_join(Running& a, float c, bool arg) {
+  const float m = warp_max(a.m);
+  if (arg) {
+    a.top = __reduce_min_sync(0xffffffffu, a.m == m ? a.top : 0x7fffffff);
+  } else {
+    a.s *= mass(a.m, m, c);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+  }
+  a.m = m;
 }
 
 // grid R * slices: block (r, slice). Also clears the requests' counts for the next kernel.
@@ -265,20 +292,14 @@ __global__ void __launch_bounds__(THREADS) stat_kernel(const dspark_sample_args 
       for (int e = 0; e < N; ++e) join(run, clean(x[e]), 1.f, 0, c, false);
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    join(run, __shfl_xor_sync(0xffffffffu, run.m, o), __shfl_xor_sync(0xffffffffu, run.s, o),
-         __shfl_xor_sync(0xffffffffu, run.top, o), c, arg);
+  warp_join(run, c, arg);
   __shared__ Stat part[THREADS / 32];
   if ((tid & 31) == 0) part[tid >> 5] = Stat{run.m, run.s, run.top, 0};
   __syncthreads();
   if (tid < 32) {
-    const Stat st = part[tid & (THREADS / 32 - 1)];
-    run.m = st.m, run.s = st.s, run.top = st.top;
-#pragma unroll
-    for (int o = THREADS / 64; o > 0; o >>= 1)
-      join(run, __shfl_xor_sync(0xffffffffu, run.m, o), __shfl_xor_sync(0xffffffffu, run.s, o),
-           __shfl_xor_sync(0xffffffffu, run.top, o), c, arg);
+    run = Running();
+    if (tid < THREADS / 32) run.m = part[tid].m, run.s = part[tid].s, run.top = part[tid].top;
+    warp_join(run, c, arg);
     if (tid == 0) stat[int64_t(r) * slices + slice] = Stat{run.m, run.s, run.top, 0};
   }
 }
@@ -364,6 +385,10 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
   const float temp = a.temperature ? a.temperature[b] : 1.f;
   const bool arg = greedy(temp);
   const float c = arg ? 0.f : slope(temp);
+  const float* e = a.noise + int64_t(b) * a.ld_noise;
+  const int w0 = int(int64_t(a.V) * slice / blocks) & ~7;
+  const int w1 = slice + 1 == blocks ? a.V : int(int64_t(a.V) * (slice + 1) / blocks) & ~7;
+  if (!arg && tid == 0) prefetch_l2(e + w0, (w1 - w0) * 4);  // on its way to L2 beside the walk
   const T* logits = static_cast<const T*>(a.logits);
   const Q* draft = static_cast<const Q*>(a.draft);
   auto up = [&](int i) {
@@ -488,9 +513,6 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
   const bool rest = draft && !arg && last + 1 < seen;  // a chain's rejection with a distribution
   const T* row = logits + int64_t(r0 + last) * a.ld_logits;
   const Q* qrow = rest ? draft + int64_t(r0 + last) * a.ld_draft : nullptr;
-  const float* e = a.noise + int64_t(b) * a.ld_noise;
-  const int w0 = int(int64_t(a.V) * slice / blocks) & ~7;
-  const int w1 = slice + 1 == blocks ? a.V : int(int64_t(a.V) * (slice + 1) / blocks) & ~7;
   const bool bar = !rest && ntried > 0;
   if (bar) {
     for (int i = tid; i < (w1 - w0 + 31) / 32; i += THREADS) s_map[i] = 0;
@@ -573,32 +595,28 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
   else if (mode == kBarred) scan(std::integral_constant<Mode, kBarred>());
   else scan(std::integral_constant<Mode, kFree>());
 
-  // the best of the slice, then of the request's slices; scores of different refs by the difference of
-  // the refs, in 64 bits (greedy and kRest: the refs are zero). inf - inf of equal scores is a tie.
-  auto beats = [&](const Pick& x, const Pick& y) {
-    if (x.place == NONE || y.place == NONE) return y.place == NONE && x.place != NONE;
-    const double d = (double(x.ref) - double(y.ref)) * c + (double(x.score) - double(y.score));
-    return d > 0 || (!(d < 0) && x.place < y.place);
-  };
+  // the best of the slice, then of the request's slices. Scores of different refs are put on the largest
+  // of them first (the winner's own shift is small: less than log2 of the noise's range, so nothing is
+  // lost in 32 bits; greedy and kRest: all refs are zero). Equal scores: the first place.
   __shared__ Pick s_pick[THREADS / 32];
-  auto block_best = [&](Pick mine) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const Pick other{__shfl_xor_sync(0xffffffffu, mine.ref, o), __shfl_xor_sync(0xffffffffu, mine.score, o),
-                       __shfl_xor_sync(0xffffffffu, mine.place, o), 0};
-      if (beats(other, mine)) mine = other;
-    }
+  auto warp_best = [&](Pick x) {
+    const bool any = x.place != NONE;
+    const float ref = warp_max(any ? x.ref : -INFINITY);
+    if (any && x.ref != ref) x.score += (x.ref - ref) * c;
+    const float top = warp_max(any ? x.score : -INFINITY);
+    x.place = __reduce_min_sync(0xffffffffu, any && x.score == top ? x.place : NONE);
+    x.ref = ref;
+    x.score = top;
+    return x;
+  };
+  auto block_best = [&](Pick x) {
+    x = warp_best(x);
     __syncthreads();
-    if (lane == 0) s_pick[warp] = mine;
+    if (lane == 0) s_pick[warp] = x;
     __syncthreads();
-    mine = s_pick[lane & (THREADS / 32 - 1)];
-#pragma unroll
-    for (int o = THREADS / 64; o > 0; o >>= 1) {
-      const Pick other{__shfl_xor_sync(0xffffffffu, mine.ref, o), __shfl_xor_sync(0xffffffffu, mine.score, o),
-                       __shfl_xor_sync(0xffffffffu, mine.place, o), 0};
-      if (beats(other, mine)) mine = other;
-    }
-    return mine;
+    x = Pick{0.f, 0.f, NONE, 0};
+    if (lane < THREADS / 32) x = s_pick[lane];
+    return warp_best(x);
   };
   const Pick mine = block_best(Pick{sc.ref, sc.best, sc.place, 0});
   __shared__ bool s_final;
@@ -613,8 +631,15 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
   Pick win{0.f, 0.f, NONE, 0};
   for (int k = tid; k < blocks; k += THREADS) {
     const int4 raw = __ldcg(reinterpret_cast<const int4*>(&picks[int64_t(b) * blocks + k]));
-    const Pick x{__int_as_float(raw.x), __int_as_float(raw.y), raw.z, 0};
-    if (beats(x, win)) win = x;
+    Pick x{__int_as_float(raw.x), __int_as_float(raw.y), raw.z, 0};
+    if (x.place == NONE) continue;
+    if (win.place != NONE) {  // (places ascend)
+      const float ref = fmaxf(x.ref, win.ref);
+      if (x.ref != ref) x.score += (x.ref - ref) * c;
+      if (win.ref != ref) win.score += (win.ref - ref) * c;
+      x.ref = win.ref = ref;
+    }
+    if (win.place == NONE || x.score > win.score) win = x;
   }
   win = block_best(win);
   if (win.place == NONE && (rest || bar)) {
