@@ -397,7 +397,8 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
   };
 
   // p of every row's token (beyond `seen` too: they are reported), and the sums of the rows that the
-  // walk can end at; eight lanes a row, a warp where every row has one (few rows have many slices). A chain's rows are decided here.
+  // walk can end at; 4 to 32 lanes a row, all rows at once where there are up to 64. A chain's rows are
+  // decided here.
   if (tid == 0) s_fail = MAX_ROWS;
   if (a.parent) {
     for (int i = tid; i < seen; i += THREADS) {
@@ -407,8 +408,10 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
     }
   }
   __syncthreads();
-  const int span = rows <= THREADS / 32 ? 32 : 8, sub = tid & (span - 1);
-  for (int i0 = tid / span; i0 < ((rows + 3) & ~3); i0 += THREADS / span) {
+  int span = 32;  // lanes a row
+  while (span > 4 && rows * span > THREADS) span >>= 1;
+  const int sub = tid & (span - 1);
+  for (int i0 = tid / span; i0 < ((rows + 7) & ~7); i0 += THREADS / span) {
     const int u = i0 < rows ? up(i0) : -1;
     Running run;
     float l = -INFINITY, q = 1.f, chance = 0.f;
@@ -425,9 +428,16 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
         join(run, st.m, st.s, st.top, c, arg);
       }
     }
-    for (int o = span / 2; o > 0; o >>= 1)
-      join(run, __shfl_xor_sync(0xffffffffu, run.m, o), __shfl_xor_sync(0xffffffffu, run.s, o),
-           __shfl_xor_sync(0xffffffffu, run.top, o), c, arg);
+    float m = run.m;
+    for (int o = span / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (arg) {
+      if (run.m != m) run.top = 0x7fffffff;
+      for (int o = span / 2; o > 0; o >>= 1) run.top = min(run.top, __shfl_xor_sync(0xffffffffu, run.top, o));
+    } else {
+      run.s *= mass(run.m, m, c);
+      for (int o = span / 2; o > 0; o >>= 1) run.s += __shfl_xor_sync(0xffffffffu, run.s, o);
+    }
+    run.m = m;
     if (sub == 0 && i0 < rows) {
       float p = 1.f;
       if (u >= 0) {
@@ -471,26 +481,34 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
         const float u = s_u[cur];
         for (int j0 = cur + 1; j0 < seen && !on; j0 += 32) {
           const int j = j0 + lane;
-          unsigned kids = __ballot_sync(0xffffffffu, j < seen && s_up[min(j, seen - 1)] == cur);
-          while (kids) {
-            const int k = j0 + __ffs(kids) - 1;
-            kids &= kids - 1;
-            const int x = s_id[k];
-            bool twin = false;
-            for (int t = lane; t < tried; t += 32) twin |= s_tried[t] == x;
-            if (__any_sync(0xffffffffu, twin)) continue;
-            if (lane == 0) s_tried[tried] = x;
-            __syncwarp();
+          const bool kid = j < seen && s_up[min(j, seen - 1)] == cur;
+          const unsigned kids = __ballot_sync(0xffffffffu, kid);
+          if (!kids) continue;
+          int x = 0;
+          float p = 0.f;
+          bool twin = false;  // a token counts once
+          if (kid) {
+            x = s_id[j];
+            p = s_p[j];
+            twin = __match_any_sync(kids, x) & ((1u << lane) - 1u);
+            for (int t = 0; t < tried; ++t) twin |= s_tried[t] == x;
+          }
+          unsigned fresh = __ballot_sync(0xffffffffu, kid && !twin);
+          while (fresh) {
+            const int l = __ffs(fresh) - 1;
+            fresh &= fresh - 1;
+            if (lane == l) s_tried[tried] = x;
             ++tried;
-            run += s_p[k];
+            run += __shfl_sync(0xffffffffu, p, l);
             if (u < run) {
-              cur = k;
+              cur = j0 + l;
               ++n;
-              if (lead && a.path && lane == 0) a.path[r0 + n] = k;
+              if (lead && a.path && lane == 0) a.path[r0 + n] = cur;
               on = true;
               break;
             }
           }
+          __syncwarp();
         }
       }
       if (lane == 0) {
