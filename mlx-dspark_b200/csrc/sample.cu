@@ -13,8 +13,8 @@
 //  * otherwise argmax p / e = argmax (l - ref) log2e / T - log2 e for any ref of the row: no sum, and
 //    no rounding of p to zero. ref is the largest logit so far, so that scores stay near zero.
 // Bound: HBM (each deciding row once), or the two launches for a single block. Measured over 151,936
-// tokens: 256 chains of up to 16 rows 153 us (0.89 of a plain copy), 16 trees of up to 61 nodes 38 us
-// (0.54: blocks of rows without a child and the walk's latency), five rows 12 us.
+// tokens: 256 chains of up to 16 rows 153 us (0.89 of a plain copy), 16 trees of up to 61 nodes 37 us
+// (0.55: blocks of rows without a child and the walk's latency), five rows 12 us.
 #include <float.h>
 
 #include <algorithm>

@@ -193,8 +193,9 @@ struct Shape {
 // Costs in half microseconds, fitted to CTA times over ragged batches: a tile of one row block 1 us
 // (more when HBM holds it: 64 KB take 1.5 us with all SMs at it), one of two row blocks 2 us, and a
 // segment 7 us (its Q, its pipeline's fill, its O, its share of the joins). 64 requests of 256 to 16k
-// keys: 372 us for the last CTA when dealt out by tiles alone; the call by these costs 206 us, by 3, 4 and
-// 12: 250, by 2, 4 and 8: 218 (each before the later steps that make it 196).
+// keys: 372 us for the last CTA when dealt out by tiles alone. Mean of eleven mixes (1 to 200 requests of
+// 1 to 61 nodes over 100 to 32k keys) by a segment's cost: 8 86.9 us, 10 86.8, 12 85.6, 14 86.2, 16 86.2;
+// the 64 requests: 12 204 us, 14 199.
 constexpr int ONE = 2, PAIR = 4, SEG = 14;
 
 __device__ __forceinline__ Shape shape_of(const dspark_tree_attn_args& a, int b) {

@@ -64,7 +64,8 @@ def sample_accept(logits: torch.Tensor, ids: torch.Tensor, cu_rows: torch.Tensor
     (kept places of each request in order, then -1); ``out``, a former call's result for as many rows and
     requests, is written again (its workspace too, on one stream). ``lens`` (int32 ``[B]``, tokens cached after the
     verify's append) loses the rejected rows in place. ``max_rows`` (<= 1024) bounds a block."""
-    stream = on_device(logits, ids, cu_rows, u, noise, temperature, draft_probs, parent, lens)
+    given = () if out is None else (out["n"], out["next"], out["prob"], out["path"])
+    stream = on_device(logits, ids, cu_rows, u, noise, temperature, draft_probs, parent, lens, *given)
     R, B = ids.numel(), cu_rows.numel() - 1
     V = logits.shape[-1]
     ld, ld_noise = _rows_of("logits", logits, R, V), _rows_of("noise", noise, B, V)
@@ -81,8 +82,6 @@ def sample_accept(logits: torch.Tensor, ids: torch.Tensor, cu_rows: torch.Tensor
         out = {"n": torch.empty(B, **e), "next": torch.empty(B, **e),
                "prob": torch.empty(R, dtype=torch.float32, device=logits.device),
                "path": torch.empty(R, **e)}
-    else:
-        on_device(logits, out["n"], out["next"], out["prob"], out["path"])
     n = _workspace(R, B, V, logits.get_device())
     # a graph has to own what its replays write, a stream what the allocator may hand on in its order
     kept, ws = out.get("workspace", (None, None))

@@ -11,6 +11,8 @@ src/mlx_dspark/tree.py, with its 32-node attention in :mod:`.multirow_attn`).
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -18,6 +20,11 @@ from ._torch import int32, on_device
 from .rope import _dtype, _strides
 
 _pack_attn = _lib.packer(_lib.TreeAttnArgs)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(B: int, Hq: int, Hk: int, D: int, max_nodes: int, device: int) -> int:
+    return _lib.lib.dspark_tree_attn_workspace(B, Hq, Hk, D, max_nodes)
 
 
 def anc_words(max_nodes: int) -> int:
@@ -82,7 +89,7 @@ def tree_sdpa(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_
         if anc.ndim != 2 or anc.shape[0] != R:
             raise _lib.DSparkError(_lib.ERR_ARG, f"anc {tuple(anc.shape)} for {R} rows")
         words = anc.shape[1]
-    n = _lib.lib.dspark_tree_attn_workspace(B, Hq, Hk, D, max_nodes)
+    n = _workspace(B, Hq, Hk, D, max_nodes, q.get_device())
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     _lib.check(_lib.lib.dspark_tree_attn(_pack_attn(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1],
