@@ -386,8 +386,11 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
   const bool arg = greedy(temp);
   const float c = arg ? 0.f : slope(temp);
   const float* e = a.noise + int64_t(b) * a.ld_noise;
-  const int w0 = int(int64_t(a.V) * slice / blocks) & ~7;
-  const int w1 = slice + 1 == blocks ? a.V : int(int64_t(a.V) * (slice + 1) / blocks) & ~7;
+  // the slice: whole groups of eight values, dealt out evenly, so that no slice is wider than MAX_SLICE
+  // (blocks_of: blocks * MAX_SLICE >= V, so blocks * (MAX_SLICE / 8) >= groups)
+  const int groups = (a.V + 7) / 8;
+  const int w0 = 8 * int(int64_t(groups) * slice / blocks);
+  const int w1 = min(a.V, 8 * int(int64_t(groups) * (slice + 1) / blocks));
   if (!arg && tid == 0) prefetch_l2(e + w0, (w1 - w0) * 4);  // on its way to L2 beside the walk
   const T* logits = static_cast<const T*>(a.logits);
   const Q* draft = static_cast<const Q*>(a.draft);

@@ -1,0 +1,58 @@
+"""Edges of the tree-round operators on the GPU: widest slices, slots that run out of room, refused
+calls, waits that run out, long tails. Bounds as in test_tree_round_gpu.py."""
+
+from __future__ import annotations
+
+import random
+
+import numpy as np
+import pytest
+import torch
+import tree_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+def _i32(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def _cu(counts, dev):
+    return _i32([0] + np.cumsum(counts).tolist(), dev)
+
+
+# ----------------------------------------------------------------- sampled accept
+
+@pytest.mark.parametrize("form", ["tree", "chain"])
+@pytest.mark.parametrize("V", [262121, 262143, 327679, 393209])
+def test_sample_accept_widest_slices(cuda, form, V):
+    """Many requests over a vocabulary just below a multiple of 65536: slices of the widest kind, the
+    tokens tried and drawn among their last values."""
+    from mlx_dspark_b200 import sampling
+
+    B, rows = 150, 3
+    g = torch.Generator().manual_seed(V)
+    row = torch.randn(V, generator=g)
+    row[-3:] = torch.tensor([15.0, 16.0, 17.0])
+    noise = torch.empty(V).exponential_(generator=g)
+    noise[-3:] = torch.tensor([0.5, 1e-3, 1e-3])  # without the bars V - 2 or V - 1 would be drawn
+    ids = _i32([7, V - 1, V - 2] * B, cuda)
+    u = torch.rand(B, rows, generator=g)
+    u[::3] = 0.9999  # nothing accepted: the token after is drawn without those tried
+    temp = torch.ones(B)
+    temp[1::7] = 0.0
+    parents = [-1, 0, 0] if form == "tree" else None
+    got = sampling.sample_accept(
+        row.to(cuda).expand(B * rows, V), ids, _cu([rows] * B, cuda), u.flatten().to(cuda),
+        noise.to(cuda).expand(B, V), temperature=temp.to(cuda), max_rows=rows,
+        parent=None if parents is None else _i32(parents * B, cuda))
+    n, nxt, path = got["n"].tolist(), got["next"].tolist(), got["path"].view(B, rows).tolist()
+    p = {T: ref.probabilities(row[None].numpy(), T).repeat(rows, 0) for T in (0.0, 1.0)}
+    for b in range(B):
+        T = float(temp[b])
+        pth, tok, close = ref.accept(p[T], [7, V - 1, V - 2], parents, u[b].numpy(), noise.numpy(), None, T == 0)
+        if not close:
+            assert (n[b], nxt[b]) == (len(pth) - 1, tok), (b, T)
+            assert path[b] == pth + [-1] * (rows - len(pth))
