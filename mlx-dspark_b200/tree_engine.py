@@ -82,10 +82,10 @@ class TreeSpec:
         if temperature is None:
             temperature = torch.zeros(self.B, device=ids.device)
         meta = tree.pack(cu_rows, parent, self.lens, R, self.max_nodes, kv_start=self.kv_start)
-        logits = self.forward(ids, meta, cu_rows)
-        self.lens.copy_(meta["kv_len_new"])
+        logits, lens = self.forward(ids, meta, cu_rows), meta["kv_len_new"]
         out = sampling.sample_accept(logits, ids, cu_rows, u, noise, temperature=temperature,
                                      draft_probs=draft_probs, parent=parent, max_rows=self.max_nodes,
-                                     lens=self.lens)
-        self.keeper.keep(out["path"], cu_rows, out["n"], self.lens, kv_start=self.kv_start)
+                                     lens=lens)
+        self.keeper.keep(out["path"], cu_rows, out["n"], lens, kv_start=self.kv_start)
+        out["lens"] = self.lens.copy_(lens)  # last: a call refused on the way leaves the slots as they were
         return out

@@ -56,3 +56,42 @@ def test_sample_accept_widest_slices(cuda, form, V):
         if not close:
             assert (n[b], nxt[b]) == (len(pth) - 1, tok), (b, T)
             assert path[b] == pth + [-1] * (rows - len(pth))
+
+
+# ----------------------------------------------------------------- engine
+
+def _engine(dev, max_nodes=8, **kw):
+    from mlx_dspark_b200.target import Target, tiny_config
+    from mlx_dspark_b200.tree_engine import TreeSpec
+
+    t = Target(tiny_config(), seed=3, max_rows=40, **(kw or dict(kv_cap=200, slots=3)))
+    return t, TreeSpec(t, max_nodes)
+
+
+def test_a_refused_step_leaves_the_slots_as_they_were(cuda):
+    from mlx_dspark_b200 import DSparkError, DSparkUnsupported
+
+    t, eng = _engine(cuda)
+    V, counts = t.cfg.vocab, [5, 0, 3]
+    g = torch.Generator().manual_seed(2)
+    ids = torch.randint(0, V, (8,), generator=g, dtype=torch.int32).to(cuda)
+    cu, par = _cu(counts, cuda), _i32([-1, 0, 0, 1, 1, -1, 0, 1], cuda)
+    u, noise = torch.rand(8, generator=g).to(cuda), torch.empty(3, V).exponential_(generator=g).to(cuda)
+    temp = torch.ones(3, device=cuda)
+    start = _i32([9, 20, 31], cuda)
+
+    def step(u=u, noise=noise, **kw):
+        return eng.step(ids, cu, u, noise, temperature=temp, **{"parent": par, **kw})
+
+    eng.lens.copy_(start)
+    want = [step()[k].tolist() for k in ("n", "next", "path")], eng.lens.tolist()
+    assert want[1] != start.tolist()
+    eng.lens.copy_(start)
+    q = torch.full((8, V), 1.0 / V, device=cuda)
+    with pytest.raises(DSparkUnsupported):
+        step(draft_probs=q)  # a tree has none
+    for bad in (dict(noise=noise[:2]), dict(noise=noise.double()), dict(u=u.double()), dict(u=u[:7])):
+        with pytest.raises(DSparkError):
+            step(**bad)
+    assert eng.lens.tolist() == start.tolist()
+    assert ([step()[k].tolist() for k in ("n", "next", "path")], eng.lens.tolist()) == want
