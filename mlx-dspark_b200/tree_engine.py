@@ -21,9 +21,9 @@ from .rope import RopeTable
 
 
 class TreeSpec:
-    """``max_nodes`` bounds the nodes of a slot's tree (its root, the pending token, among them); a step
-    holds up to ``target.max_rows`` nodes. ``rope`` replaces the target's rotary form (default: its
-    own)."""
+    """``max_nodes`` bounds the nodes of a slot's tree (its root, the pending token, among them; up to 1024
+    in :meth:`step`, the accept's limit); a step holds up to ``target.max_rows`` nodes. ``rope`` replaces
+    the target's rotary form (default: its own)."""
 
     def __init__(self, target, max_nodes: int, *, rope: RopeTable | None = None):
         t, c = target, target.cfg
@@ -51,17 +51,27 @@ class TreeSpec:
     def forward(self, ids: torch.Tensor, meta: dict, cu_rows: torch.Tensor,
                 logits: torch.Tensor | None = None) -> torch.Tensor:
         """Logits ``[R, vocab]`` of packed nodes ``ids`` (int32 ``[R]``); appends their K/V at the slots
-        that ``meta`` (:func:`.tree.pack`) gives."""
+        that ``meta`` (:func:`.tree.pack` of as many rows) gives. ``logits``: bf16, ``R`` rows of the
+        vocabulary or more (default: the target's)."""
         t, c, R = self.t, self.t.cfg, ids.numel()
         if not 1 <= R <= t.max_rows:
             raise _lib.DSparkUnsupported(_lib.ERR_UNSUPPORTED, f"{R} rows (1..{t.max_rows})")
-        stream = on_device(ids, cu_rows, *meta.values())
+        stream = on_device(ids, cu_rows, logits, *meta.values())
+        if logits is not None and (logits.dtype is not torch.bfloat16 or logits.ndim != 2 or logits.shape[0] < R or
+                                   logits.shape[1] != c.vocab or logits.stride(1) != 1 or
+                                   (R > 1 and logits.stride(0) < c.vocab)):
+            raise _lib.DSparkError(_lib.ERR_ARG, f"logits {logits.dtype} {tuple(logits.shape)}: bf16 [{R}, {c.vocab}] "
+                                   "with contiguous rows")
+        anc = meta["anc"]
+        if anc.ndim != 2 or anc.shape[0] != R:
+            raise _lib.DSparkError(_lib.ERR_ARG, f"anc {tuple(anc.shape)} for {R} rows")
         cache = self.k_caches[0]
         fwd = _lib.TreeFwd(
-            int32("cu_rows", cu_rows, self.B + 1), ptr(meta["row_pos"]), ptr(meta["row_slot"]),
-            ptr(meta["row_req"]), ptr(meta["kv_len_new"]), ptr(self.kv_start), ptr(meta["anc"]),
+            int32("cu_rows", cu_rows, self.B + 1), int32("row_pos", meta["row_pos"], R),
+            int32("row_slot", meta["row_slot"], R), int32("row_req", meta["row_req"], R),
+            int32("kv_len_new", meta["kv_len_new"], self.B), ptr(self.kv_start), int32("anc", anc),
             self.rope.freq_ptr, ptr(self.qkv), ptr(self.attn_ws), self.attn_ws.numel(), cache.stride(0),
-            self.rope.mscale, meta["anc"].shape[1], self.max_nodes, self.rope.layout_code,
+            self.rope.mscale, anc.shape[1], self.max_nodes, self.rope.layout_code,
             self.rope.rotary_dim, cache.shape[2], cache.shape[0])
         out = t.logits if logits is None else logits
         _lib.check(_lib.lib.dspark_tree_forward(

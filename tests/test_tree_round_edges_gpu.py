@@ -95,3 +95,35 @@ def test_a_refused_step_leaves_the_slots_as_they_were(cuda):
             step(**bad)
     assert eng.lens.tolist() == start.tolist()
     assert ([step()[k].tolist() for k in ("n", "next", "path")], eng.lens.tolist()) == want
+
+
+def test_forward_checks_what_its_kernels_index(cuda):
+    """Metadata of another round's size and buffers that the logits do not fit are refused."""
+    from mlx_dspark_b200 import DSparkError, tree
+
+    t, eng = _engine(cuda)
+    V = t.cfg.vocab
+    ids, cu = torch.zeros(6, dtype=torch.int32, device=cuda), _cu([4, 0, 2], cuda)
+    eng.lens.copy_(_i32([5, 6, 7], cuda))
+
+    def meta(**kw):
+        return {**tree.pack(cu, None, eng.lens, 6, 8), **kw}
+
+    want = eng.forward(ids, meta(), cu).clone()
+    short = tree.pack(_cu([3, 0, 2], cuda), None, eng.lens, 5, 8)
+    for k in ("row_pos", "row_slot", "row_req", "anc"):
+        with pytest.raises(DSparkError):
+            eng.forward(ids, meta(**{k: short[k]}), cu)
+    for k in ("row_slot", "anc", "kv_len_new"):
+        with pytest.raises(DSparkError):
+            eng.forward(ids, meta(**{k: meta()[k].long()}), cu)
+    for bad in (dict(kv_len_new=_i32([9, 6], cuda)), dict(anc=meta()["anc"].flatten())):
+        with pytest.raises(DSparkError):
+            eng.forward(ids, meta(**bad), cu)
+    for logits in (torch.empty(5, V, dtype=BF, device=cuda), torch.empty(6, V - 2, dtype=BF, device=cuda),
+                   torch.empty(6, V, device=cuda), torch.empty(V, 6, dtype=BF, device=cuda).t(),
+                   torch.empty(1, V, dtype=BF, device=cuda).expand(6, V), torch.empty(6, V, dtype=BF)):
+        with pytest.raises(DSparkError):
+            eng.forward(ids, meta(), cu, logits)
+    out = torch.empty(9, V + 8, dtype=BF, device=cuda)[:, :V]
+    assert torch.equal(eng.forward(ids, meta(), cu, out), want)
