@@ -478,10 +478,17 @@ int dspark_p2p_allgather(const dspark_p2p_gather_args* args, void* stream);
  * a row, bit j of word j / 32: place j). kv_len_new[b] = kv_len[b] + rows. With kv_start (a pool of
  * positions as one batch entry) row_slot counts from kv_start[b] and row_req is 0. parent may be NULL
  * (each block a chain). A row whose parent is not before it counts as a second root. Outputs may
- * be NULL. Rows of a request beyond 32 * anc_words get no bits of those places. */
+ * be NULL. Rows of a request beyond 32 * anc_words get no bits of those places.
+ * dspark_tree_pack_capped also takes kv_cap [B], the positions that request b may fill: a row past them
+ * has row_slot -1 (dspark_rope_append drops and records it), and room[b] (or NULL) is the number of
+ * rows that fit, for dspark_sample_args.row_limit. */
 int dspark_tree_pack(const int32_t* cu_rows, const int32_t* parent, const int32_t* kv_len,
                      const int32_t* kv_start, int B, int R, int32_t* row_pos, int32_t* row_slot, int32_t* row_req, uint32_t* anc,
                      int anc_words, int32_t* kv_len_new, void* stream);
+int dspark_tree_pack_capped(const int32_t* cu_rows, const int32_t* parent, const int32_t* kv_len,
+                            const int32_t* kv_start, const int32_t* kv_cap, int B, int R, int32_t* row_pos,
+                            int32_t* row_slot, int32_t* row_req, uint32_t* anc, int anc_words,
+                            int32_t* kv_len_new, int32_t* room, void* stream);
 
 #define DSPARK_ROPE_HALF 0         /* pairs (i, i + rot / 2) */
 #define DSPARK_ROPE_INTERLEAVED 1  /* pairs (2 i, 2 i + 1) */
@@ -565,7 +572,8 @@ size_t dspark_tree_attn_workspace(int B, int Hq, int Hk, int D, int max_rows);
  * A request without rows: n 0, next -1, length kept. Logits -inf or NaN have probability 0, +inf
  * counts as the largest finite value; a row with no mass accepts nothing and gives next -1.
  * logits bf16, fp16 or fp32, draft bf16, fp16 or fp32 (draft_dtype). max_rows bounds the rows of a
- * request (<= 1024); rows beyond it are not accepted. */
+ * request (<= 1024); rows beyond it, or beyond row_limit[b], are not accepted and count as not tried. A
+ * request whose limit leaves no row: n 0, next -1, path -1, prob 0, all its rows rejected. */
 #define DSPARK_DTYPE_F32 2
 typedef struct {
   const void* logits;
@@ -586,6 +594,7 @@ typedef struct {
   size_t ws_bytes;
   int dtype, draft_dtype;
   int R, B, V, max_rows;
+  const int32_t* row_limit;  /* [B] or NULL */
 } dspark_sample_args;
 
 int dspark_sample_accept(const dspark_sample_args* a, void* stream);

@@ -130,7 +130,7 @@ class SampleArgs(C.Structure):
                 ("noise", vp), ("temperature", vp), ("n_accept", vp), ("next_tok", vp),
                 ("prob", vp), ("path", vp), ("lens", vp), ("workspace", vp), ("ws_bytes", sz),
                 ("dtype", i32), ("draft_dtype", i32), ("R", i32), ("B", i32), ("V", i32),
-                ("max_rows", i32)]
+                ("max_rows", i32), ("row_limit", vp)]
 
 
 def packer(cls):
@@ -201,6 +201,7 @@ _SIGS = {
                                     i32, vp, i64, vp]),
     "dspark_verify_prepare": (i32, [vp, i32, C.POINTER(FwdBuffers), vp]),
     "dspark_tree_pack": (i32, [vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, i32, vp, vp]),
+    "dspark_tree_pack_capped": (i32, [vp, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, i32, vp, vp, vp]),
     "dspark_tree_forward": (i32, [C.POINTER(Model), C.POINTER(FwdBuffers), C.POINTER(TreeFwd), vp, i32,
                                   i32, vp, i64, vp]),
     "dspark_rope_append": (i32, [vp, vp]),

@@ -381,7 +381,21 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
     }
     return;
   }
-  const int seen = min(rows, a.max_rows);  // rows that can be accepted
+  int seen = min(rows, a.max_rows);  // rows that can be accepted
+  if (a.row_limit) seen = min(seen, a.row_limit[b]);
+  if (seen <= 0) {
+    if (!lead) return;
+    for (int i = tid; i < rows; i += THREADS) {
+      if (a.path) a.path[r0 + i] = -1;
+      if (a.prob) a.prob[r0 + i] = 0.f;
+    }
+    if (tid == 0) {
+      a.n_accept[b] = 0;
+      a.next_tok[b] = -1;
+      if (a.lens) a.lens[b] = max(0, a.lens[b] - rows);
+    }
+    return;
+  }
   const float temp = a.temperature ? a.temperature[b] : 1.f;
   const bool arg = greedy(temp);
   const float c = arg ? 0.f : slope(temp);

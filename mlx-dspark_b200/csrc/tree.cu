@@ -9,16 +9,19 @@ namespace tree {
 // One block a request, one thread a row: the row walks up its ancestors (places descend, so the
 // words of its bit row are finished from the top down).
 __global__ void __launch_bounds__(256) pack_kernel(const int32_t* cu, const int32_t* parent,
-                                                   const int32_t* kv_len, const int32_t* kv_start, int R,
-                                                   int32_t* row_pos,
+                                                   const int32_t* kv_len, const int32_t* kv_start,
+                                                   const int32_t* kv_cap, int R, int32_t* row_pos,
                                                    int32_t* row_slot, int32_t* row_req,
-                                                   uint32_t* anc, int words, int32_t* kv_len_new) {
+                                                   uint32_t* anc, int words, int32_t* kv_len_new,
+                                                   int32_t* room) {
   pdl_launch_dependents();
   pdl_wait();
   const int b = blockIdx.x;
   const int r0 = min(max(cu[b], 0), R), r1 = min(max(cu[b + 1], r0), R);
   const int L0 = kv_len[b];
+  const int fit = kv_cap ? min(max(kv_cap[b] - L0, 0), r1 - r0) : r1 - r0;  // rows that have a place
   if (threadIdx.x == 0 && kv_len_new) kv_len_new[b] = L0 + (r1 - r0);
+  if (threadIdx.x == 0 && room) room[b] = fit;
   for (int i = threadIdx.x; i < r1 - r0; i += blockDim.x) {
     const int r = r0 + i;
     int depth = 0;
@@ -54,7 +57,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const int32_t* cu, const int3
       }
     }
     if (row_pos) row_pos[r] = L0 + depth;
-    if (row_slot) row_slot[r] = L0 + i + (kv_start ? kv_start[b] : 0);
+    if (row_slot) row_slot[r] = i < fit ? L0 + i + (kv_start ? kv_start[b] : 0) : -1;
     if (row_req) row_req[r] = kv_start ? 0 : b;
   }
 }
@@ -116,13 +119,22 @@ extern "C" {
 int dspark_tree_pack(const int32_t* cu_rows, const int32_t* parent, const int32_t* kv_len,
                      const int32_t* kv_start, int B, int R, int32_t* row_pos, int32_t* row_slot, int32_t* row_req, uint32_t* anc,
                      int anc_words, int32_t* kv_len_new, void* stream) {
+  return dspark_tree_pack_capped(cu_rows, parent, kv_len, kv_start, nullptr, B, R, row_pos, row_slot, row_req,
+                                 anc, anc_words, kv_len_new, nullptr, stream);
+}
+
+int dspark_tree_pack_capped(const int32_t* cu_rows, const int32_t* parent, const int32_t* kv_len,
+                            const int32_t* kv_start, const int32_t* kv_cap, int B, int R, int32_t* row_pos,
+                            int32_t* row_slot, int32_t* row_req, uint32_t* anc, int anc_words,
+                            int32_t* kv_len_new, int32_t* room, void* stream) {
   if (B < 0 || R < 0) return fail(DSPARK_ERR_ARG, "tree_pack: bad shape (%d requests, %d rows)", B, R);
   if (B == 0) return DSPARK_OK;
   if (!cu_rows || !kv_len) return fail(DSPARK_ERR_ARG, "tree_pack: null pointer");
   if (anc && anc_words <= 0) return fail(DSPARK_ERR_ARG, "tree_pack: %d words a row", anc_words);
   DSPARK_CUDA_TRY(launch_ex(tree::pack_kernel, dim3(B), dim3(256), 0,
                             reinterpret_cast<cudaStream_t>(stream), 1, true, cu_rows, parent, kv_len,
-                            kv_start, R, row_pos, row_slot, row_req, anc, anc_words, kv_len_new),
+                            kv_start, kv_cap, R, row_pos, row_slot, row_req, anc, anc_words, kv_len_new,
+                            room),
                   "tree_pack");
   return DSPARK_OK;
 }

@@ -45,7 +45,8 @@ def _f32(name: str, t: torch.Tensor | None, n: int) -> int:
 def sample_accept(logits: torch.Tensor, ids: torch.Tensor, cu_rows: torch.Tensor, u: torch.Tensor,
                   noise: torch.Tensor, *, temperature: torch.Tensor | None = None,
                   draft_probs: torch.Tensor | None = None, parent: torch.Tensor | None = None,
-                  max_rows: int, lens: torch.Tensor | None = None, out: dict | None = None) -> dict:
+                  max_rows: int, row_limit: torch.Tensor | None = None, lens: torch.Tensor | None = None,
+                  out: dict | None = None) -> dict:
     """Accept each request's block against ``p = softmax(logits / T)``.
 
     ``logits [R, V]`` (bf16, fp16 or fp32), ``ids`` int32 ``[R]`` (each block's pending token, then its
@@ -63,9 +64,11 @@ def sample_accept(logits: torch.Tensor, ids: torch.Tensor, cu_rows: torch.Tensor
     drafts), ``next``, ``prob`` (p of each row's token given its parent, 1 for roots) and ``path``
     (kept places of each request in order, then -1); ``out``, a former call's result for as many rows and
     requests, is written again (its workspace too, on one stream). ``lens`` (int32 ``[B]``, tokens cached after the
-    verify's append) loses the rejected rows in place. ``max_rows`` (<= 1024) bounds a block."""
+    verify's append) loses the rejected rows in place. ``max_rows`` (<= 1024) bounds a block, ``row_limit``
+    (int32 ``[B]``) the rows of each that can be accepted: the others count as not tried, and a block of
+    which no row can gives n 0, next -1 and loses all its rows."""
     given = () if out is None else (out["n"], out["next"], out["prob"], out["path"])
-    stream = on_device(logits, ids, cu_rows, u, noise, temperature, draft_probs, parent, lens, *given)
+    stream = on_device(logits, ids, cu_rows, u, noise, temperature, draft_probs, parent, row_limit, lens, *given)
     R, B = ids.numel(), cu_rows.numel() - 1
     V = logits.shape[-1]
     ld, ld_noise = _rows_of("logits", logits, R, V), _rows_of("noise", noise, B, V)
@@ -94,6 +97,6 @@ def sample_accept(logits: torch.Tensor, ids: torch.Tensor, cu_rows: torch.Tensor
         int32("parent", parent, R), _f32("u", u, R), noise.data_ptr(), _f32("temperature", temperature, B),
         int32("n", out["n"], B), int32("next", out["next"], B), _f32("prob", out["prob"], R),
         int32("path", out["path"], R), int32("lens", lens, B), ws.data_ptr() if n else 0, n, dt, ddt, R, B, V,
-        max_rows), stream))
+        max_rows, int32("row_limit", row_limit, B)), stream))
     out["lens"] = lens
     return out

@@ -33,13 +33,16 @@ def anc_words(max_nodes: int) -> int:
 
 
 def pack(cu_rows: torch.Tensor, parent: torch.Tensor | None, kv_len: torch.Tensor, n_rows: int,
-         max_nodes: int, kv_start: torch.Tensor | None = None, out: dict | None = None) -> dict:
+         max_nodes: int, kv_start: torch.Tensor | None = None, out: dict | None = None,
+         kv_cap: torch.Tensor | None = None) -> dict:
     """Device-side metadata of one packed round: ``row_pos`` (cached tokens + depth), ``row_slot``
     (cached tokens + place), ``row_req``, ``anc`` (int32 ``[R, words]`` bit rows of each node and its
     ancestors) and ``kv_len_new``. ``kv_len`` int32 ``[B]``: tokens cached before the round;
     ``parent`` int32 ``[R]``: places within the request, -1 for the root (``None``: chains).
-    With ``kv_start`` (a position-major pool) the slots count from it and ``row_req`` is 0."""
-    stream = on_device(cu_rows, parent, kv_len, kv_start)
+    With ``kv_start`` (a position-major pool) the slots count from it and ``row_req`` is 0. With ``kv_cap``
+    (int32 ``[B]``: positions each request may fill) rows past it have slot -1, and ``room`` (``[B]``)
+    tells how many rows fit."""
+    stream = on_device(cu_rows, parent, kv_len, kv_start, kv_cap)
     R, B = int(n_rows), kv_len.numel()
     words = anc_words(max_nodes)
     if out is None:
@@ -47,14 +50,16 @@ def pack(cu_rows: torch.Tensor, parent: torch.Tensor | None, kv_len: torch.Tenso
         out = {"row_pos": torch.empty(R, **e), "row_slot": torch.empty(R, **e),
                "row_req": torch.empty(R, **e), "anc": torch.empty((R, words), **e),
                "kv_len_new": torch.empty(B, **e)}
+        if kv_cap is not None:
+            out["room"] = torch.empty(B, **e)
     else:
         on_device(cu_rows, *out.values())
     at = {k: int32(k, out[k], n) for k, n in (("row_pos", R), ("row_slot", R), ("row_req", R),
                                               ("anc", R * words), ("kv_len_new", B))}
-    _lib.check(_lib.lib.dspark_tree_pack(
+    _lib.check(_lib.lib.dspark_tree_pack_capped(
         int32("cu_rows", cu_rows, B + 1), int32("parent", parent, R), int32("kv_len", kv_len),
-        int32("kv_start", kv_start, B), B, R, at["row_pos"], at["row_slot"],
-        at["row_req"], at["anc"], words, at["kv_len_new"], stream))
+        int32("kv_start", kv_start, B), int32("kv_cap", kv_cap, B), B, R, at["row_pos"], at["row_slot"],
+        at["row_req"], at["anc"], words, at["kv_len_new"], int32("room", out.get("room"), B), stream))
     return out
 
 

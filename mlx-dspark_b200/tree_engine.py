@@ -43,15 +43,21 @@ class TreeSpec:
         self.kv_start = None
         if t.position_major:
             self.kv_start = torch.tensor(t._slot_base, dtype=torch.int32, device=dev)
+        self.kv_cap = torch.tensor(t.slot_caps, dtype=torch.int32, device=dev)
         R = t.max_rows
         self.qkv = torch.empty((R, (c.n_heads + 2 * c.n_kv_heads) * c.head_dim), dtype=torch.bfloat16, device=dev)
         n = int(_lib.lib.dspark_tree_attn_workspace(self.B, c.n_heads, c.n_kv_heads, c.head_dim, self.max_nodes))
         self.attn_ws = torch.empty(n, dtype=torch.uint8, device=dev)
 
+    def pack(self, cu_rows: torch.Tensor, parent: torch.Tensor | None, n_rows: int) -> dict:
+        """:func:`.tree.pack` of a round over the slots as they are, bounded by each slot's capacity."""
+        return tree.pack(cu_rows, parent, self.lens, n_rows, self.max_nodes, kv_start=self.kv_start,
+                         kv_cap=self.kv_cap)
+
     def forward(self, ids: torch.Tensor, meta: dict, cu_rows: torch.Tensor,
                 logits: torch.Tensor | None = None) -> torch.Tensor:
         """Logits ``[R, vocab]`` of packed nodes ``ids`` (int32 ``[R]``); appends their K/V at the slots
-        that ``meta`` (:func:`.tree.pack` of as many rows) gives. ``logits``: bf16, ``R`` rows of the
+        that ``meta`` (:meth:`pack` of as many rows) gives. ``logits``: bf16, ``R`` rows of the
         vocabulary or more (default: the target's)."""
         t, c, R = self.t, self.t.cfg, ids.numel()
         if not 1 <= R <= t.max_rows:
@@ -87,15 +93,17 @@ class TreeSpec:
         int32 ``[R]`` as in :func:`.tree.pack` (``None``: chains); ``u``, ``noise``, ``temperature``
         (``None``: greedy) and ``draft_probs`` as in :func:`.sampling.sample_accept`. Returns its
         ``n``, ``next``, ``prob`` and ``path``; ``lens`` and the caches move on to the accepted tokens,
-        and ``next`` is each slot's new pending token. A slot's nodes must fit in its capacity."""
+        and ``next`` is each slot's new pending token. Nodes past their slot's capacity are neither cached
+        nor accepted, and the device status records them; a slot without room for its pending token stays
+        as it is and has ``next`` -1."""
         R = ids.numel()
         if temperature is None:
             temperature = torch.zeros(self.B, device=ids.device)
-        meta = tree.pack(cu_rows, parent, self.lens, R, self.max_nodes, kv_start=self.kv_start)
+        meta = self.pack(cu_rows, parent, R)
         logits, lens = self.forward(ids, meta, cu_rows), meta["kv_len_new"]
         out = sampling.sample_accept(logits, ids, cu_rows, u, noise, temperature=temperature,
                                      draft_probs=draft_probs, parent=parent, max_rows=self.max_nodes,
-                                     lens=lens)
+                                     row_limit=meta["room"], lens=lens)
         self.keeper.keep(out["path"], cu_rows, out["n"], lens, kv_start=self.kv_start)
         out["lens"] = self.lens.copy_(lens)  # last: a call refused on the way leaves the slots as they were
         return out

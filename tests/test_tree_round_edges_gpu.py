@@ -127,3 +127,115 @@ def test_forward_checks_what_its_kernels_index(cuda):
             eng.forward(ids, meta(), cu, logits)
     out = torch.empty(9, V + 8, dtype=BF, device=cuda)[:, :V]
     assert torch.equal(eng.forward(ids, meta(), cu, out), want)
+
+
+# ----------------------------------------------------------------- capacity
+
+def test_pack_marks_rows_past_the_capacity(cuda):
+    from mlx_dspark_b200 import tree
+
+    counts, lens, cap, start = [5, 4, 0, 3, 2], [7, 10, 1, 20, 6], [9, 10, 4, 12, 9], [0, 9, 19, 23, 35]
+    got = tree.pack(_cu(counts, cuda), None, _i32(lens, cuda), 14, 5, kv_start=_i32(start, cuda),
+                    kv_cap=_i32(cap, cuda))
+    assert got["room"].tolist() == [2, 0, 0, 0, 2]
+    assert got["row_slot"].tolist() == [7, 8] + [-1] * 10 + [41, 42]
+    assert got["kv_len_new"].tolist() == [12, 14, 1, 23, 8]
+
+
+@pytest.mark.parametrize("form", ["chain", "draft", "tree"])
+def test_sample_accept_row_limit(cuda, form):
+    """Rows past a request's limit count as not tried: the decisions of the block cut there."""
+    from mlx_dspark_b200 import sampling
+
+    V, n = 500, 9
+    limits = [9, 5, 1, 0, 2, 20, 3, -4]
+    B = len(limits)
+    rng = np.random.default_rng(1)
+    logits = torch.tensor(2 * rng.standard_normal((B * n, V)), dtype=torch.float32)
+    ids = logits.reshape(B, n, V).argsort(-1)[:, :, -1].roll(1, 1).contiguous()  # a row's favourite next
+    parent = [-1, 0, 0, 1, 2, 2, 3, 4, 4]
+    if form == "tree":
+        top = logits.reshape(B, n, V).argsort(-1, descending=True)
+        for i in range(1, n):
+            ids[:, i] = top[:, parent[i], i % 3]
+    q = None
+    if form == "draft":
+        q = torch.softmax(logits + torch.tensor(rng.standard_normal((B * n, V)), dtype=torch.float32), -1)
+    u = torch.tensor(0.6 * rng.random(B * n), dtype=torch.float32)
+    noise = torch.tensor(rng.exponential(size=(B, V)), dtype=torch.float32)
+    lens = _i32([50] * B, cuda)
+    got = sampling.sample_accept(
+        logits.to(cuda), _i32(ids.flatten().tolist(), cuda), _cu([n] * B, cuda), u.to(cuda), noise.to(cuda),
+        draft_probs=None if q is None else q.to(cuda), parent=_i32(parent * B, cuda) if form == "tree" else None,
+        max_rows=n, row_limit=_i32(limits, cuda), lens=lens)
+    path = got["path"].view(B, n).tolist()
+    for b, lim in enumerate(limits):
+        if lim <= 0:
+            assert (int(got["n"][b]), int(got["next"][b]), int(lens[b])) == (0, -1, 50 - n)
+            assert path[b] == [-1] * n and got["prob"][b * n : (b + 1) * n].tolist() == [0.0] * n
+            continue
+        rows, lim = slice(b * n, (b + 1) * n), min(lim, n)
+        p = ref.probabilities(logits[rows].numpy(), 1.0)
+        pth, tok, close = ref.accept(p[:lim], ids[b, :lim].tolist(), parent[:lim] if form == "tree" else None,
+                                     u[rows].numpy(), noise[b].numpy(),
+                                     None if q is None else q[rows].numpy()[:lim], False)
+        assert not close
+        assert (int(got["n"][b]), int(got["next"][b]), int(lens[b])) == (len(pth) - 1, tok, 50 - n + len(pth))
+        assert path[b] == pth + [-1] * (n - len(pth))
+
+
+@pytest.mark.parametrize("position_major", [False, True])
+def test_a_tree_past_its_slots_end_stays_in_its_slot(cuda, position_major):
+    """Slot 0 has room for two of five nodes, then for none: nothing of its neighbours moves, what does not
+    fit is not accepted, and the device status tells."""
+    from mlx_dspark_b200 import _lib
+
+    caps = [40, 40, 40]
+    t, eng = _engine(cuda, **(dict(slot_caps=caps) if position_major else dict(kv_cap=40, slots=3)))
+    big, wide = _engine(cuda, **(dict(slot_caps=[90, 90, 90]) if position_major else dict(kv_cap=90, slots=3)))
+    start = [38, 3, 20]
+    g = torch.Generator(device=cuda).manual_seed(5)
+    for li in range(len(t.layers)):
+        for w in "kv":
+            for b in range(3):
+                x = torch.randn((t.cfg.n_kv_heads, 40, t.cfg.head_dim), device=cuda, generator=g).to(BF)
+                t.slot_view(li, b, w)[:] = x
+                big.slot_view(li, b, w)[:, :40] = x
+    before = [[t.slot_view(li, b, w).clone() for b in range(3)] for li in range(len(t.layers)) for w in "kv"]
+    V, counts = t.cfg.vocab, [5, 3, 0]
+    ids = torch.randint(0, V, (8,), device=cuda, dtype=torch.int32, generator=g)
+    cu, par = _cu(counts, cuda), _i32([-1, 0, 1, 2, 2, -1, 0, 0], cuda)
+    u, noise = torch.zeros(8, device=cuda), torch.empty(3, V, device=cuda).exponential_(generator=g)
+    temp = torch.full((3,), 50.0, device=cuda)  # u of zero: any tried token is accepted
+
+    def step(e):
+        return e.step(ids, cu, u, noise, parent=par, temperature=temp)
+
+    wide.lens.copy_(_i32(start, cuda))
+    all_fit = step(wide)
+    assert all_fit["n"].tolist() == [3, 1, 0] and _lib.device_status(cuda.index) == 0
+    eng.lens.copy_(_i32(start, cuda))
+    out = step(eng)
+    assert _lib.device_status(cuda.index) == 0x203  # recorded, and cleared by reading
+    assert out["n"].tolist() == [1, 1, 0] and eng.lens.tolist() == [40, 5, 20]
+    assert out["path"].tolist() == [0, 1, -1, -1, -1, 0, 1, -1]
+    assert int(out["next"][1]) == int(all_fit["next"][1])
+    assert int(out["next"][0]) >= 0 and int(out["next"][2]) == -1
+    i = 0
+    for li in range(len(t.layers)):
+        for w in "kv":
+            now = [t.slot_view(li, b, w) for b in range(3)]
+            assert torch.equal(now[0][:, :38], before[i][0][:, :38])
+            assert torch.equal(now[0][:, 38:], big.slot_view(li, 0, w)[:, 38:40])
+            assert torch.equal(now[1][:, :3], before[i][1][:, :3])
+            assert torch.equal(now[1][:, 3:5], big.slot_view(li, 1, w)[:, 3:5])
+            assert torch.equal(now[1][:, 6:], before[i][1][:, 6:]) and torch.equal(now[2], before[i][2])
+            i += 1
+    state = [t.slot_view(li, 0, w).clone() for li in range(len(t.layers)) for w in "kv"]
+    out = step(eng)  # no room at all: the slot stays, the other one goes on
+    assert _lib.device_status(cuda.index) != 0
+    assert out["n"].tolist()[0] == 0 and int(out["next"][0]) == -1 and eng.lens.tolist() == [40, 7, 20]
+    for x, y in zip(state, (t.slot_view(li, 0, w) for li in range(len(t.layers)) for w in "kv")):
+        assert torch.equal(x, y)
+    assert all(torch.equal(t.slot_view(li, 2, w), before[2 * li + (w == "v")][2])
+               for li in range(len(t.layers)) for w in "kv")
