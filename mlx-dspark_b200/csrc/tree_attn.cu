@@ -501,21 +501,32 @@ struct Cut {
 constexpr int MAX_CTA = 160;
 
 // The workspace: a count a CTA (of the item whose first part it has), two flags a CTA (of its parts),
-// then part `which` of CTA c: D values (divided by the part's sum) and the logarithm of the sum, m + log2 l, of 256 rows (row
+// the number of failures, then part `which` of CTA c: D values (divided by the part's sum) and the logarithm of the sum, m + log2 l, of 256 rows (row
 // innermost, as a warp of 32 rows writes them). An item's first part is its CTA's part 1, the others
 // are part 0.
+// words before the parts, which begin on a 128-byte line (off one, 61 nodes over 16k: 36.6 us for 35.0)
+constexpr int HEAD = 3 * MAX_CTA + 16;
 template <int D>
 __device__ __forceinline__ float* part(void* ws, int c, int which) {
-  return reinterpret_cast<float*>(static_cast<uint64_t*>(ws) + 3 * MAX_CTA) +
+  return reinterpret_cast<float*>(static_cast<uint64_t*>(ws) + HEAD) +
          int64_t(2 * c + which) * (2 * ROWS) * (D + 1);
 }
 
-// Flags and counts live in memory that nobody clears beforehand: a flag is up when it is this launch's
-// tag, a count without the tag is zero. A flag costs its writer no answer from L2; a count of the parts
+// Flags and counts live in memory that nobody clears beforehand: a flag is up when it is this run's
+// tag, a count without the tag is zero. The tag is the launch's own, changed by the number of failures in the
+// workspace: a replayed launch has the same, and after a wait that ran out flags may be left up and counts
+// short. Whoever sees such a wait adds one to that number (any start value will do), so that the next
+// run takes no flag of this one for its own. A flag costs its writer no answer from L2; a count of the parts
 // took three (1.3 us). The last of an item's CTAs to say that it has seen all flags puts zeros back,
 // so that a replayed launch (same tag) starts anew.
 __device__ __forceinline__ uint64_t* flag_of(void* ws, int c, int which) {
   return static_cast<uint64_t*>(ws) + MAX_CTA + 2 * c + which;
+}
+__device__ __forceinline__ unsigned long long* failures_of(void* ws) {
+  return static_cast<unsigned long long*>(ws) + 3 * MAX_CTA;
+}
+__device__ __forceinline__ uint64_t run_tag(uint64_t tag, uint64_t failures) {
+  return (tag ^ (failures << 16)) | 1ull << 63;  // the low 16 bits stay zero: a count's
 }
 __device__ __forceinline__ void seen_all(void* ws, int first, int parts, uint64_t tag) {
   unsigned long long* p = static_cast<unsigned long long*>(ws) + first;
@@ -528,15 +539,15 @@ __device__ __forceinline__ void seen_all(void* ws, int first, int parts, uint64_
   *reinterpret_cast<volatile unsigned long long*>(p) = 0;
   for (int x = 0; x < parts; ++x) *reinterpret_cast<volatile uint64_t*>(flag_of(ws, first + x, x == 0)) = 0;
 }
-__device__ __forceinline__ void wait_flag(const uint64_t* word, uint64_t tag, int* status) {
+__device__ __forceinline__ bool wait_flag(const uint64_t* word, uint64_t tag, int* status) {
   const uint64_t t0 = globaltimer_ns(), limit = wait_limit_ns(status);
   while (true) {
     uint64_t v;
     asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(word) : "memory");
-    if (v == tag) return;
+    if (v == tag) return true;
     if (globaltimer_ns() - t0 > limit) {
       report_error(status, kErrWaitPeer);
-      return;
+      return false;
     }
   }
 }
@@ -556,7 +567,8 @@ __device__ __noinline__ void show_and_wait(void* workspace, const Cut* cuts, int
   __syncwarp();
   for (int k = 0; k < n_cuts; ++k) {
     const int first = cuts[k].first, parts = cuts[k].parts;
-    for (int x = lane; x < parts; x += 32) wait_flag(flag_of(workspace, first + x, x == 0), tag, status);
+    for (int x = lane; x < parts; x += 32)
+      if (!wait_flag(flag_of(workspace, first + x, x == 0), tag, status)) atomicAdd(failures_of(workspace), 1ull);
     named_sync(4, 288);
     if (lane == 0) seen_all(workspace, first, parts, tag);
     __syncwarp();
@@ -1021,6 +1033,7 @@ __global__ void __launch_bounds__(NTHR, 1)
       __syncwarp();
     } else if (warp == WARP_TMA) {
       // -------------------------------------------------------------- producer
+      const uint64_t failures = *reinterpret_cast<volatile unsigned long long*>(failures_of(a.workspace));
       if (lane == 0) {
         int g = 0;
         auto load = [&](const CUtensorMap* map, int tile) {
@@ -1045,12 +1058,15 @@ __global__ void __launch_bounds__(NTHR, 1)
             if (t + ahead < n) load(&kmap, t + ahead);
           }
         }
-        // no copy may still be in flight when the CTA exits
-        for (int i = max(0, g - NB); i < g; ++i)
-          mbar_wait(&full[i % NB], uint32_t(i / NB) & 1u, status, kErrWaitKV);
+        // no copy may still be in flight when the CTA exits (under the default limit, whatever is set)
+        for (int i = max(0, g - NB); i < g; ++i) mbar_wait(&full[i % NB], uint32_t(i / NB) & 1u, nullptr, 0);
       }
       __syncwarp();
-      if (named_all(4, 288, true) && *n_cuts) show_and_wait(a.workspace, cuts, *n_cuts, cta, tag, status);
+      if (!named_all(4, 288, true)) {
+        if (lane == 0) atomicAdd(failures_of(a.workspace), 1ull);
+      } else if (*n_cuts) {
+        show_and_wait(a.workspace, cuts, *n_cuts, cta, run_tag(tag, failures), status);
+      }
     } else if (warp == WARP_MMA) {
       // -------------------------------------------------------------- products
       // The whole warp walks and waits; one lane issues. What an instruction needs is then the same in
@@ -1172,7 +1188,7 @@ __global__ void __launch_bounds__(NTHR, 1)
       }
       if (issued) {  // nothing may write tensor memory after the CTA releases it
         commit(fin);
-        mbar_wait(fin, 0, status, kErrWaitMma);
+        mbar_wait(fin, 0, nullptr, 0);  // (under the default limit)
       }
       __syncwarp();
     }
@@ -1242,7 +1258,7 @@ extern "C" {
 
 size_t dspark_tree_attn_workspace(int B, int Hq, int Hk, int D, int max_rows) {
   if (B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || D <= 0 || max_rows <= 0) return 0;
-  return 3 * tattn::MAX_CTA * sizeof(uint64_t) +
+  return tattn::HEAD * sizeof(uint64_t) +
          size_t(tattn::grid_of(current_device())) * 2 * (2 * tattn::ROWS) * (D + 1) * sizeof(float);
 }
 

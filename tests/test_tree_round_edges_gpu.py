@@ -239,3 +239,81 @@ def test_a_tree_past_its_slots_end_stays_in_its_slot(cuda, position_major):
         assert torch.equal(x, y)
     assert all(torch.equal(t.slot_view(li, 2, w), before[2 * li + (w == "v")][2])
                for li in range(len(t.layers)) for w in "kv")
+
+
+# ----------------------------------------------------------------- attention
+
+U = {BF: 2.0 ** -8, HF: 2.0 ** -11}
+
+
+def _sees(parents, n, L, chain=False):
+    """bool [n, L] on the CPU: a request's cached keys and each row's ancestors."""
+    m = torch.ones(n, L, dtype=torch.bool)
+    m[:, L - n :] = torch.ones(n, n, dtype=torch.bool).tril() if chain else False
+    if not chain:
+        for i, a in enumerate(ref.ancestors(parents)):
+            m[i, [L - n + j for j in a]] = True
+    return m
+
+
+def _exact(q, kc, vc, sees, scale, dtype):
+    """One request in 64 bits on the GPU, and the bound of test_tree_round_gpu.py."""
+    n, hq, d = q.shape
+    hk, L = kc.shape[0], sees.shape[1]
+    z = torch.einsum("nhgd,hld->hgnl", q.double().view(n, hk, hq // hk, d), kc[:, :L].double()) * scale
+    w = torch.softmax(z.masked_fill(~sees.to(q.device), float("-inf")), -1)
+    v = vc[:, :L].double()
+    o = torch.einsum("hgnl,hld->nhgd", w, v).reshape(n, hq, d)
+    absum = torch.einsum("hgnl,hld->nhgd", w, v.abs()).reshape(n, hq, d)
+    tail = 2.0 ** -25 * v.abs().sum(1).amax() if dtype == HF else 0.0
+    return o, (U[dtype] + 1e-4) * absum + U[dtype] * o.abs() + tail + 1e-7
+
+
+def test_a_wait_that_runs_out_leaves_nothing_behind(cuda):
+    """A captured call whose waits run out tells so and returns; replayed with the usual limit on other
+    rows it is right, whatever flags and counts the former run has left."""
+    from mlx_dspark_b200 import _lib, tree
+
+    rng = random.Random(0)
+    B, Hq, Hk, D, nodes = 24, 16, 4, 128, 9
+    counts = [rng.randint(1, nodes) for _ in range(B)]
+    lens = [rng.randint(nodes, 6000) for _ in counts]
+    parents = [ref.random_parents(n, rng) for n in counts]
+    g = torch.Generator(device=cuda).manual_seed(1)
+    kc, vc = (torch.randn(B, Hk, max(lens), D, device=cuda, generator=g).to(BF) for _ in range(2))
+    rows = [torch.randn(sum(counts), Hq, D, device=cuda, generator=g).to(BF) for _ in range(2)]
+    anc = _i32([w for p in parents for w in ref.words_of(ref.ancestors(p), 1)], cuda)
+    want = []
+    for x in rows:
+        r0, parts = 0, []
+        for b, n in enumerate(counts):
+            parts.append(_exact(x[r0 : r0 + n], kc[b], vc[b], _sees(parents[b], n, lens[b]), D ** -0.5, BF))
+            r0 += n
+        want.append([torch.cat(t) for t in zip(*parts)])
+    q, out = rows[0].clone(), torch.empty_like(rows[0])
+    args = (q, kc, vc, _cu(counts, cuda), _i32(lens, cuda), anc)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        tree.tree_sdpa(*args, scale=D ** -0.5, max_nodes=nodes, out=out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            tree.tree_sdpa(*args, scale=D ** -0.5, max_nodes=nodes, out=out)
+    torch.cuda.synchronize()
+    ran_out = 0
+    for k, limit_ns in enumerate((0, 300, 1000, 2000, 4000, 8000, 16000)):
+        if limit_ns:
+            _lib.set_wait_limit_ns(cuda.index, limit_ns)
+            try:
+                graph.replay()
+                torch.cuda.synchronize()
+            finally:
+                _lib.set_wait_limit_ns(cuda.index, 0)
+            ran_out += _lib.device_status(cuda.index) != 0
+        q.copy_(rows[k % 2])
+        out.fill_(float("nan"))
+        graph.replay()
+        o, bound = want[k % 2]
+        assert ((out.double() - o).abs() <= bound).all(), limit_ns
+        assert _lib.device_status(cuda.index) == 0
+    assert ran_out
