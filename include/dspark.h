@@ -533,8 +533,8 @@ int dspark_rope_append(const dspark_rope_args* a, void* stream);
  * {batch, head, position}: request b's keys start at position kv_start[b] (or 0) of batch entry b,
  * or of entry 0 when kv_batch is 1. kv_len counts are cut at the cache's end. max_rows bounds
  * rows(b) (it only chooses the launch). bf16 or fp16, D 64 or 128, 16-byte aligned rows.
- * Scratch: dspark_tree_attn_workspace bytes, nothing to clear; calls that overlap on the GPU
- * need their own. */
+ * Scratch: dspark_tree_attn_workspace bytes, 16-byte aligned, nothing to clear; calls that overlap on the
+ * GPU need their own. */
 typedef struct {
   const void* q;
   const void* k;
@@ -571,7 +571,8 @@ size_t dspark_tree_attn_workspace(int B, int Hq, int Hk, int D, int max_rows);
  * -1 after; prob[r] = p_parent(ids[r]) (1 for a root); lens[b] (optional) loses the rejected rows.
  * A request without rows: n 0, next -1, length kept. Logits -inf or NaN have probability 0, +inf
  * counts as the largest finite value; a row with no mass accepts nothing and gives next -1.
- * logits bf16, fp16 or fp32, draft bf16, fp16 or fp32 (draft_dtype). max_rows bounds the rows of a
+ * logits bf16, fp16 or fp32, draft bf16, fp16 or fp32 (draft_dtype). Scratch: dspark_sample_workspace
+ * bytes, 16-byte aligned, nothing to clear. max_rows bounds the rows of a
  * request (<= 1024); rows beyond it, or beyond row_limit[b], are not accepted and count as not tried. A
  * request whose limit leaves no row: n 0, next -1, path -1, prob 0, all its rows rejected. */
 #define DSPARK_DTYPE_F32 2

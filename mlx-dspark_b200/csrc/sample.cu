@@ -745,6 +745,8 @@ int dspark_sample_accept(const dspark_sample_args* p, void* stream) {
     return fail(DSPARK_ERR_ARG, "sample_accept: rows of %d values overlap", a.V);
   if (a.ws_bytes < dspark_sample_workspace(a.R, a.B, a.V) || (a.R && !a.workspace))
     return fail(DSPARK_ERR_ARG, "sample_accept: workspace of %zu bytes", a.ws_bytes);
+  if (reinterpret_cast<uintptr_t>(a.workspace) % 16)
+    return fail(DSPARK_ERR_ARG, "sample_accept: the workspace must be 16-byte aligned");
   const int sms = sm_count(current_device());
   const int slices = sample::slices_of(a.R, a.V, a.dtype == DSPARK_DTYPE_F32 ? 4 : 2, a.parent != nullptr, sms), blocks = sample::blocks_of(a.B, a.V, sms);
   if (int64_t(a.R) * slices > 0x7fffffff || int64_t(a.B) * blocks > 0x7fffffff)

@@ -1286,6 +1286,8 @@ int dspark_tree_attn(const dspark_tree_attn_args* p, void* stream) {
   if (!aligned) return fail(DSPARK_ERR_UNSUPPORTED, "tree_attn: rows must be 16-byte aligned");
   if (!a.workspace || a.ws_bytes < dspark_tree_attn_workspace(a.B, a.Hq, a.Hk, a.D, a.max_rows))
     return fail(DSPARK_ERR_ARG, "tree_attn: workspace of %zu bytes", a.ws_bytes);
+  if (reinterpret_cast<uintptr_t>(a.workspace) % 16)
+    return fail(DSPARK_ERR_ARG, "tree_attn: the workspace must be 16-byte aligned");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (a.dtype == DSPARK_DTYPE_BF16) return a.D == 128 ? tattn::launch<bf16, 128>(a, s) : tattn::launch<bf16, 64>(a, s);
   return a.D == 128 ? tattn::launch<__half, 128>(a, s) : tattn::launch<__half, 64>(a, s);
