@@ -478,7 +478,8 @@ int dspark_p2p_allgather(const dspark_p2p_gather_args* args, void* stream);
  * a row, bit j of word j / 32: place j). kv_len_new[b] = kv_len[b] + rows. With kv_start (a pool of
  * positions as one batch entry) row_slot counts from kv_start[b] and row_req is 0. parent may be NULL
  * (each block a chain). A row whose parent is not before it counts as a second root. Outputs may
- * be NULL. Rows of a request beyond 32 * anc_words get no bits of those places.
+ * be NULL. Rows of a request beyond 32 * anc_words get no bits of those places. Rows behind the last
+ * request's (cu_rows[B] .. R - 1) are nobody's: row_pos 0, row_slot and row_req -1, no bits.
  * dspark_tree_pack_capped also takes kv_cap [B], the positions that request b may fill: a row past them
  * has row_slot -1 (dspark_rope_append drops and records it), and room[b] (or NULL) is the number of
  * rows that fit, for dspark_sample_args.row_limit. */
@@ -500,7 +501,7 @@ int dspark_tree_pack_capped(const int32_t* cu_rows, const int32_t* parent, const
  * any length keep their phase to 2^-32 of a turn. Optional per-head RMS norm (q_norm / k_norm [D])
  * before the rotation. All in fp32, rounded once. Rotated k and v go to cache row
  * (row_req[r] or 0, head, row_slot[r]); a row outside the cache is not written and the device
- * status word records it. q_out may be q. k NULL (Hk 0): q alone. D % 16 == 0, D <= 512,
+ * status word records it (row_req -1: a row of no request, not written, no record). q_out may be q. k NULL (Hk 0): q alone. D % 16 == 0, D <= 512,
  * rot % 16 == 0, bf16 or fp16, head_dim contiguous. */
 typedef struct {
   const void* q;

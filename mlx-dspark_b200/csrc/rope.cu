@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const dspark_rope_args a,
   const int req = a.row_req ? a.row_req[r] : 0;
   const int slot = a.Hk ? a.row_slot[r] : 0;
   const bool fits = slot >= 0 && slot < a.cap && req >= 0 && req < a.batch;
-  if (a.Hk && !fits && lane == 0) report_error(status, 0x203);
+  if (a.Hk && !fits && req != -1 && lane == 0) report_error(status, 0x203);
   const int heads = a.Hq + (fits ? 2 * a.Hk : 0);
 
   auto source = [&](int h) {

@@ -10,7 +10,7 @@ namespace tree {
 // words of its bit row are finished from the top down).
 __global__ void __launch_bounds__(256) pack_kernel(const int32_t* cu, const int32_t* parent,
                                                    const int32_t* kv_len, const int32_t* kv_start,
-                                                   const int32_t* kv_cap, int R, int32_t* row_pos,
+                                                   const int32_t* kv_cap, int B, int R, int32_t* row_pos,
                                                    int32_t* row_slot, int32_t* row_req,
                                                    uint32_t* anc, int words, int32_t* kv_len_new,
                                                    int32_t* room) {
@@ -59,6 +59,16 @@ __global__ void __launch_bounds__(256) pack_kernel(const int32_t* cu, const int3
     if (row_pos) row_pos[r] = L0 + depth;
     if (row_slot) row_slot[r] = i < fit ? L0 + i + (kv_start ? kv_start[b] : 0) : -1;
     if (row_req) row_req[r] = kv_start ? 0 : b;
+  }
+  // rows behind the last request's: nobody's, so that nothing indexes with what the arrays held before
+  if (b == B - 1) {
+    for (int r = r1 + threadIdx.x; r < R; r += blockDim.x) {
+      if (row_pos) row_pos[r] = 0;
+      if (row_slot) row_slot[r] = -1;
+      if (row_req) row_req[r] = -1;
+      if (anc)
+        for (int w = 0; w < words; ++w) anc[int64_t(r) * words + w] = 0u;
+    }
   }
 }
 
@@ -133,7 +143,7 @@ int dspark_tree_pack_capped(const int32_t* cu_rows, const int32_t* parent, const
   if (anc && anc_words <= 0) return fail(DSPARK_ERR_ARG, "tree_pack: %d words a row", anc_words);
   DSPARK_CUDA_TRY(launch_ex(tree::pack_kernel, dim3(B), dim3(256), 0,
                             reinterpret_cast<cudaStream_t>(stream), 1, true, cu_rows, parent, kv_len,
-                            kv_start, kv_cap, R, row_pos, row_slot, row_req, anc, anc_words, kv_len_new,
+                            kv_start, kv_cap, B, R, row_pos, row_slot, row_req, anc, anc_words, kv_len_new,
                             room),
                   "tree_pack");
   return DSPARK_OK;

@@ -138,7 +138,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: RopeTa
     ``k`` and ``v`` to row ``row_slot[r]`` of batch entry ``row_req[r]`` (default 0) of the caches
     ``[B, Hk, cap, D]``. Returns the rotated q (``q_out``, which may be ``q``). All tensors may be
     strided views with head_dim contiguous. ``row_*`` are int32 ``[R]`` on the device; rows outside
-    the cache are dropped and recorded in the device status."""
+    the cache are dropped and recorded in the device status, rows of no request (``row_req`` -1) only
+    dropped."""
     stream = on_device(q, k, v, k_cache, v_cache, row_pos, row_slot, row_req, q_norm, k_norm, q_out,
                        table.freq)
     shape, cache = q.shape, k_cache.shape

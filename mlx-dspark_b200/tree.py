@@ -41,7 +41,8 @@ def pack(cu_rows: torch.Tensor, parent: torch.Tensor | None, kv_len: torch.Tenso
     ``parent`` int32 ``[R]``: places within the request, -1 for the root (``None``: chains).
     With ``kv_start`` (a position-major pool) the slots count from it and ``row_req`` is 0. With ``kv_cap``
     (int32 ``[B]``: positions each request may fill) rows past it have slot -1, and ``room`` (``[B]``)
-    tells how many rows fit."""
+    tells how many rows fit. Rows behind the last request's are nobody's: position 0, slot and request
+    -1, no bits."""
     stream = on_device(cu_rows, parent, kv_len, kv_start, kv_cap)
     R, B = int(n_rows), kv_len.numel()
     words = anc_words(max_nodes)

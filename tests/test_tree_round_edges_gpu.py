@@ -317,3 +317,26 @@ def test_a_wait_that_runs_out_leaves_nothing_behind(cuda):
         assert ((out.double() - o).abs() <= bound).all(), limit_ns
         assert _lib.device_status(cuda.index) == 0
     assert ran_out
+
+
+@pytest.mark.parametrize("pool", [False, True])
+def test_rows_of_no_request_are_not_appended(cuda, pool):
+    """A round packed for more rows than its requests have, into arrays of a former round."""
+    from mlx_dspark_b200 import _lib, rope, tree
+
+    R, B, Hk, cap, D = 12, 2, 2, 20, 64
+    out = {k: torch.full((R,), 5, dtype=torch.int32, device=cuda) for k in ("row_pos", "row_slot")}
+    out |= {"row_req": torch.zeros(R, dtype=torch.int32, device=cuda),
+            "anc": torch.full((R, 2), -1, dtype=torch.int32, device=cuda), "kv_len_new": _i32([0, 0], cuda)}
+    start = _i32([0, cap], cuda) if pool else None
+    meta = tree.pack(_cu([3, 4], cuda), None, _i32([8, 2], cuda), R, 40, kv_start=start, out=out)
+    assert meta["row_slot"].tolist() == [8, 9, 10] + [2 + i + cap * pool for i in range(4)] + [-1] * 5
+    assert meta["row_req"].tolist() == ([0] * 7 if pool else [0] * 3 + [1] * 4) + [-1] * 5
+    assert meta["row_pos"].tolist()[7:] == [0] * 5 and not meta["anc"][7:].any()
+    x = torch.ones(R, Hk, D, dtype=BF, device=cuda)
+    kc = torch.zeros((1, Hk, B * cap, D) if pool else (B, Hk, cap, D), dtype=BF, device=cuda)
+    vc = torch.zeros_like(kc)
+    rope.rope_append(x, x, x, rope.RopeTable(D, device=cuda), meta["row_pos"], kc, vc, meta["row_slot"],
+                     row_req=meta["row_req"])
+    assert float(vc.sum()) == 7 * Hk * D
+    assert _lib.device_status(cuda.index) == 0
