@@ -37,6 +37,8 @@ def inv_freq(rotary_dim: int, theta: float = 1e6, scaling: dict | None = None) -
       ``factor``, below ``.. / high_freq_factor`` kept, blended between.
     """
     sc = scaling or {}
+    if sc and "type" not in sc:  # another file's names for it would pass as unscaled
+        raise ValueError(f"rope scaling without a type: {sorted(sc)}")
     kind = sc.get("type") or "none"
     n, rot = rotary_dim // 2, rotary_dim
     if kind == "none":

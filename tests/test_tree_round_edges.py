@@ -4,7 +4,9 @@ from __future__ import annotations
 
 import ctypes as C
 
-from mlx_dspark_b200 import _lib
+import pytest
+
+from mlx_dspark_b200 import _lib, rope
 
 
 def _aligned():
@@ -25,3 +27,14 @@ def test_workspaces_have_to_be_aligned():
         assert "aligned" in _lib.last_error()
         assert _lib.lib.dspark_sample_accept(C.byref(_lib.SampleArgs(**accept, workspace=p + off)), None) == _lib.ERR_ARG
         assert "aligned" in _lib.last_error()
+
+
+@pytest.mark.parametrize("scaling", [{"factor": 4.0}, {"rope_type": "yarn", "factor": 4.0, "original_max_position": 8192}])
+def test_a_scaling_without_a_type_is_not_unscaled(scaling):
+    with pytest.raises(ValueError, match="type"):
+        rope.inv_freq(64, 1e6, scaling)
+
+
+def test_unscaled_forms():
+    plain = rope.inv_freq(64, 1e6)
+    assert all(rope.inv_freq(64, 1e6, s) == plain for s in (None, {}, {"type": None}, {"type": "none"}))
