@@ -684,6 +684,10 @@ __global__ void __launch_bounds__(NTHR, 1)
   constexpr uint32_t ID_PV = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) |
                              (uint32_t(D >> 3) << 17) | (uint32_t(ROWS >> 4) << 24);
   constexpr uint32_t O_COL = 256;
+  // The weights are rounded to the input's type for the product with V (their sum is not). fp16 loses what
+  // is below 2^-25, which adds up over a long row far below its largest key: all weights of all parts
+  // are 2^7 times as large there (at most 2^15, with a reference 2^8 too low), which cancels in the end.
+  constexpr float LIFT = std::is_same<T, bf16>::value ? 0.f : 7.f;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* ring = smem + L::RING;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BARS);
@@ -836,7 +840,7 @@ __global__ void __launch_bounds__(NTHR, 1)
             }
           }
           const float mc = m == -INFINITY ? 0.f : m * c_log2;
-          const f32x2 c2 = pack2(c_log2, c_log2), nm2 = pack2(-mc, -mc);
+          const f32x2 c2 = pack2(c_log2, c_log2), nm2 = pack2(LIFT - mc, LIFT - mc);
           f32x2 sum[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) sum[e] = pack2(0.f, 0.f);

@@ -340,3 +340,29 @@ def test_rows_of_no_request_are_not_appended(cuda, pool):
                      row_req=meta["row_req"])
     assert float(vc.sum()) == 7 * Hk * D
     assert _lib.device_status(cuda.index) == 0
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("late", [False, True])
+@pytest.mark.parametrize("drop", [16.0, 18.0, 20.0])
+def test_attention_keeps_the_mass_of_a_long_tail(cuda, dtype, late, drop):
+    """One key far above 30000 others whose values are all the output. The weights' bound: rounded to the
+    type relative to themselves, and for fp16 below 2^-14 of 2^7 times the row's reference by 2^-25 of that
+    at most, so by 2^-32 a key (the sum they are divided by is not below the reference)."""
+    from mlx_dspark_b200 import tree
+
+    L, n, Hq, Hk, D, B = 30011, 3, 8, 2, 64, 150  # requests enough that a row's keys are in one or two parts
+    g = torch.Generator(device=cuda).manual_seed(int(drop))
+    q = 0.01 * torch.randn(n, Hq, D, device=cuda, generator=g)
+    k = 0.5 * torch.randn(1, Hk, L, D, device=cuda, generator=g)
+    v = 1.0 + 0.25 * torch.randn(1, Hk, L, D, device=cuda, generator=g)
+    q[..., 0], k[..., 0] = 4.0, -drop / 8
+    top = L - 400 if late else 5
+    k[:, :, top, 0], v[:, :, top] = drop / 8, 0.0
+    q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+    out = tree.tree_sdpa(q.repeat(B, 1, 1), k, v, _cu([n] * B, cuda), _i32([L] * B, cuda), None, scale=1.0,
+                         max_nodes=n).view(B, n, Hq, D)
+    o, _ = _exact(q, k[0], v[0], _sees(None, n, L, chain=True), 1.0, dtype)
+    size = o.abs()  # the values are positive (but for chance): sum p |v| is the output
+    bound = (U[dtype] + 1e-4) * size + U[dtype] * size + (2.0 ** -32 * 3.0 * L if dtype == HF else 0.0) + 2.0 ** -25
+    assert ((out.double() - o).abs() <= bound).all(), float(((out.double() - o).abs() / bound).max())
