@@ -61,12 +61,13 @@ def sample_accept(logits: torch.Tensor, ids: torch.Tensor, cu_rows: torch.Tensor
 
     The token after the path is drawn by ``argmax(w / noise)``: ``w = max(p - q, 0)`` after a
     rejection with ``draft_probs``, else ``p`` without the tokens just tried. Returns ``n`` (accepted
-    drafts), ``next``, ``prob`` (p of each row's token given its parent, 1 for roots) and ``path``
-    (kept places of each request in order, then -1); ``out``, a former call's result for as many rows and
-    requests, is written again (its workspace too, on one stream). ``lens`` (int32 ``[B]``, tokens cached after the
-    verify's append) loses the rejected rows in place. ``max_rows`` (<= 1024) bounds a block, ``row_limit``
-    (int32 ``[B]``) the rows of each that can be accepted: the others count as not tried, and a block of
-    which no row can gives n 0, next -1 and loses all its rows."""
+    drafts), ``next``, ``prob`` (p of each row's token given its parent, 1 for roots), ``path``
+    (kept places of each request in order, then -1) and ``lens`` where it was given; ``out``, a former
+    call's result for as many rows and requests, is written again (its workspace too, on one stream).
+    ``lens`` (int32 ``[B]``, tokens cached after the verify's append) loses the rejected rows in place.
+    ``max_rows`` (<= 1024) bounds a block, ``row_limit`` (int32 ``[B]``) the rows of each that can be
+    accepted: the others count as not tried, and a block of which no row can gives n 0, next -1 and
+    loses all its rows."""
     given = () if out is None else (out["n"], out["next"], out["prob"], out["path"])
     stream = on_device(logits, ids, cu_rows, u, noise, temperature, draft_probs, parent, row_limit, lens, *given)
     R, B = ids.numel(), cu_rows.numel() - 1
@@ -86,17 +87,20 @@ def sample_accept(logits: torch.Tensor, ids: torch.Tensor, cu_rows: torch.Tensor
                "prob": torch.empty(R, dtype=torch.float32, device=logits.device),
                "path": torch.empty(R, **e)}
     n = _workspace(R, B, V, logits.get_device())
-    # a graph has to own what its replays write, a stream what the allocator may hand on in its order
-    kept, ws = out.get("workspace", (None, None))
+    # The workspace goes with the result's `n`, as an attribute: the dictionary holds results alone. A graph has
+    # to own what its replays write, a stream what the allocator may hand on in its order.
+    kept, ws = getattr(out["n"], "_accept_workspace", (None, None))
     if n and (kept != stream or ws.numel() < n or torch._C._cuda_isCurrentStreamCapturing()):
         ws = torch.empty(n, dtype=torch.uint8, device=logits.device)
         if not torch._C._cuda_isCurrentStreamCapturing():
-            out["workspace"] = stream, ws
+            out["n"]._accept_workspace = stream, ws
     _lib.check(_lib.lib.dspark_sample_accept(_pack(
         logits.data_ptr(), draft, ld, ld_draft, ld_noise, int32("ids", ids), int32("cu_rows", cu_rows),
         int32("parent", parent, R), _f32("u", u, R), noise.data_ptr(), _f32("temperature", temperature, B),
         int32("n", out["n"], B), int32("next", out["next"], B), _f32("prob", out["prob"], R),
         int32("path", out["path"], R), int32("lens", lens, B), ws.data_ptr() if n else 0, n, dt, ddt, R, B, V,
         max_rows, int32("row_limit", row_limit, B)), stream))
-    out["lens"] = lens
+    out.pop("lens", None)
+    if lens is not None:
+        out["lens"] = lens
     return out

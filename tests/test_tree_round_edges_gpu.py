@@ -366,3 +366,18 @@ def test_attention_keeps_the_mass_of_a_long_tail(cuda, dtype, late, drop):
     size = o.abs()  # the values are positive (but for chance): sum p |v| is the output
     bound = (U[dtype] + 1e-4) * size + U[dtype] * size + (2.0 ** -32 * 3.0 * L if dtype == HF else 0.0) + 2.0 ** -25
     assert ((out.double() - o).abs() <= bound).all(), float(((out.double() - o).abs() / bound).max())
+
+
+def test_sample_accept_returns_results_alone(cuda):
+    """The result's values are its tensors, whether it is a new one or a former one, with lengths or not."""
+    from mlx_dspark_b200 import sampling
+
+    V = 90
+    args = (torch.zeros(3, V, device=cuda), _i32([0, 0, 0], cuda), _cu([1, 2], cuda), torch.rand(3, device=cuda),
+            torch.ones(2, V, device=cuda))
+    out, lens = None, _i32([4, 5], cuda)
+    for given in (None, lens, None, lens):
+        out = sampling.sample_accept(*args, max_rows=2, lens=given, out=out)
+        want = {"n", "next", "prob", "path"} | ({"lens"} if given is not None else set())
+        assert set(out) == want and all(isinstance(v, torch.Tensor) for v in out.values())
+    assert {k: v.clone() for k, v in out.items()}["lens"].tolist() == lens.tolist()
