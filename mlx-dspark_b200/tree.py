@@ -139,6 +139,8 @@ class PathKeeper:
         ``base + path[cu_rows[b] + i]`` to ``base + i`` for ``i <= n_accept[b]``, in every layer."""
         B = n_accept.numel()
         stream = on_device(self._kp, path, cu_rows, n_accept, lens, kv_start)
+        if path.numel() == 0:  # no request has rows
+            return
         _lib.check(_lib.lib.dspark_kv_keep_path(
             self._kp_ptr, self._vp_ptr, len(self.k_caches), self._ks, self._vs, int32("path", path),
             int32("cu_rows", cu_rows, B + 1), int32("n_accept", n_accept), int32("lens", lens, B),

@@ -100,7 +100,8 @@ class TreeSpec:
         if temperature is None:
             temperature = torch.zeros(self.B, device=ids.device)
         meta = self.pack(cu_rows, parent, R)
-        logits, lens = self.forward(ids, meta, cu_rows), meta["kv_len_new"]
+        lens = meta["kv_len_new"]
+        logits = self.forward(ids, meta, cu_rows) if R else self.t.logits[:0]  # (every slot idle)
         out = sampling.sample_accept(logits, ids, cu_rows, u, noise, temperature=temperature,
                                      draft_probs=draft_probs, parent=parent, max_rows=self.max_nodes,
                                      row_limit=meta["room"], lens=lens)

@@ -381,3 +381,14 @@ def test_sample_accept_returns_results_alone(cuda):
         want = {"n", "next", "prob", "path"} | ({"lens"} if given is not None else set())
         assert set(out) == want and all(isinstance(v, torch.Tensor) for v in out.values())
     assert {k: v.clone() for k, v in out.items()}["lens"].tolist() == lens.tolist()
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_a_round_of_idle_slots(cuda, tree):
+    """No nodes at all: every slot stays."""
+    t, eng = _engine(cuda)
+    eng.lens.copy_(_i32([4, 0, 9], cuda))
+    none = torch.empty(0, dtype=torch.int32, device=cuda)
+    out = eng.step(none, _cu([0, 0, 0], cuda), torch.empty(0, device=cuda),
+                   torch.ones(3, t.cfg.vocab, device=cuda), parent=none if tree else None)
+    assert out["n"].tolist() == [0, 0, 0] and out["next"].tolist() == [-1] * 3 and eng.lens.tolist() == [4, 0, 9]
