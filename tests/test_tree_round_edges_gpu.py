@@ -392,3 +392,104 @@ def test_a_round_of_idle_slots(cuda, tree):
     out = eng.step(none, _cu([0, 0, 0], cuda), torch.empty(0, device=cuda),
                    torch.ones(3, t.cfg.vocab, device=cuda), parent=none if tree else None)
     assert out["n"].tolist() == [0, 0, 0] and out["next"].tolist() == [-1] * 3 and eng.lens.tolist() == [4, 0, 9]
+
+
+# ----------------------------------------------------------------- wider ranges of what was there
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("counts,lens,Hq,Hk,D", [
+    ([384], [1000], 16, 2, 128),
+    ([700, 3, 300], [900, 2500, 300], 8, 4, 64),
+    ([1024], [1024], 4, 4, 128),
+    ([1024, 1000], [5000, 1013], 12, 2, 128),
+])
+def test_attention_of_big_trees(cuda, dtype, counts, lens, Hq, Hk, D):
+    """Up to 1024 nodes: many row blocks a request, trees over many key tiles."""
+    from mlx_dspark_b200 import tree
+
+    rng = random.Random(sum(counts))
+    parents = [ref.random_parents(n, rng) for n in counts]
+    g = torch.Generator(device=cuda).manual_seed(len(counts))
+    q = torch.randn(sum(counts), Hq, D, device=cuda, generator=g).to(dtype)
+    kc, vc = (torch.randn(len(counts), Hk, max(lens) + 7, D, device=cuda, generator=g).to(dtype) for _ in range(2))
+    for b, L in enumerate(lens):
+        kc[b, :, L:], vc[b, :, L:] = float("inf"), float("nan")
+    words = tree.anc_words(max(counts))
+    anc = _i32([w for p in parents for w in ref.words_of(ref.ancestors(p), words)], cuda)
+    out = tree.tree_sdpa(q, kc, vc, _cu(counts, cuda), _i32(lens, cuda), anc, scale=D ** -0.5,
+                         max_nodes=max(counts))
+    r0 = 0
+    for b, n in enumerate(counts):
+        o, bound = _exact(q[r0 : r0 + n], kc[b], vc[b], _sees(parents[b], n, lens[b]), D ** -0.5, dtype)
+        assert ((out[r0 : r0 + n].double() - o).abs() <= bound).all(), b
+        r0 += n
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("counts,lens,Hq,Hk,D", [
+    ([129], [129], 8, 2, 128),
+    ([500], [1700], 16, 4, 64),
+    ([2048], [2048], 8, 2, 128),
+    ([1000, 1, 333], [1001, 4096, 2000], 4, 4, 128),
+])
+def test_attention_of_prompt_chunks(cuda, dtype, counts, lens, Hq, Hk, D):
+    """anc None over whole chunks of a prompt, in a position-major pool."""
+    from mlx_dspark_b200 import tree
+
+    g = torch.Generator(device=cuda).manual_seed(sum(lens))
+    start = [11 + sum(lens[:b]) for b in range(len(lens))]
+    q = torch.randn(sum(counts), Hq, D, device=cuda, generator=g).to(dtype)
+    kc, vc = (torch.randn(sum(lens) + 40, Hk, D, device=cuda, generator=g).to(dtype).permute(1, 0, 2)[None]
+              for _ in range(2))
+    out = tree.tree_sdpa(q, kc, vc, _cu(counts, cuda), _i32(lens, cuda), None, scale=D ** -0.5,
+                         max_nodes=max(counts), kv_start=_i32(start, cuda))
+    r0 = 0
+    for b, n in enumerate(counts):
+        o, bound = _exact(q[r0 : r0 + n], kc[0, :, start[b] :], vc[0, :, start[b] :],
+                          _sees(None, n, lens[b], chain=True), D ** -0.5, dtype)
+        assert ((out[r0 : r0 + n].double() - o).abs() <= bound).all(), b
+        r0 += n
+
+
+@pytest.mark.parametrize("form", ["chain", "draft", "tree"])
+def test_sample_accept_blocks_beyond_max_rows_and_second_roots(cuda, form):
+    """max_rows below the blocks' rows cuts them; a node whose parent is not before it is nobody's child."""
+    from mlx_dspark_b200 import sampling
+
+    V, n, cut, B = 3001, 21, 8, 70
+    rng = np.random.default_rng(3)
+    logits = torch.tensor(3 * rng.standard_normal((B * n, V)), dtype=torch.float32).to(HF)
+    best = logits.float().view(B, n, V).argsort(-1, descending=True)[:, :, :3]
+    pr = random.Random(4)
+    parents, ids = [], torch.zeros(B, n, dtype=torch.long)
+    for b in range(B):
+        par = list(range(-1, n - 1)) if form != "tree" else ref.random_parents(n, pr)
+        for i in range(1, n):
+            ids[b, i] = best[b, par[i], pr.randrange(3)]
+            if form == "tree" and pr.random() < 0.2:
+                par[i] = pr.choice([i, i + 1, n, n + 50, -1, -7])
+        parents.append(par)
+    q = None
+    if form == "draft":
+        q = torch.softmax(logits.float() + torch.tensor(rng.standard_normal((B * n, V)), dtype=torch.float32), -1)
+    u = torch.tensor(rng.random(B * n), dtype=torch.float32)
+    noise = torch.tensor(rng.exponential(size=(B, V)), dtype=torch.float32)
+    lens, close = _i32([60] * B, cuda), 0
+    got = sampling.sample_accept(
+        logits.to(cuda), _i32(ids.flatten().tolist(), cuda), _cu([n] * B, cuda), u.to(cuda), noise.to(cuda),
+        draft_probs=None if q is None else q.to(cuda),
+        parent=_i32([p for x in parents for p in x], cuda) if form == "tree" else None, max_rows=cut, lens=lens)
+    path = got["path"].view(B, n).tolist()
+    for b in range(B):
+        rows = slice(b * n, (b + 1) * n)
+        p = ref.probabilities(logits[rows].float().numpy(), 1.0)
+        want = [p[x, ids[b, i]] if 0 <= x < i else 1.0 for i, x in enumerate(parents[b])]
+        np.testing.assert_allclose(got["prob"][rows].cpu().numpy(), want, rtol=2.0 ** -23 * 208, atol=1e-30)
+        up = [x if x < i else -9 for i, x in enumerate(parents[b])][:cut]
+        pth, tok, near = ref.accept(p[:cut], ids[b, :cut].tolist(), up if form == "tree" else None, u[rows].numpy(),
+                                    noise[b].numpy(), None if q is None else q[rows].numpy()[:cut], False)
+        close += near
+        if not near:
+            assert (int(got["n"][b]), int(got["next"][b]), int(lens[b])) == (len(pth) - 1, tok, 60 - n + len(pth)), b
+            assert path[b] == pth + [-1] * (n - len(pth))
+    assert close <= 4
