@@ -45,11 +45,6 @@ constexpr int NONE = 0x7fffffff;
 // A logit as the formulas take it: NaN has no mass, +inf is the largest finite value.
 __device__ __forceinline__ float clean(float x) { return x == x ? fminf(x, FLT_MAX) : -INFINITY; }
 __device__ __forceinline__ bool greedy(float T) { return !(T > 0.f); }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // log2e / T, kept off zero and infinity, where the differences of -inf and equal logits would be lost.
 __device__ __forceinline__ float slope(float T) { return fminf(fmaxf(LOG2E / T, FLT_MIN), 1e30f); }
@@ -66,31 +61,6 @@ __device__ __forceinline__ void better(float& bv, int& bi, float v, int i) {
   }
 }
 
-// Two fp32 values in one 64-bit register, and the packed operations on them (sm_100).
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pack2(float a, float b) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpack2(f32x2 v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 // The larger of both halves of two words, NaN if one is.
 __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, bf16) {
   uint32_t r;
@@ -103,7 +73,7 @@ __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, __half) {
   return r;
 }
 __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, float) {
-  return __float_as_uint(max3_nan(__uint_as_float(a), __uint_as_float(b), __uint_as_float(b)));
+  return __float_as_uint(max3(__uint_as_float(a), __uint_as_float(b), __uint_as_float(b)));
 }
 
 // Values of 16 bytes of a row.
@@ -120,7 +90,7 @@ struct Vec {
     }
     if (sizeof(T) == 4) return __uint_as_float(m);
     const float2 f = Elem<T>::unpack(m);
-    return max3_nan(f.x, f.y, f.y);
+    return max3(f.x, f.y, f.y);
   }
   static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -304,11 +274,6 @@ __global__ void __launch_bounds__(THREADS) stat_kernel(const dspark_sample_args 
   }
 }
 
-__device__ __forceinline__ float lg2(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
