@@ -154,10 +154,9 @@ struct Shape {
 
 // Costs in half microseconds, fitted to CTA times over ragged batches: a tile of one row block 1 us
 // (more when HBM holds it: 64 KB take 1.5 us with all SMs at it), one of two row blocks 2 us, and a
-// segment 7 us (its Q, its pipeline's fill, its O, its share of the joins). 64 requests of 256 to 16k
-// keys: 372 us for the last CTA when dealt out by tiles alone. Mean of eleven mixes (1 to 200 requests of
-// 1 to 61 nodes over 100 to 32k keys) by a segment's cost: 8 86.9 us, 10 86.8, 12 85.6, 14 86.2, 16 86.2;
-// the 64 requests: 12 204 us, 14 199.
+// segment 7 us (its Q, its pipeline's fill, its O, its share of the joins). Mean of 47 mixes (1 to 250 requests
+// of 1 to 100 nodes over 64 to 32k keys, groups of 1 to 8, two runs each) by a segment's cost: 8 98.4 us,
+// 10 97.7, 12 96.8, 14 96.9, 16 97.0: flat from 12 to 16, the middle of it stands.
 constexpr int ONE = 2, PAIR = 4, SEG = 14;
 
 __device__ __forceinline__ Shape shape_of(const dspark_tree_attn_args& a, int b) {
@@ -546,10 +545,11 @@ __device__ __noinline__ void join_parts(void* workspace, T* o_base, int64_t o_ro
                                         const Cut* cuts, int n_cuts, int cta, uint8_t* smem) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int64_t STRIDE = int64_t(2) * (2 * ROWS) * (D + 1);  // floats between the CTAs' parts
-  // One request's parts with 8 kv heads on 148 SMs. Code that runs once is paid by its length: with 20
-  // the same 16 parts (one token over 2k keys) take 14.3 us a call, with 18 13.6; of more than 18 parts
-  // the rest comes a latency later (18 parts, 61 nodes over 16k: 34.9 us; with 16 held 36.0).
-  constexpr int HELD = 18;
+  // A part held costs its instructions whether it is there or not (code that runs once is paid by its length);
+  // of more parts the rest comes a latency later. Mean of 40 mixes (one request of 1 to 61 rows over 1.5k
+  // to 24k keys with 1, 2, 4 and 8 kv heads, which is 6 to 148 parts, and two and four requests) by parts
+  // held: 8 22.5 us, 12 21.3, 16 21.4, 18 21.1, 20 21.0, 24 21.6.
+  constexpr int HELD = 20;
   static_assert(MAX_CTA * 2 * ROWS * 4 <= Lay<D>::ML, "the weights' room");
   float* w = reinterpret_cast<float*>(smem);  // [parts][256]
   for (int k = 0; k < n_cuts; ++k) {
