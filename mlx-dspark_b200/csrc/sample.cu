@@ -12,9 +12,12 @@
 //  * after a rejection with a draft distribution the score is max(p - q, 0) / e, with the row's sum;
 //  * otherwise argmax p / e = argmax (l - ref) log2e / T - log2 e for any ref of the row: no sum, and
 //    no rounding of p to zero. ref is the largest logit so far, so that scores stay near zero.
+// Comparisons are made in 32 bits with the unit's exponential, logarithm and reciprocal, off by about 1e-6 of a
+// probability: what lies closer than that may be decided either way.
 // Bound: HBM (each deciding row once), or the two launches for a single block. Measured over 151,936
-// tokens: 256 chains of up to 16 rows 153 us (0.89 of a plain copy), 16 trees of up to 61 nodes 37 us
-// (0.55: blocks of rows without a child and the walk's latency), five rows 12 us.
+// tokens, 20 calls in a graph (a call of its own, host included): 256 chains of up to 16 rows 152 us (154 to
+// 173; 0.90 to 0.79 of a plain copy), 16 trees of up to 61 nodes 36 us (39; 0.57: blocks of rows without a
+// child and the walk's latency), five rows 12 us (17 to 22: the host).
 #include <float.h>
 
 #include <algorithm>
@@ -657,21 +660,22 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
   if (tid == 0) a.next_tok[b] = win.place == NONE ? -1 : win.place;
 }
 
+// Both rules by the mean of 35 mixes (1 to 96 requests; chains of 4 and 16 rows, trees of 16 and 61 nodes;
+// 32000 to 200064 tokens, bf16 and fp32): 19.2 us a call with what stands here. In brackets what another
+// value costs.
 // Slices of a row for stat_kernel: of 128 KB, so that many rows do not end in a half-filled last round
-// of blocks (2192 rows of 304 KB: 158 us a call; of 64 KB 175, whole rows 184); with few rows more,
-// blocks for eight an SM (a chain) or 32 (a tree: more than half of its rows are leaves, whose blocks
-// end at once); at least 8192 values each (five rows of 151936:
-// 13 us a call; 4096: 14.5, 2048: 15).
-static int slices_of(int R, int V, int size, bool tree, int sms) {
-  const int want = ((tree ? 32 : 8) * sms + R - 1) / std::max(R, 1);
+// of blocks (64 KB 0.2 %, 256 KB nothing); with few rows more, blocks for eight an SM (four 3 %, twelve nothing,
+// sixteen 1 %); at least 8192 values each (4096 2.5 %, 16384 4 %).
+static int slices_of(int R, int V, int size, int sms) {
+  const int want = (8 * sms + R - 1) / std::max(R, 1);
   return std::max(1, std::min(std::max(want, int(int64_t(V) * size / 131072)), V / 8192));
 }
-// Blocks of a request for pick_kernel: four an SM over all requests, which all run at once and walk
-// side by side (16 trees: 41 us a call; six an SM: 46), but at least four a request (256 requests: 158
-// us; three: 165, ten: 168).
+// Blocks of a request for pick_kernel: three an SM over all requests, which all run at once and walk
+// side by side (two 2.5 %, four 5 %), but at least four a request (three to six nothing here, but 256 chains of
+// up to 16 rows: three 160 us, four 152; eight 1 %), of at least 1024 values (512 1 %, 2048 1.5 %).
 static int blocks_of(int B, int V, int sms) {
-  const int want = std::max(4, (4 * sms + B - 1) / std::max(B, 1));
-  return std::max((V + MAX_SLICE - 1) / MAX_SLICE, std::max(1, std::min(want, V / 2048)));
+  const int want = std::max(4, (3 * sms + B - 1) / std::max(B, 1));
+  return std::max((V + MAX_SLICE - 1) / MAX_SLICE, std::max(1, std::min(want, V / 1024)));
 }
 
 }  // namespace sample
@@ -684,7 +688,7 @@ extern "C" {
 size_t dspark_sample_workspace(int R, int B, int V) {
   if (R <= 0 || B <= 0 || V <= 0) return 0;
   const int sms = sm_count(current_device());
-  return size_t(R) * sample::slices_of(R, V, 4, true, sms) * sizeof(sample::Stat) +
+  return size_t(R) * sample::slices_of(R, V, 4, sms) * sizeof(sample::Stat) +
          size_t(B) * sample::blocks_of(B, V, sms) * sizeof(sample::Pick) + size_t(B) * sizeof(unsigned);
 }
 
@@ -713,7 +717,8 @@ int dspark_sample_accept(const dspark_sample_args* p, void* stream) {
   if (reinterpret_cast<uintptr_t>(a.workspace) % 16)
     return fail(DSPARK_ERR_ARG, "sample_accept: the workspace must be 16-byte aligned");
   const int sms = sm_count(current_device());
-  const int slices = sample::slices_of(a.R, a.V, a.dtype == DSPARK_DTYPE_F32 ? 4 : 2, a.parent != nullptr, sms), blocks = sample::blocks_of(a.B, a.V, sms);
+  const int slices = sample::slices_of(a.R, a.V, a.dtype == DSPARK_DTYPE_F32 ? 4 : 2, sms);
+  const int blocks = sample::blocks_of(a.B, a.V, sms);
   if (int64_t(a.R) * slices > 0x7fffffff || int64_t(a.B) * blocks > 0x7fffffff)
     return fail(DSPARK_ERR_UNSUPPORTED, "sample_accept: %d rows, %d requests", a.R, a.B);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
