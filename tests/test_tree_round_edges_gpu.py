@@ -493,3 +493,26 @@ def test_sample_accept_blocks_beyond_max_rows_and_second_roots(cuda, form):
             assert (int(got["n"][b]), int(got["next"][b]), int(lens[b])) == (len(pth) - 1, tok, 60 - n + len(pth)), b
             assert path[b] == pth + [-1] * (n - len(pth))
     assert close <= 4
+
+
+def test_calls_repeat_themselves_bit_for_bit(cuda):
+    """The attention's joins and the accept's comparisons have one order, whatever the CTAs' timing."""
+    from mlx_dspark_b200 import sampling, tree
+
+    rng = random.Random(8)
+    for B, longest, nodes in ((1, 9000, 40), (37, 3000, 20)):
+        counts = [rng.randint(1, nodes) for _ in range(B)]
+        lens = [rng.randint(nodes, longest) for _ in counts]
+        g = torch.Generator(device=cuda).manual_seed(B)
+        q = torch.randn(sum(counts), 16, 128, device=cuda, generator=g).to(BF)
+        kc, vc = (torch.randn(B, 4, longest, 128, device=cuda, generator=g).to(BF) for _ in range(2))
+        args = (q, kc, vc, _cu(counts, cuda), _i32(lens, cuda), None)
+        outs = [tree.tree_sdpa(*args, scale=0.09, max_nodes=nodes) for _ in range(12)]
+        assert all(torch.equal(x, outs[0]) for x in outs)
+        V, R = 70001, sum(counts)
+        logits = torch.randn(R, V, device=cuda, generator=g)
+        par = _i32([p for n in counts for p in ref.random_parents(n, rng)], cuda)
+        args = (logits, logits.argmax(1).roll(1).int(), _cu(counts, cuda), torch.rand(R, device=cuda, generator=g),
+                torch.empty(B, V, device=cuda).exponential_(generator=g))
+        outs = [sampling.sample_accept(*args, parent=par, max_rows=nodes) for _ in range(12)]
+        assert all(torch.equal(x[k], outs[0][k]) for x in outs for k in ("n", "next", "prob", "path"))
