@@ -532,8 +532,10 @@ int dspark_rope_append(const dspark_rope_args* a, void* stream);
  * out = softmax(scale q.k) . v over the visible keys, zeros where there are none; keys that a row
  * does not see take no part whatever they hold. k / v [kv_batch, Hk, cap, D] with strides
  * {batch, head, position}: request b's keys start at position kv_start[b] (or 0) of batch entry b,
- * or of entry 0 when kv_batch is 1. kv_len counts are cut at the cache's end. max_rows bounds
- * rows(b) (it only chooses the launch). bf16 or fp16, D 64 or 128, 16-byte aligned rows.
+ * or of entry 0 when kv_batch is 1. kv_len counts are cut at the cache's end. max_rows (1 or more):
+ * a bound of rows(b), which no launch depends on today. Rows of no request are not written. The weights
+ * are rounded to the inputs' type before the product with v. bf16 or fp16, D 64 or 128, 16-byte aligned
+ * rows.
  * Scratch: dspark_tree_attn_workspace bytes, 16-byte aligned, nothing to clear; calls that overlap on the
  * GPU need their own. */
 typedef struct {
@@ -555,6 +557,7 @@ typedef struct {
 } dspark_tree_attn_args;
 
 int dspark_tree_attn(const dspark_tree_attn_args* a, void* stream);
+/* (0 for an empty shape, else the same for every B and max_rows: two parts an SM) */
 size_t dspark_tree_attn_workspace(int B, int Hq, int Hk, int D, int max_rows);
 
 /* Verification of drafted tokens against the target's probabilities p = softmax(logits / T) from
@@ -604,7 +607,8 @@ size_t dspark_sample_workspace(int R, int B, int V);
 
 /* dspark_verify_forward for packed trees: the same embedding, projections, norms and lm_head; between
  * the QKV projection and the O projection each layer runs dspark_rope_append (with the layer's q / k
- * norms) and dspark_tree_attn instead of the fused epilogue and the block attention. `t` holds the
+ * norms) and dspark_tree_attn instead of the fused epilogue and the block attention. The QKV product is
+ * rounded to bf16 before the norms and the rotation (the fused epilogue has it in fp32). `t` holds the
  * round's metadata (dspark_tree_pack) and scratch: qkv bf16 [R, (Hq + 2 Hk) * head_dim], and the tree
  * attention's workspace. The caches are the model's pools with a stride kv_sb between kv_batch entries.
  * R <= buf->rows_cap; the packing arrays in buf are not used. */

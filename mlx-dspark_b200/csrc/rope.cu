@@ -7,7 +7,7 @@
 // and its partner half the rotated part away; interleaved: 16 neighbours), so a rotation needs no other
 // lane, and a head's RMS norm only a sum over its lanes. A lane meets the same pairs in every head of
 // its row: cosines and sines are computed once a row and lane.
-// Measured: 16,389 rows of 32/8 heads of 128 69.5 us (5.8 TB/s, 0.88 of a plain copy); one row 2.4 us in
+// Measured: 16,389 rows of 32/8 heads of 128 69.1 us (5.8 TB/s, 0.89 of a plain copy); one row 2.4 us in
 // a graph.
 #include <algorithm>
 

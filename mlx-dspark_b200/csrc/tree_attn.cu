@@ -26,12 +26,19 @@
 // softmax and the output of the old segment; one thread issues the products: S = Q K^T (both from shared memory, K-major), O += P V (P from tensor memory, V from
 // shared memory as it lies, keys along K, so N-major). A thread of a softmax warpgroup owns a row:
 // no shuffles. The maximum in use is only raised when a tile exceeds it by more than 2^8: the
-// weights then stay within fp16 / fp32 range and O is rarely rescaled.
+// weights then stay within fp16 / fp32 range and O is rarely rescaled. (That, and starting the second product at
+// three quarters of the weights, are known from published attention kernels for this architecture.)
 //
-// Bound: HBM up to about 200 rows an item (64 ragged requests of 256 to 16k keys: 196-217 us, 0.69 to
-// 0.75 of a plain copy's rate), above that the chain of softmax and products (two trees of 384 nodes, 64/8
-// heads, 32k keys: 880 us, 940 TFLOP/s at the power cap: 3750 clocks a tile of 256 x 128, 2048 of them
-// products); a chain of latencies for few tiles (one token over 2k keys 13.6 us, 61 nodes over 16k 35 us).
+// Rounding: the weights are rounded to the input's type for the product with V, as the tensor core takes them;
+// scores, maxima, sums and O are fp32. Against 64 bits the mean error of a result is 1.3 to 1.4 times that of
+// fp32 weights (bf16 0.0023 for 0.0017, fp16 0.00029 for 0.00021, most of both the result's own rounding).
+//
+// Bound: HBM up to about 200 rows an item, above that the chain of softmax and products, a chain of latencies
+// for few tiles. Measured, 20 calls in a graph (a call of its own among others' work, host included):
+// 64 ragged requests of 256 to 16k keys 195-236 us (196-236; 0.76 to 0.63 of a plain copy's rate, lowest when
+// the GPU is at its power cap); two trees of 384 nodes, 64/8 heads, 32k keys 846-994 us (890-995; 975 to 830
+// TFLOP/s at the power cap: 3750 clocks a tile of 256 x 128, 2048 of them products); one token over 2k keys
+// 13.6 us (16); 61 nodes over 16k keys 35 us (37-39).
 //
 // Keys that a row does not see take no part whatever they hold: scores are replaced by -inf, V rows
 // past the request's keys are zeroed in shared memory, and a non-finite V among the tree's own keys

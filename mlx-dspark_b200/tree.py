@@ -72,8 +72,12 @@ def tree_sdpa(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_
     b sees the ``kv_len[b] - rows(b)`` keys before its tree and, of the tree's keys after them, its
     own ancestors by the bits ``anc[i]`` (int32 ``[R, words]``; ``None``: all places up to its own).
     ``kv_len`` int32 ``[B]`` counts the tree's rows too. A position-major pool is passed as one
-    batch entry ``[1, Hk, positions, D]`` with ``kv_start`` int32 ``[B]``. ``max_nodes`` bounds the
-    rows of a request. Returns ``out [R, Hq, D]``; a row that sees nothing is zero."""
+    batch entry ``[1, Hk, positions, D]`` with ``kv_start`` int32 ``[B]``. ``max_nodes`` (1 or more) bounds
+    the rows of a request. Returns ``out [R, Hq, D]``; a row that sees nothing is zero, a row of no request
+    is not written. For up to 32 nodes, as many in every request, :func:`.multirow_attn.multirow_sdpa` with
+    ``tree_anc`` is the faster one up to 2k keys (one request, 32/8 heads of 128: 8 to 13 us for 14 to 15)
+    and for up to 8 nodes up to 16k; from 16 nodes and 8k keys on this one is (32 nodes over 32k: 39 us
+    for 78)."""
     stream = on_device(q, k_cache, v_cache, cu_rows, kv_len, anc, kv_start, out)
     shape, cache = q.shape, k_cache.shape
     if len(shape) != 3 or len(cache) != 4 or v_cache.shape != cache:

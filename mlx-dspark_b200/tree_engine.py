@@ -91,7 +91,7 @@ class TreeSpec:
         """One round. ``ids`` int32 ``[R]``: every slot's nodes one slot after the other (``cu_rows``
         int32 ``[slots + 1]``; an idle slot has none), the first of them its pending token; ``parent``
         int32 ``[R]`` as in :func:`.tree.pack` (``None``: chains); ``u``, ``noise``, ``temperature``
-        (``None``: greedy) and ``draft_probs`` as in :func:`.sampling.sample_accept`. Returns its
+        (``None``: greedy here, 1 there) and ``draft_probs`` as in :func:`.sampling.sample_accept`. Returns its
         ``n``, ``next``, ``prob`` and ``path``; ``lens`` and the caches move on to the accepted tokens,
         and ``next`` is each slot's new pending token. Nodes past their slot's capacity are neither cached
         nor accepted, and the device status records them; a slot without room for its pending token stays
