@@ -482,7 +482,7 @@ int dspark_p2p_allgather(const dspark_p2p_gather_args* args, void* stream);
  * request's (cu_rows[B] .. R - 1) are nobody's: row_pos 0, row_slot and row_req -1, no bits.
  * dspark_tree_pack_capped also takes kv_cap [B], the positions that request b may fill: a row past them
  * has row_slot -1 (dspark_rope_append drops and records it), and room[b] (or NULL) is the number of
- * rows that fit, for dspark_sample_args.row_limit. */
+ * rows that fit, for dspark_sample_accept_limited. */
 int dspark_tree_pack(const int32_t* cu_rows, const int32_t* parent, const int32_t* kv_len,
                      const int32_t* kv_start, int B, int R, int32_t* row_pos, int32_t* row_slot, int32_t* row_req, uint32_t* anc,
                      int anc_words, int32_t* kv_len_new, void* stream);
@@ -577,8 +577,9 @@ size_t dspark_tree_attn_workspace(int B, int Hq, int Hk, int D, int max_rows);
  * counts as the largest finite value; a row with no mass accepts nothing and gives next -1.
  * logits bf16, fp16 or fp32, draft bf16, fp16 or fp32 (draft_dtype). Scratch: dspark_sample_workspace
  * bytes, 16-byte aligned, nothing to clear. max_rows bounds the rows of a
- * request (<= 1024); rows beyond it, or beyond row_limit[b], are not accepted and count as not tried. A
- * request whose limit leaves no row: n 0, next -1, path -1, prob 0, all its rows rejected. */
+ * request (<= 1024); rows beyond it are not accepted and count as not tried. dspark_sample_accept_limited
+ * also takes a bound of each request, row_limit [B] (device, or NULL); one that leaves no row: n 0, next -1,
+ * path -1, prob 0, all its rows rejected. */
 #define DSPARK_DTYPE_F32 2
 typedef struct {
   const void* logits;
@@ -599,10 +600,10 @@ typedef struct {
   size_t ws_bytes;
   int dtype, draft_dtype;
   int R, B, V, max_rows;
-  const int32_t* row_limit;  /* [B] or NULL */
 } dspark_sample_args;
 
 int dspark_sample_accept(const dspark_sample_args* a, void* stream);
+int dspark_sample_accept_limited(const dspark_sample_args* a, const int32_t* row_limit, void* stream);
 size_t dspark_sample_workspace(int R, int B, int V);
 
 /* dspark_verify_forward for packed trees: the same embedding, projections, norms and lm_head; between

@@ -130,7 +130,7 @@ class SampleArgs(C.Structure):
                 ("noise", vp), ("temperature", vp), ("n_accept", vp), ("next_tok", vp),
                 ("prob", vp), ("path", vp), ("lens", vp), ("workspace", vp), ("ws_bytes", sz),
                 ("dtype", i32), ("draft_dtype", i32), ("R", i32), ("B", i32), ("V", i32),
-                ("max_rows", i32), ("row_limit", vp)]
+                ("max_rows", i32)]
 
 
 def packer(cls):
@@ -208,6 +208,7 @@ _SIGS = {
     "dspark_tree_attn": (i32, [vp, vp]),
     "dspark_tree_attn_workspace": (sz, [i32, i32, i32, i32, i32]),
     "dspark_sample_accept": (i32, [vp, vp]),
+    "dspark_sample_accept_limited": (i32, [vp, vp, vp]),
     "dspark_sample_workspace": (sz, [i32, i32, i32]),
     "dspark_kv_keep_path": (i32, [vp, vp, i32, P_i64, P_i64, vp, vp, vp, vp, vp, i32, i32, i32, i32,
                                   i32, i32, vp]),

@@ -326,7 +326,8 @@ struct Scorer {
 };
 
 template <typename T, typename Q>
-__global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args a, const Stat* stat,
+__global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args a,
+                                                       const int32_t* row_limit, const Stat* stat,
                                                        Pick* picks, unsigned* done, const int slices,
                                                        const int blocks) {
   pdl_launch_dependents();
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const dspark_sample_args 
     return;
   }
   int seen = min(rows, a.max_rows);  // rows that can be accepted
-  if (a.row_limit) seen = min(seen, a.row_limit[b]);
+  if (row_limit) seen = min(seen, row_limit[b]);
   if (seen <= 0) {
     if (!lead) return;
     for (int i = tid; i < rows; i += THREADS) {
@@ -693,6 +694,10 @@ size_t dspark_sample_workspace(int R, int B, int V) {
 }
 
 int dspark_sample_accept(const dspark_sample_args* p, void* stream) {
+  return dspark_sample_accept_limited(p, nullptr, stream);
+}
+
+int dspark_sample_accept_limited(const dspark_sample_args* p, const int32_t* row_limit, void* stream) {
   if (!p) return fail(DSPARK_ERR_ARG, "sample_accept: null argument");
   const dspark_sample_args& a = *p;
   if (a.R < 0 || a.B < 0 || a.V <= 0) return fail(DSPARK_ERR_ARG, "sample_accept: bad shape");
@@ -731,7 +736,7 @@ int dspark_sample_accept(const dspark_sample_args* p, void* stream) {
                   "sample_accept: sums")
 #define DSPARK_PICK(T, Q)                                                                          \
   DSPARK_CUDA_TRY(launch_ex(sample::pick_kernel<T, Q>, dim3(a.B * blocks), dim3(sample::THREADS), 0, s, \
-                            1, true, a, (const sample::Stat*)st, picks, done, slices, blocks),            \
+                            1, true, a, row_limit, (const sample::Stat*)st, picks, done, slices, blocks),            \
                   "sample_accept")
 #define DSPARK_PICK_Q(T)                                                                           \
   do {                                                                                             \

@@ -94,12 +94,12 @@ def sample_accept(logits: torch.Tensor, ids: torch.Tensor, cu_rows: torch.Tensor
         ws = torch.empty(n, dtype=torch.uint8, device=logits.device)
         if not torch._C._cuda_isCurrentStreamCapturing():
             out["n"]._accept_workspace = stream, ws
-    _lib.check(_lib.lib.dspark_sample_accept(_pack(
+    _lib.check(_lib.lib.dspark_sample_accept_limited(_pack(
         logits.data_ptr(), draft, ld, ld_draft, ld_noise, int32("ids", ids), int32("cu_rows", cu_rows),
         int32("parent", parent, R), _f32("u", u, R), noise.data_ptr(), _f32("temperature", temperature, B),
         int32("n", out["n"], B), int32("next", out["next"], B), _f32("prob", out["prob"], R),
         int32("path", out["path"], R), int32("lens", lens, B), ws.data_ptr() if n else 0, n, dt, ddt, R, B, V,
-        max_rows, int32("row_limit", row_limit, B)), stream))
+        max_rows), int32("row_limit", row_limit, B), stream))
     out.pop("lens", None)
     if lens is not None:
         out["lens"] = lens
