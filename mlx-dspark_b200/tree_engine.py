@@ -58,7 +58,7 @@ class TreeSpec:
                 logits: torch.Tensor | None = None) -> torch.Tensor:
         """Logits ``[R, vocab]`` of packed nodes ``ids`` (int32 ``[R]``); appends their K/V at the slots
         that ``meta`` (:meth:`pack` of as many rows) gives. ``logits``: bf16, ``R`` rows of the
-        vocabulary or more (default: the target's)."""
+        vocabulary or more (default: the target's own, which its next forward writes again)."""
         t, c, R = self.t, self.t.cfg, ids.numel()
         if not 1 <= R <= t.max_rows:
             raise _lib.DSparkUnsupported(_lib.ERR_UNSUPPORTED, f"{R} rows (1..{t.max_rows})")
