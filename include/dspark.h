@@ -645,6 +645,107 @@ int dspark_kv_keep_path(void* const* k_layers, void* const* v_layers, int n_laye
                         const int32_t* lens, const int32_t* kv_start, int B, int H, int D,
                         int elem_size, int cap, int kv_batch, void* stream);
 
+/* ---- a paged cache of 8-bit values ------------------------------------------------------
+ * k / v pages [n_pages, Hk, page, D] of e4m3 codes (any strides {page, head, token}, D contiguous) with one fp32
+ * scale a page and head (strides {page, head}): value = code * scale. Request b's token t is token t % page of
+ * page page_table[b * table_stride + t / page] (max_pages entries a request). The reference keeps one contiguous
+ * cache a request (src/mlx_dspark/batch_engine.py:122-224) or quantizes groups of head_dim
+ * (src/mlx_dspark/target.py:166-185). D 64 or 128, page 16, 32, 64 or 128, bf16 or fp16 rows. */
+
+/* Rotary positions of packed q and k rows (as dspark_rope_append: layout, rot, freq, mscale, norms) with the
+ * append of k and v. Request b owns rows cu_rows[b] .. cu_rows[b + 1] - 1; kv_len[b] tokens are cached, its rows
+ * become tokens kv_len[b] + i; row_pos [R], or NULL: positions kv_len[b] + i. The scale of a page and head is the
+ * smallest power of two (2^-64 to 2^64) with which the largest finite value of the tokens appended to it is at most
+ * 448; where the page holds tokens of the request already (kv_len[b] % page), the larger of that and the old scale, and
+ * if it rises the old codes are rounded to it. A page begun anew (from its first token) starts a scale of its own;
+ * taking tokens back (a smaller kv_len) leaves the scale. Values are rounded to nearest even, infinities become
+ * +-448 * scale, NaN stays NaN. Rows whose page the table does not have (or an id outside 0 .. n_pages - 1) are
+ * dropped, and the device status word records it. q_out (may be q) is written for rows of a request only.
+ * len_out [B] (or NULL): kv_len + rows, at most max_pages * page. No two requests append to one page. */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_strides[2], k_strides[2], v_strides[2];  /* elements {row, head} */
+  void* q_out;
+  int64_t qo_strides[2];
+  void* k_pages;
+  void* v_pages;
+  int64_t kp_strides[3], vp_strides[3];              /* bytes {page, head, token} */
+  float* k_scale;
+  float* v_scale;
+  int64_t scale_strides[2];                          /* elements {page, head}, of both */
+  const uint64_t* freq;
+  const int32_t* row_pos;
+  const int32_t* cu_rows;
+  const int32_t* kv_len;
+  const int32_t* page_table;
+  int64_t table_stride;
+  int32_t* len_out;
+  const void* q_norm;
+  const void* k_norm;
+  float mscale, eps;
+  int dtype, layout;
+  int R, B, Hq, Hk, D, rot, page, n_pages, max_pages;
+} dspark_paged_append_args;
+
+int dspark_paged_append(const dspark_paged_append_args* a, void* stream);
+
+/* Attention of packed rows over the pages: out = softmax(scale q.k) . v over the keys that a row sees, zeros where
+ * there are none. kv_len[b] counts request b's rows too; causal: its row i sees keys before kv_len[b] - rows(b) + i + 1,
+ * else all kv_len[b]. Not seen, whatever they hold: keys past the table's pages, those of a page id outside
+ * 0 .. n_pages - 1 (recorded in the device status word) and those of a page whose scale is not positive. A row that
+ * sees a NaN is NaN. Rows of no request are not written. Weights are rounded to fp16 for the product with v.
+ * 16-byte aligned rows. Scratch: dspark_paged_attn_workspace bytes, 16-byte aligned, nothing to clear; calls that
+ * overlap on the GPU need their own. */
+typedef struct {
+  const void* q;
+  const void* k_pages;
+  const void* v_pages;
+  void* out;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t q_strides[2], o_strides[2];    /* elements {row, head} */
+  int64_t kp_strides[3], vp_strides[3];  /* bytes {page, head, token} */
+  int64_t scale_strides[2];
+  const int32_t* cu_rows;
+  const int32_t* kv_len;
+  const int32_t* page_table;
+  int64_t table_stride;
+  void* workspace;
+  size_t ws_bytes;
+  float scale;
+  int dtype, causal;
+  int R, B, Hq, Hk, D, page, n_pages, max_pages;
+} dspark_paged_attn_args;
+
+int dspark_paged_attn(const dspark_paged_attn_args* a, void* stream);
+size_t dspark_paged_attn_workspace(int R, int B, int Hq, int Hk, int D);
+
+/* Log probabilities of given tokens. With p = softmax(logits / T) of a row (T = temperature[r], NULL: 1; 1e-6 or less:
+ * all mass on the first largest logit, above 1e6: 1e6): logprob = ln p(token), entropy = -sum p ln p, rank = tokens
+ * before it in the order (larger logit, then lower token; 0: the most likely), and the first `top` (<= 32) tokens
+ * of that order with their log probabilities (top_ids, top_logprob [R, top]). A logit that is NaN, -inf, or -2^100 or
+ * less (fp16: its lowest value) is a masked token's: probability 0, logprob -inf, rank -1, never an alternative; missing
+ * alternatives have id -1 and -inf. One above 2^100 (fp16: inf) counts as 2^100 (the largest value). A row with no
+ * other tokens: logprob -inf, entropy 0, rank -1. A token outside 0 .. V - 1: its row is not read; logprob and entropy
+ * 0, rank -1, no alternatives. bf16, fp16 or fp32, fp32 arithmetic. (The reference samples only,
+ * src/mlx_dspark/sampling.py.) */
+typedef struct {
+  const void* logits;
+  int64_t ld;
+  const int32_t* tokens;     /* [R] */
+  const float* temperature;  /* [R] or NULL */
+  float* logprob;
+  float* entropy;
+  int32_t* rank;
+  int32_t* top_ids;          /* NULL when top is 0 */
+  float* top_logprob;
+  int dtype, R, V, top;
+} dspark_score_args;
+
+int dspark_token_logprobs(const dspark_score_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -133,6 +133,36 @@ class SampleArgs(C.Structure):
                 ("max_rows", i32)]
 
 
+class PagedAppendArgs(C.Structure):
+    """``dspark_paged_append_args`` (include/dspark.h)."""
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("q_strides", i64 * 2), ("k_strides", i64 * 2),
+                ("v_strides", i64 * 2), ("q_out", vp), ("qo_strides", i64 * 2), ("k_pages", vp),
+                ("v_pages", vp), ("kp_strides", i64 * 3), ("vp_strides", i64 * 3), ("k_scale", vp),
+                ("v_scale", vp), ("scale_strides", i64 * 2), ("freq", vp), ("row_pos", vp),
+                ("cu_rows", vp), ("kv_len", vp), ("page_table", vp), ("table_stride", i64),
+                ("len_out", vp), ("q_norm", vp), ("k_norm", vp), ("mscale", f32), ("eps", f32),
+                ("dtype", i32), ("layout", i32), ("R", i32), ("B", i32), ("Hq", i32), ("Hk", i32),
+                ("D", i32), ("rot", i32), ("page", i32), ("n_pages", i32), ("max_pages", i32)]
+
+
+class PagedAttnArgs(C.Structure):
+    """``dspark_paged_attn_args`` (include/dspark.h)."""
+    _fields_ = [("q", vp), ("k_pages", vp), ("v_pages", vp), ("out", vp), ("k_scale", vp),
+                ("v_scale", vp), ("q_strides", i64 * 2), ("o_strides", i64 * 2),
+                ("kp_strides", i64 * 3), ("vp_strides", i64 * 3), ("scale_strides", i64 * 2),
+                ("cu_rows", vp), ("kv_len", vp), ("page_table", vp), ("table_stride", i64),
+                ("workspace", vp), ("ws_bytes", sz), ("scale", f32), ("dtype", i32), ("causal", i32),
+                ("R", i32), ("B", i32), ("Hq", i32), ("Hk", i32), ("D", i32), ("page", i32),
+                ("n_pages", i32), ("max_pages", i32)]
+
+
+class ScoreArgs(C.Structure):
+    """``dspark_score_args`` (include/dspark.h)."""
+    _fields_ = [("logits", vp), ("ld", i64), ("tokens", vp), ("temperature", vp), ("logprob", vp),
+                ("entropy", vp), ("rank", vp), ("top_ids", vp), ("top_logprob", vp), ("dtype", i32),
+                ("R", i32), ("V", i32), ("top", i32)]
+
+
 def packer(cls):
     """``pack(*values) -> bytes`` of a struct, its fields flattened in order (null pointers 0): what a
     call passes by pointer, at a quarter of the cost of building the ctypes object."""
@@ -210,6 +240,10 @@ _SIGS = {
     "dspark_sample_accept": (i32, [vp, vp]),
     "dspark_sample_accept_limited": (i32, [vp, vp, vp]),
     "dspark_sample_workspace": (sz, [i32, i32, i32]),
+    "dspark_paged_append": (i32, [vp, vp]),
+    "dspark_paged_attn": (i32, [vp, vp]),
+    "dspark_paged_attn_workspace": (sz, [i32, i32, i32, i32, i32]),
+    "dspark_token_logprobs": (i32, [vp, vp]),
     "dspark_kv_keep_path": (i32, [vp, vp, i32, P_i64, P_i64, vp, vp, vp, vp, vp, i32, i32, i32, i32,
                                   i32, i32, vp]),
 }

@@ -1,0 +1,345 @@
+// Rotary positions of packed q and k rows with the append of k and v to pages of 8-bit values
+// (dspark_paged_append).
+//
+// A page holds `page` tokens of every head; the value of a code is e4m3(code) * scale, one scale a page and head:
+// the smallest power of two with which the page's largest value is at most 448. Powers of two, because an append
+// to a page that holds tokens may raise its scale: the old codes are then multiplied by a power of two, which
+// changes none of them but those that end below e4m3's normal range (2^-6), so that a page filled token by token
+// is all but one filled at once. Rotation, norm and the division by the scale are fp32 and rounded once.
+//
+// Blocks: first those of the cache, one a (page that the call writes to, head, k or v): a page's largest value
+// is then known inside a block, which holds its new values in registers meanwhile. Then those of q, a warp or more a
+// row. Which page a block has is found from cu_rows without a sum over the requests: request b's pages
+// start at unit cu_rows[b] / page + 2 b, which leaves room for every page that n rows can touch (n / page + 2).
+// Bound: HBM for prompts (each value is read and written once), the launch for few rows.
+#include <algorithm>
+
+#include "host_common.h"
+#include "paged.cuh"
+
+namespace dspark {
+namespace paged {
+
+constexpr int Q_THREADS = 128;
+constexpr int U = 4;  // heads of q in flight a lane
+
+// cos and sin of pos * f, f in 64-bit fixed-point turns (the product wraps at whole turns: any position keeps its
+// phase to 2^-32 of a turn); within half a turn the special-function unit's are off by less than 1e-6.
+__device__ __forceinline__ void phase(int pos, uint64_t f, float& c, float& s) {
+  const uint64_t t = uint64_t(int64_t(pos)) * f;
+  const float a = float(int32_t(uint32_t(t >> 32))) * 1.4629180792671596e-9f;  // 2 pi / 2^32
+  c = __cosf(a);
+  s = __sinf(a);
+}
+
+// Sixteen values of a row: eight at p + c0 and eight at p + c1.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load16(const T* p, int c0, int c1, uint32_t* w) {
+  if (VEC) {
+    const uint4 a = ldcg_v4(p + c0), b = ldcg_v4(p + c1);
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+  } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int at = i < 4 ? c0 + 2 * i : c1 + 2 * (i - 4);
+      w[i] = uint32_t(h[at]) | uint32_t(h[at + 1]) << 16;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint32_t* w, float* x) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = Elem<T>::unpack(w[i]);
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+
+// RMS norm of a head whose 16-value parts are on `lanes` neighbouring lanes, then the rotation of the lane's part.
+template <typename T, bool HALF>
+__device__ __forceinline__ void norm_turn(float* x, const uint32_t* weight, bool norm, int lanes, float inv_d, float eps,
+                                          bool turns, const float* cs, const float* sn) {
+  if (norm) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) ss += x[i] * x[i];
+    for (int o = 1; o < lanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float rs = rsqrtf(ss * inv_d + eps);
+    float w[16];
+    unpack16<T>(weight, w);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] *= rs * w[i];
+  }
+  if (turns) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int i0 = HALF ? i : 2 * i, i1 = HALF ? 8 + i : 2 * i + 1;
+      const float p = x[i0], q = x[i1];
+      x[i0] = p * cs[i] - q * sn[i];
+      x[i1] = q * cs[i] + p * sn[i];
+    }
+  }
+}
+
+// One (page, head, k or v). PASS rounds of 16 values a thread; threads * 16 * PASS >= page * D.
+template <typename T, bool VEC, bool HALF, int PASS>
+__device__ void append_page(const dspark_paged_append_args& a, int unit, int* status) {
+  __shared__ uint32_t s_max[8];
+  const int tid = threadIdx.x, D = a.D, lanes = D / 16, li = tid % lanes;
+  const int kv = unit & 1, hu = unit >> 1, u = hu / a.Hk, h = hu - u * a.Hk;
+  const int shift = 31 - __clz(a.page);
+  const int b = last_at_most(a.B, u, [&](int i) { return (first_row(a.cu_rows, i, a.R) >> shift) + 2 * i; });
+  const int r0 = first_row(a.cu_rows, b, a.R), n = max(first_row(a.cu_rows, b + 1, a.R) - r0, 0);
+  const int j = u - (r0 >> shift) - 2 * b;
+  const int64_t len = max(a.kv_len[b], 0), room = int64_t(a.max_pages) << shift;
+  if (j < 0) return;
+  if (j == 0 && h == 0 && kv == 0 && tid == 0 && a.len_out) a.len_out[b] = int32_t(min(len + n, max(room, len)));
+  const int64_t pi = (len >> shift) + j;
+  if (n == 0 || pi > (len + n - 1) >> shift) return;
+  const int pid = pi < a.max_pages ? a.page_table[int64_t(b) * a.table_stride + pi] : -1;
+  if (pid < 0 || pid >= a.n_pages) {
+    if (tid == 0) report_error(status, kErrAppendPage);
+    return;
+  }
+  const int begin = j == 0 ? int(len & (a.page - 1)) : 0;       // tokens that the page has
+  const int place0 = int((pi << shift) + begin - len);          // the first new one's place in the request
+  const int count = min(a.page - begin, n - place0);
+  uint8_t* codes = static_cast<uint8_t*>(kv ? a.v_pages : a.k_pages) +
+                   (kv ? pid * a.vp_strides[0] + h * a.vp_strides[1] : pid * a.kp_strides[0] + h * a.kp_strides[1]);
+  const int64_t ts = kv ? a.vp_strides[2] : a.kp_strides[2];
+  float* scale = (kv ? a.v_scale : a.k_scale) + pid * a.scale_strides[0] + h * a.scale_strides[1];
+  const float old = begin ? *scale : 0.f;
+  const T* src = static_cast<const T*>(kv ? a.v : a.k) + (kv ? h * a.v_strides[1] : h * a.k_strides[1]);
+  const int64_t row_stride = kv ? a.v_strides[0] : a.k_strides[0];
+  const bool turns = !kv && li < a.rot / 16, half = turns && HALF;
+  const int c0 = half ? 8 * li : 16 * li, c1 = half ? a.rot / 2 + 8 * li : c0 + 8;
+  const int per = blockDim.x / lanes, first = tid / lanes;
+
+  uint32_t raw[PASS][8];
+#pragma unroll
+  for (int z = 0; z < PASS; ++z) {
+    const int t = z * per + first;
+    if (t < count) load16<T, VEC>(src + (r0 + place0 + t) * row_stride, c0, c1, raw[z]);
+  }
+  const bool norm = !kv && a.k_norm;
+  uint32_t weight[8];
+  if (norm) load16<T, false>(static_cast<const T*>(a.k_norm), c0, c1, weight);
+  float x[PASS][16];
+  float top = 0.f;
+#pragma unroll
+  for (int z = 0; z < PASS; ++z) {
+    const int t = z * per + first;
+    if (z * per >= count) break;  // (a norm's lanes leave together)
+    if (t < count) unpack16<T>(raw[z], x[z]);
+    float cs[8], sn[8];
+    if (turns && t < count) {
+      const int r = r0 + place0 + t, pos = a.row_pos ? a.row_pos[r] : int(len + place0 + t);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        phase(pos, a.freq[8 * li + i], cs[i], sn[i]);
+        cs[i] *= a.mscale;
+        sn[i] *= a.mscale;
+      }
+    }
+    norm_turn<T, HALF>(x[z], weight, norm, lanes, 1.f / D, a.eps, turns && t < count, cs, sn);
+    if (t < count) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float y = fabsf(x[z][i]);
+        top = fmaxf(top, y < INFINITY ? y : 0.f);  // (NaN: 0)
+      }
+    }
+  }
+  const uint32_t wm = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+  if ((tid & 31) == 0) s_max[tid >> 5] = wm;
+  __syncthreads();
+  uint32_t m = s_max[0];
+  for (int i = 1; i < int(blockDim.x) / 32; ++i) m = max(m, s_max[i]);
+  const int e = scale_exponent(__uint_as_float(m));
+  const float need = pow2(e);
+  const float now = old > need ? old : need;  // (what is no scale gives way)
+  if (old > 0.f && now > old) {               // the old tokens' codes for the new scale
+    const float f = old / now;
+    for (int i = tid; i < begin * lanes; i += blockDim.x) {
+      uint4* p = reinterpret_cast<uint4*>(codes + (i / lanes) * ts + (i % lanes) * 16);
+      uint4 w = *p;
+      uint32_t* y = &w.x;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t l2 = e4m3_to_f16(y[k]), h2 = e4m3_to_f16_hi(y[k]);
+        const float2 lo = Elem<__half>::unpack(l2), hi = Elem<__half>::unpack(h2);
+        y[k] = f32_to_e4m3(lo.x * f, lo.y * f, hi.x * f, hi.y * f);
+      }
+      *p = w;
+    }
+  }
+  if (tid == 0 && now != old) *scale = now;
+  const float inv = old > need ? 1.f / old : pow2(-e);
+#pragma unroll
+  for (int z = 0; z < PASS; ++z) {
+    const int t = z * per + first;
+    if (t >= count) break;
+    uint32_t y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      y[i] = f32_to_e4m3(x[z][4 * i] * inv, x[z][4 * i + 1] * inv, x[z][4 * i + 2] * inv, x[z][4 * i + 3] * inv);
+    uint8_t* p = codes + (begin + t) * ts;
+    if (half) {
+      *reinterpret_cast<uint2*>(p + c0) = make_uint2(y[0], y[1]);
+      *reinterpret_cast<uint2*>(p + c1) = make_uint2(y[2], y[3]);
+    } else {
+      *reinterpret_cast<uint4*>(p + c0) = make_uint4(y[0], y[1], y[2], y[3]);
+    }
+  }
+}
+
+// Warp w: row w / warps, the heads of part w % warps.
+template <typename T, bool VEC, bool HALF>
+__device__ void turn_q(const dspark_paged_append_args& a, int w, int warps) {
+  const int lane = threadIdx.x & 31, D = a.D, lanes = D / 16, per = 32 / lanes;
+  const int r = w / warps, part = w - r * warps;
+  if (r >= a.R) return;
+  const int group = lane / lanes, li = lane % lanes;
+  const bool turns = li < a.rot / 16, half = turns && HALF;
+  const int c0 = half ? 8 * li : 16 * li, c1 = half ? a.rot / 2 + 8 * li : c0 + 8;
+  const int step = warps * per;
+  const T* src = static_cast<const T*>(a.q) + r * a.q_strides[0];
+  T* dst = static_cast<T*>(a.q_out) + r * a.qo_strides[0];
+  uint32_t raw[U][8];
+  auto fetch = [&](int h) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (h + u * step < a.Hq) load16<T, VEC>(src + (h + u * step) * a.q_strides[1], c0, c1, raw[u]);
+  };
+  fetch(part * per + group);  // under way while the request is looked for
+  int pos = 0;
+  const int b = last_at_most(a.B, r, [&](int i) { return first_row(a.cu_rows, i, a.R); });
+  const int r0 = first_row(a.cu_rows, b, a.R);
+  if (r < r0 || r >= first_row(a.cu_rows, b + 1, a.R)) return;  // a row of no request
+  pos = a.row_pos ? a.row_pos[r] : max(a.kv_len[b], 0) + r - r0;
+  float cs[8], sn[8];
+  if (turns) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      phase(pos, a.freq[8 * li + i], cs[i], sn[i]);
+      cs[i] *= a.mscale;
+      sn[i] *= a.mscale;
+    }
+  }
+  const bool norm = a.q_norm;
+  uint32_t weight[8];
+  if (norm) load16<T, false>(static_cast<const T*>(a.q_norm), c0, c1, weight);
+  for (int hb = part * per; hb < a.Hq; hb += U * step) {
+    const int h = hb + group;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int hh = h + u * step;
+      if (hb + u * step >= a.Hq) break;
+      float x[16];
+      unpack16<T>(raw[u], x);
+      norm_turn<T, HALF>(x, weight, norm, lanes, 1.f / D, a.eps, turns, cs, sn);
+      if (hh >= a.Hq) continue;
+      uint32_t y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = turns || norm ? Elem<T>::pack(x[2 * i], x[2 * i + 1]) : raw[u][i];
+      T* p = dst + hh * a.qo_strides[1];
+      if (VEC) {
+        *reinterpret_cast<uint4*>(p + c0) = make_uint4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint4*>(p + c1) = make_uint4(y[4], y[5], y[6], y[7]);
+      } else {
+        uint16_t* o = reinterpret_cast<uint16_t*>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int at = i < 4 ? c0 + 2 * i : c1 + 2 * (i - 4);
+          o[at] = uint16_t(y[i]);
+          o[at + 1] = uint16_t(y[i] >> 16);
+        }
+      }
+    }
+    if (hb + U * step < a.Hq) fetch(h + U * step);
+  }
+}
+
+template <typename T, bool VEC, bool HALF, int PASS, int THREADS>
+__global__ void __launch_bounds__(THREADS) append_kernel(const dspark_paged_append_args a, const int page_blocks,
+                                                         const int warps, int* status) {
+  pdl_launch_dependents();
+  pdl_wait();
+  if (int(blockIdx.x) < page_blocks)
+    append_page<T, VEC, HALF, PASS>(a, int(blockIdx.x), status);
+  else
+    turn_q<T, VEC, HALF>(a, int((blockIdx.x - page_blocks) * (THREADS / 32) + (threadIdx.x >> 5)), warps);
+}
+
+template <typename T, bool VEC, bool HALF, int PASS, int THREADS>
+static cudaError_t launch_as(const dspark_paged_append_args& a, cudaStream_t s) {
+  const int64_t units = int64_t(a.R) / a.page + 2 * int64_t(a.B);
+  const int64_t page_blocks = units * a.Hk * 2;
+  // warps a row of q: one, unless that leaves less than 16 warps an SM (then as many as take U heads a lane)
+  const int sms = sm_count(current_device()), per = 32 / (a.D / 16);
+  const int most = (a.Hq + per - 1) / per, want = (16 * sms + a.R - 1) / a.R;
+  const int warps = std::max(1, std::min(want, most));
+  const int64_t q_blocks = (int64_t(a.R) * warps + THREADS / 32 - 1) / (THREADS / 32);
+  if (page_blocks + q_blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  return launch_ex(append_kernel<T, VEC, HALF, PASS, THREADS>, dim3(unsigned(page_blocks + q_blocks)), dim3(THREADS), 0,
+                   s, 1, true, a, int(page_blocks), warps, status_word(current_device()));
+}
+
+template <typename T, bool VEC, bool HALF>
+static cudaError_t launch_page(const dspark_paged_append_args& a, cudaStream_t s) {
+  const int parts = a.page * a.D / 16;  // 64 to 1024 threads' worth of 16 values
+  if (parts <= 128) return launch_as<T, VEC, HALF, 1, 128>(a, s);
+  if (parts <= 256) return launch_as<T, VEC, HALF, 2, 128>(a, s);
+  if (parts <= 512) return launch_as<T, VEC, HALF, 4, 128>(a, s);
+  return launch_as<T, VEC, HALF, 4, 256>(a, s);
+}
+
+template <typename T>
+static cudaError_t launch(const dspark_paged_append_args& a, bool vec, cudaStream_t s) {
+  const bool half = a.layout == DSPARK_ROPE_HALF;
+  if (vec) return half ? launch_page<T, true, true>(a, s) : launch_page<T, true, false>(a, s);
+  return half ? launch_page<T, false, true>(a, s) : launch_page<T, false, false>(a, s);
+}
+
+}  // namespace paged
+}  // namespace dspark
+
+using namespace dspark;
+
+extern "C" int dspark_paged_append(const dspark_paged_append_args* p, void* stream) {
+  if (!p) return fail(DSPARK_ERR_ARG, "paged_append: null argument");
+  const dspark_paged_append_args& a = *p;
+  if (a.R < 0 || a.B < 0 || a.Hq <= 0 || a.Hk <= 0 || a.n_pages < 0 || a.max_pages < 0)
+    return fail(DSPARK_ERR_ARG, "paged_append: bad shape (%d rows, %d requests, %d / %d heads, %d pages)", a.R, a.B,
+                a.Hq, a.Hk, a.n_pages);
+  if (a.dtype != DSPARK_DTYPE_BF16 && a.dtype != DSPARK_DTYPE_F16)
+    return fail(DSPARK_ERR_UNSUPPORTED, "paged_append: dtype %d (bf16 = 0, fp16 = 1)", a.dtype);
+  if (a.layout != DSPARK_ROPE_HALF && a.layout != DSPARK_ROPE_INTERLEAVED)
+    return fail(DSPARK_ERR_ARG, "paged_append: layout %d", a.layout);
+  if (a.D != 64 && a.D != 128) return fail(DSPARK_ERR_UNSUPPORTED, "paged_append: head_dim %d (64 or 128)", a.D);
+  if (a.page != 16 && a.page != 32 && a.page != 64 && a.page != 128)
+    return fail(DSPARK_ERR_UNSUPPORTED, "paged_append: pages of %d tokens (16, 32, 64 or 128)", a.page);
+  if (a.rot <= 0 || a.rot % 16 || a.rot > a.D)
+    return fail(DSPARK_ERR_UNSUPPORTED, "paged_append: rotary dim %d of %d (a multiple of 16)", a.rot, a.D);
+  if (a.B == 0) return DSPARK_OK;
+  if (!a.freq || !a.cu_rows || !a.kv_len || (a.max_pages && !a.page_table))
+    return fail(DSPARK_ERR_ARG, "paged_append: null pointer");
+  if (a.R && (!a.q || !a.q_out || !a.k || !a.v || !a.k_pages || !a.v_pages || !a.k_scale || !a.v_scale))
+    return fail(DSPARK_ERR_ARG, "paged_append: null pointer");
+  bool codes = true;
+  for (const void* x : {a.k_pages, a.v_pages}) codes &= reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  for (int i = 0; i < 3; ++i) codes &= a.kp_strides[i] % 16 == 0 && a.vp_strides[i] % 16 == 0;
+  if (!codes) return fail(DSPARK_ERR_UNSUPPORTED, "paged_append: the pages' rows must be 16-byte aligned");
+  bool vec = true;
+  for (const void* x : {a.q, a.k, a.v, (const void*)a.q_out}) vec &= reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  for (int i = 0; i < 2; ++i)
+    vec &= a.q_strides[i] % 8 == 0 && a.k_strides[i] % 8 == 0 && a.v_strides[i] % 8 == 0 && a.qo_strides[i] % 8 == 0;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  DSPARK_CUDA_TRY(a.dtype == DSPARK_DTYPE_BF16 ? paged::launch<bf16>(a, vec, s) : paged::launch<__half>(a, vec, s),
+                  "paged_append");
+  return DSPARK_OK;
+}

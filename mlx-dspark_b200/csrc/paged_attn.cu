@@ -1,0 +1,734 @@
+// Attention of packed rows over pages of 8-bit values with a scale a page and head (dspark_paged_attn).
+//
+// out_i = sum_j p_ij v_j / sum_j p_ij, p_ij = exp(scale q_i.k_j - m_i), k_j = code * ks(page of j), v_j = code * vs.
+// Neither scale is ever multiplied into a code: with x_ij = log2(e) scale ks (q_i.code_j) + log2(vs) and
+// p'_ij = 2^(x_ij - max x), the sum over p' code_v is the numerator and the sum over p' / vs the denominator. The
+// codes go to the tensor core as fp16, which holds every e4m3 value, converted in registers on the way.
+//
+// Rows and items. The G = Hq / Hk heads of a kv head share its keys: row node * G + g of a product. An item is RB = 16
+// or 32 rows of one (request, kv head), its work the key tiles (128 keys) that its last row sees. All items' costs
+// lie in one line (requests in order, a request's heads, a head's row blocks), which is cut into equal shares, one a
+// block of a resident grid, from the lengths on the device (shares, Walker). A block that has a whole item writes the
+// output; of a cut item each block leaves an fp32 part, and a second launch joins the parts in order.
+//
+// Block: four warps, each on its own: a warp takes every fourth subtile of 32 keys of the segment, with a ring of
+// its own in shared memory that it fills itself (16-byte cp.async, no block-wide wait in the loop), its own running
+// maximum and its own O in registers; they are joined at the segment's end.
+// mma.m16n8k16: S = Q K^T with the head's values dealt to the four lanes of a key so that a lane reads 16 codes at a
+// time, O += P V with V transposed by ldmatrix in pairs of values.
+//
+// Rounding: q is used as fp16, bf16 rows scaled by a power of two (exact); weights p' are rounded to fp16, 2^11 times
+// as large, so that what a long tail loses is below 2^-35 of the largest a key; scores, sums and O are fp32.
+#include <algorithm>
+
+#include "host_common.h"
+#include "paged.cuh"
+
+namespace dspark {
+namespace paged {
+
+constexpr int BN = 128;      // keys a tile
+constexpr int SUB = 32;      // keys a warp's subtile
+constexpr int WARPS = 4;
+constexpr int NTHR = WARPS * 32;
+constexpr int NS = 3;        // ring buffers a warp
+constexpr int MAX_CTA = 320;
+constexpr int SEG = 3;       // cost of a segment, in tiles
+constexpr float LIFT = 11.f; // weights are 2^11 times as large in fp16 ...
+constexpr float SLACK = 4.f; // ... and the maximum in use may be 2^4 too low
+
+template <int D, int RT>
+struct Lay {
+  static constexpr int RB = 16 * RT;
+  static constexpr int TILE = SUB * D;                // a subtile's K or V codes
+  static constexpr int STAGE = 2 * TILE + 32;         // K, V, two pages' scales
+  static constexpr int RING = NS * STAGE;             // a warp's
+  static constexpr int Q = 0;                         // fragments [rt][step][lane] of 16 bytes
+  static constexpr int QF = Q + RB * D * 2;           // the rows' powers of two
+  static constexpr int ML = QF + RB * 4;              // (m, l) [warp][row]
+  static constexpr int BUF = ML + WARPS * RB * 8;
+  static constexpr int O = WARPS * RB * (D + 4) * 4;  // O [warp][row][D + 4] takes the rings' place
+  static constexpr int SIZE = WARPS * RING > O ? WARPS * RING : O;
+  static constexpr int TOTAL = BUF + SIZE;
+  static_assert(BUF % 16 == 0 && STAGE % 16 == 0, "16-byte copies");
+};
+
+__device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) { return Elem<__half>::pack(a, b); }
+
+// 16-byte chunk c of a subtile's row, swizzled so that the eight rows of an ldmatrix and the eight lanes of a 16-byte
+// load meet different banks.
+template <int D>
+__device__ __forceinline__ uint32_t at_chunk(int row, int c) {
+  return uint32_t(row * D + ((D == 128 ? c ^ (row & 7) : c ^ ((row >> 1) & 3)) << 4));
+}
+
+// ------------------------------------------------------------------ shares and segments
+
+struct Shape {
+  int rows, r0;       // packed rows, the first of them
+  int len, before;    // keys that there are, those before the rows' own
+  int M, T;           // row blocks, tiles that a row block costs (on average)
+};
+
+template <int RB>
+struct Plan {
+  const dspark_paged_attn_args& a;
+  int seg;  // cost of a segment
+
+  // Tiles of row block m: up to the last key that one of its rows sees, and one at least.
+  __device__ __forceinline__ int tiles(const Shape& s, int m) const {
+    const int G = a.Hq / a.Hk, last = min(s.rows - 1, ((m + 1) * RB - 1) / G);
+    const int n = a.causal ? min(s.len, s.before + last + 1) : s.len;
+    return max(1, (n + BN - 1) / BN);
+  }
+  __device__ __forceinline__ Shape shape(int b) const {
+    Shape s;
+    s.r0 = first_row(a.cu_rows, b, a.R);
+    s.rows = max(first_row(a.cu_rows, b + 1, a.R) - s.r0, 0);
+    const int len = max(a.kv_len[b], 0);
+    s.len = min(len, a.max_pages * a.page);
+    s.before = len - s.rows;
+    const int G = a.Hq / a.Hk;
+    s.M = (s.rows * G + RB - 1) / RB;
+    s.T = s.M ? (tiles(s, 0) + tiles(s, s.M - 1) + 1) >> 1 : 0;
+    return s;
+  }
+};
+
+// The line of costs cut into n shares.
+struct Deal {
+  int64_t q, rem, total;
+  int n;
+  __device__ __forceinline__ Deal(int64_t t, int most) : total(t), n(int(min(int64_t(most), t))) {
+    q = n ? t / n : 0;
+    rem = n ? t - q * n : 0;
+  }
+  __device__ __forceinline__ int64_t from(int c) const { return c < n ? c * q + min(int64_t(c), rem) : total; }
+  __device__ __forceinline__ int owner(int64_t x) const {
+    const int64_t wide = rem * (q + 1);
+    return x < wide ? int(x / (q + 1)) : int(rem + (x - wide) / q);
+  }
+};
+
+// A run of tiles [t0, t1) of one item.
+struct Segment {
+  int b, h, r0, rows, len, before;
+  int row_base, live;  // the item's first (node, head) row, how many
+  int t0, t1;
+  int first, parts;    // block of the item's first part, parts (1: whole)
+};
+
+template <int RB>
+struct Walker {
+  int64_t x, end, base;  // next cost, end of the share, first cost of request b
+  int b;
+  Shape s;
+  bool have;
+  __device__ __forceinline__ bool next(const Plan<RB>& p, const Deal& deal, Segment& g) {
+    const dspark_paged_attn_args& a = p.a;
+    while (x < end) {
+      if (!have) s = p.shape(b);
+      have = true;
+      const int item = p.seg + s.T;
+      const int64_t all = int64_t(s.M) * a.Hk * item;
+      if (x >= base + all) {
+        base += all;
+        ++b;
+        have = false;
+        continue;
+      }
+      const int i = int((x - base) / item);
+      const int64_t start = base + int64_t(i) * item, stop = start + item;
+      // neighbours in the line are a short and a long row block: shares of equal cost are of equal work
+      const int h = i / s.M, k = i - h * s.M, m = k & 1 ? s.M - 1 - (k >> 1) : k >> 1;
+      const int T = p.tiles(s, m);
+      auto tile_at = [&](int64_t y) {
+        const int64_t d = y - start - p.seg;
+        return d <= 0 ? 0 : d >= s.T ? T : int(d * T / s.T);
+      };
+      g.b = b;
+      g.h = h;
+      g.r0 = s.r0;
+      g.rows = s.rows;
+      g.len = s.len;
+      g.before = s.before;
+      g.row_base = m * RB;
+      g.live = min(s.rows * (a.Hq / a.Hk) - g.row_base, RB);
+      g.t0 = tile_at(x);
+      g.t1 = end >= stop ? T : tile_at(end);
+      g.first = deal.owner(start);
+      g.parts = deal.owner(stop - 1) - g.first + 1;
+      x = min(stop, end);
+      return true;
+    }
+    return false;
+  }
+};
+
+// ------------------------------------------------------------------ workspace
+
+// What a block tells the join of the cut item whose first part it has (parts 0: none).
+struct Cut {
+  int parts, r0, live, row_base, h, pad[3];
+};
+
+template <int D, int RB>
+__host__ __device__ constexpr size_t part_floats() {
+  return size_t(RB) * (D + 1);
+}
+template <int D, int RB>
+__device__ __forceinline__ float* part_of(void* ws, int cta, int which) {
+  return reinterpret_cast<float*>(static_cast<Cut*>(ws) + MAX_CTA) + (size_t(cta) * 2 + which) * part_floats<D, RB>();
+}
+
+// ------------------------------------------------------------------ the kernel
+
+template <typename T, int D, int RT>
+__global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_args a, const float c_log2, int* status) {
+  typedef Lay<D, RT> L;
+  constexpr int RB = L::RB, KS = D / 16, CH = D / 16;  // k steps of the scores, 16-byte chunks a row
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int64_t s_cost[WARPS];
+  __shared__ int64_t s_base;
+  __shared__ int s_req;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, qd = lane & 3;  // row (or key) and quarter of an mma fragment
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // ---- this block's share: the first request of it
+  Plan<RB> plan{a, SEG};
+  int64_t total = 0, tiles = 0;
+  auto cost_of = [&](int b, int seg) {
+    if (b >= a.B) return int64_t(0);
+    const Shape s = plan.shape(b);
+    return int64_t(s.M) * a.Hk * (seg + s.T);
+  };
+  auto block_sum = [&](int64_t v) {
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if (lane == 0) s_cost[warp] = v;
+    __syncthreads();
+    return s_cost[0] + s_cost[1] + s_cost[2] + s_cost[3];
+  };
+  for (int b0 = 0; b0 < a.B; b0 += NTHR) {
+    tiles += block_sum(cost_of(b0 + tid, 0));
+    total += block_sum(cost_of(b0 + tid, SEG));
+  }
+  if (tiles <= int64_t(gridDim.x)) {  // a tile a block: nothing is gained by fuller shares
+    plan.seg = 0;
+    total = tiles;
+  }
+  const Deal deal(total, int(gridDim.x));
+  Walker<RB> wk;
+  wk.x = deal.from(blockIdx.x);
+  wk.end = deal.from(blockIdx.x + 1);
+  wk.have = false;
+  if (tid == 0) s_req = a.B;
+  int64_t at = 0;
+  for (int b0 = 0; b0 < a.B && wk.x < wk.end; b0 += NTHR) {
+    const int64_t v = cost_of(b0 + tid, plan.seg);
+    int64_t sum = v;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    __syncthreads();
+    if (lane == 31) s_cost[warp] = sum;
+    __syncthreads();
+    int64_t before = at + sum - v;
+    for (int w = 0; w < warp; ++w) before += s_cost[w];
+    if (v > 0 && wk.x >= before && wk.x < before + v) {
+      s_req = b0 + tid;
+      s_base = before;
+    }
+    at += s_cost[0] + s_cost[1] + s_cost[2] + s_cost[3];
+  }
+  __syncthreads();
+  wk.b = s_req;
+  wk.base = s_base;
+  Cut cut{0, 0, 0, 0, 0, {0, 0, 0}};
+
+  const int G = a.Hq / a.Hk, shift = 31 - __clz(a.page);
+  uint8_t* ring = smem + L::BUF + warp * L::RING;
+  const uint32_t ring_a = smem_u32(ring);
+  const uint32_t q_a = smem_u32(smem + L::Q) + lane * 16;
+  float* rowf = reinterpret_cast<float*>(smem + L::QF);
+  float2* ml = reinterpret_cast<float2*>(smem + L::ML);
+  float* merge = reinterpret_cast<float*>(smem + L::BUF);
+
+  Segment s;
+  while (wk.next(plan, deal, s)) {
+    const int sub0 = s.t0 * (BN / SUB) + warp, sub1 = min(s.t1 * (BN / SUB), (s.len + SUB - 1) / SUB);
+    const int n = sub0 < sub1 ? (sub1 - sub0 + WARPS - 1) / WARPS : 0;
+    const int32_t* table = a.page_table + int64_t(s.b) * a.table_stride;
+    const uint8_t* kp = static_cast<const uint8_t*>(a.k_pages) + s.h * a.kp_strides[1];
+    const uint8_t* vp = static_cast<const uint8_t*>(a.v_pages) + s.h * a.vp_strides[1];
+
+    // Lane 0 and 1: the subtile's page or pages (16 tokens: two), -1 where there is none to read.
+    auto page_id = [&](int i) {
+      int id = -1;
+      const int key = (sub0 + i * WARPS) * SUB + lane * 16;
+      if (lane < (shift == 4 ? 2 : 1) && i < n && key < s.len) {
+        id = table[key >> shift];
+        if (id < 0 || id >= a.n_pages) {
+          report_error(status, kErrAttnPage);
+          id = -1;
+        }
+      }
+      return id;
+    };
+    int ahead = page_id(0);
+    auto issue = [&](int i) {
+      const int mine = ahead;
+      ahead = page_id(i + 1);
+      if (i < n) {
+        const uint32_t dst = ring_a + (i % NS) * L::STAGE;
+        const int key0 = (sub0 + i * WARPS) * SUB;
+        if (lane < 2) {
+          const int id = shift == 4 ? mine : __shfl_sync(3u, mine, 0);
+          const int64_t at_s = int64_t(id) * a.scale_strides[0] + s.h * a.scale_strides[1];
+          const uint32_t to = dst + 2 * L::TILE + lane * 8;
+          const float* ks = a.k_scale + (id < 0 ? 0 : at_s);
+          const float* vs = a.v_scale + (id < 0 ? 0 : at_s);
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(ks), "r"(id < 0 ? 0 : 4) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 4), "l"(vs), "r"(id < 0 ? 0 : 4)
+                       : "memory");
+        }
+        __syncwarp();
+        const int id0 = __shfl_sync(0xffffffffu, mine, 0), id1 = __shfl_sync(0xffffffffu, mine, 1);
+#pragma unroll
+        for (int z = 0; z < SUB * CH / 32; ++z) {
+          const int row = (z * 32 + lane) / CH, c = lane % CH;
+          const int id = shift == 4 && row >= 16 ? id1 : id0, key = key0 + row;
+          const bool there = id >= 0 && key < s.len;
+          const int tok = key & (a.page - 1);
+          const int64_t ko = there ? id * a.kp_strides[0] + tok * a.kp_strides[2] + c * 16 : 0;
+          const int64_t vo = there ? id * a.vp_strides[0] + tok * a.vp_strides[2] + c * 16 : 0;
+          cp_async_16_zfill(dst + at_chunk<D>(row, c), kp + ko, there);
+          cp_async_16_zfill(dst + L::TILE + at_chunk<D>(row, c), vp + vo, there);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) issue(i);
+
+    // ---- Q as fp16 fragments. 16 neighbouring values of a row a thread and round.
+    {
+      constexpr int PER = D / 16;  // threads a row
+#pragma unroll
+      for (int z = 0; z < RB * PER / NTHR + (RB * PER % NTHR ? 1 : 0); ++z) {
+        const int r = (z * NTHR + tid) / PER, p = tid % PER;
+        uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        const bool mine = r < RB && r < s.live;
+        if (mine) {
+          const int node = (s.row_base + r) / G, hq = s.h * G + s.row_base + r - node * G;
+          const T* q = static_cast<const T*>(a.q) + int64_t(s.r0 + node) * a.q_strides[0] + hq * a.q_strides[1] + p * 16;
+          const uint4 x0 = ldcg_v4(q), x1 = ldcg_v4(q + 8);
+          w[0] = x0.x; w[1] = x0.y; w[2] = x0.z; w[3] = x0.w;
+          w[4] = x1.x; w[5] = x1.y; w[6] = x1.z; w[7] = x1.w;
+        }
+        float f = 1.f;
+        if (std::is_same<T, bf16>::value) {  // largest exponent of the row; 255: infinite or NaN
+          uint32_t e = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) e = max(e, max((w[i] >> 7) & 0xffu, (w[i] >> 23) & 0xffu));
+#pragma unroll
+          for (int o = 1; o < PER; o <<= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, o));
+          // values below 2^15: the row divided by 2^(e - 127 - 14); in two steps, where that is no fp32 value
+          const int up = int(e) - 141;
+          const float inv = pow2(max(min(-up, 126), -126));
+          f = e == 255 ? NAN : pow2(max(min(up, 126), -126));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = pack_f16(bf16_lo(w[i]) * inv, bf16_hi(w[i]) * inv);
+        } else {  // an infinite q makes its row NaN whatever the codes are
+          bool bad = false;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) bad |= (w[i] & 0x7c00u) == 0x7c00u || (w[i] & 0x7c000000u) == 0x7c000000u;
+          uint32_t any = bad;
+#pragma unroll
+          for (int o = 1; o < PER; o <<= 1) any |= __shfl_xor_sync(0xffffffffu, any, o);
+          f = any ? NAN : 1.f;
+        }
+        if (r < RB) {
+          if (p == 0) rowf[r] = f * c_log2;
+          // value d = quarter * D / 4 + step * 4 + j
+          const int quarter = p * 16 / (D / 4), step0 = (p * 16 % (D / 4)) / 4, rt = r >> 4, rr = r & 15;
+          uint32_t* to = reinterpret_cast<uint32_t*>(smem + L::Q) + (rr >> 3);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int f0 = ((rt * KS + step0 + i) * 32 + (rr & 7) * 4 + quarter) * 4;
+            to[f0] = w[2 * i];
+            to[f0 + 2] = w[2 * i + 1];
+          }
+        }
+      }
+    }
+    __syncthreads();
+
+    float o[RT][D / 8][4], m[RT][2], l[RT][2], rf[RT][2];
+    int lim[RT][2];  // keys that the thread's rows see
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int x = 0; x < D / 8; ++x) o[rt][x][0] = o[rt][x][1] = o[rt][x][2] = o[rt][x][3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = rt * 16 + i * 8 + g;
+        m[rt][i] = -INFINITY;
+        l[rt][i] = 0.f;
+        rf[rt][i] = rowf[r];
+        const int place = min((s.row_base + r) / G, s.rows - 1);
+        lim[rt][i] = a.causal ? min(s.len, s.before + place + 1) : s.len;
+      }
+    }
+    const int edge0 = (a.causal ? min(s.len, s.before + s.row_base / G + 1) : s.len) - SUB;  // later: hidden keys
+
+    for (int i = 0; i < n; ++i) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(NS - 2) : "memory");
+      __syncwarp();
+      issue(i + NS - 1);
+      const int key0 = (sub0 + i * WARPS) * SUB;
+      const uint32_t kt = ring_a + (i % NS) * L::STAGE, vt = kt + L::TILE;
+      const float2 sc0 = *reinterpret_cast<const float2*>(ring + (i % NS) * L::STAGE + 2 * L::TILE);
+      const float2 sc1 = *reinterpret_cast<const float2*>(ring + (i % NS) * L::STAGE + 2 * L::TILE + 8);
+      // pages without a positive scale (absent ones have 0) are not seen
+      const bool ok0 = sc0.x > 0.f && sc0.y > 0.f, ok1 = sc1.x > 0.f && sc1.y > 0.f;
+      const bool edge = key0 > edge0 || !ok0 || !ok1;
+
+      // ---- scores
+      float x[RT][4][4];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[rt][t][0] = x[rt][t][1] = x[rt][t][2] = x[rt][t][3] = 0.f;
+#pragma unroll
+      for (int half = 0; half < KS / 4; ++half) {  // 16 codes of a key, four steps
+        uint4 kw[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          kw[t] = lds128(kt + at_chunk<D>(t * 8 + g, qd * (KS / 4) + half));
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+          uint32_t qf[RT][4];
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            const uint4 y = lds128(q_a + ((rt * KS + half * 4 + st) * 32) * 16);
+            qf[rt][0] = y.x; qf[rt][1] = y.y; qf[rt][2] = y.z; qf[rt][3] = y.w;
+          }
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const uint32_t w = st == 0 ? kw[t].x : st == 1 ? kw[t].y : st == 2 ? kw[t].z : kw[t].w;
+            const uint32_t b0 = e4m3_to_f16(w), b1 = e4m3_to_f16_hi(w);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) mma_f16(x[rt][t], qf[rt], b0, b1);
+          }
+        }
+      }
+
+      // ---- weights
+      const float lv0 = lg2(sc0.y), lv1 = lg2(sc1.y), iv0 = ok0 ? 1.f / sc0.y : 0.f, iv1 = ok1 ? 1.f / sc1.y : 0.f;
+      uint32_t pw[RT][4][2];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const float ks = t < 2 ? sc0.x : sc1.x, lv = t < 2 ? lv0 : lv1;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float y = fmaf(x[rt][t][e], rf[rt][e >> 1] * ks, lv);
+            if (edge) {
+              const int key = key0 + t * 8 + 2 * qd + (e & 1);
+              if (!(key < lim[rt][e >> 1] && (t < 2 ? ok0 : ok1))) y = -INFINITY;
+            }
+            x[rt][t][e] = y;
+            mx[e >> 1] = fmaxf(mx[e >> 1], y);
+          }
+        }
+        const bool up = mx[0] > m[rt][0] + SLACK || mx[1] > m[rt][1] + SLACK;
+        if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float y = mx[k];
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
+            if (y > m[rt][k]) {
+              const float f = ex2(m[rt][k] - y);  // (0 at first)
+              m[rt][k] = y;
+              l[rt][k] *= f;
+#pragma unroll
+              for (int z = 0; z < D / 8; ++z) {
+                o[rt][z][2 * k] *= f;
+                o[rt][z][2 * k + 1] *= f;
+              }
+            }
+          }
+        }
+        float ref[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) ref[k] = (m[rt][k] == -INFINITY ? 0.f : m[rt][k]) - LIFT;
+        float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};  // [page][row]
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const float e0 = ex2(x[rt][t][0] - ref[0]), e1 = ex2(x[rt][t][1] - ref[0]);
+          const float e2 = ex2(x[rt][t][2] - ref[1]), e3 = ex2(x[rt][t][3] - ref[1]);
+          sum[t >> 1][0] += e0 + e1;
+          sum[t >> 1][1] += e2 + e3;
+          pw[rt][t][0] = pack_f16(e0, e1);
+          pw[rt][t][1] = pack_f16(e2, e3);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) l[rt][k] += sum[0][k] * iv0 + sum[1][k] * iv1;
+      }
+
+      // ---- O += P V
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {  // 16 keys
+#pragma unroll
+        for (int c = 0; c < CH; c += 2) {
+          uint32_t w[4];
+          const int row = j * 16 + (lane & 15), ch = c + (lane >> 4);
+          ldmatrix_x4_trans(vt + at_chunk<D>(row, ch), w[0], w[1], w[2], w[3]);
+          if (edge) {
+            // A NaN code reaches only the rows that see its key: it is taken out, and its place counted.
+            bool bad = false;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) bad |= (((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+            if (__any_sync(0xffffffffu, bad)) {
+              uint32_t is[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t nan = (((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+                is[k] = nan * 0x38u;    // e4m3's 1
+                w[k] &= ~(nan * 0xffu);
+              }
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt) {
+                uint32_t see[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const int t = 2 * j + (k >> 1), key = key0 + t * 8 + 2 * qd, li = lim[rt][k & 1];
+                  const bool ok = t < 2 ? ok0 : ok1;
+                  see[k] = (ok && key < li ? 0x3c00u : 0u) | (ok && key + 1 < li ? 0x3c000000u : 0u);
+                }
+#pragma unroll
+                for (int cc = 0; cc < 2; ++cc) {
+                  const uint32_t y0 = __byte_perm(is[2 * cc], 0, 0x3120), y1 = __byte_perm(is[2 * cc + 1], 0, 0x3120);
+                  float n0[4] = {0.f, 0.f, 0.f, 0.f}, n1[4] = {0.f, 0.f, 0.f, 0.f};
+                  mma_f16(n0, see, e4m3_to_f16(y0), e4m3_to_f16(y1));
+                  mma_f16(n1, see, e4m3_to_f16_hi(y0), e4m3_to_f16_hi(y1));
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    if (n0[e] > 0.f) o[rt][2 * (c + cc)][e] = NAN;
+                    if (n1[e] > 0.f) o[rt][2 * (c + cc) + 1][e] = NAN;
+                  }
+                }
+              }
+            }
+          }
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            const uint32_t y0 = __byte_perm(w[2 * cc], 0, 0x3120), y1 = __byte_perm(w[2 * cc + 1], 0, 0x3120);
+            const uint32_t a0 = e4m3_to_f16(y0), a1 = e4m3_to_f16(y1);
+            const uint32_t b0 = e4m3_to_f16_hi(y0), b1 = e4m3_to_f16_hi(y1);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+              const uint32_t p[4] = {pw[rt][2 * j][0], pw[rt][2 * j][1], pw[rt][2 * j + 1][0], pw[rt][2 * j + 1][1]};
+              mma_f16(o[rt][2 * (c + cc)], p, a0, a1);      // values 16 c + 2 n
+              mma_f16(o[rt][2 * (c + cc) + 1], p, b0, b1);  // values 16 c + 2 n + 1
+            }
+          }
+        }
+      }
+    }
+
+    // ---- the warps' parts joined
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float y = l[rt][k];
+        y += __shfl_xor_sync(0xffffffffu, y, 1);
+        y += __shfl_xor_sync(0xffffffffu, y, 2);
+        const int r = rt * 16 + k * 8 + g;
+        if (qd == 0) ml[warp * RB + r] = make_float2(m[rt][k], y);
+        float* to = merge + (warp * RB + r) * (D + 4) + 4 * qd;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+          *reinterpret_cast<float4*>(to + 16 * c) = make_float4(o[rt][2 * c][2 * k], o[rt][2 * c + 1][2 * k],
+                                                                o[rt][2 * c][2 * k + 1], o[rt][2 * c + 1][2 * k + 1]);
+      }
+    }
+    __syncthreads();
+    const bool whole = s.parts == 1;
+    const int which = int(blockIdx.x) == s.first;
+    float* part = whole ? nullptr : part_of<D, RB>(a.workspace, blockIdx.x, which);
+    if (!whole && which) cut = Cut{s.parts, s.r0, s.live, s.row_base, s.h, {0, 0, 0}};
+#pragma unroll 4
+    for (int z = tid; z < RB * (D / 4); z += NTHR) {
+      const int r = z / (D / 4), d = z % (D / 4) * 4;
+      if (r >= s.live) break;
+      float2 y[WARPS];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        y[w] = ml[w * RB + r];
+        mx = fmaxf(mx, y[w].x);
+      }
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      float sum = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float f = ex2(y[w].x - ref);
+        const float4 u = *reinterpret_cast<const float4*>(merge + (w * RB + r) * (D + 4) + d);
+        sum += y[w].y * f;
+        v.x += u.x * f;
+        v.y += u.y * f;
+        v.z += u.z * f;
+        v.w += u.w * f;
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (nothing seen: v is zero)
+      v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+      if (whole) {
+        const int node = (s.row_base + r) / G, hq = s.h * G + s.row_base + r - node * G;
+        T* out = static_cast<T*>(a.out) + int64_t(s.r0 + node) * a.o_strides[0] + hq * a.o_strides[1] + d;
+        *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w));
+      } else {
+        *reinterpret_cast<float4*>(part + r * D + d) = v;
+        if (d == 0) part[RB * D + r] = sum == 0.f ? -INFINITY : ref + lg2(sum);
+      }
+    }
+    __syncthreads();  // the rings and Q are free again
+  }
+  if (tid == 0) static_cast<Cut*>(a.workspace)[blockIdx.x] = cut;
+}
+
+// One warp a row of a cut item: its parts in order.
+template <typename T, int D, int RB>
+__global__ void __launch_bounds__(128) join_kernel(const dspark_paged_attn_args a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, r = blockIdx.y * 4 + (threadIdx.x >> 5);
+  const Cut* cuts = static_cast<const Cut*>(a.workspace);
+  const int cta = blockIdx.x;
+  const Cut c = cuts[cta];
+  if (r >= c.live || c.parts == 0) return;
+  constexpr int V = D / 32;
+  auto at = [&](int x) { return part_of<D, RB>(a.workspace, cta + x, x == 0); };
+  float m = -INFINITY, sum = 0.f, v[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = 0.f;
+  for (int x = lane; x < c.parts; x += 32) m = fmaxf(m, __ldcg(at(x) + RB * D + r));
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 8
+  for (int x = 0; x < c.parts; ++x) {
+    const float* p = at(x);
+    const float y = __ldcg(p + RB * D + r), f = ex2(y - ref);
+    float u[V];
+    if (V == 4) {
+      const float4 t = __ldcg(reinterpret_cast<const float4*>(p + r * D) + lane);
+      u[0] = t.x; u[1] = t.y; u[V - 2] = t.z; u[V - 1] = t.w;
+    } else {
+      const float2 t = __ldcg(reinterpret_cast<const float2*>(p + r * D) + lane);
+      u[0] = t.x; u[1] = t.y;
+    }
+    if (y == -INFINITY) continue;  // a part that saw nothing
+    sum += f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] += u[i] * f;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int G = a.Hq / a.Hk, node = (c.row_base + r) / G, hq = c.h * G + c.row_base + r - node * G;
+  T* out = static_cast<T*>(a.out) + int64_t(c.r0 + node) * a.o_strides[0] + hq * a.o_strides[1] + lane * V;
+  if (V == 4)
+    *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack(v[0] * inv, v[1] * inv),
+                                                Elem<T>::pack(v[V - 2] * inv, v[V - 1] * inv));
+  else
+    *reinterpret_cast<uint32_t*>(out) = Elem<T>::pack(v[0] * inv, v[1] * inv);
+}
+
+static int grid_of(int device) { return std::min(2 * sm_count(device), MAX_CTA); }
+
+template <typename T, int D, int RT>
+static int launch(const dspark_paged_attn_args& a, cudaStream_t s) {
+  typedef Lay<D, RT> L;
+  const int dev = current_device(), n = grid_of(dev);
+  DSPARK_CUDA_TRY(configure_once((const void*)attn_kernel<T, D, RT>, L::TOTAL,
+                                 [&] {
+                                   return cudaFuncSetAttribute(attn_kernel<T, D, RT>,
+                                                               cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
+                                 }),
+                  "paged_attn: shared memory");
+  const float c = a.scale * 1.4426950408889634f;
+  DSPARK_CUDA_TRY(launch_ex(attn_kernel<T, D, RT>, dim3(n), dim3(NTHR), L::TOTAL, s, 1, true, a, c, status_word(dev)),
+                  "paged_attn");
+  DSPARK_CUDA_TRY(launch_ex(join_kernel<T, D, L::RB>, dim3(n, L::RB / 4), dim3(128), 0, s, 1, true, a), "paged_attn: join");
+  return DSPARK_OK;
+}
+
+template <typename T, int D>
+static int launch_rows(const dspark_paged_attn_args& a, cudaStream_t s) {
+  // rows of a product: 16 where requests have no more on average
+  return int64_t(a.R) * (a.Hq / a.Hk) <= int64_t(16) * a.B ? launch<T, D, 1>(a, s) : launch<T, D, 2>(a, s);
+}
+
+}  // namespace paged
+}  // namespace dspark
+
+using namespace dspark;
+
+extern "C" {
+
+size_t dspark_paged_attn_workspace(int R, int B, int Hq, int Hk, int D) {
+  if (R <= 0 || B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || D <= 0) return 0;
+  return paged::MAX_CTA * sizeof(paged::Cut) +
+         size_t(paged::grid_of(current_device())) * 2 * 32 * (D + 1) * sizeof(float);
+}
+
+int dspark_paged_attn(const dspark_paged_attn_args* p, void* stream) {
+  if (!p) return fail(DSPARK_ERR_ARG, "paged_attn: null argument");
+  const dspark_paged_attn_args& a = *p;
+  if (a.R < 0 || a.B < 0 || a.Hq <= 0 || a.Hk <= 0 || a.Hq % a.Hk || a.n_pages < 0 || a.max_pages < 0)
+    return fail(DSPARK_ERR_ARG, "paged_attn: bad shape (%d rows, %d requests, %d / %d heads, %d pages)", a.R, a.B, a.Hq,
+                a.Hk, a.n_pages);
+  if (a.dtype != DSPARK_DTYPE_BF16 && a.dtype != DSPARK_DTYPE_F16)
+    return fail(DSPARK_ERR_UNSUPPORTED, "paged_attn: dtype %d (bf16 = 0, fp16 = 1)", a.dtype);
+  if (a.D != 64 && a.D != 128) return fail(DSPARK_ERR_UNSUPPORTED, "paged_attn: head_dim %d (64 or 128)", a.D);
+  if (a.page != 16 && a.page != 32 && a.page != 64 && a.page != 128)
+    return fail(DSPARK_ERR_UNSUPPORTED, "paged_attn: pages of %d tokens (16, 32, 64 or 128)", a.page);
+  if (int64_t(a.max_pages) * a.page > 0x3fffffff)
+    return fail(DSPARK_ERR_UNSUPPORTED, "paged_attn: %d pages of %d tokens a request", a.max_pages, a.page);
+  if (int64_t(a.R) * (a.Hq / a.Hk) > 0x3fffffff || (int64_t(a.R) * (a.Hq / a.Hk) / 16 + 1) * a.Hk > 0x3fffffff)
+    return fail(DSPARK_ERR_UNSUPPORTED, "paged_attn: %d rows of %d heads in one call", a.R, a.Hq);
+  if (a.R == 0 || a.B == 0) return DSPARK_OK;
+  if (!a.q || !a.out || !a.cu_rows || !a.kv_len || (a.max_pages && !a.page_table) ||
+      (a.n_pages && (!a.k_pages || !a.v_pages || !a.k_scale || !a.v_scale)))
+    return fail(DSPARK_ERR_ARG, "paged_attn: null pointer");
+  bool aligned = true;
+  for (const void* x : {a.q, a.k_pages, a.v_pages, (const void*)a.out}) aligned &= reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  for (int i = 0; i < 2; ++i) aligned &= a.q_strides[i] % 8 == 0 && a.o_strides[i] % 8 == 0;
+  for (int i = 0; i < 3; ++i) aligned &= a.kp_strides[i] % 16 == 0 && a.vp_strides[i] % 16 == 0;
+  if (!aligned) return fail(DSPARK_ERR_UNSUPPORTED, "paged_attn: rows must be 16-byte aligned");
+  if (!a.workspace || a.ws_bytes < dspark_paged_attn_workspace(a.R, a.B, a.Hq, a.Hk, a.D))
+    return fail(DSPARK_ERR_ARG, "paged_attn: workspace of %zu bytes", a.ws_bytes);
+  if (reinterpret_cast<uintptr_t>(a.workspace) % 16)
+    return fail(DSPARK_ERR_ARG, "paged_attn: the workspace must be 16-byte aligned");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (a.dtype == DSPARK_DTYPE_BF16)
+    return a.D == 128 ? paged::launch_rows<bf16, 128>(a, s) : paged::launch_rows<bf16, 64>(a, s);
+  return a.D == 128 ? paged::launch_rows<__half, 128>(a, s) : paged::launch_rows<__half, 64>(a, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,499 @@
+// Log probabilities of given tokens with the entropy, the token's rank and the top alternatives
+// (dspark_token_logprobs).
+//
+// With x the row's logits, c = 1 / T, m = max x, l = sum exp(c (x - m)), s = sum exp(c (x - m)) c (x - m):
+//   logprob(t) = c (x_t - m) - ln l,   entropy = ln l - s / l,   rank = #{v before t in the order below}.
+// One pass: a thread keeps m, l and s of the values it has seen (fp32), raising m for 64 bytes at a time. The
+// order of tokens is by logit, then the lower token first.
+//
+// Alternatives without a second pass: a thread's m is the largest value of its strip of the row, so the top-th
+// largest m of a block bounds its top-th largest value from below, and only strips whose m reaches it hold any of
+// the block's alternatives: as many strips as alternatives (more with equal values) are read again, from L2.
+//
+// A row is a cluster of 1 to 8 blocks, each with a slice of its 16-byte vectors; the first block joins them.
+// Bound: HBM for many rows, latency for few.
+#include <algorithm>
+#include <cfloat>
+
+#include "elem.cuh"
+#include "host_common.h"
+
+namespace dspark {
+namespace score {
+
+constexpr int THREADS = 256;
+constexpr int U = 4;          // vectors in flight a thread
+constexpr int MAX_TOP = 32;
+constexpr int MAX_CLUSTER = 8;
+constexpr int CAND = 1024;    // values at or above the bound that a block sorts at once
+
+// A logit at or below kLow (NaN and -inf among them) is a masked token's, one above kHigh counts as kHigh.
+constexpr float kLow = -0x1p100f, kHigh = 0x1p100f;
+
+template <typename T>
+struct Vec;
+
+// n = VE values of a 16-byte vector, masked ones as kLow, and the largest of them (not yet held to kHigh).
+template <>
+struct Vec<bf16> {
+  static constexpr int VE = 8;
+  static constexpr float MAXV = kHigh;
+  static __device__ __forceinline__ float split(uint4 w, float* x) {
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+    uint32_t mx = 0xF180F180u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t y;  // (the number of the two where one is NaN)
+      asm("max.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(in[i]), "r"(0xF180F180u));
+      asm("max.bf16x2 %0, %0, %1;" : "+r"(mx) : "r"(y));
+      x[2 * i] = bf16_lo(y);
+      x[2 * i + 1] = bf16_hi(y);
+    }
+    return fmaxf(bf16_lo(mx), bf16_hi(mx));
+  }
+  static __device__ __forceinline__ float one(bf16 v) { return fmaxf(__bfloat162float(v), kLow); }
+};
+
+template <>
+struct Vec<__half> {
+  static constexpr int VE = 8;
+  static constexpr float MAXV = 65504.f;
+  static __device__ __forceinline__ float split(uint4 w, float* x) {
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+    uint32_t mx = 0xFBFFFBFFu;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t y;
+      asm("max.f16x2 %0, %1, %2;" : "=r"(y) : "r"(in[i]), "r"(0xFBFFFBFFu));
+      asm("max.f16x2 %0, %0, %1;" : "+r"(mx) : "r"(y));
+      const float2 f = Elem<__half>::unpack(y);
+      x[2 * i] = f.x <= -65504.f ? kLow : f.x;
+      x[2 * i + 1] = f.y <= -65504.f ? kLow : f.y;
+    }
+    const float2 f = Elem<__half>::unpack(mx);
+    const float m = fmaxf(f.x, f.y);
+    return m <= -65504.f ? kLow : m;
+  }
+  static __device__ __forceinline__ float one(__half v) {
+    const float f = fmaxf(__half2float(v), -65504.f);
+    return f <= -65504.f ? kLow : f;
+  }
+};
+
+template <>
+struct Vec<float> {
+  static constexpr int VE = 4;
+  static constexpr float MAXV = kHigh;
+  static __device__ __forceinline__ float split(uint4 w, float* x) {
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = fmaxf(__uint_as_float(in[i]), kLow);
+    return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+  }
+  static __device__ __forceinline__ float one(float v) { return fmaxf(v, kLow); }
+};
+
+// What a part of a row adds up to; sums are in units of log2.
+struct Sums {
+  float m, l, s;
+};
+
+__device__ __forceinline__ void raise(Sums& a, float m, float c) {
+  const float d = (a.m - m) * c;  // at most 0
+  a.m = m;
+  if (d < -200.f) {  // (also the start, where m was kLow)
+    a.l = 0.f;
+    a.s = 0.f;
+  } else {
+    const float f = ex2(d);
+    a.s = f * (a.s + d * a.l);
+    a.l *= f;
+  }
+}
+
+__device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  raise(a, m, c);
+  raise(b, m, c);
+  return Sums{m, a.l + b.l, a.s + b.s};
+}
+
+// Larger first, then the lower token.
+__device__ __forceinline__ uint64_t key_of(float x, int v) {
+  const uint32_t b = __float_as_uint(x);
+  return uint64_t(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | uint32_t(~v);
+}
+__device__ __forceinline__ float value_of(uint64_t key) {
+  const uint32_t b = uint32_t(key >> 32);
+  return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
+
+struct Shared {
+  Sums warp[THREADS / 32];
+  int rank[THREADS / 32];
+  uint64_t top[MAX_TOP];  // the block's alternatives in order, 0 behind the last
+  Sums sum;
+  int before;
+  float bound;
+  int n_strip, n_cand;
+  uint64_t best[THREADS / 32];
+  uint64_t cand[CAND];    // at first the threads' maxima
+  uint16_t strip[THREADS];
+};
+
+__device__ __forceinline__ uint64_t remote_u64(const void* p, uint32_t rank) {
+  uint64_t v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
+
+template <typename T>
+struct Row {
+  const T* p;     // the row
+  int V, head;    // values, those before the first 16-byte vector
+  int nvec;       // vectors
+  int v0, v1;     // the block's
+  bool first, last;
+};
+
+// Sorts the block's candidates sh.cand[0 .. n) by counting into sh.top.
+__device__ __forceinline__ void place_top(Shared& sh, const uint64_t* cand, int n, int top, uint64_t* out) {
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const uint64_t k = cand[i];
+    int before = 0;
+    for (int j = 0; j < n; ++j) before += cand[j] > k;
+    if (before < top && k) out[before] = k;
+  }
+}
+
+// The block's alternatives into sh.top. m: the largest value of the thread's strip.
+template <typename T>
+__device__ __noinline__ void find_top(Shared& sh, const Row<T>& r, float m, int top) {
+  constexpr int VE = Vec<T>::VE;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  float* maxima = reinterpret_cast<float*>(sh.cand);
+  maxima[tid] = m;
+  if (tid < MAX_TOP) sh.top[tid] = 0;
+  if (tid == 0) sh.n_strip = sh.n_cand = 0;
+  __syncthreads();
+  if (warp == 0) {  // the top-th largest maximum, bit by bit from above
+    uint32_t b[THREADS / 32], t = 0;
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) b[i] = uint32_t(key_of(maxima[32 * i + lane], 0) >> 32);
+#pragma unroll 1
+    for (int bit = 31; bit >= (sizeof(T) == 2 ? 13 : 0); --bit) {
+      const uint32_t y = t | 1u << bit;
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < THREADS / 32; ++i) n += b[i] >= y;
+      if (int(__reduce_add_sync(0xffffffffu, unsigned(n))) >= top) t = y;
+    }
+    if (lane == 0) sh.bound = value_of(uint64_t(t) << 32);
+  }
+  __syncthreads();
+  const float bound = sh.bound;
+  if (m >= bound && m > kLow) sh.strip[atomicAdd(&sh.n_strip, 1)] = uint16_t(tid);
+  __syncthreads();
+  auto offer = [&](float x, int v) {
+    if (x > kLow && x >= bound) {
+      const int at = atomicAdd(&sh.n_cand, 1);
+      if (at < CAND) sh.cand[at] = key_of(x, v);
+    }
+  };
+  const int per = (r.v1 - r.v0 + THREADS - 1) / THREADS, n = sh.n_strip * per;
+  const uint4* vec = reinterpret_cast<const uint4*>(r.p + r.head);
+  for (int j = tid; j < n; j += THREADS) {
+    const int g = j / per, v = r.v0 + (j - g * per) * THREADS + sh.strip[g];
+    if (v >= r.v1) continue;
+    float x[VE];
+    if (Vec<T>::split(ldcg_v4(vec + v), x) < bound) continue;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) offer(fminf(x[e], Vec<T>::MAXV), r.head + v * VE + e);
+  }
+  if (r.first && tid < r.head) offer(fminf(Vec<T>::one(r.p[tid]), Vec<T>::MAXV), tid);
+  const int t0 = r.head + r.nvec * VE;
+  if (r.last && tid < r.V - t0) offer(fminf(Vec<T>::one(r.p[t0 + tid]), Vec<T>::MAXV), t0 + tid);
+  __syncthreads();
+  if (sh.n_cand <= CAND) {
+    place_top(sh, sh.cand, sh.n_cand, top, sh.top);
+    __syncthreads();
+    return;
+  }
+  // Too many equal or nearly equal values for the list: the alternatives one after the other, each by a pass
+  // over the block's slice.
+  uint64_t prev = ~0ull;
+  for (int k = 0; k < top; ++k) {
+    uint64_t best = 0;
+    auto see = [&](float x, int v) {
+      const uint64_t key = key_of(x, v);
+      if (x > kLow && key < prev && key > best) best = key;
+    };
+    for (int v = r.v0 + tid; v < r.v1; v += THREADS) {
+      float x[VE];
+      Vec<T>::split(ldcg_v4(vec + v), x);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) see(fminf(x[e], Vec<T>::MAXV), r.head + v * VE + e);
+    }
+    if (r.first && tid < r.head) see(fminf(Vec<T>::one(r.p[tid]), Vec<T>::MAXV), tid);
+    if (r.last && tid < r.V - t0) see(fminf(Vec<T>::one(r.p[t0 + tid]), Vec<T>::MAXV), t0 + tid);
+    for (int o = 16; o; o >>= 1) best = max(best, uint64_t(__shfl_xor_sync(0xffffffffu, best, o)));
+    if (lane == 0) sh.best[warp] = best;
+    __syncthreads();
+    for (int i = 0; i < THREADS / 32; ++i) best = max(best, sh.best[i]);
+    if (tid == 0) sh.top[k] = best;
+    __syncthreads();
+    if (best == 0) break;
+    prev = best;
+  }
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(THREADS, 4) score_kernel(const dspark_score_args a, const int cluster) {
+  constexpr int VE = Vec<T>::VE;
+  __shared__ Shared sh;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int row = int(blockIdx.x) / cluster, part = int(blockIdx.x) - row * cluster;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int tok = a.tokens[row];
+  if (tok < 0 || tok >= a.V) {  // (every block of the cluster)
+    if (part == 0) {
+      if (tid == 0) {
+        a.logprob[row] = 0.f;
+        a.entropy[row] = 0.f;
+        a.rank[row] = -1;
+      }
+      for (int k = tid; k < a.top; k += THREADS) {
+        a.top_ids[int64_t(row) * a.top + k] = -1;
+        a.top_logprob[int64_t(row) * a.top + k] = -INFINITY;
+      }
+    }
+    return;
+  }
+  Row<T> r;
+  r.p = static_cast<const T*>(a.logits) + int64_t(row) * a.ld;
+  r.V = a.V;
+  r.head = min(int((16 - (reinterpret_cast<uintptr_t>(r.p) & 15)) & 15) / int(sizeof(T)), a.V);
+  r.nvec = (a.V - r.head) / VE;
+  r.v0 = int(int64_t(r.nvec) * part / cluster);
+  r.v1 = int(int64_t(r.nvec) * (part + 1) / cluster);
+  r.first = part == 0;
+  r.last = part == cluster - 1;
+  float T1 = 1.f;
+  bool greedy = false;
+  if (a.temperature) {
+    T1 = a.temperature[row];
+    greedy = !(T1 > 1e-6f);
+    T1 = greedy ? 1.f : fminf(T1, 1e6f);
+  }
+  const float c = 1.4426950408889634f / T1;
+  const float xt = fminf(Vec<T>::one(r.p[tok]), Vec<T>::MAXV);
+  Sums z{kLow, 0.f, 0.f};
+  int before = 0;
+  const f32x2 c2 = pack2(c, c);
+
+  // n vectors of values (masked and missing ones kLow) whose largest is bm; v[u]: the token of x[u][0]
+  auto take = [&](float (&x)[U][VE], const float (&vm)[U], const int (&tk)[U]) {
+    float bm = vm[0];
+#pragma unroll
+    for (int u = 1; u < U; ++u) bm = fmaxf(bm, vm[u]);
+    if (bm >= xt) {  // some may come before the token
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (vm[u] < xt) continue;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) before += x[u][e] > xt || (x[u][e] == xt && tk[u] + e < tok);
+      }
+    }
+    if (bm > z.m) raise(z, bm, c);
+    const f32x2 m2 = pack2(-z.m, -z.m);
+    f32x2 l2 = pack2(0.f, 0.f), s2 = pack2(0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int e = 0; e < VE; e += 2) {
+        const f32x2 y = mul2(add2(pack2(x[u][e], x[u][e + 1]), m2), c2);  // (the difference first: exact)
+        float y0, y1;
+        unpack2(y, y0, y1);
+        const f32x2 p = pack2(ex2(y0), ex2(y1));
+        l2 = add2(l2, p);
+        s2 = fma2(p, y, s2);
+      }
+    }
+    float a0, a1;
+    unpack2(l2, a0, a1);
+    z.l += a0 + a1;
+    unpack2(s2, a0, a1);
+    z.s += a0 + a1;
+  };
+  auto hold = [&](float (&x)[U][VE], float (&vm)[U]) {  // rare: values above the largest that counts
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (vm[u] <= Vec<T>::MAXV) continue;
+      vm[u] = Vec<T>::MAXV;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) x[u][e] = fminf(x[u][e], Vec<T>::MAXV);
+    }
+  };
+  const uint4* vec = reinterpret_cast<const uint4*>(r.p + r.head);
+  float x[U][VE], vm[U];
+  int tk[U];
+  for (int v = r.v0 + tid; v < r.v1; v += U * THREADS) {
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v + u * THREADS < r.v1) w[u] = ldcg_v4(vec + v + u * THREADS);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      tk[u] = r.head + (v + u * THREADS) * VE;
+      if (v + u * THREADS < r.v1) {
+        vm[u] = Vec<T>::split(w[u], x[u]);
+      } else {
+        vm[u] = kLow;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) x[u][e] = kLow;
+      }
+    }
+    hold(x, vm);
+    take(x, vm, tk);
+  }
+  const float strip = z.m;
+  const int t0 = r.head + r.nvec * VE;
+  if ((r.first && tid < r.head) || (r.last && tid >= 32 && tid - 32 < a.V - t0)) {  // the ragged ends
+    const int v = tid < 32 ? tid : t0 + tid - 32;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      vm[u] = kLow;
+      tk[u] = v;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) x[u][e] = kLow;
+    }
+    x[0][0] = vm[0] = Vec<T>::one(r.p[v]);
+    hold(x, vm);
+    take(x, vm, tk);
+  }
+  // (masked values were counted while nothing else had been seen; raise() has dropped them where something was)
+  for (int o = 16; o; o >>= 1) {
+    const Sums y{__shfl_xor_sync(0xffffffffu, z.m, o), __shfl_xor_sync(0xffffffffu, z.l, o),
+                 __shfl_xor_sync(0xffffffffu, z.s, o)};
+    z = join(z, y, c);
+  }
+  before = int(__reduce_add_sync(0xffffffffu, unsigned(before)));
+  if (lane == 0) {
+    sh.warp[warp] = z;
+    sh.rank[warp] = before;
+  }
+  if (TOP) {
+    find_top<T>(sh, r, strip, a.top);
+  } else {
+    __syncthreads();
+  }
+  if (tid == 0) {
+    Sums y = sh.warp[0];
+    int n = sh.rank[0];
+    for (int i = 1; i < THREADS / 32; ++i) {
+      y = join(y, sh.warp[i], c);
+      n += sh.rank[i];
+    }
+    sh.sum = y;
+    sh.before = n;
+  }
+  if (cluster > 1) {
+    cluster_sync_all();
+    if (part == 0) {
+      if (TOP) {
+        const int n = cluster * a.top;  // at most CAND / 4
+        for (int i = tid; i < n; i += THREADS) {
+          const int q = i / a.top;
+          sh.cand[i] = remote_u64(&sh.top[i - q * a.top], q);
+        }
+        __syncthreads();
+        place_top(sh, sh.cand, n, a.top, sh.cand + CAND / 2);
+        if (tid < a.top) {  // (nothing is left behind the last)
+          int live = 0;
+          for (int i = 0; i < n; ++i) live += sh.cand[i] != 0;
+          if (tid >= live) sh.cand[CAND / 2 + tid] = 0;
+        }
+      }
+      if (tid == 0) {
+        Sums y = sh.sum;
+        int n = sh.before;
+        for (int q = 1; q < cluster; ++q) {
+          const uint32_t at = mapa_shared(smem_u32(&sh.sum), q);
+          const Sums o{ld_dsmem_f32(at), ld_dsmem_f32(at + 4), ld_dsmem_f32(at + 8)};
+          y = join(y, o, c);
+          n += __float_as_int(ld_dsmem_f32(mapa_shared(smem_u32(&sh.before), q)));
+        }
+        sh.sum = y;
+        sh.before = n;
+      }
+    }
+  }
+  __syncthreads();
+  if (part == 0) {
+    const Sums y = sh.sum;
+    const bool any = y.m > kLow;
+    const float ln = any ? logf(y.l) : 0.f;
+    if (tid == 0) {
+      const bool live = any && xt > kLow;
+      a.logprob[row] = !live ? -INFINITY : greedy ? (sh.before == 0 ? 0.f : -INFINITY) : (xt - y.m) / T1 - ln;
+      a.entropy[row] = !any || greedy ? 0.f : fmaxf(ln - y.s / y.l * 0.6931471805599453f, 0.f);
+      a.rank[row] = live ? sh.before : -1;
+    }
+    if (TOP) {
+      const uint64_t* list = cluster > 1 ? sh.cand + CAND / 2 : sh.top;
+      for (int k = tid; k < a.top; k += THREADS) {
+        const uint64_t key = list[k];
+        const float v = value_of(key);
+        a.top_ids[int64_t(row) * a.top + k] = key ? int32_t(~uint32_t(key)) : -1;
+        a.top_logprob[int64_t(row) * a.top + k] =
+            !key ? -INFINITY : greedy ? (k == 0 ? 0.f : -INFINITY) : (v - y.m) / T1 - ln;
+      }
+    }
+  }
+  if (cluster > 1) cluster_sync_all();  // the first block has read the others' shared memory
+}
+
+template <typename T>
+static cudaError_t launch(const dspark_score_args& a, cudaStream_t s) {
+  // blocks a row: one wave of blocks or more, slices of 4 KB or more
+  const int sms = sm_count(current_device());
+  int cluster = 1;
+  while (cluster < MAX_CLUSTER && int64_t(a.R) * cluster < 4 * sms &&
+         int64_t(a.V) * int(sizeof(T)) >= int64_t(cluster) * 2 * 4096)
+    cluster *= 2;
+  const dim3 grid(unsigned(a.R) * cluster);
+  return a.top ? launch_ex(score_kernel<T, true>, grid, dim3(THREADS), 0, s, cluster, true, a, cluster)
+               : launch_ex(score_kernel<T, false>, grid, dim3(THREADS), 0, s, cluster, true, a, cluster);
+}
+
+}  // namespace score
+}  // namespace dspark
+
+using namespace dspark;
+
+extern "C" int dspark_token_logprobs(const dspark_score_args* p, void* stream) {
+  if (!p) return fail(DSPARK_ERR_ARG, "token_logprobs: null argument");
+  const dspark_score_args& a = *p;
+  if (a.R < 0 || a.V <= 0 || a.top < 0)
+    return fail(DSPARK_ERR_ARG, "token_logprobs: bad shape (%d rows, %d tokens, %d alternatives)", a.R, a.V, a.top);
+  if (a.dtype != DSPARK_DTYPE_BF16 && a.dtype != DSPARK_DTYPE_F16 && a.dtype != DSPARK_DTYPE_F32)
+    return fail(DSPARK_ERR_UNSUPPORTED, "token_logprobs: dtype %d (bf16 = 0, fp16 = 1, fp32 = 2)", a.dtype);
+  if (a.top > score::MAX_TOP)
+    return fail(DSPARK_ERR_UNSUPPORTED, "token_logprobs: %d alternatives (at most %d)", a.top, score::MAX_TOP);
+  if (a.R > 0x7fffffff / score::MAX_CLUSTER)
+    return fail(DSPARK_ERR_UNSUPPORTED, "token_logprobs: %d rows in one call", a.R);
+  if (a.V > 0x7fffffff - 65536) return fail(DSPARK_ERR_UNSUPPORTED, "token_logprobs: %d tokens", a.V);
+  if (a.R == 0) return DSPARK_OK;
+  if (!a.logits || !a.tokens || !a.logprob || !a.entropy || !a.rank || (a.top && (!a.top_ids || !a.top_logprob)))
+    return fail(DSPARK_ERR_ARG, "token_logprobs: null pointer");
+  const int size = a.dtype == DSPARK_DTYPE_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(a.logits) % size)
+    return fail(DSPARK_ERR_UNSUPPORTED, "token_logprobs: logits must be aligned to their type");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  DSPARK_CUDA_TRY(a.dtype == DSPARK_DTYPE_BF16  ? score::launch<bf16>(a, s)
+                  : a.dtype == DSPARK_DTYPE_F16 ? score::launch<__half>(a, s)
+                                                : score::launch<float>(a, s),
+                  "token_logprobs");
+  return DSPARK_OK;
+}

@@ -1,9 +1,9 @@
-"""Accept of drafted tokens for sampled targets (temperature above zero).
+"""Accept of drafted tokens for sampled targets (temperature above zero), and the log probabilities of tokens.
 
 :func:`.batch_engine.accept` is the greedy accept; this is its sampled form, on chains and on trees,
 with the random numbers given by the caller, so that a round can be repeated. The emitted tokens have
 the target's own distribution whatever was drafted (the reference's lossless sampling,
-src/mlx_dspark/sampling.py).
+src/mlx_dspark/sampling.py). :func:`token_logprobs` scores tokens: those that a round emitted, or a given text.
 """
 
 from __future__ import annotations
@@ -19,6 +19,7 @@ _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 _pack = _lib.packer(_lib.SampleArgs)
+_pack_score = _lib.packer(_lib.ScoreArgs)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -103,4 +104,46 @@ def sample_accept(logits: torch.Tensor, ids: torch.Tensor, cu_rows: torch.Tensor
     out.pop("lens", None)
     if lens is not None:
         out["lens"] = lens
+    return out
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: torch.Tensor | None = None,
+                   top: int = 0, out: dict | None = None) -> dict:
+    """Score one token a row against ``p = softmax(logits / T)``.
+
+    ``logits [R, V]`` (bf16, fp16 or fp32, contiguous rows), ``tokens`` int32 ``[R]``, ``temperature`` float32
+    ``[R]`` (``None``: 1; 1e-6 or less: greedy, all mass on the first largest logit). Returns ``logprob``
+    (``ln p(token)``), ``entropy`` (``-sum p ln p``), ``rank`` (int32: tokens before it by logit, then the lower
+    token; 0 is the most likely) and with ``top`` (up to 32) the first tokens of that order, ``top_ids`` and
+    ``top_logprobs`` ``[R, top]``; ``out``, a former call's result of as many rows and alternatives, is written again.
+
+    A logit of NaN, -inf, or at most -2^100 (fp16: its lowest value) masks its token: logprob -inf, rank -1, never
+    an alternative; where fewer tokens than ``top`` are left, the others' ids are -1 and their logprobs -inf. A row
+    whose token is outside the vocabulary (-1: a padded row) is not read: logprob and entropy 0, rank -1, no
+    alternatives."""
+    stream = on_device(logits, tokens, temperature, *(() if out is None else out.values()))
+    if logits.ndim != 2:
+        raise _lib.DSparkError(_lib.ERR_ARG, f"logits {tuple(logits.shape)}: [R, V]")
+    R, V = logits.shape
+    top = int(top)
+    dt = _DT.get(logits.dtype)
+    if dt is None:
+        raise _lib.DSparkUnsupported(_lib.ERR_UNSUPPORTED, f"logits of {logits.dtype} (bf16, fp16 or fp32)")
+    ld = _rows_of("logits", logits, R, V)
+    if not 0 <= top <= 32:
+        raise _lib.DSparkUnsupported(_lib.ERR_UNSUPPORTED, f"{top} alternatives (at most 32)")
+    if out is None:
+        f, i = (dict(dtype=t, device=logits.device) for t in (torch.float32, torch.int32))
+        out = {"logprob": torch.empty(R, **f), "entropy": torch.empty(R, **f), "rank": torch.empty(R, **i)}
+        if top:
+            out["top_ids"], out["top_logprobs"] = torch.empty((R, top), **i), torch.empty((R, top), **f)
+    elif top and out.get("top_ids") is None or not top and "top_ids" in out:
+        raise _lib.DSparkError(_lib.ERR_ARG, f"out of another call: {top} alternatives, {sorted(out)}")
+    ids = tl = 0
+    if top:
+        ids, tl = int32("top_ids", out["top_ids"], R * top), _f32("top_logprobs", out["top_logprobs"], R * top)
+    _lib.check(_lib.lib.dspark_token_logprobs(_pack_score(
+        logits.data_ptr(), ld, int32("tokens", tokens, R), _f32("temperature", temperature, R),
+        _f32("logprob", out["logprob"], R), _f32("entropy", out["entropy"], R), int32("rank", out["rank"], R), ids, tl,
+        dt, R, V, top), stream))
     return out
