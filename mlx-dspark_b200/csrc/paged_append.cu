@@ -24,12 +24,11 @@ constexpr int Q_THREADS = 128;
 constexpr int U = 4;  // heads of q in flight a lane
 
 // cos and sin of pos * f, f in 64-bit fixed-point turns (the product wraps at whole turns: any position keeps its
-// phase to 2^-32 of a turn); within half a turn the special-function unit's are off by less than 1e-6.
+// phase to 2^-32 of a turn). Not the special-function unit's, which are off by up to 1e-6: three times as many
+// values would then fall to the other side of a border between two codes as fp32 rounding alone sends there.
 __device__ __forceinline__ void phase(int pos, uint64_t f, float& c, float& s) {
   const uint64_t t = uint64_t(int64_t(pos)) * f;
-  const float a = float(int32_t(uint32_t(t >> 32))) * 1.4629180792671596e-9f;  // 2 pi / 2^32
-  c = __cosf(a);
-  s = __sinf(a);
+  sincospif(float(int32_t(uint32_t(t >> 32))) * 0x1p-31f, &s, &c);
 }
 
 // Sixteen values of a row: eight at p + c0 and eight at p + c1.

@@ -31,8 +31,7 @@ constexpr int BN = 128;      // keys a tile
 constexpr int SUB = 32;      // keys a warp's subtile
 constexpr int WARPS = 4;
 constexpr int NTHR = WARPS * 32;
-constexpr int NS = 3;        // ring buffers a warp
-constexpr int MAX_CTA = 320;
+constexpr int MAX_CTA = 480;
 constexpr int SEG = 3;       // cost of a segment, in tiles
 constexpr float LIFT = 11.f; // weights are 2^11 times as large in fp16 ...
 constexpr float SLACK = 4.f; // ... and the maximum in use may be 2^4 too low
@@ -40,6 +39,8 @@ constexpr float SLACK = 4.f; // ... and the maximum in use may be 2^4 too low
 template <int D, int RT>
 struct Lay {
   static constexpr int RB = 16 * RT;
+  static constexpr int PER_SM = RT == 1 ? 3 : 2;      // blocks an SM
+  static constexpr int NS = RT == 1 ? 2 : 3;          // ring buffers a warp
   static constexpr int TILE = SUB * D;                // a subtile's K or V codes
   static constexpr int STAGE = 2 * TILE + 32;         // K, V, two pages' scales
   static constexpr int RING = NS * STAGE;             // a warp's
@@ -190,7 +191,7 @@ __device__ __forceinline__ float* part_of(void* ws, int cta, int which) {
 // ------------------------------------------------------------------ the kernel
 
 template <typename T, int D, int RT>
-__global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_args a, const float c_log2, int* status) {
+__global__ void __launch_bounds__(NTHR, RT == 1 ? 3 : 2) attn_kernel(const dspark_paged_attn_args a, const float c_log2, int* status) {
   typedef Lay<D, RT> L;
   constexpr int RB = L::RB, KS = D / 16, CH = D / 16;  // k steps of the scores, 16-byte chunks a row
   extern __shared__ __align__(128) uint8_t smem[];
@@ -263,19 +264,24 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
   float2* ml = reinterpret_cast<float2*>(smem + L::ML);
   float* merge = reinterpret_cast<float*>(smem + L::BUF);
 
+  constexpr int RPI = 32 / CH, ROUNDS = SUB / RPI;  // tokens a round of 16-byte copies, rounds a subtile
+  const int kts = int(a.kp_strides[2]), vts = int(a.vp_strides[2]);
+  const uint32_t sw0 = at_chunk<D>(lane / CH, lane % CH), sw1 = at_chunk<D>(RPI + lane / CH, lane % CH) - RPI * D;
+
   Segment s;
   while (wk.next(plan, deal, s)) {
     const int sub0 = s.t0 * (BN / SUB) + warp, sub1 = min(s.t1 * (BN / SUB), (s.len + SUB - 1) / SUB);
     const int n = sub0 < sub1 ? (sub1 - sub0 + WARPS - 1) / WARPS : 0;
     const int32_t* table = a.page_table + int64_t(s.b) * a.table_stride;
-    const uint8_t* kp = static_cast<const uint8_t*>(a.k_pages) + s.h * a.kp_strides[1];
-    const uint8_t* vp = static_cast<const uint8_t*>(a.v_pages) + s.h * a.vp_strides[1];
+    // the lane's first 16 bytes of a subtile; the next are RPI tokens on
+    const uint8_t* kp = static_cast<const uint8_t*>(a.k_pages) + s.h * a.kp_strides[1] + lane / CH * kts + lane % CH * 16;
+    const uint8_t* vp = static_cast<const uint8_t*>(a.v_pages) + s.h * a.vp_strides[1] + lane / CH * vts + lane % CH * 16;
 
-    // Lane 0 and 1: the subtile's page or pages (16 tokens: two), -1 where there is none to read.
+    // Lane 0 and 1: the pages of the subtile's halves (one page or two), -1 where there is none to read.
     auto page_id = [&](int i) {
       int id = -1;
       const int key = (sub0 + i * WARPS) * SUB + lane * 16;
-      if (lane < (shift == 4 ? 2 : 1) && i < n && key < s.len) {
+      if (lane < 2 && i < n && key < s.len) {
         id = table[key >> shift];
         if (id < 0 || id >= a.n_pages) {
           report_error(status, kErrAttnPage);
@@ -289,36 +295,40 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
       const int mine = ahead;
       ahead = page_id(i + 1);
       if (i < n) {
-        const uint32_t dst = ring_a + (i % NS) * L::STAGE;
+        const uint32_t dst = ring_a + (i % L::NS) * L::STAGE;
         const int key0 = (sub0 + i * WARPS) * SUB;
         if (lane < 2) {
-          const int id = shift == 4 ? mine : __shfl_sync(3u, mine, 0);
-          const int64_t at_s = int64_t(id) * a.scale_strides[0] + s.h * a.scale_strides[1];
+          const int64_t at_s = mine < 0 ? 0 : int64_t(mine) * a.scale_strides[0] + s.h * a.scale_strides[1];
           const uint32_t to = dst + 2 * L::TILE + lane * 8;
-          const float* ks = a.k_scale + (id < 0 ? 0 : at_s);
-          const float* vs = a.v_scale + (id < 0 ? 0 : at_s);
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(ks), "r"(id < 0 ? 0 : 4) : "memory");
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 4), "l"(vs), "r"(id < 0 ? 0 : 4)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(a.k_scale + at_s), "r"(mine < 0 ? 0 : 4)
+                       : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 4), "l"(a.v_scale + at_s),
+                       "r"(mine < 0 ? 0 : 4)
                        : "memory");
         }
         __syncwarp();
         const int id0 = __shfl_sync(0xffffffffu, mine, 0), id1 = __shfl_sync(0xffffffffu, mine, 1);
+        const int mask = a.page - 1;
+        const uint8_t* k0 = kp + (id0 * a.kp_strides[0] + (key0 & mask) * a.kp_strides[2]);
+        const uint8_t* v0 = vp + (id0 * a.vp_strides[0] + (key0 & mask) * a.vp_strides[2]);
+        const uint8_t* k1 = kp + (id1 * a.kp_strides[0] + ((key0 + 16) & mask) * a.kp_strides[2]);
+        const uint8_t* v1 = vp + (id1 * a.vp_strides[0] + ((key0 + 16) & mask) * a.vp_strides[2]);
+        const bool whole = key0 + SUB <= s.len && id0 >= 0 && id1 >= 0;
 #pragma unroll
-        for (int z = 0; z < SUB * CH / 32; ++z) {
-          const int row = (z * 32 + lane) / CH, c = lane % CH;
-          const int id = shift == 4 && row >= 16 ? id1 : id0, key = key0 + row;
-          const bool there = id >= 0 && key < s.len;
-          const int tok = key & (a.page - 1);
-          const int64_t ko = there ? id * a.kp_strides[0] + tok * a.kp_strides[2] + c * 16 : 0;
-          const int64_t vo = there ? id * a.vp_strides[0] + tok * a.vp_strides[2] + c * 16 : 0;
-          cp_async_16_zfill(dst + at_chunk<D>(row, c), kp + ko, there);
-          cp_async_16_zfill(dst + L::TILE + at_chunk<D>(row, c), vp + vo, there);
+        for (int z = 0; z < ROUNDS; ++z) {
+          const uint32_t to = dst + z * RPI * D + (z & 1 ? sw1 : sw0);
+          const int y = z % (ROUNDS / 2) * RPI;
+          const uint8_t* k = (z < ROUNDS / 2 ? k0 : k1) + y * kts;
+          const uint8_t* v = (z < ROUNDS / 2 ? v0 : v1) + y * vts;
+          const bool there = whole || ((z < ROUNDS / 2 ? id0 : id1) >= 0 && key0 + z * RPI + lane / CH < s.len);
+          cp_async_16_zfill(to, there ? k : kp, there);
+          cp_async_16_zfill(to + L::TILE, there ? v : vp, there);
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
-    for (int i = 0; i < NS - 1; ++i) issue(i);
+    for (int i = 0; i < L::NS - 1; ++i) issue(i);
 
     // ---- Q as fp16 fragments. 16 neighbouring values of a row a thread and round.
     {
@@ -392,13 +402,13 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
     const int edge0 = (a.causal ? min(s.len, s.before + s.row_base / G + 1) : s.len) - SUB;  // later: hidden keys
 
     for (int i = 0; i < n; ++i) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(NS - 2) : "memory");
+      asm volatile("cp.async.wait_group %0;" ::"n"(L::NS - 2) : "memory");
       __syncwarp();
-      issue(i + NS - 1);
+      issue(i + L::NS - 1);
       const int key0 = (sub0 + i * WARPS) * SUB;
-      const uint32_t kt = ring_a + (i % NS) * L::STAGE, vt = kt + L::TILE;
-      const float2 sc0 = *reinterpret_cast<const float2*>(ring + (i % NS) * L::STAGE + 2 * L::TILE);
-      const float2 sc1 = *reinterpret_cast<const float2*>(ring + (i % NS) * L::STAGE + 2 * L::TILE + 8);
+      const uint32_t kt = ring_a + (i % L::NS) * L::STAGE, vt = kt + L::TILE;
+      const float2 sc0 = *reinterpret_cast<const float2*>(ring + (i % L::NS) * L::STAGE + 2 * L::TILE);
+      const float2 sc1 = *reinterpret_cast<const float2*>(ring + (i % L::NS) * L::STAGE + 2 * L::TILE + 8);
       // pages without a positive scale (absent ones have 0) are not seen
       const bool ok0 = sc0.x > 0.f && sc0.y > 0.f, ok1 = sc1.x > 0.f && sc1.y > 0.f;
       const bool edge = key0 > edge0 || !ok0 || !ok1;
@@ -659,12 +669,12 @@ __global__ void __launch_bounds__(128) join_kernel(const dspark_paged_attn_args 
     *reinterpret_cast<uint32_t*>(out) = Elem<T>::pack(v[0] * inv, v[1] * inv);
 }
 
-static int grid_of(int device) { return std::min(2 * sm_count(device), MAX_CTA); }
+static int grid_of(int device, int per_sm) { return std::min(per_sm * sm_count(device), MAX_CTA); }
 
 template <typename T, int D, int RT>
 static int launch(const dspark_paged_attn_args& a, cudaStream_t s) {
   typedef Lay<D, RT> L;
-  const int dev = current_device(), n = grid_of(dev);
+  const int dev = current_device(), n = grid_of(dev, L::PER_SM);
   DSPARK_CUDA_TRY(configure_once((const void*)attn_kernel<T, D, RT>, L::TOTAL,
                                  [&] {
                                    return cudaFuncSetAttribute(attn_kernel<T, D, RT>,
@@ -694,7 +704,7 @@ extern "C" {
 size_t dspark_paged_attn_workspace(int R, int B, int Hq, int Hk, int D) {
   if (R <= 0 || B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || D <= 0) return 0;
   return paged::MAX_CTA * sizeof(paged::Cut) +
-         size_t(paged::grid_of(current_device())) * 2 * 32 * (D + 1) * sizeof(float);
+         size_t(paged::grid_of(current_device(), 2)) * 2 * 32 * (D + 1) * sizeof(float);  // (also enough for 3 of 16 rows)
 }
 
 int dspark_paged_attn(const dspark_paged_attn_args* p, void* stream) {
@@ -721,6 +731,8 @@ int dspark_paged_attn(const dspark_paged_attn_args* p, void* stream) {
   for (int i = 0; i < 2; ++i) aligned &= a.q_strides[i] % 8 == 0 && a.o_strides[i] % 8 == 0;
   for (int i = 0; i < 3; ++i) aligned &= a.kp_strides[i] % 16 == 0 && a.vp_strides[i] % 16 == 0;
   if (!aligned) return fail(DSPARK_ERR_UNSUPPORTED, "paged_attn: rows must be 16-byte aligned");
+  for (int64_t t : {a.kp_strides[2], a.vp_strides[2]})
+    if (t < 0 || t > 1 << 24) return fail(DSPARK_ERR_UNSUPPORTED, "paged_attn: %lld bytes between tokens", (long long)t);
   if (!a.workspace || a.ws_bytes < dspark_paged_attn_workspace(a.R, a.B, a.Hq, a.Hk, a.D))
     return fail(DSPARK_ERR_ARG, "paged_attn: workspace of %zu bytes", a.ws_bytes);
   if (reinterpret_cast<uintptr_t>(a.workspace) % 16)
