@@ -25,10 +25,16 @@ constexpr int U = 4;  // heads of q in flight a lane
 
 // cos and sin of pos * f, f in 64-bit fixed-point turns (the product wraps at whole turns: any position keeps its
 // phase to 2^-32 of a turn). Not the special-function unit's, which are off by up to 1e-6: three times as many
-// values would then fall to the other side of a border between two codes as fp32 rounding alone sends there.
+// values would then fall to the other side of a border between two codes as fp32 rounding alone sends there. Within an
+// eighth of a turn of the nearest quarter their Taylor series to the 9th and 8th power are off by 2e-9 and 2.5e-8.
 __device__ __forceinline__ void phase(int pos, uint64_t f, float& c, float& s) {
-  const uint64_t t = uint64_t(int64_t(pos)) * f;
-  sincospif(float(int32_t(uint32_t(t >> 32))) * 0x1p-31f, &s, &c);
+  const uint32_t t = uint32_t((uint64_t(int64_t(pos)) * f) >> 32), quarter = (t + 0x20000000u) >> 30;
+  const float a = float(int32_t(t - (quarter << 30))) * 1.4629180792671596e-9f, z = a * a;  // 2 pi / 2^32
+  const float sn = fmaf(a * z, fmaf(z, fmaf(z, fmaf(z, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), a);
+  const float cs = fmaf(z, fmaf(z, fmaf(z, fmaf(z, 1.f / 40320, -1.f / 720), 1.f / 24), -0.5f), 1.f);
+  const float x = quarter & 1 ? sn : cs, y = quarter & 1 ? cs : sn;
+  c = __uint_as_float(__float_as_uint(x) ^ ((quarter + 1) & 2) << 30);
+  s = __uint_as_float(__float_as_uint(y) ^ (quarter & 2) << 30);
 }
 
 // Sixteen values of a row: eight at p + c0 and eight at p + c1.
@@ -99,19 +105,9 @@ __device__ void append_page(const dspark_paged_append_args& a, int unit, int* st
   if (j == 0 && h == 0 && kv == 0 && tid == 0 && a.len_out) a.len_out[b] = int32_t(min(len + n, max(room, len)));
   const int64_t pi = (len >> shift) + j;
   if (n == 0 || pi > (len + n - 1) >> shift) return;
-  const int pid = pi < a.max_pages ? a.page_table[int64_t(b) * a.table_stride + pi] : -1;
-  if (pid < 0 || pid >= a.n_pages) {
-    if (tid == 0) report_error(status, kErrAppendPage);
-    return;
-  }
   const int begin = j == 0 ? int(len & (a.page - 1)) : 0;       // tokens that the page has
   const int place0 = int((pi << shift) + begin - len);          // the first new one's place in the request
   const int count = min(a.page - begin, n - place0);
-  uint8_t* codes = static_cast<uint8_t*>(kv ? a.v_pages : a.k_pages) +
-                   (kv ? pid * a.vp_strides[0] + h * a.vp_strides[1] : pid * a.kp_strides[0] + h * a.kp_strides[1]);
-  const int64_t ts = kv ? a.vp_strides[2] : a.kp_strides[2];
-  float* scale = (kv ? a.v_scale : a.k_scale) + pid * a.scale_strides[0] + h * a.scale_strides[1];
-  const float old = begin ? *scale : 0.f;
   const T* src = static_cast<const T*>(kv ? a.v : a.k) + (kv ? h * a.v_strides[1] : h * a.k_strides[1]);
   const int64_t row_stride = kv ? a.v_strides[0] : a.k_strides[0];
   const bool turns = !kv && li < a.rot / 16, half = turns && HALF;
@@ -124,6 +120,16 @@ __device__ void append_page(const dspark_paged_append_args& a, int unit, int* st
     const int t = z * per + first;
     if (t < count) load16<T, VEC>(src + (r0 + place0 + t) * row_stride, c0, c1, raw[z]);
   }
+  const int pid = pi < a.max_pages ? a.page_table[int64_t(b) * a.table_stride + pi] : -1;
+  if (pid < 0 || pid >= a.n_pages) {
+    if (tid == 0) report_error(status, kErrAppendPage);
+    return;
+  }
+  uint8_t* codes = static_cast<uint8_t*>(kv ? a.v_pages : a.k_pages) +
+                   (kv ? pid * a.vp_strides[0] + h * a.vp_strides[1] : pid * a.kp_strides[0] + h * a.kp_strides[1]);
+  const int64_t ts = kv ? a.vp_strides[2] : a.kp_strides[2];
+  float* scale = (kv ? a.v_scale : a.k_scale) + pid * a.scale_strides[0] + h * a.scale_strides[1];
+  const float old = begin ? *scale : 0.f;
   const bool norm = !kv && a.k_norm;
   uint32_t weight[8];
   if (norm) load16<T, false>(static_cast<const T*>(a.k_norm), c0, c1, weight);
@@ -263,8 +269,8 @@ __device__ void turn_q(const dspark_paged_append_args& a, int w, int warps) {
   }
 }
 
-template <typename T, bool VEC, bool HALF, int PASS, int THREADS>
-__global__ void __launch_bounds__(THREADS) append_kernel(const dspark_paged_append_args a, const int page_blocks,
+template <typename T, bool VEC, bool HALF, int PASS, int THREADS, int MIN_BLOCKS>
+__global__ void __launch_bounds__(THREADS, MIN_BLOCKS) append_kernel(const dspark_paged_append_args a, const int page_blocks,
                                                          const int warps, int* status) {
   pdl_launch_dependents();
   pdl_wait();
@@ -284,7 +290,7 @@ static cudaError_t launch_as(const dspark_paged_append_args& a, cudaStream_t s) 
   const int warps = std::max(1, std::min(want, most));
   const int64_t q_blocks = (int64_t(a.R) * warps + THREADS / 32 - 1) / (THREADS / 32);
   if (page_blocks + q_blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  return launch_ex(append_kernel<T, VEC, HALF, PASS, THREADS>, dim3(unsigned(page_blocks + q_blocks)), dim3(THREADS), 0,
+  return launch_ex(append_kernel<T, VEC, HALF, PASS, THREADS, PASS == 4 ? 512 / THREADS : 5>, dim3(unsigned(page_blocks + q_blocks)), dim3(THREADS), 0,
                    s, 1, true, a, int(page_blocks), warps, status_word(current_device()));
 }
 

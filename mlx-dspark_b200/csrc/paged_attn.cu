@@ -62,6 +62,10 @@ __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0
 
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) { return Elem<__half>::pack(a, b); }
 
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // 16-byte chunk c of a subtile's row, swizzled so that the eight rows of an ldmatrix and the eight lanes of a 16-byte
 // load meet different banks.
 template <int D>
@@ -102,17 +106,17 @@ struct Plan {
   }
 };
 
-// The line of costs cut into n shares.
+// The line of costs (32 bits: refused above) cut into n shares.
 struct Deal {
-  int64_t q, rem, total;
+  uint32_t q, rem, total;
   int n;
-  __device__ __forceinline__ Deal(int64_t t, int most) : total(t), n(int(min(int64_t(most), t))) {
+  __device__ __forceinline__ Deal(uint32_t t, int most) : total(t), n(int(min(uint32_t(most), t))) {
     q = n ? t / n : 0;
     rem = n ? t - q * n : 0;
   }
-  __device__ __forceinline__ int64_t from(int c) const { return c < n ? c * q + min(int64_t(c), rem) : total; }
-  __device__ __forceinline__ int owner(int64_t x) const {
-    const int64_t wide = rem * (q + 1);
+  __device__ __forceinline__ uint32_t from(int c) const { return c < n ? c * q + min(uint32_t(c), rem) : total; }
+  __device__ __forceinline__ int owner(uint32_t x) const {
+    const uint32_t wide = rem * (q + 1);
     return x < wide ? int(x / (q + 1)) : int(rem + (x - wide) / q);
   }
 };
@@ -127,7 +131,7 @@ struct Segment {
 
 template <int RB>
 struct Walker {
-  int64_t x, end, base;  // next cost, end of the share, first cost of request b
+  uint32_t x, end, base;  // next cost, end of the share, first cost of request b
   int b;
   Shape s;
   bool have;
@@ -136,22 +140,20 @@ struct Walker {
     while (x < end) {
       if (!have) s = p.shape(b);
       have = true;
-      const int item = p.seg + s.T;
-      const int64_t all = int64_t(s.M) * a.Hk * item;
+      const uint32_t item = p.seg + s.T, all = s.M * a.Hk * item;
       if (x >= base + all) {
         base += all;
         ++b;
         have = false;
         continue;
       }
-      const int i = int((x - base) / item);
-      const int64_t start = base + int64_t(i) * item, stop = start + item;
+      const uint32_t i = (x - base) / item, start = base + i * item, stop = start + item;
       // neighbours in the line are a short and a long row block: shares of equal cost are of equal work
-      const int h = i / s.M, k = i - h * s.M, m = k & 1 ? s.M - 1 - (k >> 1) : k >> 1;
+      const int h = i / uint32_t(s.M), k = i - h * s.M, m = k & 1 ? s.M - 1 - (k >> 1) : k >> 1;
       const int T = p.tiles(s, m);
-      auto tile_at = [&](int64_t y) {
-        const int64_t d = y - start - p.seg;
-        return d <= 0 ? 0 : d >= s.T ? T : int(d * T / s.T);
+      auto tile_at = [&](uint32_t y) {
+        const int d = int(y - start) - p.seg;
+        return d <= 0 ? 0 : d >= s.T ? T : T == s.T ? d : int(int64_t(d) * T / s.T);
       };
       g.b = b;
       g.h = h;
@@ -191,13 +193,12 @@ __device__ __forceinline__ float* part_of(void* ws, int cta, int which) {
 // ------------------------------------------------------------------ the kernel
 
 template <typename T, int D, int RT>
-__global__ void __launch_bounds__(NTHR, RT == 1 ? 3 : 2) attn_kernel(const dspark_paged_attn_args a, const float c_log2, int* status) {
+__global__ void __launch_bounds__(NTHR, RT == 1 ? 3 : 2) attn_kernel(const dspark_paged_attn_args a, const float c_log2,
+                                                                          const uint32_t q_sign, int* status) {
   typedef Lay<D, RT> L;
   constexpr int RB = L::RB, KS = D / 16, CH = D / 16;  // k steps of the scores, 16-byte chunks a row
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t s_cost[WARPS];
-  __shared__ int64_t s_base;
-  __shared__ int s_req;
+  __shared__ uint2 s_cost[WARPS], s_req;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, qd = lane & 3;  // row (or key) and quarter of an mma fragment
   pdl_launch_dependents();
@@ -205,55 +206,59 @@ __global__ void __launch_bounds__(NTHR, RT == 1 ? 3 : 2) attn_kernel(const dspar
 
   // ---- this block's share: the first request of it
   Plan<RB> plan{a, SEG};
-  int64_t total = 0, tiles = 0;
-  auto cost_of = [&](int b, int seg) {
-    if (b >= a.B) return int64_t(0);
+  uint32_t items = 0, tiles = 0;  // of the thread's request; of the first NTHR requests they are kept
+  auto weigh = [&](int b) {
+    items = tiles = 0;
+    if (b >= a.B) return;
     const Shape s = plan.shape(b);
-    return int64_t(s.M) * a.Hk * (seg + s.T);
+    items = s.M * a.Hk;
+    tiles = items * s.T;
   };
-  auto block_sum = [&](int64_t v) {
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  uint32_t all_items = 0, all_tiles = 0;
+  for (int b0 = (a.B - 1) / NTHR * NTHR; b0 >= 0; b0 -= NTHR) {
+    weigh(b0 + tid);
+    const uint32_t i = __reduce_add_sync(0xffffffffu, items), t = __reduce_add_sync(0xffffffffu, tiles);
     __syncthreads();
-    if (lane == 0) s_cost[warp] = v;
+    if (lane == 0) s_cost[warp] = make_uint2(i, t);
     __syncthreads();
-    return s_cost[0] + s_cost[1] + s_cost[2] + s_cost[3];
-  };
-  for (int b0 = 0; b0 < a.B; b0 += NTHR) {
-    tiles += block_sum(cost_of(b0 + tid, 0));
-    total += block_sum(cost_of(b0 + tid, SEG));
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      all_items += s_cost[w].x;
+      all_tiles += s_cost[w].y;
+    }
   }
-  if (tiles <= int64_t(gridDim.x)) {  // a tile a block: nothing is gained by fuller shares
-    plan.seg = 0;
-    total = tiles;
-  }
-  const Deal deal(total, int(gridDim.x));
+  // a tile a block: nothing is gained by fuller shares
+  if (all_tiles <= gridDim.x) plan.seg = 0;
+  const Deal deal(all_tiles + plan.seg * all_items, int(gridDim.x));
   Walker<RB> wk;
   wk.x = deal.from(blockIdx.x);
   wk.end = deal.from(blockIdx.x + 1);
   wk.have = false;
-  if (tid == 0) s_req = a.B;
-  int64_t at = 0;
+  if (tid == 0) s_req = make_uint2(a.B, 0);
+  uint32_t at = 0;
   for (int b0 = 0; b0 < a.B && wk.x < wk.end; b0 += NTHR) {
-    const int64_t v = cost_of(b0 + tid, plan.seg);
-    int64_t sum = v;
+    if (b0 > 0) weigh(b0 + tid);
+    const uint32_t v = tiles + plan.seg * items;
+    uint32_t sum = v;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+      const uint32_t y = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += y;
     }
     __syncthreads();
-    if (lane == 31) s_cost[warp] = sum;
+    if (lane == 31) s_cost[warp].x = sum;
     __syncthreads();
-    int64_t before = at + sum - v;
-    for (int w = 0; w < warp; ++w) before += s_cost[w];
-    if (v > 0 && wk.x >= before && wk.x < before + v) {
-      s_req = b0 + tid;
-      s_base = before;
+    uint32_t before = at + sum - v;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) before += s_cost[w].x;
+      at += s_cost[w].x;
     }
-    at += s_cost[0] + s_cost[1] + s_cost[2] + s_cost[3];
+    if (v > 0 && wk.x >= before && wk.x < before + v) s_req = make_uint2(b0 + tid, before);
   }
   __syncthreads();
-  wk.b = s_req;
-  wk.base = s_base;
+  wk.b = s_req.x;
+  wk.base = s_req.y;
   Cut cut{0, 0, 0, 0, 0, {0, 0, 0}};
 
   const int G = a.Hq / a.Hk, shift = 31 - __clz(a.page);
@@ -266,6 +271,7 @@ __global__ void __launch_bounds__(NTHR, RT == 1 ? 3 : 2) attn_kernel(const dspar
 
   constexpr int RPI = 32 / CH, ROUNDS = SUB / RPI;  // tokens a round of 16-byte copies, rounds a subtile
   const int kts = int(a.kp_strides[2]), vts = int(a.vp_strides[2]);
+  const bool packed = kts == D && vts == D;
   const uint32_t sw0 = at_chunk<D>(lane / CH, lane % CH), sw1 = at_chunk<D>(RPI + lane / CH, lane % CH) - RPI * D;
 
   Segment s;
@@ -277,11 +283,11 @@ __global__ void __launch_bounds__(NTHR, RT == 1 ? 3 : 2) attn_kernel(const dspar
     const uint8_t* kp = static_cast<const uint8_t*>(a.k_pages) + s.h * a.kp_strides[1] + lane / CH * kts + lane % CH * 16;
     const uint8_t* vp = static_cast<const uint8_t*>(a.v_pages) + s.h * a.vp_strides[1] + lane / CH * vts + lane % CH * 16;
 
-    // Lane 0 and 1: the pages of the subtile's halves (one page or two), -1 where there is none to read.
-    auto page_id = [&](int i) {
+    // The pages of 16 subtiles' halves, a half a lane (-1 where there is none to read): read 16 subtiles ahead.
+    auto page_ids = [&](int i0) {
       int id = -1;
-      const int key = (sub0 + i * WARPS) * SUB + lane * 16;
-      if (lane < 2 && i < n && key < s.len) {
+      const int i = i0 + (lane >> 1), key = (sub0 + i * WARPS) * SUB + (lane & 1) * 16;
+      if (i < n && key < s.len) {
         id = table[key >> shift];
         if (id < 0 || id >= a.n_pages) {
           report_error(status, kErrAttnPage);
@@ -290,14 +296,18 @@ __global__ void __launch_bounds__(NTHR, RT == 1 ? 3 : 2) attn_kernel(const dspar
       }
       return id;
     };
-    int ahead = page_id(0);
+    int ids = page_ids(0), later = page_ids(16);
     auto issue = [&](int i) {
-      const int mine = ahead;
-      ahead = page_id(i + 1);
       if (i < n) {
+        if (i > 0 && (i & 15) == 0) {
+          ids = later;
+          later = page_ids(i + 16);
+        }
         const uint32_t dst = ring_a + (i % L::NS) * L::STAGE;
         const int key0 = (sub0 + i * WARPS) * SUB;
+        const int id0 = __shfl_sync(0xffffffffu, ids, (i & 15) * 2), id1 = __shfl_sync(0xffffffffu, ids, (i & 15) * 2 + 1);
         if (lane < 2) {
+          const int mine = lane ? id1 : id0;
           const int64_t at_s = mine < 0 ? 0 : int64_t(mine) * a.scale_strides[0] + s.h * a.scale_strides[1];
           const uint32_t to = dst + 2 * L::TILE + lane * 8;
           asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(a.k_scale + at_s), "r"(mine < 0 ? 0 : 4)
@@ -306,15 +316,21 @@ __global__ void __launch_bounds__(NTHR, RT == 1 ? 3 : 2) attn_kernel(const dspar
                        "r"(mine < 0 ? 0 : 4)
                        : "memory");
         }
-        __syncwarp();
-        const int id0 = __shfl_sync(0xffffffffu, mine, 0), id1 = __shfl_sync(0xffffffffu, mine, 1);
         const int mask = a.page - 1;
         const uint8_t* k0 = kp + (id0 * a.kp_strides[0] + (key0 & mask) * a.kp_strides[2]);
         const uint8_t* v0 = vp + (id0 * a.vp_strides[0] + (key0 & mask) * a.vp_strides[2]);
         const uint8_t* k1 = kp + (id1 * a.kp_strides[0] + ((key0 + 16) & mask) * a.kp_strides[2]);
         const uint8_t* v1 = vp + (id1 * a.vp_strides[0] + ((key0 + 16) & mask) * a.vp_strides[2]);
         const bool whole = key0 + SUB <= s.len && id0 >= 0 && id1 >= 0;
+        if (whole && packed) {  // the usual case: no address arithmetic a copy
 #pragma unroll
+          for (int z = 0; z < ROUNDS; ++z) {
+            const uint32_t to = dst + z * RPI * D + (z & 1 ? sw1 : sw0);
+            cp_async_16(to, (z < ROUNDS / 2 ? k0 : k1) + z % (ROUNDS / 2) * RPI * D);
+            cp_async_16(to + L::TILE, (z < ROUNDS / 2 ? v0 : v1) + z % (ROUNDS / 2) * RPI * D);
+          }
+        } else {
+#pragma unroll 1
         for (int z = 0; z < ROUNDS; ++z) {
           const uint32_t to = dst + z * RPI * D + (z & 1 ? sw1 : sw0);
           const int y = z % (ROUNDS / 2) * RPI;
@@ -323,6 +339,7 @@ __global__ void __launch_bounds__(NTHR, RT == 1 ? 3 : 2) attn_kernel(const dspar
           const bool there = whole || ((z < ROUNDS / 2 ? id0 : id1) >= 0 && key0 + z * RPI + lane / CH < s.len);
           cp_async_16_zfill(to, there ? k : kp, there);
           cp_async_16_zfill(to + L::TILE, there ? v : vp, there);
+        }
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -375,8 +392,8 @@ __global__ void __launch_bounds__(NTHR, RT == 1 ? 3 : 2) attn_kernel(const dspar
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int f0 = ((rt * KS + step0 + i) * 32 + (rr & 7) * 4 + quarter) * 4;
-            to[f0] = w[2 * i];
-            to[f0 + 2] = w[2 * i + 1];
+            to[f0] = w[2 * i] ^ q_sign;
+            to[f0 + 2] = w[2 * i + 1] ^ q_sign;
           }
         }
       }
@@ -444,24 +461,30 @@ __global__ void __launch_bounds__(NTHR, RT == 1 ? 3 : 2) attn_kernel(const dspar
       }
 
       // ---- weights
-      const float lv0 = lg2(sc0.y), lv1 = lg2(sc1.y), iv0 = ok0 ? 1.f / sc0.y : 0.f, iv1 = ok1 ? 1.f / sc1.y : 0.f;
+      if (edge) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!(key0 + t * 8 + 2 * qd + (e & 1) < lim[rt][e >> 1] && (t < 2 ? ok0 : ok1))) x[rt][t][e] = -INFINITY;
+      }
+      const float ks[2] = {ok0 ? sc0.x : 1.f, ok1 ? sc1.x : 1.f}, lv[2] = {ok0 ? lg2(sc0.y) : 0.f, ok1 ? lg2(sc1.y) : 0.f};
+      const float iv[2] = {ex2(-lv[0]), ex2(-lv[1])};
       uint32_t pw[RT][4][2];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        float mx[2] = {-INFINITY, -INFINITY};
+        float f[2][2], mx[2];  // [row][page]: the factor of its scores; at least 1e-35, so that -inf stays that
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const float ks = t < 2 ? sc0.x : sc1.x, lv = t < 2 ? lv0 : lv1;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float y = fmaf(x[rt][t][e], rf[rt][e >> 1] * ks, lv);
-            if (edge) {
-              const int key = key0 + t * 8 + 2 * qd + (e & 1);
-              if (!(key < lim[rt][e >> 1] && (t < 2 ? ok0 : ok1))) y = -INFINITY;
-            }
-            x[rt][t][e] = y;
-            mx[e >> 1] = fmaxf(mx[e >> 1], y);
-          }
+        for (int k = 0; k < 2; ++k) {
+          f[k][0] = rf[rt][k] * ks[0];
+          f[k][1] = rf[rt][k] * ks[1];
+          f[k][0] = f[k][0] < 1e-35f ? 1e-35f : f[k][0];
+          f[k][1] = f[k][1] < 1e-35f ? 1e-35f : f[k][1];
+          const float m0 = fmaxf(fmaxf(x[rt][0][2 * k], x[rt][0][2 * k + 1]), fmaxf(x[rt][1][2 * k], x[rt][1][2 * k + 1]));
+          const float m1 = fmaxf(fmaxf(x[rt][2][2 * k], x[rt][2][2 * k + 1]), fmaxf(x[rt][3][2 * k], x[rt][3][2 * k + 1]));
+          mx[k] = fmaxf(fmaf(m0, f[k][0], lv[0]), fmaf(m1, f[k][1], lv[1]));
         }
         const bool up = mx[0] > m[rt][0] + SLACK || mx[1] > m[rt][1] + SLACK;
         if (__any_sync(0xffffffffu, up)) {
@@ -471,32 +494,34 @@ __global__ void __launch_bounds__(NTHR, RT == 1 ? 3 : 2) attn_kernel(const dspar
             y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
             y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
             if (y > m[rt][k]) {
-              const float f = ex2(m[rt][k] - y);  // (0 at first)
+              const float g = ex2(m[rt][k] - y);  // (0 at first)
               m[rt][k] = y;
-              l[rt][k] *= f;
+              l[rt][k] *= g;
 #pragma unroll
               for (int z = 0; z < D / 8; ++z) {
-                o[rt][z][2 * k] *= f;
-                o[rt][z][2 * k + 1] *= f;
+                o[rt][z][2 * k] *= g;
+                o[rt][z][2 * k + 1] *= g;
               }
             }
           }
         }
-        float ref[2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) ref[k] = (m[rt][k] == -INFINITY ? 0.f : m[rt][k]) - LIFT;
-        float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};  // [page][row]
+        for (int k = 0; k < 2; ++k) {
+          const float ref = LIFT - (m[rt][k] == -INFINITY ? 0.f : m[rt][k]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const float e0 = ex2(x[rt][t][0] - ref[0]), e1 = ex2(x[rt][t][1] - ref[0]);
-          const float e2 = ex2(x[rt][t][2] - ref[1]), e3 = ex2(x[rt][t][3] - ref[1]);
-          sum[t >> 1][0] += e0 + e1;
-          sum[t >> 1][1] += e2 + e3;
-          pw[rt][t][0] = pack_f16(e0, e1);
-          pw[rt][t][1] = pack_f16(e2, e3);
+          for (int page = 0; page < 2; ++page) {
+            const float add = lv[page] + ref;
+            float sum = 0.f;
+#pragma unroll
+            for (int t = 2 * page; t < 2 * page + 2; ++t) {
+              const float e0 = ex2(fmaf(x[rt][t][2 * k], f[k][page], add));
+              const float e1 = ex2(fmaf(x[rt][t][2 * k + 1], f[k][page], add));
+              sum += e0 + e1;
+              pw[rt][t][k] = pack_f16(e0, e1);
+            }
+            l[rt][k] = fmaf(sum, iv[page], l[rt][k]);
+          }
         }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) l[rt][k] += sum[0][k] * iv0 + sum[1][k] * iv1;
       }
 
       // ---- O += P V
@@ -639,25 +664,40 @@ __global__ void __launch_bounds__(128) join_kernel(const dspark_paged_attn_args 
   float m = -INFINITY, sum = 0.f, v[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] = 0.f;
-  for (int x = lane; x < c.parts; x += 32) m = fmaxf(m, __ldcg(at(x) + RB * D + r));
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll 8
-  for (int x = 0; x < c.parts; ++x) {
-    const float* p = at(x);
-    const float y = __ldcg(p + RB * D + r), f = ex2(y - ref);
-    float u[V];
-    if (V == 4) {
-      const float4 t = __ldcg(reinterpret_cast<const float4*>(p + r * D) + lane);
-      u[0] = t.x; u[1] = t.y; u[V - 2] = t.z; u[V - 1] = t.w;
-    } else {
-      const float2 t = __ldcg(reinterpret_cast<const float2*>(p + r * D) + lane);
-      u[0] = t.x; u[1] = t.y;
-    }
-    if (y == -INFINITY) continue;  // a part that saw nothing
-    sum += f;
+  constexpr int HELD = 8;  // parts under way together
+  for (int x0 = 0; x0 < c.parts; x0 += HELD) {
+    float y[HELD], u[HELD][V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] += u[i] * f;
+    for (int x = 0; x < HELD; ++x) {
+      const float* p = at(min(x0 + x, c.parts - 1));
+      y[x] = __ldcg(p + RB * D + r);
+      if (V == 4) {
+        const float4 t = __ldcg(reinterpret_cast<const float4*>(p + r * D) + lane);
+        u[x][0] = t.x; u[x][1] = t.y; u[x][V - 2] = t.z; u[x][V - 1] = t.w;
+      } else {
+        const float2 t = __ldcg(reinterpret_cast<const float2*>(p + r * D) + lane);
+        u[x][0] = t.x; u[x][1] = t.y;
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int x = 0; x < HELD; ++x) {
+      if (x0 + x >= c.parts) y[x] = -INFINITY;
+      top = fmaxf(top, y[x]);
+    }
+    const float ref = top == -INFINITY ? 0.f : top, old = ex2(m - ref);
+    m = top;
+    sum *= old;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] *= old;
+#pragma unroll
+    for (int x = 0; x < HELD; ++x) {
+      if (y[x] == -INFINITY) continue;  // a part that saw nothing, or none
+      const float f = ex2(y[x] - ref);
+      sum += f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = fmaf(u[x][i], f, v[i]);
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int G = a.Hq / a.Hk, node = (c.row_base + r) / G, hq = c.h * G + c.row_base + r - node * G;
@@ -681,8 +721,11 @@ static int launch(const dspark_paged_attn_args& a, cudaStream_t s) {
                                                                cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
                                  }),
                   "paged_attn: shared memory");
-  const float c = a.scale * 1.4426950408889634f;
-  DSPARK_CUDA_TRY(launch_ex(attn_kernel<T, D, RT>, dim3(n), dim3(NTHR), L::TOTAL, s, 1, true, a, c, status_word(dev)),
+  // the running maximum needs a positive factor: a negative scale goes into q, and zero becomes one that leaves all
+  // weights equal
+  const float c = a.scale == 0.f ? 1e-30f : fabsf(a.scale) * 1.4426950408889634f;
+  DSPARK_CUDA_TRY(launch_ex(attn_kernel<T, D, RT>, dim3(n), dim3(NTHR), L::TOTAL, s, 1, true, a, c,
+                            a.scale < 0.f ? 0x80008000u : 0u, status_word(dev)),
                   "paged_attn");
   DSPARK_CUDA_TRY(launch_ex(join_kernel<T, D, L::RB>, dim3(n, L::RB / 4), dim3(128), 0, s, 1, true, a), "paged_attn: join");
   return DSPARK_OK;
@@ -722,6 +765,9 @@ int dspark_paged_attn(const dspark_paged_attn_args* p, void* stream) {
     return fail(DSPARK_ERR_UNSUPPORTED, "paged_attn: %d pages of %d tokens a request", a.max_pages, a.page);
   if (int64_t(a.R) * (a.Hq / a.Hk) > 0x3fffffff || (int64_t(a.R) * (a.Hq / a.Hk) / 16 + 1) * a.Hk > 0x3fffffff)
     return fail(DSPARK_ERR_UNSUPPORTED, "paged_attn: %d rows of %d heads in one call", a.R, a.Hq);
+  // costs are summed in 32 bits
+  if ((int64_t(a.R) * (a.Hq / a.Hk) / 16 + a.B) * a.Hk > 0x7fffffff / (int64_t(a.max_pages) * a.page / paged::BN + paged::SEG + 2))
+    return fail(DSPARK_ERR_UNSUPPORTED, "paged_attn: %d rows over %d pages a request in one call", a.R, a.max_pages);
   if (a.R == 0 || a.B == 0) return DSPARK_OK;
   if (!a.q || !a.out || !a.cu_rows || !a.kv_len || (a.max_pages && !a.page_table) ||
       (a.n_pages && (!a.k_pages || !a.v_pages || !a.k_scale || !a.v_scale)))

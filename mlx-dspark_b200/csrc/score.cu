@@ -247,6 +247,66 @@ __device__ __noinline__ void find_top(Shared& sh, const Row<T>& r, float m, int 
   }
 }
 
+// What a thread has taken in, and the token that it looks out for: its logit, the next larger value, log2(e) / T.
+struct Taken {
+  Sums z;
+  float xt, after, c;
+  int tok, before;
+};
+
+// N vectors of a thread (masked values kLow); vm[u] is the largest of x[u], tk + u * step the token of x[u][0].
+template <typename T, int N>
+__device__ __forceinline__ void take(Taken& t, float (&x)[N][Vec<T>::VE], float (&vm)[N], int tk, int step) {
+  constexpr int VE = Vec<T>::VE;
+  float bm = vm[0];
+#pragma unroll
+  for (int u = 1; u < N; ++u) bm = fmaxf(bm, vm[u]);
+  if (bm > Vec<T>::MAXV) {  // rare: values above the largest that counts
+    bm = Vec<T>::MAXV;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      vm[u] = fminf(vm[u], Vec<T>::MAXV);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) x[u][e] = fminf(x[u][e], Vec<T>::MAXV);
+    }
+  }
+  if (bm >= t.xt) {  // some may come before the token: as large ones before it, and larger ones
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int t0 = tk + u * step;
+      if (vm[u] < t.xt) continue;
+      if (t0 <= t.tok && t.tok < t0 + VE) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) t.before += x[u][e] >= (t0 + e < t.tok ? t.xt : t.after);
+      } else {
+        const float at = t0 < t.tok ? t.xt : t.after;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) t.before += x[u][e] >= at;
+      }
+    }
+  }
+  if (bm > t.z.m) raise(t.z, bm, t.c);
+  const f32x2 m2 = pack2(-t.z.m, -t.z.m), c2 = pack2(t.c, t.c);
+  f32x2 l2 = pack2(0.f, 0.f), s2 = pack2(0.f, 0.f);
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+#pragma unroll
+    for (int e = 0; e < VE; e += 2) {
+      const f32x2 y = mul2(add2(pack2(x[u][e], x[u][e + 1]), m2), c2);  // (the difference first: exact)
+      float y0, y1;
+      unpack2(y, y0, y1);
+      const f32x2 p = pack2(ex2(y0), ex2(y1));
+      l2 = add2(l2, p);
+      s2 = fma2(p, y, s2);
+    }
+  }
+  float a0, a1;
+  unpack2(l2, a0, a1);
+  t.z.l += a0 + a1;
+  unpack2(s2, a0, a1);
+  t.z.s += a0 + a1;
+}
+
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(THREADS, 4) score_kernel(const dspark_score_args a, const int cluster) {
   constexpr int VE = Vec<T>::VE;
@@ -289,89 +349,38 @@ __global__ void __launch_bounds__(THREADS, 4) score_kernel(const dspark_score_ar
   const float c = 1.4426950408889634f / T1;
   const float xt = fminf(Vec<T>::one(r.p[tok]), Vec<T>::MAXV);
   Sums z{kLow, 0.f, 0.f};
-  int before = 0;
-  const f32x2 c2 = pack2(c, c);
 
-  // n vectors of values (masked and missing ones kLow) whose largest is bm; v[u]: the token of x[u][0]
-  auto take = [&](float (&x)[U][VE], const float (&vm)[U], const int (&tk)[U]) {
-    float bm = vm[0];
-#pragma unroll
-    for (int u = 1; u < U; ++u) bm = fmaxf(bm, vm[u]);
-    if (bm >= xt) {  // some may come before the token
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (vm[u] < xt) continue;
-#pragma unroll
-        for (int e = 0; e < VE; ++e) before += x[u][e] > xt || (x[u][e] == xt && tk[u] + e < tok);
-      }
-    }
-    if (bm > z.m) raise(z, bm, c);
-    const f32x2 m2 = pack2(-z.m, -z.m);
-    f32x2 l2 = pack2(0.f, 0.f), s2 = pack2(0.f, 0.f);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int e = 0; e < VE; e += 2) {
-        const f32x2 y = mul2(add2(pack2(x[u][e], x[u][e + 1]), m2), c2);  // (the difference first: exact)
-        float y0, y1;
-        unpack2(y, y0, y1);
-        const f32x2 p = pack2(ex2(y0), ex2(y1));
-        l2 = add2(l2, p);
-        s2 = fma2(p, y, s2);
-      }
-    }
-    float a0, a1;
-    unpack2(l2, a0, a1);
-    z.l += a0 + a1;
-    unpack2(s2, a0, a1);
-    z.s += a0 + a1;
-  };
-  auto hold = [&](float (&x)[U][VE], float (&vm)[U]) {  // rare: values above the largest that counts
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (vm[u] <= Vec<T>::MAXV) continue;
-      vm[u] = Vec<T>::MAXV;
-#pragma unroll
-      for (int e = 0; e < VE; ++e) x[u][e] = fminf(x[u][e], Vec<T>::MAXV);
-    }
-  };
+  Taken t{z, xt, xt == 0.f ? __int_as_float(1) : xt >= Vec<T>::MAXV ? INFINITY : __int_as_float(__float_as_int(xt) + (xt > 0.f ? 1 : -1)),
+          c, tok, 0};
   const uint4* vec = reinterpret_cast<const uint4*>(r.p + r.head);
-  float x[U][VE], vm[U];
-  int tk[U];
-  for (int v = r.v0 + tid; v < r.v1; v += U * THREADS) {
+  int v = r.v0 + tid;
+  for (; v + (U - 1) * THREADS < r.v1; v += U * THREADS) {
     uint4 w[U];
+    float x[U][VE], vm[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v + u * THREADS < r.v1) w[u] = ldcg_v4(vec + v + u * THREADS);
+    for (int u = 0; u < U; ++u) w[u] = ldcg_v4(vec + v + u * THREADS);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      tk[u] = r.head + (v + u * THREADS) * VE;
-      if (v + u * THREADS < r.v1) {
-        vm[u] = Vec<T>::split(w[u], x[u]);
-      } else {
-        vm[u] = kLow;
-#pragma unroll
-        for (int e = 0; e < VE; ++e) x[u][e] = kLow;
-      }
-    }
-    hold(x, vm);
-    take(x, vm, tk);
+    for (int u = 0; u < U; ++u) vm[u] = Vec<T>::split(w[u], x[u]);
+    take<T, U>(t, x, vm, r.head + v * VE, THREADS * VE);
   }
-  const float strip = z.m;
+  for (; v < r.v1; v += THREADS) {
+    float x[1][VE], vm[1];
+    vm[0] = Vec<T>::split(ldcg_v4(vec + v), x[0]);
+    take<T, 1>(t, x, vm, r.head + v * VE, 0);
+  }
+  const float strip = t.z.m;
   const int t0 = r.head + r.nvec * VE;
   if ((r.first && tid < r.head) || (r.last && tid >= 32 && tid - 32 < a.V - t0)) {  // the ragged ends
-    const int v = tid < 32 ? tid : t0 + tid - 32;
+    const int at = tid < 32 ? tid : t0 + tid - 32;
+    float x[1][VE], vm[1];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      vm[u] = kLow;
-      tk[u] = v;
-#pragma unroll
-      for (int e = 0; e < VE; ++e) x[u][e] = kLow;
-    }
-    x[0][0] = vm[0] = Vec<T>::one(r.p[v]);
-    hold(x, vm);
-    take(x, vm, tk);
+    for (int e = 1; e < VE; ++e) x[0][e] = kLow;
+    x[0][0] = vm[0] = Vec<T>::one(r.p[at]);
+    // (the others are nobody's: they add nothing, and a token among them is not this thread's)
+    take<T, 1>(t, x, vm, at, 0);
   }
+  z = t.z;
+  int before = t.before;
   // (masked values were counted while nothing else had been seen; raise() has dropped them where something was)
   for (int o = 16; o; o >>= 1) {
     const Sums y{__shfl_xor_sync(0xffffffffu, z.m, o), __shfl_xor_sync(0xffffffffu, z.l, o),
