@@ -1,0 +1,822 @@
+// Attention over pages of 8-bit values for blocks of many rows (verify blocks, prompts' chunks), on the 5th-generation
+// tensor cores. The formulas, the cache and the shares are paged_attn.cu's; here an item is up to 256 rows of one
+// (request, kv head).
+//
+// Block (one an SM): two slots of 128 rows (TMEM lanes), each with a softmax warpgroup, a score tile S (TMEM, overwritten
+// by the 16-bit weights P) and an output accumulator O (TMEM).
+//  * items of more than 128 rows: the slots are the two halves of the rows and share each K/V tile;
+//  * items of up to 128 rows: the slots take the even and the odd key tiles and are joined at the segment's end.
+// Either way one slot's softmax runs under the other slot's products.
+//  * Four converting warps read the codes (16-byte cp.async into a ring of their own of 8-token pieces, page ids read 12
+//    tiles ahead) and write them as fp16, which holds every e4m3 value, into the ring of tiles that the products read:
+//    128 keys x D, 128-byte swizzled, K as it is multiplied (K-major) and V as it lies (N-major). A row is converted once for
+//    up to 256 rows of q; neither scale is multiplied in. Beside a K tile go its 16-key groups' factors.
+//  * Two warps walk ahead and write the next segment's Q as fp16 (bf16 rows scaled by a power of two: exact).
+//  * One thread issues the products: S = Q K^T (both from shared memory), O += P V (P from tensor memory).
+//  * A thread of a softmax warpgroup owns a row: no shuffles. x = f s + log2(vs), f = log2(e) scale 2^e ks, of each group;
+//    the maximum in use is only raised when a tile exceeds it by more than 2^8; weights are 2^7 times as large.
+//
+// Rounding: weights are rounded to fp16 for the product with V (their sum is not); scores, maxima, sums and O are fp32.
+#include <algorithm>
+
+#include "host_common.h"
+#include "paged_share.cuh"
+#include "tcgen05.cuh"
+
+namespace dspark {
+namespace paged {
+namespace wide {
+
+constexpr int ROWS = 128;            // rows a slot
+constexpr int RB = 2 * ROWS;         // rows an item
+constexpr int NTHR = 512;            // two softmax warpgroups, one of the products and Q, one that converts
+constexpr int WARP_MMA = 8, WARP_PREP = 10, WARP_CONV = 12;
+constexpr int SEG = 7;               // cost of a segment, in tiles of up to 128 rows
+constexpr int NB = 4;                // tiles in the ring
+constexpr int PIECE = 8;             // tokens of a piece of codes
+constexpr int NP = 7;                // pieces in a converting warp's ring
+constexpr int NSC = 4;               // tiles whose factors are kept: until V of tile t is read, K of t + 4 is not written
+
+template <int D>
+struct Lay {
+  static constexpr int TILE = BN * D * 2;         // a K or V tile (and a slot's Q)
+  static constexpr int HALF = BN * 128;           // 64 values of 128 rows, 128-byte swizzled
+  static constexpr int CODES = PIECE * D + 16;    // a piece: its codes, {ks, vs}, a note
+  static constexpr int Q = 0;
+  static constexpr int RING = 2 * TILE;
+  static constexpr int STAGE = RING + NB * TILE;
+  static constexpr int ML = STAGE + 4 * NP * CODES;   // [slot][row] (m, l) at the segment's end
+  static constexpr int RF = ML + 2 * ROWS * 8;        // [segment & 1][slot][row] the rows' powers of two
+  static constexpr int SC = RF + 2 * RB * 4;          // [tile & 3][16-key group] (ks, log2 vs)
+  static constexpr int FLAG = SC + NSC * 8 * 8;
+  static constexpr int SEGS = FLAG + 16;              // two segments for the softmax threads
+  static constexpr int BARS = SEGS + 2 * 64;
+  static constexpr int NBAR = 2 * NB + 2 * 8 + NSC + 1;
+  static constexpr int MISC = BARS + NBAR * 8;        // tensor memory's address; 17 pairs of find_share
+  static constexpr int TOTAL = MISC + 8 + 17 * 8;
+  static_assert(TOTAL <= 232448, "shared memory of one SM");
+  static_assert(CODES % 16 == 0 && BARS % 8 == 0, "alignment");
+};
+
+__device__ __forceinline__ void st_x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ void ld_x32(uint32_t taddr, float* d) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, "
+      "[%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) d[i] = __uint_as_float(r[i]);
+}
+
+// D[tmem] (+)= A[smem] . B[smem]^T
+__device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 128-byte-swizzled operand: K-major (lbo unused, 8-row groups 1024 bytes apart) or MN-major (lbo between 64-value
+// blocks of MN, 8-row groups of K 1024 bytes apart). Only the low word (address, lbo) varies.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) {
+  return ((addr >> 4) & 0x3FFF) | ((lbo >> 4) << 16);
+}
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t lo) {
+  constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);  // sbo, version, 128-byte swizzle
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(HI));
+  return d;
+}
+
+__device__ __forceinline__ void named_sync(int id, int n) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
+}
+
+// named_sync that tells all its threads whether `ok` held in every one of them.
+__device__ __forceinline__ bool named_all(int id, int n, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(uint32_t(ok)), "r"(id), "r"(n)
+      : "memory");
+  return r != 0;
+}
+
+// A segment as the walking warps hand it to the softmax threads.
+struct Handed {
+  Segment s;
+  int more;
+};
+static_assert(sizeof(Handed) <= 64, "Lay::SEGS");
+
+__device__ __forceinline__ bool is_pair(const Segment& s) { return s.live > ROWS; }
+
+// Load u of a segment of n tiles, in the order that the products take them: K0 V0 K1 V1 .. (pair) or K0 K1 V0 K2 V1 ..
+// (tiles alternate between the slots). Returns the tile; `value`: V.
+__device__ __forceinline__ int load_of(bool pair, int u, int n, bool& value) {
+  if (pair) {
+    value = u & 1;
+    return u >> 1;
+  }
+  if (u == 2 * n - 1) {
+    value = true;
+    return n - 1;
+  }
+  value = u > 0 && !(u & 1);
+  return value ? (u - 2) >> 1 : (u + 1) >> 1;
+}
+
+// Use of the ring (within the segment) by the V tile of tile t.
+__device__ __forceinline__ int v_use(bool pair, int t, int n) {
+  return pair ? 2 * t + 1 : t == n - 1 ? 2 * n - 1 : 2 * t + 2;
+}
+
+// The NaN codes that were taken out of the segment's V tiles, added to what a row that sees them has stored (`out`: the
+// output, or `part`: the fp32 part).
+template <typename T>
+__device__ __noinline__ void add_hidden(const dspark_paged_attn_args& a, const Segment& s, int lim, int d0, int d1, T* out,
+                                        float* part) {
+  const int k0 = max(s.t0 * BN, max(s.before, 0)), k1 = min(min(s.t1 * BN, s.len), lim);
+  for (int k = k0; k < k1; ++k) {
+    const int id = a.page_table[int64_t(s.b) * a.table_stride + k / a.page];
+    if (id < 0 || id >= a.n_pages) continue;
+    const int64_t sc = id * a.scale_strides[0] + s.h * a.scale_strides[1];
+    if (!(a.k_scale[sc] > 0.f && a.v_scale[sc] > 0.f)) continue;
+    const uint8_t* v = static_cast<const uint8_t*>(a.v_pages) + id * a.vp_strides[0] + s.h * a.vp_strides[1] +
+                       (k % a.page) * a.vp_strides[2];
+    for (int d = d0; d < d1; ++d) {
+      if ((v[d] & 0x7f) != 0x7f) continue;
+      if (part) part[d] = NAN;
+      else out[d] = Elem<T>::from_f(NAN);
+    }
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_args a, const float c_log2,
+                                                       const uint32_t q_sign, int* status) {
+  typedef Lay<D> L;
+  constexpr uint32_t ID_QK = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(ROWS >> 4) << 24);  // fp16, fp32 sums
+  constexpr uint32_t ID_PV = (1u << 4) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(ROWS >> 4) << 24);
+  constexpr uint32_t O_COL = 256;
+  constexpr float LIFT = 7.f, SLACK = 8.f;  // weights are at most 2^15
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* ring = smem + L::RING;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BARS);
+  uint64_t* empty = full + NB;
+  uint64_t* q_full = empty + NB;
+  uint64_t* s_full = q_full + 2;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* p_part = p_full + 2;
+  uint64_t* o_full = p_part + 2;
+  uint64_t* q_empty = o_full + 2;
+  uint64_t* seg_full = q_empty + 2;
+  uint64_t* seg_empty = seg_full + 2;
+  uint64_t* sc_full = seg_empty + 2;
+  uint64_t* fin = sc_full + NSC;
+  float2* ml = reinterpret_cast<float2*>(smem + L::ML);
+  float* rowf = reinterpret_cast<float*>(smem + L::RF);
+  float2* factors = reinterpret_cast<float2*>(smem + L::SC);
+  int* flag = reinterpret_cast<int*>(smem + L::FLAG);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
+  uint2* pairs = reinterpret_cast<uint2*>(smem + L::MISC + 8);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (smem_u32(smem) & 1023u) {  // the swizzled tiles need it; never seen without static arrays
+    if (tid == 0) report_error(status, 0x208);
+    return;
+  }
+  if (tid == 0) {
+    for (int i = 0; i < NB; ++i) {
+      mbar_init(&full[i], 4);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {  // p_*, q_full and seg_empty count warps
+      mbar_init(&q_full[i], 2);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&seg_full[i], 1);
+      mbar_init(&seg_empty[i], 8);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_part[i], 4);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) flag[i] = 0;
+    for (int i = 0; i < NSC; ++i) mbar_init(&sc_full[i], 4);
+    mbar_init(fin, 1);
+    fence_mbar_init();
+  }
+  if (warp == WARP_MMA) tcg::tmem_alloc(tmem_slot, 512);
+  pdl_launch_dependents();
+  pdl_wait();
+  Plan<RB> plan{a, 0};
+  Walker<RB> wk;
+  const Deal deal = find_share<RB, NTHR>(plan, SEG, wk, pairs, pairs + 16);
+  tcg::tc_fence_before();
+  __syncthreads();
+  tcg::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int G = a.Hq / a.Hk;
+  bool ok = true;
+
+  if (warp < WARP_MMA) {
+    // ------------------------------------------- softmax: slot = warpgroup, row = TMEM lane
+    // (registers: 256 * 184 + 256 * 72 = 512 * 128, what the block was launched with)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    const int slot = warp >> 2, row = tid & 127;
+    const uint32_t t_s = tmem + (uint32_t((warp & 3) * 32) << 16) + uint32_t(slot * 128);
+    const uint32_t t_o = t_s + O_COL;
+    uint32_t n_s = 0;              // completed phases of s_full
+    uint32_t n_o0 = 0, n_o1 = 0;   // of o_full
+    int use0 = 0, tiles0 = 0;      // ring uses and tiles before this segment
+    auto arrive = [&](uint64_t* bar) {  // this warp's stores to tensor memory are done
+      tcg::tmem_wait_st();
+      tcg::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    // flag[seg & 3] == seg: a hidden NaN in segment `seg`. The converting warps are two segments ahead at most: beyond the
+    // first product of the next one, which needs no weights, they have room for NB = 4 tiles.
+    for (int seg = 1;; ++seg) {
+      const int hand = (seg - 1) & 1;
+      const Handed& sh = *reinterpret_cast<const Handed*>(smem + L::SEGS + 64 * hand);
+      if (ok) ok = mbar_wait(&seg_full[hand], uint32_t((seg - 1) >> 1) & 1u, status, kErrWaitPeer);
+      // after a wait that ran out all leave together: the barriers below count all of them
+      ok = named_all(3, 256, ok);
+      if (!ok || !sh.more) break;
+      const Segment& s = sh.s;
+      const int n = s.t1 - s.t0;
+      const bool pair = is_pair(s);
+      const int steps = pair ? n : (n - slot + 1) >> 1;
+      const int my = s.row_base + (pair ? slot * ROWS : 0) + row;  // (node, head) row of this thread
+      const bool alive = my < s.rows * G;
+      const bool warp_alive = s.row_base + (pair ? slot * ROWS : 0) + (warp & 3) * 32 < s.rows * G;
+      const int place = alive ? my / G : 0;
+      const int lim = a.causal ? min(s.len, s.before + place + 1) : s.len;  // keys that the row sees
+      const int edge0 = (a.causal ? min(s.len, s.before + s.row_base / G + 1) : s.len) - BN;  // later: hidden keys
+      const float rf = rowf[hand * RB + (pair ? slot * ROWS : 0) + row];
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < steps; ++j) {
+        const int t = pair ? j : 2 * j + slot, k0 = (s.t0 + t) * BN, tile = tiles0 + t;
+        const bool edge = k0 > edge0;
+        if (ok) ok = mbar_wait(&sc_full[tile % NSC], uint32_t(tile / NSC) & 1u, status, kErrWaitKV);
+        if (ok) ok = mbar_wait(&s_full[slot], n_s & 1, status, kErrWaitMma);
+        ++n_s;
+        tcg::tc_fence_after();
+        if (edge && (slot == 0 || !pair)) {
+          // NaN codes have been taken out of V and noted. Not before the scores: they are made of K(t), and the previous use
+          // of V(t)'s buffer was loaded before K(t) (NB - 1 uses lie between at most), so the parity waited for here cannot
+          // be that of an earlier, still missing load
+          const int g = use0 + v_use(pair, t, n);
+          if (ok) ok = mbar_wait(&full[g % NB], uint32_t(g / NB) & 1u, status, kErrWaitKV);
+        }
+        if (warp_alive) {
+          float x[128];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ld_x32(t_s + uint32_t(32 * i), x + 32 * i);
+          const float2* fa = factors + (tile % NSC) * 8;
+          tcg::tmem_wait_ld();
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            const float2 y = fa[g];
+            const float f = rf * y.x;
+            const f32x2 f2 = pack2(f, f), l2 = pack2(y.y, y.y);
+#pragma unroll
+            for (int i = 16 * g; i < 16 * g + 16; i += 2) {
+              const f32x2 z = fma2(pack2(x[i], x[i + 1]), f2, l2);
+              unpack2(z, x[i], x[i + 1]);
+            }
+          }
+          if (edge) {
+            const int left = lim - k0;
+#pragma unroll
+            for (int i = 0; i < 128; ++i) x[i] = i < left ? x[i] : -INFINITY;
+          }
+          float mx[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mx[e] = max3(x[2 * e], x[2 * e + 1], x[16 + e]);
+#pragma unroll
+          for (int i = 24; i < 120; i += 16) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx[e] = max3(mx[e], x[i + 2 * e], x[i + 2 * e + 1]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[120 + 2 * e], x[120 + 2 * e + 1]);
+          const float mt = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max3(mx[6], mx[7], mx[7]));
+          if (!(mt < INFINITY)) m = NAN;  // a visible score of +inf or NaN: the row is NaN
+          const bool up = mt - m > SLACK;
+          if (__any_sync(0xffffffffu, up)) {
+            const float mn = up ? mt : m;
+            const float f = up ? ex2(m - mn) : 1.f;
+            m = mn;
+            l *= f;
+            if (j > 0) {
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) {
+                float o[16];
+                tcg::tmem_ld16(t_o + uint32_t(16 * i), o);
+                tcg::tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] *= f;
+                st_x16(t_o + uint32_t(16 * i), reinterpret_cast<const uint32_t*>(o));
+              }
+            }
+          }
+          const float ref = LIFT - (m == -INFINITY ? 0.f : m);
+          const f32x2 r2 = pack2(ref, ref);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {  // 32 columns: two groups
+            uint32_t p[16];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float lv = fa[2 * q + h].y, iv = lv == -INFINITY ? 0.f : ex2(-lv);
+              f32x2 sum = pack2(0.f, 0.f);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int z = 32 * q + 16 * h + 2 * i;
+                float e0, e1;
+                unpack2(add2(pack2(x[z], x[z + 1]), r2), e0, e1);
+                const f32x2 e = pack2(ex2(e0), ex2(e1));
+                unpack2(e, e0, e1);
+                sum = add2(sum, e);
+                p[8 * h + i] = Elem<__half>::pack(e0, e1);
+              }
+              float s0, s1;
+              unpack2(sum, s0, s1);
+              l = fmaf(s0 + s1, iv, l);
+            }
+            st_x16(t_s + uint32_t(16 * q), p);
+            if (q == 2) arrive(&p_part[slot]);  // three quarters' products may start
+          }
+        } else {
+          arrive(&p_part[slot]);
+        }
+        arrive(&p_full[slot]);
+      }
+      use0 += 2 * n;
+      tiles0 += n;
+      // ---- end of the segment: with one row block, both slots' O of half of the values
+      const bool both = !pair && n > 1;
+      if (n > 0) {
+        if (ok && steps > 0) ok = mbar_wait(&o_full[slot], (slot ? n_o1 : n_o0) & 1, status, kErrWaitMma);
+        if (ok && both) ok = mbar_wait(&o_full[slot ^ 1], (slot ? n_o0 : n_o1) & 1, status, kErrWaitMma);
+        if (!pair && slot == 1 && n == 1 && ok) ok = mbar_wait(&o_full[0], n_o0 & 1, status, kErrWaitMma);
+        ++n_o0;
+        n_o1 += pair || n > 1;
+      }
+      tcg::tc_fence_after();
+      const bool whole = s.parts == 1;
+      float f0 = 1.f, f1 = 0.f;
+      if (!pair) {
+        ml[slot * ROWS + row] = make_float2(m, l);
+        named_sync(3, 256);
+        const float2 a0 = ml[row], a1 = ml[ROWS + row];
+        // (a NaN in either is the row's: fmaxf would lose it)
+        const float mn = a0.x != a0.x || a1.x != a1.x ? NAN : fmaxf(a0.x, a1.x), ref = mn == -INFINITY ? 0.f : mn;
+        f0 = ex2(a0.x - ref);
+        f1 = ex2(a1.x - ref);
+        l = a0.y * f0 + a1.y * f1;
+        m = mn;
+      }
+      const bool hidden = *reinterpret_cast<volatile int*>(&flag[seg & 3]) == seg;
+      if (warp_alive) {
+        const int hq = s.h * G + my - place * G;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int prow = (pair ? slot * ROWS : 0) + row;
+        float* pp = whole ? nullptr : part_of<D, RB>(a.workspace, blockIdx.x, int(blockIdx.x) == s.first);
+        // 32-value chunks: all of the slot's own, or every second one of both slots'
+        const int i0 = pair ? 0 : slot * (D / 64), i1 = pair ? D / 32 : i0 + D / 64;
+        const uint32_t t_0 = pair ? t_o : tmem + (uint32_t((warp & 3) * 32) << 16) + O_COL;
+        T* out = static_cast<T*>(a.out) + int64_t(s.r0 + place) * a.o_strides[0] + hq * a.o_strides[1];
+        if (!whole && alive && (pair || slot == 0)) pp[RB * D + prow] = l == 0.f ? -INFINITY : m + lg2(l);
+        if (n > 0) {
+#pragma unroll 1
+          for (int i = i0; i < i1; ++i) {
+            float o[32];
+            ld_x32(t_0 + uint32_t(32 * i), o);
+            tcg::tmem_wait_ld();
+            if (both) {
+              float o1[32];
+              ld_x32(t_0 + 128u + uint32_t(32 * i), o1);
+              tcg::tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = o[e] * f0 + o1[e] * f1;
+            }
+            if (alive && !whole) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<float4*>(pp + prow * D + 32 * i + e) =
+                    l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                             : make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+            } else if (alive) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 8) {
+                uint4 v;
+                v.x = Elem<T>::pack(o[e] * inv, o[e + 1] * inv);
+                v.y = Elem<T>::pack(o[e + 2] * inv, o[e + 3] * inv);
+                v.z = Elem<T>::pack(o[e + 4] * inv, o[e + 5] * inv);
+                v.w = Elem<T>::pack(o[e + 6] * inv, o[e + 7] * inv);
+                *reinterpret_cast<uint4*>(out + 32 * i + e) = l == 0.f ? make_uint4(0u, 0u, 0u, 0u) : v;
+              }
+            }
+          }
+          if (hidden && alive) add_hidden<T>(a, s, lim, 32 * i0, 32 * i1, out, whole ? nullptr : pp + prow * D);
+        }
+      }
+      tcg::tc_fence_before();
+      if (!pair) named_sync(3, 256);  // both have read both: the next weights may be given
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_empty[hand]);
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    Segment s{};
+    if (warp >= WARP_CONV) {
+      // -------------------------------------------------------------- codes to fp16 tiles
+      constexpr int CH = D / 16, RPI = 32 / CH, ROUNDS = PIECE / RPI;  // 16-byte chunks a row, rows a round of copies
+      const int w = warp - WARP_CONV, shift = 31 - __clz(a.page);
+      uint8_t* stage = smem + L::STAGE + w * NP * L::CODES;
+      const uint32_t stage_a = smem_u32(stage);
+      const int kts = int(a.kp_strides[2]), vts = int(a.vp_strides[2]);
+      // the copies' cursor: load u of the segment, its piece
+      int u = 0, piece = 0, n = 0, issued = 0, tiles0 = 0, seg = 0;
+      bool more = true;
+      int ids_even = -1, ids_odd = -1;  // pages of 16 tiles' halves of this warp's 32 rows: tile lane >> 1, half lane & 1
+      auto page_ids = [&](int window) {
+        int id = -1;
+        const int t = window * 16 + (lane >> 1), key = (s.t0 + t) * BN + w * 32 + (lane & 1) * 16;
+        if (t < n && key < s.len) {
+          id = a.page_table[int64_t(s.b) * a.table_stride + (key >> shift)];
+          if (id < 0 || id >= a.n_pages) {
+            report_error(status, kErrAttnPage);
+            id = -1;
+          }
+        }
+        return id;
+      };
+      auto issue = [&]() {
+        while (more && u == 2 * n) {  // the next segment
+          tiles0 += n;
+          more = wk.next(plan, deal, s);
+          ++seg;
+          n = more ? s.t1 - s.t0 : 0;
+          u = 0;
+          if (more && n > 0) {
+            ids_even = page_ids(0);
+            ids_odd = page_ids(1);
+          }
+          if (!more) break;
+        }
+        if (more) {
+          bool value;
+          const int t = load_of(is_pair(s), u, n, value);
+          if (!value && piece == 0 && t >= 16 && (t & 15) == 4) {  // (V is at most two tiles behind K)
+            if ((t >> 4) & 1) ids_even = page_ids((t >> 4) + 1);
+            else ids_odd = page_ids((t >> 4) + 1);
+          }
+          const int id = __shfl_sync(0xffffffffu, (t >> 4) & 1 ? ids_odd : ids_even, (t & 15) * 2 + (piece >> 1));
+          const int key0 = (s.t0 + t) * BN + w * 32 + piece * PIECE;
+          const uint32_t dst = stage_a + (issued % NP) * L::CODES;
+          const bool page = id >= 0 && key0 < s.len;
+          if (lane < 2) {
+            const int64_t at = page ? id * a.scale_strides[0] + s.h * a.scale_strides[1] : 0;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + PIECE * D + lane * 4),
+                         "l"((lane ? a.v_scale : a.k_scale) + at), "r"(page ? 4 : 0)
+                         : "memory");
+          }
+          if (lane == 2)  // K: 1 + 2 tile; V with keys that not every row sees: - segment
+            *reinterpret_cast<int*>(stage + (issued % NP) * L::CODES + PIECE * D + 8) =
+                !value ? 1 + 2 * (tiles0 + t) : key0 + PIECE > s.before ? -seg : 0;
+          const int64_t ps = value ? a.vp_strides[0] : a.kp_strides[0], hs = value ? a.vp_strides[1] : a.kp_strides[1];
+          const int ts = value ? vts : kts;
+          const uint8_t* src = static_cast<const uint8_t*>(value ? a.v_pages : a.k_pages);
+          const uint8_t* p = src + (page ? id * ps + s.h * hs + int64_t((key0 & (a.page - 1)) + lane / CH) * ts : 0) + lane % CH * 16;
+#pragma unroll
+          for (int z = 0; z < ROUNDS; ++z) {
+            const bool there = page && key0 + z * RPI + lane / CH < s.len;
+            cp_async_16_zfill(dst + (z * 32 + lane) * 16, there ? p + z * RPI * ts : src, there);
+          }
+          ++issued;
+          if (++piece == 4) {
+            piece = 0;
+            ++u;
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+#pragma unroll 1
+      for (int i = 0; i < NP - 1; ++i) issue();
+      for (int done = 0; done < issued && ok; ++done) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(NP - 2) : "memory");
+        __syncwarp();
+        issue();
+        const int load = done >> 2, pc = done & 3, x = load % NB;
+        if (pc == 0 && load >= NB) {
+          ok = mbar_wait(&empty[x], uint32_t(load / NB - 1) & 1u, status, kErrWaitKVEmpty);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
+        const uint8_t* from = stage + (done % NP) * L::CODES;
+        const int note = *reinterpret_cast<const int*>(from + PIECE * D + 8);
+        const float ks = *reinterpret_cast<const float*>(from + PIECE * D), vs = *reinterpret_cast<const float*>(from + PIECE * D + 4);
+        const bool fine = ks > 0.f && vs > 0.f;  // a page without a positive scale (or none) is not seen
+        uint8_t* tile = ring + x * L::TILE;
+#pragma unroll
+        for (int z = 0; z < ROUNDS; ++z) {
+          const int r = w * 32 + pc * PIECE + z * RPI + lane / CH, c = lane % CH;
+          uint4 v = *reinterpret_cast<const uint4*>(from + (z * 32 + lane) * 16);
+          if (!fine) v = make_uint4(0u, 0u, 0u, 0u);
+          if (note < 0) {
+            uint32_t* y = &v.x;
+            uint32_t any = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t nan = (((y[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+              any |= nan;
+              y[k] &= ~(nan * 0xffu);
+            }
+            if (any) *reinterpret_cast<volatile int*>(&flag[(-note) & 3]) = -note;
+          }
+          const uint4 h0 = make_uint4(e4m3_to_f16(v.x), e4m3_to_f16_hi(v.x), e4m3_to_f16(v.y), e4m3_to_f16_hi(v.y));
+          const uint4 h1 = make_uint4(e4m3_to_f16(v.z), e4m3_to_f16_hi(v.z), e4m3_to_f16(v.w), e4m3_to_f16_hi(v.w));
+          // the lanes of the upper 64 values store their halves the other way round: no two on one bank
+          uint8_t* base = tile + (c >> 2) * L::HALF + r * 128;
+          const int cc = (c & 3) * 2, sw = r & 7, first = c >> 2;
+          *reinterpret_cast<uint4*>(base + (((cc + first) ^ sw) << 4)) = first ? h1 : h0;
+          *reinterpret_cast<uint4*>(base + (((cc + (first ^ 1)) ^ sw) << 4)) = first ? h0 : h1;
+        }
+        if (note > 0 && !(pc & 1) && lane == 0)
+          factors[((note >> 1) % NSC) * 8 + w * 2 + (pc >> 1)] = fine ? make_float2(ks, lg2(vs)) : make_float2(1.f, -INFINITY);
+        if (pc == 3) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&full[x]);
+            if (note > 0) mbar_arrive(&sc_full[(note >> 1) % NSC]);
+          }
+        }
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
+    } else if (warp >= WARP_PREP) {
+      // -------------------------------------------------------------- segments and Q, ahead
+      constexpr int CH = D / 8, STEP = 64 / CH;  // 16-byte chunks a row, rows the 64 threads load at a time
+      const int t = tid - WARP_PREP * 32, c = t % CH, first_row = t / CH;
+      uint32_t n_q[2] = {0, 0};
+      Cut cut{0, 0, 0, 0, 0, {0, 0, 0}};
+      auto load_q = [&](int slot, int hand) {
+        if (n_q[slot] > 0 && ok) ok = mbar_wait(&q_empty[slot], (n_q[slot] - 1) & 1u, status, kErrWaitMma);
+        ++n_q[slot];
+        const int row0 = s.row_base + (is_pair(s) ? slot * ROWS : 0);
+        const int live = min(ROWS, s.rows * G - row0);  // rows past it are never looked at
+        const T* q = static_cast<const T*>(a.q) + int64_t(s.r0) * a.q_strides[0] + s.h * G * a.q_strides[1] + c * 8;
+        uint8_t* dst = smem + L::Q + slot * L::TILE + (c >> 3) * L::HALF;
+        float* rf = rowf + hand * RB + (is_pair(s) ? slot * ROWS : 0);
+        constexpr int FLY = 4;
+        for (int r0 = 0; r0 < live; r0 += FLY * STEP) {
+          uint4 v[FLY];
+#pragma unroll
+          for (int z = 0; z < FLY; ++z) {
+            const int r = r0 + z * STEP + first_row, node = (row0 + r) / G, g = row0 + r - node * G;
+            v[z] = r < live ? ldcg_v4(q + node * a.q_strides[0] + g * a.q_strides[1]) : make_uint4(0u, 0u, 0u, 0u);
+          }
+#pragma unroll
+          for (int z = 0; z < FLY; ++z) {
+            const int r = r0 + z * STEP + first_row;
+            uint32_t* y = &v[z].x;
+            float f = 1.f;
+            if (std::is_same<T, bf16>::value) {  // largest exponent of the row; 255: infinite or NaN
+              uint32_t e = 0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) e = max(e, max((y[i] >> 7) & 0xffu, (y[i] >> 23) & 0xffu));
+#pragma unroll
+              for (int o = 1; o < CH; o <<= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, o));
+              const int up = int(e) - 141;  // values below 2^15
+              const float inv = pow2(max(min(-up, 126), -126));
+              f = e == 255 ? NAN : pow2(max(min(up, 126), -126));
+#pragma unroll
+              for (int i = 0; i < 4; ++i) y[i] = Elem<__half>::pack(bf16_lo(y[i]) * inv, bf16_hi(y[i]) * inv);
+            } else {  // an infinite q makes its row NaN whatever the codes are
+              uint32_t bad = 0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) bad |= (y[i] & 0x7c00u) == 0x7c00u || (y[i] & 0x7c000000u) == 0x7c000000u;
+#pragma unroll
+              for (int o = 1; o < CH; o <<= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+              f = bad ? NAN : 1.f;
+            }
+            if (r < live) {
+              if (c == 0) rf[r] = f * c_log2;
+              *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+                  make_uint4(y[0] ^ q_sign, y[1] ^ q_sign, y[2] ^ q_sign, y[3] ^ q_sign);
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[slot]);
+      };
+      for (int k = 0;; ++k) {
+        const int hand = k & 1;
+        ok = named_all(5, 64, ok);  // (both warps leave together)
+        const bool more = ok && wk.next(plan, deal, s);
+        if (k >= 2 && ok) ok = mbar_wait(&seg_empty[hand], uint32_t((k >> 1) - 1) & 1u, status, kErrWaitPeer);
+        if (more && s.t0 < s.t1) {
+          load_q(0, hand);
+          if (is_pair(s) || s.t1 - s.t0 > 1) load_q(1, hand);  // (the same rows for both where there are up to 128)
+        }
+        // handed over when the rows' factors are written: both warps'
+        named_sync(5, 64);
+        if (warp == WARP_PREP && lane == 0) {
+          Handed* h = reinterpret_cast<Handed*>(smem + L::SEGS + 64 * hand);
+          if (more) {
+            h->s = s;
+            if (s.parts > 1 && int(blockIdx.x) == s.first) cut = Cut{s.parts, s.r0, s.live, s.row_base, s.h, {0, 0, 0}};
+          }
+          h->more = more;
+          mbar_arrive(&seg_full[hand]);
+        }
+        if (!more) break;
+      }
+      if (warp == WARP_PREP && lane == 0) static_cast<Cut*>(a.workspace)[blockIdx.x] = cut;
+      __syncwarp();
+    } else if (warp == WARP_MMA) {
+      // -------------------------------------------------------------- products
+      // The whole warp walks and waits; one lane issues.
+      const uint32_t leader = tcg::elect_one() ? 1u : 0u;
+      const uint32_t q_lo = desc_lo(smem_u32(smem + L::Q), 16), ring_a = smem_u32(ring);
+      int x_ring = 0, g_phase = 0;
+      uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0};
+      bool issued = false;
+      auto take = [&]() {  // the next ring buffer, filled
+        const int x = x_ring;
+        if (ok) ok = mbar_wait(&full[x], uint32_t(g_phase), status, kErrWaitKV);
+        tcg::tc_fence_after();
+        if (++x_ring == NB) {
+          x_ring = 0;
+          g_phase ^= 1;
+        }
+        return x;
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (leader) tcg::umma_commit(bar);
+      };
+      auto scores = [&](int slot, int x, bool last) {
+        if (!ok) return;
+        const uint32_t qd = q_lo + uint32_t(slot) * (L::TILE >> 4);
+        const uint32_t kd = desc_lo(ring_a + uint32_t(x) * L::TILE, 16);
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = uint32_t((k >> 2) * (L::HALF >> 4) + (k & 3) * 2);
+            umma_ss(tmem + uint32_t(slot * 128), desc_sw128(qd + off), desc_sw128(kd + off), ID_QK, k ? 1u : 0u);
+          }
+          tcg::umma_commit(&s_full[slot]);
+          if (last) tcg::umma_commit(&q_empty[slot]);  // the segment's last use of this Q
+        }
+        issued = true;
+      };
+      auto values = [&](int slot, int x, bool first) {
+        const uint32_t vd = desc_lo(ring_a + uint32_t(x) * L::TILE, L::HALF);
+        const uint32_t ph = n_p[slot]++ & 1u;
+        const uint32_t d = tmem + O_COL + uint32_t(slot * 128), p = tmem + uint32_t(slot * 128);
+        if (ok) ok = mbar_wait(&p_part[slot], ph, status, kErrWaitMma);
+        if (!ok) return;
+        tcg::tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < 6; ++k)
+            tcg::umma_ts(d, p + uint32_t(8 * k), desc_sw128(vd + uint32_t(k * (2048 >> 4))), ID_PV, first && k == 0 ? 0u : 1u);
+        }
+        ok = mbar_wait(&p_full[slot], ph, status, kErrWaitMma);
+        if (!ok) return;
+        tcg::tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int k = 6; k < BN / 16; ++k)
+            tcg::umma_ts(d, p + uint32_t(8 * k), desc_sw128(vd + uint32_t(k * (2048 >> 4))), ID_PV, 1u);
+        }
+      };
+      auto release = [&](int x) {
+        if (ok) commit(&empty[x]);
+      };
+      auto q_ready = [&](int slot) {
+        if (ok) ok = mbar_wait(&q_full[slot], n_q[slot]++ & 1u, status, kErrWaitMma);
+        tcg::tc_fence_after();
+      };
+      while (__all_sync(0xffffffffu, ok) && wk.next(plan, deal, s)) {
+        const int n = __shfl_sync(0xffffffffu, s.t1 - s.t0, 0);
+        const bool pair = __shfl_sync(0xffffffffu, int(is_pair(s)), 0);
+        if (n <= 0) continue;
+        if (pair) {
+          int x = take();
+          q_ready(0);
+          scores(0, x, n == 1);
+          q_ready(1);
+          scores(1, x, n == 1);
+          release(x);
+          for (int t = 0; t < n; ++t) {
+            const int v = take();
+            const bool more = t + 1 < n;
+            values(0, v, t == 0);
+            if (more) {
+              x = take();
+              scores(0, x, t + 2 == n);
+            } else if (ok) {
+              commit(&o_full[0]);
+            }
+            values(1, v, t == 0);
+            release(v);
+            if (more) {
+              scores(1, x, t + 2 == n);
+              release(x);
+            } else if (ok) {
+              commit(&o_full[1]);
+            }
+            if (!__all_sync(0xffffffffu, ok)) break;
+          }
+        } else {
+          for (int z = 0; z < min(n, 2); ++z) {
+            const int x = take();
+            q_ready(z);
+            scores(z, x, z + 2 >= n);
+            release(x);
+          }
+          for (int t = 0; t < n; ++t) {
+            const int v = take(), z = t & 1;
+            values(z, v, t < 2);
+            release(v);
+            if (t + 2 < n) {
+              const int x = take();
+              scores(z, x, t + 4 >= n);
+              release(x);
+            } else if (ok) {
+              commit(&o_full[z]);
+            }
+            if (!__all_sync(0xffffffffu, ok)) break;
+          }
+        }
+      }
+      if (issued) {  // nothing may write tensor memory after the block releases it
+        commit(fin);
+        mbar_wait(fin, 0, nullptr, 0);  // (under the default limit)
+      }
+      __syncwarp();
+    }
+  }
+  tcg::tc_fence_before();
+  __syncthreads();
+  tcg::tc_fence_after();
+  if (warp == WARP_MMA) tcg::tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int D>
+static int launch(const dspark_paged_attn_args& a, cudaStream_t s) {
+  constexpr int TOTAL = Lay<D>::TOTAL;
+  const int dev = current_device(), n = std::min(sm_count(dev), MAX_CTA);
+  DSPARK_CUDA_TRY(configure_once((const void*)attn_kernel<T, D>, TOTAL,
+                                 [&] {
+                                   return cudaFuncSetAttribute(attn_kernel<T, D>,
+                                                               cudaFuncAttributeMaxDynamicSharedMemorySize, TOTAL);
+                                 }),
+                  "paged_attn: shared memory");
+  const float c = a.scale == 0.f ? 1e-30f : fabsf(a.scale) * 1.4426950408889634f;
+  DSPARK_CUDA_TRY(launch_ex(attn_kernel<T, D>, dim3(n), dim3(NTHR), TOTAL, s, 1, true, a, c,
+                            a.scale < 0.f ? 0x80008000u : 0u, status_word(dev)),
+                  "paged_attn");
+  DSPARK_CUDA_TRY(launch_ex(join_kernel<T, D, RB>, dim3(n, RB / 4), dim3(128), 0, s, 1, true, a), "paged_attn: join");
+  return DSPARK_OK;
+}
+
+}  // namespace wide
+
+size_t wide_workspace(int D) {
+  return MAX_CTA * sizeof(Cut) + size_t(std::min(sm_count(current_device()), MAX_CTA)) * 2 * wide::RB * (D + 1) * sizeof(float);
+}
+
+int launch_wide(const dspark_paged_attn_args& a, cudaStream_t s) {
+  if (a.dtype == DSPARK_DTYPE_BF16) return a.D == 128 ? wide::launch<bf16, 128>(a, s) : wide::launch<bf16, 64>(a, s);
+  return a.D == 128 ? wide::launch<__half, 128>(a, s) : wide::launch<__half, 64>(a, s);
+}
+
+}  // namespace paged
+}  // namespace dspark
