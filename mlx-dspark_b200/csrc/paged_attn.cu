@@ -30,7 +30,7 @@ namespace paged {
 constexpr int SUB = 32;      // keys a warp's subtile
 constexpr int WARPS = 4;
 constexpr int NTHR = WARPS * 32;
-constexpr int WIDE_ROWS = 32;
+constexpr int WIDE_ROWS = 128;
 constexpr int SEG = 5;       // cost of a segment, in tiles
 constexpr float LIFT = 11.f; // weights are 2^11 times as large in fp16 ...
 constexpr float SLACK = 4.f; // ... and the maximum in use may be 2^4 too low
@@ -500,7 +500,7 @@ static int launch(const dspark_paged_attn_args& a, cudaStream_t s) {
   return DSPARK_OK;
 }
 
-// Rows of a request and kv head, on average: more than 32 go to the 5th-generation tensor cores.
+// Rows of a request and kv head, on average: more than 128 go to the 5th-generation tensor cores.
 static bool is_wide(int R, int B, int Hq, int Hk) { return int64_t(R) * (Hq / Hk) > int64_t(WIDE_ROWS) * B; }
 
 template <typename T, int D>

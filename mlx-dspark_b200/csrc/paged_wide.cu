@@ -7,8 +7,7 @@
 //  * items of more than 128 rows: the slots are the two halves of the rows and share each K/V tile;
 //  * items of up to 128 rows: the slots take the even and the odd key tiles and are joined at the segment's end.
 // Either way one slot's softmax runs under the other slot's products.
-//  * Four converting warps read the codes (16-byte cp.async into a ring of their own of 8-token pieces, page ids read 12
-//    tiles ahead) and write them as fp16, which holds every e4m3 value, into the ring of tiles that the products read:
+//  * Four converting warps read the codes (16-byte cp.async into a ring of their own, page ids read 12 tiles ahead) and write them as fp16, which holds every e4m3 value, into the ring of tiles that the products read:
 //    128 keys x D, 128-byte swizzled, K as it is multiplied (K-major) and V as it lies (N-major). A row is converted once for
 //    up to 256 rows of q; neither scale is multiplied in. Beside a K tile go its 16-key groups' factors.
 //  * Two warps walk ahead and write the next segment's Q as fp16 (bf16 rows scaled by a power of two: exact).
@@ -32,16 +31,16 @@ constexpr int RB = 2 * ROWS;         // rows an item
 constexpr int NTHR = 512;            // two softmax warpgroups, one of the products and Q, one that converts
 constexpr int WARP_MMA = 8, WARP_PREP = 10, WARP_CONV = 12;
 constexpr int SEG = 7;               // cost of a segment, in tiles of up to 128 rows
-constexpr int NB = 4;                // tiles in the ring
-constexpr int PIECE = 8;             // tokens of a piece of codes
-constexpr int NP = 7;                // pieces in a converting warp's ring
+constexpr int NB = 3;                // tiles in the ring
+constexpr int PIECE = 32;            // tokens of a tile that one converting warp has
+constexpr int NP = 3;                // pieces in its ring
 constexpr int NSC = 4;               // tiles whose factors are kept: until V of tile t is read, K of t + 4 is not written
 
 template <int D>
 struct Lay {
   static constexpr int TILE = BN * D * 2;         // a K or V tile (and a slot's Q)
   static constexpr int HALF = BN * 128;           // 64 values of 128 rows, 128-byte swizzled
-  static constexpr int CODES = PIECE * D + 16;    // a piece: its codes, {ks, vs}, a note
+  static constexpr int CODES = PIECE * D + 32;    // a piece: its codes, two pages' {ks, vs}, a note
   static constexpr int Q = 0;
   static constexpr int RING = 2 * TILE;
   static constexpr int STAGE = RING + NB * TILE;
@@ -151,6 +150,10 @@ __device__ __forceinline__ int v_use(bool pair, int t, int n) {
   return pair ? 2 * t + 1 : t == n - 1 ? 2 * n - 1 : 2 * t + 2;
 }
 
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // The NaN codes that were taken out of the segment's V tiles, added to what a row that sees them has stored (`out`: the
 // output, or `part`: the fp32 part).
 template <typename T>
@@ -256,7 +259,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
       if (lane == 0) mbar_arrive(bar);
     };
     // flag[seg & 3] == seg: a hidden NaN in segment `seg`. The converting warps are two segments ahead at most: beyond the
-    // first product of the next one, which needs no weights, they have room for NB = 4 tiles.
+    // first product of the next one, which needs no weights, they have room for NB tiles.
     for (int seg = 1;; ++seg) {
       const int hand = (seg - 1) & 1;
       const Handed& sh = *reinterpret_cast<const Handed*>(smem + L::SEGS + 64 * hand);
@@ -285,7 +288,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
         tcg::tc_fence_after();
         if (edge && (slot == 0 || !pair)) {
           // NaN codes have been taken out of V and noted. Not before the scores: they are made of K(t), and the previous use
-          // of V(t)'s buffer was loaded before K(t) (NB - 1 uses lie between at most), so the parity waited for here cannot
+          // of V(t)'s buffer was loaded before K(t) or is K(t) itself, so the parity waited for here cannot
           // be that of an earlier, still missing load
           const int g = use0 + v_use(pair, t, n);
           if (ok) ok = mbar_wait(&full[g % NB], uint32_t(g / NB) & 1u, status, kErrWaitKV);
@@ -454,13 +457,14 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
     if (warp >= WARP_CONV) {
       // -------------------------------------------------------------- codes to fp16 tiles
       constexpr int CH = D / 16, RPI = 32 / CH, ROUNDS = PIECE / RPI;  // 16-byte chunks a row, rows a round of copies
-      const int w = warp - WARP_CONV, shift = 31 - __clz(a.page);
+      const int w = warp - WARP_CONV, shift = 31 - __clz(a.page), mask = a.page - 1;
       uint8_t* stage = smem + L::STAGE + w * NP * L::CODES;
-      const uint32_t stage_a = smem_u32(stage);
+      const uint32_t stage_a = smem_u32(stage) + lane * 16;
       const int kts = int(a.kp_strides[2]), vts = int(a.vp_strides[2]);
-      // the copies' cursor: load u of the segment, its piece
-      int u = 0, piece = 0, n = 0, issued = 0, tiles0 = 0, seg = 0;
-      bool more = true;
+      const int64_t k_lane = int64_t(lane / CH) * kts + lane % CH * 16, v_lane = int64_t(lane / CH) * vts + lane % CH * 16;
+      // the copies' cursor: load u of the segment
+      int u = 0, n = 0, tiles0 = 0, seg = 0, to = 0, issued = 0;
+      bool more = true, pair = false;
       int ids_even = -1, ids_odd = -1;  // pages of 16 tiles' halves of this warp's 32 rows: tile lane >> 1, half lane & 1
       auto page_ids = [&](int window) {
         int id = -1;
@@ -480,100 +484,125 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
           more = wk.next(plan, deal, s);
           ++seg;
           n = more ? s.t1 - s.t0 : 0;
+          pair = is_pair(s);
           u = 0;
           if (more && n > 0) {
             ids_even = page_ids(0);
             ids_odd = page_ids(1);
           }
-          if (!more) break;
         }
         if (more) {
           bool value;
-          const int t = load_of(is_pair(s), u, n, value);
-          if (!value && piece == 0 && t >= 16 && (t & 15) == 4) {  // (V is at most two tiles behind K)
+          const int t = load_of(pair, u, n, value);
+          if (!value && t >= 16 && (t & 15) == 4) {  // (V is at most two tiles behind K)
             if ((t >> 4) & 1) ids_even = page_ids((t >> 4) + 1);
             else ids_odd = page_ids((t >> 4) + 1);
           }
-          const int id = __shfl_sync(0xffffffffu, (t >> 4) & 1 ? ids_odd : ids_even, (t & 15) * 2 + (piece >> 1));
-          const int key0 = (s.t0 + t) * BN + w * 32 + piece * PIECE;
-          const uint32_t dst = stage_a + (issued % NP) * L::CODES;
-          const bool page = id >= 0 && key0 < s.len;
-          if (lane < 2) {
-            const int64_t at = page ? id * a.scale_strides[0] + s.h * a.scale_strides[1] : 0;
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + PIECE * D + lane * 4),
-                         "l"((lane ? a.v_scale : a.k_scale) + at), "r"(page ? 4 : 0)
+          const int ids = (t >> 4) & 1 ? ids_odd : ids_even, key0 = (s.t0 + t) * BN + w * 32;
+          const int id0 = __shfl_sync(0xffffffffu, ids, (t & 15) * 2), id1 = __shfl_sync(0xffffffffu, ids, (t & 15) * 2 + 1);
+          const uint32_t dst = stage_a + to * L::CODES;
+          if (lane < 4) {  // ks, vs of both halves
+            const int id = lane < 2 ? id0 : id1;
+            const int64_t at = id < 0 ? 0 : id * a.scale_strides[0] + s.h * a.scale_strides[1];
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst - lane * 12 + PIECE * D),
+                         "l"((lane & 1 ? a.v_scale : a.k_scale) + at), "r"(id < 0 ? 0 : 4)
                          : "memory");
           }
-          if (lane == 2)  // K: 1 + 2 tile; V with keys that not every row sees: - segment
-            *reinterpret_cast<int*>(stage + (issued % NP) * L::CODES + PIECE * D + 8) =
+          if (lane == 4)  // K: 1 + 2 tile; V with keys that not every row sees: - segment
+            *reinterpret_cast<int*>(stage + to * L::CODES + PIECE * D + 16) =
                 !value ? 1 + 2 * (tiles0 + t) : key0 + PIECE > s.before ? -seg : 0;
-          const int64_t ps = value ? a.vp_strides[0] : a.kp_strides[0], hs = value ? a.vp_strides[1] : a.kp_strides[1];
+          const uint8_t* src = value ? static_cast<const uint8_t*>(a.v_pages) + s.h * a.vp_strides[1] + v_lane
+                                     : static_cast<const uint8_t*>(a.k_pages) + s.h * a.kp_strides[1] + k_lane;
+          const int64_t ps = value ? a.vp_strides[0] : a.kp_strides[0];
           const int ts = value ? vts : kts;
-          const uint8_t* src = static_cast<const uint8_t*>(value ? a.v_pages : a.k_pages);
-          const uint8_t* p = src + (page ? id * ps + s.h * hs + int64_t((key0 & (a.page - 1)) + lane / CH) * ts : 0) + lane % CH * 16;
+          const uint8_t* p0 = src + (id0 * ps + int64_t(key0 & mask) * ts);
+          const uint8_t* p1 = src + (id1 * ps + int64_t((key0 + 16) & mask) * ts);
+          if (id0 >= 0 && id1 >= 0 && key0 + PIECE <= s.len) {
 #pragma unroll
-          for (int z = 0; z < ROUNDS; ++z) {
-            const bool there = page && key0 + z * RPI + lane / CH < s.len;
-            cp_async_16_zfill(dst + (z * 32 + lane) * 16, there ? p + z * RPI * ts : src, there);
+            for (int z = 0; z < ROUNDS; ++z)
+              cp_async_16(dst + z * 512, (z < ROUNDS / 2 ? p0 : p1) + z % (ROUNDS / 2) * RPI * ts);
+          } else {
+#pragma unroll 1
+            for (int z = 0; z < ROUNDS; ++z) {
+              const bool low = z < ROUNDS / 2, there = (low ? id0 : id1) >= 0 && key0 + z * RPI + lane / CH < s.len;
+              cp_async_16_zfill(dst + z * 512, there ? (low ? p0 : p1) + z % (ROUNDS / 2) * RPI * ts : src, there);
+            }
           }
           ++issued;
-          if (++piece == 4) {
-            piece = 0;
-            ++u;
-          }
+          ++u;
+          if (++to == NP) to = 0;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
 #pragma unroll 1
       for (int i = 0; i < NP - 1; ++i) issue();
-      for (int done = 0; done < issued && ok; ++done) {
+      int from = 0, x = 0, use = 0;
+      for (int done = 0; done < issued; ++done) {
         asm volatile("cp.async.wait_group %0;" ::"n"(NP - 2) : "memory");
         __syncwarp();
         issue();
-        const int load = done >> 2, pc = done & 3, x = load % NB;
-        if (pc == 0 && load >= NB) {
-          ok = mbar_wait(&empty[x], uint32_t(load / NB - 1) & 1u, status, kErrWaitKVEmpty);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
+        if (use > 0) {
+          ok = mbar_wait(&empty[x], uint32_t(use - 1) & 1u, status, kErrWaitKVEmpty);
+          if (!__all_sync(0xffffffffu, ok)) break;
         }
-        const uint8_t* from = stage + (done % NP) * L::CODES;
-        const int note = *reinterpret_cast<const int*>(from + PIECE * D + 8);
-        const float ks = *reinterpret_cast<const float*>(from + PIECE * D), vs = *reinterpret_cast<const float*>(from + PIECE * D + 4);
-        const bool fine = ks > 0.f && vs > 0.f;  // a page without a positive scale (or none) is not seen
-        uint8_t* tile = ring + x * L::TILE;
-#pragma unroll
-        for (int z = 0; z < ROUNDS; ++z) {
-          const int r = w * 32 + pc * PIECE + z * RPI + lane / CH, c = lane % CH;
-          uint4 v = *reinterpret_cast<const uint4*>(from + (z * 32 + lane) * 16);
-          if (!fine) v = make_uint4(0u, 0u, 0u, 0u);
-          if (note < 0) {
-            uint32_t* y = &v.x;
-            uint32_t any = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t nan = (((y[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-              any |= nan;
-              y[k] &= ~(nan * 0xffu);
-            }
-            if (any) *reinterpret_cast<volatile int*>(&flag[(-note) & 3]) = -note;
-          }
+        const uint8_t* codes = stage + from * L::CODES;
+        const float4 sc = *reinterpret_cast<const float4*>(codes + PIECE * D);
+        const int note = *reinterpret_cast<const int*>(codes + PIECE * D + 16);
+        // a page without a positive scale (or none) is not seen
+        const bool fine0 = sc.x > 0.f && sc.y > 0.f, fine1 = sc.z > 0.f && sc.w > 0.f;
+        const int r = lane / CH, c = lane % CH;  // the lane's row of a round, its chunk
+        // the lanes of the upper 64 values store their halves the other way round: no two on one bank
+        uint8_t* base = ring + x * L::TILE + (c >> 2) * L::HALF + (w * 32 + r) * 128;
+        const int cc = (c & 3) * 2, first = c >> 2;
+        auto put = [&](int z, uint4 v) {
           const uint4 h0 = make_uint4(e4m3_to_f16(v.x), e4m3_to_f16_hi(v.x), e4m3_to_f16(v.y), e4m3_to_f16_hi(v.y));
           const uint4 h1 = make_uint4(e4m3_to_f16(v.z), e4m3_to_f16_hi(v.z), e4m3_to_f16(v.w), e4m3_to_f16_hi(v.w));
-          // the lanes of the upper 64 values store their halves the other way round: no two on one bank
-          uint8_t* base = tile + (c >> 2) * L::HALF + r * 128;
-          const int cc = (c & 3) * 2, sw = r & 7, first = c >> 2;
-          *reinterpret_cast<uint4*>(base + (((cc + first) ^ sw) << 4)) = first ? h1 : h0;
-          *reinterpret_cast<uint4*>(base + (((cc + (first ^ 1)) ^ sw) << 4)) = first ? h0 : h1;
-        }
-        if (note > 0 && !(pc & 1) && lane == 0)
-          factors[((note >> 1) % NSC) * 8 + w * 2 + (pc >> 1)] = fine ? make_float2(ks, lg2(vs)) : make_float2(1.f, -INFINITY);
-        if (pc == 3) {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&full[x]);
-            if (note > 0) mbar_arrive(&sc_full[(note >> 1) % NSC]);
+          const int sw = (r + z * RPI) & 7;  // (w * 32 is a multiple of 8)
+          *reinterpret_cast<uint4*>(base + z * RPI * 128 + (((cc + first) ^ sw) << 4)) = first ? h1 : h0;
+          *reinterpret_cast<uint4*>(base + z * RPI * 128 + (((cc + (first ^ 1)) ^ sw) << 4)) = first ? h0 : h1;
+        };
+        if (note >= 0 && fine0 && fine1) {
+#pragma unroll
+          for (int z0 = 0; z0 < ROUNDS; z0 += 4) {  // four in flight
+            uint4 v[4];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) v[z] = *reinterpret_cast<const uint4*>(codes + ((z0 + z) * 32 + lane) * 16);
+#pragma unroll
+            for (int z = 0; z < 4; ++z) put(z0 + z, v[z]);
           }
+        } else {
+#pragma unroll 1
+          for (int z = 0; z < ROUNDS; ++z) {
+            uint4 v = *reinterpret_cast<const uint4*>(codes + (z * 32 + lane) * 16);
+            if (!(z < ROUNDS / 2 ? fine0 : fine1)) v = make_uint4(0u, 0u, 0u, 0u);
+            if (note < 0) {
+              uint32_t* y = &v.x;
+              uint32_t any = 0;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t nan = (((y[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+                any |= nan;
+                y[k] &= ~(nan * 0xffu);
+              }
+              if (any) *reinterpret_cast<volatile int*>(&flag[(-note) & 3]) = -note;
+            }
+            put(z, v);
+          }
+        }
+        if (note > 0 && lane < 2)
+          factors[((note >> 1) % NSC) * 8 + w * 2 + lane] =
+              lane ? (fine1 ? make_float2(sc.z, lg2(sc.w)) : make_float2(1.f, -INFINITY))
+                   : (fine0 ? make_float2(sc.x, lg2(sc.y)) : make_float2(1.f, -INFINITY));
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&full[x]);
+          if (note > 0) mbar_arrive(&sc_full[(note >> 1) % NSC]);
+        }
+        if (++from == NP) from = 0;
+        if (++x == NB) {
+          x = 0;
+          ++use;
         }
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
