@@ -725,9 +725,9 @@ size_t dspark_paged_attn_workspace(int R, int B, int Hq, int Hk, int D);
 /* Log probabilities of given tokens. With p = softmax(logits / T) of a row (T = temperature[r], NULL: 1; 1e-6 or less:
  * all mass on the first largest logit, above 1e6: 1e6): logprob = ln p(token), entropy = -sum p ln p, rank = tokens
  * before it in the order (larger logit, then lower token; 0: the most likely), and the first `top` (<= 32) tokens
- * of that order with their log probabilities (top_ids, top_logprob [R, top]). A logit that is NaN, -inf, or -2^100 or
+ * of that order with their log probabilities (top_ids, top_logprob [R, top]). A logit that is NaN, -inf, or -2^28 or
  * less (fp16: its lowest value) is a masked token's: probability 0, logprob -inf, rank -1, never an alternative; missing
- * alternatives have id -1 and -inf. One above 2^100 (fp16: inf) counts as 2^100 (the largest value). A row with no
+ * alternatives have id -1 and -inf. One above 2^28 (fp16: inf) counts as 2^28 (the largest value). A row with no
  * other tokens: logprob -inf, entropy 0, rank -1. A token outside 0 .. V - 1: its row is not read; logprob and entropy
  * 0, rank -1, no alternatives. bf16, fp16 or fp32, fp32 arithmetic. (The reference samples only,
  * src/mlx_dspark/sampling.py.) */

@@ -22,13 +22,15 @@ namespace dspark {
 namespace score {
 
 constexpr int THREADS = 256;
-constexpr int U = 4;          // vectors in flight a thread
+constexpr int U = 4;          // vectors of a chunk a thread
+constexpr int CHUNK = U * THREADS;
 constexpr int MAX_TOP = 32;
 constexpr int MAX_CLUSTER = 8;
-constexpr int CAND = 1024;    // values at or above the bound that a block sorts at once
+constexpr int CAND = 512;     // values at or above the bound that a block sorts at once
+constexpr int PARTS = 4;      // parts of the block's chunks whose largest values are kept by thread
 
 // A logit at or below kLow (NaN and -inf among them) is a masked token's, one above kHigh counts as kHigh.
-constexpr float kLow = -0x1p100f, kHigh = 0x1p100f;
+constexpr float kLow = -0x1p28f, kHigh = 0x1p28f;
 
 template <typename T>
 struct Vec;
@@ -40,16 +42,14 @@ struct Vec<bf16> {
   static constexpr float MAXV = kHigh;
   static __device__ __forceinline__ float split(uint4 w, float* x) {
     const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-    uint32_t mx = 0xF180F180u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t y;  // (the number of the two where one is NaN)
-      asm("max.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(in[i]), "r"(0xF180F180u));
-      asm("max.bf16x2 %0, %0, %1;" : "+r"(mx) : "r"(y));
+      asm("max.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(in[i]), "r"(0xCD80CD80u));
       x[2 * i] = bf16_lo(y);
       x[2 * i + 1] = bf16_hi(y);
     }
-    return fmaxf(bf16_lo(mx), bf16_hi(mx));
+    return max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7]));
   }
   static __device__ __forceinline__ float one(bf16 v) { return fmaxf(__bfloat162float(v), kLow); }
 };
@@ -60,19 +60,21 @@ struct Vec<__half> {
   static constexpr float MAXV = 65504.f;
   static __device__ __forceinline__ float split(uint4 w, float* x) {
     const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-    uint32_t mx = 0xFBFFFBFFu;
+    uint32_t low = 0x7BFF7BFFu;  // the smallest
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t y;
       asm("max.f16x2 %0, %1, %2;" : "=r"(y) : "r"(in[i]), "r"(0xFBFFFBFFu));
-      asm("max.f16x2 %0, %0, %1;" : "+r"(mx) : "r"(y));
+      asm("min.f16x2 %0, %0, %1;" : "+r"(low) : "r"(y));
       const float2 f = Elem<__half>::unpack(y);
-      x[2 * i] = f.x <= -65504.f ? kLow : f.x;
-      x[2 * i + 1] = f.y <= -65504.f ? kLow : f.y;
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
     }
-    const float2 f = Elem<__half>::unpack(mx);
-    const float m = fmaxf(f.x, f.y);
-    return m <= -65504.f ? kLow : m;
+    if ((low & 0xffffu) == 0xFBFFu || (low >> 16) == 0xFBFFu) {  // masked values: below all that an fp16 can be
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = x[i] <= -65504.f ? kLow : x[i];
+    }
+    return max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7]));
   }
   static __device__ __forceinline__ float one(__half v) {
     const float f = fmaxf(__half2float(v), -65504.f);
@@ -88,18 +90,21 @@ struct Vec<float> {
     const uint32_t in[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = fmaxf(__uint_as_float(in[i]), kLow);
-    return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    return fmaxf(max3(x[0], x[1], x[2]), x[3]);
   }
   static __device__ __forceinline__ float one(float v) { return fmaxf(v, kLow); }
 };
 
-// What a part of a row adds up to; sums are in units of log2.
+// What a part of a row adds up to; sums are in units of log2, relative to the reference of m. Without a temperature
+// that is m c as it is rounded, y = x c - (m c) one operation (x c is exact in it) and no value is lost to the rounding of the
+// reference (|m c| < 2^29: it is off by less than 2^6). With one it is m itself, y = (x - m) c.
 struct Sums {
   float m, l, s;
 };
 
+template <bool TEMP>
 __device__ __forceinline__ void raise(Sums& a, float m, float c) {
-  const float d = (a.m - m) * c;  // at most 0
+  const float d = TEMP ? (a.m - m) * c : __fmul_rn(a.m, c) - __fmul_rn(m, c);  // at most 0
   a.m = m;
   if (d < -200.f) {  // (also the start, where m was kLow)
     a.l = 0.f;
@@ -111,10 +116,11 @@ __device__ __forceinline__ void raise(Sums& a, float m, float c) {
   }
 }
 
+template <bool TEMP>
 __device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
   const float m = fmaxf(a.m, b.m);
-  raise(a, m, c);
-  raise(b, m, c);
+  raise<TEMP>(a, m, c);
+  raise<TEMP>(b, m, c);
   return Sums{m, a.l + b.l, a.s + b.s};
 }
 
@@ -129,6 +135,7 @@ __device__ __forceinline__ float value_of(uint64_t key) {
 }
 
 struct Shared {
+  float last[THREADS];  // the threads' largest values
   Sums warp[THREADS / 32];
   int rank[THREADS / 32];
   uint64_t top[MAX_TOP];  // the block's alternatives in order, 0 behind the last
@@ -137,8 +144,11 @@ struct Shared {
   float bound;
   int n_strip, n_cand;
   uint64_t best[THREADS / 32];
-  uint64_t cand[CAND];    // at first the threads' maxima
-  uint16_t strip[THREADS];
+  union {
+    float maxima[PARTS][THREADS];  // of the strips
+    uint64_t cand[CAND];
+  };
+  uint16_t strip[PARTS * THREADS];
 };
 
 __device__ __forceinline__ uint64_t remote_u64(const void* p, uint32_t rank) {
@@ -153,6 +163,7 @@ struct Row {
   int V, head;    // values, those before the first 16-byte vector
   int nvec;       // vectors
   int v0, v1;     // the block's
+  int chunks, part;  // its chunks, those of a part
   bool first, last;
 };
 
@@ -161,54 +172,79 @@ __device__ __forceinline__ void place_top(Shared& sh, const uint64_t* cand, int 
   for (int i = threadIdx.x; i < n; i += THREADS) {
     const uint64_t k = cand[i];
     int before = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) before += cand[j] > k;
     if (before < top && k) out[before] = k;
   }
 }
 
-// The block's alternatives into sh.top. m: the largest value of the thread's strip.
+// The block's alternatives into sh.top. m: the largest value that the thread has seen in its vectors, all parts' strips.
 template <typename T>
 __device__ __noinline__ void find_top(Shared& sh, const Row<T>& r, float m, int top) {
   constexpr int VE = Vec<T>::VE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  float* maxima = reinterpret_cast<float*>(sh.cand);
-  maxima[tid] = m;
-  if (tid < MAX_TOP) sh.top[tid] = 0;
-  if (tid == 0) sh.n_strip = sh.n_cand = 0;
-  __syncthreads();
-  if (warp == 0) {  // the top-th largest maximum, bit by bit from above
-    uint32_t b[THREADS / 32], t = 0;
+  if (warp == 0) {  // the top-th largest of the threads' values, two bits at a time below what all have in common
+    uint32_t b[THREADS / 32], t, hi = 0, lo = ~0u;
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) b[i] = uint32_t(key_of(maxima[32 * i + lane], 0) >> 32);
+    for (int i = 0; i < THREADS / 32; ++i) {
+      b[i] = uint32_t(key_of(sh.last[32 * i + lane], 0) >> 32);
+      hi = max(hi, b[i]);
+      lo = min(lo, b[i]);
+    }
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    const int from = hi == lo ? -2 : (31 - __clz(hi ^ lo)) & ~1;  // the pair of the first bit that differs
+    t = from < 0 ? hi : from == 30 ? 0u : hi >> (from + 2) << (from + 2);
 #pragma unroll 1
-    for (int bit = 31; bit >= (sizeof(T) == 2 ? 13 : 0); --bit) {
-      const uint32_t y = t | 1u << bit;
-      int n = 0;
+    for (int bit = from; bit >= (sizeof(T) == 2 ? 12 : 0); bit -= 2) {
+      const uint32_t one = 1u << bit, y1 = t + one, y2 = t + 2 * one, y3 = t + 3 * one;
+      uint32_t n12 = 0, n3 = 0;
 #pragma unroll
-      for (int i = 0; i < THREADS / 32; ++i) n += b[i] >= y;
-      if (int(__reduce_add_sync(0xffffffffu, unsigned(n))) >= top) t = y;
+      for (int i = 0; i < THREADS / 32; ++i) {
+        n12 += (b[i] >= y1) + ((b[i] >= y2) << 16);
+        n3 += b[i] >= y3;
+      }
+      n12 = __reduce_add_sync(0xffffffffu, n12);
+      n3 = __reduce_add_sync(0xffffffffu, n3);
+      const uint32_t want = uint32_t(top);
+      t = n3 >= want ? y3 : (n12 >> 16) >= want ? y2 : (n12 & 0xffffu) >= want ? y1 : t;
     }
     if (lane == 0) sh.bound = value_of(uint64_t(t) << 32);
   }
   __syncthreads();
   const float bound = sh.bound;
-  if (m >= bound && m > kLow) sh.strip[atomicAdd(&sh.n_strip, 1)] = uint16_t(tid);
-  __syncthreads();
+  if (m >= bound && m > kLow) {
+    for (int p = 0; p < PARTS; ++p) {
+      const float x = sh.maxima[p][tid];
+      if (x >= bound && x > kLow) sh.strip[atomicAdd(&sh.n_strip, 1)] = uint16_t(p * THREADS + tid);
+    }
+  }
+  __syncthreads();  // (the maxima have been read: the candidates take their place)
   auto offer = [&](float x, int v) {
     if (x > kLow && x >= bound) {
       const int at = atomicAdd(&sh.n_cand, 1);
       if (at < CAND) sh.cand[at] = key_of(x, v);
     }
   };
-  const int per = (r.v1 - r.v0 + THREADS - 1) / THREADS, n = sh.n_strip * per;
+  const int per = r.part * U, n = sh.n_strip * per;
   const uint4* vec = reinterpret_cast<const uint4*>(r.p + r.head);
-  for (int j = tid; j < n; j += THREADS) {
-    const int g = j / per, v = r.v0 + (j - g * per) * THREADS + sh.strip[g];
-    if (v >= r.v1) continue;
-    float x[VE];
-    if (Vec<T>::split(ldcg_v4(vec + v), x) < bound) continue;
+  for (int j0 = tid; j0 < n; j0 += 4 * THREADS) {
+    uint4 w[4];
+    int at[4];
 #pragma unroll
-    for (int e = 0; e < VE; ++e) offer(fminf(x[e], Vec<T>::MAXV), r.head + v * VE + e);
+    for (int i = 0; i < 4; ++i) {
+      const int j = j0 + i * THREADS, g = j / per, k = j - g * per, s = j < n ? sh.strip[g] : 0;
+      at[i] = r.v0 + (s / THREADS * r.part * U + k) * THREADS + s % THREADS;
+      if (j >= n || at[i] >= r.v1) at[i] = -1;
+      if (at[i] >= 0) w[i] = ldcg_v4(vec + at[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x[VE];
+      if (at[i] < 0 || Vec<T>::split(w[i], x) < bound) continue;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) offer(fminf(x[e], Vec<T>::MAXV), r.head + at[i] * VE + e);
+    }
   }
   if (r.first && tid < r.head) offer(fminf(Vec<T>::one(r.p[tid]), Vec<T>::MAXV), tid);
   const int t0 = r.head + r.nvec * VE;
@@ -255,7 +291,7 @@ struct Taken {
 };
 
 // N vectors of a thread (masked values kLow); vm[u] is the largest of x[u], tk + u * step the token of x[u][0].
-template <typename T, int N>
+template <typename T, bool TEMP, int N>
 __device__ __forceinline__ void take(Taken& t, float (&x)[N][Vec<T>::VE], float (&vm)[N], int tk, int step) {
   constexpr int VE = Vec<T>::VE;
   float bm = vm[0];
@@ -285,14 +321,15 @@ __device__ __forceinline__ void take(Taken& t, float (&x)[N][Vec<T>::VE], float 
       }
     }
   }
-  if (bm > t.z.m) raise(t.z, bm, t.c);
-  const f32x2 m2 = pack2(-t.z.m, -t.z.m), c2 = pack2(t.c, t.c);
+  if (bm > t.z.m) raise<TEMP>(t.z, bm, t.c);
+  const float ref = TEMP ? -t.z.m : -__fmul_rn(t.z.m, t.c);
+  const f32x2 m2 = pack2(ref, ref), c2 = pack2(t.c, t.c);
   f32x2 l2 = pack2(0.f, 0.f), s2 = pack2(0.f, 0.f);
 #pragma unroll
   for (int u = 0; u < N; ++u) {
 #pragma unroll
     for (int e = 0; e < VE; e += 2) {
-      const f32x2 y = mul2(add2(pack2(x[u][e], x[u][e + 1]), m2), c2);  // (the difference first: exact)
+      const f32x2 v = pack2(x[u][e], x[u][e + 1]), y = TEMP ? mul2(add2(v, m2), c2) : fma2(v, c2, m2);
       float y0, y1;
       unpack2(y, y0, y1);
       const f32x2 p = pack2(ex2(y0), ex2(y1));
@@ -307,8 +344,8 @@ __device__ __forceinline__ void take(Taken& t, float (&x)[N][Vec<T>::VE], float 
   t.z.s += a0 + a1;
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(THREADS, 4) score_kernel(const dspark_score_args a, const int cluster) {
+template <typename T, bool TOP, bool TEMP>
+__global__ void __launch_bounds__(THREADS, 5) score_kernel(const dspark_score_args a, const int cluster) {
   constexpr int VE = Vec<T>::VE;
   __shared__ Shared sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -337,11 +374,13 @@ __global__ void __launch_bounds__(THREADS, 4) score_kernel(const dspark_score_ar
   r.nvec = (a.V - r.head) / VE;
   r.v0 = int(int64_t(r.nvec) * part / cluster);
   r.v1 = int(int64_t(r.nvec) * (part + 1) / cluster);
+  r.chunks = (r.v1 - r.v0 + CHUNK - 1) / CHUNK;
+  r.part = max(1, (r.chunks + PARTS - 1) / PARTS);
   r.first = part == 0;
   r.last = part == cluster - 1;
   float T1 = 1.f;
   bool greedy = false;
-  if (a.temperature) {
+  if (TEMP) {
     T1 = a.temperature[row];
     greedy = !(T1 > 1e-6f);
     T1 = greedy ? 1.f : fminf(T1, 1e6f);
@@ -352,21 +391,37 @@ __global__ void __launch_bounds__(THREADS, 4) score_kernel(const dspark_score_ar
 
   Taken t{z, xt, xt == 0.f ? __int_as_float(1) : xt >= Vec<T>::MAXV ? INFINITY : __int_as_float(__float_as_int(xt) + (xt > 0.f ? 1 : -1)),
           c, tok, 0};
-  const uint4* vec = reinterpret_cast<const uint4*>(r.p + r.head);
-  int v = r.v0 + tid;
-  for (; v + (U - 1) * THREADS < r.v1; v += U * THREADS) {
+  const uint4* vec = reinterpret_cast<const uint4*>(r.p + r.head) + r.v0 + tid;
+  float part_max = kLow;
+  int left = r.part;
+  for (int k = 0; k < r.chunks; ++k) {
+    const int tk = r.head + (r.v0 + k * CHUNK + tid) * VE, n = r.v1 - r.v0 - k * CHUNK;
     uint4 w[U];
     float x[U][VE], vm[U];
+    if (n >= CHUNK) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = ldcg_v4(vec + v + u * THREADS);
+      for (int u = 0; u < U; ++u) w[u] = ldcg_v4(vec + k * CHUNK + u * THREADS);
+    } else {  // the last chunk: missing vectors are masked ones
+      const uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, bf16>::value ? 0xff80ff80u : 0xfc00fc00u;  // -inf
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        w[u] = u * THREADS + tid < n ? ldcg_v4(vec + k * CHUNK + u * THREADS) : make_uint4(none, none, none, none);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) vm[u] = Vec<T>::split(w[u], x[u]);
-    take<T, U>(t, x, vm, r.head + v * VE, THREADS * VE);
+    take<T, TEMP, U>(t, x, vm, tk, THREADS * VE);
+    if (TOP) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) part_max = fmaxf(part_max, vm[u]);
+    }
+    if (TOP && (--left == 0 || k + 1 == r.chunks)) {
+      sh.maxima[k / r.part][tid] = fminf(part_max, Vec<T>::MAXV);
+      part_max = kLow;
+      left = r.part;
+    }
   }
-  for (; v < r.v1; v += THREADS) {
-    float x[1][VE], vm[1];
-    vm[0] = Vec<T>::split(ldcg_v4(vec + v), x[0]);
-    take<T, 1>(t, x, vm, r.head + v * VE, 0);
+  if (TOP) {  // parts without chunks
+    for (int p = (r.chunks + r.part - 1) / r.part; p < PARTS; ++p) sh.maxima[p][tid] = kLow;
   }
   const float strip = t.z.m;
   const int t0 = r.head + r.nvec * VE;
@@ -377,7 +432,7 @@ __global__ void __launch_bounds__(THREADS, 4) score_kernel(const dspark_score_ar
     for (int e = 1; e < VE; ++e) x[0][e] = kLow;
     x[0][0] = vm[0] = Vec<T>::one(r.p[at]);
     // (the others are nobody's: they add nothing, and a token among them is not this thread's)
-    take<T, 1>(t, x, vm, at, 0);
+    take<T, TEMP, 1>(t, x, vm, at, 0);
   }
   z = t.z;
   int before = t.before;
@@ -385,7 +440,7 @@ __global__ void __launch_bounds__(THREADS, 4) score_kernel(const dspark_score_ar
   for (int o = 16; o; o >>= 1) {
     const Sums y{__shfl_xor_sync(0xffffffffu, z.m, o), __shfl_xor_sync(0xffffffffu, z.l, o),
                  __shfl_xor_sync(0xffffffffu, z.s, o)};
-    z = join(z, y, c);
+    z = join<TEMP>(z, y, c);
   }
   before = int(__reduce_add_sync(0xffffffffu, unsigned(before)));
   if (lane == 0) {
@@ -393,20 +448,26 @@ __global__ void __launch_bounds__(THREADS, 4) score_kernel(const dspark_score_ar
     sh.rank[warp] = before;
   }
   if (TOP) {
-    find_top<T>(sh, r, strip, a.top);
-  } else {
-    __syncthreads();
+    sh.last[tid] = strip;
+    if (tid < MAX_TOP) sh.top[tid] = 0;
+    if (tid == 0) sh.n_strip = sh.n_cand = 0;
   }
-  if (tid == 0) {
-    Sums y = sh.warp[0];
-    int n = sh.rank[0];
-    for (int i = 1; i < THREADS / 32; ++i) {
-      y = join(y, sh.warp[i], c);
-      n += sh.rank[i];
+  __syncthreads();
+  if (warp == 1) {  // (warp 0 has the alternatives' bound to find)
+    Sums y = sh.warp[lane & 7];
+#pragma unroll
+    for (int o = 1; o < THREADS / 32; o <<= 1) {
+      const Sums q{__shfl_xor_sync(0xffffffffu, y.m, o), __shfl_xor_sync(0xffffffffu, y.l, o),
+                   __shfl_xor_sync(0xffffffffu, y.s, o)};
+      y = join<TEMP>(y, q, c);
     }
-    sh.sum = y;
-    sh.before = n;
+    const int n = __reduce_add_sync(0xffffffffu, lane < THREADS / 32 ? unsigned(sh.rank[lane]) : 0u);
+    if (lane == 0) {
+      sh.sum = y;
+      sh.before = n;
+    }
   }
+  if (TOP) find_top<T>(sh, r, strip, a.top);
   if (cluster > 1) {
     cluster_sync_all();
     if (part == 0) {
@@ -430,7 +491,7 @@ __global__ void __launch_bounds__(THREADS, 4) score_kernel(const dspark_score_ar
         for (int q = 1; q < cluster; ++q) {
           const uint32_t at = mapa_shared(smem_u32(&sh.sum), q);
           const Sums o{ld_dsmem_f32(at), ld_dsmem_f32(at + 4), ld_dsmem_f32(at + 8)};
-          y = join(y, o, c);
+          y = join<TEMP>(y, o, c);
           n += __float_as_int(ld_dsmem_f32(mapa_shared(smem_u32(&sh.before), q)));
         }
         sh.sum = y;
@@ -443,9 +504,12 @@ __global__ void __launch_bounds__(THREADS, 4) score_kernel(const dspark_score_ar
     const Sums y = sh.sum;
     const bool any = y.m > kLow;
     const float ln = any ? logf(y.l) : 0.f;
+    auto lp = [&](float v) {
+      return (TEMP ? (v - y.m) / T1 : fmaf(v, c, -__fmul_rn(y.m, c)) * 0.6931471805599453f) - ln;
+    };
     if (tid == 0) {
       const bool live = any && xt > kLow;
-      a.logprob[row] = !live ? -INFINITY : greedy ? (sh.before == 0 ? 0.f : -INFINITY) : (xt - y.m) / T1 - ln;
+      a.logprob[row] = !live ? -INFINITY : greedy ? (sh.before == 0 ? 0.f : -INFINITY) : lp(xt);
       a.entropy[row] = !any || greedy ? 0.f : fmaxf(ln - y.s / y.l * 0.6931471805599453f, 0.f);
       a.rank[row] = live ? sh.before : -1;
     }
@@ -456,7 +520,7 @@ __global__ void __launch_bounds__(THREADS, 4) score_kernel(const dspark_score_ar
         const float v = value_of(key);
         a.top_ids[int64_t(row) * a.top + k] = key ? int32_t(~uint32_t(key)) : -1;
         a.top_logprob[int64_t(row) * a.top + k] =
-            !key ? -INFINITY : greedy ? (k == 0 ? 0.f : -INFINITY) : (v - y.m) / T1 - ln;
+            !key ? -INFINITY : greedy ? (k == 0 ? 0.f : -INFINITY) : lp(v);
       }
     }
   }
@@ -468,12 +532,13 @@ static cudaError_t launch(const dspark_score_args& a, cudaStream_t s) {
   // blocks a row: one wave of blocks or more, slices of 4 KB or more
   const int sms = sm_count(current_device());
   int cluster = 1;
-  while (cluster < MAX_CLUSTER && int64_t(a.R) * cluster < 4 * sms &&
+  while (cluster < MAX_CLUSTER && int64_t(a.R) * cluster < 2 * sms &&
          int64_t(a.V) * int(sizeof(T)) >= int64_t(cluster) * 2 * 4096)
     cluster *= 2;
   const dim3 grid(unsigned(a.R) * cluster);
-  return a.top ? launch_ex(score_kernel<T, true>, grid, dim3(THREADS), 0, s, cluster, true, a, cluster)
-               : launch_ex(score_kernel<T, false>, grid, dim3(THREADS), 0, s, cluster, true, a, cluster);
+  auto kernel = a.top ? (a.temperature ? score_kernel<T, true, true> : score_kernel<T, true, false>)
+                      : (a.temperature ? score_kernel<T, false, true> : score_kernel<T, false, false>);
+  return launch_ex(kernel, grid, dim3(THREADS), 0, s, cluster, true, a, cluster);
 }
 
 }  // namespace score

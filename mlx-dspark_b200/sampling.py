@@ -117,7 +117,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: t
     token; 0 is the most likely) and with ``top`` (up to 32) the first tokens of that order, ``top_ids`` and
     ``top_logprobs`` ``[R, top]``; ``out``, a former call's result of as many rows and alternatives, is written again.
 
-    A logit of NaN, -inf, or at most -2^100 (fp16: its lowest value) masks its token: logprob -inf, rank -1, never
+    A logit of NaN, -inf, or at most -2^28 (fp16: its lowest value) masks its token: logprob -inf, rank -1, never
     an alternative; where fewer tokens than ``top`` are left, the others' ids are -1 and their logprobs -inf. A row
     whose token is outside the vocabulary (-1: a padded row) is not read: logprob and entropy 0, rank -1, no
     alternatives."""

@@ -69,7 +69,7 @@ def score(row: torch.Tensor, token: int, temperature: float, top: int, low: floa
     that masks its token."""
     x = row.double().clone()
     x[torch.isnan(x) | (x <= low)] = -math.inf
-    x[x == math.inf] = 2.0 ** 100 if row.dtype is not torch.float16 else 65504.0
+    x = x.clamp(max=2.0 ** 28 if row.dtype is not torch.float16 else 65504.0)  # larger ones count as that
     live = x > -math.inf
     order = [int(i) for i in torch.sort(x, descending=True, stable=True).indices if live[int(i)]] if top else []
     V = x.numel()

@@ -135,7 +135,7 @@ def test_reference_rounding_is_the_types():
 def test_reference_scale_and_score():
     assert ref.scale_of(448.0) == 1.0 and ref.scale_of(448.5) == 2.0 and ref.scale_of(224.0) == 0.5
     assert ref.scale_of(0.0) == 2.0 ** -64 and ref.scale_of(1e38) == 2.0 ** 64
-    lp, ent, rank, ids, tl = ref.score(torch.tensor([1.0, 3.0, -math.inf, 3.0]), 3, 1.0, 4, -2.0 ** 100)
+    lp, ent, rank, ids, tl = ref.score(torch.tensor([1.0, 3.0, -math.inf, 3.0]), 3, 1.0, 4, -2.0 ** 28)
     z = math.exp(1) + 2 * math.exp(3)
     assert rank == 1 and ids == [1, 3, 0, -1] and abs(lp - (3 - math.log(z))) < 1e-12
     p = [math.exp(1) / z, math.exp(3) / z, math.exp(3) / z]

@@ -507,7 +507,7 @@ def test_attention_long_context(cuda, rows):
 
 # ------------------------------------------------------------------------------- scores
 
-LOW = {BF: -2.0 ** 100, FP: -2.0 ** 100, HF: -65504.0}
+LOW = {BF: -2.0 ** 28, FP: -2.0 ** 28, HF: -65504.0}
 
 
 def _check_scores(cuda, logits, tokens, temp, top, out=None):
