@@ -505,7 +505,10 @@ static bool is_wide(int R, int B, int Hq, int Hk) { return int64_t(R) * (Hq / Hk
 
 template <typename T, int D>
 static int launch_rows(const dspark_paged_attn_args& a, cudaStream_t s) {
-  if (is_wide(a.R, a.B, a.Hq, a.Hk)) return launch_wide(a, s);
+  if (is_wide(a.R, a.B, a.Hq, a.Hk) && a.n_pages > 0) {
+    const int rc = launch_wide(a, s);
+    if (rc != NO_MAP) return rc;  // (the workspace is enough for either)
+  }
   // rows of a product: 16 where requests have no more on average
   return int64_t(a.R) * (a.Hq / a.Hk) <= int64_t(16) * a.B ? launch<T, D, 1>(a, s) : launch<T, D, 2>(a, s);
 }

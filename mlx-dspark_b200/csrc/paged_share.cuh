@@ -14,6 +14,7 @@ constexpr int MAX_CTA = 320;
 // paged_wide.cu: blocks of many rows.
 size_t wide_workspace(int D);
 int launch_wide(const dspark_paged_attn_args& a, cudaStream_t s);
+constexpr int NO_MAP = -1;  // launch_wide: pages of strides that no tensor map has
 
 // ------------------------------------------------------------------ shares and segments
 

@@ -7,9 +7,10 @@
 //  * items of more than 128 rows: the slots are the two halves of the rows and share each K/V tile;
 //  * items of up to 128 rows: the slots take the even and the odd key tiles and are joined at the segment's end.
 // Either way one slot's softmax runs under the other slot's products.
-//  * Four converting warps read the codes (16-byte cp.async into a ring of their own, page ids read 12 tiles ahead) and write them as fp16, which holds every e4m3 value, into the ring of tiles that the products read:
-//    128 keys x D, 128-byte swizzled, K as it is multiplied (K-major) and V as it lies (N-major). A row is converted once for
-//    up to 256 rows of q; neither scale is multiplied in. Beside a K tile go its 16-key groups' factors.
+//  * One warp asks for the codes' tiles by TMA, a box a page (ids read two windows of four tiles ahead), 128 keys x D. Four
+//    converting warps write them as fp16, which holds every e4m3 value, into the ring that the products read: 128-byte
+//    swizzle, K as it is multiplied (K-major) and V as it lies (N-major). A row is converted once for up to 256 rows of
+//    q; neither scale is multiplied in. Beside a K tile go its 16-key groups' factors.
 //  * Two warps walk ahead and write the next segment's Q as fp16 (bf16 rows scaled by a power of two: exact).
 //  * One thread issues the products: S = Q K^T (both from shared memory), O += P V (P from tensor memory).
 //  * A thread of a softmax warpgroup owns a row: no shuffles. x = f s + log2(vs), f = log2(e) scale 2^e ks, of each group;
@@ -29,32 +30,33 @@ namespace wide {
 constexpr int ROWS = 128;            // rows a slot
 constexpr int RB = 2 * ROWS;         // rows an item
 constexpr int NTHR = 512;            // two softmax warpgroups, one of the products and Q, one that converts
-constexpr int WARP_MMA = 8, WARP_PREP = 10, WARP_CONV = 12;
+constexpr int WARP_MMA = 8, WARP_LOAD = 9, WARP_PREP = 10, WARP_CONV = 12;
 constexpr int SEG = 7;               // cost of a segment, in tiles of up to 128 rows
 constexpr int NB = 3;                // tiles in the ring
-constexpr int PIECE = 32;            // tokens of a tile that one converting warp has
-constexpr int NP = 3;                // pieces in its ring
-constexpr int NSC = 4;               // tiles whose factors are kept: until V of tile t is read, K of t + 4 is not written
+constexpr int NC = 3;                // tiles of codes on their way or waiting to be converted
+constexpr int NSC = 8;               // tiles whose factors are kept: K of tile t + 5 is asked for after V of tile t is read
+                                     // (it is NB + NC loads behind it)
 
 template <int D>
 struct Lay {
   static constexpr int TILE = BN * D * 2;         // a K or V tile (and a slot's Q)
   static constexpr int HALF = BN * 128;           // 64 values of 128 rows, 128-byte swizzled
-  static constexpr int CODES = PIECE * D + 32;    // a piece: its codes, two pages' {ks, vs}, a note
+  static constexpr int CODES = BN * D;            // a K or V tile's codes
   static constexpr int Q = 0;
   static constexpr int RING = 2 * TILE;
   static constexpr int STAGE = RING + NB * TILE;
-  static constexpr int ML = STAGE + 4 * NP * CODES;   // [slot][row] (m, l) at the segment's end
+  static constexpr int ML = STAGE + NC * CODES;       // [slot][row] (m, l) at the segment's end
   static constexpr int RF = ML + 2 * ROWS * 8;        // [segment & 1][slot][row] the rows' powers of two
   static constexpr int SC = RF + 2 * RB * 4;          // [tile & 3][16-key group] (ks, log2 vs)
   static constexpr int FLAG = SC + NSC * 8 * 8;
   static constexpr int SEGS = FLAG + 16;              // two segments for the softmax threads
-  static constexpr int BARS = SEGS + 2 * 64;
-  static constexpr int NBAR = 2 * NB + 2 * 8 + NSC + 1;
+  static constexpr int NOTE = SEGS + 2 * 64;          // what a tile of codes is (Note)
+  static constexpr int BARS = NOTE + NC * 8;
+  static constexpr int NBAR = 2 * NB + 2 * NC + 2 * 8 + NSC + 1;
   static constexpr int MISC = BARS + NBAR * 8;        // tensor memory's address; 17 pairs of find_share
   static constexpr int TOTAL = MISC + 8 + 17 * 8;
   static_assert(TOTAL <= 232448, "shared memory of one SM");
-  static_assert(CODES % 16 == 0 && BARS % 8 == 0, "alignment");
+  static_assert(CODES % 1024 == 0 && BARS % 8 == 0, "alignment");
 };
 
 __device__ __forceinline__ void st_x16(uint32_t taddr, const uint32_t* r) {
@@ -121,6 +123,12 @@ __device__ __forceinline__ bool named_all(int id, int n, bool ok) {
   return r != 0;
 }
 
+// kind: 0 K, 1 V, - segment: V with keys that not every row sees (its NaN codes are taken out), 2: no more tiles; left: rows
+// that are keys.
+struct Note {
+  int kind, left;
+};
+
 // A segment as the walking warps hand it to the softmax threads.
 struct Handed {
   Segment s;
@@ -150,10 +158,6 @@ __device__ __forceinline__ int v_use(bool pair, int t, int n) {
   return pair ? 2 * t + 1 : t == n - 1 ? 2 * n - 1 : 2 * t + 2;
 }
 
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-
 // The NaN codes that were taken out of the segment's V tiles, added to what a row that sees them has stored (`out`: the
 // output, or `part`: the fp32 part).
 template <typename T>
@@ -176,7 +180,9 @@ __device__ __noinline__ void add_hidden(const dspark_paged_attn_args& a, const S
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_args a, const float c_log2,
+__global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ CUtensorMap kmap,
+                                                       const __grid_constant__ CUtensorMap vmap,
+                                                       const dspark_paged_attn_args a, const float c_log2,
                                                        const uint32_t q_sign, int* status) {
   typedef Lay<D> L;
   constexpr uint32_t ID_QK = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(ROWS >> 4) << 24);  // fp16, fp32 sums
@@ -187,7 +193,9 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
   uint8_t* ring = smem + L::RING;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BARS);
   uint64_t* empty = full + NB;
-  uint64_t* q_full = empty + NB;
+  uint64_t* c_full = empty + NB;
+  uint64_t* c_empty = c_full + NC;
+  uint64_t* q_full = c_empty + NC;
   uint64_t* s_full = q_full + 2;
   uint64_t* p_full = s_full + 2;
   uint64_t* p_part = p_full + 2;
@@ -201,6 +209,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
   float* rowf = reinterpret_cast<float*>(smem + L::RF);
   float2* factors = reinterpret_cast<float2*>(smem + L::SC);
   int* flag = reinterpret_cast<int*>(smem + L::FLAG);
+  Note* notes = reinterpret_cast<Note*>(smem + L::NOTE);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   uint2* pairs = reinterpret_cast<uint2*>(smem + L::MISC + 8);
 
@@ -225,9 +234,15 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
       mbar_init(&o_full[i], 1);
     }
     for (int i = 0; i < 4; ++i) flag[i] = 0;
-    for (int i = 0; i < NSC; ++i) mbar_init(&sc_full[i], 4);
+    for (int i = 0; i < NC; ++i) {
+      mbar_init(&c_full[i], 1);
+      mbar_init(&c_empty[i], 4);
+    }
+    for (int i = 0; i < NSC; ++i) mbar_init(&sc_full[i], 1);
     mbar_init(fin, 1);
     fence_mbar_init();
+    prefetch_tmap(&kmap);
+    prefetch_tmap(&vmap);
   }
   if (warp == WARP_MMA) tcg::tmem_alloc(tmem_slot, 512);
   pdl_launch_dependents();
@@ -456,126 +471,49 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
     Segment s{};
     if (warp >= WARP_CONV) {
       // -------------------------------------------------------------- codes to fp16 tiles
-      constexpr int CH = D / 16, RPI = 32 / CH, ROUNDS = PIECE / RPI;  // 16-byte chunks a row, rows a round of copies
-      const int w = warp - WARP_CONV, shift = 31 - __clz(a.page), mask = a.page - 1;
-      uint8_t* stage = smem + L::STAGE + w * NP * L::CODES;
-      const uint32_t stage_a = smem_u32(stage) + lane * 16;
-      const int kts = int(a.kp_strides[2]), vts = int(a.vp_strides[2]);
-      const int64_t k_lane = int64_t(lane / CH) * kts + lane % CH * 16, v_lane = int64_t(lane / CH) * vts + lane % CH * 16;
-      // the copies' cursor: load u of the segment
-      int u = 0, n = 0, tiles0 = 0, seg = 0, to = 0, issued = 0;
-      bool more = true, pair = false;
-      int ids_even = -1, ids_odd = -1;  // pages of 16 tiles' halves of this warp's 32 rows: tile lane >> 1, half lane & 1
-      auto page_ids = [&](int window) {
-        int id = -1;
-        const int t = window * 16 + (lane >> 1), key = (s.t0 + t) * BN + w * 32 + (lane & 1) * 16;
-        if (t < n && key < s.len) {
-          id = a.page_table[int64_t(s.b) * a.table_stride + (key >> shift)];
-          if (id < 0 || id >= a.n_pages) {
-            report_error(status, kErrAttnPage);
-            id = -1;
-          }
-        }
-        return id;
-      };
-      auto issue = [&]() {
-        while (more && u == 2 * n) {  // the next segment
-          tiles0 += n;
-          more = wk.next(plan, deal, s);
-          ++seg;
-          n = more ? s.t1 - s.t0 : 0;
-          pair = is_pair(s);
-          u = 0;
-          if (more && n > 0) {
-            ids_even = page_ids(0);
-            ids_odd = page_ids(1);
-          }
-        }
-        if (more) {
-          bool value;
-          const int t = load_of(pair, u, n, value);
-          if (!value && t >= 16 && (t & 15) == 4) {  // (V is at most two tiles behind K)
-            if ((t >> 4) & 1) ids_even = page_ids((t >> 4) + 1);
-            else ids_odd = page_ids((t >> 4) + 1);
-          }
-          const int ids = (t >> 4) & 1 ? ids_odd : ids_even, key0 = (s.t0 + t) * BN + w * 32;
-          const int id0 = __shfl_sync(0xffffffffu, ids, (t & 15) * 2), id1 = __shfl_sync(0xffffffffu, ids, (t & 15) * 2 + 1);
-          const uint32_t dst = stage_a + to * L::CODES;
-          if (lane < 4) {  // ks, vs of both halves
-            const int id = lane < 2 ? id0 : id1;
-            const int64_t at = id < 0 ? 0 : id * a.scale_strides[0] + s.h * a.scale_strides[1];
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst - lane * 12 + PIECE * D),
-                         "l"((lane & 1 ? a.v_scale : a.k_scale) + at), "r"(id < 0 ? 0 : 4)
-                         : "memory");
-          }
-          if (lane == 4)  // K: 1 + 2 tile; V with keys that not every row sees: - segment
-            *reinterpret_cast<int*>(stage + to * L::CODES + PIECE * D + 16) =
-                !value ? 1 + 2 * (tiles0 + t) : key0 + PIECE > s.before ? -seg : 0;
-          const uint8_t* src = value ? static_cast<const uint8_t*>(a.v_pages) + s.h * a.vp_strides[1] + v_lane
-                                     : static_cast<const uint8_t*>(a.k_pages) + s.h * a.kp_strides[1] + k_lane;
-          const int64_t ps = value ? a.vp_strides[0] : a.kp_strides[0];
-          const int ts = value ? vts : kts;
-          const uint8_t* p0 = src + (id0 * ps + int64_t(key0 & mask) * ts);
-          const uint8_t* p1 = src + (id1 * ps + int64_t((key0 + 16) & mask) * ts);
-          if (id0 >= 0 && id1 >= 0 && key0 + PIECE <= s.len) {
-#pragma unroll
-            for (int z = 0; z < ROUNDS; ++z)
-              cp_async_16(dst + z * 512, (z < ROUNDS / 2 ? p0 : p1) + z % (ROUNDS / 2) * RPI * ts);
-          } else {
-#pragma unroll 1
-            for (int z = 0; z < ROUNDS; ++z) {
-              const bool low = z < ROUNDS / 2, there = (low ? id0 : id1) >= 0 && key0 + z * RPI + lane / CH < s.len;
-              cp_async_16_zfill(dst + z * 512, there ? (low ? p0 : p1) + z % (ROUNDS / 2) * RPI * ts : src, there);
-            }
-          }
-          ++issued;
-          ++u;
-          if (++to == NP) to = 0;
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      };
-#pragma unroll 1
-      for (int i = 0; i < NP - 1; ++i) issue();
-      int from = 0, x = 0, use = 0;
-      for (int done = 0; done < issued; ++done) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(NP - 2) : "memory");
-        __syncwarp();
-        issue();
+      constexpr int CH = D / 16, RPI = 32 / CH, ROUNDS = 32 / RPI;  // 16-byte chunks a row, rows a round, rounds a warp
+      const int w = warp - WARP_CONV, r = lane / CH, c = lane % CH;  // the lane's row of a round, its chunk
+      // the lanes of the upper 64 values store their halves the other way round: no two on one bank
+      const int cc = (c & 3) * 2, first = c >> 2;
+      int st = 0, st_phase = 0, x = 0, use = 0;
+      while (true) {
+        ok = mbar_wait(&c_full[st], uint32_t(st_phase), status, kErrWaitKV);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        const Note note = notes[st];
+        if (note.kind == 2) break;  // no more
         if (use > 0) {
           ok = mbar_wait(&empty[x], uint32_t(use - 1) & 1u, status, kErrWaitKVEmpty);
           if (!__all_sync(0xffffffffu, ok)) break;
         }
-        const uint8_t* codes = stage + from * L::CODES;
-        const float4 sc = *reinterpret_cast<const float4*>(codes + PIECE * D);
-        const int note = *reinterpret_cast<const int*>(codes + PIECE * D + 16);
-        // a page without a positive scale (or none) is not seen
-        const bool fine0 = sc.x > 0.f && sc.y > 0.f, fine1 = sc.z > 0.f && sc.w > 0.f;
-        const int r = lane / CH, c = lane % CH;  // the lane's row of a round, its chunk
-        // the lanes of the upper 64 values store their halves the other way round: no two on one bank
-        uint8_t* base = ring + x * L::TILE + (c >> 2) * L::HALF + (w * 32 + r) * 128;
-        const int cc = (c & 3) * 2, first = c >> 2;
+        const uint8_t* codes = smem + L::STAGE + st * L::CODES;
+        uint8_t* base = ring + x * L::TILE + (c >> 2) * L::HALF;
+        auto get = [&](int z) {
+          const int row = w * 32 + z * RPI + r;
+          const int sw = D == 128 ? row & 7 : (row >> 1) & 3;
+          return *reinterpret_cast<const uint4*>(codes + row * D + ((c ^ sw) << 4));
+        };
         auto put = [&](int z, uint4 v) {
           const uint4 h0 = make_uint4(e4m3_to_f16(v.x), e4m3_to_f16_hi(v.x), e4m3_to_f16(v.y), e4m3_to_f16_hi(v.y));
           const uint4 h1 = make_uint4(e4m3_to_f16(v.z), e4m3_to_f16_hi(v.z), e4m3_to_f16(v.w), e4m3_to_f16_hi(v.w));
-          const int sw = (r + z * RPI) & 7;  // (w * 32 is a multiple of 8)
-          *reinterpret_cast<uint4*>(base + z * RPI * 128 + (((cc + first) ^ sw) << 4)) = first ? h1 : h0;
-          *reinterpret_cast<uint4*>(base + z * RPI * 128 + (((cc + (first ^ 1)) ^ sw) << 4)) = first ? h0 : h1;
+          const int row = w * 32 + z * RPI + r, sw = row & 7;
+          *reinterpret_cast<uint4*>(base + row * 128 + (((cc + first) ^ sw) << 4)) = first ? h1 : h0;
+          *reinterpret_cast<uint4*>(base + row * 128 + (((cc + (first ^ 1)) ^ sw) << 4)) = first ? h0 : h1;
         };
-        if (note >= 0 && fine0 && fine1) {
+        if (note.kind >= 0 && note.left >= BN) {
 #pragma unroll
           for (int z0 = 0; z0 < ROUNDS; z0 += 4) {  // four in flight
             uint4 v[4];
 #pragma unroll
-            for (int z = 0; z < 4; ++z) v[z] = *reinterpret_cast<const uint4*>(codes + ((z0 + z) * 32 + lane) * 16);
+            for (int z = 0; z < 4; ++z) v[z] = get(z0 + z);
 #pragma unroll
             for (int z = 0; z < 4; ++z) put(z0 + z, v[z]);
           }
         } else {
 #pragma unroll 1
           for (int z = 0; z < ROUNDS; ++z) {
-            uint4 v = *reinterpret_cast<const uint4*>(codes + (z * 32 + lane) * 16);
-            if (!(z < ROUNDS / 2 ? fine0 : fine1)) v = make_uint4(0u, 0u, 0u, 0u);
-            if (note < 0) {
+            uint4 v = get(z);
+            if (w * 32 + z * RPI + r >= note.left) v = make_uint4(0u, 0u, 0u, 0u);  // no key: whatever the page holds there
+            if (note.kind < 0) {
               uint32_t* y = &v.x;
               uint32_t any = 0;
 #pragma unroll
@@ -584,28 +522,108 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
                 any |= nan;
                 y[k] &= ~(nan * 0xffu);
               }
-              if (any) *reinterpret_cast<volatile int*>(&flag[(-note) & 3]) = -note;
+              if (any) *reinterpret_cast<volatile int*>(&flag[(-note.kind) & 3]) = -note.kind;
             }
             put(z, v);
           }
         }
-        if (note > 0 && lane < 2)
-          factors[((note >> 1) % NSC) * 8 + w * 2 + lane] =
-              lane ? (fine1 ? make_float2(sc.z, lg2(sc.w)) : make_float2(1.f, -INFINITY))
-                   : (fine0 ? make_float2(sc.x, lg2(sc.y)) : make_float2(1.f, -INFINITY));
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
+          mbar_arrive(&c_empty[st]);
           mbar_arrive(&full[x]);
-          if (note > 0) mbar_arrive(&sc_full[(note >> 1) % NSC]);
         }
-        if (++from == NP) from = 0;
+        if (++st == NC) {
+          st = 0;
+          st_phase ^= 1;
+        }
         if (++x == NB) {
           x = 0;
           ++use;
         }
       }
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
+    } else if (warp == WARP_LOAD) {
+      // -------------------------------------------------------------- codes, by TMA from the pages
+      // A lane has one 16-key group of four tiles (a window): page ids are read two windows ahead, scales one.
+      const int shift = 31 - __clz(a.page), boxes = BN >> shift;
+      int load = 0, tiles0 = 0, seg = 0;
+      auto wait_free = [&]() {  // the next stage
+        const int st = load % NC;
+        if (load >= NC && ok) ok = mbar_wait(&c_empty[st], uint32_t(load / NC - 1) & 1u, status, kErrWaitKVEmpty);
+        ok = __all_sync(0xffffffffu, ok);
+        return st;
+      };
+      while (ok && wk.next(plan, deal, s)) {
+        ++seg;
+        const int n = s.t1 - s.t0;
+        const bool pair = is_pair(s);
+        const int32_t* table = a.page_table + int64_t(s.b) * a.table_stride;
+        auto page_ids = [&](int window) {
+          int id = -1;
+          const int t = window * 4 + (lane >> 3), key = (s.t0 + t) * BN + (lane & 7) * 16;
+          if (t < n && key < s.len) {
+            id = table[key >> shift];
+            if (id < 0 || id >= a.n_pages) {
+              report_error(status, kErrAttnPage);
+              id = -1;
+            }
+          }
+          return id;
+        };
+        auto scales = [&](int id) {
+          float2 y = make_float2(0.f, 0.f);
+          if (id >= 0) {
+            const int64_t at = id * a.scale_strides[0] + s.h * a.scale_strides[1];
+            y = make_float2(a.k_scale[at], a.v_scale[at]);
+          }
+          return y;
+        };
+        // ids: of the window in work (-1: not seen), `before` of the one before (V is up to two tiles behind K)
+        int window = -1, ids = -1, before = -1, ids1 = n > 0 ? page_ids(0) : -1, ids2 = n > 0 ? page_ids(1) : -1;
+        float2 sc = make_float2(0.f, 0.f), sc1 = scales(ids1);
+        for (int u = 0; u < 2 * n && ok; ++u) {
+          bool value;
+          const int t = load_of(pair, u, n, value);
+          if (!value && (t >> 2) != window) {
+            window = t >> 2;
+            before = ids;
+            sc = sc1;
+            ids = sc.x > 0.f && sc.y > 0.f ? ids1 : -1;  // a page without a positive scale is not seen
+            ids1 = ids2;
+            sc1 = scales(ids1);
+            ids2 = page_ids(window + 2);
+          }
+          const int st = wait_free();
+          if (!ok) break;
+          // lane i: the page of the tile's i-th box
+          const int id = __shfl_sync(0xffffffffu, (t >> 2) != window ? before : ids, (t & 3) * 8 + ((lane << (shift - 4)) & 7));
+          const int key0 = (s.t0 + t) * BN;
+          if (!value && (lane >> 3) == (t & 3))
+            factors[((tiles0 + t) % NSC) * 8 + (lane & 7)] = ids >= 0 ? make_float2(sc.x, lg2(sc.y)) : make_float2(1.f, -INFINITY);
+          if (lane == 0) {
+            notes[st] = Note{!value ? 0 : key0 + BN > s.before ? -seg : 1, s.len - key0};
+            mbar_arrive_expect_tx(&c_full[st], L::CODES);
+          }
+          __syncwarp();
+          if (lane == 0 && !value) mbar_arrive(&sc_full[(tiles0 + t) % NSC]);
+          if (lane < boxes)  // a page that is not seen: past the last one, where the copy writes zeros
+            tma_load_4d(smem + L::STAGE + st * L::CODES + lane * a.page * D, value ? &vmap : &kmap, &c_full[st], 0, 0, s.h,
+                        id < 0 ? a.n_pages : id);
+          ++load;
+        }
+        tiles0 += n;
+      }
+      // no copy may still be in flight when the block exits (under the default limit, whatever is set); before the
+      // end is told, which is one more phase of its stage
+      if (lane == 0)
+        for (int i = max(0, load - NC); i < load; ++i) mbar_wait(&c_full[i % NC], uint32_t(i / NC) & 1u, nullptr, 0);
+      __syncwarp();
+      const int end = wait_free();
+      if (ok && lane == 0) {
+        notes[end] = Note{2, 0};
+        mbar_arrive(&c_full[end]);
+      }
       __syncwarp();
     } else if (warp >= WARP_PREP) {
       // -------------------------------------------------------------- segments and Q, ahead
@@ -616,48 +634,56 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
       auto load_q = [&](int slot, int hand) {
         if (n_q[slot] > 0 && ok) ok = mbar_wait(&q_empty[slot], (n_q[slot] - 1) & 1u, status, kErrWaitMma);
         ++n_q[slot];
-        const int row0 = s.row_base + (is_pair(s) ? slot * ROWS : 0);
+        const int row0 = s.row_base + slot * ROWS;
         const int live = min(ROWS, s.rows * G - row0);  // rows past it are never looked at
         const T* q = static_cast<const T*>(a.q) + int64_t(s.r0) * a.q_strides[0] + s.h * G * a.q_strides[1] + c * 8;
         uint8_t* dst = smem + L::Q + slot * L::TILE + (c >> 3) * L::HALF;
-        float* rf = rowf + hand * RB + (is_pair(s) ? slot * ROWS : 0);
-        constexpr int FLY = 4;
-        for (int r0 = 0; r0 < live; r0 += FLY * STEP) {
-          uint4 v[FLY];
-#pragma unroll
-          for (int z = 0; z < FLY; ++z) {
-            const int r = r0 + z * STEP + first_row, node = (row0 + r) / G, g = row0 + r - node * G;
-            v[z] = r < live ? ldcg_v4(q + node * a.q_strides[0] + g * a.q_strides[1]) : make_uint4(0u, 0u, 0u, 0u);
+        float* rf = rowf + hand * RB + slot * ROWS;
+        // all rows on their way at once, to where they stay; then every thread makes what it copied fp16
+        const int dn = STEP / G, dg = STEP - dn * G;  // a step in (node, head of the group)
+        int node = (row0 + first_row) / G, g = row0 + first_row - node * G;
+        for (int r = first_row; r < live; r += STEP) {
+          cp_async_16_zfill(smem_u32(dst) + uint32_t(r * 128 + (((c & 7) ^ (r & 7)) << 4)),
+                            q + node * a.q_strides[0] + g * a.q_strides[1], true);
+          node += dn;
+          g += dg;
+          if (g >= G) {
+            g -= G;
+            ++node;
           }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();
+#pragma unroll 4
+        for (int r0 = 0; r0 < live; r0 += STEP) {
+          const int r = r0 + first_row;
+          uint4* at = reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+          uint4 v = r < live ? *at : make_uint4(0u, 0u, 0u, 0u);
+          uint32_t* y = &v.x;
+          float f = 1.f;
+          if (std::is_same<T, bf16>::value) {  // largest exponent of the row; 255: infinite or NaN
+            uint32_t e = 0;
 #pragma unroll
-          for (int z = 0; z < FLY; ++z) {
-            const int r = r0 + z * STEP + first_row;
-            uint32_t* y = &v[z].x;
-            float f = 1.f;
-            if (std::is_same<T, bf16>::value) {  // largest exponent of the row; 255: infinite or NaN
-              uint32_t e = 0;
+            for (int i = 0; i < 4; ++i) e = max(e, max((y[i] >> 7) & 0xffu, (y[i] >> 23) & 0xffu));
 #pragma unroll
-              for (int i = 0; i < 4; ++i) e = max(e, max((y[i] >> 7) & 0xffu, (y[i] >> 23) & 0xffu));
+            for (int o = 1; o < CH; o <<= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, o));
+            const int up = int(e) - 141;  // values below 2^15
+            const float inv = pow2(max(min(-up, 126), -126));
+            f = e == 255 ? NAN : pow2(max(min(up, 126), -126));
 #pragma unroll
-              for (int o = 1; o < CH; o <<= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, o));
-              const int up = int(e) - 141;  // values below 2^15
-              const float inv = pow2(max(min(-up, 126), -126));
-              f = e == 255 ? NAN : pow2(max(min(up, 126), -126));
+            for (int i = 0; i < 4; ++i) y[i] = Elem<__half>::pack(bf16_lo(y[i]) * inv, bf16_hi(y[i]) * inv);
+          } else {  // an infinite q makes its row NaN whatever the codes are
+            uint32_t bad = 0;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) y[i] = Elem<__half>::pack(bf16_lo(y[i]) * inv, bf16_hi(y[i]) * inv);
-            } else {  // an infinite q makes its row NaN whatever the codes are
-              uint32_t bad = 0;
+            for (int i = 0; i < 4; ++i) bad |= (y[i] & 0x7c00u) == 0x7c00u || (y[i] & 0x7c000000u) == 0x7c000000u;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) bad |= (y[i] & 0x7c00u) == 0x7c00u || (y[i] & 0x7c000000u) == 0x7c000000u;
-#pragma unroll
-              for (int o = 1; o < CH; o <<= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, o);
-              f = bad ? NAN : 1.f;
-            }
-            if (r < live) {
-              if (c == 0) rf[r] = f * c_log2;
-              *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
-                  make_uint4(y[0] ^ q_sign, y[1] ^ q_sign, y[2] ^ q_sign, y[3] ^ q_sign);
-            }
+            for (int o = 1; o < CH; o <<= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+            f = bad ? NAN : 1.f;
+          }
+          if (r < live) {
+            if (c == 0) rf[r] = f * c_log2;
+            *at = make_uint4(y[0] ^ q_sign, y[1] ^ q_sign, y[2] ^ q_sign, y[3] ^ q_sign);
           }
         }
         fence_proxy_async_smem();
@@ -671,7 +697,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
         if (k >= 2 && ok) ok = mbar_wait(&seg_empty[hand], uint32_t((k >> 1) - 1) & 1u, status, kErrWaitPeer);
         if (more && s.t0 < s.t1) {
           load_q(0, hand);
-          if (is_pair(s) || s.t1 - s.t0 > 1) load_q(1, hand);  // (the same rows for both where there are up to 128)
+          if (is_pair(s)) load_q(1, hand);
         }
         // handed over when the rows' factors are written: both warps'
         named_sync(5, 64);
@@ -709,9 +735,9 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
       auto commit = [&](uint64_t* bar) {
         if (leader) tcg::umma_commit(bar);
       };
-      auto scores = [&](int slot, int x, bool last) {
+      auto scores = [&](int slot, int qt, int x, bool last) {  // qt: the tile of Q
         if (!ok) return;
-        const uint32_t qd = q_lo + uint32_t(slot) * (L::TILE >> 4);
+        const uint32_t qd = q_lo + uint32_t(qt) * (L::TILE >> 4);
         const uint32_t kd = desc_lo(ring_a + uint32_t(x) * L::TILE, 16);
         if (leader) {
 #pragma unroll
@@ -720,7 +746,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
             umma_ss(tmem + uint32_t(slot * 128), desc_sw128(qd + off), desc_sw128(kd + off), ID_QK, k ? 1u : 0u);
           }
           tcg::umma_commit(&s_full[slot]);
-          if (last) tcg::umma_commit(&q_empty[slot]);  // the segment's last use of this Q
+          if (last) tcg::umma_commit(&q_empty[qt]);  // the segment's last use of this Q
         }
         issued = true;
       };
@@ -759,9 +785,9 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
         if (pair) {
           int x = take();
           q_ready(0);
-          scores(0, x, n == 1);
+          scores(0, 0, x, n == 1);
           q_ready(1);
-          scores(1, x, n == 1);
+          scores(1, 1, x, n == 1);
           release(x);
           for (int t = 0; t < n; ++t) {
             const int v = take();
@@ -769,14 +795,14 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
             values(0, v, t == 0);
             if (more) {
               x = take();
-              scores(0, x, t + 2 == n);
+              scores(0, 0, x, t + 2 == n);
             } else if (ok) {
               commit(&o_full[0]);
             }
             values(1, v, t == 0);
             release(v);
             if (more) {
-              scores(1, x, t + 2 == n);
+              scores(1, 1, x, t + 2 == n);
               release(x);
             } else if (ok) {
               commit(&o_full[1]);
@@ -786,8 +812,8 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
         } else {
           for (int z = 0; z < min(n, 2); ++z) {
             const int x = take();
-            q_ready(z);
-            scores(z, x, z + 2 >= n);
+            if (z == 0) q_ready(0);
+            scores(z, 0, x, z + 1 == n);
             release(x);
           }
           for (int t = 0; t < n; ++t) {
@@ -796,7 +822,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const dspark_paged_attn_a
             release(v);
             if (t + 2 < n) {
               const int x = take();
-              scores(z, x, t + 4 >= n);
+              scores(z, 0, x, t + 3 == n);
               release(x);
             } else if (ok) {
               commit(&o_full[z]);
@@ -822,6 +848,17 @@ template <typename T, int D>
 static int launch(const dspark_paged_attn_args& a, cudaStream_t s) {
   constexpr int TOTAL = Lay<D>::TOTAL;
   const int dev = current_device(), n = std::min(sm_count(dev), MAX_CTA);
+  CUtensorMap maps[2];
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* st = i ? a.vp_strides : a.kp_strides;
+    // (a dimension of one entry is never stepped: any valid stride does)
+    const uint64_t dims[4] = {uint64_t(D), uint64_t(a.page), uint64_t(a.Hk), uint64_t(a.n_pages)};
+    const uint64_t strides[3] = {uint64_t(st[2]), uint64_t(a.Hk > 1 ? st[1] : D), uint64_t(a.n_pages > 1 ? st[0] : D)};
+    const uint32_t box[4] = {uint32_t(D), uint32_t(a.page), 1, 1};
+    if (!encode_tmap_nd(&maps[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, i ? a.v_pages : a.k_pages, dims, strides, box,
+                        D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
+      return NO_MAP;
+  }
   DSPARK_CUDA_TRY(configure_once((const void*)attn_kernel<T, D>, TOTAL,
                                  [&] {
                                    return cudaFuncSetAttribute(attn_kernel<T, D>,
@@ -829,7 +866,7 @@ static int launch(const dspark_paged_attn_args& a, cudaStream_t s) {
                                  }),
                   "paged_attn: shared memory");
   const float c = a.scale == 0.f ? 1e-30f : fabsf(a.scale) * 1.4426950408889634f;
-  DSPARK_CUDA_TRY(launch_ex(attn_kernel<T, D>, dim3(n), dim3(NTHR), TOTAL, s, 1, true, a, c,
+  DSPARK_CUDA_TRY(launch_ex(attn_kernel<T, D>, dim3(n), dim3(NTHR), TOTAL, s, 1, true, maps[0], maps[1], a, c,
                             a.scale < 0.f ? 0x80008000u : 0u, status_word(dev)),
                   "paged_attn");
   DSPARK_CUDA_TRY(launch_ex(join_kernel<T, D, RB>, dim3(n, RB / 4), dim3(128), 0, s, 1, true, a), "paged_attn: join");
