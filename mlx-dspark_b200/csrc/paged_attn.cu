@@ -30,7 +30,6 @@ namespace paged {
 constexpr int SUB = 32;      // keys a warp's subtile
 constexpr int WARPS = 4;
 constexpr int NTHR = WARPS * 32;
-constexpr int WIDE_ROWS = 128;
 constexpr int SEG = 5;       // cost of a segment, in tiles
 constexpr float LIFT = 11.f; // weights are 2^11 times as large in fp16 ...
 constexpr float SLACK = 4.f; // ... and the maximum in use may be 2^4 too low
@@ -500,12 +499,21 @@ static int launch(const dspark_paged_attn_args& a, cudaStream_t s) {
   return DSPARK_OK;
 }
 
-// Rows of a request and kv head, on average: more than 128 go to the 5th-generation tensor cores.
-static bool is_wide(int R, int B, int Hq, int Hk) { return int64_t(R) * (Hq / Hk) > int64_t(WIDE_ROWS) * B; }
+// Which calls go to the 5th-generation tensor cores (paged_wide.cu): those with more than 32 rows a request and kv head on
+// average and with work enough, in tiles of 32 rows by 128 keys (the table's width stands for the lengths, which are
+// on the device). Measured, this kernel / the other, us, 32/8 heads of 128: 16 rows over 4k keys, 1 request (2048 of
+// such tiles with their 64 rows a head) 21 / 30, 4 requests 36 / 39, 16 requests (8192) 90 / 77; 32 rows over 16k, 1
+// request (4096) 49 / 43; 64 requests of 64 rows over 4k 1105 / 420.
+constexpr int FEW_ROWS = 32, WIDE_TILES = 3000;
+static bool has_many_rows(int R, int B, int Hq, int Hk) { return int64_t(R) * (Hq / Hk) > int64_t(FEW_ROWS) * B; }
+static bool is_wide(const dspark_paged_attn_args& a) {
+  const int64_t blocks = (int64_t(a.R) * (a.Hq / a.Hk) + FEW_ROWS - 1) / FEW_ROWS * a.Hk;
+  return has_many_rows(a.R, a.B, a.Hq, a.Hk) && blocks * (int64_t(a.max_pages) * a.page / BN + 1) > WIDE_TILES && a.n_pages > 0;
+}
 
 template <typename T, int D>
 static int launch_rows(const dspark_paged_attn_args& a, cudaStream_t s) {
-  if (is_wide(a.R, a.B, a.Hq, a.Hk) && a.n_pages > 0) {
+  if (is_wide(a)) {
     const int rc = launch_wide(a, s);
     if (rc != NO_MAP) return rc;  // (the workspace is enough for either)
   }
@@ -522,7 +530,7 @@ extern "C" {
 
 size_t dspark_paged_attn_workspace(int R, int B, int Hq, int Hk, int D) {
   if (R <= 0 || B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || D <= 0) return 0;
-  if (paged::is_wide(R, B, Hq, Hk)) return paged::wide_workspace(D);
+  if (paged::has_many_rows(R, B, Hq, Hk)) return paged::wide_workspace(D);
   return paged::MAX_CTA * sizeof(paged::Cut) +
          size_t(paged::grid_of(current_device(), 2)) * 2 * 32 * (D + 1) * sizeof(float);  // (also enough for 3 of 16 rows)
 }

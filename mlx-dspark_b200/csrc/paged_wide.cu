@@ -47,8 +47,8 @@ struct Lay {
   static constexpr int STAGE = RING + NB * TILE;
   static constexpr int ML = STAGE + NC * CODES;       // [slot][row] (m, l) at the segment's end
   static constexpr int RF = ML + 2 * ROWS * 8;        // [segment & 1][slot][row] the rows' powers of two
-  static constexpr int SC = RF + 2 * RB * 4;          // [tile & 3][16-key group] (ks, log2 vs)
-  static constexpr int FLAG = SC + NSC * 8 * 8;
+  static constexpr int SC = RF + 2 * RB * 4;          // [tile % NSC][16-key group] (ks, log2 vs, 1 / vs)
+  static constexpr int FLAG = SC + NSC * 8 * 16;
   static constexpr int SEGS = FLAG + 16;              // two segments for the softmax threads
   static constexpr int NOTE = SEGS + 2 * 64;          // what a tile of codes is (Note)
   static constexpr int BARS = NOTE + NC * 8;
@@ -158,6 +158,12 @@ __device__ __forceinline__ int v_use(bool pair, int t, int n) {
   return pair ? 2 * t + 1 : t == n - 1 ? 2 * n - 1 : 2 * t + 2;
 }
 
+// A group's factor, 1e-35 at least: -inf stays that (and NaN too).
+__device__ __forceinline__ float factor_of(float rf, float ks) {
+  const float f = rf * ks;
+  return f < 1e-35f ? 1e-35f : f;
+}
+
 // The NaN codes that were taken out of the segment's V tiles, added to what a row that sees them has stored (`out`: the
 // output, or `part`: the fp32 part).
 template <typename T>
@@ -207,7 +213,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
   uint64_t* fin = sc_full + NSC;
   float2* ml = reinterpret_cast<float2*>(smem + L::ML);
   float* rowf = reinterpret_cast<float*>(smem + L::RF);
-  float2* factors = reinterpret_cast<float2*>(smem + L::SC);
+  float4* factors = reinterpret_cast<float4*>(smem + L::SC);
   int* flag = reinterpret_cast<int*>(smem + L::FLAG);
   Note* notes = reinterpret_cast<Note*>(smem + L::NOTE);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
@@ -312,35 +318,22 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
           float x[128];
 #pragma unroll
           for (int i = 0; i < 4; ++i) ld_x32(t_s + uint32_t(32 * i), x + 32 * i);
-          const float2* fa = factors + (tile % NSC) * 8;
+          const float4* fa = factors + (tile % NSC) * 8;
           tcg::tmem_wait_ld();
-#pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            const float2 y = fa[g];
-            const float f = rf * y.x;
-            const f32x2 f2 = pack2(f, f), l2 = pack2(y.y, y.y);
-#pragma unroll
-            for (int i = 16 * g; i < 16 * g + 16; i += 2) {
-              const f32x2 z = fma2(pack2(x[i], x[i + 1]), f2, l2);
-              unpack2(z, x[i], x[i + 1]);
-            }
-          }
           if (edge) {
             const int left = lim - k0;
 #pragma unroll
             for (int i = 0; i < 128; ++i) x[i] = i < left ? x[i] : -INFINITY;
           }
-          float mx[8];
+          // (the factors are positive: a group's largest score is that of its largest product)
+          float mt = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) mx[e] = max3(x[2 * e], x[2 * e + 1], x[16 + e]);
-#pragma unroll
-          for (int i = 24; i < 120; i += 16) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mx[e] = max3(mx[e], x[i + 2 * e], x[i + 2 * e + 1]);
+          for (int g = 0; g < 8; ++g) {
+            const float* y = x + 16 * g;
+            const float mg = max3(max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], y[5]), max3(y[6], y[7], y[8])),
+                                  max3(y[9], y[10], y[11]), max3(max3(y[12], y[13], y[14]), y[15], y[15]));
+            mt = max3(mt, fmaf(mg, factor_of(rf, fa[g].x), fa[g].y), mt);
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[120 + 2 * e], x[120 + 2 * e + 1]);
-          const float mt = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max3(mx[6], mx[7], mx[7]));
           if (!(mt < INFINITY)) m = NAN;  // a visible score of +inf or NaN: the row is NaN
           const bool up = mt - m > SLACK;
           if (__any_sync(0xffffffffu, up)) {
@@ -361,30 +354,37 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
             }
           }
           const float ref = LIFT - (m == -INFINITY ? 0.f : m);
-          const f32x2 r2 = pack2(ref, ref);
+          // pair by pair, sums and packing LAG pairs behind the exponentials: the special-function unit (8 clocks a warp
+          // instruction) then never waits for them
+          constexpr int LAG = 4;
+          f32x2 e[64], sum = pack2(0.f, 0.f), f2 = sum, l2 = sum;
+          uint32_t p[64];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {  // 32 columns: two groups
-            uint32_t p[16];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float lv = fa[2 * q + h].y, iv = lv == -INFINITY ? 0.f : ex2(-lv);
-              f32x2 sum = pack2(0.f, 0.f);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int z = 32 * q + 16 * h + 2 * i;
-                float e0, e1;
-                unpack2(add2(pack2(x[z], x[z + 1]), r2), e0, e1);
-                const f32x2 e = pack2(ex2(e0), ex2(e1));
-                unpack2(e, e0, e1);
-                sum = add2(sum, e);
-                p[8 * h + i] = Elem<__half>::pack(e0, e1);
+          for (int i = 0; i < 64 + LAG; ++i) {
+            if (i < 64) {
+              if ((i & 7) == 0) {
+                const float4 y = fa[i >> 3];
+                const float f = factor_of(rf, y.x), lv = y.y + ref;
+                f2 = pack2(f, f);
+                l2 = pack2(lv, lv);
               }
-              float s0, s1;
-              unpack2(sum, s0, s1);
-              l = fmaf(s0 + s1, iv, l);
+              float e0, e1;
+              unpack2(fma2(pack2(x[2 * i], x[2 * i + 1]), f2, l2), e0, e1);
+              e[i] = pack2(ex2(e0), ex2(e1));
             }
-            st_x16(t_s + uint32_t(16 * q), p);
-            if (q == 2) arrive(&p_part[slot]);  // three quarters' products may start
+            const int z = i - LAG;
+            if (z >= 0) {
+              float e0, e1;
+              unpack2(e[z], e0, e1);
+              sum = (z & 7) == 0 ? e[z] : add2(sum, e[z]);
+              p[z] = Elem<__half>::pack(e0, e1);
+              if ((z & 7) == 7) {
+                unpack2(sum, e0, e1);
+                l = fmaf(e0 + e1, fa[z >> 3].z, l);
+              }
+              if ((z & 15) == 15) st_x16(t_s + uint32_t(z - 15), p + z - 15);
+              if (z == 47) arrive(&p_part[slot]);  // three quarters' products may start
+            }
           }
         } else {
           arrive(&p_part[slot]);
@@ -600,7 +600,8 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
           const int id = __shfl_sync(0xffffffffu, (t >> 2) != window ? before : ids, (t & 3) * 8 + ((lane << (shift - 4)) & 7));
           const int key0 = (s.t0 + t) * BN;
           if (!value && (lane >> 3) == (t & 3))
-            factors[((tiles0 + t) % NSC) * 8 + (lane & 7)] = ids >= 0 ? make_float2(sc.x, lg2(sc.y)) : make_float2(1.f, -INFINITY);
+            factors[((tiles0 + t) % NSC) * 8 + (lane & 7)] =
+                ids >= 0 ? make_float4(sc.x, lg2(sc.y), 1.f / sc.y, 0.f) : make_float4(1.f, -INFINITY, 0.f, 0.f);
           if (lane == 0) {
             notes[st] = Note{!value ? 0 : key0 + BN > s.before ? -seg : 1, s.len - key0};
             mbar_arrive_expect_tx(&c_full[st], L::CODES);
