@@ -11,9 +11,9 @@
 //    converting warps write them as fp16, which holds every e4m3 value, into the ring that the products read: 128-byte
 //    swizzle, K as it is multiplied (K-major) and V as it lies (N-major). A row is converted once for up to 256 rows of
 //    q; neither scale is multiplied in. Beside a K tile go its 16-key groups' factors.
-//  * Two warps walk ahead and write the next segment's Q as fp16 (bf16 rows scaled by a power of two: exact).
 //  * One thread issues the products: S = Q K^T (both from shared memory), O += P V (P from tensor memory).
-//  * A thread of a softmax warpgroup owns a row: no shuffles. x = f s + log2(vs), f = log2(e) scale 2^e ks, of each group;
+//  * A thread of a softmax warpgroup owns a row: no shuffles. It writes the row's q as fp16 (bf16: scaled by a power of two,
+//    exact). x = f s + log2(vs), f = log2(e) scale 2^e ks, of each group;
 //    the maximum in use is only raised when a tile exceeds it by more than 2^8; weights are 2^7 times as large.
 //
 // Rounding: weights are rounded to fp16 for the product with V (their sum is not); scores, maxima, sums and O are fp32.
@@ -46,13 +46,13 @@ struct Lay {
   static constexpr int RING = 2 * TILE;
   static constexpr int STAGE = RING + NB * TILE;
   static constexpr int ML = STAGE + NC * CODES;       // [slot][row] (m, l) at the segment's end
-  static constexpr int RF = ML + 2 * ROWS * 8;        // [segment & 1][slot][row] the rows' powers of two
-  static constexpr int SC = RF + 2 * RB * 4;          // [tile % NSC][16-key group] (ks, log2 vs, 1 / vs)
+  static constexpr int RF = ML + 2 * ROWS * 8;        // [row] the rows' powers of two, for the other slot
+  static constexpr int SC = RF + ROWS * 4;          // [tile % NSC][16-key group] (ks, log2 vs, 1 / vs)
   static constexpr int FLAG = SC + NSC * 8 * 16;
   static constexpr int SEGS = FLAG + 16;              // two segments for the softmax threads
   static constexpr int NOTE = SEGS + 2 * 64;          // what a tile of codes is (Note)
   static constexpr int BARS = NOTE + NC * 8;
-  static constexpr int NBAR = 2 * NB + 2 * NC + 2 * 8 + NSC + 1;
+  static constexpr int NBAR = 2 * NB + 2 * NC + 2 * 7 + NSC + 1;
   static constexpr int MISC = BARS + NBAR * 8;        // tensor memory's address; 17 pairs of find_share
   static constexpr int TOTAL = MISC + 8 + 17 * 8;
   static_assert(TOTAL <= 232448, "shared memory of one SM");
@@ -129,7 +129,7 @@ struct Note {
   int kind, left;
 };
 
-// A segment as the walking warps hand it to the softmax threads.
+// A segment as the walking warp hands it to the softmax threads.
 struct Handed {
   Segment s;
   int more;
@@ -179,7 +179,7 @@ __device__ __noinline__ void add_hidden(const dspark_paged_attn_args& a, const S
                        (k % a.page) * a.vp_strides[2];
     for (int d = d0; d < d1; ++d) {
       if ((v[d] & 0x7f) != 0x7f) continue;
-      if (part) part[d] = NAN;
+      if (part) part[d * RB] = NAN;
       else out[d] = Elem<T>::from_f(NAN);
     }
   }
@@ -206,8 +206,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
   uint64_t* p_full = s_full + 2;
   uint64_t* p_part = p_full + 2;
   uint64_t* o_full = p_part + 2;
-  uint64_t* q_empty = o_full + 2;
-  uint64_t* seg_full = q_empty + 2;
+  uint64_t* seg_full = o_full + 2;
   uint64_t* seg_empty = seg_full + 2;
   uint64_t* sc_full = seg_empty + 2;
   uint64_t* fin = sc_full + NSC;
@@ -230,8 +229,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {  // p_*, q_full and seg_empty count warps
-      mbar_init(&q_full[i], 2);
-      mbar_init(&q_empty[i], 1);
+      mbar_init(&q_full[i], 4);
       mbar_init(&seg_full[i], 1);
       mbar_init(&seg_empty[i], 8);
       mbar_init(&s_full[i], 1);
@@ -298,7 +296,52 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
       const int place = alive ? my / G : 0;
       const int lim = a.causal ? min(s.len, s.before + place + 1) : s.len;  // keys that the row sees
       const int edge0 = (a.causal ? min(s.len, s.before + s.row_base / G + 1) : s.len) - BN;  // later: hidden keys
-      const float rf = rowf[hand * RB + (pair ? slot * ROWS : 0) + row];
+      // ---- Q as fp16, a row a thread (the first slot's for both where there are up to 128). The products that read the
+      // last segment's are done: their O has been waited for.
+      float rf = 1.f;
+      if (n > 0 && (pair || slot == 0)) {
+        if (alive) {
+          const T* q = static_cast<const T*>(a.q) + int64_t(s.r0 + place) * a.q_strides[0] +
+                       (s.h * G + my - place * G) * a.q_strides[1];
+          uint4 v[D / 8];
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) v[c] = ldcg_v4(q + 8 * c);
+          constexpr uint32_t SHIFT = std::is_same<T, bf16>::value ? 7 : 10, ONES = std::is_same<T, bf16>::value ? 0xff : 0x1f;
+          uint32_t e = 0;  // the largest exponent; all ones: infinite or NaN, and the row is NaN whatever the codes are
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            const uint32_t* y = &v[c].x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e = max(e, max((y[i] >> SHIFT) & ONES, (y[i] >> (SHIFT + 16)) & ONES));
+          }
+          float inv = 1.f;
+          if (std::is_same<T, bf16>::value) {
+            const int up = int(e) - 141;  // values below 2^15
+            inv = pow2(max(min(-up, 126), -126));
+            rf = pow2(max(min(up, 126), -126));
+          }
+          rf = e == ONES ? NAN : rf * c_log2;
+          uint8_t* dst = smem + L::Q + slot * L::TILE + row * 128;
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            uint32_t* y = &v[c].x;
+            if (std::is_same<T, bf16>::value) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) y[i] = Elem<__half>::pack(bf16_lo(y[i]) * inv, bf16_hi(y[i]) * inv);
+            }
+            *reinterpret_cast<uint4*>(dst + (c >> 3) * L::HALF + (((c & 7) ^ (row & 7)) << 4)) =
+                make_uint4(y[0] ^ q_sign, y[1] ^ q_sign, y[2] ^ q_sign, y[3] ^ q_sign);
+          }
+        }
+        if (!pair) rowf[row] = rf;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[slot]);
+      }
+      if (!pair) {
+        named_sync(3, 256);
+        rf = rowf[row];
+      }
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < steps; ++j) {
         const int t = pair ? j : 2 * j + slot, k0 = (s.t0 + t) * BN, tile = tiles0 + t;
@@ -442,10 +485,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
             }
             if (alive && !whole) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 4)
-                *reinterpret_cast<float4*>(pp + prow * D + 32 * i + e) =
-                    l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                             : make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+              for (int e = 0; e < 32; ++e) pp[(32 * i + e) * RB + prow] = l == 0.f ? 0.f : o[e] * inv;
             } else if (alive) {
 #pragma unroll
               for (int e = 0; e < 32; e += 8) {
@@ -458,7 +498,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
               }
             }
           }
-          if (hidden && alive) add_hidden<T>(a, s, lim, 32 * i0, 32 * i1, out, whole ? nullptr : pp + prow * D);
+          if (hidden && alive) add_hidden<T>(a, s, lim, 32 * i0, 32 * i1, out, whole ? nullptr : pp + prow);
         }
       }
       tcg::tc_fence_before();
@@ -626,83 +666,14 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
         mbar_arrive(&c_full[end]);
       }
       __syncwarp();
-    } else if (warp >= WARP_PREP) {
-      // -------------------------------------------------------------- segments and Q, ahead
-      constexpr int CH = D / 8, STEP = 64 / CH;  // 16-byte chunks a row, rows the 64 threads load at a time
-      const int t = tid - WARP_PREP * 32, c = t % CH, first_row = t / CH;
-      uint32_t n_q[2] = {0, 0};
+    } else if (warp == WARP_PREP) {
+      // -------------------------------------------------------------- segments, one ahead
       Cut cut{0, 0, 0, 0, 0, {0, 0, 0}};
-      auto load_q = [&](int slot, int hand) {
-        if (n_q[slot] > 0 && ok) ok = mbar_wait(&q_empty[slot], (n_q[slot] - 1) & 1u, status, kErrWaitMma);
-        ++n_q[slot];
-        const int row0 = s.row_base + slot * ROWS;
-        const int live = min(ROWS, s.rows * G - row0);  // rows past it are never looked at
-        const T* q = static_cast<const T*>(a.q) + int64_t(s.r0) * a.q_strides[0] + s.h * G * a.q_strides[1] + c * 8;
-        uint8_t* dst = smem + L::Q + slot * L::TILE + (c >> 3) * L::HALF;
-        float* rf = rowf + hand * RB + slot * ROWS;
-        // all rows on their way at once, to where they stay; then every thread makes what it copied fp16
-        const int dn = STEP / G, dg = STEP - dn * G;  // a step in (node, head of the group)
-        int node = (row0 + first_row) / G, g = row0 + first_row - node * G;
-        for (int r = first_row; r < live; r += STEP) {
-          cp_async_16_zfill(smem_u32(dst) + uint32_t(r * 128 + (((c & 7) ^ (r & 7)) << 4)),
-                            q + node * a.q_strides[0] + g * a.q_strides[1], true);
-          node += dn;
-          g += dg;
-          if (g >= G) {
-            g -= G;
-            ++node;
-          }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        __syncwarp();
-#pragma unroll 4
-        for (int r0 = 0; r0 < live; r0 += STEP) {
-          const int r = r0 + first_row;
-          uint4* at = reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-          uint4 v = r < live ? *at : make_uint4(0u, 0u, 0u, 0u);
-          uint32_t* y = &v.x;
-          float f = 1.f;
-          if (std::is_same<T, bf16>::value) {  // largest exponent of the row; 255: infinite or NaN
-            uint32_t e = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) e = max(e, max((y[i] >> 7) & 0xffu, (y[i] >> 23) & 0xffu));
-#pragma unroll
-            for (int o = 1; o < CH; o <<= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, o));
-            const int up = int(e) - 141;  // values below 2^15
-            const float inv = pow2(max(min(-up, 126), -126));
-            f = e == 255 ? NAN : pow2(max(min(up, 126), -126));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = Elem<__half>::pack(bf16_lo(y[i]) * inv, bf16_hi(y[i]) * inv);
-          } else {  // an infinite q makes its row NaN whatever the codes are
-            uint32_t bad = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) bad |= (y[i] & 0x7c00u) == 0x7c00u || (y[i] & 0x7c000000u) == 0x7c000000u;
-#pragma unroll
-            for (int o = 1; o < CH; o <<= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, o);
-            f = bad ? NAN : 1.f;
-          }
-          if (r < live) {
-            if (c == 0) rf[r] = f * c_log2;
-            *at = make_uint4(y[0] ^ q_sign, y[1] ^ q_sign, y[2] ^ q_sign, y[3] ^ q_sign);
-          }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full[slot]);
-      };
       for (int k = 0;; ++k) {
+        const bool more = __all_sync(0xffffffffu, ok) && wk.next(plan, deal, s);
         const int hand = k & 1;
-        ok = named_all(5, 64, ok);  // (both warps leave together)
-        const bool more = ok && wk.next(plan, deal, s);
         if (k >= 2 && ok) ok = mbar_wait(&seg_empty[hand], uint32_t((k >> 1) - 1) & 1u, status, kErrWaitPeer);
-        if (more && s.t0 < s.t1) {
-          load_q(0, hand);
-          if (is_pair(s)) load_q(1, hand);
-        }
-        // handed over when the rows' factors are written: both warps'
-        named_sync(5, 64);
-        if (warp == WARP_PREP && lane == 0) {
+        if (lane == 0) {
           Handed* h = reinterpret_cast<Handed*>(smem + L::SEGS + 64 * hand);
           if (more) {
             h->s = s;
@@ -713,7 +684,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
         }
         if (!more) break;
       }
-      if (warp == WARP_PREP && lane == 0) static_cast<Cut*>(a.workspace)[blockIdx.x] = cut;
+      if (lane == 0) static_cast<Cut*>(a.workspace)[blockIdx.x] = cut;
       __syncwarp();
     } else if (warp == WARP_MMA) {
       // -------------------------------------------------------------- products
@@ -736,7 +707,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
       auto commit = [&](uint64_t* bar) {
         if (leader) tcg::umma_commit(bar);
       };
-      auto scores = [&](int slot, int qt, int x, bool last) {  // qt: the tile of Q
+      auto scores = [&](int slot, int qt, int x) {  // qt: the tile of Q
         if (!ok) return;
         const uint32_t qd = q_lo + uint32_t(qt) * (L::TILE >> 4);
         const uint32_t kd = desc_lo(ring_a + uint32_t(x) * L::TILE, 16);
@@ -747,7 +718,6 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
             umma_ss(tmem + uint32_t(slot * 128), desc_sw128(qd + off), desc_sw128(kd + off), ID_QK, k ? 1u : 0u);
           }
           tcg::umma_commit(&s_full[slot]);
-          if (last) tcg::umma_commit(&q_empty[qt]);  // the segment's last use of this Q
         }
         issued = true;
       };
@@ -786,9 +756,9 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
         if (pair) {
           int x = take();
           q_ready(0);
-          scores(0, 0, x, n == 1);
+          scores(0, 0, x);
           q_ready(1);
-          scores(1, 1, x, n == 1);
+          scores(1, 1, x);
           release(x);
           for (int t = 0; t < n; ++t) {
             const int v = take();
@@ -796,14 +766,14 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
             values(0, v, t == 0);
             if (more) {
               x = take();
-              scores(0, 0, x, t + 2 == n);
+              scores(0, 0, x);
             } else if (ok) {
               commit(&o_full[0]);
             }
             values(1, v, t == 0);
             release(v);
             if (more) {
-              scores(1, 1, x, t + 2 == n);
+              scores(1, 1, x);
               release(x);
             } else if (ok) {
               commit(&o_full[1]);
@@ -814,7 +784,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
           for (int z = 0; z < min(n, 2); ++z) {
             const int x = take();
             if (z == 0) q_ready(0);
-            scores(z, 0, x, z + 1 == n);
+            scores(z, 0, x);
             release(x);
           }
           for (int t = 0; t < n; ++t) {
@@ -823,7 +793,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
             release(v);
             if (t + 2 < n) {
               const int x = take();
-              scores(z, 0, x, t + 3 == n);
+              scores(z, 0, x);
               release(x);
             } else if (ok) {
               commit(&o_full[z]);
@@ -843,6 +813,55 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
   __syncthreads();
   tcg::tc_fence_after();
   if (warp == WARP_MMA) tcg::tmem_dealloc(tmem, 512);
+}
+
+// A block: 32 rows (lanes) of a cut item, a warp D / 4 of their values; the parts in order. The parts' values lie with
+// the row innermost, as a warp of 32 rows writes them.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) join_wide_kernel(const dspark_paged_attn_args a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int N = D / 4, HELD = 4;  // values a thread, parts under way together
+  const int cta = blockIdx.x, r = blockIdx.y * 32 + (threadIdx.x & 31), d0 = (threadIdx.x >> 5) * N;
+  const Cut c = static_cast<const Cut*>(a.workspace)[cta];
+  if (r >= c.live || c.parts == 0) return;
+  auto at = [&](int x) { return part_of<D, RB>(a.workspace, cta + x, x == 0); };
+  float m = -INFINITY;
+  for (int x0 = 0; x0 < c.parts; x0 += HELD) {
+    float y[HELD];
+#pragma unroll
+    for (int x = 0; x < HELD; ++x) y[x] = __ldcg(at(min(x0 + x, c.parts - 1)) + RB * D + r);
+#pragma unroll
+    for (int x = 0; x < HELD; ++x) m = fmaxf(m, y[x]);
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+  float sum = 0.f, v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = 0.f;
+  for (int x = 0; x < c.parts; ++x) {
+    const float* p = at(x) + d0 * RB + r;
+    const float y = __ldcg(at(x) + RB * D + r);
+    float u[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) u[i] = __ldcg(p + i * RB);
+    if (y == -INFINITY) continue;  // a part that saw nothing
+    const float f = ex2(y - ref);
+    sum += f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = fmaf(u[i], f, v[i]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int G = a.Hq / a.Hk, node = (c.row_base + r) / G, hq = c.h * G + c.row_base + r - node * G;
+  T* out = static_cast<T*>(a.out) + int64_t(c.r0 + node) * a.o_strides[0] + hq * a.o_strides[1] + d0;
+#pragma unroll
+  for (int i = 0; i < N; i += 8) {
+    uint4 w;
+    w.x = Elem<T>::pack(v[i] * inv, v[i + 1] * inv);
+    w.y = Elem<T>::pack(v[i + 2] * inv, v[i + 3] * inv);
+    w.z = Elem<T>::pack(v[i + 4] * inv, v[i + 5] * inv);
+    w.w = Elem<T>::pack(v[i + 6] * inv, v[i + 7] * inv);
+    *reinterpret_cast<uint4*>(out + i) = w;
+  }
 }
 
 template <typename T, int D>
@@ -870,7 +889,7 @@ static int launch(const dspark_paged_attn_args& a, cudaStream_t s) {
   DSPARK_CUDA_TRY(launch_ex(attn_kernel<T, D>, dim3(n), dim3(NTHR), TOTAL, s, 1, true, maps[0], maps[1], a, c,
                             a.scale < 0.f ? 0x80008000u : 0u, status_word(dev)),
                   "paged_attn");
-  DSPARK_CUDA_TRY(launch_ex(join_kernel<T, D, RB>, dim3(n, RB / 4), dim3(128), 0, s, 1, true, a), "paged_attn: join");
+  DSPARK_CUDA_TRY(launch_ex(join_wide_kernel<T, D>, dim3(n, RB / 32), dim3(128), 0, s, 1, true, a), "paged_attn: join");
   return DSPARK_OK;
 }
 
