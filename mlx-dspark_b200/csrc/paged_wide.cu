@@ -512,9 +512,13 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
     if (warp >= WARP_CONV) {
       // -------------------------------------------------------------- codes to fp16 tiles
       constexpr int CH = D / 16, RPI = 32 / CH, ROUNDS = 32 / RPI;  // 16-byte chunks a row, rows a round, rounds a warp
-      const int w = warp - WARP_CONV, r = lane / CH, c = lane % CH;  // the lane's row of a round, its chunk
-      // the lanes of the upper 64 values store their halves the other way round: no two on one bank
-      const int cc = (c & 3) * 2, first = c >> 2;
+      // A lane's chunk and row of a round. D = 128: eight lanes that go together have four chunks of one 64-value half of rows
+      // r and r ^ 5, whose places differ in both swizzles: no two on one bank, reading or writing.
+      const int w = warp - WARP_CONV, c = D == 128 ? (lane & 3) + (lane >> 4) * 4 : lane & 3;
+      auto row_of = [&](int z) {
+        const int q = (lane >> 2) & 3;
+        return w * 32 + (D == 128 ? 8 * (z >> 1) + ((2 * (z & 1) + (q >> 1)) ^ ((q & 1) * 5)) : z * RPI + (lane >> 2));
+      };
       int st = 0, st_phase = 0, x = 0, use = 0;
       while (true) {
         ok = mbar_wait(&c_full[st], uint32_t(st_phase), status, kErrWaitKV);
@@ -528,16 +532,15 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
         const uint8_t* codes = smem + L::STAGE + st * L::CODES;
         uint8_t* base = ring + x * L::TILE + (c >> 2) * L::HALF;
         auto get = [&](int z) {
-          const int row = w * 32 + z * RPI + r;
-          const int sw = D == 128 ? row & 7 : (row >> 1) & 3;
+          const int row = row_of(z), sw = D == 128 ? row & 7 : (row >> 1) & 3;
           return *reinterpret_cast<const uint4*>(codes + row * D + ((c ^ sw) << 4));
         };
         auto put = [&](int z, uint4 v) {
           const uint4 h0 = make_uint4(e4m3_to_f16(v.x), e4m3_to_f16_hi(v.x), e4m3_to_f16(v.y), e4m3_to_f16_hi(v.y));
           const uint4 h1 = make_uint4(e4m3_to_f16(v.z), e4m3_to_f16_hi(v.z), e4m3_to_f16(v.w), e4m3_to_f16_hi(v.w));
-          const int row = w * 32 + z * RPI + r, sw = row & 7;
-          *reinterpret_cast<uint4*>(base + row * 128 + (((cc + first) ^ sw) << 4)) = first ? h1 : h0;
-          *reinterpret_cast<uint4*>(base + row * 128 + (((cc + (first ^ 1)) ^ sw) << 4)) = first ? h0 : h1;
+          const int row = row_of(z), at = (c & 3) * 2, sw = row & 7;
+          *reinterpret_cast<uint4*>(base + row * 128 + ((at ^ sw) << 4)) = h0;
+          *reinterpret_cast<uint4*>(base + row * 128 + (((at + 1) ^ sw) << 4)) = h1;
         };
         if (note.kind >= 0 && note.left >= BN) {
 #pragma unroll
@@ -552,7 +555,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
 #pragma unroll 1
           for (int z = 0; z < ROUNDS; ++z) {
             uint4 v = get(z);
-            if (w * 32 + z * RPI + r >= note.left) v = make_uint4(0u, 0u, 0u, 0u);  // no key: whatever the page holds there
+            if (row_of(z) >= note.left) v = make_uint4(0u, 0u, 0u, 0u);  // no key: whatever the page holds there
             if (note.kind < 0) {
               uint32_t* y = &v.x;
               uint32_t any = 0;
