@@ -94,6 +94,9 @@ APPENDS = [
     ([33, 64, 16, 15], [0, 64, 1, 17], 16, 2, 128, 16, "half", 16, HF, False, "heads", False),
     ([1] * 70, list(range(70)), 2, 1, 64, 64, "interleaved", 16, BF, True, "heads", False),
     ([0, 0, 0], [5, 0, 64], 4, 2, 64, 64, "half", 32, BF, False, "heads", False),
+    # a page of one request with more rows than the others' average: its rows are made twice
+    ([1] * 20 + [70] + [2] * 9, list(range(40, 70)), 4, 3, 128, 128, "half", 64, BF, True, "heads", False),
+    ([150] + [1] * 40, [7] + [3] * 40, 2, 2, 64, 32, "interleaved", 128, HF, False, "tokens", True),
 ]
 
 
@@ -344,6 +347,125 @@ def test_attention(cuda, case):
     out = torch.full(q.shape, 5.0, dtype=dt, device=cuda)
     _check(cuda, cache, q, counts, lens, rows, causal, D ** -0.5, out)
     assert bool((out[sum(counts):] == 5.0).all())  # rows of nobody
+
+
+def _far(rows, page):
+    """The tables widened to 200,000 tokens: with that much room, calls of more than 32 rows a request and kv head on
+    average go to the kernel for many rows (the narrow tables of small tests do not)."""
+    width = 200000 // page
+    return [r + [-1] * (width - len(r)) for r in rows]
+
+
+MANY = [
+    # counts, lens, Hq, Hk, D, page, type, causal, pool layout
+    ([17], [17], 4, 1, 128, 64, BF, True, "heads"),              # one slot's rows, one tile
+    ([40, 3, 0, 90], [40, 700, 9, 333], 8, 2, 128, 16, HF, True, "heads"),
+    ([40, 3, 0, 90], [40, 700, 9, 333], 8, 2, 128, 16, BF, False, "tokens"),
+    ([65, 1], [1300, 96], 8, 2, 64, 32, BF, True, "heads"),      # 260 rows: two blocks of rows, the last of four
+    ([64], [257], 8, 2, 64, 128, HF, False, "heads"),            # 256 rows: both slots full
+    ([33, 33, 33], [128, 129, 640], 7, 1, 128, 128, BF, True, "tokens"),
+    ([200], [200], 4, 2, 128, 64, HF, True, "heads"),            # a prompt of its own keys alone
+    ([45] * 20, [45 + 61 * i % 500 for i in range(20)], 4, 4, 64, 64, BF, True, "heads"),
+]
+
+
+@pytest.mark.parametrize("case", MANY, ids=range(len(MANY)))
+def test_attention_many_rows(cuda, case):
+    counts, lens, Hq, Hk, D, page, dt, causal, layout = case
+    rng, g = random.Random(D + page), torch.Generator().manual_seed(len(counts) + page + 1)
+    need = [-(-x // page) for x in lens]
+    cache = _finite_pool(cuda, sum(need) + 4, Hk, page, D, g, layout)
+    rows = _far(_tables(need, sum(need) + 4, rng, max(need) + 1), page)
+    q = torch.randn(sum(counts) + 2, Hq + 1, D, generator=g).to(dt).to(cuda)[:, :Hq]
+    out = torch.full(q.shape, 5.0, dtype=dt, device=cuda)
+    _check(cuda, cache, q, counts, lens, rows, causal, D ** -0.5, out)
+    assert bool((out[sum(counts):] == 5.0).all())
+    again = cache.attention(q, _cu(counts, cuda), _i32(lens, cuda), _i32(rows, cuda), scale=D ** -0.5, causal=causal)
+    assert torch.equal(again[: sum(counts)], out[: sum(counts)])  # no order of blocks shows
+
+
+@pytest.mark.parametrize("n", [20, 80])  # 40 rows: the slots share them; 160: a slot each
+def test_attention_many_rows_edges(cuda, n):
+    """What the tests below hold a few rows to: scales of the scores, scales far apart, q of any size, NaN in hidden
+    places, pages that are not there, rows that see nothing."""
+    from mlx_dspark_b200 import _lib
+
+    g, dev = torch.Generator().manual_seed(n), cuda.index
+    cache = _finite_pool(cuda, 40, 1, 16, 64, g, span=0)
+    base = torch.randn(n, 2, 64, generator=g)
+    q, cu = base.to(BF).to(cuda), _cu([n], cuda)
+    rows = _far([list(range(30))], 16)
+    for scale in (0.0, -0.2, 3.0):
+        _check(cuda, cache, q, [n], [470], rows, True, scale)
+    sizes = torch.tensor([1e-38, 1e-20, 1.0, 1e3, 1e-3, 0.0] * n)[:n, None, None]
+    _check(cuda, cache, (base * sizes).to(BF).to(cuda), [n], [470], rows, True, 0.125)
+    table, ln = _i32(rows, cuda), _i32([470], cuda)
+    bad = q.clone()
+    bad[1, 0, 5], bad[n - 1, 1, 9] = math.inf, math.nan
+    out, fine = (cache.attention(x, cu, ln, table, scale=0.125) for x in (bad, q))
+    want = torch.zeros(n, 2, dtype=torch.bool)
+    want[1, 0] = want[n - 1, 1] = True
+    assert torch.equal(out.isnan().any(-1).cpu(), want) and torch.equal(out[~want.to(cuda)], fine[~want.to(cuda)])
+    # NaN codes: behind the last key, and in keys of the rows' own
+    clean = fine
+    for t in (cache.k, cache.v):
+        t.view(torch.uint8)[29, 0, 6:] = 0x7F
+    assert torch.equal(cache.attention(q, cu, ln, table, scale=0.125), clean)
+    own = 470 - n + 7  # the eighth row's own token
+    for t in (cache.v, cache.k):
+        old = t[own // 16, 0, own % 16].view(torch.uint8).clone()
+        t.view(torch.uint8)[own // 16, 0, own % 16, 10] = 0xFF
+        out = cache.attention(q, cu, ln, table, scale=0.125)
+        assert torch.equal(out[:7], clean[:7])
+        nan = out[7:].isnan()
+        if t is cache.v:
+            assert bool(nan[..., 10].all()) and int(nan.sum()) == (n - 7) * 2
+        else:
+            assert bool(nan.all())
+        t.view(torch.uint8)[own // 16, 0, own % 16] = old
+    # a key of everybody's
+    t = cache.v.view(torch.uint8)
+    old = t[3, 0, 4].clone()
+    t[3, 0, 4, 11] = 0x7F
+    nan = cache.attention(q, cu, ln, table, scale=0.125).isnan()
+    assert bool(nan[..., 11].all()) and int(nan.sum()) == n * 2
+    t[3, 0, 4] = old
+    # pages outside the pool and without a positive scale: as if they were not in the table
+    short = cache.attention(q, cu, _i32([464], cuda), _i32(_far([list(range(5)) + list(range(6, 30))], 16), cuda), scale=0.2,
+                            causal=False)
+    assert _lib.device_status(dev) == 0
+    for page in (-7, 40, 2 ** 31 - 1):
+        r = list(range(30))
+        r[5] = page
+        out = cache.attention(q, cu, _i32([480], cuda), _i32(_far([r], 16), cuda), scale=0.2, causal=False)
+        assert _lib.device_status(dev) != 0 and _lib.device_status(dev) == 0
+        # (page 29's last ten tokens hold NaN codes: 480 keys see them)
+        assert bool(out.isnan().all())
+    for t in (cache.k, cache.v):
+        t.view(torch.uint8)[29, 0, 6:] = 0x30
+    short = cache.attention(q, cu, _i32([464], cuda), _i32(_far([list(range(5)) + list(range(6, 30))], 16), cuda), scale=0.2,
+                            causal=False)
+    for page in (-7, 40):
+        r = list(range(30))
+        r[5] = page
+        out = cache.attention(q, cu, _i32([480], cuda), _i32(_far([r], 16), cuda), scale=0.2, causal=False)
+        assert torch.allclose(out.float(), short.float(), rtol=2e-2, atol=2e-2) and _lib.device_status(dev) != 0
+    for s in (0.0, -1.0, math.nan):
+        keep = cache.k_scale[5].clone()
+        cache.k_scale[5] = s
+        out = cache.attention(q, cu, _i32([480], cuda), table, scale=0.2, causal=False)
+        assert torch.allclose(out.float(), short.float(), rtol=2e-2, atol=2e-2)
+        cache.k_scale[5] = keep
+    # rows that see nothing
+    out = cache.attention(q, cu, _i32([n - 9], cuda), table, scale=0.2)
+    assert bool((out[:9] == 0).all()) and bool((out[9:] != 0).any(-1).all())
+    assert bool((cache.attention(q, cu, _i32([0], cuda), table, scale=0.2) == 0).all())
+    none = cache.attention(q, cu, _i32([64], cuda), _i32(_far([[-1] * 4], 16), cuda), scale=0.2)
+    assert bool((none == 0).all()) and _lib.device_status(dev) != 0
+    # scales 2^80 apart, the largest weights where the values are smallest
+    cache.v_scale[:8].copy_(torch.exp2(torch.tensor([[-40.0], [30.0], [0.0], [-40.0], [10.0], [-20.0], [0.0], [-60.0]])))
+    for r in ([0, 3, 7, 5], [2, 6, 9], [0, 1, 2], [7]):
+        _check(cuda, cache, q, [n], [16 * len(r) - 2], _far([r], 16), False, 0.125)
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
