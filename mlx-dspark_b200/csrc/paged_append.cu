@@ -25,14 +25,20 @@ constexpr int U = 4;  // heads of q in flight a lane
 constexpr int64_t ROUNDS = 1;
 
 // cos and sin of pos * f, f in 64-bit fixed-point turns (the product wraps at whole turns: any position keeps its
-// phase to 2^-32 of a turn). Not the special-function unit's, which are off by up to 1e-6: three times as many
-// values would then fall to the other side of a border between two codes as fp32 rounding alone sends there. Within an
-// eighth of a turn of the nearest quarter their Taylor series to the 9th and 8th power are off by 2e-9 and 2.5e-8.
+// phase to 2^-32 of a turn), to a little more than half an fp32 step: not the special-function unit's, which are off by
+// up to 1e-6, for every error sends its share of values to the other side of a border between two codes. The angle
+// from the nearest quarter turn, up to pi / 4, is a + d, d what is lost in fp32: its first 23 bits a product with its
+// rounding, the others' product. Taylor series to the 9th and 10th power (off by 2e-9 and 1e-10), d by their derivatives,
+// the largest term added last.
 __device__ __forceinline__ void phase(int pos, uint64_t f, float& c, float& s) {
+  constexpr float K = 0x1.921fb60000000p-30f, K_LOW = -0x1.777a5c0000000p-55f;  // 2 pi / 2^32, and what fp32 leaves of it
   const uint32_t t = uint32_t((uint64_t(int64_t(pos)) * f) >> 32), quarter = (t + 0x20000000u) >> 30;
-  const float a = float(int32_t(t - (quarter << 30))) * 1.4629180792671596e-9f, z = a * a;  // 2 pi / 2^32
-  const float sn = fmaf(a * z, fmaf(z, fmaf(z, fmaf(z, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), a);
-  const float cs = fmaf(z, fmaf(z, fmaf(z, fmaf(z, 1.f / 40320, -1.f / 720), 1.f / 24), -0.5f), 1.f);
+  const int r = int(t - (quarter << 30));
+  const float hi = float(r & ~127), a = hi * K, z = a * a;
+  const float d = fmaf(float(r & 127), K, fmaf(hi, K_LOW, fmaf(hi, K, -a)));
+  const float p = fmaf(z, fmaf(z, fmaf(z, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6);
+  const float q = fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24), -0.5f);
+  const float sn = a + fmaf(a * z, p, d * fmaf(z, q, 1.f)), cs = 1.f + fmaf(z, q, -d * a);
   const float x = quarter & 1 ? sn : cs, y = quarter & 1 ? cs : sn;
   c = __uint_as_float(__float_as_uint(x) ^ ((quarter + 1) & 2) << 30);
   s = __uint_as_float(__float_as_uint(y) ^ (quarter & 2) << 30);
