@@ -7,8 +7,8 @@ namespace dspark {
 namespace paged {
 
 // Device status of what an append dropped (no room, or a page id outside the pool) and of pages outside the
-// pool that an attention did not see.
-constexpr int kErrAppendPage = 0x206, kErrAttnPage = 0x207;
+// pool that an attention did not see; shared memory that begins off a 1024-byte boundary.
+constexpr int kErrAppendPage = 0x206, kErrAttnPage = 0x207, kErrAlign = 0x208;
 
 // Two codes (the low byte first) as two fp16 values: every e4m3 value is an fp16 one.
 __device__ __forceinline__ uint32_t e4m3_to_f16(uint32_t codes) {

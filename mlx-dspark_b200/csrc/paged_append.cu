@@ -22,7 +22,6 @@ namespace paged {
 
 constexpr int Q_THREADS = 128;
 constexpr int U = 4;  // heads of q in flight a lane
-constexpr int64_t ROUNDS = 1;
 
 // cos and sin of pos * f, f in 64-bit fixed-point turns (the product wraps at whole turns: any position keeps its
 // phase to 2^-32 of a turn), to a little more than half an fp32 step: not the special-function unit's, which are off by
@@ -363,12 +362,12 @@ template <typename T, bool VEC, bool HALF, int PASS, int THREADS, int MIN_BLOCKS
 static cudaError_t launch_as(const dspark_paged_append_args& a, cudaStream_t s) {
   const int64_t units = int64_t(a.R) / a.page + 2 * int64_t(a.B);
   // groups of heads: as few as leave a round of blocks (a page that is not written ends its block at once)
-  const int64_t least = ROUNDS * MIN_BLOCKS * sm_count(current_device());
+  const int64_t least = int64_t(MIN_BLOCKS) * sm_count(current_device());
   const int groups = int(std::min<int64_t>(a.Hk, std::max<int64_t>(1, (least + 2 * units - 1) / (2 * units))));
   const int64_t page_blocks = units * groups * 2;
   // warps a row of q: one, unless that leaves less than 16 warps an SM (then as many as take U heads a lane)
   const int sms = sm_count(current_device()), per = 32 / (a.D / 16);
-  const int most = (a.Hq + per - 1) / per, want = (16 * sms + a.R - 1) / a.R;
+  const int most = (a.Hq + per - 1) / per, want = (16 * sms + a.R - 1) / std::max(a.R, 1);
   const int warps = std::max(1, std::min(want, most));
   const int64_t q_blocks = (int64_t(a.R) * warps + THREADS / 32 - 1) / (THREADS / 32);
   if (page_blocks + q_blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;

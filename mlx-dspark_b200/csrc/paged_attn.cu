@@ -75,7 +75,7 @@ __device__ __forceinline__ uint32_t at_chunk(int row, int c) {
 
 template <typename T, int D, int RT>
 __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_args a, const float c_log2,
-                                                                          const uint32_t q_sign, int* status) {
+                                                       const uint32_t q_sign, int* status) {
   typedef Lay<D, RT> L;
   constexpr int RB = L::RB, KS = D / 16, CH = D / 16;  // k steps of the scores, 16-byte chunks a row
   extern __shared__ __align__(128) uint8_t smem[];
@@ -159,15 +159,15 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
           }
         } else {
 #pragma unroll 1
-        for (int z = 0; z < ROUNDS; ++z) {
-          const uint32_t to = dst + z * RPI * D + (z & 1 ? sw1 : sw0);
-          const int y = z % (ROUNDS / 2) * RPI;
-          const uint8_t* k = (z < ROUNDS / 2 ? k0 : k1) + y * kts;
-          const uint8_t* v = (z < ROUNDS / 2 ? v0 : v1) + y * vts;
-          const bool there = whole || ((z < ROUNDS / 2 ? id0 : id1) >= 0 && key0 + z * RPI + lane / CH < s.len);
-          cp_async_16_zfill(to, there ? k : kp, there);
-          cp_async_16_zfill(to + L::TILE, there ? v : vp, there);
-        }
+          for (int z = 0; z < ROUNDS; ++z) {
+            const uint32_t to = dst + z * RPI * D + (z & 1 ? sw1 : sw0);
+            const int y = z % (ROUNDS / 2) * RPI;
+            const uint8_t* k = (z < ROUNDS / 2 ? k0 : k1) + y * kts;
+            const uint8_t* v = (z < ROUNDS / 2 ? v0 : v1) + y * vts;
+            const bool there = whole || ((z < ROUNDS / 2 ? id0 : id1) >= 0 && key0 + z * RPI + lane / CH < s.len);
+            cp_async_16_zfill(to, there ? k : kp, there);
+            cp_async_16_zfill(to + L::TILE, there ? v : vp, there);
+          }
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -489,9 +489,9 @@ static int launch(const dspark_paged_attn_args& a, cudaStream_t s) {
                                                                cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
                                  }),
                   "paged_attn: shared memory");
-  // the running maximum needs a positive factor: a negative scale goes into q, and zero becomes one that leaves all
-  // weights equal
-  const float c = a.scale == 0.f ? 1e-30f : fabsf(a.scale) * 1.4426950408889634f;
+  // the running maximum needs a positive factor: a negative scale goes into q (none is below 1e-35, with which all weights
+  // are equal)
+  const float c = fabsf(a.scale) * 1.4426950408889634f;
   DSPARK_CUDA_TRY(launch_ex(attn_kernel<T, D, RT>, dim3(n), dim3(NTHR), L::TOTAL, s, 1, true, a, c,
                             a.scale < 0.f ? 0x80008000u : 0u, status_word(dev)),
                   "paged_attn");
@@ -504,11 +504,13 @@ static int launch(const dspark_paged_attn_args& a, cudaStream_t s) {
 // on the device). Measured, this kernel / the other, us, 32/8 heads of 128: 16 rows over 4k keys, 1 request (2048 of
 // such tiles with their 64 rows a head) 21 / 30, 4 requests 36 / 39, 16 requests (8192) 90 / 77; 32 rows over 16k, 1
 // request (4096) 49 / 43; 64 requests of 64 rows over 4k 1105 / 420.
-constexpr int FEW_ROWS = 32, WIDE_TILES = 3000;
+// Not where a request may have more than 2^25 keys: a wait there can last a segment, which has to end within the limit.
+constexpr int FEW_ROWS = 32, WIDE_TILES = 3000, LONGEST = 1 << 25;
 static bool has_many_rows(int R, int B, int Hq, int Hk) { return int64_t(R) * (Hq / Hk) > int64_t(FEW_ROWS) * B; }
 static bool is_wide(const dspark_paged_attn_args& a) {
-  const int64_t blocks = (int64_t(a.R) * (a.Hq / a.Hk) + FEW_ROWS - 1) / FEW_ROWS * a.Hk;
-  return has_many_rows(a.R, a.B, a.Hq, a.Hk) && blocks * (int64_t(a.max_pages) * a.page / BN + 1) > WIDE_TILES && a.n_pages > 0;
+  const int64_t blocks = (int64_t(a.R) * (a.Hq / a.Hk) + FEW_ROWS - 1) / FEW_ROWS * a.Hk, keys = int64_t(a.max_pages) * a.page;
+  return has_many_rows(a.R, a.B, a.Hq, a.Hk) && blocks * (keys / BN + 1) > WIDE_TILES &&
+         keys <= LONGEST && a.n_pages > 0;
 }
 
 template <typename T, int D>
@@ -532,7 +534,7 @@ size_t dspark_paged_attn_workspace(int R, int B, int Hq, int Hk, int D) {
   if (R <= 0 || B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || D <= 0) return 0;
   if (paged::has_many_rows(R, B, Hq, Hk)) return paged::wide_workspace(D);
   return paged::MAX_CTA * sizeof(paged::Cut) +
-         size_t(paged::grid_of(current_device(), 2)) * 2 * 32 * (D + 1) * sizeof(float);  // (also enough for 3 of 16 rows)
+         size_t(paged::grid_of(current_device(), 2)) * 2 * 32 * (D + 1) * sizeof(float);
 }
 
 int dspark_paged_attn(const dspark_paged_attn_args* p, void* stream) {

@@ -83,7 +83,7 @@ struct Walker {
   bool have;
   __device__ __forceinline__ bool next(const Plan<RB>& p, const Deal& deal, Segment& g) {
     const dspark_paged_attn_args& a = p.a;
-    while (x < end) {
+    while (x < end && b < a.B) {
       if (!have) s = p.shape(b);
       have = true;
       const uint32_t item = p.seg + s.C, all = s.M * a.Hk * item;

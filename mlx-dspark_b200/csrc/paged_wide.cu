@@ -222,7 +222,11 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (smem_u32(smem) & 1023u) {  // the swizzled tiles need it; never seen without static arrays
-    if (tid == 0) report_error(status, 0x208);
+    pdl_wait();
+    if (tid == 0) {
+      report_error(status, kErrAlign);
+      static_cast<Cut*>(a.workspace)[blockIdx.x] = Cut{0, 0, 0, 0, 0, {0, 0, 0}};
+    }
     return;
   }
   if (tid == 0) {
@@ -886,11 +890,16 @@ static int launch(const dspark_paged_attn_args& a, cudaStream_t s) {
   }
   DSPARK_CUDA_TRY(configure_once((const void*)attn_kernel<T, D>, TOTAL,
                                  [&] {
+                                   // setmaxnreg.inc waits for registers that the block was launched with
+                                   cudaFuncAttributes f;
+                                   const cudaError_t e = cudaFuncGetAttributes(&f, attn_kernel<T, D>);
+                                   if (e != cudaSuccess) return e;
+                                   if (f.numRegs * NTHR < 256 * (184 + 72)) return cudaErrorLaunchOutOfResources;
                                    return cudaFuncSetAttribute(attn_kernel<T, D>,
                                                                cudaFuncAttributeMaxDynamicSharedMemorySize, TOTAL);
                                  }),
                   "paged_attn: shared memory");
-  const float c = a.scale == 0.f ? 1e-30f : fabsf(a.scale) * 1.4426950408889634f;
+  const float c = fabsf(a.scale) * 1.4426950408889634f;
   DSPARK_CUDA_TRY(launch_ex(attn_kernel<T, D>, dim3(n), dim3(NTHR), TOTAL, s, 1, true, maps[0], maps[1], a, c,
                             a.scale < 0.f ? 0x80008000u : 0u, status_word(dev)),
                   "paged_attn");

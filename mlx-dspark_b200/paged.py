@@ -85,8 +85,8 @@ class PagedCache:
         The scale of a page and head is the smallest power of two with which the largest value appended to it is at
         most 448; a page that holds tokens already keeps its scale or raises it, and then its codes are rounded to
         the new one. Rows for which the table has no page (or one outside the pool) are dropped and recorded in the
-        device status. Rows behind the last request's are left as they are. Two requests of one call must not append to
-        one page."""
+        device status. Rows behind the last request's are left as they are. One call must not append to a page twice (two
+        requests with one page, or a request whose table repeats it)."""
         stream = on_device(q, k, v, cu_rows, kv_len, page_table, row_pos, q_norm, k_norm, q_out, len_out, table.freq,
                            self.k)
         shape, D = q.shape, self.head_dim
@@ -102,7 +102,7 @@ class PagedCache:
             raise _lib.DSparkError(_lib.ERR_ARG, f"q_out {tuple(q_out.shape)} for {tuple(shape)}")
         if len_out is None:
             len_out = torch.empty(B, dtype=torch.int32, device=q.device)
-        elif len_out.data_ptr() == kv_len.data_ptr() and B:
+        elif abs(len_out.data_ptr() - kv_len.data_ptr()) < 4 * B:
             raise _lib.DSparkError(_lib.ERR_ARG, "len_out must not be kv_len: blocks of one launch read the old lengths")
         qs, ks, vs, os = _strides("q", q), _strides("k", k), _strides("v", v), _strides("q_out", q_out)
         dt = _dtype(q, k, v, q_out, q_norm, k_norm)

@@ -174,6 +174,27 @@ def test_append(cuda, case):
         assert torch.equal(after.view(torch.uint8)[keep], before_.view(torch.uint8)[keep])  # nothing else is written
 
 
+@pytest.mark.parametrize("off", [0, 1, 2, 4])
+def test_append_of_rows_at_any_alignment(cuda, off):
+    """q, k, v and q_out as slices that begin and step off the 16-byte boundaries; q rotated in place."""
+    from mlx_dspark_b200 import rope
+
+    g, Hq, Hk, D, page, R = torch.Generator().manual_seed(off), 3, 2, 64, 16, 21
+    table = rope.RopeTable(D, 32, theta=1e4, device=cuda)
+    x = torch.randn(R, (Hq + 2 * Hk) * D + 8, generator=g).to(BF).to(cuda)
+    cut = [x[:, off + a * D : off + b * D].unflatten(1, (-1, D)) for a, b in ((0, 3), (3, 5), (5, 7))]
+    plain = [t.contiguous() for t in cut]
+    got = []
+    for q, k, v in (cut, plain):
+        cache = _pool(cuda, 4, Hk, page, D, torch.Generator().manual_seed(1))
+        out, _ = cache.append(q, k, v, table, _cu([R], cuda), _i32([9], cuda), _i32([[3, 0]], cuda), q_out=q)
+        assert out is q
+        got.append((out.clone(), cache))
+    assert torch.equal(got[0][0], got[1][0])
+    assert _same_codes(got[0][1].k, got[1][1].k) and _same_codes(got[0][1].v, got[1][1].v)
+    assert torch.equal(got[0][1].k_scale, got[1][1].k_scale)
+
+
 def _identity(cuda, D):
     """A rotation by nothing: positions 0."""
     from mlx_dspark_b200 import rope
@@ -750,6 +771,36 @@ def test_scores_of_padded_rows_and_out(cuda):
         sampling.token_logprobs(x.to(cuda), _i32([0] * 5, cuda))
     empty = sampling.token_logprobs(x.to(cuda)[:0], _i32([], cuda), top=2)
     assert empty["top_ids"].shape == (0, 2)
+
+
+@pytest.mark.parametrize("n", [6, 500])
+def test_attention_without_a_scale(cuda, n):
+    """scale = 0: every visible key weighs the same, whatever q is (both kernels)."""
+    g = torch.Generator().manual_seed(n)
+    L, D = 4000, 64
+    cache = _finite_pool(cuda, 125, 2, 32, D, g)
+    q = (torch.randn(n, 8, D, generator=g) * 1e37).to(BF).to(cuda)
+    rows = [list(range(125))]
+    args = _cu([n], cuda), _i32([L], cuda), _i32(rows, cuda)
+    out = cache.attention(q, *args, scale=0.0)
+    assert torch.equal(out, cache.attention(torch.ones_like(q), *args, scale=0.0))
+    _check(cuda, cache, torch.ones_like(q), [n], [L], rows, True, 0.0)
+
+
+def test_append_of_no_rows(cuda):
+    from mlx_dspark_b200 import rope
+
+    cache = _pool(cuda, 3, 2, 16, 64, torch.Generator().manual_seed(0))
+    q, k = (torch.empty(0, h, 64, dtype=BF, device=cuda) for h in (4, 2))
+    keep = cache.k.clone(), cache.k_scale.clone()
+    out, now = cache.append(q, k, k, rope.RopeTable(64, device=cuda), _cu([0, 0], cuda), _i32([5, 17], cuda),
+                            _i32([[0, 0], [1, 2]], cuda))
+    assert out.shape == (0, 4, 64) and now.tolist() == [5, 17]
+    assert torch.equal(keep[0].view(torch.uint8), cache.k.view(torch.uint8)) and torch.equal(keep[1], cache.k_scale)
+    both = torch.tensor([5, 17, 0], dtype=torch.int32, device=cuda)
+    with pytest.raises(Exception, match="len_out"):
+        cache.append(q, k, k, rope.RopeTable(64, device=cuda), _cu([0, 0], cuda), both[:2], _i32([[0, 0], [1, 2]], cuda),
+                     len_out=both[1:])
 
 
 # ------------------------------------------------------------------------------- together
