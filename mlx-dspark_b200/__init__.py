@@ -11,6 +11,8 @@ Modules mirror the reference operator surface (``src/mlx_dspark/``):
 * :mod:`.rope`, :mod:`.tree`, :mod:`.sampling` — rounds of drafted trees for sampled targets: rotary
   positions and append, attention with ancestor masks, accept, the kept path; :mod:`.tree_engine`
   runs them together over a target,
+* :mod:`.paged` — a paged cache of 8-bit values: append with rotary positions, attention over the pages;
+  :func:`.sampling.token_logprobs` scores tokens (log probability, entropy, rank, alternatives),
 * :mod:`.quant` — MLX-layout affine quantization of device tensors.
 
 All compute runs in ``libdspark.so`` (hand-written sm_100a CUDA) through a C ABI; torch only

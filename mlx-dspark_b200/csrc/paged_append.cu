@@ -11,7 +11,8 @@
 // value is then known inside a block, which holds a head's new values in registers meanwhile. Then those of q, a warp or more a
 // row. Which page a block has is found from cu_rows without a sum over the requests: request b's pages
 // start at unit cu_rows[b] / page + 2 b, which leaves room for every page that n rows can touch (n / page + 2).
-// Bound: HBM for prompts (each value is read and written once), the launch for few rows.
+// Bound: HBM and instructions for prompts (each value is read and written once; 16,389 rows of 32/8 heads of 128 84 us, 0.67
+// of the measured rate, 59 % of the issue slots), the launch for few rows (one row 3.2 us).
 #include <algorithm>
 
 #include "host_common.h"
@@ -384,8 +385,8 @@ static cudaError_t launch_as(const dspark_paged_append_args& a, cudaStream_t s) 
 template <typename T, bool VEC, bool HALF>
 static cudaError_t launch_page(const dspark_paged_append_args& a, cudaStream_t s) {
   // Threads by the rows that a page gets on average (a page with more than its block holds is made twice): in registers
-  // 64 * 16 values of few rows, else the whole page. 200 requests of 1 to 16 rows 12.9 us with 128 threads, a prompt's
-  // 16,389 rows in pages of 64 80.8 with 256 threads of two rows (4 rows 94).
+  // 64 * 16 values of few rows, else the whole page. 200 requests of 1 to 16 rows 13.4 us with 128 threads, a prompt's
+  // 16,389 rows in pages of 64 84 with 256 threads of two rows (4 rows a thread: 94 beside 81, with a coarser sine).
   const int64_t rows = std::min<int64_t>(a.page, (int64_t(a.R) + a.B - 1) / a.B), parts = rows * a.D / 16;
   if (parts <= 32) return launch_as<T, VEC, HALF, 1, 64, 10>(a, s);
   if (parts <= 128) return launch_as<T, VEC, HALF, 1, 128, 5>(a, s);

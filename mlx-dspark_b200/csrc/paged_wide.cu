@@ -17,6 +17,10 @@
 //    the maximum in use is only raised when a tile exceeds it by more than 2^8; weights are 2^7 times as large.
 //
 // Rounding: weights are rounded to fp16 for the product with V (their sum is not); scores, maxima, sums and O are fp32.
+//
+// Bound: softmax and products in turn (two chunks of 509 rows over 16k keys, 64/8 heads of 128: 537 to 549 us, 0.6 of the
+// products' measured rate, 2.06 us a 256 x 128 tile); for slots of few rows the conversion of codes (24 blocks of 1 to 16 rows
+// over 256 to 16k keys, 32/8 heads: 93 us, about 1.3 a tile).
 #include <algorithm>
 
 #include "host_common.h"
