@@ -83,7 +83,7 @@ struct Walker {
   bool have;
   __device__ __forceinline__ bool next(const Plan<RB>& p, const Deal& deal, Segment& g) {
     const dspark_paged_attn_args& a = p.a;
-    while (x < end && b < a.B) {
+    while (x < end) {
       if (!have) s = p.shape(b);
       have = true;
       const uint32_t item = p.seg + s.C, all = s.M * a.Hk * item;
@@ -177,6 +177,7 @@ __device__ __forceinline__ Deal find_share(Plan<RB>& plan, int seg, Walker<RB>& 
   __syncthreads();
   wk.b = s_req->x;
   wk.base = s_req->y;
+  if (wk.b >= a.B) wk.end = wk.x;  // (no share, and never a request that is not there)
   return deal;
 }
 
