@@ -185,33 +185,33 @@ template <typename T>
 __device__ __noinline__ void find_top(Shared& sh, const Row<T>& r, float m, int top) {
   constexpr int VE = Vec<T>::VE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (warp == 0) {  // the top-th largest of the threads' values, two bits at a time below what all have in common
-    uint32_t b[THREADS / 32], t, hi = 0, lo = ~0u;
+  if (warp == 0) {
+    // The top-th largest of 32 values, each the largest of 8 threads' (of 64 and 4 threads' for more than 16 alternatives):
+    // a value's place is the number of those before it, equal ones by lane.
+    float y[THREADS / 32];
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) {
-      b[i] = uint32_t(key_of(sh.last[32 * i + lane], 0) >> 32);
-      hi = max(hi, b[i]);
-      lo = min(lo, b[i]);
+    for (int i = 0; i < THREADS / 32; ++i) y[i] = sh.last[32 * i + lane];
+    float g0 = fmaxf(max3(y[0], y[1], y[2]), y[3]), g1 = fmaxf(max3(y[4], y[5], y[6]), y[7]);
+    const bool wide = top > 16;
+    if (!wide) g0 = fmaxf(g0, g1);
+    int at0 = 0, at1 = 0;
+#pragma unroll
+    for (int o = 1; o < 32; ++o) {
+      const float x = __shfl_xor_sync(0xffffffffu, g0, o);
+      at0 += x > g0 || (x == g0 && (lane ^ o) < lane);
     }
-    hi = __reduce_max_sync(0xffffffffu, hi);
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    const int from = hi == lo ? -2 : (31 - __clz(hi ^ lo)) & ~1;  // the pair of the first bit that differs
-    t = from < 0 ? hi : from == 30 ? 0u : hi >> (from + 2) << (from + 2);
-#pragma unroll 1
-    for (int bit = from; bit >= (sizeof(T) == 2 ? 12 : 0); bit -= 2) {
-      const uint32_t one = 1u << bit, y1 = t + one, y2 = t + 2 * one, y3 = t + 3 * one;
-      uint32_t n12 = 0, n3 = 0;
+    if (wide) {
+      at0 += g1 > g0;
+      at1 = g0 >= g1;
 #pragma unroll
-      for (int i = 0; i < THREADS / 32; ++i) {
-        n12 += (b[i] >= y1) + ((b[i] >= y2) << 16);
-        n3 += b[i] >= y3;
+      for (int o = 1; o < 32; ++o) {
+        const float x0 = __shfl_xor_sync(0xffffffffu, g0, o), x1 = __shfl_xor_sync(0xffffffffu, g1, o);
+        at0 += x1 > g0;
+        at1 += (x0 >= g1) + (x1 > g1 || (x1 == g1 && (lane ^ o) < lane));
       }
-      n12 = __reduce_add_sync(0xffffffffu, n12);
-      n3 = __reduce_add_sync(0xffffffffu, n3);
-      const uint32_t want = uint32_t(top);
-      t = n3 >= want ? y3 : (n12 >> 16) >= want ? y2 : (n12 & 0xffffu) >= want ? y1 : t;
     }
-    if (lane == 0) sh.bound = value_of(uint64_t(t) << 32);
+    if (at0 == top - 1) sh.bound = g0;
+    if (wide && at1 == top - 1) sh.bound = g1;
   }
   __syncthreads();
   const float bound = sh.bound;
@@ -474,30 +474,31 @@ __global__ void __launch_bounds__(THREADS, 5) score_kernel(const dspark_score_ar
     cluster_sync_all();
     if (part == 0) {
       if (TOP) {
-        const int n = cluster * a.top;  // at most CAND / 4
-        for (int i = tid; i < n; i += THREADS) {
-          const int q = i / a.top;
-          sh.cand[i] = remote_u64(&sh.top[i - q * a.top], q);
+        const int n = cluster * a.top;  // at most CAND / 2
+        if (tid < n) {
+          const int q = tid / a.top;
+          sh.cand[tid] = remote_u64(&sh.top[tid - q * a.top], q);
         }
-        __syncthreads();
-        place_top(sh, sh.cand, n, a.top, sh.cand + CAND / 2);
-        if (tid < a.top) {  // (nothing is left behind the last)
-          int live = 0;
-          for (int i = 0; i < n; ++i) live += sh.cand[i] != 0;
-          if (tid >= live) sh.cand[CAND / 2 + tid] = 0;
+        if (tid < a.top) sh.cand[CAND / 2 + tid] = 0;  // (nothing is left behind the last)
+      }
+      if (warp == THREADS / 32 - 1) {  // a lane a block
+        const uint32_t q = lane < cluster ? lane : 0, at = mapa_shared(smem_u32(&sh.sum), q);
+        Sums y{ld_dsmem_f32(at), ld_dsmem_f32(at + 4), ld_dsmem_f32(at + 8)};
+        int n = __float_as_int(ld_dsmem_f32(mapa_shared(smem_u32(&sh.before), q)));
+        for (int o = 1; o < cluster; o <<= 1) {
+          const Sums z1{__shfl_xor_sync(0xffffffffu, y.m, o), __shfl_xor_sync(0xffffffffu, y.l, o),
+                        __shfl_xor_sync(0xffffffffu, y.s, o)};
+          y = join<TEMP>(y, z1, c);
+          n += __shfl_xor_sync(0xffffffffu, n, o);
+        }
+        if (lane == 0) {
+          sh.sum = y;
+          sh.before = n;
         }
       }
-      if (tid == 0) {
-        Sums y = sh.sum;
-        int n = sh.before;
-        for (int q = 1; q < cluster; ++q) {
-          const uint32_t at = mapa_shared(smem_u32(&sh.sum), q);
-          const Sums o{ld_dsmem_f32(at), ld_dsmem_f32(at + 4), ld_dsmem_f32(at + 8)};
-          y = join<TEMP>(y, o, c);
-          n += __float_as_int(ld_dsmem_f32(mapa_shared(smem_u32(&sh.before), q)));
-        }
-        sh.sum = y;
-        sh.before = n;
+      if (TOP) {
+        __syncthreads();
+        place_top(sh, sh.cand, cluster * a.top, a.top, sh.cand + CAND / 2);
       }
     }
   }
@@ -531,10 +532,13 @@ __global__ void __launch_bounds__(THREADS, 5) score_kernel(const dspark_score_ar
 
 template <typename T>
 static cudaError_t launch(const dspark_score_args& a, cudaStream_t s) {
-  // blocks a row: one wave of blocks or more, slices of 4 KB or more
-  const int sms = sm_count(current_device());
+  // Blocks a row: as many as there is room for at once (five an SM), for two of them some more, in slices of 4 KB or
+  // more. 151,936 values in bf16 without / with 5 alternatives, us by blocks a row (1, 2, 4, 8): 74 rows 26 16 14 12 / 32 21 20
+  // 18, 110 rows 33 23 17 18 / 38 29 24 30, 200 rows 42 29 24 28 / 48 35 35 45, 296 rows 46 30 30 39 / 52 36 42 61, 500
+  // rows 50 43 45 61 / 57 55 62 95, 740 rows 52 55 63 86 / 59 69 88 136.
+  const int64_t sms = sm_count(current_device());
   int cluster = 1;
-  while (cluster < MAX_CLUSTER && int64_t(a.R) * cluster < 2 * sms &&
+  while (cluster < MAX_CLUSTER && int64_t(a.R) * cluster * 4 <= (cluster == 1 ? 14 : cluster == 2 ? 11 : 10) * sms &&
          int64_t(a.V) * int(sizeof(T)) >= int64_t(cluster) * 2 * 4096)
     cluster *= 2;
   const dim3 grid(unsigned(a.R) * cluster);

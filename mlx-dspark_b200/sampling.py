@@ -132,18 +132,23 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: t
     ld = _rows_of("logits", logits, R, V)
     if not 0 <= top <= 32:
         raise _lib.DSparkUnsupported(_lib.ERR_UNSUPPORTED, f"{top} alternatives (at most 32)")
-    if out is None:
-        f, i = (dict(dtype=t, device=logits.device) for t in (torch.float32, torch.int32))
-        out = {"logprob": torch.empty(R, **f), "entropy": torch.empty(R, **f), "rank": torch.empty(R, **i)}
+    if out is None:  # parts of one buffer
+        n = R * top
+        buf = torch.empty(3 * R + 2 * n, dtype=torch.float32, device=logits.device)
+        lp = buf.data_ptr()
+        ent, rank, ids, tl = lp + 4 * R, lp + 8 * R, lp + 12 * R, lp + 4 * (3 * R + n)
+        x = buf.split_with_sizes((R, R, R, n, n) if top else (R, R, R))
+        out = {"logprob": x[0], "entropy": x[1], "rank": x[2].view(torch.int32)}
         if top:
-            out["top_ids"], out["top_logprobs"] = torch.empty((R, top), **i), torch.empty((R, top), **f)
-    elif top and out.get("top_ids") is None or not top and "top_ids" in out:
-        raise _lib.DSparkError(_lib.ERR_ARG, f"out of another call: {top} alternatives, {sorted(out)}")
-    ids = tl = 0
-    if top:
-        ids, tl = int32("top_ids", out["top_ids"], R * top), _f32("top_logprobs", out["top_logprobs"], R * top)
+            out["top_ids"], out["top_logprobs"] = x[3].view(torch.int32).view(R, top), x[4].view(R, top)
+    else:
+        if top and out.get("top_ids") is None or not top and "top_ids" in out:
+            raise _lib.DSparkError(_lib.ERR_ARG, f"out of another call: {top} alternatives, {sorted(out)}")
+        lp, ent, rank = _f32("logprob", out["logprob"], R), _f32("entropy", out["entropy"], R), int32("rank", out["rank"], R)
+        ids = tl = 0
+        if top:
+            ids, tl = int32("top_ids", out["top_ids"], R * top), _f32("top_logprobs", out["top_logprobs"], R * top)
     _lib.check(_lib.lib.dspark_token_logprobs(_pack_score(
-        logits.data_ptr(), ld, int32("tokens", tokens, R), _f32("temperature", temperature, R),
-        _f32("logprob", out["logprob"], R), _f32("entropy", out["entropy"], R), int32("rank", out["rank"], R), ids, tl,
-        dt, R, V, top), stream))
+        logits.data_ptr(), ld, int32("tokens", tokens, R), _f32("temperature", temperature, R), lp, ent, rank,
+        ids if top else 0, tl if top else 0, dt, R, V, top), stream))
     return out
