@@ -9,7 +9,8 @@
 // or 32 rows of one (request, kv head), its work the key tiles (128 keys) that its last row sees. All items' costs
 // lie in one line (requests in order, a request's heads, a head's row blocks), which is cut into equal shares, one a
 // block of a resident grid, from the lengths on the device (shares, Walker). A block that has a whole item writes the
-// output; of a cut item each block leaves an fp32 part, and a second launch joins the parts in order.
+// output; of a cut item each block leaves an fp32 part, and a second launch joins the parts in order. Where a call has few
+// items, each is a cluster of blocks instead, which join their parts through shared memory.
 //
 // Block: four warps, each on its own: a warp takes every fourth subtile of 32 keys of the segment, with a ring of
 // its own in shared memory that it fills itself (16-byte cp.async, no block-wide wait in the loop), its own running
@@ -21,7 +22,7 @@
 // as large, so that what a long tail loses is below 2^-36 of the largest a key; scores, sums and O are fp32.
 //
 // Bound: HBM for decoded tokens (96 requests over 256 to 16k keys, 32/8 heads of 128, pages of 16: 137 to 153 us, 111.5 of
-// them the bytes at the measured rate), latency for one (2k keys 11.0 us, both launches). fp16 products, because the 8-bit
+// them the bytes at the measured rate), latency for one (2k keys 9.2 us). fp16 products, because the 8-bit
 // form of this instruction is as slow as a conversion of its operands and needs q and the weights in parts: 313 us.
 #include <algorithm>
 
@@ -77,20 +78,46 @@ __device__ __forceinline__ uint32_t at_chunk(int row, int c) {
 
 // ------------------------------------------------------------------ the kernel
 
-template <typename T, int D, int RT>
+// Item i of the line as one segment, for up to 32 requests. A warp together.
+template <int RB>
+__device__ __forceinline__ bool find_item(const Plan<RB>& p, int i, Segment& g) {
+  const dspark_paged_attn_args& a = p.a;
+  const int lane = threadIdx.x & 31;
+  const int n = lane < a.B ? p.shape(lane).M * a.Hk : 0;
+  int to = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, to, o);
+    if (lane >= o) to += y;
+  }
+  const unsigned past = __ballot_sync(0xffffffffu, i < to);
+  if (past == 0) return false;
+  const int b = __ffs(past) - 1;
+  i -= __shfl_sync(0xffffffffu, to - n, b);
+  const Shape s = p.shape(b);
+  const int h = i / s.M, m = i - h * s.M;
+  g = Segment{b, h, s.r0, s.rows, s.len, s.before, m * RB, min(s.rows * (a.Hq / a.Hk) - m * RB, RB), 0, p.tiles(s, m), 0, 1};
+  return true;
+}
+
+// CL = 1: a block takes its share of the line. CL > 1: a cluster an item, its warps in turn through the subtiles; the
+// blocks' parts are joined through their shared memory.
+template <typename T, int D, int RT, int CL>
 __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_args a, const float c_log2,
                                                        const uint32_t q_sign, int* status) {
   typedef Lay<D, RT> L;
   constexpr int RB = L::RB, KS = D / 16, CH = D / 16;  // k steps of the scores, 16-byte chunks a row
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint2 s_cost[WARPS], s_req;
+  __shared__ float s_lse[RB];  // (CL > 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, qd = lane & 3;  // row (or key) and quarter of an mma fragment
   pdl_launch_dependents();
   pdl_wait();
   Plan<RB> plan{a, 0};
   Walker<RB> wk;
-  const Deal deal = find_share<RB, NTHR>(plan, SEG, wk, s_cost, &s_req);
+  Deal deal(0, 1);
+  if (CL == 1) deal = find_share<RB, NTHR>(plan, SEG, wk, s_cost, &s_req);
   Cut cut{0, 0, 0, 0, 0, {0, 0, 0}};
 
   const int G = a.Hq / a.Hk, shift = 31 - __clz(a.page);
@@ -106,10 +133,13 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
   const bool packed = kts == D && vts == D;
   const uint32_t sw0 = at_chunk<D>(lane / CH, lane % CH), sw1 = at_chunk<D>(RPI + lane / CH, lane % CH) - RPI * D;
 
+  constexpr int STEP = CL * WARPS;  // subtiles between a warp's
   Segment s;
-  while (wk.next(plan, deal, s)) {
-    const int sub0 = s.t0 * (BN / SUB) + warp, sub1 = min(s.t1 * (BN / SUB), (s.len + SUB - 1) / SUB);
-    const int n = sub0 < sub1 ? (sub1 - sub0 + WARPS - 1) / WARPS : 0;
+  bool more = CL == 1 ? wk.next(plan, deal, s) : find_item(plan, int(blockIdx.x) / CL, s);
+  while (more) {
+    const int sub0 = s.t0 * (BN / SUB) + (CL == 1 ? 0 : int(blockIdx.x) % CL * WARPS) + warp;
+    const int sub1 = min(s.t1 * (BN / SUB), (s.len + SUB - 1) / SUB);
+    const int n = sub0 < sub1 ? (sub1 - sub0 + STEP - 1) / STEP : 0;
     const int32_t* table = a.page_table + int64_t(s.b) * a.table_stride;
     // the lane's first 16 bytes of a subtile; the next are RPI tokens on
     const uint8_t* kp = static_cast<const uint8_t*>(a.k_pages) + s.h * a.kp_strides[1] + lane / CH * kts + lane % CH * 16;
@@ -118,7 +148,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
     // The pages of 16 subtiles' halves, a half a lane (-1 where there is none to read): read 16 subtiles ahead.
     auto page_ids = [&](int i0) {
       int id = -1;
-      const int i = i0 + (lane >> 1), key = (sub0 + i * WARPS) * SUB + (lane & 1) * 16;
+      const int i = i0 + (lane >> 1), key = (sub0 + i * STEP) * SUB + (lane & 1) * 16;
       if (i < n && key < s.len) {
         id = table[key >> shift];
         if (id < 0 || id >= a.n_pages) {
@@ -136,7 +166,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
           later = page_ids(i + 16);
         }
         const uint32_t dst = ring_a + (i % L::NS) * L::STAGE;
-        const int key0 = (sub0 + i * WARPS) * SUB;
+        const int key0 = (sub0 + i * STEP) * SUB;
         const int id0 = __shfl_sync(0xffffffffu, ids, (i & 15) * 2), id1 = __shfl_sync(0xffffffffu, ids, (i & 15) * 2 + 1);
         if (lane < 2) {
           const int mine = lane ? id1 : id0;
@@ -254,7 +284,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
       asm volatile("cp.async.wait_group %0;" ::"n"(L::NS - 2) : "memory");
       __syncwarp();
       issue(i + L::NS - 1);
-      const int key0 = (sub0 + i * WARPS) * SUB;
+      const int key0 = (sub0 + i * STEP) * SUB;
       const uint32_t kt = ring_a + (i % L::NS) * L::STAGE, vt = kt + L::TILE;
       const float2 sc0 = *reinterpret_cast<const float2*>(ring + (i % L::NS) * L::STAGE + 2 * L::TILE);
       const float2 sc1 = *reinterpret_cast<const float2*>(ring + (i % L::NS) * L::STAGE + 2 * L::TILE + 8);
@@ -437,10 +467,10 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
       }
     }
     __syncthreads();
-    const bool whole = s.parts == 1;
+    const bool whole = CL == 1 && s.parts == 1;
     const int which = int(blockIdx.x) == s.first;
-    float* part = whole ? nullptr : part_of<D, RB>(a.workspace, blockIdx.x, which);
-    if (!whole && which) cut = Cut{s.parts, s.r0, s.live, s.row_base, s.h, {0, 0, 0}};
+    float* part = CL > 1 || whole ? nullptr : part_of<D, RB>(a.workspace, blockIdx.x, which);
+    if (CL == 1 && !whole && which) cut = Cut{s.parts, s.r0, s.live, s.row_base, s.h, {0, 0, 0}};
 #pragma unroll 4
     for (int z = tid; z < RB * (D / 4); z += NTHR) {
       const int r = z / (D / 4), d = z % (D / 4) * 4;
@@ -471,36 +501,102 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
         const int node = (s.row_base + r) / G, hq = s.h * G + s.row_base + r - node * G;
         T* out = static_cast<T*>(a.out) + int64_t(s.r0 + node) * a.o_strides[0] + hq * a.o_strides[1] + d;
         *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w));
+      } else if (CL > 1) {  // in the place of the first warp's
+        *reinterpret_cast<float4*>(merge + r * (D + 4) + d) = v;
+        if (d == 0) s_lse[r] = sum == 0.f ? -INFINITY : ref + lg2(sum);
       } else {
         *reinterpret_cast<float4*>(part + r * D + d) = v;
         if (d == 0) part[RB * D + r] = sum == 0.f ? -INFINITY : ref + lg2(sum);
       }
     }
-    __syncthreads();  // the rings and Q are free again
+    if (CL > 1) {
+      cluster_sync_all();
+#pragma unroll
+      for (int z0 = 0; z0 < RB * (D / 4); z0 += CL * NTHR) {
+        const int z = z0 + int(blockIdx.x) % CL * NTHR + tid, r = z / (D / 4), d = z % (D / 4) * 4;
+        if (r >= min(s.live, RB)) break;
+        float y[CL], top = -INFINITY, sum = 0.f;
+        float4 u[CL], v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int q = 0; q < CL; ++q) {
+          y[q] = ld_dsmem_f32(mapa_shared(smem_u32(s_lse + r), q));
+          u[q] = ld_dsmem_f4(mapa_shared(smem_u32(merge + r * (D + 4) + d), q));
+        }
+#pragma unroll
+        for (int q = 0; q < CL; ++q) top = fmaxf(top, y[q]);
+        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int q = 0; q < CL; ++q) {
+          const float f = ex2(y[q] - ref);  // (a part that saw nothing: 0, and its values are)
+          sum += f;
+          v.x = fmaf(u[q].x, f, v.x);
+          v.y = fmaf(u[q].y, f, v.y);
+          v.z = fmaf(u[q].z, f, v.z);
+          v.w = fmaf(u[q].w, f, v.w);
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int node = (s.row_base + r) / G, hq = s.h * G + s.row_base + r - node * G;
+        T* out = static_cast<T*>(a.out) + int64_t(s.r0 + node) * a.o_strides[0] + hq * a.o_strides[1] + d;
+        *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack(v.x * inv, v.y * inv), Elem<T>::pack(v.z * inv, v.w * inv));
+      }
+      cluster_sync_all();  // the others have read this block's part
+    } else {
+      __syncthreads();  // the rings and Q are free again
+    }
+    more = CL == 1 && wk.next(plan, deal, s);
   }
-  if (tid == 0) static_cast<Cut*>(a.workspace)[blockIdx.x] = cut;
+  if (CL == 1 && tid == 0) static_cast<Cut*>(a.workspace)[blockIdx.x] = cut;
 }
 
 static int grid_of(int device, int per_sm) { return std::min(per_sm * sm_count(device), MAX_CTA); }
 
-template <typename T, int D, int RT>
+// Items of a call at most.
+static int64_t most_items(const dspark_paged_attn_args& a, int rb) {
+  return (int64_t(a.R) * (a.Hq / a.Hk) + int64_t(a.B) * (rb - 1)) / rb * a.Hk;
+}
+
+template <typename T, int D, int RT, int CL>
 static int launch(const dspark_paged_attn_args& a, cudaStream_t s) {
   typedef Lay<D, RT> L;
-  const int dev = current_device(), n = grid_of(dev, L::PER_SM);
-  DSPARK_CUDA_TRY(configure_once((const void*)attn_kernel<T, D, RT>, L::TOTAL,
+  const int dev = current_device(), n = CL > 1 ? int(most_items(a, L::RB)) * CL : grid_of(dev, L::PER_SM);
+  auto kernel = attn_kernel<T, D, RT, CL>;
+  DSPARK_CUDA_TRY(configure_once((const void*)kernel, L::TOTAL,
                                  [&] {
-                                   return cudaFuncSetAttribute(attn_kernel<T, D, RT>,
-                                                               cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
+                                   if (CL > 8) {
+                                     const cudaError_t e =
+                                         cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+                                     if (e != cudaSuccess) return e;
+                                   }
+                                   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
                                  }),
                   "paged_attn: shared memory");
   // the running maximum needs a positive factor: a negative scale goes into q (none is below 1e-35, with which all weights
   // are equal)
   const float c = fabsf(a.scale) * 1.4426950408889634f;
-  DSPARK_CUDA_TRY(launch_ex(attn_kernel<T, D, RT>, dim3(n), dim3(NTHR), L::TOTAL, s, 1, true, a, c,
-                            a.scale < 0.f ? 0x80008000u : 0u, status_word(dev)),
+  DSPARK_CUDA_TRY(launch_ex(kernel, dim3(n), dim3(NTHR), L::TOTAL, s, CL, true, a, c, a.scale < 0.f ? 0x80008000u : 0u,
+                            status_word(dev)),
                   "paged_attn");
-  DSPARK_CUDA_TRY(launch_ex(join_kernel<T, D, L::RB>, dim3(n, L::RB / 4), dim3(128), 0, s, 1, true, a), "paged_attn: join");
+  if (CL == 1)
+    DSPARK_CUDA_TRY(launch_ex(join_kernel<T, D, L::RB>, dim3(n, L::RB / 4), dim3(128), 0, s, 1, true, a), "paged_attn: join");
   return DSPARK_OK;
+}
+
+// Which calls go to clusters, without a second launch: those whose items (a request's rows taken as the average) all run at
+// once, over keys that a cluster is done with soon. Clusters of 16 begin a microsecond later, and more than
+// a block an SM of them not all at once (16 items over 1k keys 13.7): for few items with more than three subtiles a warp in
+// clusters of 8. One launch and a join / clusters of
+// 8 / of 16, us, 32/8 heads of 128: one row over 1k keys 9.1 / 6.6 / 7.9, 2049 11.0 / 9.2 / 9.5, 4k 12.0 / 10.5 / 9.6, 8k 15.7 /
+// 15.5 / 12.6, 16k 19.8 / 24.9 / 19.2; 4 requests of 8 rows over 2k 22.6 / 16.0, 16k 51.3 / 45.6, 32k 78.8 / 78.2.
+constexpr int CLUSTER_KEYS = 8192;
+template <typename T, int D, int RT>
+static int launch_few(const dspark_paged_attn_args& a, cudaStream_t s) {
+  const int64_t sms = sm_count(current_device()), rows = (int64_t(a.R) * (a.Hq / a.Hk) + a.B - 1) / a.B;
+  const int64_t items = (rows + 16 * RT - 1) / (16 * RT) * a.B * a.Hk, keys = int64_t(a.max_pages) * a.page;
+  if (a.B <= 32) {
+    if (items * 16 <= sms && keys > 3 * 8 * WARPS * SUB && keys <= 2 * CLUSTER_KEYS) return launch<T, D, RT, 16>(a, s);
+    if (items * 8 <= 2 * sms && keys <= (items * 8 > sms ? 4 : 1) * CLUSTER_KEYS) return launch<T, D, RT, 8>(a, s);
+  }
+  return launch<T, D, RT, 1>(a, s);
 }
 
 // Which calls go to the 5th-generation tensor cores (paged_wide.cu): those with more than 32 rows a request and kv head on
@@ -524,7 +620,7 @@ static int launch_rows(const dspark_paged_attn_args& a, cudaStream_t s) {
     if (rc != NO_MAP) return rc;  // (the workspace is enough for either)
   }
   // rows of a product: 16 where requests have no more on average
-  return int64_t(a.R) * (a.Hq / a.Hk) <= int64_t(16) * a.B ? launch<T, D, 1>(a, s) : launch<T, D, 2>(a, s);
+  return int64_t(a.R) * (a.Hq / a.Hk) <= int64_t(16) * a.B ? launch_few<T, D, 1>(a, s) : launch_few<T, D, 2>(a, s);
 }
 
 }  // namespace paged
