@@ -21,8 +21,8 @@
 // Rounding: q is used as fp16, bf16 rows scaled by a power of two (exact); weights p' are rounded to fp16, 2^11 times
 // as large, so that what a long tail loses is below 2^-36 of the largest a key; scores, sums and O are fp32.
 //
-// Bound: HBM for decoded tokens (96 requests over 256 to 16k keys, 32/8 heads of 128, pages of 16: 137 to 153 us, 111.5 of
-// them the bytes at the measured rate), latency for one (2k keys 9.2 us). fp16 products, because the 8-bit
+// Bound: HBM for decoded tokens (96 requests over 256 to 16k keys, 32/8 heads of 128, pages of 16: 128 us, 111.5 of
+// them the bytes at the measured rate), latency for one (2k keys 8.7 us). fp16 products, because the 8-bit
 // form of this instruction is as slow as a conversion of its operands and needs q and the weights in parts: 313 us.
 #include <algorithm>
 
@@ -35,7 +35,9 @@ namespace paged {
 constexpr int SUB = 32;      // keys a warp's subtile
 constexpr int WARPS = 4;
 constexpr int NTHR = WARPS * 32;
-constexpr int SEG = 5;       // cost of a segment, in tiles
+// Cost of a segment, in tiles. Us for 2, 3, 4, 5: 96 decoded tokens over 256 to 16k keys 131, 128, 131, 133, 200 over 256 to 4k
+// 113, 114, 117, 121, 64 blocks of 1 to 8 rows over 256 to 2k 63, 61, 62, 62.
+constexpr int SEG = 3;
 constexpr float LIFT = 11.f; // weights are 2^11 times as large in fp16 ...
 constexpr float SLACK = 4.f; // ... and the maximum in use may be 2^4 too low
 
@@ -51,10 +53,11 @@ struct Lay {
   static constexpr int QF = Q + RB * D * 2;           // the rows' powers of two
   static constexpr int ML = QF + RB * 4;              // (m, l) [warp][row]
   static constexpr int BUF = ML + WARPS * RB * 8;
-  static constexpr int O = WARPS * RB * (D + 4) * 4;  // O [warp][row][D + 4] takes the rings' place
-  static constexpr int SIZE = WARPS * RING > O ? WARPS * RING : O;
-  static constexpr int TOTAL = BUF + SIZE;
+  static constexpr int AHEAD = NS - RT;               // loads of the next segment while a warp's O [row][D] is in the other buffers
+  static constexpr int O = AHEAD * STAGE;             // ... in its ring, from here
+  static constexpr int TOTAL = BUF + WARPS * RING;
   static_assert(BUF % 16 == 0 && STAGE % 16 == 0, "16-byte copies");
+  static_assert(O + RB * D * 4 <= RING, "O");
 };
 
 __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -126,7 +129,10 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
   const uint32_t q_a = smem_u32(smem + L::Q) + lane * 16;
   float* rowf = reinterpret_cast<float*>(smem + L::QF);
   float2* ml = reinterpret_cast<float2*>(smem + L::ML);
-  float* merge = reinterpret_cast<float*>(smem + L::BUF);
+  // float4 d / 4 of row r of a warp's O
+  auto merge = [&](int w, int r, int d) {
+    return reinterpret_cast<float4*>(smem + L::BUF + w * L::RING + L::O) + (r * (D / 4) + (d / 4 ^ (r & 1) << 2));
+  };
 
   constexpr int RPI = 32 / CH, ROUNDS = SUB / RPI;  // tokens a round of 16-byte copies, rounds a subtile
   const int kts = int(a.kp_strides[2]), vts = int(a.vp_strides[2]);
@@ -134,96 +140,125 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
   const uint32_t sw0 = at_chunk<D>(lane / CH, lane % CH), sw1 = at_chunk<D>(RPI + lane / CH, lane % CH) - RPI * D;
 
   constexpr int STEP = CL * WARPS;  // subtiles between a warp's
+  // The segment whose subtiles are on their way: the one in work, from its end on the next one.
+  int sub0 = 0, n = 0, len = 0, ids = -1, later = -1;
+  const int32_t* table = nullptr;
+  const uint8_t *kp = nullptr, *vp = nullptr;
+  const float *ksc = nullptr, *vsc = nullptr;
+  // The pages of 16 subtiles' halves, a half a lane (-1 where there is none to read): read 16 subtiles ahead.
+  auto page_ids = [&](int i0) {
+    int id = -1;
+    const int i = i0 + (lane >> 1), key = (sub0 + i * STEP) * SUB + (lane & 1) * 16;
+    if (i < n && key < len) {
+      id = table[key >> shift];
+      if (id < 0 || id >= a.n_pages) {
+        report_error(status, kErrAttnPage);
+        id = -1;
+      }
+    }
+    return id;
+  };
+  auto issue = [&](int i) {
+    if (i < n) {
+      if (i > 0 && (i & 15) == 0) {
+        ids = later;
+        later = page_ids(i + 16);
+      }
+      const uint32_t dst = ring_a + (i % L::NS) * L::STAGE;
+      const int key0 = (sub0 + i * STEP) * SUB;
+      const int id0 = __shfl_sync(0xffffffffu, ids, (i & 15) * 2), id1 = __shfl_sync(0xffffffffu, ids, (i & 15) * 2 + 1);
+      if (lane < 2) {
+        const int mine = lane ? id1 : id0;
+        const int64_t at_s = mine < 0 ? 0 : int64_t(mine) * a.scale_strides[0];
+        const uint32_t to = dst + 2 * L::TILE + lane * 8;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(ksc + at_s), "r"(mine < 0 ? 0 : 4)
+                     : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 4), "l"(vsc + at_s),
+                     "r"(mine < 0 ? 0 : 4)
+                     : "memory");
+      }
+      const int mask = a.page - 1;
+      const uint8_t* k0 = kp + (id0 * a.kp_strides[0] + (key0 & mask) * a.kp_strides[2]);
+      const uint8_t* v0 = vp + (id0 * a.vp_strides[0] + (key0 & mask) * a.vp_strides[2]);
+      const uint8_t* k1 = kp + (id1 * a.kp_strides[0] + ((key0 + 16) & mask) * a.kp_strides[2]);
+      const uint8_t* v1 = vp + (id1 * a.vp_strides[0] + ((key0 + 16) & mask) * a.vp_strides[2]);
+      const bool whole = key0 + SUB <= len && id0 >= 0 && id1 >= 0;
+      if (whole && packed) {  // the usual case: no address arithmetic a copy
+#pragma unroll
+        for (int z = 0; z < ROUNDS; ++z) {
+          const uint32_t to = dst + z * RPI * D + (z & 1 ? sw1 : sw0);
+          cp_async_16(to, (z < ROUNDS / 2 ? k0 : k1) + z % (ROUNDS / 2) * RPI * D);
+          cp_async_16(to + L::TILE, (z < ROUNDS / 2 ? v0 : v1) + z % (ROUNDS / 2) * RPI * D);
+        }
+      } else {
+#pragma unroll 1
+        for (int z = 0; z < ROUNDS; ++z) {
+          const uint32_t to = dst + z * RPI * D + (z & 1 ? sw1 : sw0);
+          const int y = z % (ROUNDS / 2) * RPI;
+          const uint8_t* k = (z < ROUNDS / 2 ? k0 : k1) + y * kts;
+          const uint8_t* v = (z < ROUNDS / 2 ? v0 : v1) + y * vts;
+          const bool there = whole || ((z < ROUNDS / 2 ? id0 : id1) >= 0 && key0 + z * RPI + lane / CH < len);
+          cp_async_16_zfill(to, there ? k : kp, there);
+          cp_async_16_zfill(to + L::TILE, there ? v : vp, there);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto start = [&](const Segment& g) {
+    sub0 = g.t0 * (BN / SUB) + (CL == 1 ? 0 : int(blockIdx.x) % CL * WARPS) + warp;
+    const int sub1 = min(g.t1 * (BN / SUB), (g.len + SUB - 1) / SUB);
+    n = sub0 < sub1 ? (sub1 - sub0 + STEP - 1) / STEP : 0;
+    len = g.len;
+    table = a.page_table + int64_t(g.b) * a.table_stride;
+    // the lane's first 16 bytes of a subtile; the next are RPI tokens on
+    kp = static_cast<const uint8_t*>(a.k_pages) + g.h * a.kp_strides[1] + lane / CH * kts + lane % CH * 16;
+    vp = static_cast<const uint8_t*>(a.v_pages) + g.h * a.vp_strides[1] + lane / CH * vts + lane % CH * 16;
+    ksc = a.k_scale + g.h * a.scale_strides[1];
+    vsc = a.v_scale + g.h * a.scale_strides[1];
+    ids = page_ids(0);
+    later = page_ids(16);
+    __syncwarp();  // the last segment's buffers have been read
+#pragma unroll
+    for (int i = 0; i < L::AHEAD; ++i) issue(i);
+  };
+
+  // 16 neighbouring values of a row of Q a thread and round; of 16 rows a segment ahead (of 32 the registers are not there:
+  // 62.4 us for 61.3).
+  constexpr bool Q_AHEAD = RT == 1;
+  constexpr int PER = D / 16, Q_ROUNDS = (RB * PER + NTHR - 1) / NTHR;  // threads a row
+  uint4 q0[Q_ROUNDS], q1[Q_ROUNDS];
+  auto fetch_q = [&](const Segment& g) {
+#pragma unroll
+    for (int z = 0; z < Q_ROUNDS; ++z) {
+      const int r = (z * NTHR + tid) / PER, p = tid % PER;
+      q0[z] = q1[z] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < min(g.live, RB)) {
+        const int node = (g.row_base + r) / G, hq = g.h * G + g.row_base + r - node * G;
+        const T* q = static_cast<const T*>(a.q) + int64_t(g.r0 + node) * a.q_strides[0] + hq * a.q_strides[1] + p * 16;
+        q0[z] = ldcg_v4(q);
+        q1[z] = ldcg_v4(q + 8);
+      }
+    }
+  };
+
   Segment s;
   bool more = CL == 1 ? wk.next(plan, deal, s) : find_item(plan, int(blockIdx.x) / CL, s);
+  if (more) {
+    start(s);
+    if (Q_AHEAD) fetch_q(s);
+  }
   while (more) {
-    const int sub0 = s.t0 * (BN / SUB) + (CL == 1 ? 0 : int(blockIdx.x) % CL * WARPS) + warp;
-    const int sub1 = min(s.t1 * (BN / SUB), (s.len + SUB - 1) / SUB);
-    const int n = sub0 < sub1 ? (sub1 - sub0 + STEP - 1) / STEP : 0;
-    const int32_t* table = a.page_table + int64_t(s.b) * a.table_stride;
-    // the lane's first 16 bytes of a subtile; the next are RPI tokens on
-    const uint8_t* kp = static_cast<const uint8_t*>(a.k_pages) + s.h * a.kp_strides[1] + lane / CH * kts + lane % CH * 16;
-    const uint8_t* vp = static_cast<const uint8_t*>(a.v_pages) + s.h * a.vp_strides[1] + lane / CH * vts + lane % CH * 16;
-
-    // The pages of 16 subtiles' halves, a half a lane (-1 where there is none to read): read 16 subtiles ahead.
-    auto page_ids = [&](int i0) {
-      int id = -1;
-      const int i = i0 + (lane >> 1), key = (sub0 + i * STEP) * SUB + (lane & 1) * 16;
-      if (i < n && key < s.len) {
-        id = table[key >> shift];
-        if (id < 0 || id >= a.n_pages) {
-          report_error(status, kErrAttnPage);
-          id = -1;
-        }
-      }
-      return id;
-    };
-    int ids = page_ids(0), later = page_ids(16);
-    auto issue = [&](int i) {
-      if (i < n) {
-        if (i > 0 && (i & 15) == 0) {
-          ids = later;
-          later = page_ids(i + 16);
-        }
-        const uint32_t dst = ring_a + (i % L::NS) * L::STAGE;
-        const int key0 = (sub0 + i * STEP) * SUB;
-        const int id0 = __shfl_sync(0xffffffffu, ids, (i & 15) * 2), id1 = __shfl_sync(0xffffffffu, ids, (i & 15) * 2 + 1);
-        if (lane < 2) {
-          const int mine = lane ? id1 : id0;
-          const int64_t at_s = mine < 0 ? 0 : int64_t(mine) * a.scale_strides[0] + s.h * a.scale_strides[1];
-          const uint32_t to = dst + 2 * L::TILE + lane * 8;
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(a.k_scale + at_s), "r"(mine < 0 ? 0 : 4)
-                       : "memory");
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 4), "l"(a.v_scale + at_s),
-                       "r"(mine < 0 ? 0 : 4)
-                       : "memory");
-        }
-        const int mask = a.page - 1;
-        const uint8_t* k0 = kp + (id0 * a.kp_strides[0] + (key0 & mask) * a.kp_strides[2]);
-        const uint8_t* v0 = vp + (id0 * a.vp_strides[0] + (key0 & mask) * a.vp_strides[2]);
-        const uint8_t* k1 = kp + (id1 * a.kp_strides[0] + ((key0 + 16) & mask) * a.kp_strides[2]);
-        const uint8_t* v1 = vp + (id1 * a.vp_strides[0] + ((key0 + 16) & mask) * a.vp_strides[2]);
-        const bool whole = key0 + SUB <= s.len && id0 >= 0 && id1 >= 0;
-        if (whole && packed) {  // the usual case: no address arithmetic a copy
 #pragma unroll
-          for (int z = 0; z < ROUNDS; ++z) {
-            const uint32_t to = dst + z * RPI * D + (z & 1 ? sw1 : sw0);
-            cp_async_16(to, (z < ROUNDS / 2 ? k0 : k1) + z % (ROUNDS / 2) * RPI * D);
-            cp_async_16(to + L::TILE, (z < ROUNDS / 2 ? v0 : v1) + z % (ROUNDS / 2) * RPI * D);
-          }
-        } else {
-#pragma unroll 1
-          for (int z = 0; z < ROUNDS; ++z) {
-            const uint32_t to = dst + z * RPI * D + (z & 1 ? sw1 : sw0);
-            const int y = z % (ROUNDS / 2) * RPI;
-            const uint8_t* k = (z < ROUNDS / 2 ? k0 : k1) + y * kts;
-            const uint8_t* v = (z < ROUNDS / 2 ? v0 : v1) + y * vts;
-            const bool there = whole || ((z < ROUNDS / 2 ? id0 : id1) >= 0 && key0 + z * RPI + lane / CH < s.len);
-            cp_async_16_zfill(to, there ? k : kp, there);
-            cp_async_16_zfill(to + L::TILE, there ? v : vp, there);
-          }
-        }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-#pragma unroll
-    for (int i = 0; i < L::NS - 1; ++i) issue(i);
+    for (int i = L::AHEAD; i < L::NS - 1; ++i) issue(i);
 
-    // ---- Q as fp16 fragments. 16 neighbouring values of a row a thread and round.
+    // ---- Q as fp16 fragments
+    if (!Q_AHEAD) fetch_q(s);
     {
-      constexpr int PER = D / 16;  // threads a row
 #pragma unroll
-      for (int z = 0; z < RB * PER / NTHR + (RB * PER % NTHR ? 1 : 0); ++z) {
+      for (int z = 0; z < Q_ROUNDS; ++z) {
         const int r = (z * NTHR + tid) / PER, p = tid % PER;
-        uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        const bool mine = r < RB && r < s.live;
-        if (mine) {
-          const int node = (s.row_base + r) / G, hq = s.h * G + s.row_base + r - node * G;
-          const T* q = static_cast<const T*>(a.q) + int64_t(s.r0 + node) * a.q_strides[0] + hq * a.q_strides[1] + p * 16;
-          const uint4 x0 = ldcg_v4(q), x1 = ldcg_v4(q + 8);
-          w[0] = x0.x; w[1] = x0.y; w[2] = x0.z; w[3] = x0.w;
-          w[4] = x1.x; w[5] = x1.y; w[6] = x1.z; w[7] = x1.w;
-        }
+        uint32_t w[8] = {q0[z].x, q0[z].y, q0[z].z, q0[z].w, q1[z].x, q1[z].y, q1[z].z, q1[z].w};
         float f = 1.f;
         if (std::is_same<T, bf16>::value) {  // largest exponent of the row; 255: infinite or NaN
           uint32_t e = 0;
@@ -447,9 +482,13 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
       }
     }
 
-    // ---- the warps' parts joined
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();
+    // ---- the warps' parts joined, the next segment's first subtiles on their way
+    Segment next;
+    const bool again = CL == 1 && wk.next(plan, deal, next);
+    if (again) {
+      start(next);
+      if (Q_AHEAD) fetch_q(next);
+    }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
@@ -459,11 +498,10 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
         y += __shfl_xor_sync(0xffffffffu, y, 2);
         const int r = rt * 16 + k * 8 + g;
         if (qd == 0) ml[warp * RB + r] = make_float2(m[rt][k], y);
-        float* to = merge + (warp * RB + r) * (D + 4) + 4 * qd;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
-          *reinterpret_cast<float4*>(to + 16 * c) = make_float4(o[rt][2 * c][2 * k], o[rt][2 * c + 1][2 * k],
-                                                                o[rt][2 * c][2 * k + 1], o[rt][2 * c + 1][2 * k + 1]);
+          *merge(warp, r, 16 * c + 4 * qd) = make_float4(o[rt][2 * c][2 * k], o[rt][2 * c + 1][2 * k],
+                                                         o[rt][2 * c][2 * k + 1], o[rt][2 * c + 1][2 * k + 1]);
       }
     }
     __syncthreads();
@@ -488,7 +526,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
         const float f = ex2(y[w].x - ref);
-        const float4 u = *reinterpret_cast<const float4*>(merge + (w * RB + r) * (D + 4) + d);
+        const float4 u = *merge(w, r, d);
         sum += y[w].y * f;
         v.x += u.x * f;
         v.y += u.y * f;
@@ -502,7 +540,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
         T* out = static_cast<T*>(a.out) + int64_t(s.r0 + node) * a.o_strides[0] + hq * a.o_strides[1] + d;
         *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w));
       } else if (CL > 1) {  // in the place of the first warp's
-        *reinterpret_cast<float4*>(merge + r * (D + 4) + d) = v;
+        *merge(0, r, d) = v;
         if (d == 0) s_lse[r] = sum == 0.f ? -INFINITY : ref + lg2(sum);
       } else {
         *reinterpret_cast<float4*>(part + r * D + d) = v;
@@ -520,7 +558,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
 #pragma unroll
         for (int q = 0; q < CL; ++q) {
           y[q] = ld_dsmem_f32(mapa_shared(smem_u32(s_lse + r), q));
-          u[q] = ld_dsmem_f4(mapa_shared(smem_u32(merge + r * (D + 4) + d), q));
+          u[q] = ld_dsmem_f4(mapa_shared(smem_u32(merge(0, r, d)), q));
         }
 #pragma unroll
         for (int q = 0; q < CL; ++q) top = fmaxf(top, y[q]);
@@ -541,9 +579,10 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
       }
       cluster_sync_all();  // the others have read this block's part
     } else {
-      __syncthreads();  // the rings and Q are free again
+      __syncthreads();  // the buffers of O and Q are free again
     }
-    more = CL == 1 && wk.next(plan, deal, s);
+    more = again;
+    if (again) s = next;
   }
   if (CL == 1 && tid == 0) static_cast<Cut*>(a.workspace)[blockIdx.x] = cut;
 }
