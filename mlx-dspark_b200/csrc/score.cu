@@ -12,7 +12,8 @@
 //
 // A row is a cluster of 1 to 8 blocks, each with a slice of its 16-byte vectors; the first block joins them.
 // Bound: HBM and the exponentials' unit for many rows (2049 of 151,936 in bf16 124 us, 0.77 of the measured rate; 272 in
-// fp32 with 20 alternatives 48.7, 0.52, for the search and an uneven last round), latency for few (one row 10.7). A ring of
+// fp32 with 20 alternatives 42.4, 0.59, for the search of alternatives, which no other block's pass covers), latency for few
+// (one row 8.7). A ring of
 // bulk copies in shared memory in place of plain loads: 132 beside 132, one row 14.
 #include <algorithm>
 #include <cfloat>
@@ -292,9 +293,10 @@ struct Taken {
   int tok, before;
 };
 
-// N vectors of a thread (masked values kLow); vm[u] is the largest of x[u], tk + u * step the token of x[u][0].
+// N vectors of a thread (masked values kLow); vm[u] is the largest of x[u], tk + u * step the token of x[u][0]. Returns the
+// largest of all.
 template <typename T, bool TEMP, int N>
-__device__ __forceinline__ void take(Taken& t, float (&x)[N][Vec<T>::VE], float (&vm)[N], int tk, int step) {
+__device__ __forceinline__ float take(Taken& t, float (&x)[N][Vec<T>::VE], float (&vm)[N], int tk, int step) {
   constexpr int VE = Vec<T>::VE;
   float bm = vm[0];
 #pragma unroll
@@ -344,10 +346,11 @@ __device__ __forceinline__ void take(Taken& t, float (&x)[N][Vec<T>::VE], float 
   t.z.l += a0 + a1;
   unpack2(s2, a0, a1);
   t.z.s += a0 + a1;
+  return bm;
 }
 
-template <typename T, bool TOP, bool TEMP>
-__global__ void __launch_bounds__(THREADS, 5) score_kernel(const dspark_score_args a, const int cluster) {
+template <typename T, bool TOP, bool TEMP, int PER_SM>
+__global__ void __launch_bounds__(THREADS, PER_SM) score_kernel(const dspark_score_args a, const int cluster) {
   constexpr int VE = Vec<T>::VE;
   __shared__ Shared sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -411,13 +414,9 @@ __global__ void __launch_bounds__(THREADS, 5) score_kernel(const dspark_score_ar
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) vm[u] = Vec<T>::split(w[u], x[u]);
-    take<T, TEMP, U>(t, x, vm, tk, THREADS * VE);
-    if (TOP) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) part_max = fmaxf(part_max, vm[u]);
-    }
+    part_max = fmaxf(part_max, take<T, TEMP, U>(t, x, vm, tk, THREADS * VE));
     if (TOP && (--left == 0 || k + 1 == r.chunks)) {
-      sh.maxima[k / r.part][tid] = fminf(part_max, Vec<T>::MAXV);
+      sh.maxima[k / r.part][tid] = part_max;
       part_max = kLow;
       left = r.part;
     }
@@ -530,10 +529,16 @@ __global__ void __launch_bounds__(THREADS, 5) score_kernel(const dspark_score_ar
   if (cluster > 1) cluster_sync_all();  // the first block has read the others' shared memory
 }
 
+template <typename T, int PER_SM>
+static cudaError_t launch_as(const dspark_score_args& a, int cluster, cudaStream_t s) {
+  auto kernel = a.top ? (a.temperature ? score_kernel<T, true, true, PER_SM> : score_kernel<T, true, false, PER_SM>)
+                      : (a.temperature ? score_kernel<T, false, true, PER_SM> : score_kernel<T, false, false, PER_SM>);
+  return launch_ex(kernel, dim3(unsigned(a.R) * cluster), dim3(THREADS), 0, s, cluster, true, a, cluster);
+}
+
 template <typename T>
 static cudaError_t launch(const dspark_score_args& a, cudaStream_t s) {
-  // Blocks a row: as many as there is room for at once (five an SM), for two of them some more, in slices of 4 KB or
-  // more. 151,936 values in bf16 without / with 5 alternatives, us by blocks a row (1, 2, 4, 8): 74 rows 26 16 14 12 / 32 21 20
+  // Blocks a row: as many as there is room for at once, for two of them some more, in slices of 4 KB or more. 151,936 values in bf16 without / with 5 alternatives, us by blocks a row (1, 2, 4, 8): 74 rows 26 16 14 12 / 32 21 20
   // 18, 110 rows 33 23 17 18 / 38 29 24 30, 200 rows 42 29 24 28 / 48 35 35 45, 296 rows 46 30 30 39 / 52 36 42 61, 500
   // rows 50 43 45 61 / 57 55 62 95, 740 rows 52 55 63 86 / 59 69 88 136.
   const int64_t sms = sm_count(current_device());
@@ -541,10 +546,12 @@ static cudaError_t launch(const dspark_score_args& a, cudaStream_t s) {
   while (cluster < MAX_CLUSTER && int64_t(a.R) * cluster * 4 <= (cluster == 1 ? 14 : cluster == 2 ? 11 : 10) * sms &&
          int64_t(a.V) * int(sizeof(T)) >= int64_t(cluster) * 2 * 4096)
     cluster *= 2;
-  const dim3 grid(unsigned(a.R) * cluster);
-  auto kernel = a.top ? (a.temperature ? score_kernel<T, true, true> : score_kernel<T, true, false>)
-                      : (a.temperature ? score_kernel<T, false, true> : score_kernel<T, false, false>);
-  return launch_ex(kernel, grid, dim3(THREADS), 0, s, cluster, true, a, cluster);
+  // Four or five blocks an SM (64 or 48 registers a thread) by which takes fewer rounds of blocks; clusters of more than two are
+  // not packed that closely. Us, 5 / 4: 272 rows in bf16 29.3 / 25.5, in fp32 with 20 alternatives 46.7 / 42.4, 1480 in bf16
+  // 94.6 / 98.7, 2049 with 5 alternatives 140 / 149.
+  const int64_t n = int64_t(a.R) * cluster, rounds4 = (n + 4 * sms - 1) / (4 * sms), rounds5 = (n + 5 * sms - 1) / (5 * sms);
+  const bool four = cluster <= 2 && 4 * rounds4 <= 5 * rounds5;
+  return four ? launch_as<T, 4>(a, cluster, s) : launch_as<T, 5>(a, cluster, s);
 }
 
 }  // namespace score
