@@ -6,15 +6,14 @@
 // One pass: a thread keeps m, l and s of the values it has seen (fp32), raising m for 64 bytes at a time. The
 // order of tokens is by logit, then the lower token first.
 //
-// Alternatives without a second pass: a thread's m is the largest value of its strip of the row, so the top-th
-// largest m of a block bounds its top-th largest value from below, and only strips whose m reaches it hold any of
-// the block's alternatives: as many strips as alternatives (more with equal values) are read again, from L2.
+// Alternatives without a second pass: a thread's m is the largest value of its strips of the row, so the top-th
+// largest of several groups' maxima bounds the block's top-th largest value from below, and only strips whose largest
+// value reaches it hold any of the block's alternatives: little more than as many strips as alternatives are read again.
 //
 // A row is a cluster of 1 to 8 blocks, each with a slice of its 16-byte vectors; the first block joins them.
 // Bound: HBM and the exponentials' unit for many rows (2049 of 151,936 in bf16 124 us, 0.77 of the measured rate; 272 in
 // fp32 with 20 alternatives 42.4, 0.59, for the search of alternatives, which no other block's pass covers), latency for few
-// (one row 8.7). A ring of
-// bulk copies in shared memory in place of plain loads: 132 beside 132, one row 14.
+// (one row 8.7). A ring of bulk copies in shared memory in place of plain loads: 132 beside 132, one row 14.
 #include <algorithm>
 #include <cfloat>
 
