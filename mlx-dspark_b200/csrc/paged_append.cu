@@ -11,8 +11,8 @@
 // value is then known inside a block, which holds a head's new values in registers meanwhile. Then those of q, a warp or more a
 // row. Which page a block has is found from cu_rows without a sum over the requests: request b's pages
 // start at unit cu_rows[b] / page + 2 b, which leaves room for every page that n rows can touch (n / page + 2).
-// Bound: HBM and instructions for prompts (each value is read and written once; 16,389 rows of 32/8 heads of 128 84 us, 0.67
-// of the measured rate, 59 % of the issue slots), the launch for few rows (one row 3.2 us).
+// Bound: HBM and instructions for prompts (each value is read and written once; 16,389 rows of 32/8 heads of 128 79 us, 0.71
+// of the measured rate; 84 with operations on single values instead of pairs), the launch for few rows (one row 3.2 us).
 #include <algorithm>
 
 #include "host_common.h"
@@ -61,47 +61,83 @@ __device__ __forceinline__ void load16(const T* p, int c0, int c1, uint32_t* w) 
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void unpack16(const uint32_t* w, float* x) {
+// A lane's sixteen values in pairs: p[j] has those of rotary pairs 2 j and 2 j + 1 that come first, q[j] their partners (in the
+// half layout values 2 j, 2 j + 1 and 8 + 2 j, 9 + 2 j, else 4 j, 4 j + 2 and 4 j + 1, 4 j + 3).
+struct Vals {
+  f32x2 p[4], q[4];
+};
+
+template <typename T, bool HALF>
+__device__ __forceinline__ Vals unpack16(const uint32_t* w) {
+  Vals x;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 f = Elem<T>::unpack(w[i]);
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
+  for (int j = 0; j < 4; ++j) {
+    const float2 a = Elem<T>::unpack(w[HALF ? j : 2 * j]), b = Elem<T>::unpack(w[HALF ? 4 + j : 2 * j + 1]);
+    x.p[j] = HALF ? pack2(a.x, a.y) : pack2(a.x, b.x);
+    x.q[j] = HALF ? pack2(b.x, b.y) : pack2(a.y, b.y);
+  }
+  return x;
+}
+
+// The values in their order.
+template <bool HALF>
+__device__ __forceinline__ void in_order(const Vals& v, float* x) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    unpack2(v.p[j], x[HALF ? 2 * j : 4 * j], x[HALF ? 2 * j + 1 : 4 * j + 2]);
+    unpack2(v.q[j], x[HALF ? 8 + 2 * j : 4 * j + 1], x[HALF ? 9 + 2 * j : 4 * j + 3]);
   }
 }
 
-// RMS norm of a head whose 16-value parts are on `lanes` neighbouring lanes, then the rotation of the lane's part.
+// RMS norm of a head whose 16-value parts are on `lanes` neighbouring lanes, then the rotation of the lane's part. cs, sn: two
+// pairs' cosines and sines.
 template <typename T, bool HALF>
-__device__ __forceinline__ void norm_turn(float* x, const uint32_t* weight, bool norm, int lanes, float inv_d, float eps,
-                                          bool turns, const float* cs, const float* sn) {
+__device__ __forceinline__ void norm_turn(Vals& x, const uint32_t* weight, bool norm, int lanes, float inv_d, float eps,
+                                          bool turns, const f32x2* cs, const f32x2* sn) {
   if (norm) {
-    float ss = 0.f;
+    f32x2 s2 = mul2(x.p[0], x.p[0]);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) ss += x[i] * x[i];
+    for (int j = 1; j < 4; ++j) s2 = fma2(x.p[j], x.p[j], s2);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s2 = fma2(x.q[j], x.q[j], s2);
+    float ss, other;
+    unpack2(s2, ss, other);
+    ss += other;
     for (int o = 1; o < lanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     const float rs = rsqrtf(ss * inv_d + eps);
-    float w[16];
-    unpack16<T>(weight, w);
+    const Vals w = unpack16<T, HALF>(weight);
+    const f32x2 r2 = pack2(rs, rs);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] *= rs * w[i];
-  }
-  if (turns) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int i0 = HALF ? i : 2 * i, i1 = HALF ? 8 + i : 2 * i + 1;
-      const float p = x[i0], q = x[i1];
-      x[i0] = p * cs[i] - q * sn[i];
-      x[i1] = q * cs[i] + p * sn[i];
+    for (int j = 0; j < 4; ++j) {
+      x.p[j] = mul2(x.p[j], mul2(r2, w.p[j]));
+      x.q[j] = mul2(x.q[j], mul2(r2, w.q[j]));
     }
   }
+  if (turns) {
+    const f32x2 minus = pack2(-1.f, -1.f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x2 p = x.p[j], q = x.q[j];
+      x.p[j] = fma2(q, mul2(sn[j], minus), mul2(p, cs[j]));
+      x.q[j] = fma2(p, sn[j], mul2(q, cs[j]));
+    }
+  }
+}
+
+// cos and sin of two neighbouring pairs, times mscale.
+__device__ __forceinline__ void two_phases(int pos, const uint64_t* f, float mscale, f32x2& cs, f32x2& sn) {
+  float c0, s0, c1, s1;
+  phase(pos, f[0], c0, s0);
+  phase(pos, f[1], c1, s1);
+  cs = pack2(c0 * mscale, c1 * mscale);
+  sn = pack2(s0 * mscale, s1 * mscale);
 }
 
 // One (page, some heads, k or v). PASS rounds of 16 values a thread. Cosines and sines
 // are the same for all heads: they wait in shared memory, where each thread reads its own.
 template <typename T, bool VEC, bool HALF, int PASS, int THREADS>
 __device__ void append_page(const dspark_paged_append_args& a, int unit, int groups, int* status) {
-  extern __shared__ float4 s_turn[];  // [PASS][4][THREADS]: (cos, sin) of two pairs
+  extern __shared__ ulonglong2 s_turn[];  // [PASS][4][THREADS]: two pairs' cosines, their sines
   __shared__ uint32_t s_max[2][THREADS / 32];
   const int tid = threadIdx.x, D = a.D, lanes = D / 16, li = tid % lanes;
   const int kv = unit & 1, hu = unit >> 1, u = hu / groups, group = hu - u * groups;
@@ -144,11 +180,19 @@ __device__ void append_page(const dspark_paged_append_args& a, int unit, int gro
   uint32_t weight[8];
   if (norm) load16<T, false>(static_cast<const T*>(a.k_norm), c0, c1, weight);
   // The codes of 16 values of the page's new row t.
-  auto put = [&](uint8_t* codes, int t, const float* x, float inv) {
+  auto put = [&](uint8_t* codes, int t, const Vals& v, float inv) {
+    const f32x2 i2 = pack2(inv, inv);
+    Vals z;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      z.p[j] = mul2(v.p[j], i2);
+      z.q[j] = mul2(v.q[j], i2);
+    }
+    float x[16];
+    in_order<HALF>(z, x);
     uint32_t y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      y[i] = f32_to_e4m3(x[4 * i] * inv, x[4 * i + 1] * inv, x[4 * i + 2] * inv, x[4 * i + 3] * inv);
+    for (int i = 0; i < 4; ++i) y[i] = f32_to_e4m3(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
     uint8_t* p = codes + (begin + t) * ts;
     if (half) {
       *reinterpret_cast<uint2*>(p + c0) = make_uint2(y[0], y[1]);
@@ -157,9 +201,14 @@ __device__ void append_page(const dspark_paged_append_args& a, int unit, int gro
       *reinterpret_cast<uint4*>(p + c0) = make_uint4(y[0], y[1], y[2], y[3]);
     }
   };
-  auto larger = [](float top, const float* x) {  // the largest finite value (NaN: 0)
+  auto larger = [](float top, const Vals& v) {  // the largest finite value (NaN: 0)
+    float x[16], m = top;
+    in_order<HALF>(v, x);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 16; i += 2) m = max3(m, fabsf(x[i]), fabsf(x[i + 1]));
+    if (m < INFINITY) return m;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {  // rare
       const float y = fabsf(x[i]);
       top = fmaxf(top, y < INFINITY ? y : 0.f);
     }
@@ -206,16 +255,12 @@ __device__ void append_page(const dspark_paged_append_args& a, int unit, int gro
           const int t = min(t0 + first, count - 1), r = r0 + place0 + t;
           uint32_t w[8];
           load16<T, VEC>(src + (t - first) * row_stride + h * head_stride, c0, c1, w);
-          float x[16], cs[8], sn[8];
-          unpack16<T>(w, x);
+          Vals x = unpack16<T, HALF>(w);
+          f32x2 cs[4], sn[4];
           if (turns) {
             const int pos = a.row_pos ? a.row_pos[r] : int(len + place0 + t);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              phase(pos, a.freq[8 * li + i], cs[i], sn[i]);
-              cs[i] *= a.mscale;
-              sn[i] *= a.mscale;
-            }
+            for (int j = 0; j < 4; ++j) two_phases(pos, a.freq + 8 * li + 2 * j, a.mscale, cs[j], sn[j]);
           }
           norm_turn<T, HALF>(x, weight, norm, lanes, 1.f / D, a.eps, turns, cs, sn);
           if (turn == 0) top = larger(top, x);
@@ -234,10 +279,9 @@ __device__ void append_page(const dspark_paged_append_args& a, int unit, int gro
       const int r = r0 + place0 + t, pos = a.row_pos ? a.row_pos[r] : int(len + place0 + t);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float4 y;
-        phase(pos, a.freq[8 * li + 2 * i], y.x, y.y);
-        phase(pos, a.freq[8 * li + 2 * i + 1], y.z, y.w);
-        s_turn[(z * 4 + i) * THREADS + tid] = make_float4(y.x * a.mscale, y.y * a.mscale, y.z * a.mscale, y.w * a.mscale);
+        ulonglong2 y;
+        two_phases(pos, a.freq + 8 * li + 2 * i, a.mscale, y.x, y.y);
+        s_turn[(z * 4 + i) * THREADS + tid] = y;
       }
     }
   }
@@ -247,9 +291,9 @@ __device__ void append_page(const dspark_paged_append_args& a, int unit, int gro
       fetch(h);
       old = begin ? scales[h * a.scale_strides[1]] : 0.f;
     }
-    float x[PASS][16];
+    Vals x[PASS];
 #pragma unroll
-    for (int z = 0; z < PASS; ++z) unpack16<T>(raw[z], x[z]);
+    for (int z = 0; z < PASS; ++z) x[z] = unpack16<T, HALF>(raw[z]);
     const float before = old;
     if (AHEAD && h + 1 < h1) {  // the next head under this one's work
       fetch(h + 1);
@@ -260,15 +304,13 @@ __device__ void append_page(const dspark_paged_append_args& a, int unit, int gro
     for (int z = 0; z < PASS; ++z) {
       const int t = z * per + first;
       if (z * per >= count) break;  // (a norm's lanes leave together)
-      float cs[8], sn[8];
+      f32x2 cs[4], sn[4];
       if (turns && t < count) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float4 y = s_turn[(z * 4 + i) * THREADS + tid];
-          cs[2 * i] = y.x;
-          sn[2 * i] = y.y;
-          cs[2 * i + 1] = y.z;
-          sn[2 * i + 1] = y.w;
+          const ulonglong2 y = s_turn[(z * 4 + i) * THREADS + tid];
+          cs[i] = y.x;
+          sn[i] = y.y;
         }
       }
       norm_turn<T, HALF>(x[z], weight, norm, lanes, 1.f / D, a.eps, turns && t < count, cs, sn);
@@ -305,14 +347,10 @@ __device__ void turn_q(const dspark_paged_append_args& a, int w, int warps) {
   const int r0 = first_row(a.cu_rows, b, a.R);
   if (r < r0 || r >= first_row(a.cu_rows, b + 1, a.R)) return;  // a row of no request
   pos = a.row_pos ? a.row_pos[r] : max(a.kv_len[b], 0) + r - r0;
-  float cs[8], sn[8];
+  f32x2 cs[4], sn[4];
   if (turns) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      phase(pos, a.freq[8 * li + i], cs[i], sn[i]);
-      cs[i] *= a.mscale;
-      sn[i] *= a.mscale;
-    }
+    for (int j = 0; j < 4; ++j) two_phases(pos, a.freq + 8 * li + 2 * j, a.mscale, cs[j], sn[j]);
   }
   const bool norm = a.q_norm;
   uint32_t weight[8];
@@ -323,10 +361,11 @@ __device__ void turn_q(const dspark_paged_append_args& a, int w, int warps) {
     for (int u = 0; u < U; ++u) {
       const int hh = h + u * step;
       if (hb + u * step >= a.Hq) break;
-      float x[16];
-      unpack16<T>(raw[u], x);
-      norm_turn<T, HALF>(x, weight, norm, lanes, 1.f / D, a.eps, turns, cs, sn);
+      Vals v = unpack16<T, HALF>(raw[u]);
+      norm_turn<T, HALF>(v, weight, norm, lanes, 1.f / D, a.eps, turns, cs, sn);
       if (hh >= a.Hq) continue;
+      float x[16];
+      in_order<HALF>(v, x);
       uint32_t y[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = turns || norm ? Elem<T>::pack(x[2 * i], x[2 * i + 1]) : raw[u][i];
@@ -385,8 +424,8 @@ static cudaError_t launch_as(const dspark_paged_append_args& a, cudaStream_t s) 
 template <typename T, bool VEC, bool HALF>
 static cudaError_t launch_page(const dspark_paged_append_args& a, cudaStream_t s) {
   // Threads by the rows that a page gets on average (a page with more than its block holds is made twice): in registers
-  // 64 * 16 values of few rows, else the whole page. 200 requests of 1 to 16 rows 13.4 us with 128 threads, a prompt's
-  // 16,389 rows in pages of 64 84 with 256 threads of two rows (4 rows a thread: 94 beside 81, with a coarser sine).
+  // 64 * 16 values of few rows, else the whole page. 200 requests of 1 to 16 rows 13.2 us with 128 threads, a prompt's
+  // 16,389 rows in pages of 64 79 with 256 threads of two rows (4 rows a thread: 94 beside 81, in an earlier form).
   const int64_t rows = std::min<int64_t>(a.page, (int64_t(a.R) + a.B - 1) / a.B), parts = rows * a.D / 16;
   if (parts <= 32) return launch_as<T, VEC, HALF, 1, 64, 10>(a, s);
   if (parts <= 128) return launch_as<T, VEC, HALF, 1, 128, 5>(a, s);
