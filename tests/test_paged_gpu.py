@@ -370,6 +370,77 @@ def test_attention(cuda, case):
     assert bool((out[sum(counts):] == 5.0).all())  # rows of nobody
 
 
+def _with_room(rows, page, tokens):
+    """The tables widened to so many tokens: small calls go to clusters of 8 blocks a row block, with room for 6000 tokens of
+    16 where there are few of them, with room for 40,000 tokens as shares of a line over the whole grid."""
+    width = max(-(-tokens // page), len(rows[0]))
+    return [r + [-1] * (width - len(r)) for r in rows]
+
+
+FORMS = [
+    # counts, lens, Hq, Hk, D, page, type, causal, pool layout
+    ([1], [5000], 4, 1, 128, 64, BF, True, "heads"),
+    ([2, 0, 1], [1030, 9, 3001], 8, 2, 64, 16, HF, True, "tokens"),
+    ([7], [4099], 8, 2, 128, 128, HF, True, "heads"),                # 28 rows of a product
+    ([16, 5, 1], [31, 2049, 700], 4, 2, 64, 32, BF, False, "heads"),
+    ([1] * 33, [1 + 97 * i % 900 for i in range(33)], 4, 1, 64, 16, BF, True, "heads"),  # more requests than a warp has lanes
+    ([20], [3], 4, 4, 128, 64, BF, True, "heads"),                   # more rows than keys
+]
+
+
+@pytest.mark.parametrize("tokens", [0, 6000, 40000])
+@pytest.mark.parametrize("case", FORMS, ids=range(len(FORMS)))
+def test_attention_few_rows_forms(cuda, case, tokens):
+    counts, lens, Hq, Hk, D, page, dt, causal, layout = case
+    rng, g = random.Random(D + page), torch.Generator().manual_seed(len(counts) + page + 2)
+    need = [-(-x // page) for x in lens]
+    cache = _finite_pool(cuda, sum(need) + 4, Hk, page, D, g, layout)
+    rows = _with_room(_tables(need, sum(need) + 4, rng, max(need) + 1), page, tokens)
+    q = torch.randn(sum(counts) + 2, Hq + 1, D, generator=g).to(dt).to(cuda)[:, :Hq]
+    out = torch.full(q.shape, 5.0, dtype=dt, device=cuda)
+    _check(cuda, cache, q, counts, lens, rows, causal, D ** -0.5, out)
+    assert bool((out[sum(counts):] == 5.0).all())
+    again = cache.attention(q, _cu(counts, cuda), _i32(lens, cuda), _i32(rows, cuda), scale=D ** -0.5, causal=causal)
+    assert torch.equal(again[: sum(counts)], out[: sum(counts)])
+
+
+@pytest.mark.parametrize("tokens", [0, 6000, 40000])
+@pytest.mark.parametrize("n", [3, 12])
+def test_attention_few_rows_hidden_values(cuda, n, tokens):
+    """A NaN code reaches the rows that see its key and no others; infinite q makes its own head NaN; a page without a
+    positive scale is not seen."""
+    g = torch.Generator().manual_seed(n)
+    L, D, page = 2000, 64, 16
+    cache = _finite_pool(cuda, 125, 2, page, D, g)
+    table = _i32(_with_room([list(range(125))], page, tokens), cuda)
+    q = torch.randn(n, 4, D, generator=g).to(BF).to(cuda)
+    args = _cu([n], cuda), _i32([L], cuda), table
+    clean = cache.attention(q, *args, scale=0.1)
+    own = L - 2  # the last row but one's token
+    for t in (cache.v, cache.k):
+        at = t.view(torch.uint8)[own // page, 0, own % page]
+        old = at.clone()
+        at[10] = 0x7F
+        out = cache.attention(q, *args, scale=0.1)
+        assert torch.equal(out[: n - 2], clean[: n - 2]) and torch.equal(out[:, 2:], clean[:, 2:])
+        bad = out[n - 2 :, :2].isnan()
+        assert bool(bad[..., 10].all()) and bool(bad.all()) == (t is cache.k)
+        at.copy_(old)
+    x = q.clone()
+    x[1, 2, 5] = math.inf
+    out = cache.attention(x, *args, scale=0.1)
+    assert bool(out[1, 2].isnan().all()) and torch.equal(out[2:], clean[2:]) and torch.equal(out[1, :2], clean[1, :2])
+    cache.k_scale[3] = 0.0
+    cache.v_scale[7] = -1.0
+    seen = cache.attention(q, *args, scale=0.1)
+    gone = [x for x in range(125) if x not in (3, 7)]  # the same keys without them
+    want = cache.attention(q, args[0], _i32([L - 2 * page], cuda), _i32(_with_room([gone], page, tokens), cuda), scale=0.1)
+    # weights rounded in another grouping: two fp16 roundings (2^-11 each) of sums whose values are at most vmax, and bf16's
+    # own half steps (2^-8) of either result
+    vmax = 448 * float(cache.v_scale.abs().max())
+    assert float((seen - want).abs().max()) <= (2 * 2.0 ** -11 + 2 * 2.0 ** -8) * vmax
+
+
 def _far(rows, page):
     """The tables widened to 200,000 tokens: with that much room, calls of more than 32 rows a request and kv head on
     average go to the kernel for many rows (the narrow tables of small tests do not)."""
