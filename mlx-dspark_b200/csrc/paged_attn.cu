@@ -640,9 +640,10 @@ static int launch_few(const dspark_paged_attn_args& a, cudaStream_t s) {
 
 // Which calls go to the 5th-generation tensor cores (paged_wide.cu): those with more than 32 rows a request and kv head on
 // average and with work enough, in tiles of 32 rows by 128 keys (the table's width stands for the lengths, which are
-// on the device). Measured, this kernel / the other, us, 32/8 heads of 128: 16 rows over 4k keys, 1 request (2048 of
-// such tiles with their 64 rows a head) 21 / 30, 4 requests 36 / 39, 16 requests (8192) 90 / 77; 32 rows over 16k, 1
-// request (4096) 49 / 43; 64 requests of 64 rows over 4k 1105 / 420.
+// on the device). Measured, this kernel / the other, us, 32/8 heads of 128: 16 rows over 4k keys, 1 request (528 of
+// such tiles with their 64 rows a head) 17 / 28, 4 requests (2112) 34 / 29, 8 (4224) 51 / 41, 16 84 / 62; one request of 64 rows
+// over 4k (2112) 33 / 37, of 16 over 16k (2064) 35 / 38, of 32 over 16k (4128) 43 / 39; 64 requests over 4k, 8 rows (32 a head)
+// 150 / 182, 16 rows 281 / 194.
 // Not where a request may have more than 2^25 keys: a wait there can last a segment, which has to end within the limit.
 constexpr int FEW_ROWS = 32, WIDE_TILES = 3000, LONGEST = 1 << 25;
 static bool has_many_rows(int R, int B, int Hq, int Hk) { return int64_t(R) * (Hq / Hk) > int64_t(FEW_ROWS) * B; }

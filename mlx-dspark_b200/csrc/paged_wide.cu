@@ -33,7 +33,7 @@ namespace wide {
 
 constexpr int ROWS = 128;            // rows a slot
 constexpr int RB = 2 * ROWS;         // rows an item
-constexpr int NTHR = 512;            // two softmax warpgroups, one of the products and Q, one that converts
+constexpr int NTHR = 512;            // two softmax warpgroups, one of the products, loads and segments, one that converts
 constexpr int WARP_MMA = 8, WARP_LOAD = 9, WARP_PREP = 10, WARP_CONV = 12;
 // Cost of a segment, in tiles of up to 128 rows. Mean of 12 mixes (1 to 60 requests of 16 to 509 rows over 3k to 30k
 // keys), us: 4 121.5, 7 117.9, 10 118.5, 14 121.1, 20 124.9.
