@@ -171,11 +171,12 @@ __device__ __forceinline__ float factor_of(float rf, float ks) {
 }
 
 // The NaN codes that were taken out of the segment's V tiles, added to what a row that sees them has stored (`out`: the
-// output, or `part`: the fp32 part).
+// output, or `part`: the fp32 part). They are taken out of whole tiles: from the first key of the one that holds the rows' own
+// first key on, keys before the rows' own among them.
 template <typename T>
 __device__ __noinline__ void add_hidden(const dspark_paged_attn_args& a, const Segment& s, int lim, int d0, int d1, T* out,
                                         float* part) {
-  const int k0 = max(s.t0 * BN, max(s.before, 0)), k1 = min(min(s.t1 * BN, s.len), lim);
+  const int k0 = max(s.t0 * BN, max(s.before, 0) / BN * BN), k1 = min(min(s.t1 * BN, s.len), lim);
   for (int k = k0; k < k1; ++k) {
     const int id = a.page_table[int64_t(s.b) * a.table_stride + k / a.page];
     if (id < 0 || id >= a.n_pages) continue;

@@ -1,0 +1,57 @@
+"""The paged 8-bit cache and token scores on the GPU where calls meet an edge: NaN codes beside the rows' own keys."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+from test_paged_gpu import BF, E4M3, HF, _cu, _far, _finite_pool, _i32, _tables
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------- NaN codes of v
+
+NAN_VALUES = [
+    # counts, lens, Hq, Hk, D, page, type: with far tables all go to the kernel for many rows
+    ([20], [470], 2, 1, 64, 16, BF),                     # 40 rows: the slots share them; items cut at every tile
+    ([80], [470], 2, 1, 64, 16, HF),                     # 160 rows: a slot each
+    ([40, 3, 90], [129, 700, 333], 8, 2, 128, 32, HF),   # requests that begin inside a tile
+    ([33] * 70, [33 + 37 * i % 800 for i in range(70)], 8, 4, 64, 64, BF),   # whole items and cut ones, 66 rows each
+    ([50] * 60, [128 + 53 * i % 700 for i in range(60)], 16, 2, 64, 128, BF),  # 400 rows: pairs of slots and a rest
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("far", [True, False])
+@pytest.mark.parametrize("case", NAN_VALUES, ids=range(len(NAN_VALUES)))
+def test_nan_values_reach_all_rows_that_see_them(cuda, case, far, causal):
+    """A NaN code of v just before the rows' own keys, at the first key of the 128 that hold the first of them, just before
+    those, and among the own ones: it makes exactly the values NaN that it belongs to, of every row that sees its key."""
+    counts, lens, Hq, Hk, D, page, dt = case
+    rng, g = random.Random(D + page), torch.Generator().manual_seed(len(counts) + page)
+    need = [-(-x // page) for x in lens]
+    cache = _finite_pool(cuda, sum(need) + 2, Hk, page, D, g)
+    rows = _tables(need, sum(need) + 2, rng)
+    table = _i32(_far(rows, page) if far else rows, cuda)
+    q = torch.randn(sum(counts), Hq, D, generator=g).to(dt).to(cuda)
+    cu, ln = _cu(counts, cuda), _i32(lens, cuda)
+    clean = cache.attention(q, cu, ln, table, scale=0.1, causal=causal)
+    assert not bool(clean.isnan().any())
+    codes, before = cache.v.view(torch.uint8), [x - n for n, x in zip(counts, lens)]
+    for place in range(4):
+        kept, want = codes.clone(), torch.zeros(clean.shape, dtype=torch.bool)
+        r0 = 0
+        for b, (n, x) in enumerate(zip(counts, lens)):
+            first = before[b] // 128 * 128
+            key = max((before[b] - 1, first, first - 1, before[b] + n // 2)[place], 0)
+            h, d = rng.randrange(Hk), rng.randrange(D)
+            codes[rows[b][key // page], h, key % page, d] = rng.choice([0x7F, 0xFF])
+            sees = max(0, key - before[b]) if causal else 0  # the first row that does
+            want[r0 + sees : r0 + n, h * (Hq // Hk) : (h + 1) * (Hq // Hk), d] = True
+            r0 += n
+        out = cache.attention(q, cu, ln, table, scale=0.1, causal=causal)
+        codes.copy_(kept)
+        assert torch.equal(out.isnan().cpu(), want), place
+        assert torch.equal(out.cpu()[~want], clean.cpu()[~want]), place
