@@ -126,9 +126,9 @@ __device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
   return Sums{m, a.l + b.l, a.s + b.s};
 }
 
-// Larger first, then the lower token.
+// Larger first, then the lower token; a zero of either sign is the same value.
 __device__ __forceinline__ uint64_t key_of(float x, int v) {
-  const uint32_t b = __float_as_uint(x);
+  const uint32_t b = x == 0.f ? 0u : __float_as_uint(x);
   return uint64_t(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | uint32_t(~v);
 }
 __device__ __forceinline__ float value_of(uint64_t key) {

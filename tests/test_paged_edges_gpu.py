@@ -1,4 +1,5 @@
-"""The paged 8-bit cache and token scores on the GPU where calls meet an edge: NaN codes beside the rows' own keys."""
+"""The paged 8-bit cache and token scores on the GPU where calls meet an edge: NaN codes beside the rows' own keys,
+zeros of either sign among the logits."""
 
 from __future__ import annotations
 
@@ -6,7 +7,7 @@ import random
 
 import pytest
 import torch
-from test_paged_gpu import BF, E4M3, HF, _cu, _far, _finite_pool, _i32, _tables
+from test_paged_gpu import BF, FP, HF, _check_scores, _cu, _far, _finite_pool, _i32, _tables
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +56,51 @@ def test_nan_values_reach_all_rows_that_see_them(cuda, case, far, causal):
         codes.copy_(kept)
         assert torch.equal(out.isnan().cpu(), want), place
         assert torch.equal(out.cpu()[~want], clean.cpu()[~want]), place
+
+
+# ------------------------------------------------------------------------------- zeros of either sign
+
+def _zeros(V, dt, at, g):
+    """Rows of negative logits with zeros at the given places: {token: sign}."""
+    x = (-1 - torch.rand(len(at), V, generator=g)).to(dt)
+    for r, row in enumerate(at):
+        for token, sign in row.items():
+            x[r, token] = sign * 0.0
+    return x
+
+
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("rows,V", [(1, 600), (1, 151937), (40, 9001)])  # one block a row, a cluster, ragged rows of a cluster
+def test_zeros_of_either_sign_are_one_logit(cuda, dt, rows, V):
+    """-0 and +0 are equal: the lower token comes first, in the rank and in the alternatives, greedy or not, at the head and at
+    the end of the list, and where more values are equal than a block sorts at once."""
+    from mlx_dspark_b200 import sampling
+
+    g = torch.Generator().manual_seed(V)
+    at = [{5: -1, V - 2: 1}, {5: 1, V - 2: -1}, {0: -1, 7: 1, V // 2: -1, V - 1: 1}, {V - 1: -1, V // 2: 1, 3: 1}]
+    x = _zeros(V, dt, at, g)
+    many = x.repeat(rows, 1).to(cuda)
+    for temp in (None, 0.0, 0.7):
+        T = None if temp is None else torch.full((4 * rows,), temp, device=cuda)
+        for pick in (min, max):
+            tokens = [pick(a) for a in at]
+            _check_scores(cuda, x, tokens, None if temp is None else [temp] * 4, 3)
+            for top in (1, 2, 3, 20, 32):
+                got = sampling.token_logprobs(many, _i32(tokens * rows, cuda), temperature=T, top=top)
+                ids, rank, lp = (got[k].tolist() for k in ("top_ids", "rank", "logprob"))
+                for r in range(4 * rows):
+                    a = at[r % 4]
+                    assert ids[r][: len(a)] == sorted(a)[:top] and rank[r] == sorted(a).index(pick(a))
+                    if rank[r] < top:  # the alternative in its place is the token itself
+                        assert got["top_logprobs"][r, rank[r]].item() == lp[r]
+    # a larger value before them, and the list's end among them
+    x[:, 11] = 1.0
+    _check_scores(cuda, x[:4], [max(a) for a in at], None, 2)
+    # zeros of both signs everywhere, in turn and at random
+    y = torch.zeros(3, V, dtype=dt)
+    y[0, ::2] = -0.0
+    y[1, 1::2] = -0.0
+    y[2] = torch.where(torch.rand(V, generator=g) < 0.5, -0.0, 0.0).to(dt)
+    for temp in (None, [0.0, 1.0, 0.0]):
+        got = _check_scores(cuda, y, [0, 1, V - 1], temp, 32)
+        assert got["top_ids"].tolist() == [list(range(32))] * 3 and got["rank"].tolist() == [0, 1, V - 1]
