@@ -657,7 +657,7 @@ int dspark_kv_keep_path(void* const* k_layers, void* const* v_layers, int n_laye
  * become tokens kv_len[b] + i; row_pos [R], or NULL: positions kv_len[b] + i. The scale of a page and head is the
  * smallest power of two (2^-64 to 2^64) with which the largest finite value of the tokens appended to it is at most
  * 448; where the page holds tokens of the request already (kv_len[b] % page), the larger of that and the old scale, and
- * if it rises the old codes are rounded to it. A page begun anew (from its first token) starts a scale of its own;
+ * if it rises the old codes are rounded to it (an old scale of NaN gives way too, and its tokens become zeros). A page begun anew (from its first token) starts a scale of its own;
  * taking tokens back (a smaller kv_len) leaves the scale. Values are rounded to nearest even, infinities become
  * +-448 * scale, NaN stays NaN. Rows whose page the table does not have (or an id outside 0 .. n_pages - 1) are
  * dropped, and the device status word records it. q_out (may be q) is written for rows of a request only.

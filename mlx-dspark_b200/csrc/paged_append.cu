@@ -226,8 +226,8 @@ __device__ void append_page(const dspark_paged_append_args& a, int unit, int gro
     const float need = pow2(e);
     const float now = before > need ? before : need;  // (what is no scale gives way)
     uint8_t* codes = page + h * hs;
-    if (before > 0.f && now > before) {
-      const float f = before / now;
+    if (begin && now != before) {
+      const float f = before == before ? before / now : 0.f;  // (a scale of zero or NaN: the page's tokens are zeros)
       for (int i = tid; i < begin * lanes; i += THREADS) {
         uint4* p = reinterpret_cast<uint4*>(codes + (i / lanes) * ts + (i % lanes) * 16);
         uint4 w = *p;

@@ -1,13 +1,16 @@
 """The paged 8-bit cache and token scores on the GPU where calls meet an edge: NaN codes beside the rows' own keys,
-zeros of either sign among the logits."""
+zeros of either sign among the logits, begun pages without a scale."""
 
 from __future__ import annotations
 
+import math
 import random
 
+import paged_reference as ref
 import pytest
 import torch
-from test_paged_gpu import BF, FP, HF, _check_scores, _cu, _far, _finite_pool, _i32, _tables
+from test_paged_gpu import (BF, FP, HF, _append_values, _check_scores, _cpu, _cu, _far, _finite_pool, _i32, _identity, _pool,
+                            _tables)
 
 pytestmark = pytest.mark.gpu
 
@@ -104,3 +107,25 @@ def test_zeros_of_either_sign_are_one_logit(cuda, dt, rows, V):
     for temp in (None, [0.0, 1.0, 0.0]):
         got = _check_scores(cuda, y, [0, 1, V - 1], temp, 32)
         assert got["top_ids"].tolist() == [list(range(32))] * 3 and got["rank"].tolist() == [0, 1, V - 1]
+
+
+# ------------------------------------------------------------------------------- begun pages without a scale
+
+@pytest.mark.parametrize("scale", [0.0, -0.25, -1e30, math.nan])
+@pytest.mark.parametrize("page,D,n", [(16, 64, 3), (64, 128, 50), (128, 64, 120)])
+def test_append_to_a_begun_page_without_a_scale(cuda, page, D, n, scale):
+    """Tokens of a page whose scale is not positive keep their values, code * scale, under the scale that the new tokens give the
+    page (a NaN one: zeros), instead of becoming whatever their codes mean under it."""
+    begin, g = 5, torch.Generator().manual_seed(page)
+    cache = _pool(cuda, 3, 2, page, D, g)
+    for t in (cache.k_scale, cache.v_scale):
+        t[1, 0] = scale  # the other head's page has one
+    x, y = (3 * torch.randn(n, 2, D, generator=g).to(BF) for _ in range(2))
+    old = _cpu(cache)
+    _append_values(cuda, cache, _i32([[1]], cuda), begin, x, y, _identity(cuda, D))
+    new = _cpu(cache)
+    for i, z in ((0, x), (1, y)):
+        lo, hi, s_lo, s_hi = ref.append(old[i], old[i + 2].nan_to_num(0.0), [1], begin, z.double(), torch.zeros(n, 2, D))
+        assert torch.equal(lo.nan_to_num(-1), hi.nan_to_num(-1)) and torch.equal(new[i + 2].double(), s_lo)
+        got, want = new[i].double(), lo
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
