@@ -466,6 +466,14 @@ extern "C" int dspark_paged_append(const dspark_paged_append_args* p, void* stre
     return fail(DSPARK_ERR_ARG, "paged_append: null pointer");
   if (a.R && (!a.q || !a.q_out || !a.k || !a.v || !a.k_pages || !a.v_pages || !a.k_scale || !a.v_scale))
     return fail(DSPARK_ERR_ARG, "paged_append: null pointer");
+  // blocks of one launch read these while another writes the new lengths
+  auto apart = [&](const int32_t* x, int64_t n) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(x), out = reinterpret_cast<uintptr_t>(a.len_out);
+    return !x || at + n * sizeof(int32_t) <= out || out + a.B * sizeof(int32_t) <= at;
+  };
+  if (a.len_out && !(apart(a.kv_len, a.B) && apart(a.cu_rows, int64_t(a.B) + 1) && apart(a.row_pos, a.R) &&
+                     (a.max_pages == 0 || apart(a.page_table, (a.B - 1) * a.table_stride + a.max_pages))))
+    return fail(DSPARK_ERR_ARG, "paged_append: len_out overlaps kv_len, cu_rows, row_pos or page_table");
   bool codes = true;
   for (const void* x : {a.k_pages, a.v_pages}) codes &= reinterpret_cast<uintptr_t>(x) % 16 == 0;
   for (int i = 0; i < 3; ++i) codes &= a.kp_strides[i] % 16 == 0 && a.vp_strides[i] % 16 == 0;

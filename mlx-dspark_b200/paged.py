@@ -80,7 +80,7 @@ class PagedCache:
         requests' pages: row i of request b becomes token ``kv_len[b] + i`` (int32 ``[B]``: tokens cached before). The
         rotary position is ``row_pos`` (int32 ``[R]``) or that token. ``q_norm`` / ``k_norm`` as in
         :func:`.rope.rope_append`. Returns the rotated q (``q_out``, which may be ``q``) and the new lengths
-        (``len_out``, not ``kv_len`` itself), which :meth:`attention` takes.
+        (``len_out``, apart from ``kv_len`` and the call's other int32 inputs), which :meth:`attention` takes.
 
         The scale of a page and head is the smallest power of two with which the largest value appended to it is at
         most 448; a page that holds tokens already keeps its scale or raises it, and then its codes are rounded to
@@ -102,8 +102,6 @@ class PagedCache:
             raise _lib.DSparkError(_lib.ERR_ARG, f"q_out {tuple(q_out.shape)} for {tuple(shape)}")
         if len_out is None:
             len_out = torch.empty(B, dtype=torch.int32, device=q.device)
-        elif abs(len_out.data_ptr() - kv_len.data_ptr()) < 4 * B:
-            raise _lib.DSparkError(_lib.ERR_ARG, "len_out must not be kv_len: blocks of one launch read the old lengths")
         qs, ks, vs, os = _strides("q", q), _strides("k", k), _strides("v", v), _strides("q_out", q_out)
         dt = _dtype(q, k, v, q_out, q_norm, k_norm)
         tp, ts, width = self._table(page_table, B)

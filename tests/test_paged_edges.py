@@ -1,0 +1,33 @@
+"""The paged 8-bit cache without a GPU: what a call may not be given."""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import mlx_dspark_b200  # noqa: F401
+from mlx_dspark_b200 import _lib
+
+
+def test_append_refuses_lengths_that_overlap_its_inputs():
+    """One block writes len_out while others read kv_len, cu_rows, row_pos and page_table."""
+    buf = (C.c_int32 * 256)()
+    p = C.cast(buf, C.c_void_p).value
+    p += -p % 16
+    B, R = 5, 9
+    ok = dict(q=p, k=p, v=p, q_out=p, k_pages=p, v_pages=p, k_scale=p, v_scale=p, freq=p, dtype=0, layout=0,
+              R=R, B=B, Hq=2, Hk=1, D=64, rot=64, page=16, n_pages=4, max_pages=2, table_stride=3)
+    at = dict(kv_len=(p + 256, B), cu_rows=(p + 384, B + 1), row_pos=(p + 512, R), page_table=(p + 640, 4 * 3 + 2))
+
+    def rc(out, **kw):
+        args = {**ok, **{k: v[0] for k, v in at.items()}, "len_out": out, **kw}
+        return _lib.lib.dspark_paged_append(C.byref(_lib.PagedAppendArgs(**args)), None)
+
+    for name, (first, n) in at.items():
+        for out in (first, first + 4 * (n - 1), first - 4 * (B - 1)):
+            assert rc(out) == _lib.ERR_ARG and "len_out" in _lib.last_error(), (name, out - first)
+        # beside them: refused for the next reason instead, the pages' alignment
+        for out in (first + 4 * n, first - 4 * B):
+            assert rc(out, k_pages=p + 8) == _lib.ERR_UNSUPPORTED, (name, out - first)
+    assert rc(at["row_pos"][0], row_pos=None, k_pages=p + 8) == _lib.ERR_UNSUPPORTED
+    assert rc(None, k_pages=p + 8) == _lib.ERR_UNSUPPORTED
+
