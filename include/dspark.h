@@ -662,7 +662,8 @@ int dspark_kv_keep_path(void* const* k_layers, void* const* v_layers, int n_laye
  * +-448 * scale, NaN stays NaN. Rows whose page the table does not have (or an id outside 0 .. n_pages - 1) are
  * dropped, and the device status word records it. q_out (may be q) is written for rows of a request only.
  * len_out [B] (or NULL): kv_len + rows, at most max_pages * page (a kv_len above that stays); it may not overlap kv_len,
- * cu_rows, row_pos or page_table. No two requests append to one page. */
+ * cu_rows, row_pos or page_table. No two requests append to one page; pages, heads, tokens and k and v (scales too) have
+ * memory of their own, no strides of zero. */
 typedef struct {
   const void* q;
   const void* k;

@@ -35,7 +35,8 @@ def _workspace(R: int, B: int, Hq: int, Hk: int, D: int, device: int) -> int:
 class PagedCache:
     """One layer's pages: codes ``k`` / ``v`` (``torch.float8_e4m3fn`` ``[pages, heads, page_size, head_dim]``, any
     strides of multiples of 16 with head_dim contiguous) and scales ``k_scale`` / ``v_scale`` (float32
-    ``[pages, heads]``): value = code * scale. :meth:`empty` makes a pool."""
+    ``[pages, heads]``): value = code * scale. :meth:`empty` makes a pool. :meth:`append` needs pages and
+    scales that share no memory (no expanded ones, ``k`` and ``v`` apart); :meth:`attention` reads any."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.ndim != 4 or v.shape != k.shape or k.dtype is not torch.float8_e4m3fn or v.dtype is not k.dtype:

@@ -31,3 +31,21 @@ def test_append_refuses_lengths_that_overlap_its_inputs():
     assert rc(at["row_pos"][0], row_pos=None, k_pages=p + 8) == _lib.ERR_UNSUPPORTED
     assert rc(None, k_pages=p + 8) == _lib.ERR_UNSUPPORTED
 
+
+
+def test_append_refuses_pages_that_share_their_memory():
+    """Blocks of one launch write pages, heads, keys and values side by side."""
+    buf = (C.c_int32 * 256)()
+    p = C.cast(buf, C.c_void_p).value
+    p += -p % 16
+    page = (4096, 1024, 64)
+    ok = dict(q=p, k=p, v=p, q_out=p, k_pages=p, v_pages=p + 64, k_scale=p, v_scale=p + 64, kp_strides=page, vp_strides=page,
+              scale_strides=(2, 1), freq=p, cu_rows=p, kv_len=p, page_table=p, dtype=0, layout=0, R=1, B=1, Hq=2, Hk=2, D=64,
+              rot=64, page=16, n_pages=4, max_pages=2)
+
+    def rc(**kw):
+        return _lib.lib.dspark_paged_append(C.byref(_lib.PagedAppendArgs(**{**ok, **kw})), None)
+
+    for bad in (dict(v_pages=p), dict(v_scale=p), dict(kp_strides=(0, 1024, 64)), dict(vp_strides=(4096, 0, 64)),
+                dict(kp_strides=(4096, 1024, 0)), dict(scale_strides=(0, 1)), dict(scale_strides=(2, 0))):
+        assert rc(**bad) == _lib.ERR_ARG and "share" in _lib.last_error(), bad

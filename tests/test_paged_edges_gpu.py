@@ -129,3 +129,32 @@ def test_append_to_a_begun_page_without_a_scale(cuda, page, D, n, scale):
         assert torch.equal(lo.nan_to_num(-1), hi.nan_to_num(-1)) and torch.equal(new[i + 2].double(), s_lo)
         got, want = new[i].double(), lo
         assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+
+
+# ------------------------------------------------------------------------------- pools that share their memory
+
+def test_pools_that_share_memory_are_read_but_not_written(cuda):
+    """One scale for all pages, as an expanded tensor, and k that is v: the attention reads them, an append is refused. A pool of
+    one page or one head may have any stride there."""
+    from mlx_dspark_b200 import DSparkError, paged
+
+    g = torch.Generator().manual_seed(1)
+    own = _finite_pool(cuda, 4, 2, 16, 64, g)
+    own.k_scale.fill_(0.5), own.v_scale.fill_(0.5)
+    one = torch.full((1, 1), 0.5, device=cuda).expand(4, 2)
+    x, table = torch.randn(5, 2, 64, generator=g).to(BF).to(cuda), _i32([[3, 1]], cuda)
+    args = x, _cu([5], cuda), _i32([20], cuda), table
+    want = own.attention(*args, scale=0.1)
+    shared = paged.PagedCache(own.k, own.v, one, one)
+    assert torch.equal(shared.attention(*args, scale=0.1), want)
+    same = paged.PagedCache(own.k, own.k, own.k_scale, own.k_scale)
+    assert not bool(same.attention(*args, scale=0.1).isnan().any())
+    for bad in (shared, same, paged.PagedCache(own.k, own.v, own.k_scale, own.k_scale),
+                paged.PagedCache(own.k[:1].expand(4, 2, 16, 64), own.v, own.k_scale, own.v_scale)):
+        with pytest.raises(DSparkError, match="share"):
+            _append_values(cuda, bad, table, 15, x.cpu(), x.cpu(), _identity(cuda, 64))
+    single = paged.PagedCache(own.k[:1, :1].as_strided((1, 1, 16, 64), (0, 0, 64, 1)), own.v[:1, :1],
+                              one[:1, :1].clone().as_strided((1, 1), (0, 0)), one[:1, :1].clone().as_strided((1, 1), (0, 0)))
+    y = torch.zeros(1, 1, 64, dtype=BF)
+    _append_values(cuda, single, _i32([[0]], cuda), 0, y, y, _identity(cuda, 64))
+    assert single.k_scale.item() == 2.0 ** -64
