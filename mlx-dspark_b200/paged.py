@@ -38,6 +38,14 @@ class PagedCache:
     ``[pages, heads]``): value = code * scale. :meth:`empty` makes a pool. :meth:`append` needs pages and
     scales that share no memory (no expanded ones, ``k`` and ``v`` apart); :meth:`attention` reads any."""
 
+    _FIXED = frozenset(("k", "v", "k_scale", "v_scale", "n_pages", "heads", "page_size", "head_dim"))
+
+    def __setattr__(self, name, value):
+        # calls pass the addresses and sizes that the pool was made with
+        if name in self._FIXED and self.__dict__.get(name, value) is not value:  # (the same one: `cache.k_scale *= 2`)
+            raise AttributeError(f"{name} of a PagedCache is fixed: write into its tensors, or make another pool")
+        super().__setattr__(name, value)
+
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.ndim != 4 or v.shape != k.shape or k.dtype is not torch.float8_e4m3fn or v.dtype is not k.dtype:
             raise _lib.DSparkError(_lib.ERR_ARG, f"pages {k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)}: "

@@ -4,8 +4,11 @@ from __future__ import annotations
 
 import ctypes as C
 
+import pytest
+import torch
+
 import mlx_dspark_b200  # noqa: F401
-from mlx_dspark_b200 import _lib
+from mlx_dspark_b200 import _lib, paged
 
 
 def test_append_refuses_lengths_that_overlap_its_inputs():
@@ -49,3 +52,22 @@ def test_append_refuses_pages_that_share_their_memory():
     for bad in (dict(v_pages=p), dict(v_scale=p), dict(kp_strides=(0, 1024, 64)), dict(vp_strides=(4096, 0, 64)),
                 dict(kp_strides=(4096, 1024, 0)), dict(scale_strides=(0, 1)), dict(scale_strides=(2, 0))):
         assert rc(**bad) == _lib.ERR_ARG and "share" in _lib.last_error(), bad
+
+
+def test_a_pools_tensors_and_sizes_are_fixed(monkeypatch):
+    """Calls use the addresses and sizes that the pool was made with: another tensor in the place of one of them would leave the
+    old one's memory, which may be gone, to be read and written."""
+    monkeypatch.setattr(paged, "on_device", lambda *a: 0)
+    cache = paged.PagedCache.empty(4, 2, 16, 64, "cpu")
+    for name in ("k", "v", "k_scale", "v_scale"):
+        with pytest.raises(AttributeError, match=name):
+            setattr(cache, name, getattr(cache, name).clone())
+    for name in ("n_pages", "heads", "page_size", "head_dim"):
+        with pytest.raises(AttributeError, match=name):
+            setattr(cache, name, 8)
+    cache.k_scale[1] = 2.0  # their values are not
+    cache.v_scale.fill_(4.0)
+    cache.v_scale *= 2
+    cache.owner = "a request"
+    cache.owner = None
+    assert cache.k_scale[1, 1] == 2.0 and cache.v_scale[0, 0] == 8.0 and cache.n_pages == 4 and cache._at[2] == cache.k_scale.data_ptr()
