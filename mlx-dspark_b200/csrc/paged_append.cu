@@ -21,7 +21,6 @@
 namespace dspark {
 namespace paged {
 
-constexpr int Q_THREADS = 128;
 constexpr int U = 4;  // heads of q in flight a lane
 
 // cos and sin of pos * f, f in 64-bit fixed-point turns (the product wraps at whole turns: any position keeps its
@@ -158,6 +157,7 @@ __device__ void append_page(const dspark_paged_append_args& a, int unit, int gro
   const bool turns = !kv && li < a.rot / 16, half = turns && HALF;
   const int c0 = half ? 8 * li : 16 * li, c1 = half ? a.rot / 2 + 8 * li : c0 + 8;
   constexpr int W = THREADS * 16;  // values a round
+  static_assert(PASS <= 2, "a head's rows and the next one's in registers");
   const int per = W / D, first = tid / lanes;
   const T* src = static_cast<const T*>(kv ? a.v : a.k) + (r0 + place0 + first) * row_stride;
   uint32_t raw[PASS][8];
@@ -285,17 +285,12 @@ __device__ void append_page(const dspark_paged_append_args& a, int unit, int gro
       }
     }
   }
-  constexpr bool AHEAD = PASS <= 2;  // (registers)
   for (int h = h0; h < h1; ++h) {
-    if (!AHEAD && h > h0) {
-      fetch(h);
-      old = begin ? scales[h * a.scale_strides[1]] : 0.f;
-    }
     Vals x[PASS];
 #pragma unroll
     for (int z = 0; z < PASS; ++z) x[z] = unpack16<T, HALF>(raw[z]);
     const float before = old;
-    if (AHEAD && h + 1 < h1) {  // the next head under this one's work
+    if (h + 1 < h1) {  // the next head under this one's work
       fetch(h + 1);
       old = begin ? scales[(h + 1) * a.scale_strides[1]] : 0.f;
     }

@@ -537,9 +537,10 @@ static cudaError_t launch_as(const dspark_score_args& a, int cluster, cudaStream
 
 template <typename T>
 static cudaError_t launch(const dspark_score_args& a, cudaStream_t s) {
-  // Blocks a row: as many as there is room for at once, for two of them some more, in slices of 4 KB or more. 151,936 values in bf16 without / with 5 alternatives, us by blocks a row (1, 2, 4, 8): 74 rows 26 16 14 12 / 32 21 20
-  // 18, 110 rows 33 23 17 18 / 38 29 24 30, 200 rows 42 29 24 28 / 48 35 35 45, 296 rows 46 30 30 39 / 52 36 42 61, 500
-  // rows 50 43 45 61 / 57 55 62 95, 740 rows 52 55 63 86 / 59 69 88 136.
+  // Blocks a row: as many as there is room for at once, for two of them some more, in slices of 4 KB or more. 151,936 values
+  // in bf16 without / with 5 alternatives, us by blocks a row (1, 2, 4, 8): 74 rows 26 16 14 12 / 32 21 20 18, 110 rows 33 23 17
+  // 18 / 38 29 24 30, 200 rows 42 29 24 28 / 48 35 35 45, 296 rows 46 30 30 39 / 52 36 42 61, 500 rows 50 43 45 61 / 57 55 62
+  // 95, 740 rows 52 55 63 86 / 59 69 88 136.
   const int64_t sms = sm_count(current_device());
   int cluster = 1;
   while (cluster < MAX_CLUSTER && int64_t(a.R) * cluster * 4 <= (cluster == 1 ? 14 : cluster == 2 ? 11 : 10) * sms &&
