@@ -697,7 +697,7 @@ int dspark_paged_append(const dspark_paged_append_args* a, void* stream);
  * there are none. kv_len[b] counts request b's rows too; causal: its row i sees keys before kv_len[b] - rows(b) + i + 1,
  * else all kv_len[b]. Not seen, whatever they hold: keys past the table's pages, those of a page id outside
  * 0 .. n_pages - 1 (recorded in the device status word) and those of a page whose scale is not positive. A row that
- * sees a NaN is NaN. Rows of no request are not written. Weights are rounded to fp16 for the product with v.
+ * sees a NaN is NaN, and so is one with an infinite or NaN q that sees a key. Rows of no request are not written. Weights are rounded to fp16 for the product with v.
  * 16-byte aligned rows. Scratch: dspark_paged_attn_workspace bytes, 16-byte aligned, nothing to clear; calls that
  * overlap on the GPU need their own. */
 typedef struct {

@@ -260,6 +260,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
         const int r = (z * NTHR + tid) / PER, p = tid % PER;
         uint32_t w[8] = {q0[z].x, q0[z].y, q0[z].z, q0[z].w, q1[z].x, q1[z].y, q1[z].z, q1[z].w};
         float f = 1.f;
+        bool bad = false;
         if (std::is_same<T, bf16>::value) {  // largest exponent of the row; 255: infinite or NaN
           uint32_t e = 0;
 #pragma unroll
@@ -269,17 +270,21 @@ __global__ void __launch_bounds__(NTHR, 2) attn_kernel(const dspark_paged_attn_a
           // values below 2^15: the row divided by 2^(e - 127 - 14); in two steps, where that is no fp32 value
           const int up = int(e) - 141;
           const float inv = pow2(max(min(-up, 126), -126));
-          f = e == 255 ? NAN : pow2(max(min(up, 126), -126));
+          bad = e == 255;
+          f = bad ? 1.f : pow2(max(min(up, 126), -126));
 #pragma unroll
           for (int i = 0; i < 8; ++i) w[i] = pack_f16(bf16_lo(w[i]) * inv, bf16_hi(w[i]) * inv);
-        } else {  // an infinite q makes its row NaN whatever the codes are
-          bool bad = false;
+        } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) bad |= (w[i] & 0x7c00u) == 0x7c00u || (w[i] & 0x7c000000u) == 0x7c000000u;
           uint32_t any = bad;
 #pragma unroll
           for (int o = 1; o < PER; o <<= 1) any |= __shfl_xor_sync(0xffffffffu, any, o);
-          f = any ? NAN : 1.f;
+          bad = any;
+        }
+        if (bad) {  // an infinite q makes its row NaN whatever the codes are: by its scores, of which those of hidden keys are dropped
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = 0x7fff7fffu;
         }
         if (r < RB) {
           if (p == 0) rowf[r] = f * c_log2;

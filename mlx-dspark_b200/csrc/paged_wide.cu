@@ -164,7 +164,7 @@ __device__ __forceinline__ int v_use(bool pair, int t, int n) {
   return pair ? 2 * t + 1 : t == n - 1 ? 2 * n - 1 : 2 * t + 2;
 }
 
-// A group's factor, 1e-35 at least: -inf stays that (and NaN too).
+// A group's factor, 1e-35 at least (of a negative rf too): -inf stays that, and NaN.
 __device__ __forceinline__ float factor_of(float rf, float ks) {
   const float f = rf * ks;
   return f < 1e-35f ? 1e-35f : f;
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
 #pragma unroll
           for (int c = 0; c < D / 8; ++c) v[c] = ldcg_v4(q + 8 * c);
           constexpr uint32_t SHIFT = std::is_same<T, bf16>::value ? 7 : 10, ONES = std::is_same<T, bf16>::value ? 0xff : 0x1f;
-          uint32_t e = 0;  // the largest exponent; all ones: infinite or NaN, and the row is NaN whatever the codes are
+          uint32_t e = 0;  // the largest exponent; all ones: infinite or NaN (its factor is negative then, its q zeros)
 #pragma unroll
           for (int c = 0; c < D / 8; ++c) {
             const uint32_t* y = &v[c].x;
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
             inv = pow2(max(min(-up, 126), -126));
             rf = pow2(max(min(up, 126), -126));
           }
-          rf = e == ONES ? NAN : rf * c_log2;
+          rf = e == ONES ? -1.f : rf * c_log2;
           uint8_t* dst = smem + L::Q + slot * L::TILE + row * 128;
 #pragma unroll
           for (int c = 0; c < D / 8; ++c) {
@@ -340,6 +340,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
 #pragma unroll
               for (int i = 0; i < 4; ++i) y[i] = Elem<__half>::pack(bf16_lo(y[i]) * inv, bf16_hi(y[i]) * inv);
             }
+            if (e == ONES) y[0] = y[1] = y[2] = y[3] = 0u;
             *reinterpret_cast<uint4*>(dst + (c >> 3) * L::HALF + (((c & 7) ^ (row & 7)) << 4)) =
                 make_uint4(y[0] ^ q_sign, y[1] ^ q_sign, y[2] ^ q_sign, y[3] ^ q_sign);
           }
@@ -470,6 +471,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
         l = a0.y * f0 + a1.y * f1;
         m = mn;
       }
+      if (rf < 0.f && l > 0.f) l = NAN;  // an infinite or NaN q: NaN whatever the codes are, where the row sees a key
       const bool hidden = *reinterpret_cast<volatile int*>(&flag[seg & 3]) == seg;
       if (warp_alive) {
         const int hq = s.h * G + my - place * G;

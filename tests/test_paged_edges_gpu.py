@@ -1,5 +1,6 @@
 """The paged 8-bit cache and token scores on the GPU where calls meet an edge: NaN codes beside the rows' own keys,
-zeros of either sign among the logits, begun pages without a scale."""
+zeros of either sign among the logits, begun pages without a scale,
+q of no number in rows that see nothing."""
 
 from __future__ import annotations
 
@@ -10,7 +11,7 @@ import paged_reference as ref
 import pytest
 import torch
 from test_paged_gpu import (BF, FP, HF, _append_values, _check_scores, _cpu, _cu, _far, _finite_pool, _i32, _identity, _pool,
-                            _tables)
+                            _tables, _with_room)
 
 pytestmark = pytest.mark.gpu
 
@@ -158,3 +159,46 @@ def test_pools_that_share_memory_are_read_but_not_written(cuda):
     y = torch.zeros(1, 1, 64, dtype=BF)
     _append_values(cuda, single, _i32([[0]], cuda), 0, y, y, _identity(cuda, 64))
     assert single.k_scale.item() == 2.0 ** -64
+
+
+# ------------------------------------------------------------------------------- q of no number
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("room", ["tight", "clusters", "shares", "far"])
+@pytest.mark.parametrize("n,dt", [(3, BF), (3, HF), (12, BF), (40, HF), (90, BF)])
+def test_q_of_no_number_in_rows_that_see_nothing(cuda, n, dt, room, causal):
+    """An infinite or NaN q makes its head NaN where the row sees a key, and takes no part where it sees none: more rows than keys,
+    no keys, pages that are not there or have no positive scale."""
+    from mlx_dspark_b200 import _lib
+
+    g, D, page, dev = torch.Generator().manual_seed(n), 64, 16, cuda.index
+    cache = _finite_pool(cuda, 40, 2, page, D, g)
+    cache.k_scale[20:30] = 0.0
+    rows = [list(range(20)), list(range(30, 36)), [33], [20, 21, 22], [-1, -1], [20, 34, -1]]
+    lens = [300, max(n - 2, 1), 0, 40, 20, 48]
+    tables = {"tight": lambda r: r, "clusters": lambda r: _with_room(r, page, 6000),
+              "shares": lambda r: _with_room(r, page, 40000), "far": lambda r: _far(r, page)}[room]
+    width = max(map(len, rows))
+    table = _i32(tables([r + [-1] * (width - len(r)) for r in rows]), cuda)
+    counts = [n] * len(rows)
+    q = torch.randn(n * len(rows), 4, D, generator=g).to(dt)
+    bad = torch.zeros(n * len(rows), 4, dtype=torch.bool)
+    for r in range(bad.shape[0]):
+        if r % 3 != 1:
+            h, value = r % 4, (math.inf, math.nan, -math.inf)[r % 7 % 3]
+            q[r, h, (5 * r) % D] = value
+            bad[r, h] = True
+    sees = torch.zeros(n * len(rows), dtype=torch.bool)
+    for b, x in enumerate(lens):
+        for i in range(n):
+            last = x - n + i + 1 if causal else x  # keys before it
+            seen = [j for j in range(max(0, min(x, last))) if 0 <= rows[b][j // page] < 20 or rows[b][j // page] >= 30]
+            sees[b * n + i] = bool(seen)
+    out = cache.attention(q.to(cuda), _cu(counts, cuda), _i32(lens, cuda), table, scale=0.2, causal=causal).cpu()
+    clean = cache.attention(torch.where(bad[..., None], 1.0, q).to(dt).to(cuda), _cu(counts, cuda), _i32(lens, cuda), table,
+                            scale=0.2, causal=causal).cpu()
+    assert _lib.device_status(dev) != 0  # (the pages that are not there)
+    assert bool((out[~sees] == 0).all())
+    want = bad & sees[:, None]
+    assert torch.equal(out.isnan().any(-1), want) and bool(out[want].isnan().all())
+    assert torch.equal(out[~want], clean[~want])
