@@ -730,7 +730,7 @@ size_t dspark_paged_attn_workspace(int R, int B, int Hq, int Hk, int D);
  * of that order with their log probabilities (top_ids, top_logprob [R, top]). A logit that is NaN, -inf, or -2^28 or
  * less (fp16: its lowest value) is a masked token's: probability 0, logprob -inf, rank -1, never an alternative; missing
  * alternatives have id -1 and -inf. One above 2^28 (fp16: inf) counts as 2^28 (the largest value). A row with no
- * other tokens: logprob -inf, entropy 0, rank -1. A token outside 0 .. V - 1: its row is not read; logprob and entropy
+ * other tokens: logprob -inf, entropy 0, rank -1. Zeros of either sign are one logit. A token outside 0 .. V - 1: its row is not read; logprob and entropy
  * 0, rank -1, no alternatives. bf16, fp16 or fp32, fp32 arithmetic. (The reference samples only,
  * src/mlx_dspark/sampling.py.) */
 typedef struct {

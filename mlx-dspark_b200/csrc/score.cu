@@ -13,7 +13,7 @@
 // A row is a cluster of 1 to 8 blocks, each with a slice of its 16-byte vectors; the first block joins them.
 // Bound: HBM and the exponentials' unit for many rows (2049 of 151,936 in bf16 124 us, 0.77 of the measured rate; 272 in
 // fp32 with 20 alternatives 42.4, 0.59, for the search of alternatives, which no other block's pass covers), latency for few
-// (one row 8.7). A ring of bulk copies in shared memory in place of plain loads: 132 beside 132, one row 14.
+// (one row 9). A ring of bulk copies in shared memory in place of plain loads: 132 beside 132, one row 14.
 #include <algorithm>
 #include <cfloat>
 

@@ -35,8 +35,9 @@ def _workspace(R: int, B: int, Hq: int, Hk: int, D: int, device: int) -> int:
 class PagedCache:
     """One layer's pages: codes ``k`` / ``v`` (``torch.float8_e4m3fn`` ``[pages, heads, page_size, head_dim]``, any
     strides of multiples of 16 with head_dim contiguous) and scales ``k_scale`` / ``v_scale`` (float32
-    ``[pages, heads]``): value = code * scale. :meth:`empty` makes a pool. :meth:`append` needs pages and
-    scales that share no memory (no expanded ones, ``k`` and ``v`` apart); :meth:`attention` reads any."""
+    ``[pages, heads]``): value = code * scale, scales of 2^-64 to 2^64 as :meth:`append` makes them. :meth:`empty`
+    makes a pool. :meth:`append` needs pages and scales that share no memory (no expanded ones, ``k`` and ``v`` apart);
+    :meth:`attention` reads any."""
 
     _FIXED = frozenset(("k", "v", "k_scale", "v_scale", "n_pages", "heads", "page_size", "head_dim"))
 
@@ -95,7 +96,10 @@ class PagedCache:
         most 448; a page that holds tokens already keeps its scale or raises it, and then its codes are rounded to
         the new one. Rows for which the table has no page (or one outside the pool) are dropped and recorded in the
         device status. Rows behind the last request's are left as they are. One call must not append to a page twice (two
-        requests with one page, or a request whose table repeats it)."""
+        requests with one page, or a request whose table repeats it).
+
+        How many rows a block takes goes by the call's mean rows a request: a prompt's chunk is appended faster apart from
+        decoded tokens (512 rows 6.6 us, 96 tokens 5.8, in one call 36)."""
         stream = on_device(q, k, v, cu_rows, kv_len, page_table, row_pos, q_norm, k_norm, q_out, len_out, table.freq,
                            self.k)
         shape, D = q.shape, self.head_dim
@@ -131,7 +135,16 @@ class PagedCache:
         counts a request's own rows too; ``causal``: its row i sees keys before ``kv_len[b] - rows(b) + i + 1``, else
         every row all ``kv_len[b]``. Returns ``out [R, Hq, D]``; a row that sees nothing is zero, a row of no request is
         not written. Keys of a page outside the pool are not seen (the device status records them), nor are those
-        of a page whose scale is not positive."""
+        of a page whose scale is not positive.
+
+        Scores and sums are fp32; the weights are rounded to fp16 for the product with v (fp16 results are off by 2.6e-4 of
+        themselves on average where their own rounding alone gives 2.1e-4; bf16 results do not show it).
+
+        The kernel is chosen for the whole call, before the lengths are known, by the mean number of rows a request and by the
+        table's width in place of the longest length. So a table no wider than its requests need is fastest (one row over 2049
+        keys 8.8 us, in a table of 131,072 tokens 10.7; 16 rows over 4096 keys 17 and 28), and a prompt's chunk apart from
+        decoded tokens (96 of them 134 us and 512 rows over 16k keys 150, in one call 671). Neither changes a result but
+        for the rounding of its weights."""
         stream = on_device(q, cu_rows, kv_len, page_table, out, self.k)
         shape, D, Hk = q.shape, self.head_dim, self.heads
         if len(shape) != 3 or shape[2] != D or Hk == 0 or shape[1] % Hk or shape[1] == 0:

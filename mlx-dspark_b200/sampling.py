@@ -120,7 +120,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: t
     A logit of NaN, -inf, or at most -2^28 (fp16: its lowest value) masks its token: logprob -inf, rank -1, never
     an alternative; where fewer tokens than ``top`` are left, the others' ids are -1 and their logprobs -inf. A row
     whose token is outside the vocabulary (-1: a padded row) is not read: logprob and entropy 0, rank -1, no
-    alternatives."""
+    alternatives. Zeros of either sign are one logit.
+
+    Alternatives of a row with more than 512 values at or near the last of them (a constant row, one of few distinct values) are
+    found by a pass each: 272 such rows of 151,936 in bf16 take 443 us with 5 and 1703 with 32, others 36 and 40."""
     stream = on_device(logits, tokens, temperature, *(() if out is None else out.values()))
     if logits.ndim != 2:
         raise _lib.DSparkError(_lib.ERR_ARG, f"logits {tuple(logits.shape)}: [R, V]")
