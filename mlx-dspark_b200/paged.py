@@ -66,6 +66,9 @@ class PagedCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self._at = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k_scale.stride())
 
+    def __reduce__(self):  # a copy is made of its own tensors, whose addresses are others
+        return type(self), (self.k, self.v, self.k_scale, self.v_scale)
+
     @classmethod
     def empty(cls, pages: int, heads: int, page_size: int, head_dim: int, device="cuda") -> "PagedCache":
         """A pool of zeros (scales 1)."""

@@ -2,7 +2,9 @@
 
 from __future__ import annotations
 
+import copy
 import ctypes as C
+import io
 
 import pytest
 import torch
@@ -71,3 +73,20 @@ def test_a_pools_tensors_and_sizes_are_fixed(monkeypatch):
     cache.owner = "a request"
     cache.owner = None
     assert cache.k_scale[1, 1] == 2.0 and cache.v_scale[0, 0] == 8.0 and cache.n_pages == 4 and cache._at[2] == cache.k_scale.data_ptr()
+
+
+def test_a_copied_pool_is_its_own(monkeypatch):
+    """A deep copy and a loaded pool use their own tensors' addresses, a shallow copy the same ones."""
+    monkeypatch.setattr(paged, "on_device", lambda *a: 0)
+    k, v = (torch.randint(0, 256, (4, 16, 2, 64), dtype=torch.uint8).view(torch.float8_e4m3fn).permute(0, 2, 1, 3) for _ in range(2))
+    cache = paged.PagedCache(k, v, torch.rand(4, 2), torch.rand(4, 2))
+    file = io.BytesIO()
+    torch.save(cache, file)
+    file.seek(0)
+    for other in (copy.deepcopy(cache), torch.load(file, weights_only=False), copy.copy(cache)):
+        for i, name in enumerate(("k", "v", "k_scale", "v_scale")):
+            mine, its = getattr(cache, name), getattr(other, name)
+            assert other._at[i] == its.data_ptr() and its.stride() == mine.stride()
+            assert torch.equal(its.view(torch.uint8) if i < 2 else its, mine.view(torch.uint8) if i < 2 else mine)
+        assert other._at[4:] == cache._at[4:] and other._kst == cache._kst and other.page_size == 16
+    assert copy.deepcopy(cache)._at[0] != cache._at[0] and copy.copy(cache)._at == cache._at
