@@ -657,10 +657,10 @@ int dspark_kv_keep_path(void* const* k_layers, void* const* v_layers, int n_laye
  * become tokens kv_len[b] + i; row_pos [R], or NULL: positions kv_len[b] + i. The scale of a page and head is the
  * smallest power of two (2^-64 to 2^64) with which the largest finite value of the tokens appended to it is at most
  * 448; where the page holds tokens of the request already (kv_len[b] % page), the larger of that and the old scale, and
- * if it rises the old codes are rounded to it (an old scale of NaN gives way too, and its tokens become zeros). A page begun anew (from its first token) starts a scale of its own;
- * taking tokens back (a smaller kv_len) leaves the scale. Values are rounded to nearest even, infinities become
- * +-448 * scale, NaN stays NaN. Rows whose page the table does not have (or an id outside 0 .. n_pages - 1) are
- * dropped, and the device status word records it. q_out (may be q) is written for rows of a request only.
+ * if it rises the old codes are rounded to it (an old scale of NaN gives way too, and its tokens become zeros). A page
+ * begun anew (from its first token) starts a scale of its own; taking tokens back (a smaller kv_len) leaves the scale.
+ * Values are rounded to nearest even, infinities become +-448 * scale, NaN stays NaN. Rows whose page the table does not
+ * have (or an id outside 0 .. n_pages - 1) are dropped, and the device status word records it. q_out (may be q) is written for rows of a request only.
  * len_out [B] (or NULL): kv_len + rows, at most max_pages * page (a kv_len above that stays); it may not overlap kv_len,
  * cu_rows, row_pos or page_table. No two requests append to one page; pages, heads, tokens and k and v (scales too) have
  * memory of their own, no strides of zero. */
@@ -697,7 +697,8 @@ int dspark_paged_append(const dspark_paged_append_args* a, void* stream);
  * there are none. kv_len[b] counts request b's rows too; causal: its row i sees keys before kv_len[b] - rows(b) + i + 1,
  * else all kv_len[b]. Not seen, whatever they hold: keys past the table's pages, those of a page id outside
  * 0 .. n_pages - 1 (recorded in the device status word) and those of a page whose scale is not positive. A row that
- * sees a NaN is NaN, and so is one with an infinite or NaN q that sees a key. Rows of no request are not written. Weights are rounded to fp16 for the product with v.
+ * sees a NaN is NaN, and so is one with an infinite or NaN q that sees a key. Rows of no request are not written.
+ * Weights are rounded to fp16 for the product with v. Which kernel runs goes by R / B and max_pages * page.
  * 16-byte aligned rows. Scratch: dspark_paged_attn_workspace bytes, 16-byte aligned, nothing to clear; calls that
  * overlap on the GPU need their own. */
 typedef struct {
@@ -730,7 +731,8 @@ size_t dspark_paged_attn_workspace(int R, int B, int Hq, int Hk, int D);
  * of that order with their log probabilities (top_ids, top_logprob [R, top]). A logit that is NaN, -inf, or -2^28 or
  * less (fp16: its lowest value) is a masked token's: probability 0, logprob -inf, rank -1, never an alternative; missing
  * alternatives have id -1 and -inf. One above 2^28 (fp16: inf) counts as 2^28 (the largest value). A row with no
- * other tokens: logprob -inf, entropy 0, rank -1. Zeros of either sign are one logit. A token outside 0 .. V - 1: its row is not read; logprob and entropy
+ * other tokens: logprob -inf, entropy 0, rank -1. Zeros of either sign are one logit. A token outside 0 .. V - 1: its
+ * row is not read; logprob and entropy
  * 0, rank -1, no alternatives. bf16, fp16 or fp32, fp32 arithmetic. (The reference samples only,
  * src/mlx_dspark/sampling.py.) */
 typedef struct {

@@ -474,11 +474,11 @@ extern "C" int dspark_paged_append(const dspark_paged_append_args* p, void* stre
   for (int i = 0; i < 3; ++i) codes &= a.kp_strides[i] % 16 == 0 && a.vp_strides[i] % 16 == 0;
   if (!codes) return fail(DSPARK_ERR_UNSUPPORTED, "paged_append: the pages' rows must be 16-byte aligned");
   // what is written has a place of its own: blocks write pages, heads, keys and values at the same time
-  bool own = a.R == 0 || (a.k_pages != a.v_pages && a.k_scale != a.v_scale);
+  bool own = a.k_pages != a.v_pages && a.k_scale != a.v_scale;
   for (const int64_t* st : {a.kp_strides, a.vp_strides})
     own &= (st[0] || a.n_pages <= 1) && (st[1] || a.Hk == 1) && st[2];
   own &= (a.scale_strides[0] || a.n_pages <= 1) && (a.scale_strides[1] || a.Hk == 1);
-  if (!own) return fail(DSPARK_ERR_ARG, "paged_append: pages or scales share their memory");
+  if (a.R && !own) return fail(DSPARK_ERR_ARG, "paged_append: pages or scales share their memory");
   bool vec = true;
   for (const void* x : {a.q, a.k, a.v, (const void*)a.q_out}) vec &= reinterpret_cast<uintptr_t>(x) % 16 == 0;
   for (int i = 0; i < 2; ++i)

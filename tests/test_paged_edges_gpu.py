@@ -154,6 +154,8 @@ def test_pools_that_share_memory_are_read_but_not_written(cuda):
                 paged.PagedCache(own.k[:1].expand(4, 2, 16, 64), own.v, own.k_scale, own.v_scale)):
         with pytest.raises(DSparkError, match="share"):
             _append_values(cuda, bad, table, 15, x.cpu(), x.cpu(), _identity(cuda, 64))
+    none = torch.empty(0, 2, 64, dtype=BF)  # no rows: nothing is written but the lengths
+    assert _append_values(cuda, shared, table, 15, none, none, _identity(cuda, 64))[1].tolist() == [15]
     single = paged.PagedCache(own.k[:1, :1].as_strided((1, 1, 16, 64), (0, 0, 64, 1)), own.v[:1, :1],
                               one[:1, :1].clone().as_strided((1, 1), (0, 0)), one[:1, :1].clone().as_strided((1, 1), (0, 0)))
     y = torch.zeros(1, 1, 64, dtype=BF)
