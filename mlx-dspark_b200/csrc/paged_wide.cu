@@ -145,6 +145,11 @@ static_assert(sizeof(Handed) <= 64, "Lay::SEGS");
 
 __device__ __forceinline__ bool is_pair(const Segment& s) { return s.live > ROWS; }
 
+// Keys that the item's first row sees, and with it all of them.
+__device__ __forceinline__ int seen_by_all(const dspark_paged_attn_args& a, const Segment& s) {
+  return a.causal ? min(s.len, s.before + s.row_base / (a.Hq / a.Hk) + 1) : s.len;
+}
+
 // Load u of a segment of n tiles, in the order that the products take them: K0 V0 K1 V1 .. (pair) or K0 K1 V0 K2 V1 ..
 // (tiles alternate between the slots). Returns the tile; `value`: V.
 __device__ __forceinline__ int load_of(bool pair, int u, int n, bool& value) {
@@ -172,12 +177,12 @@ __device__ __forceinline__ float factor_of(float rf, float ks) {
 }
 
 // The NaN codes that were taken out of the segment's V tiles, added to what a row that sees them has stored (`out`: the
-// output, or `part`: the fp32 part). They are taken out of whole tiles: from the first key of the one that holds the rows' own
-// first key on, keys before the rows' own among them.
+// output, or `part`: the fp32 part). They are taken out of whole tiles, those that not all rows of the item see whole: two or
+// three, however many rows the request has.
 template <typename T>
 __device__ __noinline__ void add_hidden(const dspark_paged_attn_args& a, const Segment& s, int lim, int d0, int d1, T* out,
                                         float* part) {
-  const int k0 = max(s.t0 * BN, max(s.before, 0) / BN * BN), k1 = min(min(s.t1 * BN, s.len), lim);
+  const int k0 = max(s.t0 * BN, max(seen_by_all(a, s), 0) / BN * BN), k1 = min(min(s.t1 * BN, s.len), lim);
   for (int k = k0; k < k1; ++k) {
     const int id = a.page_table[int64_t(s.b) * a.table_stride + k / a.page];
     if (id < 0 || id >= a.n_pages) continue;
@@ -307,7 +312,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
       const bool warp_alive = s.row_base + (pair ? slot * ROWS : 0) + (warp & 3) * 32 < s.rows * G;
       const int place = alive ? my / G : 0;
       const int lim = a.causal ? min(s.len, s.before + place + 1) : s.len;  // keys that the row sees
-      const int edge0 = (a.causal ? min(s.len, s.before + s.row_base / G + 1) : s.len) - BN;  // later: hidden keys
+      const int edge0 = seen_by_all(a, s) - BN;  // later: hidden keys
       // ---- Q as fp16, a row a thread (the first slot's for both where there are up to 128). The products that read the
       // last segment's are done: their O has been waited for.
       float rf = 1.f;
@@ -615,6 +620,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
         ++seg;
         const int n = s.t1 - s.t0;
         const bool pair = is_pair(s);
+        const int edge0 = seen_by_all(a, s) - BN;
         const int32_t* table = a.page_table + int64_t(s.b) * a.table_stride;
         auto page_ids = [&](int window) {
           int id = -1;
@@ -660,7 +666,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_kernel(const __grid_constant__ C
             factors[((tiles0 + t) % NSC) * 8 + (lane & 7)] =
                 ids >= 0 ? make_float4(sc.x, lg2(sc.y), 1.f / sc.y, 0.f) : make_float4(1.f, -INFINITY, 0.f, 0.f);
           if (lane == 0) {
-            notes[st] = Note{!value ? 0 : key0 + BN > s.before ? -seg : 1, s.len - key0};
+            notes[st] = Note{!value ? 0 : key0 > edge0 ? -seg : 1, s.len - key0};
             mbar_arrive_expect_tx(&c_full[st], L::CODES);
           }
           __syncwarp();

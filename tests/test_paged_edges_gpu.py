@@ -62,6 +62,34 @@ def test_nan_values_reach_all_rows_that_see_them(cuda, case, far, causal):
         assert torch.equal(out.cpu()[~want], clean.cpu()[~want]), place
 
 
+def test_a_nan_value_in_a_long_prompt_holds_nobody_up(cuda):
+    """Putting a NaN code back is a few tiles' work for every row block, however many rows the request has: the kernel's waits
+    do not run out meanwhile, here after 20 ms."""
+    from mlx_dspark_b200 import _lib
+
+    R, before, page, D, Hk, Hq = 16384, 77, 64, 128, 1, 4
+    g = torch.Generator().manual_seed(3)
+    n = -(-(R + before) // page)
+    cache = _finite_pool(cuda, n, Hk, page, D, g)
+    q = torch.randn(R, Hq, D, generator=g).to(BF).to(cuda)
+    args = _cu([R], cuda), _i32([R + before], cuda), _i32([list(range(n))], cuda)
+    clean = cache.attention(q, *args, scale=0.1)
+    places = [R // 3, R - 1]
+    for i in places:
+        cache.v.view(torch.uint8)[(before + i) // page, 0, (before + i) % page, 7 + i % 3] = 0x7F
+    _lib.set_wait_limit_ns(cuda.index, 20_000_000)
+    try:
+        out = cache.attention(q, *args, scale=0.1)
+        torch.cuda.synchronize()
+        assert _lib.device_status(cuda.index) == 0
+    finally:
+        _lib.set_wait_limit_ns(cuda.index, 0)
+    want = torch.zeros(out.shape, dtype=torch.bool, device=cuda)
+    for i in places:
+        want[i:, :, 7 + i % 3] = True
+    assert torch.equal(out.isnan(), want) and torch.equal(out[~want], clean[~want])
+
+
 # ------------------------------------------------------------------------------- zeros of either sign
 
 def _zeros(V, dt, at, g):
