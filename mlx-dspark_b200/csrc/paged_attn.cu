@@ -22,7 +22,7 @@
 // as large, so that what a long tail loses is below 2^-36 of the largest a key; scores, sums and O are fp32.
 //
 // Bound: HBM for decoded tokens (96 requests over 256 to 16k keys, 32/8 heads of 128, pages of 16: 128 us in a graph of such
-// calls, 146 in calls one by one, 111.5 of them the bytes at the measured rate), latency for one (2k keys 8.8 us). fp16
+// calls, 138 to 149 in calls one by one, 111.5 of them the bytes at the measured rate), latency for one (2k keys 8.8 us). fp16
 // products, because the 8-bit form of this instruction is as slow as a conversion of its operands and needs q and the weights
 // in parts: 313 us.
 #include <algorithm>

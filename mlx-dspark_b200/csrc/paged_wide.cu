@@ -18,9 +18,9 @@
 //
 // Rounding: weights are rounded to fp16 for the product with V (their sum is not); scores, maxima, sums and O are fp32.
 //
-// Bound: softmax and products in turn (two chunks of 509 rows over 16k keys, 64/8 heads of 128: 530 to 550 us in a graph of such
-// calls, 0.6 of the products' measured rate, 2.06 us a 256 x 128 tile, 566 to 576 in calls one by one); for slots of few rows
-// the latency of the four converting warps (24 blocks of 1 to 16 rows over 256 to 16k keys, 32/8 heads: 94 us, about 1.3 a tile
+// Bound: softmax and products in turn (two chunks of 509 rows over 16k keys, 64/8 heads of 128: 515 to 550 us in a graph of such
+// calls, 0.6 of the products' measured rate, 2.06 us a 256 x 128 tile, 562 to 576 in calls one by one); for slots of few rows
+// the latency of the four converting warps (24 blocks of 1 to 16 rows over 256 to 16k keys, 32/8 heads: 93 us, about 1.3 a tile
 // of K and V, with no unit above a third of its rate).
 #include <algorithm>
 

@@ -146,7 +146,7 @@ class PagedCache:
         The kernel is chosen for the whole call, before the lengths are known, by the mean number of rows a request and by the
         table's width in place of the longest length. So a table no wider than its requests need is fastest (one row over 2049
         keys 8.8 us, in a table of 131,072 tokens 10.7; 16 rows over 4096 keys 17 and 28), and a prompt's chunk apart from
-        decoded tokens (96 of them 134 us and 512 rows over 16k keys 150, in one call 671). Neither changes a result but
+        decoded tokens (96 of them 134 us and 512 rows over 16k keys 150, in one call 672). Neither changes a result but
         for the rounding of its weights."""
         stream = on_device(q, cu_rows, kv_len, page_table, out, self.k)
         shape, D, Hk = q.shape, self.head_dim, self.heads
